@@ -42,6 +42,7 @@ enum {
   VB_STATUS_MISS = 1,     /* routed expert not resident (slot -1) */
   VB_STATUS_BOUNDS = 2,   /* id or slot out of range; access skipped */
   VB_STATUS_TIMEOUT = 4,  /* a bounded inter-CTA wait gave up */
+  VB_STATUS_NONFINITE = 8, /* a NaN or infinity was stored as 0 or +-127 */
 };
 
 int vb_version(void);
@@ -502,6 +503,106 @@ int vb_kv_bf16_attn_at(const uint16_t *q, const uint16_t *k_cache, const uint16_
                        int32_t cap, float scale, int32_t causal, const uint16_t *gate_proj,
                        int32_t gate_stride, uint16_t *out, void *workspace,
                        size_t workspace_bytes, vb_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged 8-bit KV cache (no reference counterpart): int8 codes with one float32
+ * scale per page and kv head, for K and for V; a stored value is code * scale.
+ * page_table[b][i] is the pool page of positions [i * page, (i + 1) * page) of
+ * sequence b. Pages written by a call must not be shared between sequences.
+ * dim in {64, 128, 256}, page in {16, 32, 64, 128}; codes 16-byte aligned. A
+ * table entry outside [0, pages) or past max_pages flags VB_STATUS_BOUNDS and
+ * its rows are skipped (write), zero (read) or masked (attention). */
+typedef struct VbKv8Cache {
+  int8_t *k_codes, *v_codes;  /* [pages, kv_heads, page, dim] */
+  float *k_scales, *v_scales; /* [pages, kv_heads] */
+  const int32_t *page_table;  /* [batch, max_pages] */
+  int32_t pages, kv_heads, page, dim, batch, max_pages;
+} VbKv8Cache;
+
+/* Quantise bf16 rows as they are written: row i < counts[b] (nullable: n) of
+ * sequence b goes to position pos[b] + pos_add + i. A page's scale is
+ * max|x| / 127 (at least 2^-40; 0 while every value is 0) over all rows written
+ * since its first row; when it grows, the older rows of the page are rewritten
+ * as rint(code * old / new). Positions read on the device. Infinities are
+ * stored as +-127 * scale, NaN as 0, and flag VB_STATUS_NONFINITE. keys and
+ * values [batch, kv_heads, n, dim] with element strides {batch, head, row} and
+ * contiguous dims. */
+typedef struct VbKv8AppendArgs {
+  VbKv8Cache cache;
+  const uint16_t *keys, *values; /* bf16 */
+  int64_t k_strides[3], v_strides[3];
+  const int32_t *pos;    /* [batch] */
+  const int32_t *counts; /* [batch] or NULL */
+  int32_t *status;       /* nullable */
+  int32_t pos_add, n;
+} VbKv8AppendArgs;
+int vb_kv8_append(const VbKv8AppendArgs *args, vb_stream_t stream);
+
+/* Read rows back as bf16(code * scale): keys/values [batch, kv_heads, n, dim],
+ * row i is position start[b] + i (start nullable: 0); zero from lens[b] on. */
+typedef struct VbKv8ReadArgs {
+  VbKv8Cache cache;
+  const int32_t *lens;  /* [batch] */
+  const int32_t *start; /* [batch] or NULL */
+  uint16_t *keys, *values;
+  int32_t *status; /* nullable */
+  int32_t n;
+} VbKv8ReadArgs;
+int vb_kv8_read(const VbKv8ReadArgs *args, vb_stream_t stream);
+
+/* Attention over the cache: out = softmax(scale * q K^T) V in float32, one
+ * rounding to bf16, and lse (nullable) = log sum exp of the scaled scores.
+ * Sequence b holds keys_b = lens[b] + len_add keys and q_lens[b] (nullable: L)
+ * query rows; causal: query i sees keys < keys_b - q_lens[b] + i + 1, else all
+ * keys_b. A row that sees nothing, and every row from q_lens[b] on, is 0 with
+ * lse -inf. q bf16 [batch, q_heads, L, dim] with element strides {batch, head,
+ * row}; out bf16 [batch, q_heads, L, dim] and lse float32 [batch, q_heads, L]
+ * contiguous; query head hq reads kv head hq / (q_heads / kv_heads).
+ * workspace: vb_kv8_attn_workspace_size bytes, no initial contents needed. */
+typedef struct VbKv8AttnArgs {
+  VbKv8Cache cache;
+  const uint16_t *q;
+  int64_t q_strides[3];
+  const int32_t *lens;   /* [batch] */
+  const int32_t *q_lens; /* [batch] or NULL */
+  uint16_t *out;
+  float *lse;      /* nullable */
+  int32_t *status; /* nullable */
+  void *workspace;
+  size_t workspace_bytes;
+  float scale;
+  int32_t q_heads, L, len_add, causal;
+} VbKv8AttnArgs;
+size_t vb_kv8_attn_workspace_size(const VbKv8AttnArgs *args);
+int vb_kv8_attn(const VbKv8AttnArgs *args, vb_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Log probabilities of given tokens (no reference counterpart). Per row of
+ * logits [rows, vocab] (dtype 0 = bf16, 1 = float32; row_stride elements):
+ *   logprob = x_t / T - lse,   lse = log sum_j exp(x_j / T)
+ *   rank    = number of tokens ahead of t (greater logit, or equal and a lower
+ *             id), entropy = lse - sum_j p_j x_j / T
+ *   top_ids, top_logprobs [rows, top]: the best tokens, best first, ties to
+ *             the lowest id; top in [0, 32], top <= vocab.
+ * Sums in float32. Logits of -inf are tokens that cannot follow. A row with a
+ * NaN or +inf, or of -inf alone, has NaN logprob, entropy and top_logprobs. A
+ * token outside [0, vocab) flags VB_STATUS_BOUNDS: logprob NaN, rank -1.
+ * Workspace: zero-filled once, left reusable by every call. */
+typedef struct VbTokenLogprobsArgs {
+  const void *logits;
+  const int32_t *tokens; /* [rows] */
+  float *logprob, *entropy;
+  int32_t *rank, *top_ids;
+  float *top_logprobs;
+  int32_t *status; /* nullable */
+  void *workspace;
+  size_t workspace_bytes;
+  int64_t row_stride;
+  float temperature;
+  int32_t rows, vocab, top, dtype;
+} VbTokenLogprobsArgs;
+size_t vb_token_logprobs_workspace_size(int32_t rows, int32_t vocab, int32_t top);
+int vb_token_logprobs(const VbTokenLogprobsArgs *args, vb_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Expert residency: per-layer expert -> slot state of a pool of `cap` slots

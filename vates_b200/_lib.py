@@ -15,6 +15,7 @@ VB_OK = 0
 VB_STATUS_MISS = 1
 VB_STATUS_BOUNDS = 2
 VB_STATUS_TIMEOUT = 4
+VB_STATUS_NONFINITE = 8
 VB_ERR_CAPACITY = 4
 VB_DECODE_ROUTE_ONLY = 1
 
@@ -37,6 +38,43 @@ class VbMoeDecodeArgs(C.Structure):
         ("status", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("timing_events", C.c_void_p), ("trace", C.c_void_p),
     ]
+
+
+class VbKv8Cache(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p),
+                ("v_scales", C.c_void_p), ("page_table", C.c_void_p), ("pages", C.c_int32),
+                ("kv_heads", C.c_int32), ("page", C.c_int32), ("dim", C.c_int32),
+                ("batch", C.c_int32), ("max_pages", C.c_int32)]
+
+
+class VbKv8AppendArgs(C.Structure):
+    _fields_ = [("cache", VbKv8Cache), ("keys", C.c_void_p), ("values", C.c_void_p),
+                ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3), ("pos", C.c_void_p),
+                ("counts", C.c_void_p), ("status", C.c_void_p), ("pos_add", C.c_int32),
+                ("n", C.c_int32)]
+
+
+class VbKv8ReadArgs(C.Structure):
+    _fields_ = [("cache", VbKv8Cache), ("lens", C.c_void_p), ("start", C.c_void_p),
+                ("keys", C.c_void_p), ("values", C.c_void_p), ("status", C.c_void_p),
+                ("n", C.c_int32)]
+
+
+class VbKv8AttnArgs(C.Structure):
+    _fields_ = [("cache", VbKv8Cache), ("q", C.c_void_p), ("q_strides", C.c_int64 * 3),
+                ("lens", C.c_void_p), ("q_lens", C.c_void_p), ("out", C.c_void_p),
+                ("lse", C.c_void_p), ("status", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("scale", C.c_float), ("q_heads", C.c_int32),
+                ("L", C.c_int32), ("len_add", C.c_int32), ("causal", C.c_int32)]
+
+
+class VbTokenLogprobsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("tokens", C.c_void_p), ("logprob", C.c_void_p),
+                ("entropy", C.c_void_p), ("rank", C.c_void_p), ("top_ids", C.c_void_p),
+                ("top_logprobs", C.c_void_p), ("status", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("row_stride", C.c_int64),
+                ("temperature", C.c_float), ("rows", C.c_int32), ("vocab", C.c_int32),
+                ("top", C.c_int32), ("dtype", C.c_int32)]
 
 
 class VbMoePrefillArgs(C.Structure):
@@ -142,6 +180,12 @@ _SIGNATURES = {
     "vb_kv_decode_attn": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32,
                                  _I32, _I32, _I32, _I32, _I32, _I32, C.c_float, _I32, _P,
                                  _P, _SZ, _P]),
+    "vb_kv8_append": (_I32, [C.POINTER(VbKv8AppendArgs), _P]),
+    "vb_kv8_read": (_I32, [C.POINTER(VbKv8ReadArgs), _P]),
+    "vb_kv8_attn_workspace_size": (_SZ, [C.POINTER(VbKv8AttnArgs)]),
+    "vb_kv8_attn": (_I32, [C.POINTER(VbKv8AttnArgs), _P]),
+    "vb_token_logprobs_workspace_size": (_SZ, [_I32, _I32, _I32]),
+    "vb_token_logprobs": (_I32, [C.POINTER(VbTokenLogprobsArgs), _P]),
     "vb_res_create": (_P, [_I32, _I32, _I32, _I32, _I32]),
     "vb_res_destroy": (None, [_P]),
     "vb_res_demand": (_I32, [_P, _I32, _P, _I32, _P, _P, _P, _P, _P]),

@@ -34,6 +34,9 @@ SOURCES = [
     "dense.cu",
     "qwen_next.cu",
     "gdn_fused.cu",
+    "kv8_cache.cu",
+    "kv8_attn.cu",
+    "logprobs.cu",
 ]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

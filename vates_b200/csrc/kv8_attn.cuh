@@ -1,0 +1,79 @@
+// What the attention kernels over the paged 8-bit cache share.
+#pragma once
+
+#include "kv8.cuh"
+
+namespace vb {
+
+struct Kv8AttnParams {
+  VbKv8Cache c;
+  const uint16_t *q;
+  int64_t qb, qh, ql;  // element strides of batch, head, row
+  const int32_t *lens, *q_lens;
+  uint16_t *out;
+  float *lse;
+  int32_t *status;
+  // partial results of a key range: rows of float32 O, then (m, l) per row
+  float *o_part;
+  float2 *ml_part;
+  float scale_log2;  // scale * log2(e)
+  int Hq, L, rep, len_add, causal, shift, vec;
+  int row_tiles, splits;
+};
+
+// A row tile's share of the sequence: query row R of the flattened (row, head
+// of the group) order is query R / rep, head R % rep, and sees the first
+// visible(R / rep) keys.
+struct Kv8Span {
+  int keys, q_len, off, causal;
+  __device__ int visible(int i) const {
+    return i >= q_len ? 0 : causal ? max(0, off + i + 1) : keys;
+  }
+};
+
+__device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnParams &p, int b, bool flag) {
+  Kv8Span s;
+  int32_t *status = flag ? p.status : nullptr;
+  const long long cap = (long long)p.c.max_pages * p.c.page;
+  const long long keys = (long long)p.lens[b] + p.len_add;
+  if (keys < 0 || keys > cap) flag_status(status, VB_STATUS_BOUNDS);
+  s.keys = (int)min(max(keys, 0ll), cap);
+  s.q_len = kv8_rows(p.q_lens, b, p.L, status);
+  s.off = s.keys - s.q_len;
+  s.causal = p.causal;
+  return s;
+}
+
+__device__ __forceinline__ float kv8_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Query values enter the products as f16 after a power of two that puts the
+// row's largest one in [2^8, 2^9): exact for every bf16 down to 2^-23 of it.
+// Returns the power (1 for a row with an infinity: that row is NaN anyway).
+__device__ __forceinline__ float kv8_q_power(float amax) {
+  const int e = (int)(__float_as_uint(amax) >> 23) & 255;
+  return __uint_as_float((uint32_t)(e == 255 ? 127 : min(254, 262 - e)) << 23);
+}
+
+// Shift of the exponentials before they are rounded to f16 (2^14, largest f16
+// 65504): the smallest kept weight is 2^-38 of the largest, so even a long
+// tail of small weights is not flushed. It cancels in O / l.
+constexpr float KV8_P_SHIFT = 14.f;
+
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two codes + 128 in the low bytes of 0x64xx halves (1024 + 128 + code) minus
+// 1152: exact f16 codes.
+__device__ __forceinline__ uint32_t h2_codes(uint32_t magic) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(magic), "r"(0x64806480u));
+  return r;
+}
+
+}  // namespace vb

@@ -1,0 +1,462 @@
+// Log probabilities of given tokens, their rank, the entropy and the best
+// alternatives of every row, in one pass over the logits.
+//
+// With m the largest logit so far, c = log2(e) / T and y_j = (x_j - m) c:
+//   s = sum 2^y_j,  t = sum 2^y_j y_j   (float32)
+//   logprob = ((x_t - m) c - log2 s) ln 2,  entropy = (log2 s - t / s) ln 2.
+// When m moves, with d = (m_old - m_new) c: t <- 2^d (t + d s), s <- 2^d s, so
+// the running maximum is carried per thread and the row is read once. y stops
+// at -1000 (2^y = 0), which keeps 0 * inf out of t for logits of -inf; NaN and
+// +inf go through and give NaN. The difference is taken before the product: it
+// is exactly 0 at the maximum however large the logits are.
+//
+// Best alternatives: the k-th largest of the threads' own maxima is a lower
+// bound v of the k-th largest logit (k threads hold one at least that large),
+// so only threads whose maximum reaches v can hold any of the k best. Their
+// vectors, about k / 512 of the row, are looked at again (they are in L2) and
+// the logits >= v collected as 64-bit keys (ordered value, ~id), which have no
+// ties; the k largest keys are the answer.
+//
+// One CTA per row, or per slice of a row when there are few rows: the last
+// slice of a row (ticket) joins the slices in order.
+#include "common.cuh"
+
+namespace vb {
+namespace {
+
+constexpr int LP_THREADS = 512;
+constexpr int LP_WARPS = LP_THREADS / 32;
+constexpr int LP_UNROLL = 4;
+constexpr int LP_MAX_TOP = 32;
+constexpr int LP_BATCH = LP_THREADS * 8;         // most keys one look can add
+constexpr int LP_CAP = LP_BATCH + LP_MAX_TOP;
+constexpr int LP_RANK_ALL = 2 * LP_THREADS;      // up to here every key is ranked at once
+constexpr int LP_MAX_PARTS = 64;
+constexpr int LP_FILL = 2 * 148;                 // CTAs that fill the GPU, two per SM
+constexpr size_t LP_TICKETS = 1024;              // bytes: a word per row of a split call
+static_assert(LP_FILL / 2 * sizeof(uint32_t) <= LP_TICKETS, "rows of a split call");
+static_assert(LP_MAX_PARTS * LP_MAX_TOP <= LP_CAP, "keys of a split row");
+constexpr float LP_NONE = -3.402823466e38f;      // m before any logit
+constexpr float LP_LN2 = 0.693147180559945309f;
+
+struct LpStats {
+  float m, s, t;  // maximum, sum, weighted sum
+  float best;     // largest logit (NaN ignored), -inf if there is none above it
+  int32_t ahead;  // logits ahead of the token
+  int32_t pad[3];
+};
+
+struct LpParams {
+  const void *logits;
+  const int32_t *tokens;
+  float *logprob, *entropy, *top_logprobs;
+  int32_t *rank, *top_ids, *status;
+  LpStats *part_stats;            // [rows, parts]
+  unsigned long long *part_keys;  // [rows, parts, top]
+  uint32_t *tickets;              // [rows], zero between calls
+  int64_t row_stride;
+  float c;                        // log2(e) / temperature
+  int vocab, top, parts;
+};
+
+__device__ __forceinline__ float lp_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Unsigned order of floats (NaN as -inf, -0 as 0).
+__device__ __forceinline__ uint32_t lp_order(float x) {
+  x = x == x ? x + 0.f : -INFINITY;
+  const uint32_t u = __float_as_uint(x);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float lp_unorder(uint32_t o) {
+  return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ unsigned long long lp_key(float x, int id) {
+  return ((unsigned long long)lp_order(x) << 32) | (uint32_t)~id;
+}
+// The next larger value of the type (NaN after +inf: nothing compares).
+__device__ __forceinline__ float lp_next(float x, bool bf16) {
+  const uint32_t step = bf16 ? 0x10000u : 1u;
+  if (x == 0.f) return __uint_as_float(step);
+  const uint32_t u = __float_as_uint(x);
+  if (u == 0x7F800000u) return __uint_as_float(0x7FC00000u);
+  return __uint_as_float((u & 0x80000000u) ? u - step : u + step);
+}
+
+// 16 bytes of a row: 8 bf16 or 4 float32 values.
+template <typename T>
+struct LpVec;
+template <>
+struct LpVec<uint16_t> {
+  static constexpr int N = 8;
+  static constexpr bool BF16 = true;
+  __device__ static float at(const uint4 &v, int j) {
+    const uint32_t w = (&v.x)[j >> 1];
+    return __uint_as_float((j & 1) ? (w & 0xFFFF0000u) : (w << 16));
+  }
+  __device__ static float load(const uint16_t *p) { return bf2f(*p); }
+};
+template <>
+struct LpVec<float> {
+  static constexpr int N = 4;
+  static constexpr bool BF16 = false;
+  __device__ static float at(const uint4 &v, int j) { return __uint_as_float((&v.x)[j]); }
+  __device__ static float load(const float *p) { return *p; }
+};
+
+// A row's vectors: vector v holds ids [v N - off, v N - off + N); those outside
+// [0, vocab) are not part of the row (first and last vector only).
+template <typename T>
+struct LpRow {
+  const T *x;
+  int off, vocab, nvec, w_lo, w_hi;  // whole vectors: [w_lo, w_hi)
+  __device__ LpRow(const void *logits, int64_t row, int64_t stride, int n) {
+    x = static_cast<const T *>(logits) + row * stride;
+    off = (int)(((uintptr_t)x & 15) / sizeof(T));
+    vocab = n;
+    nvec = (n + off + LpVec<T>::N - 1) / LpVec<T>::N;
+    w_lo = off > 0;
+    w_hi = (n + off) / LpVec<T>::N;
+  }
+  __device__ bool whole(int v) const { return v >= w_lo && v < w_hi; }
+  __device__ uint4 load(int v) const {  // whole vectors only
+    return ldg_nc_v4(x + ((int64_t)v * LpVec<T>::N - off));
+  }
+};
+
+__device__ __forceinline__ float lp_y(float x, float m, float c) {
+  float y;  // NaN stays NaN
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"((x - m) * c), "f"(-1000.f));
+  return y;
+}
+__device__ __forceinline__ void lp_move(float &m, float &s, float &t, float to, float c) {
+  if (to > m) {
+    const float d = fmaxf((m - to) * c, -1000.f), a = lp_ex2(d);
+    t = a * fmaf(d, s, t);
+    s = a * s;
+    m = to;
+  }
+}
+__device__ __forceinline__ void lp_join(float &m, float &s, float &t, float m2, float s2,
+                                        float t2, float c) {
+  const float to = fmaxf(m, m2);
+  lp_move(m, s, t, to, c);
+  lp_move(m2, s2, t2, to, c);
+  s += s2;
+  t += t2;
+}
+
+// The k largest of buf[0, n) (distinct keys) in descending order into list;
+// zeros beyond n. Called by every thread; buf and list are reusable after the
+// closing barrier.
+__device__ void lp_select(unsigned long long *buf, int n, int k, unsigned long long *list,
+                          unsigned long long *tmp, int *s_n, int *s_cnt) {
+  const int tid = threadIdx.x;
+  if (n > LP_RANK_ALL) {  // many candidates (ties): bisect for the k-th key first
+    unsigned long long thr = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const unsigned long long cand = thr | (1ull << bit);
+      int c = 0;
+      for (int i = tid; i < n; i += LP_THREADS) c += buf[i] >= cand;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if ((tid & 31) == 0) s_cnt[tid >> 5] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int w = 0; w < LP_WARPS; ++w) c += s_cnt[w];
+      if (c >= k) thr = cand;
+      __syncthreads();
+    }
+    if (tid == 0) *s_n = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += LP_THREADS)
+      if (buf[i] >= thr) tmp[atomicAdd(s_n, 1)] = buf[i];  // exactly k
+    __syncthreads();
+    if (tid < k) buf[tid] = tmp[tid];
+    n = k;
+    __syncthreads();
+  }
+  if (tid >= n && tid < k) list[tid] = 0;
+  for (int i = tid; i < n; i += LP_THREADS) {
+    const unsigned long long key = buf[i];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += buf[j] > key;
+    if (r < k) list[r] = key;
+  }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams p) {
+  using V = LpVec<T>;
+  __shared__ unsigned long long s_buf[LP_CAP];
+  __shared__ unsigned long long s_list[LP_MAX_TOP], s_tmp[LP_MAX_TOP];
+  __shared__ float s_m[LP_WARPS], s_s[LP_WARPS], s_t[LP_WARPS], s_b[LP_WARPS];
+  __shared__ int s_a[LP_WARPS], s_cnt[LP_WARPS];
+  __shared__ uint16_t s_owner[LP_THREADS];
+  __shared__ int s_n, s_owners, s_last;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x;
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const LpRow<T> r(p.logits, row, p.row_stride, p.vocab);
+  const int tok = p.tokens[row];
+  const bool tok_ok = (unsigned)tok < (unsigned)p.vocab;
+  const float xt = tok_ok ? V::load(r.x + tok) : 0.f;
+  const float xt_next = lp_next(xt, V::BF16);
+  const int tok_vec = tok_ok ? (tok + r.off) / V::N : -1;
+  const int v_lo = (int)((int64_t)r.nvec * part / p.parts);
+  const int v_hi = (int)((int64_t)r.nvec * (part + 1) / p.parts);
+  const float c = p.c;
+
+  float m = LP_NONE, s = 0.f, t = 0.f, best = -INFINITY;
+  int ahead = 0;
+  for (int v0 = v_lo + tid; v0 < v_hi; v0 += LP_THREADS * LP_UNROLL) {
+    uint4 x[LP_UNROLL];
+    bool in[LP_UNROLL];
+#pragma unroll
+    for (int u = 0; u < LP_UNROLL; ++u) {
+      const int v = v0 + u * LP_THREADS;
+      in[u] = v < v_hi && r.whole(v) && v != tok_vec;
+      if (in[u]) x[u] = r.load(v);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < LP_UNROLL; ++u)
+      if (in[u])
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) top = fmaxf(top, V::at(x[u], j));
+    best = fmaxf(best, top);
+    lp_move(m, s, t, top, c);
+#pragma unroll
+    for (int u = 0; u < LP_UNROLL; ++u) {
+      const int v = v0 + u * LP_THREADS;
+      if (in[u]) {
+        // ids below the token's count when equal
+        const float bar = v < tok_vec ? xt : xt_next;
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) {
+          const float f = V::at(x[u], j);
+          const float y = lp_y(f, m, c);
+          const float e = lp_ex2(y);
+          s += e;
+          t = fmaf(e, y, t);
+          ahead += f >= bar;
+        }
+      } else if (v < v_hi) {  // the row's ends and the token's own vector
+        for (int j = 0; j < V::N; ++j) {
+          const int64_t id = (int64_t)v * V::N - r.off + j;
+          if (id < 0 || id >= p.vocab) continue;
+          const float f = V::load(r.x + id);
+          best = fmaxf(best, f);
+          lp_move(m, s, t, f, c);
+          const float y = lp_y(f, m, c);
+          const float e = lp_ex2(y);
+          s += e;
+          t = fmaf(e, y, t);
+          ahead += f > xt || (f == xt && id < tok);
+        }
+      }
+    }
+  }
+  // ---- the k best of this slice
+  const int k = p.top;
+  if (k > 0) {
+    const uint32_t mine = v_lo + tid < v_hi ? lp_order(best) : 0u;
+    uint32_t thr = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t cand = thr | (1u << bit);
+      if (__syncthreads_count(mine >= cand) >= k) thr = cand;
+    }
+    if (tid == 0) s_owners = s_n = 0;
+    __syncthreads();
+    if (mine >= thr && v_lo + tid < v_hi) s_owner[atomicAdd(&s_owners, 1)] = (uint16_t)tid;
+    __syncthreads();
+    const int owners = s_owners;
+    const int turns = (v_hi - v_lo + LP_THREADS - 1) / LP_THREADS;
+    const int64_t items = (int64_t)turns * owners;
+    unsigned long long kth = 0;
+    int have = 0;
+    for (int64_t i0 = 0; i0 < items; i0 += LP_THREADS) {
+      const int64_t i = i0 + tid;
+      const int v = i < items ? v_lo + (int)(i / owners) * LP_THREADS + s_owner[i % owners] : v_hi;
+      if (v < v_hi) {
+        const bool whole = r.whole(v);
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (whole) x = r.load(v);
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) {
+          const int64_t id = (int64_t)v * V::N - r.off + j;
+          if (id < 0 || id >= p.vocab) continue;
+          const float f = whole ? V::at(x, j) : V::load(r.x + id);
+          if (lp_order(f) >= thr) {
+            const unsigned long long key = lp_key(f, (int)id);
+            if (key > kth) s_buf[atomicAdd(&s_n, 1)] = key;
+          }
+        }
+      }
+      __syncthreads();
+      const int n = s_n;
+      const bool last = i0 + LP_THREADS >= items;
+      if (last || n > LP_CAP - LP_BATCH) {
+        lp_select(s_buf, n, k, s_list, s_tmp, &s_n, s_cnt);
+        have = min(n, k);
+        if (have == k) kth = s_list[k - 1];
+        if (!last) {
+          if (tid < have) s_buf[tid] = s_list[tid];
+          if (tid == 0) s_n = have;
+        }
+      }
+      __syncthreads();
+    }
+  }
+
+  // ---- sums over the CTA
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o),
+                t2 = __shfl_xor_sync(0xffffffffu, t, o);
+    lp_join(m, s, t, m2, s2, t2, c);
+    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  }
+  ahead = __reduce_add_sync(0xffffffffu, ahead);
+  if ((tid & 31) == 0) {
+    s_m[tid >> 5] = m; s_s[tid >> 5] = s; s_t[tid >> 5] = t;
+    s_b[tid >> 5] = best; s_a[tid >> 5] = ahead;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < LP_WARPS; ++w) {
+      lp_join(m, s, t, s_m[w], s_s[w], s_t[w], c);
+      best = fmaxf(best, s_b[w]);
+      ahead += s_a[w];
+    }
+  }
+  if (p.parts > 1) {  // leave the slice's sums and keys; the row's last slice joins them
+    const size_t at = (size_t)row * p.parts + part;
+    if (tid == 0) {
+      LpStats st;
+      st.m = m; st.s = s; st.t = t; st.best = best; st.ahead = ahead;
+      st.pad[0] = st.pad[1] = st.pad[2] = 0;
+      p.part_stats[at] = st;
+    }
+    if (tid < k) p.part_keys[at * k + tid] = s_list[tid];
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      s_last = atomicAdd(p.tickets + row, 1u) == (uint32_t)p.parts - 1;
+      if (s_last) p.tickets[row] = 0;
+      s_n = 0;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    if (k > 0) {
+      const unsigned long long *keys = p.part_keys + (size_t)row * p.parts * k;
+      for (int i = tid; i < p.parts * k; i += LP_THREADS) {
+        const unsigned long long key = __ldcg(keys + i);
+        if (key) s_buf[atomicAdd(&s_n, 1)] = key;
+      }
+      __syncthreads();
+      const int n = s_n;
+      lp_select(s_buf, n, k, s_list, s_tmp, &s_n, s_cnt);
+    }
+    if (tid == 0) {
+      const LpStats *st = p.part_stats + (size_t)row * p.parts;
+      m = LP_NONE; s = t = 0.f; best = -INFINITY; ahead = 0;
+      for (int i = 0; i < p.parts; ++i) {
+        lp_join(m, s, t, __ldcg(&st[i].m), __ldcg(&st[i].s), __ldcg(&st[i].t), c);
+        best = fmaxf(best, __ldcg(&st[i].best));
+        ahead += __ldcg(&st[i].ahead);
+      }
+    }
+  }
+  if (tid == 0) {
+    s_m[0] = m;
+    s_s[0] = best == -INFINITY ? NAN : log2f(s);
+    const float l2 = s_s[0];
+    p.logprob[row] = tok_ok ? ((xt - m) * c - l2) * LP_LN2 : NAN;
+    p.entropy[row] = (l2 - t / s) * LP_LN2;
+    p.rank[row] = tok_ok ? ahead : -1;
+    if (!tok_ok) flag_status(p.status, VB_STATUS_BOUNDS);
+  }
+  __syncthreads();
+  if (tid < k) {
+    const unsigned long long key = s_list[tid];
+    p.top_ids[(size_t)row * k + tid] = (int32_t)~(uint32_t)key;
+    p.top_logprobs[(size_t)row * k + tid] =
+        ((lp_unorder((uint32_t)(key >> 32)) - s_m[0]) * c - s_s[0]) * LP_LN2;
+  }
+}
+
+// Slices per row: one CTA per row once the rows alone fill the GPU, else
+// slices of at least one vector per thread.
+int lp_parts(int rows, int vocab) {
+  const int most = (vocab - 1) / (LP_THREADS * 8) + 1;
+  int parts = rows > 0 ? LP_FILL / rows : 1;
+  if (parts > most) parts = most;
+  return parts < 1 ? 1 : parts > LP_MAX_PARTS ? LP_MAX_PARTS : parts;
+}
+
+}  // namespace
+}  // namespace vb
+
+using namespace vb;
+
+extern "C" {
+
+size_t vb_token_logprobs_workspace_size(int32_t rows, int32_t vocab, int32_t top) {
+  if (rows < 1 || vocab < 1 || top < 0 || top > LP_MAX_TOP) return 0;
+  const size_t parts = lp_parts(rows, vocab);
+  return LP_TICKETS +
+         (parts > 1 ? rows * parts * (sizeof(LpStats) + top * sizeof(unsigned long long)) : 0);
+}
+
+int vb_token_logprobs(const VbTokenLogprobsArgs *a, vb_stream_t stream) {
+  VB_REQUIRE(a, "vb_token_logprobs: null args");
+  VB_REQUIRE(a->rows >= 0 && a->rows <= (1 << 24) && a->vocab >= 1 && a->vocab <= (1 << 30),
+             "vb_token_logprobs: rows=%d (<= 2^24) vocab=%d (<= 2^30)", a->rows, a->vocab);
+  VB_REQUIRE(a->top >= 0 && a->top <= LP_MAX_TOP && a->top <= a->vocab,
+             "vb_token_logprobs: top=%d (at most %d and the vocabulary)", a->top, LP_MAX_TOP);
+  VB_REQUIRE(a->dtype == 0 || a->dtype == 1, "vb_token_logprobs: dtype %d", a->dtype);
+  VB_REQUIRE(a->temperature >= 1e-3f && a->temperature <= 1e3f,
+             "vb_token_logprobs: temperature %g (1e-3 .. 1e3)", (double)a->temperature);
+  if (a->rows == 0) return VB_OK;
+  VB_REQUIRE(a->logits && a->tokens && a->logprob && a->entropy && a->rank &&
+                 (a->top == 0 || (a->top_ids && a->top_logprobs)),
+             "vb_token_logprobs: null tensor");
+  VB_REQUIRE(((uintptr_t)a->logits % (a->dtype ? 4 : 2)) == 0,
+             "vb_token_logprobs: logits not aligned to their type");
+  VB_REQUIRE(a->row_stride >= a->vocab || a->rows == 1 || a->row_stride == 0,
+             "vb_token_logprobs: row stride %lld below the vocabulary", (long long)a->row_stride);
+  const size_t need = vb_token_logprobs_workspace_size(a->rows, a->vocab, a->top);
+  if (!a->workspace || a->workspace_bytes < need)
+    return set_error(VB_ERR_WORKSPACE, "vb_token_logprobs: workspace %zu < %zu bytes",
+                     a->workspace_bytes, need);
+  VB_REQUIRE(((uintptr_t)a->workspace % 16) == 0, "vb_token_logprobs: workspace alignment");
+  LpParams p;
+  p.logits = a->logits; p.tokens = a->tokens;
+  p.logprob = a->logprob; p.entropy = a->entropy; p.top_logprobs = a->top_logprobs;
+  p.rank = a->rank; p.top_ids = a->top_ids; p.status = a->status;
+  p.parts = lp_parts(a->rows, a->vocab);
+  uint8_t *w = static_cast<uint8_t *>(a->workspace);
+  p.tickets = reinterpret_cast<uint32_t *>(w);
+  w += LP_TICKETS;
+  p.part_stats = reinterpret_cast<LpStats *>(w);
+  w += (size_t)a->rows * p.parts * sizeof(LpStats);
+  p.part_keys = reinterpret_cast<unsigned long long *>(w);
+  p.row_stride = a->row_stride;
+  p.c = (float)(1.4426950408889634 / (double)a->temperature);
+  p.vocab = a->vocab; p.top = a->top;
+  const dim3 grid(a->rows * p.parts), block(LP_THREADS);
+  if (a->dtype == 0)
+    vb_launch(token_logprobs_kernel<uint16_t>, grid, block, 0, as_stream(stream), false, p);
+  else
+    vb_launch(token_logprobs_kernel<float>, grid, block, 0, as_stream(stream), false, p);
+  return check_launch("token_logprobs_kernel");
+}
+
+}  // extern "C"

@@ -1,0 +1,180 @@
+"""Paged 8-bit KV cache on B200: writing, reading back and attention.
+
+A pool of pages holds int8 codes ``[pages, kv_heads, page, head_dim]`` for K
+and for V with one float32 scale per page and head (``value = code * scale``);
+a table ``[batch, max_pages]`` names the pool page of every ``page``
+consecutive positions of a sequence. Positions and lengths are device tensors,
+so a step that writes and attends can be captured in a CUDA graph.
+
+Half the bytes of a bf16 cache, several sequences of different lengths, any
+number of query heads per key/value head and head sizes 64, 128 and 256; the
+IsoQuant cache (:mod:`vates_b200.quant_kv`) is smaller still, for one head
+size and one common length. The kernels are in ``libvates_b200`` (no
+fallback).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ._lib import (VbKv8AppendArgs, VbKv8AttnArgs, VbKv8Cache, VbKv8ReadArgs, check, lib)
+from .pool import on_stream, ptr, stream_handle
+
+PAGE_SIZES = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128, 256)
+
+
+def _rows(t: torch.Tensor, what: str, shape) -> torch.Tensor:
+    """``t`` as bf16 rows on the GPU with contiguous dims (other strides stay)."""
+    if t.dtype != torch.bfloat16 or not t.is_cuda:
+        raise ValueError(f"{what}: a bfloat16 CUDA tensor is needed, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t if t.stride(3) == 1 else t.contiguous()
+
+
+def _ints(t: torch.Tensor | None, what: str, batch: int) -> int | None:
+    """Device pointer of a contiguous int32 ``[batch]`` tensor."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_cuda or t.numel() != batch or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 CUDA tensor of {batch} values is needed")
+    return t.data_ptr()
+
+
+class PagedKV8Cache:
+    """One layer's cache. The tensors are the caller's (or :meth:`empty`'s) and
+    may be shared between caches with different tables; a page that is written
+    must belong to one sequence only. ``page_table`` may be replaced or edited
+    in place between calls."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales, page_table):
+        if k_codes.dim() != 4 or page_table.dim() != 2:
+            raise ValueError("codes are [pages, kv_heads, page, head_dim], the table "
+                             "[batch, max_pages]")
+        pages, heads, page, dim = k_codes.shape
+        if page not in PAGE_SIZES or dim not in HEAD_DIMS:
+            raise ValueError(f"page of {page} rows (one of {PAGE_SIZES}), head_dim {dim} "
+                             f"(one of {HEAD_DIMS})")
+        for t, shape, dt in ((k_codes, k_codes.shape, torch.int8),
+                             (v_codes, k_codes.shape, torch.int8),
+                             (k_scales, (pages, heads), torch.float32),
+                             (v_scales, (pages, heads), torch.float32),
+                             (page_table, page_table.shape, torch.int32)):
+            if tuple(t.shape) != tuple(shape) or t.dtype != dt or not t.is_contiguous() \
+                    or not t.is_cuda:
+                raise ValueError(f"cache tensor: contiguous CUDA {dt} {tuple(shape)} is needed, "
+                                 f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+        self.k_codes, self.v_codes = k_codes, v_codes
+        self.k_scales, self.v_scales = k_scales, v_scales
+        self.pages, self.kv_heads, self.page, self.head_dim = pages, heads, page, dim
+        self.page_table = page_table
+        self._ws = {}
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, batch: int, max_pages: int,
+              page: int = 64, device="cuda"):
+        """A cache of ``pages`` unused pages whose table names none yet (-1)."""
+        codes = [torch.zeros((pages, kv_heads, page, head_dim), dtype=torch.int8, device=device)
+                 for _ in range(2)]
+        scales = [torch.zeros((pages, kv_heads), dtype=torch.float32, device=device)
+                  for _ in range(2)]
+        table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=device)
+        return cls(*codes, *scales, table)
+
+    @property
+    def batch(self) -> int:
+        return self.page_table.shape[0]
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in
+                   (self.k_codes, self.v_codes, self.k_scales, self.v_scales))
+
+    def _cache(self) -> VbKv8Cache:
+        t = self.page_table
+        return VbKv8Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(),
+                          self.k_scales.data_ptr(), self.v_scales.data_ptr(), t.data_ptr(),
+                          self.pages, self.kv_heads, self.page, self.head_dim, t.shape[0],
+                          t.shape[1])
+
+    # ------------------------------------------------------------------ write
+    def append(self, keys, values, pos, counts=None, pos_add: int = 0, status=None, stream=None):
+        """Quantise rows as they are written: row ``i < counts[b]`` (all ``n``
+        without ``counts``) of ``keys``/``values`` bf16 ``[batch, kv_heads, n,
+        head_dim]`` goes to position ``pos[b] + pos_add + i``. A page's scale is
+        max|x| / 127 over the rows it received; when new rows raise it, the
+        page's older codes are rounded again under the new scale. Rows past the
+        table set VB_STATUS_BOUNDS in ``status`` and are dropped; an infinity is
+        stored as the page's largest value, a NaN as 0, with
+        VB_STATUS_NONFINITE."""
+        B, n = self.page_table.shape[0], keys.shape[2] if keys.dim() == 4 else -1
+        shape = (B, self.kv_heads, n, self.head_dim)
+        with on_stream(stream):
+            keys, values = _rows(keys, "keys", shape), _rows(values, "values", shape)
+        a = VbKv8AppendArgs(self._cache(), keys.data_ptr(), values.data_ptr(),
+                            keys.stride()[:3], values.stride()[:3], _ints(pos, "pos", B),
+                            _ints(counts, "counts", B), ptr(status), pos_add, n)
+        check(lib.vb_kv8_append(C.byref(a), stream_handle(stream)), "vb_kv8_append")
+
+    # -------------------------------------------------------------- read back
+    def read(self, lens, n: int, start=None, status=None, stream=None):
+        """``(keys, values)`` bf16 ``[batch, kv_heads, n, head_dim]``: the rows
+        at positions ``start[b] + i`` (``start`` None: 0), zero from ``lens[b]``
+        on."""
+        B = self.page_table.shape[0]
+        dev = self.k_codes.device
+        shape = (B, self.kv_heads, n, self.head_dim)
+        with on_stream(stream):
+            keys = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+            values = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        a = VbKv8ReadArgs(self._cache(), _ints(lens, "lens", B), _ints(start, "start", B),
+                          keys.data_ptr(), values.data_ptr(), ptr(status), n)
+        check(lib.vb_kv8_read(C.byref(a), stream_handle(stream)), "vb_kv8_read")
+        return keys, values
+
+    # -------------------------------------------------------------- attention
+    def attend(self, q, lens, q_lens=None, len_add: int = 0, scale: float | None = None,
+               causal: bool = True, out=None, return_lse: bool = False, status=None, stream=None):
+        """``softmax(scale * q K^T) V`` over the ``lens[b] + len_add`` keys of
+        every sequence. ``q`` bf16 ``[batch, q_heads, L, head_dim]``; query row
+        ``i < q_lens[b]`` (``L`` without) is the sequence's row ``keys - q_lens
+        + i`` and with ``causal`` sees the keys up to itself. Rows that see
+        nothing, and rows from ``q_lens[b]`` on, are zero (log-sum-exp -inf).
+        Returns bf16 ``[batch, q_heads, L, head_dim]``, with ``return_lse``
+        also float32 ``[batch, q_heads, L]`` (natural log)."""
+        B, D = self.page_table.shape[0], self.head_dim
+        if q.dim() != 4:
+            raise ValueError(f"q: [batch, q_heads, L, head_dim] is needed, got {tuple(q.shape)}")
+        Hq, L = q.shape[1], q.shape[2]
+        with on_stream(stream):
+            q = _rows(q, "q", (B, Hq, L, D))
+            if out is None:
+                out = torch.empty((B, Hq, L, D), dtype=torch.bfloat16, device=q.device)
+            elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+                raise ValueError("out: contiguous bfloat16 of q's shape is needed")
+            lse = torch.empty((B, Hq, L), dtype=torch.float32,
+                              device=q.device) if return_lse else None
+        a = VbKv8AttnArgs(self._cache(), q.data_ptr(), q.stride()[:3], _ints(lens, "lens", B),
+                          _ints(q_lens, "q_lens", B), out.data_ptr(), ptr(lse), ptr(status),
+                          None, 0, D ** -0.5 if scale is None else scale, Hq, L, len_add,
+                          int(causal))
+        need = lib.vb_kv8_attn_workspace_size(C.byref(a))
+        st = stream_handle(stream)
+        if need:
+            ws = self._workspace(need, st, q.device, stream)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        check(lib.vb_kv8_attn(C.byref(a), st), "vb_kv8_attn")
+        return (out, lse) if return_lse else out
+
+    def _workspace(self, need: int, st: int, device, stream) -> torch.Tensor:
+        """Scratch of the key ranges' partial results, one per stream."""
+        ws = self._ws.get(st)
+        if ws is None or ws.numel() < need:
+            with on_stream(stream):
+                ws = self._ws[st] = torch.empty(need, dtype=torch.uint8, device=device)
+        return ws
+
+
+__all__ = ["PagedKV8Cache"]

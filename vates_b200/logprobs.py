@@ -1,0 +1,78 @@
+"""Log probabilities of given tokens, with rank, entropy and the best
+alternatives, in one pass over the logits (``vb_token_logprobs``)."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from ._lib import VbTokenLogprobsArgs, check, lib
+from .pool import on_stream, ptr, stream_handle
+
+MAX_TOP = 32
+_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+_workspaces: dict = {}
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor       # float32 [rows]: log p of the row's token
+    rank: torch.Tensor          # int32 [rows]: tokens ahead of it (0: the most likely)
+    entropy: torch.Tensor       # float32 [rows], nats
+    top_ids: torch.Tensor       # int32 [rows, top], best first, ties to the lowest id
+    top_logprobs: torch.Tensor  # float32 [rows, top]
+
+
+def _workspace(need: int, st: int, device, stream) -> torch.Tensor:
+    """Scratch of rows split over several CTAs, one per device and stream;
+    zeroed when made, left reusable by every call."""
+    key = (device, st)
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < need:
+        with on_stream(stream):
+            ws = _workspaces[key] = torch.zeros(max(need, 1 << 16), dtype=torch.uint8,
+                                                device=device)
+    return ws
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
+                   temperature: float = 1.0, status=None, stream=None) -> TokenLogprobs:
+    """``log_softmax(logits / temperature)`` of row ``r`` at ``tokens[r]`` and
+    what a server reports beside it.
+
+    ``logits`` bf16 or float32 ``[rows, vocab]`` (any row stride), ``tokens``
+    int32 ``[rows]``, ``top`` alternatives (0 to 32). Logits of -inf are tokens
+    that cannot follow. A NaN or +inf in a row makes its floating results NaN;
+    a token outside the vocabulary gives NaN and rank -1 and sets
+    VB_STATUS_BOUNDS in ``status``."""
+    if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
+        raise ValueError("logits: bfloat16 or float32 CUDA [rows, vocab] are needed, got "
+                         f"{logits.dtype} {tuple(logits.shape)} on {logits.device}")
+    rows, vocab = logits.shape
+    if tokens.dtype != torch.int32 or tuple(tokens.shape) != (rows,) or not tokens.is_cuda \
+            or not tokens.is_contiguous():
+        raise ValueError(f"tokens: contiguous int32 CUDA [{rows}] is needed, got {tokens.dtype} "
+                         f"{tuple(tokens.shape)}")
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top={top}: 0 to {MAX_TOP} and at most the vocabulary ({vocab})")
+    dev = logits.device
+    with on_stream(stream):
+        if logits.stride(1) != 1 and vocab > 1:
+            logits = logits.contiguous()
+        # one allocation: logprob, entropy, rank, then the top pairs
+        buf = torch.empty((3 + 2 * top) * rows, dtype=torch.float32, device=dev)
+    lp, ent = buf[:rows], buf[rows:2 * rows]
+    rank = buf[2 * rows:3 * rows].view(torch.int32)
+    ids = buf[3 * rows:(3 + top) * rows].view(torch.int32).view(rows, top)
+    tlp = buf[(3 + top) * rows:].view(rows, top)
+    st = stream_handle(stream)
+    ws = _workspace(lib.vb_token_logprobs_workspace_size(rows, vocab, top), st, dev, stream)
+    a = VbTokenLogprobsArgs(logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(),
+                            rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), ptr(status),
+                            ws.data_ptr(), ws.numel(), logits.stride(0), temperature, rows, vocab,
+                            top, _DTYPES[logits.dtype])
+    check(lib.vb_token_logprobs(C.byref(a), st), "vb_token_logprobs")
+    return TokenLogprobs(lp, rank, ent, ids, tlp)
+
+
+__all__ = ["TokenLogprobs", "token_logprobs"]

@@ -10,6 +10,7 @@ streaming, eviction or residency miss handling in the timed path.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -24,6 +25,12 @@ KEYS = ("gate_w", "gate_s", "gate_b", "up_w", "up_s", "up_b",
 def stream_handle(stream=None) -> int:
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+def on_stream(stream=None):
+    """Context in which new tensors belong to ``stream`` (None: the current
+    one), so that memory freed after a call on it is reused in its order."""
+    return nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
 def ptr(t) -> int | None:
