@@ -36,6 +36,7 @@ SOURCES = [
     "gdn_fused.cu",
     "kv8_cache.cu",
     "kv8_attn.cu",
+    "kv8_prefill.cu",
     "logprobs.cu",
 ]
 

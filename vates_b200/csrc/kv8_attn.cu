@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(KA_THREADS, 2) kv8_attn_kernel(Kv8AttnParams p
       const int dim0 = 32 * dg + 8 * c;
       if (p.splits > 1) {
         if (dg == 0 && c == 0)
-          p.ml_part[tile_id * ROWS + r] = make_float2(m[mt][u], ls);
+          p.ml_part[tile_id * ROWS + r] = make_float2(m[mt][u] - KV8_P_SHIFT, ls);
         if (t0 < t1) {
           float4 *dst = reinterpret_cast<float4 *>(p.o_part + (tile_id * ROWS + r) * D + dim0);
           dst[0] = make_float4(f[0] * vref, f[1] * vref, f[2] * vref, f[3] * vref);
@@ -487,27 +487,29 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_combine_kernel(Kv8AttnParams p
       make_uint2(pack_bf2(a.x * inv, a.y * inv), pack_bf2(a.z * inv, a.w * inv));
   if (p.lse && tid == 0)
     p.lse[row] =
-        ls == 0.f ? -INFINITY : (M - KV8_P_SHIFT + log2f(ls)) * 0.69314718055994531f;
+        ls == 0.f ? -INFINITY : (M + log2f(ls)) * 0.69314718055994531f;
 }
 
 // ---------------------------------------------------------------------- plan
 struct Kv8Plan {
   int tile_rows, row_tiles, splits;
+  bool tensor;
   size_t bytes;
 };
 
-// Rows per tile: 16 up to 16 rows per kv head, else 32. Key ranges: as many as
-// bring the grid to two CTAs on each of 148 SMs, and no more than there are
-// tiles of keys in the table.
+// Up to 32 rows per kv head: kv8_attn_kernel, row tiles of 16 or 32 and two
+// CTAs per SM; more rows: the tcgen05 kernel, one CTA per SM. Key ranges: as
+// many as fill 148 SMs, and no more than there are tiles of keys in the table.
 Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   Kv8Plan pl;
   const long long rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
-  pl.tile_rows = rows <= 16 ? 16 : 32;
+  pl.tensor = rows > 32;
+  pl.tile_rows = pl.tensor ? kv8_prefill_rows(a->cache.dim) : rows <= 16 ? 16 : 32;
   pl.row_tiles = (int)((rows + pl.tile_rows - 1) / pl.tile_rows);
   const long long base = (long long)a->cache.batch * a->cache.kv_heads * pl.row_tiles;
-  const long long kt = KA_TILE / a->cache.dim;
+  const long long kt = pl.tensor ? 128 : KA_TILE / a->cache.dim;
   const long long most = ((long long)a->cache.max_pages * a->cache.page + kt - 1) / kt;
-  long long s = 2 * 148 / base;
+  long long s = (pl.tensor ? 148 : 2 * 148) / base;
   s = s < 1 ? 1 : s > most ? most : s;
   pl.splits = (int)(s > KC_MAX_SPLITS ? KC_MAX_SPLITS : s);
   pl.bytes = pl.splits == 1 ? 0
@@ -528,10 +530,17 @@ int kv8_launch(const Kv8AttnParams &p, cudaStream_t s) {
   }
   vb_launch(kv8_attn_kernel<D, MT>, dim3(p.splits, p.c.kv_heads * p.row_tiles, p.c.batch),
             dim3(KA_THREADS), T::SMEM, s, false, p);
-  int rc = check_launch("kv8_attn_kernel");
+  return check_launch("kv8_attn_kernel");
+}
+
+template <int D>
+int kv8_run(const Kv8AttnParams &p, const Kv8Plan &pl, cudaStream_t s) {
+  const int rc = pl.tensor ? kv8_prefill_launch(p, s)
+                 : pl.tile_rows == 16 ? kv8_launch<D, 1>(p, s)
+                                      : kv8_launch<D, 2>(p, s);
   if (rc != VB_OK || p.splits == 1) return rc;
   vb_launch(kv8_combine_kernel<D>, dim3(p.c.batch * p.c.kv_heads * p.L * p.rep),
-            dim3(KC_THREADS), 0, s, true, p, 16 * MT);
+            dim3(KC_THREADS), 0, s, true, p, pl.tile_rows);
   return check_launch("kv8_combine_kernel");
 }
 
@@ -592,11 +601,10 @@ int vb_kv8_attn(const VbKv8AttnArgs *a, vb_stream_t stream) {
       p.o_part + (size_t)a->cache.batch * a->cache.kv_heads * pl.row_tiles * pl.splits *
                      pl.tile_rows * a->cache.dim);
   cudaStream_t s = as_stream(stream);
-  const bool small = pl.tile_rows == 16;
   switch (a->cache.dim) {
-    case 64: return small ? kv8_launch<64, 1>(p, s) : kv8_launch<64, 2>(p, s);
-    case 128: return small ? kv8_launch<128, 1>(p, s) : kv8_launch<128, 2>(p, s);
-    default: return small ? kv8_launch<256, 1>(p, s) : kv8_launch<256, 2>(p, s);
+    case 64: return kv8_run<64>(p, pl, s);
+    case 128: return kv8_run<128>(p, pl, s);
+    default: return kv8_run<256>(p, pl, s);
   }
 }
 

@@ -13,7 +13,8 @@ struct Kv8AttnParams {
   uint16_t *out;
   float *lse;
   int32_t *status;
-  // partial results of a key range: rows of float32 O, then (m, l) per row
+  // partial results of a key range: rows of float32 O, then (m, l) per row:
+  // the range's weights are 2^(z - m), their sum l
   float *o_part;
   float2 *ml_part;
   float scale_log2;  // scale * log2(e)
@@ -75,5 +76,9 @@ __device__ __forceinline__ uint32_t h2_codes(uint32_t magic) {
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(magic), "r"(0x64806480u));
   return r;
 }
+
+// Rows per row tile of the prefill kernel, and its launch (kv8_prefill.cu).
+int kv8_prefill_rows(int dim);
+int kv8_prefill_launch(const Kv8AttnParams &p, cudaStream_t s);
 
 }  // namespace vb
