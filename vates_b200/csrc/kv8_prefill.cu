@@ -287,26 +287,23 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
     constexpr int CT = 128 * H::CONV_WG, CPR = D / 16, STEP = CT / CPR, NC = KP_KT / STEP;
     const int ctid = tid - 128;
     const int ch = ctid % CPR, key0 = ctid / CPR;
-    int pid[NC];
     uint4 kr[NC], vr[NC];
-    auto load_ids = [&](int t) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int key = t * KP_KT + key0 + i * STEP;
-        pid[i] = t < t1 && key < kend
-                     ? kv8_page(table, p.c.max_pages, p.c.pages, key >> p.shift,
-                                ch == 0 ? p.status : nullptr)
-                     : -1;
-      }
+    // pool page of the 16-key group lane % 8 of tile t; rows without a page (past
+    // the last key, or flagged) read page 0: their weights are 0
+    auto group_page = [&](int t) {
+      const int key = t * KP_KT + (lane & 7) * 16;
+      return t < t1 && key < kend
+                 ? max(0, kv8_page(table, p.c.max_pages, p.c.pages, key >> p.shift, p.status)) : 0;
     };
-    auto load = [&](uint4 (&x)[NC], const int8_t *codes, int t) {  // a page not there: zeros
+    const size_t pool_step = (size_t)p.c.kv_heads * p.c.page * D;
+    const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + ch * 16;
+    const int8_t *vbase = p.c.v_codes + (size_t)h * p.c.page * D + ch * 16;
+    auto load = [&](uint4 (&x)[NC], const int8_t *base, int id) {
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const int key = t * KP_KT + key0 + i * STEP;
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (pid[i] >= 0)
-          x[i] = ldg_nc_v4(codes + (((size_t)pid[i] * p.c.kv_heads + h) * p.c.page +
-                                    (key & (p.c.page - 1))) * D + ch * 16);
+        const int key = key0 + i * STEP;  // a tile starts on a page boundary (page <= 128)
+        const int pg = __shfl_sync(0xffffffffu, id, key >> 4);
+        x[i] = ldg_nc_v4(base + pg * pool_step + (key & (p.c.page - 1)) * D);
       }
     };
     // 16 codes -> two 16-byte chunks; neighbouring 64-dim blocks store them in
@@ -338,28 +335,35 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(full);
     };
-    load_ids(t0);
-    load(kr, p.c.k_codes, t0);
+    // K runs a tile ahead of V: S of the next tile is issued before O of this one
+    auto wait = [&](uint64_t *m, int n) {  // n-th completion of a barrier (n < 0: none needed)
+      if (n >= 0 && !tc::mbar_wait(m, (uint32_t)(n & 1), abort, KP_WAIT_NS)) s_abort = 1;
+      return !__any_sync(0xffffffffu, *abort != 0);
+    };
+    int id_v = group_page(t0), id_k = group_page(t0 + 1);  // of tiles n + 1 and n + 2
+    load(kr, kbase, id_v);
+    load(vr, vbase, id_v);
     bool ok = true;
-    for (int t = t0; t < t1 && ok; ++t) {
-      const int n = t - t0, st = n % ST;
-      load(vr, p.c.v_codes, t);
-      load_ids(t + 1);
-      if (n >= ST && !tc::mbar_wait(&bar.k_empty[st], (uint32_t)((n / ST - 1) & 1), abort,
-                                    KP_WAIT_NS))
-        s_abort = 1;
-      ok = !__any_sync(0xffffffffu, *abort != 0);
-      if (!ok) break;
-      store(kr, smem + H::K_OFF + st * H::TILE);
-      publish(&bar.k_full[st]);
-      load(kr, p.c.k_codes, t + 1);
-      if (n >= ST && !tc::mbar_wait(&bar.v_empty[st], (uint32_t)((n / ST - 1) & 1), abort,
-                                    KP_WAIT_NS))
-        s_abort = 1;
-      ok = !__any_sync(0xffffffffu, *abort != 0);
-      if (!ok) break;
-      store(vr, smem + H::V_OFF + st * H::TILE);
-      publish(&bar.v_full[st]);
+    for (int n = -1; n < t1 - t0; ++n) {  // K of tile n + 1, V of tile n
+      const int id_next = group_page(t0 + n + 3);
+      if (n + 1 < t1 - t0) {
+        const int st = (n + 1) % ST;
+        ok = wait(&bar.k_empty[st], (n + 1) / ST - 1);
+        if (!ok) break;
+        store(kr, smem + H::K_OFF + st * H::TILE);
+        publish(&bar.k_full[st]);
+        load(kr, kbase, id_k);
+      }
+      if (n >= 0) {
+        const int st = n % ST;
+        ok = wait(&bar.v_empty[st], n / ST - 1);
+        if (!ok) break;
+        store(vr, smem + H::V_OFF + st * H::TILE);
+        publish(&bar.v_full[st]);
+        load(vr, vbase, id_v);
+      }
+      id_v = id_k;
+      id_k = id_next;
     }
   } else {
     // ================================================== softmax, a thread per row

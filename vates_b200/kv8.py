@@ -29,7 +29,7 @@ def _rows(t: torch.Tensor, what: str, shape) -> torch.Tensor:
     """``t`` as bf16 rows on the GPU with contiguous dims (other strides stay)."""
     if t.dtype != torch.bfloat16 or not t.is_cuda:
         raise ValueError(f"{what}: a bfloat16 CUDA tensor is needed, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     return t if t.stride(3) == 1 else t.contiguous()
 
@@ -46,13 +46,12 @@ def _ints(t: torch.Tensor | None, what: str, batch: int) -> int | None:
 class PagedKV8Cache:
     """One layer's cache. The tensors are the caller's (or :meth:`empty`'s) and
     may be shared between caches with different tables; a page that is written
-    must belong to one sequence only. ``page_table`` may be replaced or edited
-    in place between calls."""
+    must belong to one sequence only. The table may be edited in place or
+    replaced (:attr:`page_table`) between calls."""
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales, page_table):
-        if k_codes.dim() != 4 or page_table.dim() != 2:
-            raise ValueError("codes are [pages, kv_heads, page, head_dim], the table "
-                             "[batch, max_pages]")
+        if k_codes.dim() != 4:
+            raise ValueError("codes are [pages, kv_heads, page, head_dim]")
         pages, heads, page, dim = k_codes.shape
         if page not in PAGE_SIZES or dim not in HEAD_DIMS:
             raise ValueError(f"page of {page} rows (one of {PAGE_SIZES}), head_dim {dim} "
@@ -60,8 +59,7 @@ class PagedKV8Cache:
         for t, shape, dt in ((k_codes, k_codes.shape, torch.int8),
                              (v_codes, k_codes.shape, torch.int8),
                              (k_scales, (pages, heads), torch.float32),
-                             (v_scales, (pages, heads), torch.float32),
-                             (page_table, page_table.shape, torch.int32)):
+                             (v_scales, (pages, heads), torch.float32)):
             if tuple(t.shape) != tuple(shape) or t.dtype != dt or not t.is_contiguous() \
                     or not t.is_cuda:
                 raise ValueError(f"cache tensor: contiguous CUDA {dt} {tuple(shape)} is needed, "
@@ -69,8 +67,27 @@ class PagedKV8Cache:
         self.k_codes, self.v_codes = k_codes, v_codes
         self.k_scales, self.v_scales = k_scales, v_scales
         self.pages, self.kv_heads, self.page, self.head_dim = pages, heads, page, dim
-        self.page_table = page_table
         self._ws = {}
+        self.page_table = page_table
+
+    @property
+    def page_table(self) -> torch.Tensor:
+        return self._table
+
+    @page_table.setter
+    def page_table(self, t: torch.Tensor):
+        if t.dim() != 2 or t.dtype != torch.int32 or not t.is_contiguous() or not t.is_cuda:
+            raise ValueError("page_table: a contiguous int32 CUDA [batch, max_pages] tensor is "
+                             f"needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        self._table = t
+        self.batch = t.shape[0]
+        # argument structures with the cache filled in, copied for each call
+        c = VbKv8Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(),
+                       self.k_scales.data_ptr(), self.v_scales.data_ptr(), t.data_ptr(),
+                       self.pages, self.kv_heads, self.page, self.head_dim, *t.shape)
+        self._append_args = bytes(VbKv8AppendArgs(c))
+        self._read_args = bytes(VbKv8ReadArgs(c))
+        self._attn_args = bytes(VbKv8AttnArgs(c))
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, batch: int, max_pages: int,
@@ -84,20 +101,9 @@ class PagedKV8Cache:
         return cls(*codes, *scales, table)
 
     @property
-    def batch(self) -> int:
-        return self.page_table.shape[0]
-
-    @property
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in
                    (self.k_codes, self.v_codes, self.k_scales, self.v_scales))
-
-    def _cache(self) -> VbKv8Cache:
-        t = self.page_table
-        return VbKv8Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(),
-                          self.k_scales.data_ptr(), self.v_scales.data_ptr(), t.data_ptr(),
-                          self.pages, self.kv_heads, self.page, self.head_dim, t.shape[0],
-                          t.shape[1])
 
     # ------------------------------------------------------------------ write
     def append(self, keys, values, pos, counts=None, pos_add: int = 0, status=None, stream=None):
@@ -109,13 +115,15 @@ class PagedKV8Cache:
         table set VB_STATUS_BOUNDS in ``status`` and are dropped; an infinity is
         stored as the page's largest value, a NaN as 0, with
         VB_STATUS_NONFINITE."""
-        B, n = self.page_table.shape[0], keys.shape[2] if keys.dim() == 4 else -1
+        B, n = self.batch, keys.shape[2] if keys.dim() == 4 else -1
         shape = (B, self.kv_heads, n, self.head_dim)
         with on_stream(stream):
             keys, values = _rows(keys, "keys", shape), _rows(values, "values", shape)
-        a = VbKv8AppendArgs(self._cache(), keys.data_ptr(), values.data_ptr(),
-                            keys.stride()[:3], values.stride()[:3], _ints(pos, "pos", B),
-                            _ints(counts, "counts", B), ptr(status), pos_add, n)
+        a = VbKv8AppendArgs.from_buffer_copy(self._append_args)
+        a.keys, a.values = keys.data_ptr(), values.data_ptr()
+        a.k_strides, a.v_strides = keys.stride()[:3], values.stride()[:3]
+        a.pos, a.counts = _ints(pos, "pos", B), _ints(counts, "counts", B)
+        a.status, a.pos_add, a.n = ptr(status), pos_add, n
         check(lib.vb_kv8_append(C.byref(a), stream_handle(stream)), "vb_kv8_append")
 
     # -------------------------------------------------------------- read back
@@ -123,14 +131,15 @@ class PagedKV8Cache:
         """``(keys, values)`` bf16 ``[batch, kv_heads, n, head_dim]``: the rows
         at positions ``start[b] + i`` (``start`` None: 0), zero from ``lens[b]``
         on."""
-        B = self.page_table.shape[0]
-        dev = self.k_codes.device
-        shape = (B, self.kv_heads, n, self.head_dim)
+        B = self.batch
         with on_stream(stream):
-            keys = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-            values = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-        a = VbKv8ReadArgs(self._cache(), _ints(lens, "lens", B), _ints(start, "start", B),
-                          keys.data_ptr(), values.data_ptr(), ptr(status), n)
+            keys = torch.empty((B, self.kv_heads, n, self.head_dim), dtype=torch.bfloat16,
+                               device=self.k_codes.device)
+            values = torch.empty_like(keys)
+        a = VbKv8ReadArgs.from_buffer_copy(self._read_args)
+        a.lens, a.start = _ints(lens, "lens", B), _ints(start, "start", B)
+        a.keys, a.values = keys.data_ptr(), values.data_ptr()
+        a.status, a.n = ptr(status), n
         check(lib.vb_kv8_read(C.byref(a), stream_handle(stream)), "vb_kv8_read")
         return keys, values
 
@@ -144,22 +153,25 @@ class PagedKV8Cache:
         nothing, and rows from ``q_lens[b]`` on, are zero (log-sum-exp -inf).
         Returns bf16 ``[batch, q_heads, L, head_dim]``, with ``return_lse``
         also float32 ``[batch, q_heads, L]`` (natural log)."""
-        B, D = self.page_table.shape[0], self.head_dim
+        B, D = self.batch, self.head_dim
         if q.dim() != 4:
             raise ValueError(f"q: [batch, q_heads, L, head_dim] is needed, got {tuple(q.shape)}")
         Hq, L = q.shape[1], q.shape[2]
+        lse = None
         with on_stream(stream):
             q = _rows(q, "q", (B, Hq, L, D))
             if out is None:
-                out = torch.empty((B, Hq, L, D), dtype=torch.bfloat16, device=q.device)
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
             elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
                 raise ValueError("out: contiguous bfloat16 of q's shape is needed")
-            lse = torch.empty((B, Hq, L), dtype=torch.float32,
-                              device=q.device) if return_lse else None
-        a = VbKv8AttnArgs(self._cache(), q.data_ptr(), q.stride()[:3], _ints(lens, "lens", B),
-                          _ints(q_lens, "q_lens", B), out.data_ptr(), ptr(lse), ptr(status),
-                          None, 0, D ** -0.5 if scale is None else scale, Hq, L, len_add,
-                          int(causal))
+            if return_lse:
+                lse = torch.empty((B, Hq, L), dtype=torch.float32, device=q.device)
+        a = VbKv8AttnArgs.from_buffer_copy(self._attn_args)
+        a.q, a.q_strides = q.data_ptr(), q.stride()[:3]
+        a.lens, a.q_lens = _ints(lens, "lens", B), _ints(q_lens, "q_lens", B)
+        a.out, a.lse, a.status = out.data_ptr(), ptr(lse), ptr(status)
+        a.scale = D ** -0.5 if scale is None else scale
+        a.q_heads, a.L, a.len_add, a.causal = Hq, L, len_add, causal
         need = lib.vb_kv8_attn_workspace_size(C.byref(a))
         st = stream_handle(stream)
         if need:

@@ -59,12 +59,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     with on_stream(stream):
         if logits.stride(1) != 1 and vocab > 1:
             logits = logits.contiguous()
-        # one allocation: logprob, entropy, rank, then the top pairs
-        buf = torch.empty((3 + 2 * top) * rows, dtype=torch.float32, device=dev)
-    lp, ent = buf[:rows], buf[rows:2 * rows]
-    rank = buf[2 * rows:3 * rows].view(torch.int32)
-    ids = buf[3 * rows:(3 + top) * rows].view(torch.int32).view(rows, top)
-    tlp = buf[(3 + top) * rows:].view(rows, top)
+        lp = logits.new_empty(rows, dtype=torch.float32)
+        ent = torch.empty_like(lp)
+        rank = torch.empty_like(tokens)
+        tlp = lp.new_empty((rows, top))
+        ids = rank.new_empty((rows, top))
     st = stream_handle(stream)
     ws = _workspace(lib.vb_token_logprobs_workspace_size(rows, vocab, top), st, dev, stream)
     a = VbTokenLogprobsArgs(logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(),

@@ -23,8 +23,10 @@ KEYS = ("gate_w", "gate_s", "gate_b", "up_w", "up_s", "up_b",
 
 
 def stream_handle(stream=None) -> int:
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is None:
+        # the handle of torch.cuda.current_stream() without building its object
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return stream.cuda_stream
 
 
 def on_stream(stream=None):
