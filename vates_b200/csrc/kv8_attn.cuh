@@ -17,9 +17,16 @@ struct Kv8AttnParams {
   // the range's weights are 2^(z - m), their sum l
   float *o_part;
   float2 *ml_part;
+  int2 *units;  // kv8_attn_kernel: first CTA and number of CTAs of a unit
   float scale_log2;  // scale * log2(e)
   int Hq, L, rep, len_add, causal, shift, vec;
   int row_tiles, splits;
+  uint32_t rep_inv;  // floor(2^32 / rep) + 1
+  // Query row R (< 2^24) of the flattened (row, head of the group) order is
+  // query R / rep: exact by one product while R * rep < 2^32.
+  __device__ __forceinline__ int row_of(int R) const {
+    return rep == 1 ? R : (int)__umulhi((uint32_t)R, rep_inv);
+  }
 };
 
 // A row tile's share of the sequence: query row R of the flattened (row, head

@@ -144,8 +144,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
   const int i_last = min(min(r_base + ROWS, rows) - 1, sp.q_len * p.rep - 1) / p.rep;
   const int kend = r_base < sp.q_len * p.rep ? sp.visible(i_last) : 0;
   const int tiles = (kend + KP_KT - 1) / KP_KT;
-  const int t0 = (int)((long long)tiles * split / p.splits);
-  const int t1 = (int)((long long)tiles * (split + 1) / p.splits);
+  const int share = tiles / p.splits, rest = tiles % p.splits;
+  const int t0 = split * share + min(split, rest);
+  const int t1 = t0 + share + (split < rest);
   const int n_items = (t1 - t0) * NT;
   const size_t tile_id = (((size_t)b * p.c.kv_heads + h) * p.row_tiles + rt) * p.splits + split;
   const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
   // ---- queries: a warp per row, f16 after the row's power of two
   for (int r = warp; r < ROWS; r += KP_THREADS / 32) {
     constexpr int PL = D / 32;
-    const int R = r_base + r, i = R / p.rep, hr = R % p.rep;
+    const int R = r_base + r, i = p.row_of(R), hr = R - i * p.rep;
     const bool valid = n_items > 0 && R < rows && i < sp.q_len;
     const uint16_t *src = p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql +
                           lane * PL;
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
     kp_regs_inc<H::R_SOFT>();
     const int tile = wg - 1 - H::CONV_WG;
     const int r = tile * 128 + (tid & 127), R = r_base + r;
-    const int vis = R < rows ? sp.visible(R / p.rep) : 0;
+    const int vis = R < rows ? sp.visible(p.row_of(R)) : 0;
     const float fac = s_fac[r];
     const uint32_t trow = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
     const bool one = t1 - t0 == 1;
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
     }
     if (ok) {
       const float v = kv8_ex2(lvref);
-      const int i = R / p.rep, hr = R % p.rep;
+      const int i = p.row_of(R), hr = R - i * p.rep;
       const size_t row = ((size_t)b * p.Hq + h * p.rep + hr) * p.L + i;
       const bool live = R < rows;
       if (p.splits > 1) {
