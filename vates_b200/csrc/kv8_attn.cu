@@ -9,36 +9,44 @@
 // after a factor s_V(page) / v, v the largest V scale so far; l is summed in
 // float32 from the unrounded weights.
 //
-// A CTA (8 warps) owns an equal share of all sequences' key tiles (16 KB of K
-// and of V each) and all query rows, up to 32, of the kv head it is at. cp.async
-// brings the tiles into a ring (the rows
-// of a page are contiguous; chunks of 16 bytes are XOR-swizzled so that both
-// fragment reads below are free of bank conflicts):
-//   S: warp w takes 2048 / D keys of the tile over all of D; lane (g, c) of an
-//      8-key group reads 16 consecutive bytes of key g, four k-steps of the
-//      product (the order of dims within a 64-dim span is the same permutation
-//      for q);
-//   max over the warps through shared memory, weights as PV's A fragments;
-//   PV: warp takes 32 dims and four 16-key steps; lane (g, c) reads 4 bytes of
-//      its four keys and interleaves them into key pairs.
+// A CTA (4 warps, two or three CTAs per SM) owns an equal share of all sequences' key
+// tiles (16 KB of K and of V each) and all query rows, up to 32, of the kv head
+// it is at. cp.async brings the tiles into a ring (the rows of a page are
+// contiguous; chunks of 16 bytes are XOR-swizzled so that both fragment reads
+// below are free of bank conflicts). Both products are transposed, so that rows
+// come in eights and a converted K or V fragment serves every group of rows:
+//   S^T = K q^T: a warp takes 4096 / D keys; lane (g, c) reads 16 consecutive
+//      bytes of keys g and g + 8, four k-steps of the product (the order of
+//      dims within a 64-dim span is the same permutation for q);
+//   O^T += V^T P^T: a warp takes D / 4 dims of every key; lane (g, c) reads 4
+//      bytes of its four keys and interleaves them into key pairs.
+// The running maximum and the largest V scale only move when a score passes the
+// maximum by 2^2 or a tile brings a larger scale: all warps then meet, take the
+// new values and form the weights again. Otherwise the weights stand as
+// they are and a tile costs two barriers.
 // Shares of one (sequence, kv head) meet in kv8_combine_kernel.
 #include "kv8_attn.cuh"
 
 namespace vb {
 namespace {
 
-constexpr int KA_THREADS = 256;
-constexpr int KA_TILE = 16384;  // bytes of K, and of V, per tile
+constexpr int KA_THREADS = 128;
+constexpr int KA_TILE = 16384;          // bytes of K, and of V, per tile
+constexpr int KA_STAGES = 2;
+constexpr float KA_SHIFT = 13.f;        // weights as f16 are at most 2^(13 + 2)
+constexpr float KA_MOVE = 2.f;
 
-template <int D, int MT>
+template <int D, int NR>  // NR groups of 8 query rows
 struct Kv8Tile {
-  static constexpr int KT = KA_TILE / D;            // keys per tile
-  static constexpr int NTW = KT / 64;               // 8-key groups per warp
-  static constexpr int NKG = KT / 64;               // key groups of PV (32-dim groups: 8 / NKG)
-  static constexpr int STAGES = MT == 1 ? 3 : 2;
-  static constexpr int Q_BYTES = MT * D / 16 * 512;
-  static constexpr int P_BYTES = MT * KT / 16 * 512;
-  static constexpr int RING = STAGES * 2 * KA_TILE;
+  static constexpr int KT = KA_TILE / D;     // keys per tile
+  static constexpr int CTAS = NR > 2 ? 2 : 3;  // per SM (shared memory, registers)
+  static constexpr int MW = KT / 64;         // 16-key groups per warp (S)
+  static constexpr int DW = D / 4;           // dims per warp (PV)
+  static constexpr int ND = DW >= 32 ? DW / 32 : 1;  // 32-dim groups per warp (16 dims: D = 64)
+  static constexpr int NM = DW / 16;         // 16-dim fragments per warp
+  static constexpr int RING = KA_STAGES * 2 * KA_TILE;
+  static constexpr int Q_BYTES = NR * D * 16;
+  static constexpr int P_BYTES = NR * KT * 16;
   static constexpr int SMEM = RING + Q_BYTES + P_BYTES;
 };
 
@@ -107,17 +115,22 @@ __device__ __forceinline__ unsigned long long kv8_all_tiles(const Kv8AttnParams 
   return y;
 }
 
-template <int D, int MT>
-__global__ void __launch_bounds__(KA_THREADS, 2) kv8_attn_kernel(Kv8AttnParams p) {
-  using T = Kv8Tile<D, MT>;
-  constexpr int KT = T::KT, ROWS = 16 * MT;
+__device__ __forceinline__ void ldsm_x2_trans(uint32_t &r0, uint32_t &r1, const void *p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+               : "=r"(r0), "=r"(r1)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)));
+}
+
+template <int D, int NR>
+__global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_kernel(Kv8AttnParams p) {
+  using T = Kv8Tile<D, NR>;
+  constexpr int KT = T::KT, ROWS = 8 * NR, MW = T::MW, NM = T::NM;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint4 *s_q = reinterpret_cast<uint4 *>(smem + T::RING);                // [MT][D/16][32]
-  uint32_t *s_p = reinterpret_cast<uint32_t *>(smem + T::RING + T::Q_BYTES);  // [MT][KT/16][32][4]
-  __shared__ __align__(16) float s_max[ROWS][8];
-  __shared__ float s_fac[ROWS], s_l[8][ROWS];
+  uint32_t *s_q = reinterpret_cast<uint32_t *>(smem + T::RING);  // [NR][D/32][32 lanes][4]
+  uint8_t *s_p = smem + T::RING + T::Q_BYTES;                    // f16 [NR][KT keys][8 rows]
+  __shared__ float s_fac[ROWS], s_max[4][ROWS], s_l[4][ROWS];
   __shared__ unsigned long long s_sum[KA_THREADS / 32], s_begin;
-  __shared__ int s_b;
+  __shared__ int s_b, s_move[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   pdl_launch_dependents();
   pdl_wait();
@@ -160,10 +173,22 @@ __global__ void __launch_bounds__(KA_THREADS, 2) kv8_attn_kernel(Kv8AttnParams p
   }
 
   // thread owns chunk tid % (D/16) of keys tid / (D/16) + i * STEP of a tile
-  constexpr int CPR = D / 16, STEP = KA_THREADS / CPR, NG = KT / 16;
+  constexpr int CPR = D / 16, STEP = KA_THREADS / CPR, NC = KT / STEP, NG = KT / 16;
   const int ch = tid % CPR, key0 = tid / CPR;
   const uint32_t pool_step = (uint32_t)(H * p.c.page * D);
-  const int kg = warp % T::NKG, dg = warp / T::NKG;
+  // Offsets in a stage (K, then V): the copy's first chunk; the first key of
+  // this warp's 16-key groups, spans of 64 dims of either parity (the swizzle of
+  // a key is the same 8 keys on); the first two keys of this lane's PV step.
+  const uint32_t copy_at = ka_chunk<D>(key0, ch);
+  const uint32_t k_at0 = ka_chunk<D>(16 * warp * MW + g, c), k_at1 = k_at0 ^ 64;
+  const int v_ch = D == 64 ? warp : 2 * T::ND * warp + (g >> 2);
+  const uint32_t v_in = D == 64 ? g * 2 : (g & 3) * 4;
+  const uint32_t v_at0 = KA_TILE + ka_chunk<D>(2 * c, v_ch) + v_in;
+  const uint32_t v_at1 = KA_TILE + ka_chunk<D>(2 * c + 1, v_ch) + v_in;
+  // (32 dims on, two chunks: the swizzle flips bits 1 and 2 of the chunk number)
+  const uint32_t v_next0 = D == 256 ? KA_TILE + ka_chunk<D>(2 * c, v_ch + 2) + v_in - v_at0 : 0;
+  const uint32_t v_next1 =
+      D == 256 ? KA_TILE + ka_chunk<D>(2 * c + 1, v_ch + 2) + v_in - v_at1 : 0;
 
   while (w0 < w1) {
     // ---- the unit at w0: sequence b, head h, tiles [t0, t1) of `tiles`
@@ -199,33 +224,31 @@ __global__ void __launch_bounds__(KA_THREADS, 2) kv8_attn_kernel(Kv8AttnParams p
       ks = id >= 0 ? __ldg(p.c.k_scales + (size_t)id * H + h) : -1.f;
       vs = id >= 0 ? __ldg(p.c.v_scales + (size_t)id * H + h) : 0.f;
     };
-    auto issue = [&](int t, int id) {
-      uint8_t *kb = smem + (t % T::STAGES) * 2 * KA_TILE, *vb = kb + KA_TILE;
+    auto issue = [&](int t, int stage, int id) {
+      uint8_t *dst = smem + stage * (2 * KA_TILE) + copy_at;
+      const int in_page = (t * KT) & (p.c.page - 1);  // 0 unless a page is longer than a tile
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NC; ++i) {
         const int kl = key0 + i * STEP;
         const uint32_t pg = (uint32_t)max(0, __shfl_sync(0xffffffffu, id, kl >> 4));
         const unsigned long long at = (unsigned long long)pg * pool_step +
-                                      ((t * KT + kl) & (p.c.page - 1)) * D;
-        const uint32_t so = ka_chunk<D>(kl, ch);
-        cp_async16(kb + so, kbase + at);
-        cp_async16(vb + so, vbase + at);
+                                      (uint32_t)((in_page + (kl & (p.c.page - 1))) * D);
+        cp_async16(dst + i * STEP * D, kbase + at);
+        cp_async16(dst + KA_TILE + i * STEP * D, vbase + at);
       }
     };
-    int id_next = group_page(t0);
+    // pages of the tiles t + 1 (id1) and t + 2 (id2) at the start of tile t
+    int id1 = group_page(t0);
     float ks_l, vs_l;
-    group_scales(id_next, ks_l, vs_l);
-#pragma unroll
-    for (int s = 0; s < T::STAGES - 1; ++s) {
-      if (t0 + s < t1) issue(t0 + s, id_next);
-      cp_async_commit();
-      id_next = group_page(t0 + s + 1);
-    }
-    // scales run one tile ahead of their use, page numbers with the copies
-    int id_scale = T::STAGES == 2 ? id_next : group_page(t0 + 1);
+    group_scales(id1, ks_l, vs_l);
+    issue(t0, 0, id1);
+    cp_async_commit();
+    id1 = group_page(t0 + 1);
+    int id2 = group_page(t0 + 2);
+    if (tid < 2) s_move[tid] = 0;
 
-    // ---- queries, in the order of the A fragments
-    for (int r = warp; r < ROWS; r += 8) {
+    // ---- queries, in the order of the B fragments
+    for (int r = warp; r < ROWS; r += 4) {
       const int i = p.row_of(r), hr = r - i * p.rep;
       constexpr int PL = D / 32;  // elements per lane
       float x[PL];
@@ -261,274 +284,274 @@ __global__ void __launch_bounds__(KA_THREADS, 2) kv8_attn_kernel(Kv8AttnParams p
       if (lane == 0) s_fac[r] = p.scale_log2 / pw;
 #pragma unroll
       for (int j = 0; j < PL; j += 2) {
-        const int d = lane * PL + j, span = d >> 6, y = d & 15;
-        const int fl = (r & 7) * 4 + ((d & 63) >> 4), reg = ((y & 2) ? 2 : 0) + ((r >> 3) & 1);
-        uint32_t *dst = reinterpret_cast<uint32_t *>(
-            s_q + ((r >> 4) * (D / 16) + span * 4 + (y >> 2)) * 32 + fl);
-        dst[reg] = pack_h2(x[j] * pw, x[j + 1] * pw);
+        // dim d = 64 span + 16 c + 4 step + y: lane (row, c), register pair of the step
+        const int d = lane * PL + j, step = (d >> 6) * 4 + ((d & 15) >> 2);
+        const int fl = (r & 7) * 4 + ((d & 63) >> 4);
+        s_q[(((r >> 3) * (D / 32) + (step >> 1)) * 32 + fl) * 4 + (step & 1) * 2 +
+            ((d & 2) >> 1)] = pack_h2(x[j] * pw, x[j + 1] * pw);
       }
     }
 
-    int vis[MT][2];
-    float fac[MT][2], m[MT][2], l[MT][2];
-    float o[MT][4][4];
+    // row 8 n + 2 c + u of this lane
+    int vis[NR][2];
+    float fac[NR][2], m[NR][2], l[NR][2];
+    float o[NM][NR][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int r = mt * 16 + g + 8 * u;
-        vis[mt][u] = r < rows ? sp.visible(p.row_of(r)) : 0;
-        m[mt][u] = -INFINITY;
-        l[mt][u] = 0.f;
+        const int r = n * 8 + 2 * c + u;
+        vis[n][u] = r < rows ? sp.visible(p.row_of(r)) : 0;
+        m[n][u] = -INFINITY;
+        l[n][u] = 0.f;
       }
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int i = 0; i < NM; ++i)
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) o[mt][n][u] = 0.f;
-    float vref = 0.f;
+        for (int u = 0; u < 4; ++u) o[i][n][u] = 0.f;
+    float vref = 0.f, vinv = 0.f;
     __syncthreads();
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) fac[mt][u] = s_fac[mt * 16 + g + 8 * u];
+      for (int u = 0; u < 2; ++u) fac[n][u] = s_fac[n * 8 + 2 * c + u];
 
+    int stage = 0;
     for (int t = t0; t < t1; ++t) {
-      cp_async_wait<T::STAGES - 2>();
+      cp_async_wait<0>();
       __syncthreads();  // tile t is in; every warp is done with tile t - 1
-      if (t + T::STAGES - 1 < t1) {
-        issue(t + T::STAGES - 1, id_next);
-        id_next = group_page(t + T::STAGES);
-      }
+      if (t + 1 < t1) issue(t + 1, stage ^ 1, id1);
       cp_async_commit();
+      if (tid == 0) s_move[(t + 1) & 1] = 0;
       float ks_n, vs_n;  // of tile t + 1
-      group_scales(id_scale, ks_n, vs_n);
-      id_scale = group_page(t + 2);
-      const uint8_t *kb = smem + (t % T::STAGES) * 2 * KA_TILE, *vb = kb + KA_TILE;
+      group_scales(id1, ks_n, vs_n);
+      id1 = id2;
+      id2 = group_page(t + 3);
+      const uint8_t *st = smem + stage * (2 * KA_TILE);
+      stage ^= 1;
 
-      // ---- S = q K^T
-      float acc[MT][T::NTW][4];
+      // ---- S^T = K q^T
+      float acc[MW][NR][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int j = 0; j < MW; ++j)
 #pragma unroll
-        for (int j = 0; j < T::NTW; ++j)
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) acc[mt][j][u] = 0.f;
+          for (int u = 0; u < 4; ++u) acc[j][n][u] = 0.f;
 #pragma unroll
       for (int s = 0; s < D / 64; ++s) {
-        uint4 kw[T::NTW];
 #pragma unroll
-        for (int j = 0; j < T::NTW; ++j) {
-          kw[j] = *reinterpret_cast<const uint4 *>(
-              kb + ka_chunk<D>(8 * (warp * T::NTW + j) + g, 4 * s + c));
-          kw[j].x ^= 0x80808080u; kw[j].y ^= 0x80808080u;
-          kw[j].z ^= 0x80808080u; kw[j].w ^= 0x80808080u;
-        }
+        for (int j = 0; j < MW; ++j) {
+          const uint8_t *kp = st + ((s & 1) ? k_at1 : k_at0) + 16 * j * D + (s >> 1) * 128;
+          const uint4 lo = *reinterpret_cast<const uint4 *>(kp);
+          const uint4 hi = *reinterpret_cast<const uint4 *>(kp + 8 * D);
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          uint4 a[MT];
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const uint32_t w = (r4 == 0 ? lo.x : r4 == 1 ? lo.y : r4 == 2 ? lo.z : lo.w) ^ 0x80808080u;
+            const uint32_t v = (r4 == 0 ? hi.x : r4 == 1 ? hi.y : r4 == 2 ? hi.z : hi.w) ^ 0x80808080u;
+            const uint4 a = make_uint4(h2_codes(__byte_perm(w, 0x64646464u, 0x4140)),
+                                       h2_codes(__byte_perm(v, 0x64646464u, 0x4140)),
+                                       h2_codes(__byte_perm(w, 0x64646464u, 0x4342)),
+                                       h2_codes(__byte_perm(v, 0x64646464u, 0x4342)));
+            const int step = s * 4 + r4;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) a[mt] = s_q[(mt * (D / 16) + s * 4 + r4) * 32 + lane];
-#pragma unroll
-          for (int j = 0; j < T::NTW; ++j) {
-            const uint32_t w = r4 == 0 ? kw[j].x : r4 == 1 ? kw[j].y : r4 == 2 ? kw[j].z : kw[j].w;
-            const uint32_t b0 = h2_codes(__byte_perm(w, 0x64646464u, 0x4140));
-            const uint32_t b1 = h2_codes(__byte_perm(w, 0x64646464u, 0x4342));
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_f16(acc[mt][j], a[mt], b0, b1);
+            for (int n = 0; n < NR; ++n) {
+              const uint2 bq = *reinterpret_cast<const uint2 *>(
+                  s_q + ((n * (D / 32) + (step >> 1)) * 32 + lane) * 4 + (step & 1) * 2);
+              mma_f16(acc[j][n], a, bq.x, bq.y);
+            }
           }
         }
       }
 
-      // ---- scores, their maximum over the tile
+      // ---- scores; does a row's maximum or the V scale have to move?
       float vmax = vs_l;
 #pragma unroll
       for (int o2 = NG / 2; o2 > 0; o2 >>= 1)
         vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o2));
-      float tmax[MT][2], vfac[T::NTW];
+      float vs[MW];
+      bool over = vmax > vref;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) tmax[mt][0] = tmax[mt][1] = -INFINITY;
+      for (int j = 0; j < MW; ++j) {
+        const int grp = warp * MW + j;
+        const float ks = __shfl_sync(0xffffffffu, ks_l, grp);
+        vs[j] = __shfl_sync(0xffffffffu, vs_l, grp);
+        const int key = ks < 0.f ? 0x7fffffff - 64 : t * KT + grp * 16 + g;
 #pragma unroll
-      for (int j = 0; j < T::NTW; ++j) {
-        const int kl = 8 * (warp * T::NTW + j);
-        const float ks = __shfl_sync(0xffffffffu, ks_l, kl >> 4);
-        vfac[j] = __shfl_sync(0xffffffffu, vs_l, kl >> 4);
-        const int key = ks < 0.f ? 0x7fffffff - 64 : t * KT + kl + 2 * c;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float z = acc[mt][j][u] * (fac[mt][u >> 1] * ks);
-            acc[mt][j][u] = key + (u & 1) < vis[mt][u >> 1] ? z : -INFINITY;
-            tmax[mt][u >> 1] = fmaxf(tmax[mt][u >> 1], acc[mt][j][u]);
+            const float z = acc[j][n][u] * (fac[n][u & 1] * ks);
+            acc[j][n][u] = key + (u >> 1) * 8 < vis[n][u & 1] ? z : -INFINITY;
+            over |= acc[j][n][u] > m[n][u & 1] + KA_MOVE;
           }
       }
       ks_l = ks_n;
       vs_l = vs_n;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float x = tmax[mt][u];
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          if (c == 0) s_max[mt * 16 + g + 8 * u][warp] = x;
-        }
-      __syncthreads();
+      if (over) s_move[t & 1] = 1;
 
-      // ---- weights as A fragments of the second product
-      const float vnew = fmaxf(vref, vmax);
-      const float vinv = vnew > 0.f ? __frcp_rn(vnew) : 0.f;
-      const float vold = vref * vinv;
-      vref = vnew;
+      // ---- weights as B fragments of the second product: [key][8 rows] f16
+      float add[NR][2];
+      auto weights = [&]() {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        float sub[2];
+        for (int n = 0; n < NR; ++n) {
+          const float sub0 = KA_SHIFT - (m[n][0] == -INFINITY ? 0.f : m[n][0]);
+          const float sub1 = KA_SHIFT - (m[n][1] == -INFINITY ? 0.f : m[n][1]);
+          add[n][0] = add[n][1] = 0.f;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float4 *mx = reinterpret_cast<const float4 *>(s_max[mt * 16 + g + 8 * u]);
-          const float4 x = mx[0], y = mx[1];
-          const float mn = fmaxf(fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)),
-                                       fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w))), m[mt][u]);
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          const float alpha = kv8_ex2(m[mt][u] - ref);
-          m[mt][u] = mn;
-          l[mt][u] *= alpha;
-          const float ao = alpha * vold;
+          for (int j = 0; j < MW; ++j) {
+            const float f = vs[j] * vinv;
+            const int key = (warp * MW + j) * 16 + g;
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            o[mt][n][2 * u] *= ao;
-            o[mt][n][2 * u + 1] *= ao;
+            for (int u = 0; u < 2; ++u) {  // keys g and g + 8
+              const float e0 = kv8_ex2(acc[j][n][2 * u] + sub0);
+              const float e1 = kv8_ex2(acc[j][n][2 * u + 1] + sub1);
+              add[n][0] += e0;
+              add[n][1] += e1;
+              *reinterpret_cast<uint32_t *>(s_p + (n * KT + key + 8 * u) * 16 + c * 4) =
+                  pack_h2(e0 * f, e1 * f);
+            }
           }
-          sub[u] = KV8_P_SHIFT - ref;
         }
+      };
+      weights();
+      __syncthreads();
+      if (s_move[t & 1]) {  // (every warp alike) take the new maximum and scale
 #pragma unroll
-        for (int j = 0; j < T::NTW; ++j) {
-          const float f = vfac[j] * vinv;
-          uint32_t pk[2];
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const float e0 = kv8_ex2(acc[mt][j][2 * u] + sub[u]);
-            const float e1 = kv8_ex2(acc[mt][j][2 * u + 1] + sub[u]);
-            l[mt][u] += e0 + e1;
-            pk[u] = pack_h2(e0 * f, e1 * f);
+            float x = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < MW; ++j) x = fmaxf(x, fmaxf(acc[j][n][u], acc[j][n][2 + u]));
+#pragma unroll
+            for (int o2 = 4; o2 < 32; o2 <<= 1)
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o2));
+            if (g == 0) s_max[warp][n * 8 + 2 * c + u] = x;
           }
-          const int nt = warp * T::NTW + j;  // 8-key group of the tile
-          *reinterpret_cast<uint2 *>(
-              s_p + ((mt * (KT / 16) + (nt >> 1)) * 32 + lane) * 4 + (nt & 1) * 2) =
-              make_uint2(pk[0], pk[1]);
-        }
+        __syncthreads();
+        const float vnew = fmaxf(vref, vmax);
+        vinv = vnew > 0.f ? __frcp_rn(vnew) : 0.f;
+        const float vold = vref * vinv;
+        vref = vnew;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int r = n * 8 + 2 * c + u;
+            const float mn = fmaxf(fmaxf(fmaxf(s_max[0][r], s_max[1][r]),
+                                         fmaxf(s_max[2][r], s_max[3][r])), m[n][u]);
+            const float alpha = mn == -INFINITY ? 0.f : kv8_ex2(m[n][u] - mn);
+            m[n][u] = mn;
+            l[n][u] *= alpha;
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+              o[i][n][u] *= alpha * vold;
+              o[i][n][2 + u] *= alpha * vold;
+            }
+          }
+        weights();
+        __syncthreads();
       }
-      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        l[n][0] += add[n][0];
+        l[n][1] += add[n][1];
+      }
 
-      // ---- O += P V
+      // ---- O^T += V^T P^T
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int ks = kg * 4 + s;
-        uint32_t w[4];
+      for (int s = 0; s < KT / 16; ++s) {
+        uint32_t bp[NR][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = ks * 16 + 2 * c + (i & 1) + (i >> 1) * 8;
-          w[i] = *reinterpret_cast<const uint32_t *>(
-                     vb + ka_chunk<D>(key, 2 * dg + (g >> 2)) + (g & 3) * 4) ^ 0x80808080u;
-        }
-        uint4 a[MT];
+        for (int n = 0; n < NR; ++n)
+          ldsm_x2_trans(bp[n][0], bp[n][1], s_p + (n * KT + s * 16 + (lane & 15)) * 16);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          a[mt] = *reinterpret_cast<const uint4 *>(s_p + ((mt * (KT / 16) + ks) * 32 + lane) * 4);
-        const uint32_t x0 = __byte_perm(w[0], w[1], 0x5140), x1 = __byte_perm(w[0], w[1], 0x7362);
-        const uint32_t y0 = __byte_perm(w[2], w[3], 0x5140), y1 = __byte_perm(w[2], w[3], 0x7362);
+        for (int d = 0; d < T::ND; ++d) {
+          uint32_t w[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint32_t sel = (n & 1) ? 0x4342 : 0x4140;
-          const uint32_t b0 = h2_codes(__byte_perm(n < 2 ? x0 : x1, 0x64646464u, sel));
-          const uint32_t b1 = h2_codes(__byte_perm(n < 2 ? y0 : y1, 0x64646464u, sel));
+          for (int i = 0; i < 4; ++i) {
+            const uint8_t *vp = st + ((i & 1) ? v_at1 + d * v_next1 : v_at0 + d * v_next0) +
+                                (s * 16 + (i >> 1) * 8) * D;
+            w[i] = (D == 64 ? (uint32_t)*reinterpret_cast<const uint16_t *>(vp)
+                            : *reinterpret_cast<const uint32_t *>(vp)) ^ 0x80808080u;
+          }
+          const uint32_t x0 = __byte_perm(w[0], w[1], 0x5140), x1 = __byte_perm(w[0], w[1], 0x7362);
+          const uint32_t y0 = __byte_perm(w[2], w[3], 0x5140), y1 = __byte_perm(w[2], w[3], 0x7362);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][n], a[mt], b0, b1);
+          for (int i = 0; i < (D == 64 ? 1 : 2); ++i) {  // dims 4 g + 2 i, + 1
+            const uint32_t x = i ? x1 : x0, y = i ? y1 : y0;
+            const uint4 a = make_uint4(h2_codes(__byte_perm(x, 0x64646464u, 0x4140)),
+                                       h2_codes(__byte_perm(x, 0x64646464u, 0x4342)),
+                                       h2_codes(__byte_perm(y, 0x64646464u, 0x4140)),
+                                       h2_codes(__byte_perm(y, 0x64646464u, 0x4342)));
+#pragma unroll
+            for (int n = 0; n < NR; ++n) mma_f16(o[2 * d + i][n], a, bp[n][0], bp[n][1]);
+          }
         }
       }
     }
-    cp_async_wait<0>();
-    __syncthreads();
 
-    // ---- sums over the warps: l over all eight, O over the key groups
-    float *s_o = reinterpret_cast<float *>(smem);  // [NKG - 1][8 / NKG][ROWS][32]
+    // ---- l over the lanes of a row and the warps
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float x = l[mt][u];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        if (c == 0) s_l[warp][mt * 16 + g + 8 * u] = x;
+        float x = l[n][u];
+#pragma unroll
+        for (int o2 = 4; o2 < 32; o2 <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o2);
+        if (g == 0) s_l[warp][n * 8 + 2 * c + u] = x;
       }
-    constexpr int NDG = 8 / T::NKG;
-    if (kg > 0) {
+    __syncthreads();  // (and the ring, s_q and s_p are free for the next unit)
+    const bool whole = t0 == 0 && t1 == tiles;
+    const size_t slot = (size_t)blockIdx.x * 2 + (t0 == 0);
+    constexpr int DL = D == 64 ? 2 : 4;  // consecutive dims of this lane per group
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float4 *d = reinterpret_cast<float4 *>(
-              s_o + (((kg - 1) * NDG + dg) * ROWS + mt * 16 + g + 8 * u) * 32 + 8 * c);
-          d[0] = make_float4(o[mt][0][2 * u], o[mt][1][2 * u], o[mt][2][2 * u], o[mt][3][2 * u]);
-          d[1] = make_float4(o[mt][0][2 * u + 1], o[mt][1][2 * u + 1], o[mt][2][2 * u + 1],
-                             o[mt][3][2 * u + 1]);
+      for (int u = 0; u < 2; ++u) {
+        const int r = n * 8 + 2 * c + u;
+        if (r >= rows) continue;
+        const float ls = (s_l[0][r] + s_l[1][r]) + (s_l[2][r] + s_l[3][r]);
+        const int i = p.row_of(r);
+        const size_t row = ((size_t)b * p.Hq + h * p.rep + r - i * p.rep) * p.L + i;
+        const float mul = !whole ? vref : ls == 0.f ? 0.f : vref / ls;  // 0: sees no key
+        if (warp == 0 && g == 0) {
+          if (!whole)
+            p.ml_part[slot * ROWS + r] = make_float2(m[n][u] - KA_SHIFT, ls);
+          else if (p.lse)
+            p.lse[row] = ls == 0.f ? -INFINITY
+                                   : (m[n][u] - KA_SHIFT + log2f(ls)) * 0.69314718055994531f;
         }
-    }
-    __syncthreads();
-    if (kg == 0) {
-      const bool whole = t0 == 0 && t1 == tiles;
-      const size_t slot = (size_t)blockIdx.x * 2 + (t0 == 0);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+        for (int d = 0; d < T::ND; ++d) {
+          float f[4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = mt * 16 + g + 8 * u;
-          if (r >= rows) continue;
-          float f[8];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            f[n] = o[mt][n][2 * u];
-            f[n + 4] = o[mt][n][2 * u + 1];
-          }
-#pragma unroll
-          for (int k2 = 0; k2 < T::NKG - 1; ++k2) {
-            const float4 *d = reinterpret_cast<const float4 *>(
-                s_o + ((k2 * NDG + dg) * ROWS + r) * 32 + 8 * c);
-            const float4 x = d[0], y = d[1];
-            f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w;
-            f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
-          }
-          float ls = 0.f;
-#pragma unroll
-          for (int w = 0; w < 8; ++w) ls += s_l[w][r];
-          const int dim0 = 32 * dg + 8 * c;
+          for (int k = 0; k < DL; ++k) f[k] = o[2 * d + (k >> 1)][n][(k & 1) * 2 + u] * mul;
+          const int dim = warp * T::DW + d * 32 + g * DL;
           if (!whole) {
-            if (dg == 0 && c == 0)
-              p.ml_part[slot * ROWS + r] = make_float2(m[mt][u] - KV8_P_SHIFT, ls);
-            float4 *dst = reinterpret_cast<float4 *>(p.o_part + (slot * ROWS + r) * D + dim0);
-            dst[0] = make_float4(f[0] * vref, f[1] * vref, f[2] * vref, f[3] * vref);
-            dst[1] = make_float4(f[4] * vref, f[5] * vref, f[6] * vref, f[7] * vref);
+            float *dst = p.o_part + (slot * ROWS + r) * D + dim;
+            if constexpr (DL == 4)
+              *reinterpret_cast<float4 *>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+            else
+              *reinterpret_cast<float2 *>(dst) = make_float2(f[0], f[1]);
           } else {
-            const int i = p.row_of(r);
-            const size_t row = ((size_t)b * p.Hq + h * p.rep + r - i * p.rep) * p.L + i;
-            const float inv = ls == 0.f ? 0.f : vref / ls;  // 0: the row sees no key
-            *reinterpret_cast<uint4 *>(p.out + row * D + dim0) =
-                make_uint4(pack_bf2(f[0] * inv, f[1] * inv), pack_bf2(f[2] * inv, f[3] * inv),
-                           pack_bf2(f[4] * inv, f[5] * inv), pack_bf2(f[6] * inv, f[7] * inv));
-            if (p.lse && dg == 0 && c == 0)
-              p.lse[row] = ls == 0.f
-                               ? -INFINITY
-                               : (m[mt][u] - KV8_P_SHIFT + log2f(ls)) * 0.69314718055994531f;
+            uint16_t *dst = p.out + row * D + dim;
+            if constexpr (DL == 4)
+              *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]));
+            else
+              *reinterpret_cast<uint32_t *>(dst) = pack_bf2(f[0], f[1]);
           }
         }
-    }
-    if (w0 < w1) __syncthreads();  // the ring, s_q and s_l are free for the next unit
+      }
+    if (w0 < w1) __syncthreads();  // s_l has been read
   }
 }
 
 // ------------------------------------------------------------------- combine
+constexpr int KC_THREADS = 256;
 constexpr int KC_MAX = 512;  // most partial results of one row
 
 // Where a row's partial results are. kv8_attn_kernel's units (`units` not
@@ -573,10 +596,10 @@ __device__ __forceinline__ void kv8_finish(const Kv8AttnParams &p, int D, int b,
 // them in order. For few partial results per row a thread joins four dims of
 // one row.
 template <int D>
-__global__ void __launch_bounds__(KA_THREADS) kv8_combine_kernel(Kv8AttnParams p, int tile_rows) {
+__global__ void __launch_bounds__(KC_THREADS) kv8_combine_kernel(Kv8AttnParams p, int tile_rows) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int RPC = KA_THREADS * 4 / D;  // rows per CTA
+  constexpr int RPC = KC_THREADS * 4 / D;  // rows per CTA
   const int rows = p.L * p.rep, groups = (rows + RPC - 1) / RPC;
   const int bh = blockIdx.x / groups, R = blockIdx.x % groups * RPC + threadIdx.x / (D / 4);
   const int b = bh / p.c.kv_heads, h = bh % p.c.kv_heads, d4 = threadIdx.x % (D / 4);
@@ -607,11 +630,11 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_combine_kernel(Kv8AttnParams p
 // per partial result and 32 of them at a time, so that all loads are in flight
 // at once.
 template <int D>
-__global__ void __launch_bounds__(KA_THREADS) kv8_combine_wide_kernel(Kv8AttnParams p,
+__global__ void __launch_bounds__(KC_THREADS) kv8_combine_wide_kernel(Kv8AttnParams p,
                                                                       int tile_rows) {
   __shared__ float s_w[KC_MAX];
-  __shared__ float4 s_acc[KA_THREADS];
-  __shared__ float s_red[KA_THREADS / 32], s_ls[KA_THREADS / 32];
+  __shared__ float4 s_acc[KC_THREADS];
+  __shared__ float s_red[KC_THREADS / 32], s_ls[KC_THREADS / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, rows = p.L * p.rep;
@@ -621,10 +644,10 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_combine_wide_kernel(Kv8AttnPar
   const Kv8Parts q = kv8_parts<D>(p, bh, b, R / tile_rows);
   if (p.units && q.n == 1) return;
   float M = -INFINITY, ls = 0.f;
-  float2 ml[KC_MAX / KA_THREADS];
+  float2 ml[KC_MAX / KC_THREADS];
 #pragma unroll
-  for (int k = 0; k < KC_MAX / KA_THREADS; ++k) {
-    const int s = tid + k * KA_THREADS;
+  for (int k = 0; k < KC_MAX / KC_THREADS; ++k) {
+    const int s = tid + k * KC_THREADS;
     ml[k] = s < q.n ? __ldcg(p.ml_part + q.at(s) * tile_rows + r) : make_float2(-INFINITY, 0.f);
     M = fmaxf(M, ml[k].x);
   }
@@ -633,11 +656,11 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_combine_wide_kernel(Kv8AttnPar
   if ((tid & 31) == 0) s_red[tid >> 5] = M;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < KA_THREADS / 32; ++w) M = fmaxf(M, s_red[w]);
+  for (int w = 0; w < KC_THREADS / 32; ++w) M = fmaxf(M, s_red[w]);
 #pragma unroll
-  for (int k = 0; k < KC_MAX / KA_THREADS; ++k) {
+  for (int k = 0; k < KC_MAX / KC_THREADS; ++k) {
     const float wgt = ml[k].x == -INFINITY ? 0.f : kv8_ex2(ml[k].x - M);
-    s_w[tid + k * KA_THREADS] = wgt;
+    s_w[tid + k * KC_THREADS] = wgt;
     ls = fmaf(wgt, ml[k].y, ls);
   }
 #pragma unroll
@@ -646,7 +669,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv8_combine_wide_kernel(Kv8AttnPar
   __syncthreads();
   ls = 0.f;
 #pragma unroll
-  for (int w = 0; w < KA_THREADS / 32; ++w) ls += s_ls[w];
+  for (int w = 0; w < KC_THREADS / 32; ++w) ls += s_ls[w];
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
   for (int s = grp; s < q.n; s += 32) {
@@ -677,8 +700,8 @@ struct Kv8Plan {
   bool wide;            // many partial results per row
 };
 
-// Up to 32 rows per kv head: kv8_attn_kernel, row tiles of 16 or 32, two CTAs
-// on each of 148 SMs (fewer when the table holds fewer tiles). More rows: the
+// Up to 32 rows per kv head: kv8_attn_kernel, 8, 16 or 32 rows, its CTAs on
+// each of 148 SMs (fewer when the table holds fewer tiles). More rows: the
 // tcgen05 kernel, one CTA per SM, key ranges as many as fill 148 SMs.
 Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   Kv8Plan pl;
@@ -696,10 +719,11 @@ Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
     pl.ctas = 0;
     pl.parts = s == 1 ? 0 : (size_t)(base * s);
   } else {
-    pl.tile_rows = rows <= 16 ? 16 : 32;
+    pl.tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     pl.row_tiles = pl.splits = 1;
     const long long kt = KA_TILE / a->cache.dim, tiles = units * ((cap + kt - 1) / kt);
-    pl.ctas = (int)(tiles < 2 * 148 ? tiles : 2 * 148);
+    const int full = 148 * (pl.tile_rows == 32 ? Kv8Tile<64, 4>::CTAS : Kv8Tile<64, 1>::CTAS);
+    pl.ctas = (int)(tiles < full ? tiles : full);
     pl.parts = (size_t)pl.ctas * 2;
   }
   // results per row on average: the wide kernel pays from about 8
@@ -709,34 +733,35 @@ Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   return pl;
 }
 
-template <int D, int MT>
+template <int D, int NR>
 int kv8_launch(const Kv8AttnParams &p, int ctas, cudaStream_t s) {
-  using T = Kv8Tile<D, MT>;
+  using T = Kv8Tile<D, NR>;
   static bool ready = false;
   if (!ready) {
     const cudaError_t e = cudaFuncSetAttribute(
-        kv8_attn_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+        kv8_attn_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
     if (e != cudaSuccess)
       return set_error(VB_ERR_CUDA, "kv8_attn_kernel attributes: %s", cudaGetErrorString(e));
     ready = true;
   }
-  vb_launch(kv8_attn_kernel<D, MT>, dim3(ctas), dim3(KA_THREADS), T::SMEM, s, false, p);
+  vb_launch(kv8_attn_kernel<D, NR>, dim3(ctas), dim3(KA_THREADS), T::SMEM, s, false, p);
   return check_launch("kv8_attn_kernel");
 }
 
 template <int D>
 int kv8_run(const Kv8AttnParams &p, const Kv8Plan &pl, cudaStream_t s) {
   const int rc = pl.tensor ? kv8_prefill_launch(p, s)
-                 : pl.tile_rows == 16 ? kv8_launch<D, 1>(p, pl.ctas, s)
-                                      : kv8_launch<D, 2>(p, pl.ctas, s);
+                 : pl.tile_rows == 8  ? kv8_launch<D, 1>(p, pl.ctas, s)
+                 : pl.tile_rows == 16 ? kv8_launch<D, 2>(p, pl.ctas, s)
+                                      : kv8_launch<D, 4>(p, pl.ctas, s);
   if (rc != VB_OK || pl.parts == 0) return rc;
   const unsigned units = p.c.batch * p.c.kv_heads, rows = p.L * p.rep;
-  constexpr unsigned RPC = KA_THREADS * 4 / D;
+  constexpr unsigned RPC = KC_THREADS * 4 / D;
   if (pl.wide)
-    vb_launch(kv8_combine_wide_kernel<D>, dim3(units * rows, D / 32), dim3(KA_THREADS), 0, s, true,
+    vb_launch(kv8_combine_wide_kernel<D>, dim3(units * rows, D / 32), dim3(KC_THREADS), 0, s, true,
               p, pl.tile_rows);
   else
-    vb_launch(kv8_combine_kernel<D>, dim3(units * ((rows + RPC - 1) / RPC)), dim3(KA_THREADS), 0, s,
+    vb_launch(kv8_combine_kernel<D>, dim3(units * ((rows + RPC - 1) / RPC)), dim3(KC_THREADS), 0, s,
               true, p, pl.tile_rows);
   return check_launch("kv8_combine_kernel");
 }

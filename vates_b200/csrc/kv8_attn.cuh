@@ -66,11 +66,9 @@ __device__ __forceinline__ float kv8_q_power(float amax) {
   return __uint_as_float((uint32_t)(e == 255 ? 127 : min(254, 262 - e)) << 23);
 }
 
-// Shift of the exponentials before they are rounded to f16 (2^14, largest f16
-// 65504): the smallest kept weight is 2^-38 of the largest, so even a long
-// tail of small weights is not flushed. It cancels in O / l.
-constexpr float KV8_P_SHIFT = 14.f;
-
+// (The exponentials are shifted up before they are rounded to f16, whose
+// largest value is 65504, so that a long tail of small weights is not flushed:
+// the kernels' *_SHIFT. It cancels in O / l.)
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
