@@ -280,6 +280,27 @@ def test_attend_many_rows(cuda, dim, rep, L, lens, q_lens, causal):
     check_attend(c, q, lens, q_lens, causal)
 
 
+@pytest.mark.parametrize("dim,rep,L,batch,heads", [(256, 2, 64, 2, 8), (256, 8, 8, 16, 8),
+                                                   (128, 8, 64, 2, 8), (64, 4, 70, 4, 8)])
+def test_attend_every_key_tile_counts(cuda, dim, rep, L, batch, heads):
+    """Equal keys and equal values: every weight is the same, so the result is
+    the value itself, and a key tile that is missed (also for a moment, at the
+    end of a short range of tiles) shows at once."""
+    rng = np.random.default_rng(dim + L)
+    page = 16
+    for keys in (200, 300, 1100, 2182):
+        c = make_cache(rng, batch, heads, dim, page, -(-keys // page))
+        c.k_codes.zero_()
+        c.v_codes.fill_(100)
+        c.v_scales.fill_(0.02)
+        q = bf16(rng, (batch, heads * rep, L, dim)).cuda()
+        for _ in range(3):
+            out, lse = c.attend(q, ints([keys] * batch), causal=False, return_lse=True)
+            # one f16 rounding of equal weights (2^-11) and one to bf16 (2^-8)
+            assert (out.float() - 2.0).abs().max() <= 2.0 * (2.0 ** -8 + 2.0 ** -11)
+            assert (lse - math.log(keys)).abs().max() <= 2.0 ** -18 * math.log(keys)
+
+
 def test_attend_long_sequence(cuda):
     """Splits over a long axis, one sequence beside short ones."""
     rng = np.random.default_rng(11)

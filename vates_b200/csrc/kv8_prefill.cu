@@ -21,8 +21,10 @@
 //     and l are rescaled), and stores P = 2^(z - m) s_V / v over S in TMEM as
 //     the f16 A operand of the second product. v is a power of two at least
 //     every V scale so far. l is summed in float32 from the unrounded weights.
-// tcgen05 operations of one thread execute in issue order, which is what keeps
-// S of an item behind the O product that reads the P in its slot.
+// A wait names the n-th completion of a barrier by its parity alone, so when it
+// begins, completion n - 1 must have happened and n + 1 must not: S of an item
+// waits for O of the last item in its slot, and the last O of a row tile has a
+// barrier of its own.
 // NT = 2 for head sizes 64 and 128, 1 for 256 (TMEM: 2 x 128 columns of S and
 // NT * D of O are all 512). Every wait is bounded (2 s, then VB_STATUS_TIMEOUT).
 #include "kv8_attn.cuh"
@@ -117,7 +119,8 @@ __device__ __forceinline__ void kp_regs_inc() {
 }
 
 struct KpBarriers {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2],
+      o_last[2];
 };
 
 template <int D>
@@ -160,6 +163,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
       tc::mbar_init(&bar.s_full[i], 1);
       tc::mbar_init(&bar.p_full[i], 4);
       tc::mbar_init(&bar.o_done[i], 1);
+      tc::mbar_init(&bar.o_last[i], 1);
     }
     s_abort = 0;
     tc::fence_mbar_init();
@@ -242,7 +246,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
       for (int w = 0; w <= n_items && ok; ++w) {
         if (w < n_items) {  // S of item w
           const int kt = w / NT, tile = w % NT, st = kt % ST;
-          if (tile == 0) ok = wait(&bar.k_full[st], kt / ST);
+          // the slot's P has been read: O of item w - 2 is done
+          if (w >= 2) ok = wait(&bar.o_done[tile], (w - 2) / NT);
+          if (tile == 0) ok = ok && wait(&bar.k_full[st], kt / ST);
           if (!ok) break;
           tc::tc_fence_after();
           const uint32_t qa = sbase + H::Q_OFF + tile * H::TILE;
@@ -269,6 +275,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
             kp_mma_ts(tmem + 256 + tile * D, tmem + (v & 1) * 128 + kk * 8,
                       kp_desc_mn(va + kk * 2048), ID_O, (kt > 0 || kk > 0) ? 1u : 0u);
           tc::mma_commit(&bar.o_done[tile]);
+          if (v >= n_items - NT) tc::mma_commit(&bar.o_last[tile]);
           if (tile == NT - 1) tc::mma_commit(&bar.v_empty[st]);
           ++o_sent;
         }
@@ -491,8 +498,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
     }
     // ---- O of this tile's last product
     if (ok && t1 > t0) {
-      if (!tc::mbar_wait(&bar.o_done[tile], (uint32_t)((t1 - t0 - 1) & 1), abort, KP_WAIT_NS))
-        s_abort = 1;
+      if (!tc::mbar_wait(&bar.o_last[tile], 0, abort, KP_WAIT_NS)) s_abort = 1;
       ok = !__any_sync(0xffffffffu, *abort != 0);
       tc::tc_fence_after();
     }
@@ -520,8 +526,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
         float y[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(x[j]) * inv;
-        if (!live) continue;
-        if (p.splits > 1) {
+        __syncwarp();
+        if (!live) {
+        } else if (p.splits > 1) {
           if (t1 > t0) {
             float4 *d4 = reinterpret_cast<float4 *>(p.o_part + (tile_id * ROWS + r) * D + c0);
 #pragma unroll

@@ -5,10 +5,12 @@
 //   s = sum 2^y_j,  t = sum 2^y_j y_j   (float32)
 //   logprob = ((x_t - m) c - log2 s) ln 2,  entropy = (log2 s - t / s) ln 2.
 // When m moves, with d = (m_old - m_new) c: t <- 2^d (t + d s), s <- 2^d s, so
-// the running maximum is carried per thread and the row is read once. y stops
-// at -1000 (2^y = 0), which keeps 0 * inf out of t for logits of -inf; NaN and
-// +inf go through and give NaN. The difference is taken before the product: it
-// is exactly 0 at the maximum however large the logits are.
+// the running maximum is carried per thread and the row is read once. Logits
+// enter the sums at no less than -1e32 (2^y = 0 beside any larger one), which
+// keeps 0 * inf out of t; NaN and +inf go through and give NaN. The difference
+// is taken before the product: it is exactly 0 at the maximum however large the
+// logits are. Instruction-bound before it is HBM-bound, so bf16 pairs are
+// compared and clamped two at a time and the sums run on pairs of float32.
 //
 // Best alternatives: the k-th largest of the threads' own maxima is a lower
 // bound v of the k-th largest logit (k threads hold one at least that large),
@@ -30,13 +32,14 @@ constexpr int LP_UNROLL = 4;
 constexpr int LP_MAX_TOP = 32;
 constexpr int LP_BATCH = LP_THREADS * 8;         // most keys one look can add
 constexpr int LP_CAP = LP_BATCH + LP_MAX_TOP;
-constexpr int LP_RANK_ALL = 2 * LP_THREADS;      // up to here every key is ranked at once
+constexpr int LP_RANK_ALL = LP_THREADS;          // up to here every key is ranked at once
 constexpr int LP_MAX_PARTS = 64;
 constexpr int LP_FILL = 2 * 148;                 // CTAs that fill the GPU, two per SM
 constexpr size_t LP_TICKETS = 1024;              // bytes: a word per row of a split call
 static_assert(LP_FILL / 2 * sizeof(uint32_t) <= LP_TICKETS, "rows of a split call");
 static_assert(LP_MAX_PARTS * LP_MAX_TOP <= LP_CAP, "keys of a split row");
-constexpr float LP_NONE = -3.402823466e38f;      // m before any logit
+// Least logit of the sums, and m at first: about -1e32, a bf16 value (0xF49E).
+constexpr float LP_FLOOR = -1.0014439741803012e32f;
 constexpr float LP_LN2 = 0.693147180559945309f;
 
 struct LpStats {
@@ -85,25 +88,109 @@ __device__ __forceinline__ float lp_next(float x, bool bf16) {
   return __uint_as_float((u & 0x80000000u) ? u - step : u + step);
 }
 
-// 16 bytes of a row: 8 bf16 or 4 float32 values.
+// Pairs of float32.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 f2_make(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(f2 v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 16 bytes of a row: 8 bf16 or 4 float32 values. `bar` is what a logit has to
+// reach to count as ahead of the token, in the form of the type.
 template <typename T>
 struct LpVec;
 template <>
 struct LpVec<uint16_t> {
   static constexpr int N = 8;
   static constexpr bool BF16 = true;
+  static constexpr uint32_t NONE = 0xFF80FF80u;  // -inf
+  static constexpr uint32_t NO_BAR = 0x7FC07FC0u;
+  __device__ static uint32_t bar(float x) { return (__float_as_uint(x) >> 16) * 0x10001u; }
   __device__ static float at(const uint4 &v, int j) {
-    const uint32_t w = (&v.x)[j >> 1];
+    const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
     return __uint_as_float((j & 1) ? (w & 0xFFFF0000u) : (w << 16));
   }
   __device__ static float load(const uint16_t *p) { return bf2f(*p); }
+  __device__ static uint32_t max2(uint32_t a, uint32_t b) {  // NaN loses
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  // largest of a vector's logits and r
+  __device__ static void top(uint32_t &r, const uint4 &v) {
+    r = max2(r, max2(max2(v.x, v.y), max2(v.z, v.w)));
+  }
+  __device__ static float top_value(uint32_t r) {
+    return fmaxf(__uint_as_float(r << 16), __uint_as_float(r & 0xFFFF0000u));
+  }
+  // the j-th pair of a vector, no less than LP_FLOOR (NaN stays)
+  static constexpr int PAIRS = 4;
+  __device__ static f2 pair(const uint4 &v, int j) {
+    uint32_t w = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w) : "r"(0xF49EF49Eu));  // LP_FLOOR
+    return f2_make(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  }
+  // number of a vector's logits that reach the bar, added to two bf16 counts
+  // (exact up to 256 each)
+  __device__ static void count(uint32_t &n, const uint4 &v, uint32_t bar) {
+    uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      asm("set.ge.bf16x2.bf16x2 %0, %0, %1;" : "+r"(x[j]) : "r"(bar));
+      asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(n) : "r"(x[j]));
+    }
+  }
+  __device__ static int counted(uint32_t n) {
+    return (int)(__uint_as_float(n << 16) + __uint_as_float(n & 0xFFFF0000u));
+  }
 };
 template <>
 struct LpVec<float> {
   static constexpr int N = 4;
   static constexpr bool BF16 = false;
-  __device__ static float at(const uint4 &v, int j) { return __uint_as_float((&v.x)[j]); }
+  static constexpr uint32_t NONE = 0xFF800000u;
+  static constexpr uint32_t NO_BAR = 0x7FC00000u;
+  __device__ static uint32_t bar(float x) { return __float_as_uint(x); }
+  __device__ static float at(const uint4 &v, int j) {
+    return __uint_as_float(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w);
+  }
   __device__ static float load(const float *p) { return *p; }
+  __device__ static void top(uint32_t &r, const uint4 &v) {
+    r = __float_as_uint(fmaxf(fmaxf(fmaxf(__uint_as_float(r), at(v, 0)), at(v, 1)),
+                              fmaxf(at(v, 2), at(v, 3))));
+  }
+  __device__ static float top_value(uint32_t r) { return __uint_as_float(r); }
+  static constexpr int PAIRS = 2;
+  __device__ static f2 pair(const uint4 &v, int j) {
+    float a = at(v, 2 * j), b = at(v, 2 * j + 1);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(LP_FLOOR));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(LP_FLOOR));
+    return f2_make(a, b);
+  }
+  __device__ static void count(uint32_t &n, const uint4 &v, uint32_t bar) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n += at(v, j) >= __uint_as_float(bar);
+  }
+  __device__ static int counted(uint32_t n) { return (int)n; }
 };
 
 // A row's vectors: vector v holds ids [v N - off, v N - off + N); those outside
@@ -126,10 +213,9 @@ struct LpRow {
   }
 };
 
-__device__ __forceinline__ float lp_y(float x, float m, float c) {
-  float y;  // NaN stays NaN
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"((x - m) * c), "f"(-1000.f));
-  return y;
+// A logit as it enters y (-inf stays, for results of that token alone).
+__device__ __forceinline__ float lp_floor(float x) {
+  return x < LP_FLOOR && x > -INFINITY ? LP_FLOOR : x;
 }
 __device__ __forceinline__ void lp_move(float &m, float &s, float &t, float to, float c) {
   if (to > m) {
@@ -211,56 +297,90 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
   const int v_hi = (int)((int64_t)r.nvec * (part + 1) / p.parts);
   const float c = p.c;
 
-  float m = LP_NONE, s = 0.f, t = 0.f, best = -INFINITY;
+  float m = LP_FLOOR, s = 0.f, t = 0.f, best = -INFINITY;
   int ahead = 0;
-  for (int v0 = v_lo + tid; v0 < v_hi; v0 += LP_THREADS * LP_UNROLL) {
-    uint4 x[LP_UNROLL];
-    bool in[LP_UNROLL];
+  {
+    const int w_lo = max(v_lo, r.w_lo), w_hi = min(v_hi, r.w_hi);  // whole vectors
+    const uint32_t bar_lo = tok_ok ? V::bar(xt) : V::NO_BAR;       // ids below the token's count
+    const uint32_t bar_hi = tok_ok ? V::bar(xt_next) : V::NO_BAR;  // when equal
+    const f2 cc = f2_make(c, c);
+    f2 ss = 0, tt = 0;
+    uint4 next[LP_UNROLL];
+    auto fetch = [&](int v0) {
 #pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u) {
-      const int v = v0 + u * LP_THREADS;
-      in[u] = v < v_hi && r.whole(v) && v != tok_vec;
-      if (in[u]) x[u] = r.load(v);
-    }
-    float top = -INFINITY;
+      for (int u = 0; u < LP_UNROLL; ++u) {
+        const int v = v0 + u * LP_THREADS;
+        next[u] = make_uint4(V::NONE, V::NONE, V::NONE, V::NONE);
+        if (v >= w_lo && v < w_hi) next[u] = r.load(v);
+      }
+    };
+    fetch(v_lo + tid);
+    for (int v0 = v_lo + tid; v0 < w_hi; v0 += LP_THREADS * LP_UNROLL) {
+      uint4 x[LP_UNROLL];
 #pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u)
-      if (in[u])
+      for (int u = 0; u < LP_UNROLL; ++u) x[u] = next[u];
+      fetch(v0 + LP_THREADS * LP_UNROLL);
+      uint32_t top = V::NONE;
 #pragma unroll
-        for (int j = 0; j < V::N; ++j) top = fmaxf(top, V::at(x[u], j));
-    best = fmaxf(best, top);
-    lp_move(m, s, t, top, c);
+      for (int u = 0; u < LP_UNROLL; ++u) V::top(top, x[u]);
+      const float top_x = V::top_value(top);
+      best = fmaxf(best, top_x);
+      if (top_x > m) {
+        float s0, s1, t0, t1;
+        f2_split(ss, s0, s1);
+        f2_split(tt, t0, t1);
+        s = s0 + s1;
+        t = t0 + t1;
+        lp_move(m, s, t, top_x, c);
+        ss = f2_make(s, 0.f);
+        tt = f2_make(t, 0.f);
+      }
+      const f2 mm = f2_make(-m, -m);
+      uint32_t n = 0;
 #pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u) {
-      const int v = v0 + u * LP_THREADS;
-      if (in[u]) {
-        // ids below the token's count when equal
-        const float bar = v < tok_vec ? xt : xt_next;
+      for (int u = 0; u < LP_UNROLL; ++u) {
+        const int v = v0 + u * LP_THREADS;
+        V::count(n, x[u], v >= w_hi || v < w_lo ? V::NO_BAR : v < tok_vec ? bar_lo : bar_hi);
 #pragma unroll
-        for (int j = 0; j < V::N; ++j) {
-          const float f = V::at(x[u], j);
-          const float y = lp_y(f, m, c);
-          const float e = lp_ex2(y);
-          s += e;
-          t = fmaf(e, y, t);
-          ahead += f >= bar;
-        }
-      } else if (v < v_hi) {  // the row's ends and the token's own vector
-        for (int j = 0; j < V::N; ++j) {
-          const int64_t id = (int64_t)v * V::N - r.off + j;
-          if (id < 0 || id >= p.vocab) continue;
-          const float f = V::load(r.x + id);
-          best = fmaxf(best, f);
-          lp_move(m, s, t, f, c);
-          const float y = lp_y(f, m, c);
-          const float e = lp_ex2(y);
-          s += e;
-          t = fmaf(e, y, t);
-          ahead += f > xt || (f == xt && id < tok);
+        for (int j = 0; j < V::PAIRS; ++j) {
+          const f2 y = f2_mul(f2_add(V::pair(x[u], j), mm), cc);
+          float y0, y1;
+          f2_split(y, y0, y1);
+          const f2 e = f2_make(lp_ex2(y0), lp_ex2(y1));
+          ss = f2_add(ss, e);
+          tt = f2_fma(e, y, tt);
         }
       }
+      ahead += V::counted(n);
     }
+    float s0, s1, t0, t1;
+    f2_split(ss, s0, s1);
+    f2_split(tt, t0, t1);
+    s = s0 + s1;
+    t = t0 + t1;
+    // the row's ends, logit by logit, in the threads that own these vectors
+    auto ragged = [&](int v) {
+      if (v < v_lo || v >= v_hi || (v - v_lo) % LP_THREADS != tid) return;
+      for (int j = 0; j < V::N; ++j) {
+        const int id = v * V::N - r.off + j;
+        if (id < 0 || id >= p.vocab) continue;
+        const float f = V::load(r.x + id);
+        best = fmaxf(best, f);
+        lp_move(m, s, t, f, c);
+        const float y = ((f < LP_FLOOR ? LP_FLOOR : f) - m) * c, e = lp_ex2(y);
+        s += e;
+        t = fmaf(e, y, t);
+        ahead += tok_ok && (v < tok_vec ? f >= xt : f >= xt_next);
+      }
+    };
+    if (r.w_lo > 0) ragged(0);
+    if (r.w_hi < r.nvec && (r.w_hi > 0 || r.w_lo == 0)) ragged(r.w_hi);
+    // equal logits of lower id in the token's own vector
+    if (tok_ok && tid == 0 && tok_vec >= v_lo && tok_vec < v_hi)
+      for (int id = max(0, tok_vec * V::N - r.off); id < tok; ++id)
+        ahead += V::load(r.x + id) == xt;
   }
+
   // ---- the k best of this slice
   const int k = p.top;
   if (k > 0) {
@@ -277,40 +397,55 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
     __syncthreads();
     const int owners = s_owners;
     const int turns = (v_hi - v_lo + LP_THREADS - 1) / LP_THREADS;
-    const int64_t items = (int64_t)turns * owners;
-    unsigned long long kth = 0;
-    int have = 0;
-    for (int64_t i0 = 0; i0 < items; i0 += LP_THREADS) {
-      const int64_t i = i0 + tid;
-      const int v = i < items ? v_lo + (int)(i / owners) * LP_THREADS + s_owner[i % owners] : v_hi;
-      if (v < v_hi) {
-        const bool whole = r.whole(v);
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (whole) x = r.load(v);
+    const int items = turns * owners;
+    // keys of item i (owner i % owners, its vector i / owners) that reach the bounds
+    auto look = [&](int i, unsigned long long least) {
+      const int v = v_lo + (i / owners) * LP_THREADS + s_owner[i % owners];
+      if (v >= v_hi) return;
+      const bool whole = r.whole(v);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (whole) x = r.load(v);
 #pragma unroll
-        for (int j = 0; j < V::N; ++j) {
-          const int64_t id = (int64_t)v * V::N - r.off + j;
-          if (id < 0 || id >= p.vocab) continue;
-          const float f = whole ? V::at(x, j) : V::load(r.x + id);
-          if (lp_order(f) >= thr) {
-            const unsigned long long key = lp_key(f, (int)id);
-            if (key > kth) s_buf[atomicAdd(&s_n, 1)] = key;
+      for (int j = 0; j < V::N; ++j) {
+        const int id = v * V::N - r.off + j;
+        if (id < 0 || id >= p.vocab) continue;
+        const float f = whole ? V::at(x, j) : V::load(r.x + id);
+        if (lp_order(f) >= thr) {
+          const unsigned long long key = lp_key(f, id);
+          if (key > least) {
+            const int at = atomicAdd(&s_n, 1);
+            if (at < LP_CAP) s_buf[at] = key;
           }
         }
       }
+    };
+#pragma unroll 2
+    for (int i = tid; i < items; i += LP_THREADS) look(i, 0);
+    __syncthreads();
+    int n = s_n;
+    if (n <= LP_CAP) {
+      lp_select(s_buf, n, k, s_list, s_tmp, &s_n, s_cnt);
+    } else {  // (many equal logits) look again, a bounded number of keys at a time
       __syncthreads();
-      const int n = s_n;
-      const bool last = i0 + LP_THREADS >= items;
-      if (last || n > LP_CAP - LP_BATCH) {
-        lp_select(s_buf, n, k, s_list, s_tmp, &s_n, s_cnt);
-        have = min(n, k);
-        if (have == k) kth = s_list[k - 1];
-        if (!last) {
-          if (tid < have) s_buf[tid] = s_list[tid];
-          if (tid == 0) s_n = have;
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+      unsigned long long kth = 0;
+      for (int i0 = 0; i0 < items; i0 += LP_THREADS) {
+        if (i0 + tid < items) look(i0 + tid, kth);
+        __syncthreads();
+        n = s_n;
+        const bool last = i0 + LP_THREADS >= items;
+        if (last || n > LP_CAP - LP_BATCH) {
+          lp_select(s_buf, n, k, s_list, s_tmp, &s_n, s_cnt);
+          const int have = min(n, k);
+          if (have == k) kth = s_list[k - 1];
+          if (!last) {
+            if (tid < have) s_buf[tid] = s_list[tid];
+            if (tid == 0) s_n = have;
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
     }
   }
 
@@ -328,11 +463,19 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
     s_b[tid >> 5] = best; s_a[tid >> 5] = ahead;
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < LP_WARPS; ++w) {
-      lp_join(m, s, t, s_m[w], s_s[w], s_t[w], c);
-      best = fmaxf(best, s_b[w]);
-      ahead += s_a[w];
+  if (tid < 32) {  // lane w < 16 holds warp w's, the others nothing
+    const int w = tid & (LP_WARPS - 1);
+    m = s_m[w]; s = tid < LP_WARPS ? s_s[w] : 0.f; t = tid < LP_WARPS ? s_t[w] : 0.f;
+    best = s_b[w];
+    ahead = tid < LP_WARPS ? s_a[w] : 0;
+#pragma unroll
+    for (int o = LP_WARPS / 2; o > 0; o >>= 1) {
+      const float m2 = __shfl_down_sync(0xffffffffu, m, o);
+      const float s2 = __shfl_down_sync(0xffffffffu, s, o);
+      const float t2 = __shfl_down_sync(0xffffffffu, t, o);
+      lp_join(m, s, t, m2, s2, t2, c);
+      best = fmaxf(best, __shfl_down_sync(0xffffffffu, best, o));
+      ahead += __shfl_down_sync(0xffffffffu, ahead, o);
     }
   }
   if (p.parts > 1) {  // leave the slice's sums and keys; the row's last slice joins them
@@ -366,7 +509,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
     }
     if (tid == 0) {
       const LpStats *st = p.part_stats + (size_t)row * p.parts;
-      m = LP_NONE; s = t = 0.f; best = -INFINITY; ahead = 0;
+      m = LP_FLOOR; s = t = 0.f; best = -INFINITY; ahead = 0;
       for (int i = 0; i < p.parts; ++i) {
         lp_join(m, s, t, __ldcg(&st[i].m), __ldcg(&st[i].s), __ldcg(&st[i].t), c);
         best = fmaxf(best, __ldcg(&st[i].best));
@@ -375,10 +518,14 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
     }
   }
   if (tid == 0) {
+    if (best <= LP_FLOOR) {  // every logit counts as LP_FLOOR: all are equal
+      s = (float)p.vocab;
+      t = 0.f;
+    }
     s_m[0] = m;
     s_s[0] = best == -INFINITY ? NAN : log2f(s);
     const float l2 = s_s[0];
-    p.logprob[row] = tok_ok ? ((xt - m) * c - l2) * LP_LN2 : NAN;
+    p.logprob[row] = tok_ok ? ((lp_floor(xt) - m) * c - l2) * LP_LN2 : NAN;
     p.entropy[row] = (l2 - t / s) * LP_LN2;
     p.rank[row] = tok_ok ? ahead : -1;
     if (!tok_ok) flag_status(p.status, VB_STATUS_BOUNDS);
@@ -388,7 +535,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
     const unsigned long long key = s_list[tid];
     p.top_ids[(size_t)row * k + tid] = (int32_t)~(uint32_t)key;
     p.top_logprobs[(size_t)row * k + tid] =
-        ((lp_unorder((uint32_t)(key >> 32)) - s_m[0]) * c - s_s[0]) * LP_LN2;
+        ((lp_floor(lp_unorder((uint32_t)(key >> 32))) - s_m[0]) * c - s_s[0]) * LP_LN2;
   }
 }
 
