@@ -15,7 +15,7 @@
 // Best alternatives: the k-th largest of the threads' own maxima is a lower
 // bound v of the k-th largest logit (k threads hold one at least that large),
 // so only threads whose maximum reaches v can hold any of the k best. Their
-// vectors, about k / 512 of the row, are looked at again (they are in L2) and
+// vectors, about k / 256 of the row, are looked at again (they are in L2) and
 // the logits >= v collected as 64-bit keys (ordered value, ~id), which have no
 // ties; the k largest keys are the answer.
 //
@@ -26,17 +26,20 @@
 namespace vb {
 namespace {
 
-constexpr int LP_THREADS = 512;
+constexpr int LP_THREADS = 256;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_UNROLL = 4;
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_SHORT = 8 * LP_THREADS;         // rows up to here go logit by logit
 constexpr int LP_BATCH = LP_THREADS * 8;         // most keys one look can add
 constexpr int LP_CAP = LP_BATCH + LP_MAX_TOP;
 constexpr int LP_RANK_ALL = LP_THREADS;          // up to here every key is ranked at once
 constexpr int LP_MAX_PARTS = 64;
-constexpr int LP_FILL = 2 * 148;                 // CTAs that fill the GPU, two per SM
-constexpr size_t LP_TICKETS = 1024;              // bytes: a word per row of a split call
+constexpr int LP_CTAS = 4;                       // per SM: one's tail behind the others' loads
+constexpr int LP_FILL = LP_CTAS * 148;
+constexpr size_t LP_TICKETS = 2048;              // bytes: a word per row of a split call
 static_assert(LP_FILL / 2 * sizeof(uint32_t) <= LP_TICKETS, "rows of a split call");
+static_assert(LP_SHORT <= LP_CAP, "keys of a short row");
 static_assert(LP_MAX_PARTS * LP_MAX_TOP <= LP_CAP, "keys of a split row");
 // Least logit of the sums, and m at first: about -1e32, a bf16 value (0xF49E).
 constexpr float LP_FLOOR = -1.0014439741803012e32f;
@@ -198,18 +201,17 @@ struct LpVec<float> {
 template <typename T>
 struct LpRow {
   const T *x;
-  int off, vocab, nvec, w_lo, w_hi;  // whole vectors: [w_lo, w_hi)
+  int off, nvec, w_lo, w_hi;  // whole vectors: [w_lo, w_hi)
   __device__ LpRow(const void *logits, int64_t row, int64_t stride, int n) {
     x = static_cast<const T *>(logits) + row * stride;
     off = (int)(((uintptr_t)x & 15) / sizeof(T));
-    vocab = n;
     nvec = (n + off + LpVec<T>::N - 1) / LpVec<T>::N;
     w_lo = off > 0;
     w_hi = (n + off) / LpVec<T>::N;
   }
-  __device__ bool whole(int v) const { return v >= w_lo && v < w_hi; }
-  __device__ uint4 load(int v) const {  // whole vectors only
-    return ldg_nc_v4(x + ((int64_t)v * LpVec<T>::N - off));
+  // where vector v begins: inside the row for whole vectors, which alone are read
+  __device__ const uint4 *at(int v) const {
+    return reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(x) & ~uintptr_t(15)) + v;
   }
 };
 
@@ -275,7 +277,7 @@ __device__ void lp_select(unsigned long long *buf, int n, int k, unsigned long l
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams p) {
+__global__ void __launch_bounds__(LP_THREADS, LP_CTAS) token_logprobs_kernel(LpParams p) {
   using V = LpVec<T>;
   __shared__ unsigned long long s_buf[LP_CAP];
   __shared__ unsigned long long s_list[LP_MAX_TOP], s_tmp[LP_MAX_TOP];
@@ -288,38 +290,56 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
   const int tid = threadIdx.x;
   const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
   const LpRow<T> r(p.logits, row, p.row_stride, p.vocab);
+  const int v_lo = (int)((int64_t)r.nvec * part / p.parts);
+  const int v_hi = (int)((int64_t)r.nvec * (part + 1) / p.parts);
+  // whole vectors [w_lo, w_hi), thread t takes w_lo + t + i LP_THREADS; the
+  // row's ragged ends, if this slice has them, are looked at logit by logit
+  // (a short row all of it, thread t the ids t + i LP_THREADS)
+  const bool brief = p.vocab <= LP_SHORT;
+  const int w_lo = max(v_lo, r.w_lo), w_hi = brief ? w_lo : max(w_lo, min(v_hi, r.w_hi));
+  const int end0 = !brief && v_lo < r.w_lo ? 0 : -1;
+  const int end1 = !brief && v_hi == r.nvec && r.w_hi < r.nvec ? r.w_hi : -1;
+  constexpr int STEP = LP_THREADS * LP_UNROLL;
+  const int n_full = (w_hi - w_lo) / STEP;  // turns in which every thread has LP_UNROLL vectors
+  const float c = p.c;
+
   const int tok = p.tokens[row];
+  const uint4 *src = r.at(w_lo + tid);
+  uint4 next[LP_UNROLL];
+  auto fetch = [&](int turn) {
+    if (turn < n_full) {
+#pragma unroll
+      for (int u = 0; u < LP_UNROLL; ++u) next[u] = ldg_nc_v4(src + u * LP_THREADS);
+    } else {  // the last turn, short of vectors
+#pragma unroll
+      for (int u = 0; u < LP_UNROLL; ++u) {
+        next[u] = make_uint4(V::NONE, V::NONE, V::NONE, V::NONE);
+        if (w_lo + turn * STEP + u * LP_THREADS + tid < w_hi)
+          next[u] = ldg_nc_v4(src + u * LP_THREADS);
+      }
+    }
+    src += STEP;
+  };
+  fetch(0);
   const bool tok_ok = (unsigned)tok < (unsigned)p.vocab;
   const float xt = tok_ok ? V::load(r.x + tok) : 0.f;
   const float xt_next = lp_next(xt, V::BF16);
   const int tok_vec = tok_ok ? (tok + r.off) / V::N : -1;
-  const int v_lo = (int)((int64_t)r.nvec * part / p.parts);
-  const int v_hi = (int)((int64_t)r.nvec * (part + 1) / p.parts);
-  const float c = p.c;
+  // ids below the token's count when equal; without a token (or a NaN) nothing does
+  const uint32_t bar_lo = tok_ok ? V::bar(xt) : V::NO_BAR;
+  const uint32_t bar_hi = tok_ok ? V::bar(xt_next) : V::NO_BAR;
 
   float m = LP_FLOOR, s = 0.f, t = 0.f, best = -INFINITY;
   int ahead = 0;
   {
-    const int w_lo = max(v_lo, r.w_lo), w_hi = min(v_hi, r.w_hi);  // whole vectors
-    const uint32_t bar_lo = tok_ok ? V::bar(xt) : V::NO_BAR;       // ids below the token's count
-    const uint32_t bar_hi = tok_ok ? V::bar(xt_next) : V::NO_BAR;  // when equal
     const f2 cc = f2_make(c, c);
     f2 ss = 0, tt = 0;
-    uint4 next[LP_UNROLL];
-    auto fetch = [&](int v0) {
-#pragma unroll
-      for (int u = 0; u < LP_UNROLL; ++u) {
-        const int v = v0 + u * LP_THREADS;
-        next[u] = make_uint4(V::NONE, V::NONE, V::NONE, V::NONE);
-        if (v >= w_lo && v < w_hi) next[u] = r.load(v);
-      }
-    };
-    fetch(v_lo + tid);
-    for (int v0 = v_lo + tid; v0 < w_hi; v0 += LP_THREADS * LP_UNROLL) {
+    const int turns = n_full + (n_full * STEP < w_hi - w_lo);
+    for (int turn = 0; turn < turns; ++turn) {
       uint4 x[LP_UNROLL];
 #pragma unroll
       for (int u = 0; u < LP_UNROLL; ++u) x[u] = next[u];
-      fetch(v0 + LP_THREADS * LP_UNROLL);
+      if (turn + 1 < turns) fetch(turn + 1);
       uint32_t top = V::NONE;
 #pragma unroll
       for (int u = 0; u < LP_UNROLL; ++u) V::top(top, x[u]);
@@ -335,12 +355,18 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
         ss = f2_make(s, 0.f);
         tt = f2_make(t, 0.f);
       }
-      const f2 mm = f2_make(-m, -m);
-      uint32_t n = 0;
+      if (top_x >= xt) {  // some logit may be ahead of the token
+        uint32_t n = 0;
 #pragma unroll
-      for (int u = 0; u < LP_UNROLL; ++u) {
-        const int v = v0 + u * LP_THREADS;
-        V::count(n, x[u], v >= w_hi || v < w_lo ? V::NO_BAR : v < tok_vec ? bar_lo : bar_hi);
+        for (int u = 0; u < LP_UNROLL; ++u) {
+          const int v = w_lo + turn * STEP + u * LP_THREADS + tid;
+          V::count(n, x[u], v >= w_hi ? V::NO_BAR : v < tok_vec ? bar_lo : bar_hi);
+        }
+        ahead += V::counted(n);
+      }
+      const f2 mm = f2_make(-m, -m);
+#pragma unroll
+      for (int u = 0; u < LP_UNROLL; ++u)
 #pragma unroll
         for (int j = 0; j < V::PAIRS; ++j) {
           const f2 y = f2_mul(f2_add(V::pair(x[u], j), mm), cc);
@@ -350,33 +376,33 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
           ss = f2_add(ss, e);
           tt = f2_fma(e, y, tt);
         }
-      }
-      ahead += V::counted(n);
     }
     float s0, s1, t0, t1;
     f2_split(ss, s0, s1);
     f2_split(tt, t0, t1);
     s = s0 + s1;
     t = t0 + t1;
-    // the row's ends, logit by logit, in the threads that own these vectors
+    auto one = [&](int id, bool first) {  // first: ahead when equal
+      const float f = V::load(r.x + id);
+      best = fmaxf(best, f);
+      lp_move(m, s, t, f, c);
+      const float y = ((f < LP_FLOOR ? LP_FLOOR : f) - m) * c, e = lp_ex2(y);
+      s += e;
+      t = fmaf(e, y, t);
+      ahead += tok_ok && (first ? f >= xt : f >= xt_next);
+    };
+    if (brief)
+      for (int id = tid; id < p.vocab; id += LP_THREADS) one(id, id < tok);
     auto ragged = [&](int v) {
-      if (v < v_lo || v >= v_hi || (v - v_lo) % LP_THREADS != tid) return;
       for (int j = 0; j < V::N; ++j) {
         const int id = v * V::N - r.off + j;
-        if (id < 0 || id >= p.vocab) continue;
-        const float f = V::load(r.x + id);
-        best = fmaxf(best, f);
-        lp_move(m, s, t, f, c);
-        const float y = ((f < LP_FLOOR ? LP_FLOOR : f) - m) * c, e = lp_ex2(y);
-        s += e;
-        t = fmaf(e, y, t);
-        ahead += tok_ok && (v < tok_vec ? f >= xt : f >= xt_next);
+        if (id >= 0 && id < p.vocab) one(id, v < tok_vec);
       }
     };
-    if (r.w_lo > 0) ragged(0);
-    if (r.w_hi < r.nvec && (r.w_hi > 0 || r.w_lo == 0)) ragged(r.w_hi);
+    if (end0 >= 0 && tid == 0) ragged(end0);
+    if (end1 >= 0 && tid == 1) ragged(end1);
     // equal logits of lower id in the token's own vector
-    if (tok_ok && tid == 0 && tok_vec >= v_lo && tok_vec < v_hi)
+    if (!brief && tok_ok && tid == 2 && tok_vec >= v_lo && tok_vec < v_hi)
       for (int id = max(0, tok_vec * V::N - r.off); id < tok; ++id)
         ahead += V::load(r.x + id) == xt;
   }
@@ -384,7 +410,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
   // ---- the k best of this slice
   const int k = p.top;
   if (k > 0) {
-    const uint32_t mine = v_lo + tid < v_hi ? lp_order(best) : 0u;
+    const uint32_t mine = lp_order(best);  // (-inf for a thread without vectors)
     uint32_t thr = 0;
 #pragma unroll 1
     for (int bit = 31; bit >= 16; --bit) {
@@ -393,32 +419,40 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
     }
     if (tid == 0) s_owners = s_n = 0;
     __syncthreads();
-    if (mine >= thr && v_lo + tid < v_hi) s_owner[atomicAdd(&s_owners, 1)] = (uint16_t)tid;
+    if (mine >= thr && w_lo + tid < w_hi) s_owner[atomicAdd(&s_owners, 1)] = (uint16_t)tid;
     __syncthreads();
     const int owners = s_owners;
-    const int turns = (v_hi - v_lo + LP_THREADS - 1) / LP_THREADS;
-    const int items = turns * owners;
-    // keys of item i (owner i % owners, its vector i / owners) that reach the bounds
+    const int items = owners * ((w_hi - w_lo + LP_THREADS - 1) / LP_THREADS) + 2;
+    auto keep = [&](float f, int id, unsigned long long least) {
+      if (lp_order(f) < thr) return;
+      const unsigned long long key = lp_key(f, id);
+      if (key <= least) return;
+      const int at = atomicAdd(&s_n, 1);
+      if (at < LP_CAP) s_buf[at] = key;
+    };
+    // keys of item i that reach the bounds: vector (i - 2) / owners of an owner,
+    // items 0 and 1 the ragged ends
     auto look = [&](int i, unsigned long long least) {
-      const int v = v_lo + (i / owners) * LP_THREADS + s_owner[i % owners];
-      if (v >= v_hi) return;
-      const bool whole = r.whole(v);
+      int v;
+      if (i < 2) {
+        v = i ? end1 : end0;
+        if (v < 0) return;
+      } else {
+        v = w_lo + (i - 2) / owners * LP_THREADS + s_owner[(i - 2) % owners];
+        if (v >= w_hi) return;
+      }
       uint4 x = make_uint4(0, 0, 0, 0);
-      if (whole) x = r.load(v);
+      if (i >= 2) x = ldg_nc_v4(r.at(v));
 #pragma unroll
       for (int j = 0; j < V::N; ++j) {
         const int id = v * V::N - r.off + j;
         if (id < 0 || id >= p.vocab) continue;
-        const float f = whole ? V::at(x, j) : V::load(r.x + id);
-        if (lp_order(f) >= thr) {
-          const unsigned long long key = lp_key(f, id);
-          if (key > least) {
-            const int at = atomicAdd(&s_n, 1);
-            if (at < LP_CAP) s_buf[at] = key;
-          }
-        }
+        keep(i >= 2 ? V::at(x, j) : V::load(r.x + id), id, least);
       }
     };
+    if (brief)  // (at most LP_SHORT keys)
+      for (int id = tid; id < p.vocab; id += LP_THREADS) keep(V::load(r.x + id), id, 0);
+    else
 #pragma unroll 2
     for (int i = tid; i < items; i += LP_THREADS) look(i, 0);
     __syncthreads();
@@ -540,9 +574,9 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpParams 
 }
 
 // Slices per row: one CTA per row once the rows alone fill the GPU, else
-// slices of at least one vector per thread.
+// slices of at least one turn of the loop (bf16 vectors).
 int lp_parts(int rows, int vocab) {
-  const int most = (vocab - 1) / (LP_THREADS * 8) + 1;
+  const int most = (vocab - 1) / (LP_THREADS * LP_UNROLL * 8) + 1;
   int parts = rows > 0 ? LP_FILL / rows : 1;
   if (parts > most) parts = most;
   return parts < 1 ? 1 : parts > LP_MAX_PARTS ? LP_MAX_PARTS : parts;
