@@ -22,7 +22,7 @@ struct Kv8AppendParams {
   int64_t sb[2], sh[2], st[2];  // element strides of batch, head, row
   const int32_t *pos, *counts;
   int32_t *status;
-  int pos_add, n, shift, dshift, vec;  // log2 of the page and of dim / 8
+  int pos_add, n, shift, dshift, align;  // log2 of the page and of dim / 16; bytes
 };
 
 // 0x4B400000 + c as a float is 1.5 * 2^23 + c: adding 1.5 * 2^23 rounds to the
@@ -45,9 +45,38 @@ __device__ __forceinline__ uint32_t code_any(float x, float inv) {
   return rint_bits(v);
 }
 
+// 16 bf16 values: one 32-byte access where the address allows it.
+__device__ __forceinline__ void load16(uint32_t (&x)[8], const uint16_t *q, int align) {
+  if (align >= 32) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]),
+                   "=r"(x[6]), "=r"(x[7])
+                 : "l"(q));
+  } else if (align >= 16) {
+    const uint4 a = ldg_v4(q), b = ldg_v4(q + 8);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = q[2 * j] | ((uint32_t)q[2 * j + 1] << 16);
+  }
+}
+__device__ __forceinline__ void store16(uint16_t *q, const uint32_t (&x)[8], int align) {
+  if (align >= 32) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(q), "r"(x[0]),
+                 "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4 *>(q)[0] = make_uint4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<uint4 *>(q)[1] = make_uint4(x[4], x[5], x[6], x[7]);
+  }
+}
+
 // One CTA per (page window, K or V of one head, sequence): the window's new
 // rows stay in registers between the maximum and the codes, so each is read
-// once. NV 8-element vectors per thread cover page * dim <= NV * 2048.
+// once. NV vectors of 16 elements per thread cover page * dim <= NV * 4096.
+// HBM-bound (2 bytes read and 1 written per element); 16 elements per thread
+// and 32-byte loads keep it from being instruction-bound.
 template <int NV>
 __global__ void __launch_bounds__(KW_THREADS) kv8_append_kernel(Kv8AppendParams p) {
   __shared__ uint32_t s_max[KW_THREADS / 32];
@@ -55,7 +84,7 @@ __global__ void __launch_bounds__(KW_THREADS) kv8_append_kernel(Kv8AppendParams 
   pdl_wait();
   const int tid = threadIdx.x, b = blockIdx.z;
   const int kv = blockIdx.y & 1, h = blockIdx.y >> 1;
-  const int page = p.c.page, dim = p.c.dim;
+  const int page = p.c.page;
   const int pos = p.pos[b] + p.pos_add;
   const int rows = kv8_rows(p.counts, b, p.n, blockIdx.x == 0 && tid == 0 ? p.status : nullptr);
   if (pos < 0) {
@@ -65,44 +94,36 @@ __global__ void __launch_bounds__(KW_THREADS) kv8_append_kernel(Kv8AppendParams 
   const int idx = (pos >> p.shift) + blockIdx.x;         // page of the sequence
   const long long first = (long long)idx << p.shift;     // its first position
   if (rows == 0 || first >= (long long)pos + rows) return;
+  const int lo = max(0, (int)(pos - first));                            // new rows of the page:
+  const int hi = (int)min((long long)page, (long long)pos + rows - first);  // [lo, hi)
+  // thread's row r0 + i step of the page, elements col .. col + 15
+  const int r0 = tid >> p.dshift, col = (tid & ((1 << p.dshift) - 1)) * 16;
+  const int step = KW_THREADS >> p.dshift;
+  const int64_t row_step = kv ? p.st[1] : p.st[0];
+  const uint16_t *src = (kv ? p.src[1] + b * p.sb[1] + h * p.sh[1]
+                            : p.src[0] + b * p.sb[0] + h * p.sh[0]) +
+                        (first - pos + r0) * row_step + col;
+  uint32_t x[NV][8];
+  uint32_t mx = 0;  // max |x| as bf16 bits, two halves
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[i][j] = 0;
+    const int r = r0 + i * step;
+    if (r >= lo && r < hi) load16(x[i], src + i * step * row_step, p.align);
+  }
   const int id = kv8_page(p.c.page_table + (size_t)b * p.c.max_pages, p.c.max_pages, p.c.pages,
                           idx, tid == 0 ? p.status : nullptr);
   if (id < 0) return;
-  const int lo = max(0, (int)(pos - first));                            // new rows of the page:
-  const int hi = (int)min((long long)page, (long long)pos + rows - first);  // [lo, hi)
   const size_t ph = (size_t)id * p.c.kv_heads + h;
   float *scale_p = (kv ? p.c.v_scales : p.c.k_scales) + ph;
-  int8_t *codes = (kv ? p.c.v_codes : p.c.k_codes) + ph * (size_t)(page * dim);
+  uint4 *codes = reinterpret_cast<uint4 *>((kv ? p.c.v_codes : p.c.k_codes) +
+                                           ph * (size_t)(page * p.c.dim)) + tid;
   const float s0 = lo > 0 ? *scale_p : 0.f;
-  const uint16_t *src = kv ? p.src[1] + b * p.sb[1] + h * p.sh[1]
-                           : p.src[0] + b * p.sb[0] + h * p.sh[0];
-  const int64_t row_step = kv ? p.st[1] : p.st[0];
-  const int row0 = (int)(first - pos);                   // source row of page row 0
-
-  uint4 x[NV];
-  uint32_t mx = 0;                                        // max |x| as bf16 bits, two halves
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = tid + i * KW_THREADS, r = v >> p.dshift;
-    const int col = (v & ((1 << p.dshift) - 1)) * 8;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (r >= lo && r < hi) {
-      const uint16_t *q = src + (int64_t)(row0 + r) * row_step + col;
-      if (p.vec) {
-        x[i] = ldg_nc_v4(q);
-      } else {
-        x[i].x = q[0] | ((uint32_t)q[1] << 16);
-        x[i].y = q[2] | ((uint32_t)q[3] << 16);
-        x[i].z = q[4] | ((uint32_t)q[5] << 16);
-        x[i].w = q[6] | ((uint32_t)q[7] << 16);
-      }
-    }
-  }
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    constexpr uint32_t A = 0x7FFF7FFFu;
-    mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[i].x & A, x[i].y & A), __vmaxu2(x[i].z & A, x[i].w & A)));
-  }
+    for (int j = 0; j < 8; ++j) mx = __vmaxu2(mx, x[i][j] & 0x7FFF7FFFu);
   uint32_t m = max(mx & 0xFFFFu, mx >> 16);
   m = __reduce_max_sync(0xffffffffu, m);
   if ((tid & 31) == 0) s_max[tid >> 5] = m;
@@ -114,14 +135,12 @@ __global__ void __launch_bounds__(KW_THREADS) kv8_append_kernel(Kv8AppendParams 
     if (tid == 0) flag_status(p.status, VB_STATUS_NONFINITE);
     m = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t a = u[j] & 0x7FFFu, c = (u[j] >> 16) & 0x7FFFu;
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t a = x[i][j] & 0x7FFFu, c = (x[i][j] >> 16) & 0x7FFFu;
         m = max(m, max(a < 0x7F80u ? a : 0u, c < 0x7F80u ? c : 0u));
       }
-    }
     m = __reduce_max_sync(0xffffffffu, m);
     __syncthreads();
     if ((tid & 31) == 0) s_max[tid >> 5] = m;
@@ -137,35 +156,35 @@ __global__ void __launch_bounds__(KW_THREADS) kv8_append_kernel(Kv8AppendParams 
   const float ratio = grown ? __fdiv_rn(s0, s) : 1.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = tid + i * KW_THREADS, r = v >> p.dshift;
-    uint2 *dst = reinterpret_cast<uint2 *>(codes) + v;
+    const int r = r0 + i * step;
+    uint4 *dst = codes + i * KW_THREADS;
+    uint32_t c[16];
     if (r >= lo && r < hi) {
-      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint32_t c[8];
       if (finite) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          c[2 * j] = rint_bits(__fmul_rn(__uint_as_float(u[j] << 16), inv));
-          c[2 * j + 1] = rint_bits(__fmul_rn(__uint_as_float(u[j] & 0xFFFF0000u), inv));
+        for (int j = 0; j < 8; ++j) {
+          c[2 * j] = rint_bits(__fmul_rn(__uint_as_float(x[i][j] << 16), inv));
+          c[2 * j + 1] = rint_bits(__fmul_rn(__uint_as_float(x[i][j] & 0xFFFF0000u), inv));
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          c[2 * j] = code_any(__uint_as_float(u[j] << 16), inv);
-          c[2 * j + 1] = code_any(__uint_as_float(u[j] & 0xFFFF0000u), inv);
+        for (int j = 0; j < 8; ++j) {
+          c[2 * j] = code_any(__uint_as_float(x[i][j] << 16), inv);
+          c[2 * j + 1] = code_any(__uint_as_float(x[i][j] & 0xFFFF0000u), inv);
         }
       }
-      *dst = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
     } else if (grown && r < lo) {
-      const uint2 o = *dst;
-      uint32_t c[8];
+      const uint4 o = *dst;
+      const uint32_t w[4] = {o.x ^ 0x80808080u, o.y ^ 0x80808080u, o.z ^ 0x80808080u,
+                             o.w ^ 0x80808080u};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t w = j < 4 ? o.x : o.y;
-        c[j] = rint_bits(__fmul_rn(code_f32(w ^ 0x80808080u, j & 3), ratio));
-      }
-      *dst = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+      for (int j = 0; j < 16; ++j)
+        c[j] = rint_bits(__fmul_rn(code_f32(w[j >> 2], j & 3), ratio));
+    } else {
+      continue;
     }
+    *dst = make_uint4(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]),
+                      pack4(c[8], c[9], c[10], c[11]), pack4(c[12], c[13], c[14], c[15]));
   }
 }
 
@@ -178,55 +197,59 @@ struct Kv8ReadParams {
   const int32_t *lens, *start;
   uint16_t *dst[2];
   int32_t *status;
-  int n, shift, dshift;
+  int n, shift, dshift, align;
 };
 
-// One thread turns 8 codes into 8 bf16 values (8 bytes in, 16 out), KR_UNROLL
-// times; rows past the sequence's length are written as zeros.
+// A thread turns 16 codes into 16 bf16 values (16 bytes in, 32 out), KR_UNROLL
+// times; rows past the sequence's length are written as zeros. HBM-bound.
 __global__ void __launch_bounds__(KR_THREADS) kv8_read_kernel(Kv8ReadParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.z, kv = blockIdx.y & 1, h = blockIdx.y >> 1;
-  const int dim = p.c.dim;
   const int start = p.start ? p.start[b] : 0, len = p.lens[b];
   if (start < 0 && threadIdx.x == 0) flag_status(p.status, VB_STATUS_BOUNDS);
-  const long long total = (long long)p.n << p.dshift;
-  const float *scales = kv ? p.c.v_scales : p.c.k_scales;
-  const int8_t *codes = kv ? p.c.v_codes : p.c.k_codes;
-  uint4 *dst = reinterpret_cast<uint4 *>(kv ? p.dst[1] : p.dst[0]) +
-              ((long long)b * p.c.kv_heads + h) * total;
-  const long long base = (long long)blockIdx.x * (KR_THREADS * KR_UNROLL) + threadIdx.x;
+  const int total = p.n << p.dshift;  // (n <= 2^26)
+  const float *scales = (kv ? p.c.v_scales : p.c.k_scales) + h;
+  const int8_t *codes = (kv ? p.c.v_codes : p.c.k_codes) + (size_t)h * p.c.page * p.c.dim;
+  const uint32_t pool_step = (uint32_t)(p.c.kv_heads * p.c.page * p.c.dim);
+  uint16_t *dst = (kv ? p.dst[1] : p.dst[0]) +
+                  ((size_t)b * p.c.kv_heads + h) * ((size_t)p.n * p.c.dim);
+  const int base = blockIdx.x * (KR_THREADS * KR_UNROLL) + threadIdx.x;
   const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
-  uint2 w[KR_UNROLL];
+  int id[KR_UNROLL];
+#pragma unroll
+  for (int i = 0; i < KR_UNROLL; ++i) {
+    const int v = base + i * KR_THREADS;
+    const long long at = (long long)start + (v >> p.dshift);
+    id[i] = v < total && at >= 0 && at < len
+                ? kv8_page(table, p.c.max_pages, p.c.pages, (int)(at >> p.shift), p.status) : -1;
+  }
+  uint4 w[KR_UNROLL];
   float s[KR_UNROLL];
 #pragma unroll
   for (int i = 0; i < KR_UNROLL; ++i) {
-    const long long v = base + i * KR_THREADS;
-    w[i] = make_uint2(0, 0);
+    w[i] = make_uint4(0, 0, 0, 0);
     s[i] = 0.f;
-    if (v < total) {
-      const long long at = start + (v >> p.dshift);
-      if (at >= 0 && at < len) {
-        const int id = kv8_page(table, p.c.max_pages, p.c.pages, (int)(at >> p.shift), p.status);
-        if (id >= 0) {
-          const size_t ph = (size_t)id * p.c.kv_heads + h;
-          s[i] = __ldg(scales + ph);
-          w[i] = ldg_nc_v2(codes + (ph * p.c.page + (at & (p.c.page - 1))) * dim +
-                           (int)(v & ((1 << p.dshift) - 1)) * 8);
-        }
-      }
+    if (id[i] >= 0) {
+      const int v = base + i * KR_THREADS;
+      const int r = (start + (v >> p.dshift)) & (p.c.page - 1);
+      s[i] = __ldg(scales + (size_t)id[i] * p.c.kv_heads);
+      w[i] = ldg_nc_v4(codes + (size_t)id[i] * pool_step + r * p.c.dim +
+                       (v & ((1 << p.dshift) - 1)) * 16);
     }
   }
 #pragma unroll
   for (int i = 0; i < KR_UNROLL; ++i) {
-    const long long v = base + i * KR_THREADS;
+    const int v = base + i * KR_THREADS;
     if (v >= total) continue;
-    float f[8];
+    const uint32_t u[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u,
+                           w[i].w ^ 0x80808080u};
+    uint32_t o[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      f[j] = __fmul_rn(code_f32((j < 4 ? w[i].x : w[i].y) ^ 0x80808080u, j & 3), s[i]);
-    dst[v] = make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]),
-                        pack_bf2(f[6], f[7]));
+      o[j] = pack_bf2(__fmul_rn(code_f32(u[j >> 1], 2 * (j & 1)), s[i]),
+                      __fmul_rn(code_f32(u[j >> 1], 2 * (j & 1) + 1), s[i]));
+    store16(dst + (size_t)v * 16, o, p.align);
   }
 }
 
@@ -247,25 +270,26 @@ int vb_kv8_append(const VbKv8AppendArgs *a, vb_stream_t stream) {
   Kv8AppendParams p;
   p.c = a->cache;
   p.src[0] = a->keys; p.src[1] = a->values;
-  int vec = 1;
+  int64_t odd = 0;  // low bits of every row's offset in elements
   for (int i = 0; i < 2; ++i) {
     const int64_t *st = i ? a->v_strides : a->k_strides;
     p.sb[i] = st[0]; p.sh[i] = st[1]; p.st[i] = st[2];
-    if (((uintptr_t)p.src[i] % 16) || st[0] % 8 || st[1] % 8 || st[2] % 8) vec = 0;
+    odd |= (int64_t)((uintptr_t)p.src[i] / 2) | st[0] | st[1] | st[2];
+    VB_REQUIRE((uintptr_t)p.src[i] % 2 == 0, "vb_kv8_append: odd address");
   }
   p.pos = a->pos; p.counts = a->counts; p.status = a->status;
-  p.pos_add = a->pos_add; p.n = a->n; p.vec = vec;
+  p.pos_add = a->pos_add; p.n = a->n;
+  p.align = odd % 16 == 0 ? 32 : odd % 8 == 0 ? 16 : 2;
   p.shift = kv8_page_shift(p.c.page);
-  p.dshift = p.c.dim == 64 ? 3 : p.c.dim == 128 ? 4 : 5;
+  p.dshift = p.c.dim == 64 ? 2 : p.c.dim == 128 ? 3 : 4;
   const int windows = (int)(((long long)a->n + p.c.page - 2) / p.c.page) + 1;
   const dim3 grid(windows, p.c.kv_heads * 2, p.c.batch), block(KW_THREADS);
   cudaStream_t s = as_stream(stream);
-  switch (p.c.page * p.c.dim / (8 * KW_THREADS)) {
+  switch (p.c.page * p.c.dim / (16 * KW_THREADS)) {
     case 0: case 1: vb_launch(kv8_append_kernel<1>, grid, block, 0, s, false, p); break;
     case 2: vb_launch(kv8_append_kernel<2>, grid, block, 0, s, false, p); break;
     case 4: vb_launch(kv8_append_kernel<4>, grid, block, 0, s, false, p); break;
-    case 8: vb_launch(kv8_append_kernel<8>, grid, block, 0, s, false, p); break;
-    default: vb_launch(kv8_append_kernel<16>, grid, block, 0, s, false, p); break;
+    default: vb_launch(kv8_append_kernel<8>, grid, block, 0, s, false, p); break;
   }
   return check_launch("kv8_append_kernel");
 }
@@ -274,7 +298,7 @@ int vb_kv8_read(const VbKv8ReadArgs *a, vb_stream_t stream) {
   VB_REQUIRE(a, "vb_kv8_read: null args");
   const int rc = kv8_check(&a->cache, "vb_kv8_read");
   if (rc != VB_OK) return rc;
-  VB_REQUIRE(a->n >= 0, "vb_kv8_read: n=%d", a->n);
+  VB_REQUIRE(a->n >= 0 && a->n <= 1 << 26, "vb_kv8_read: n=%d (<= 2^26)", a->n);
   if (a->n == 0) return VB_OK;
   VB_REQUIRE(a->lens && a->keys && a->values, "vb_kv8_read: null tensor");
   VB_REQUIRE(((uintptr_t)a->keys % 16) == 0 && ((uintptr_t)a->values % 16) == 0,
@@ -284,10 +308,11 @@ int vb_kv8_read(const VbKv8ReadArgs *a, vb_stream_t stream) {
   p.lens = a->lens; p.start = a->start;
   p.dst[0] = a->keys; p.dst[1] = a->values;
   p.status = a->status; p.n = a->n;
+  p.align = ((uintptr_t)a->keys % 32) || ((uintptr_t)a->values % 32) ? 16 : 32;
   p.shift = kv8_page_shift(p.c.page);
-  p.dshift = p.c.dim == 64 ? 3 : p.c.dim == 128 ? 4 : 5;
+  p.dshift = p.c.dim == 64 ? 2 : p.c.dim == 128 ? 3 : 4;
   const long long per = KR_THREADS * KR_UNROLL;
-  const long long blocks = ((long long)a->n * (p.c.dim / 8) + per - 1) / per;
+  const long long blocks = ((long long)a->n * (p.c.dim / 16) + per - 1) / per;
   vb_launch(kv8_read_kernel, dim3((unsigned)blocks, p.c.kv_heads * 2, p.c.batch),
             dim3(KR_THREADS), 0, as_stream(stream), false, p);
   return check_launch("kv8_read_kernel");
