@@ -558,7 +558,8 @@ int vb_kv8_read(const VbKv8ReadArgs *args, vb_stream_t stream);
  * lse -inf. q bf16 [batch, q_heads, L, dim] with element strides {batch, head,
  * row}; out bf16 [batch, q_heads, L, dim] and lse float32 [batch, q_heads, L]
  * contiguous; query head hq reads kv head hq / (q_heads / kv_heads).
- * workspace: vb_kv8_attn_workspace_size bytes, no initial contents needed. */
+ * workspace: vb_kv8_attn_workspace_size bytes, zero-filled once, left reusable
+ * by every call (of one stream at a time). */
 typedef struct VbKv8AttnArgs {
   VbKv8Cache cache;
   const uint16_t *q;

@@ -17,7 +17,11 @@ struct Kv8AttnParams {
   // the range's weights are 2^(z - m), their sum l
   float *o_part;
   float2 *ml_part;
-  int2 *units;  // kv8_attn_kernel: first CTA and number of CTAs of a unit
+  // kv8_attn_kernel: a unit's first CTA and number of CTAs for the wide combine
+  // kernel (`wide`), else a ticket word per unit, zero between calls
+  int2 *units;
+  uint32_t *tickets;
+  bool wide;
   float scale_log2;  // scale * log2(e)
   int Hq, L, rep, len_add, causal, shift, vec;
   int row_tiles, splits;

@@ -286,10 +286,10 @@ int vb_kv8_append(const VbKv8AppendArgs *a, vb_stream_t stream) {
   const dim3 grid(windows, p.c.kv_heads * 2, p.c.batch), block(KW_THREADS);
   cudaStream_t s = as_stream(stream);
   switch (p.c.page * p.c.dim / (16 * KW_THREADS)) {
-    case 0: case 1: vb_launch(kv8_append_kernel<1>, grid, block, 0, s, false, p); break;
-    case 2: vb_launch(kv8_append_kernel<2>, grid, block, 0, s, false, p); break;
-    case 4: vb_launch(kv8_append_kernel<4>, grid, block, 0, s, false, p); break;
-    default: vb_launch(kv8_append_kernel<8>, grid, block, 0, s, false, p); break;
+    case 0: case 1: vb_launch(kv8_append_kernel<1>, grid, block, 0, s, true, p); break;
+    case 2: vb_launch(kv8_append_kernel<2>, grid, block, 0, s, true, p); break;
+    case 4: vb_launch(kv8_append_kernel<4>, grid, block, 0, s, true, p); break;
+    default: vb_launch(kv8_append_kernel<8>, grid, block, 0, s, true, p); break;
   }
   return check_launch("kv8_append_kernel");
 }
@@ -314,7 +314,7 @@ int vb_kv8_read(const VbKv8ReadArgs *a, vb_stream_t stream) {
   const long long per = KR_THREADS * KR_UNROLL;
   const long long blocks = ((long long)a->n * (p.c.dim / 16) + per - 1) / per;
   vb_launch(kv8_read_kernel, dim3((unsigned)blocks, p.c.kv_heads * 2, p.c.batch),
-            dim3(KR_THREADS), 0, as_stream(stream), false, p);
+            dim3(KR_THREADS), 0, as_stream(stream), true, p);
   return check_launch("kv8_read_kernel");
 }
 

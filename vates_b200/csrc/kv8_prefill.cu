@@ -572,7 +572,7 @@ int kp_launch(const Kv8AttnParams &p, cudaStream_t s) {
     ready = true;
   }
   vb_launch(kv8_prefill_kernel<D>, dim3(p.row_tiles * p.splits, p.c.kv_heads, p.c.batch),
-            dim3(KP_THREADS), H::SMEM, s, false, p);
+            dim3(KP_THREADS), H::SMEM, s, true, p);
   return check_launch("kv8_prefill_kernel");
 }
 

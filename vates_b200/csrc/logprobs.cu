@@ -634,9 +634,9 @@ int vb_token_logprobs(const VbTokenLogprobsArgs *a, vb_stream_t stream) {
   p.vocab = a->vocab; p.top = a->top;
   const dim3 grid(a->rows * p.parts), block(LP_THREADS);
   if (a->dtype == 0)
-    vb_launch(token_logprobs_kernel<uint16_t>, grid, block, 0, as_stream(stream), false, p);
+    vb_launch(token_logprobs_kernel<uint16_t>, grid, block, 0, as_stream(stream), true, p);
   else
-    vb_launch(token_logprobs_kernel<float>, grid, block, 0, as_stream(stream), false, p);
+    vb_launch(token_logprobs_kernel<float>, grid, block, 0, as_stream(stream), true, p);
   return check_launch("token_logprobs_kernel");
 }
 

@@ -19,7 +19,7 @@ import ctypes as C
 import torch
 
 from ._lib import (VbKv8AppendArgs, VbKv8AttnArgs, VbKv8Cache, VbKv8ReadArgs, check, lib)
-from .pool import on_stream, ptr, stream_handle
+from .pool import ptr, stream_handle
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
@@ -41,6 +41,20 @@ def _ints(t: torch.Tensor | None, what: str, batch: int) -> int | None:
     if t.dtype != torch.int32 or not t.is_cuda or t.numel() != batch or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous int32 CUDA tensor of {batch} values is needed")
     return t.data_ptr()
+
+
+_STRIDES: dict = {}
+
+
+def _strides(t: torch.Tensor):
+    """Strides of batch, head and row as the C array (made once per layout)."""
+    s = t.stride()
+    a = _STRIDES.get(s)
+    if a is None:
+        if len(_STRIDES) > 4096:
+            _STRIDES.clear()
+        a = _STRIDES[s] = (C.c_int64 * 3)(*s[:3])
+    return a
 
 
 class PagedKV8Cache:
@@ -88,6 +102,7 @@ class PagedKV8Cache:
         self._append_args = bytes(VbKv8AppendArgs(c))
         self._read_args = bytes(VbKv8ReadArgs(c))
         self._attn_args = bytes(VbKv8AttnArgs(c))
+        self._need = {}  # workspace bytes by (q_heads, L)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, batch: int, max_pages: int,
@@ -115,32 +130,35 @@ class PagedKV8Cache:
         table set VB_STATUS_BOUNDS in ``status`` and are dropped; an infinity is
         stored as the page's largest value, a NaN as 0, with
         VB_STATUS_NONFINITE."""
+        if stream is not None:  # with it as the current stream, copies are made on it
+            with torch.cuda.stream(stream):
+                return self.append(keys, values, pos, counts, pos_add, status)
         B, n = self.batch, keys.shape[2] if keys.dim() == 4 else -1
         shape = (B, self.kv_heads, n, self.head_dim)
-        with on_stream(stream):
-            keys, values = _rows(keys, "keys", shape), _rows(values, "values", shape)
+        keys, values = _rows(keys, "keys", shape), _rows(values, "values", shape)
         a = VbKv8AppendArgs.from_buffer_copy(self._append_args)
         a.keys, a.values = keys.data_ptr(), values.data_ptr()
-        a.k_strides, a.v_strides = keys.stride()[:3], values.stride()[:3]
+        a.k_strides, a.v_strides = _strides(keys), _strides(values)
         a.pos, a.counts = _ints(pos, "pos", B), _ints(counts, "counts", B)
         a.status, a.pos_add, a.n = ptr(status), pos_add, n
-        check(lib.vb_kv8_append(C.byref(a), stream_handle(stream)), "vb_kv8_append")
+        check(lib.vb_kv8_append(C.byref(a), stream_handle()), "vb_kv8_append")
 
     # -------------------------------------------------------------- read back
     def read(self, lens, n: int, start=None, status=None, stream=None):
         """``(keys, values)`` bf16 ``[batch, kv_heads, n, head_dim]``: the rows
         at positions ``start[b] + i`` (``start`` None: 0), zero from ``lens[b]``
         on."""
+        if stream is not None:  # with it as the current stream, results belong to it
+            with torch.cuda.stream(stream):
+                return self.read(lens, n, start, status)
         B = self.batch
-        with on_stream(stream):
-            keys = torch.empty((B, self.kv_heads, n, self.head_dim), dtype=torch.bfloat16,
-                               device=self.k_codes.device)
-            values = torch.empty_like(keys)
+        keys = self.k_codes.new_empty((B, self.kv_heads, n, self.head_dim), dtype=torch.bfloat16)
+        values = torch.empty_like(keys)
         a = VbKv8ReadArgs.from_buffer_copy(self._read_args)
         a.lens, a.start = _ints(lens, "lens", B), _ints(start, "start", B)
         a.keys, a.values = keys.data_ptr(), values.data_ptr()
         a.status, a.n = ptr(status), n
-        check(lib.vb_kv8_read(C.byref(a), stream_handle(stream)), "vb_kv8_read")
+        check(lib.vb_kv8_read(C.byref(a), stream_handle()), "vb_kv8_read")
         return keys, values
 
     # -------------------------------------------------------------- attention
@@ -153,39 +171,42 @@ class PagedKV8Cache:
         nothing, and rows from ``q_lens[b]`` on, are zero (log-sum-exp -inf).
         Returns bf16 ``[batch, q_heads, L, head_dim]``, with ``return_lse``
         also float32 ``[batch, q_heads, L]`` (natural log)."""
+        if stream is not None:  # with it as the current stream, results belong to it
+            with torch.cuda.stream(stream):
+                return self.attend(q, lens, q_lens, len_add, scale, causal, out, return_lse,
+                                   status)
         B, D = self.batch, self.head_dim
         if q.dim() != 4:
             raise ValueError(f"q: [batch, q_heads, L, head_dim] is needed, got {tuple(q.shape)}")
         Hq, L = q.shape[1], q.shape[2]
-        lse = None
-        with on_stream(stream):
-            q = _rows(q, "q", (B, Hq, L, D))
-            if out is None:
-                out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
-                raise ValueError("out: contiguous bfloat16 of q's shape is needed")
-            if return_lse:
-                lse = torch.empty((B, Hq, L), dtype=torch.float32, device=q.device)
+        q = _rows(q, "q", (B, Hq, L, D))
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+            raise ValueError("out: contiguous bfloat16 of q's shape is needed")
+        lse = q.new_empty((B, Hq, L), dtype=torch.float32) if return_lse else None
         a = VbKv8AttnArgs.from_buffer_copy(self._attn_args)
-        a.q, a.q_strides = q.data_ptr(), q.stride()[:3]
+        a.q, a.q_strides = q.data_ptr(), _strides(q)
         a.lens, a.q_lens = _ints(lens, "lens", B), _ints(q_lens, "q_lens", B)
         a.out, a.lse, a.status = out.data_ptr(), ptr(lse), ptr(status)
         a.scale = D ** -0.5 if scale is None else scale
         a.q_heads, a.L, a.len_add, a.causal = Hq, L, len_add, causal
-        need = lib.vb_kv8_attn_workspace_size(C.byref(a))
-        st = stream_handle(stream)
+        need = self._need.get((Hq, L))
+        if need is None:
+            need = self._need[Hq, L] = lib.vb_kv8_attn_workspace_size(C.byref(a))
+        st = stream_handle()
         if need:
-            ws = self._workspace(need, st, q.device, stream)
+            ws = self._workspace(need, st, q.device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         check(lib.vb_kv8_attn(C.byref(a), st), "vb_kv8_attn")
         return (out, lse) if return_lse else out
 
-    def _workspace(self, need: int, st: int, device, stream) -> torch.Tensor:
-        """Scratch of the key ranges' partial results, one per stream."""
+    def _workspace(self, need: int, st: int, device) -> torch.Tensor:
+        """Scratch of the key ranges' partial results, one per stream; zeroed when
+        made, left reusable by every call."""
         ws = self._ws.get(st)
         if ws is None or ws.numel() < need:
-            with on_stream(stream):
-                ws = self._ws[st] = torch.empty(need, dtype=torch.uint8, device=device)
+            ws = self._ws[st] = torch.zeros(need, dtype=torch.uint8, device=device)
         return ws
 
 

@@ -8,7 +8,7 @@ from typing import NamedTuple
 import torch
 
 from ._lib import VbTokenLogprobsArgs, check, lib
-from .pool import on_stream, ptr, stream_handle
+from .pool import ptr, stream_handle
 
 MAX_TOP = 32
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
@@ -23,15 +23,21 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor  # float32 [rows, top]
 
 
-def _workspace(need: int, st: int, device, stream) -> torch.Tensor:
+_needs: dict = {}
+
+
+def _workspace(rows: int, vocab: int, top: int, st: int, device) -> torch.Tensor:
     """Scratch of rows split over several CTAs, one per device and stream;
     zeroed when made, left reusable by every call."""
-    key = (device, st)
-    ws = _workspaces.get(key)
+    need = _needs.get((rows, vocab, top))
+    if need is None:
+        if len(_needs) > 4096:
+            _needs.clear()
+        need = _needs[rows, vocab, top] = lib.vb_token_logprobs_workspace_size(rows, vocab, top)
+    ws = _workspaces.get((device, st))
     if ws is None or ws.numel() < need:
-        with on_stream(stream):
-            ws = _workspaces[key] = torch.zeros(max(need, 1 << 16), dtype=torch.uint8,
-                                                device=device)
+        ws = torch.zeros(max(need, 1 << 16), dtype=torch.uint8, device=device)
+        _workspaces[device, st] = ws
     return ws
 
 
@@ -45,6 +51,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     that cannot follow. A NaN or +inf in a row makes its floating results NaN;
     a token outside the vocabulary gives NaN and rank -1 and sets
     VB_STATUS_BOUNDS in ``status``."""
+    if stream is not None:  # with it as the current stream, results belong to it
+        with torch.cuda.stream(stream):
+            return token_logprobs(logits, tokens, top, temperature, status)
     if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
         raise ValueError("logits: bfloat16 or float32 CUDA [rows, vocab] are needed, got "
                          f"{logits.dtype} {tuple(logits.shape)} on {logits.device}")
@@ -55,17 +64,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
                          f"{tuple(tokens.shape)}")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top={top}: 0 to {MAX_TOP} and at most the vocabulary ({vocab})")
-    dev = logits.device
-    with on_stream(stream):
-        if logits.stride(1) != 1 and vocab > 1:
-            logits = logits.contiguous()
-        lp = logits.new_empty(rows, dtype=torch.float32)
-        ent = torch.empty_like(lp)
-        rank = torch.empty_like(tokens)
-        tlp = lp.new_empty((rows, top))
-        ids = rank.new_empty((rows, top))
-    st = stream_handle(stream)
-    ws = _workspace(lib.vb_token_logprobs_workspace_size(rows, vocab, top), st, dev, stream)
+    if logits.stride(1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    lp = logits.new_empty(rows, dtype=torch.float32)
+    ent = torch.empty_like(lp)
+    rank = torch.empty_like(tokens)
+    tlp = lp.new_empty((rows, top))
+    ids = rank.new_empty((rows, top))
+    st = stream_handle()
+    ws = _workspace(rows, vocab, top, st, logits.device)
     a = VbTokenLogprobsArgs(logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(),
                             rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), ptr(status),
                             ws.data_ptr(), ws.numel(), logits.stride(0), temperature, rows, vocab,

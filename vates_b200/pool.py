@@ -10,7 +10,6 @@ streaming, eviction or residency miss handling in the timed path.
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -27,12 +26,6 @@ def stream_handle(stream=None) -> int:
         # the handle of torch.cuda.current_stream() without building its object
         return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     return stream.cuda_stream
-
-
-def on_stream(stream=None):
-    """Context in which new tensors belong to ``stream`` (None: the current
-    one), so that memory freed after a call on it is reused in its order."""
-    return nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
 def ptr(t) -> int | None:
