@@ -118,6 +118,20 @@ __device__ __forceinline__ void kp_regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// The order of volatile statements is kept, so a group's exponentials are issued
+// back to back.
+__device__ __forceinline__ float kp_ex2(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float kp_max3(uint32_t a, uint32_t b, uint32_t c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;"
+      : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return r;
+}
+
 struct KpBarriers {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2],
       o_last[2];
@@ -438,11 +452,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
         const float ks = __shfl_sync(0xffffffffu, ks_l, g);
         // scale 0: every code of the page is 0 (1 keeps -inf * 0 out)
         f[g] = fac * (ks > 0.f ? ks : 1.f);
-        float x = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          x = fmaxf(x, __uint_as_float(s[g >> 1][(g & 1) * 16 + j]));
-        top = fmaxf(top, x * f[g]);
+        const uint32_t *v = s[g >> 1] + (g & 1) * 16;
+        float x0 = kp_max3(v[0], v[1], v[2]), x1 = kp_max3(v[3], v[4], v[5]);
+        float x2 = kp_max3(v[6], v[7], v[8]), x3 = kp_max3(v[9], v[10], v[11]);
+        x0 = kp_max3(__float_as_uint(x0), v[12], v[13]);
+        x1 = kp_max3(__float_as_uint(x1), v[14], v[15]);
+        top = fmaxf(top, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * f[g]);
       }
       const bool move = top > m + KP_MOVE;
       const float to = move ? top : m;
@@ -469,28 +484,43 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
       }
       lvref = lv_new;
       const float sub = shift - (m == -INFINITY ? 0.f : m);
+      // Groups of 16: the arguments of the next one are formed before this one's
+      // exponentials are used, so that a warp alone on its scheduler does not
+      // wait for each.
+      float x[2][16], cg[8];
+      auto arguments = [&](int g) {
+        const float lv = __shfl_sync(0xffffffffu, lv_l, g);
+        cg[g] = lv > KP_NO_SCALE ? lv - lvref : 0.f;
+        const f2 ff = f2_make(f[g], f[g]), cc = f2_make(sub + cg[g], sub + cg[g]);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int gg = 0; gg < 4; ++gg) {
-          const int g = half * 4 + gg;
-          const float lv = __shfl_sync(0xffffffffu, lv_l, g);
-          const float dv = lv > KP_NO_SCALE ? lv - lvref : 0.f;
-          const float cg = sub + dv;
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            const float e0 = kv8_ex2(fmaf(__uint_as_float(s[g >> 1][(g & 1) * 16 + j]), f[g], cg));
-            const float e1 =
-                kv8_ex2(fmaf(__uint_as_float(s[g >> 1][(g & 1) * 16 + j + 1]), f[g], cg));
-            sum += e0 + e1;
-            pk[gg * 8 + (j >> 1)] = pack_h2(e0, e1);
-          }
-          l = fmaf(sum, kv8_ex2(fminf(-dv, 126.f)), l);
+        for (int j = 0; j < 16; j += 2) {
+          const uint32_t *v = s[g >> 1] + (g & 1) * 16 + j;
+          f2_split(f2_fma(f2_make(__uint_as_float(v[0]), __uint_as_float(v[1])), ff, cc),
+                   x[g & 1][j], x[g & 1][j + 1]);
         }
-        kp_tmem_st32(trow + slot * 128 + half * 32, pk);
+      };
+      arguments(0);
+      uint32_t pk[2][32];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        float e[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) e[j] = kp_ex2(x[g & 1][j]);
+        if (g < 7) arguments(g + 1);
+        f2 sum0 = f2_make(e[0], e[1]), sum1 = f2_make(e[2], e[3]);
+#pragma unroll
+        for (int j = 4; j < 16; j += 4) {
+          sum0 = f2_add(sum0, f2_make(e[j], e[j + 1]));
+          sum1 = f2_add(sum1, f2_make(e[j + 2], e[j + 3]));
+        }
+        float s0, s1;
+        f2_split(f2_add(sum0, sum1), s0, s1);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) pk[g >> 2][(g & 3) * 8 + (j >> 1)] = pack_h2(e[j], e[j + 1]);
+        l = fmaf(s0 + s1, kp_ex2(fminf(-cg[g], 126.f)), l);
+        if (g == 3) kp_tmem_st32(trow + slot * 128, pk[0]);
       }
+      kp_tmem_st32(trow + slot * 128 + 32, pk[1]);
       kp_tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();
