@@ -295,48 +295,35 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
     int id2 = group_page(t0 + 2);
     if (tid < 2) s_move[tid] = 0;
 
-    // ---- queries, in the order of the B fragments
-    for (int r = warp; r < ROWS; r += 4) {
-      const int i = p.row_of(r), hr = r - i * p.rep;
-      constexpr int PL = D / 32;  // elements per lane
-      float x[PL];
-      float amax = 0.f;
-      const uint16_t *src = p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh +
-                            (int64_t)i * p.ql + lane * PL;
-      uint32_t w[PL / 2];
+    // ---- queries, in the order of the B fragments: D / 8 lanes per row
+    {
+      constexpr int LPR = D / 8, PASS = KA_THREADS / LPR, NP = (ROWS + PASS - 1) / PASS;
+      const int c8 = tid % LPR;
+      uint4 w[NP];
 #pragma unroll
-      for (int j = 0; j < PL / 2; ++j) w[j] = 0;
-      if (r < rows && i < sp.q_len) {
-        if (p.vec) {
-          if constexpr (PL == 8) {
-            const uint4 v = ldg_v4(src);
-            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-          } else if constexpr (PL == 4) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(src);
-            w[0] = v.x; w[1] = v.y;
-          } else {
-            w[0] = *reinterpret_cast<const uint32_t *>(src);
-          }
-        } else {
+      for (int k = 0; k < NP; ++k) {
+        const int r = tid / LPR + k * PASS, i = p.row_of(r), hr = r - i * p.rep;
+        w[k] = make_uint4(0, 0, 0, 0);
+        if (r < rows && i < sp.q_len)
+          w[k] = kv8_load8(p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh +
+                               (int64_t)i * p.ql + c8 * 8,
+                           p.vec);
+      }
 #pragma unroll
-          for (int j = 0; j < PL / 2; ++j) w[j] = src[2 * j] | ((uint32_t)src[2 * j + 1] << 16);
+      for (int k = 0; k < NP; ++k) {
+        const int r = tid / LPR + k * PASS;
+        const float pw = kv8_q_scale<LPR>(w[k]);
+        if (r >= ROWS) continue;  // (8 rows of 64: half of the threads)
+        if (c8 == 0) s_fac[r] = p.scale_log2 / pw;
+        // dims 8 c8 .. + 7: d = 64 span + 16 c + 4 step + y; two steps of lane (row, c)
+        const int fl = (r & 7) * 4 + ((c8 & 7) >> 1);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int step = (c8 >> 3) * 4 + (c8 & 1) * 2 + j;
+          *reinterpret_cast<uint2 *>(
+              s_q + (((r >> 3) * (D / 32) + (step >> 1)) * 32 + fl) * 4 + (step & 1) * 2) =
+              j ? make_uint2(w[k].z, w[k].w) : make_uint2(w[k].x, w[k].y);
         }
-      }
-#pragma unroll
-      for (int j = 0; j < PL; ++j) {
-        x[j] = __uint_as_float((j & 1) ? (w[j >> 1] & 0xFFFF0000u) : (w[j >> 1] << 16));
-        amax = fmaxf(amax, fabsf(x[j]));
-      }
-      amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-      const float pw = kv8_q_power(amax);
-      if (lane == 0) s_fac[r] = p.scale_log2 / pw;
-#pragma unroll
-      for (int j = 0; j < PL; j += 2) {
-        // dim d = 64 span + 16 c + 4 step + y: lane (row, c), register pair of the step
-        const int d = lane * PL + j, step = (d >> 6) * 4 + ((d & 15) >> 2);
-        const int fl = (r & 7) * 4 + ((d & 63) >> 4);
-        s_q[(((r >> 3) * (D / 32) + (step >> 1)) * 32 + fl) * 4 + (step & 1) * 2 +
-            ((d & 2) >> 1)] = pack_h2(x[j] * pw, x[j + 1] * pw);
       }
     }
 

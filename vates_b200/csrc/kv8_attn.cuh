@@ -86,6 +86,32 @@ __device__ __forceinline__ uint32_t h2_codes(uint32_t magic) {
   return r;
 }
 
+// 8 bf16 of a query row.
+__device__ __forceinline__ uint4 kv8_load8(const uint16_t *q, bool vec) {
+  if (vec) return ldg_v4(q);
+  return make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16),
+                    q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
+}
+// The lane's 8 bf16 of a row that LPR lanes hold together become f16 times the
+// row's power of two, which is returned.
+template <int LPR>
+__device__ __forceinline__ float kv8_q_scale(uint4 &v) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float x[8], amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] = __uint_as_float((j & 1) ? (w[j >> 1] & 0xFFFF0000u) : (w[j >> 1] << 16));
+    amax = fmaxf(amax, fabsf(x[j]));
+  }
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const float pw = kv8_q_power(amax);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = pack_h2(x[2 * j] * pw, x[2 * j + 1] * pw);
+  v = make_uint4(w[0], w[1], w[2], w[3]);
+  return pw;
+}
+
 // Rows per row tile of the prefill kernel, and its launch (kv8_prefill.cu).
 int kv8_prefill_rows(int dim);
 int kv8_prefill_launch(const Kv8AttnParams &p, cudaStream_t s);

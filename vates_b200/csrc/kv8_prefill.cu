@@ -187,53 +187,29 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
     tc::tmem_relinquish();
   }
 
-  // ---- queries: a warp per row, f16 after the row's power of two
-  for (int r = warp; r < ROWS; r += KP_THREADS / 32) {
-    constexpr int PL = D / 32;
-    const int R = r_base + r, i = p.row_of(R), hr = R - i * p.rep;
-    const bool valid = n_items > 0 && R < rows && i < sp.q_len;
-    const uint16_t *src = p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql +
-                          lane * PL;
-    uint32_t w[PL / 2];
+  // ---- queries: D / 8 lanes per row, f16 after the row's power of two; all
+  // loads before the first use
+  {
+    constexpr int LPR = D / 8, PASS = KP_THREADS / LPR, NP = ROWS / PASS;
+    const int c8 = tid % LPR;
+    uint4 w[NP];
 #pragma unroll
-    for (int j = 0; j < PL / 2; ++j) w[j] = 0;
-    if (valid) {
-      if (p.vec) {
-        if constexpr (PL == 8) {
-          const uint4 v = ldg_v4(src);
-          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-        } else if constexpr (PL == 4) {
-          const uint2 v = *reinterpret_cast<const uint2 *>(src);
-          w[0] = v.x; w[1] = v.y;
-        } else {
-          w[0] = *reinterpret_cast<const uint32_t *>(src);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < PL / 2; ++j) w[j] = src[2 * j] | ((uint32_t)src[2 * j + 1] << 16);
-      }
-    }
-    float x[PL], amax = 0.f;
-#pragma unroll
-    for (int j = 0; j < PL; ++j) {
-      x[j] = __uint_as_float((j & 1) ? (w[j >> 1] & 0xFFFF0000u) : (w[j >> 1] << 16));
-      amax = fmaxf(amax, fabsf(x[j]));
+    for (int k = 0; k < NP; ++k) {
+      const int R = r_base + tid / LPR + k * PASS, i = p.row_of(R), hr = R - i * p.rep;
+      w[k] = make_uint4(0, 0, 0, 0);
+      if (n_items > 0 && R < rows && i < sp.q_len)
+        w[k] = kv8_load8(p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql +
+                             c8 * 8,
+                         p.vec);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float pw = kv8_q_power(amax);
-    if (lane == 0) s_fac[r] = p.scale_log2 / pw;
-#pragma unroll
-    for (int j = 0; j < PL / 2; ++j) w[j] = pack_h2(x[2 * j] * pw, x[2 * j + 1] * pw);
-    const int d = lane * PL;
-    uint8_t *dst = smem + H::Q_OFF + (r >> 7) * H::TILE + (d >> 6) * KP_BLOCK +
-                   kp_sw(r & 127, (d & 63) >> 3) + (d & 7) * 2;
-    if constexpr (PL == 8)
-      *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    else if constexpr (PL == 4)
-      *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
-    else
-      *reinterpret_cast<uint32_t *>(dst) = w[0];
+    for (int k = 0; k < NP; ++k) {
+      const int r = tid / LPR + k * PASS;
+      const float pw = kv8_q_scale<LPR>(w[k]);
+      if (c8 == 0) s_fac[r] = p.scale_log2 / pw;
+      *reinterpret_cast<uint4 *>(smem + H::Q_OFF + (r >> 7) * H::TILE + (c8 >> 3) * KP_BLOCK +
+                                 kp_sw(r & 127, c8 & 7)) = w[k];
+    }
   }
   tc::fence_proxy_async_smem();
   tc::tc_fence_before();
