@@ -794,7 +794,7 @@ struct Kv8Plan {
 
 // Up to 32 rows per kv head: kv8_attn_kernel, 8, 16 or 32 rows, its CTAs on
 // each of 148 SMs (fewer when the table holds fewer tiles). More rows: the
-// tcgen05 kernel, one CTA per SM, key ranges as many as fill 148 SMs.
+// tcgen05 kernel, a pair of CTAs per two SMs, key ranges as many as fill 148 SMs.
 Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   Kv8Plan pl;
   const long long rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
@@ -802,10 +802,10 @@ Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   const long long cap = (long long)a->cache.max_pages * a->cache.page;
   pl.tensor = rows > 32;
   if (pl.tensor) {
-    pl.tile_rows = kv8_prefill_rows(a->cache.dim);
+    pl.tile_rows = kv8_prefill_rows();
     pl.row_tiles = (int)((rows + pl.tile_rows - 1) / pl.tile_rows);
     const long long base = units * pl.row_tiles, most = (cap + 127) / 128;
-    long long s = 148 / base;
+    long long s = 74 / base;  // pairs of CTAs
     s = s < 1 ? 1 : s > most ? most : s;
     pl.splits = (int)s;
     pl.ctas = 0;

@@ -113,7 +113,7 @@ __device__ __forceinline__ float kv8_q_scale(uint4 &v) {
 }
 
 // Rows per row tile of the prefill kernel, and its launch (kv8_prefill.cu).
-int kv8_prefill_rows(int dim);
+int kv8_prefill_rows();
 int kv8_prefill_launch(const Kv8AttnParams &p, cudaStream_t s);
 
 }  // namespace vb

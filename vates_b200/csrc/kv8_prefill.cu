@@ -4,29 +4,31 @@
 //
 //   z = scale * s_K(page) * (q . code_K),  o = sum_j 2^(z_j log2 e - m) s_V(page_j) code_V / l
 //
-// One CTA per SM owns NT row tiles of 128 query rows of one kv head (rows are
-// the flattened (query, head of the group) pairs, so any group size fills them)
-// and a range of keys in tiles of 128. The codes are exact in f16, and so are
-// the queries after a power of two per row: both products are f16 with float32
-// sums. Roles (four warpgroups):
-//   * converters read the int8 rows from global memory (registers, one tile
-//     ahead; page numbers two ahead) and write them as f16 operands in 128-byte
-//     swizzled shared memory: K K-major, V as it lies (MN-major operand);
-//   * one thread issues S = Q K^T of the next (key tile, row tile) item before
-//     O += P V of the current one, so the tensor core works while the softmax
-//     runs; the two S slots alternate;
-//   * a softmax warpgroup per row tile (a thread per row = TMEM lane; for one
-//     row tile two warpgroups would have to split the row) takes S, keeps a
-//     running maximum that only moves when it grows by more than 2^4 (then O
-//     and l are rescaled), and stores P = 2^(z - m) s_V / v over S in TMEM as
-//     the f16 A operand of the second product. v is a power of two at least
-//     every V scale so far. l is summed in float32 from the unrounded weights.
+// A pair of CTAs on two SMs (a cluster; tcgen05 cta_group::2) owns 256 query rows
+// of one kv head, 128 each (rows are the flattened (query, head of the group)
+// pairs, so any group size fills them), and a range of keys in tiles of 128.
+// Each CTA converts and holds half of every K tile (64 keys) and half of every V
+// tile (half of the dims) for both: half the loads, conversions and shared-memory
+// reads that a CTA on its own would need (4,096 rows over 32,768 keys of 256:
+// 2.4 ms). The codes are exact in f16, and so are the queries after a power of
+// two per row: both products are f16 with float32 sums. Roles (warpgroups):
+//   * converters read the int8 rows from global memory into registers (K a tile
+//     ahead of V, page numbers another tile ahead) and write them as f16 operands
+//     in 128-byte swizzled shared memory, two stages: K K-major, V as it lies
+//     (MN-major operand);
+//   * one thread of the pair issues S = Q K^T of the next key tile before
+//     O += P V of the current one, so the tensor cores work while the softmax
+//     runs; two S slots alternate;
+//   * two softmax warpgroups per CTA, a thread per row and 64 keys (a row's two
+//     threads exchange their maxima in shared memory): the running maximum only
+//     moves when it grows by more than 2^4 (then O and l are rescaled), and
+//     P = 2^(z - m) s_V / v goes over S in TMEM as the f16 A operand of the second
+//     product. v is a power of two at least every V scale so far. l is summed in
+//     float32 from the unrounded weights.
 // A wait names the n-th completion of a barrier by its parity alone, so when it
-// begins, completion n - 1 must have happened and n + 1 must not: S of an item
-// waits for O of the last item in its slot, and the last O of a row tile has a
-// barrier of its own.
-// NT = 2 for head sizes 64 and 128, 1 for 256 (TMEM: 2 x 128 columns of S and
-// NT * D of O are all 512). Every wait is bounded (2 s, then VB_STATUS_TIMEOUT).
+// begins, completion n - 1 must have happened and n + 1 must not: S of a tile
+// waits for O of the last tile in its slot, and the last O and the end have
+// barriers of their own. Every wait is bounded (2 s, then VB_STATUS_TIMEOUT).
 #include "kv8_attn.cuh"
 #include "tc100.cuh"
 
@@ -35,6 +37,8 @@ namespace {
 
 constexpr int KP_THREADS = 512;
 constexpr int KP_KT = 128;              // keys per tile
+constexpr int KP_STAGES = 2;            // K, and V, operand tiles
+constexpr int KP_ROWS = 256;            // query rows of a pair of CTAs
 constexpr int KP_BLOCK = 16384;         // 128 rows x 64 f16, 128-byte swizzle
 constexpr uint64_t KP_WAIT_NS = 2000000000ull;
 // Weights as f16 are 2^(z - m + shift) s_V / v, at most 2^15.5. A range of one
@@ -50,21 +54,20 @@ constexpr float KP_NO_SCALE = -1000.f;  // log2 of the V scale of an all-zero pa
 
 template <int D>
 struct KpShape {
-  static constexpr int NT = D == 256 ? 1 : 2;       // row tiles
-  static constexpr int STAGES = D == 256 ? 1 : 2;   // K, and V, operand tiles
-  static constexpr int CONV_WG = D == 256 ? 2 : 1;  // converter warpgroups
-  static constexpr int BLK = D / 64;                // 64-dim blocks of an operand tile
-  static constexpr int TILE = BLK * KP_BLOCK;
-  static constexpr int Q_OFF = 0;
-  static constexpr int K_OFF = NT * TILE;
-  static constexpr int V_OFF = K_OFF + STAGES * TILE;
-  static constexpr int SMEM = V_OFF + STAGES * TILE + 1024;
-  // registers per thread of the warpgroups; 128 at launch
-  static constexpr int R_MMA = 40;
-  static constexpr int R_CONV = D == 256 ? 120 : 104;
-  static constexpr int R_SOFT = D == 256 ? 232 : 184;
-  static_assert(R_MMA + CONV_WG * R_CONV + NT * R_SOFT == 4 * 128, "register shares");
+  static constexpr int Q_BYTES = 128 * D * 2;
+  static constexpr int K_BLOCK = KP_BLOCK / 2;      // 64 keys x 64 dims
+  static constexpr int K_HALF = 64 * D * 2;
+  // Dims of this CTA's V half. Halves of 64 dims at least: for D = 64, CTA 0 holds
+  // all of V and the columns of O from 64 on are not used.
+  static constexpr int VD = D == 256 ? 128 : 64;
+  static constexpr int V_HALF = 128 * VD * 2;
+  static constexpr int K_OFF = Q_BYTES;
+  static constexpr int V_OFF = K_OFF + KP_STAGES * K_HALF;
+  static constexpr int SMEM = V_OFF + KP_STAGES * V_HALF + 1024;
 };
+// Registers per thread of the four warpgroups; 128 at launch.
+constexpr int KP_R_MMA = 40, KP_R_CONV = 104, KP_R_SOFT = 184;
+static_assert(KP_R_MMA + KP_R_CONV + 2 * KP_R_SOFT == 4 * 128, "register shares");
 
 // Byte offset of 16-byte chunk c of row r in a 128-row x 64-column block.
 __device__ __forceinline__ uint32_t kp_sw(int r, int c) {
@@ -81,19 +84,60 @@ __device__ __forceinline__ uint64_t kp_desc_mn(uint32_t saddr) {
   d |= (uint64_t)2 << 61;
   return d;
 }
-__host__ __device__ constexpr uint32_t kp_idesc(int N, bool b_mn) {  // f16 x f16 -> f32, M = 128
+__host__ __device__ constexpr uint32_t kp_idesc(int N, bool b_mn) {  // f16 x f16 -> f32, M = 256
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
-         ((uint32_t)(128 >> 4) << 24);
+         ((uint32_t)(256 >> 4) << 24);
 }
-// D[tmem] += A[tmem] * B[smem].
-__device__ __forceinline__ void kp_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
-                                          uint32_t idesc, uint32_t accumulate) {
+// The pair's products, issued by one thread of CTA 0: rows 0-127 of A and D are
+// CTA 0's, 128-255 CTA 1's; each holds half of B's N. The whole warp comes here
+// (its values are then uniform); `one` is true in the lane that issues.
+__device__ __forceinline__ uint32_t kp_elect() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void kp_mma_ss(uint32_t one, uint32_t d_tmem, uint64_t adesc,
+                                          uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
       : "memory");
 }
+__device__ __forceinline__ void kp_mma_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem,
+                                          uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+// Arrive on this barrier of both CTAs once all products issued so far are done.
+__device__ __forceinline__ void kp_commit(uint32_t one, uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+      " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster"
+      ".b64 [%0], %1;\n}\n" ::"r"(tc::smem_u32(bar)),
+      "h"((uint16_t)3), "r"(one)
+      : "memory");
+}
+// Arrive on CTA 0's barrier, from either CTA. What the arrival stands for is
+// ordered before it on its own SM: operands in shared memory by the proxy fence,
+// P and O in TMEM by tcgen05.wait. A release of cluster scope in its place costs
+// about 1,300 cycles an arrival.
+__device__ __forceinline__ void kp_arrive_leader(uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n"
+      " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(tc::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void kp_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The 256 softmax threads of a CTA.
+__device__ __forceinline__ void kp_soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void kp_tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
@@ -133,71 +177,75 @@ __device__ __forceinline__ float kp_max3(uint32_t a, uint32_t b, uint32_t c) {
 }
 
 struct KpBarriers {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2],
-      o_last[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done, o_last, drain;
 };
 
 template <int D>
-__global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParams p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
+    kv8_prefill_kernel(Kv8AttnParams p) {
   using H = KpShape<D>;
-  constexpr int NT = H::NT, ST = H::STAGES, ROWS = 128 * NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~uintptr_t(1023));
   __shared__ __align__(8) KpBarriers bar;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  __shared__ float s_fac[ROWS];
+  __shared__ float s_fac[128], s_half[2][2][128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
   pdl_launch_dependents();
   pdl_wait();
 
-  // ---- this CTA's rows and keys
-  const int split = blockIdx.x % p.splits;
-  const int rt = p.row_tiles - 1 - blockIdx.x / p.splits;  // longest (causal) rows first
+  // ---- the pair's rows and keys, this CTA's rows r_base .. + 127
+  const int rank = blockIdx.x & 1;
+  const int split = (blockIdx.x >> 1) % p.splits;
+  const int rt = p.row_tiles - 1 - (blockIdx.x >> 1) / p.splits;  // longest (causal) rows first
   const int h = blockIdx.y, b = blockIdx.z;
-  const int r_base = rt * ROWS, rows = p.L * p.rep;
+  const int pair_base = rt * KP_ROWS, r_base = pair_base + rank * 128, rows = p.L * p.rep;
   const Kv8Span sp = kv8_span(p, b, blockIdx.x == 0 && h == 0 && tid == 0);
-  const int i_last = min(min(r_base + ROWS, rows) - 1, sp.q_len * p.rep - 1) / p.rep;
-  const int kend = r_base < sp.q_len * p.rep ? sp.visible(i_last) : 0;
+  const int i_last = p.row_of(max(0, min(min(pair_base + KP_ROWS, rows), sp.q_len * p.rep) - 1));
+  const int kend = pair_base < sp.q_len * p.rep ? sp.visible(i_last) : 0;
   const int tiles = (kend + KP_KT - 1) / KP_KT;
   const int share = tiles / p.splits, rest = tiles % p.splits;
   const int t0 = split * share + min(split, rest);
   const int t1 = t0 + share + (split < rest);
-  const int n_items = (t1 - t0) * NT;
+  const int n_tiles = t1 - t0;
   const size_t tile_id = (((size_t)b * p.c.kv_heads + h) * p.row_tiles + rt) * p.splits + split;
   const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&bar.k_full[i], 4 * H::CONV_WG);
-      tc::mbar_init(&bar.v_full[i], 4 * H::CONV_WG);
+      tc::mbar_init(&bar.k_full[i], 2 * 4);   // converter warps of both CTAs
+      tc::mbar_init(&bar.v_full[i], 2 * 4);
       tc::mbar_init(&bar.k_empty[i], 1);
       tc::mbar_init(&bar.v_empty[i], 1);
       tc::mbar_init(&bar.s_full[i], 1);
-      tc::mbar_init(&bar.p_full[i], 4);
-      tc::mbar_init(&bar.o_done[i], 1);
-      tc::mbar_init(&bar.o_last[i], 1);
+      tc::mbar_init(&bar.p_full[i], 2 * 8);   // softmax warps of both CTAs
     }
+    tc::mbar_init(&bar.o_done, 1);
+    tc::mbar_init(&bar.o_last, 1);
+    tc::mbar_init(&bar.drain, 1);
     s_abort = 0;
     tc::fence_mbar_init();
   }
   if (warp == 0) {
-    tc::tmem_alloc(&s_tmem, 512);
-    tc::tmem_relinquish();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     tc::smem_u32(&s_tmem)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
 
   // ---- queries: D / 8 lanes per row, f16 after the row's power of two; all
   // loads before the first use
   {
-    constexpr int LPR = D / 8, PASS = KP_THREADS / LPR, NP = ROWS / PASS;
+    constexpr int LPR = D / 8, PASS = KP_THREADS / LPR, NP = 128 / PASS;
     const int c8 = tid % LPR;
     uint4 w[NP];
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       const int R = r_base + tid / LPR + k * PASS, i = p.row_of(R), hr = R - i * p.rep;
       w[k] = make_uint4(0, 0, 0, 0);
-      if (n_items > 0 && R < rows && i < sp.q_len)
+      if (n_tiles > 0 && R < rows && i < sp.q_len)
         w[k] = kv8_load8(p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql +
                              c8 * 8,
                          p.vec);
@@ -207,13 +255,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
       const int r = tid / LPR + k * PASS;
       const float pw = kv8_q_scale<LPR>(w[k]);
       if (c8 == 0) s_fac[r] = p.scale_log2 / pw;
-      *reinterpret_cast<uint4 *>(smem + H::Q_OFF + (r >> 7) * H::TILE + (c8 >> 3) * KP_BLOCK +
-                                 kp_sw(r & 127, c8 & 7)) = w[k];
+      *reinterpret_cast<uint4 *>(smem + (c8 >> 3) * KP_BLOCK + kp_sw(r, c8 & 7)) = w[k];
     }
   }
   tc::fence_proxy_async_smem();
   tc::tc_fence_before();
   __syncthreads();
+  kp_cluster_sync();  // barriers, TMEM and queries of both CTAs are there
   tc::tc_fence_after();
   const uint32_t tmem = s_tmem;
   volatile int *abort = &s_abort;
@@ -221,71 +269,67 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
 
   if (wg == 0) {
     // ================================================== tensor-core issuer
-    kp_regs_dec<H::R_MMA>();
-    if (tid == 0) {
-      constexpr uint32_t ID_S = kp_idesc(KP_KT, false), ID_O = kp_idesc(D, true);
+    kp_regs_dec<KP_R_MMA>();
+    if (warp == 0 && rank == 0) {
+      constexpr uint32_t ID_S = kp_idesc(KP_KT, false), ID_O = kp_idesc(2 * H::VD, true);
+      const uint32_t one = kp_elect();
+      // descriptors of the first 16-element step; a step adds to the address field
+      const uint64_t q_desc = tc::smem_desc_sw128(sbase);
+      const uint64_t k_desc = tc::smem_desc_sw128(sbase + H::K_OFF);
+      const uint64_t v_desc = kp_desc_mn(sbase + H::V_OFF);
       auto wait = [&](uint64_t *m, int n) {  // n-th completion (from 0) of a barrier
-        if (!tc::mbar_wait(m, (uint32_t)(n & 1), abort, KP_WAIT_NS)) {
-          s_abort = 1;
-          return false;
-        }
-        return true;
+        if (!tc::mbar_wait(m, (uint32_t)(n & 1), abort, KP_WAIT_NS)) s_abort = 1;
+        return !__any_sync(0xffffffffu, *abort != 0);
       };
-      int s_sent = 0, o_sent = 0;
       bool ok = true;
-      for (int w = 0; w <= n_items && ok; ++w) {
-        if (w < n_items) {  // S of item w
-          const int kt = w / NT, tile = w % NT, st = kt % ST;
-          // the slot's P has been read: O of item w - 2 is done
-          if (w >= 2) ok = wait(&bar.o_done[tile], (w - 2) / NT);
-          if (tile == 0) ok = ok && wait(&bar.k_full[st], kt / ST);
+      for (int w = 0; w <= n_tiles && ok; ++w) {
+        if (w < n_tiles) {  // S of tile w
+          const int st = w % KP_STAGES;
+          // the slot's P has been read: O of tile w - 2 is done
+          if (w >= 2) ok = wait(&bar.o_done, w - 2);
+          ok = ok && wait(&bar.k_full[st], w / KP_STAGES);
           if (!ok) break;
           tc::tc_fence_after();
-          const uint32_t qa = sbase + H::Q_OFF + tile * H::TILE;
-          const uint32_t ka = sbase + H::K_OFF + st * H::TILE;
+          const uint64_t kd = k_desc + st * (H::K_HALF >> 4);
+          const uint32_t d = tmem + (w & 1) * 128;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t o = (kk >> 2) * KP_BLOCK + (kk & 3) * 32;
-            tc::mma_bf16_ss(tmem + (w & 1) * 128, tc::smem_desc_sw128(qa + o),
-                            tc::smem_desc_sw128(ka + o), ID_S, kk > 0 ? 1u : 0u);
-          }
-          tc::mma_commit(&bar.s_full[w & 1]);
-          if (tile == NT - 1) tc::mma_commit(&bar.k_empty[st]);
-          ++s_sent;
+          for (int kk = 0; kk < D / 16; ++kk)
+            kp_mma_ss(one, d, q_desc + (((kk >> 2) * KP_BLOCK + (kk & 3) * 32) >> 4),
+                      kd + (((kk >> 2) * H::K_BLOCK + (kk & 3) * 32) >> 4), ID_S,
+                      kk > 0 ? 1u : 0u);
+          kp_commit(one, &bar.s_full[w & 1]);
+          kp_commit(one, &bar.k_empty[st]);
         }
-        if (w > 0) {  // O += P V of item w - 1
-          const int v = w - 1, kt = v / NT, tile = v % NT, st = kt % ST;
-          if (tile == 0) ok = wait(&bar.v_full[st], kt / ST);
-          ok = ok && wait(&bar.p_full[v & 1], v >> 1);
+        if (w > 0) {  // O += P V of tile w - 1
+          const int v = w - 1, st = v % KP_STAGES;
+          ok = wait(&bar.v_full[st], v / KP_STAGES) && wait(&bar.p_full[v & 1], v >> 1);
           if (!ok) break;
           tc::tc_fence_after();
-          const uint32_t va = sbase + H::V_OFF + st * H::TILE;
+          const uint64_t vd = v_desc + st * (H::V_HALF >> 4);
+          const uint32_t a = tmem + (v & 1) * 128;
 #pragma unroll
           for (int kk = 0; kk < KP_KT / 16; ++kk)
-            kp_mma_ts(tmem + 256 + tile * D, tmem + (v & 1) * 128 + kk * 8,
-                      kp_desc_mn(va + kk * 2048), ID_O, (kt > 0 || kk > 0) ? 1u : 0u);
-          tc::mma_commit(&bar.o_done[tile]);
-          if (v >= n_items - NT) tc::mma_commit(&bar.o_last[tile]);
-          if (tile == NT - 1) tc::mma_commit(&bar.v_empty[st]);
-          ++o_sent;
+            kp_mma_ts(one, tmem + 256, a + kk * 8, vd + (kk * 2048 >> 4), ID_O,
+                      kk > 0 ? 1u : (v > 0 ? 1u : 0u));
+          kp_commit(one, &bar.o_done);
+          if (v == n_tiles - 1) kp_commit(one, &bar.o_last);
+          kp_commit(one, &bar.v_empty[st]);
         }
       }
-      // nothing of this CTA may be in flight when TMEM is freed
-      for (int w = max(0, s_sent - 2); w < s_sent; ++w)
-        if (!tc::mbar_wait(&bar.s_full[w & 1], (uint32_t)((w >> 1) & 1), nullptr, KP_WAIT_NS))
-          s_abort = 1;
-      for (int v = max(0, o_sent - NT); v < o_sent; ++v)
-        if (!tc::mbar_wait(&bar.o_done[v % NT], (uint32_t)((v / NT) & 1), nullptr, KP_WAIT_NS))
-          s_abort = 1;
+      // nothing of the pair may be in flight when TMEM is freed
+      kp_commit(one, &bar.drain);
+      if (!tc::mbar_wait(&bar.drain, 0, nullptr, KP_WAIT_NS)) s_abort = 1;
     }
     __syncwarp();
-  } else if (wg <= H::CONV_WG) {
+  } else if (wg == 1) {
     // ================================================== converters
-    kp_regs_dec<H::R_CONV>();
-    constexpr int CT = 128 * H::CONV_WG, CPR = D / 16, STEP = CT / CPR, NC = KP_KT / STEP;
+    kp_regs_dec<KP_R_CONV>();
     const int ctid = tid - 128;
-    const int ch = ctid % CPR, key0 = ctid / CPR;
-    uint4 kr[NC], vr[NC];
+    // K: 64 keys of all dims; V: 128 keys of half of the dims; 16 codes at a time
+    constexpr int KC = D / 16, KSTEP = 128 / KC, KN = 64 / KSTEP;
+    constexpr int VC = H::VD / 16, VSTEP = 128 / VC, VN = 128 / VSTEP;
+    const int kch = ctid % KC, kkey = ctid / KC, vch = ctid % VC, vkey = ctid / VC;
+    uint4 kr[KN], vr[VN];
     // pool page of the 16-key group lane % 8 of tile t; rows without a page (past
     // the last key, or flagged) read page 0: their weights are 0
     auto group_page = [&](int t) {
@@ -294,84 +338,90 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
                  ? max(0, kv8_page(table, p.c.max_pages, p.c.pages, key >> p.shift, p.status)) : 0;
     };
     const size_t pool_step = (size_t)p.c.kv_heads * p.c.page * D;
-    const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + ch * 16;
-    const int8_t *vbase = p.c.v_codes + (size_t)h * p.c.page * D + ch * 16;
-    auto load = [&](uint4 (&x)[NC], const int8_t *base, int id) {
+    const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + kch * 16;
+    const int8_t *vbase = p.c.v_codes + (size_t)h * p.c.page * D + rank * H::VD + vch * 16;
+    auto load_k = [&](int id) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int key = key0 + i * STEP;  // a tile starts on a page boundary (page <= 128)
+      for (int i = 0; i < KN; ++i) {
+        const int key = rank * 64 + kkey + i * KSTEP;  // a tile starts on a page boundary
         const int pg = __shfl_sync(0xffffffffu, id, key >> 4);
-        x[i] = ldg_nc_v4(base + pg * pool_step + (key & (p.c.page - 1)) * D);
+        kr[i] = ldg_nc_v4(kbase + pg * pool_step + (key & (p.c.page - 1)) * D);
       }
     };
-    // 16 codes -> two 16-byte chunks; neighbouring 64-dim blocks store them in
-    // opposite order so that the eight lanes of a store pass hit all banks
-    auto store = [&](const uint4 (&x)[NC], uint8_t *tile) {
-      const int e0 = (ch >> 2) & 1;
+    auto load_v = [&](int id) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int key = key0 + i * STEP;
-        uint4 o[2];
-        const uint32_t w[4] = {x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u,
-                               x[i].w ^ 0x80808080u};
-        o[0] = make_uint4(h2_codes(__byte_perm(w[0], 0x64646464u, 0x4140)),
-                          h2_codes(__byte_perm(w[0], 0x64646464u, 0x4342)),
-                          h2_codes(__byte_perm(w[1], 0x64646464u, 0x4140)),
-                          h2_codes(__byte_perm(w[1], 0x64646464u, 0x4342)));
-        o[1] = make_uint4(h2_codes(__byte_perm(w[2], 0x64646464u, 0x4140)),
-                          h2_codes(__byte_perm(w[2], 0x64646464u, 0x4342)),
-                          h2_codes(__byte_perm(w[3], 0x64646464u, 0x4140)),
-                          h2_codes(__byte_perm(w[3], 0x64646464u, 0x4342)));
-        uint8_t *base = tile + (ch >> 2) * KP_BLOCK;
-        const int c = 2 * (ch & 3);
-        *reinterpret_cast<uint4 *>(base + kp_sw(key, c + e0)) = e0 ? o[1] : o[0];
-        *reinterpret_cast<uint4 *>(base + kp_sw(key, c + 1 - e0)) = e0 ? o[0] : o[1];
+      for (int i = 0; i < VN; ++i) {
+        const int key = vkey + i * VSTEP;
+        const int pg = __shfl_sync(0xffffffffu, id, key >> 4);
+        vr[i] = ldg_nc_v4(vbase + pg * pool_step + (key & (p.c.page - 1)) * D);
       }
+    };
+    // 16 codes of chunk ch -> two 16-byte chunks of row r; neighbouring 64-dim
+    // blocks store them in opposite order so that the eight lanes of a store pass
+    // hit all banks
+    auto store = [&](const uint4 &x, uint8_t *tile, int block, int r, int ch) {
+      const int e0 = (ch >> 2) & 1, c = 2 * (ch & 3);
+      const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u,
+                             x.w ^ 0x80808080u};
+      uint4 o[2];
+      o[0] = make_uint4(h2_codes(__byte_perm(w[0], 0x64646464u, 0x4140)),
+                        h2_codes(__byte_perm(w[0], 0x64646464u, 0x4342)),
+                        h2_codes(__byte_perm(w[1], 0x64646464u, 0x4140)),
+                        h2_codes(__byte_perm(w[1], 0x64646464u, 0x4342)));
+      o[1] = make_uint4(h2_codes(__byte_perm(w[2], 0x64646464u, 0x4140)),
+                        h2_codes(__byte_perm(w[2], 0x64646464u, 0x4342)),
+                        h2_codes(__byte_perm(w[3], 0x64646464u, 0x4140)),
+                        h2_codes(__byte_perm(w[3], 0x64646464u, 0x4342)));
+      uint8_t *base = tile + (ch >> 2) * block;
+      *reinterpret_cast<uint4 *>(base + kp_sw(r, c + e0)) = e0 ? o[1] : o[0];
+      *reinterpret_cast<uint4 *>(base + kp_sw(r, c + 1 - e0)) = e0 ? o[0] : o[1];
     };
     auto publish = [&](uint64_t *full) {
       tc::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(full);
+      if (lane == 0) kp_arrive_leader(full);
     };
-    // K runs a tile ahead of V: S of the next tile is issued before O of this one
     auto wait = [&](uint64_t *m, int n) {  // n-th completion of a barrier (n < 0: none needed)
       if (n >= 0 && !tc::mbar_wait(m, (uint32_t)(n & 1), abort, KP_WAIT_NS)) s_abort = 1;
       return !__any_sync(0xffffffffu, *abort != 0);
     };
+    const bool has_v = D > 64 || rank == 0;
     int id_v = group_page(t0), id_k = group_page(t0 + 1);  // of tiles n + 1 and n + 2
-    load(kr, kbase, id_v);
-    load(vr, vbase, id_v);
-    bool ok = true;
-    for (int n = -1; n < t1 - t0; ++n) {  // K of tile n + 1, V of tile n
+    load_k(id_v);
+    if (has_v) load_v(id_v);
+    for (int n = -1; n < n_tiles; ++n) {  // K of tile n + 1, V of tile n
       const int id_next = group_page(t0 + n + 3);
-      if (n + 1 < t1 - t0) {
-        const int st = (n + 1) % ST;
-        ok = wait(&bar.k_empty[st], (n + 1) / ST - 1);
-        if (!ok) break;
-        store(kr, smem + H::K_OFF + st * H::TILE);
+      if (n + 1 < n_tiles) {
+        const int st = (n + 1) % KP_STAGES;
+        if (!wait(&bar.k_empty[st], (n + 1) / KP_STAGES - 1)) break;
+        uint8_t *tile = smem + H::K_OFF + st * H::K_HALF;
+#pragma unroll
+        for (int i = 0; i < KN; ++i) store(kr[i], tile, H::K_BLOCK, kkey + i * KSTEP, kch);
         publish(&bar.k_full[st]);
-        load(kr, kbase, id_k);
+        load_k(id_k);
       }
       if (n >= 0) {
-        const int st = n % ST;
-        ok = wait(&bar.v_empty[st], n / ST - 1);
-        if (!ok) break;
-        store(vr, smem + H::V_OFF + st * H::TILE);
+        const int st = n % KP_STAGES;
+        if (!wait(&bar.v_empty[st], n / KP_STAGES - 1)) break;
+        if (has_v) {
+          uint8_t *tile = smem + H::V_OFF + st * H::V_HALF;
+#pragma unroll
+          for (int i = 0; i < VN; ++i) store(vr[i], tile, KP_BLOCK, vkey + i * VSTEP, vch);
+        }
         publish(&bar.v_full[st]);
-        load(vr, vbase, id_v);
+        if (has_v) load_v(id_v);
       }
       id_v = id_k;
       id_k = id_next;
     }
   } else {
-    // ================================================== softmax, a thread per row
-    kp_regs_inc<H::R_SOFT>();
-    const int tile = wg - 1 - H::CONV_WG;
-    const int r = tile * 128 + (tid & 127), R = r_base + r;
+    // ============================== softmax, a thread per row and 64 keys of a tile
+    kp_regs_inc<KP_R_SOFT>();
+    const int hf = wg - 2, r = tid & 127, R = r_base + r;
     const int vis = R < rows ? sp.visible(p.row_of(R)) : 0;
     const float fac = s_fac[r];
     const uint32_t trow = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
-    const bool one = t1 - t0 == 1;
+    const bool one = n_tiles == 1;
     const float shift = one ? KP_SHIFT_ONE : KP_SHIFT;
     float m = -INFINITY, l = 0.f, lvref = KP_NO_SCALE;
     // scales of the 16-key group lane % 8 of a tile: K scale (-1: no such page)
@@ -388,9 +438,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
     float ks_n, vs_n;
     group_scales(group_page(t0), ks_n, vs_n);
     int id_n = group_page(t0 + 1);
+    // After a wait has given up, the tiles are gone through without their work:
+    // the two warpgroups meet in every tile.
     bool ok = true;
-    for (int t = t0; t < t1; ++t) {
-      const int n = t - t0, w = n * NT + tile, slot = w & 1;
+    for (int n = 0; n < n_tiles; ++n) {
+      const int t = t0 + n, slot = n & 1;
       const float ks_l = ks_n, lv_l = vs_n > 0.f ? log2f(vs_n) : KP_NO_SCALE;
       group_scales(id_n, ks_n, vs_n);
       id_n = group_page(t + 2);
@@ -402,30 +454,31 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
       const float lv_new = one ? lv_top : fmaxf(lvref, ceilf(lv_top));
       const uint32_t missing = __ballot_sync(0xffffffffu, ks_l < 0.f) & 0xFFu;
 
-      if (!tc::mbar_wait(&bar.s_full[slot], (uint32_t)((w >> 1) & 1), abort, KP_WAIT_NS))
+      if (ok && !tc::mbar_wait(&bar.s_full[slot], (uint32_t)((n >> 1) & 1), abort, KP_WAIT_NS))
         s_abort = 1;
       ok = !__any_sync(0xffffffffu, *abort != 0);
-      if (!ok) break;
       tc::tc_fence_after();
-      uint32_t s[4][32];
+      uint32_t s[2][32];
+      if (ok) {
+        tc::tmem_ld32(trow + slot * 128 + hf * 64, s[0]);
+        tc::tmem_ld32(trow + slot * 128 + hf * 64 + 32, s[1]);
+        tc::tmem_ld_wait();
+      }
+      const int lim = vis - t * KP_KT - hf * 64;  // visible keys of these 64
+      if (lim < 64 || missing) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) tc::tmem_ld32(trow + slot * 128 + q * 32, s[q]);
-      tc::tmem_ld_wait();
-      const int lim = vis - t * KP_KT;  // visible keys of this tile
-      if (lim < KP_KT || missing) {
-#pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          const bool gone = (missing >> g) & 1;
+        for (int g = 0; g < 4; ++g) {
+          const bool gone = (missing >> (hf * 4 + g)) & 1;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (gone || g * 16 + j >= lim) s[g >> 1][(g & 1) * 16 + j] = 0xFF800000u;
         }
       }
-      float f[8];
+      float f[4];
       float top = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        const float ks = __shfl_sync(0xffffffffu, ks_l, g);
+      for (int g = 0; g < 4; ++g) {
+        const float ks = __shfl_sync(0xffffffffu, ks_l, hf * 4 + g);
         // scale 0: every code of the page is 0 (1 keeps -inf * 0 out)
         f[g] = fac * (ks > 0.f ? ks : 1.f);
         const uint32_t *v = s[g >> 1] + (g & 1) * 16;
@@ -435,37 +488,43 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
         x1 = kp_max3(__float_as_uint(x1), v[14], v[15]);
         top = fmaxf(top, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * f[g]);
       }
+      // the row's other half; both have S in registers from here on
+      s_half[slot][hf][r] = top;
+      tc::tc_fence_before();
+      kp_soft_sync();
+      tc::tc_fence_after();
+      top = fmaxf(top, s_half[slot][hf ^ 1][r]);
       const bool move = top > m + KP_MOVE;
       const float to = move ? top : m;
-      const float alpha = move ? kv8_ex2(m - to) : 1.f;
+      const float alpha = move ? kp_ex2(m - to) : 1.f;
       m = to;
       l *= alpha;
-      if (n > 0 && (lv_new > lvref || __any_sync(0xffffffffu, move))) {  // rescale O
-        if (!tc::mbar_wait(&bar.o_done[tile], (uint32_t)((n - 1) & 1), abort, KP_WAIT_NS))
-          s_abort = 1;
+      if (ok && n > 0 && (lv_new > lvref || __any_sync(0xffffffffu, move))) {
+        // rescale this thread's half of the row's O
+        if (!tc::mbar_wait(&bar.o_done, (uint32_t)((n - 1) & 1), abort, KP_WAIT_NS)) s_abort = 1;
         ok = !__any_sync(0xffffffffu, *abort != 0);
-        if (!ok) break;
         tc::tc_fence_after();
-        const float a = alpha * kv8_ex2(lvref - lv_new);
+        const float a = alpha * kp_ex2(lvref - lv_new);
+        if (ok) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t v[32];
-          tc::tmem_ld32(trow + 256 + tile * D + c0, v);
-          tc::tmem_ld_wait();
+          for (int c0 = 0; c0 < D / 2; c0 += 32) {
+            uint32_t v[32];
+            tc::tmem_ld32(trow + 256 + hf * (D / 2) + c0, v);
+            tc::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
-          kp_tmem_st32(trow + 256 + tile * D + c0, v);
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
+            kp_tmem_st32(trow + 256 + hf * (D / 2) + c0, v);
+          }
+          kp_tmem_st_wait();
         }
-        kp_tmem_st_wait();
       }
       lvref = lv_new;
       const float sub = shift - (m == -INFINITY ? 0.f : m);
       // Groups of 16: the arguments of the next one are formed before this one's
-      // exponentials are used, so that a warp alone on its scheduler does not
-      // wait for each.
-      float x[2][16], cg[8];
+      // exponentials are used, so that a warp does not wait for each.
+      float x[2][16], cg[4];
       auto arguments = [&](int g) {
-        const float lv = __shfl_sync(0xffffffffu, lv_l, g);
+        const float lv = __shfl_sync(0xffffffffu, lv_l, hf * 4 + g);
         cg[g] = lv > KP_NO_SCALE ? lv - lvref : 0.f;
         const f2 ff = f2_make(f[g], f[g]), cc = f2_make(sub + cg[g], sub + cg[g]);
 #pragma unroll
@@ -476,13 +535,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
         }
       };
       arguments(0);
-      uint32_t pk[2][32];
+      uint32_t pk[32];
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
+      for (int g = 0; g < 4; ++g) {
         float e[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) e[j] = kp_ex2(x[g & 1][j]);
-        if (g < 7) arguments(g + 1);
+        if (g < 3) arguments(g + 1);
         f2 sum0 = f2_make(e[0], e[1]), sum1 = f2_make(e[2], e[3]);
 #pragma unroll
         for (int j = 4; j < 16; j += 4) {
@@ -492,38 +551,43 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
         float s0, s1;
         f2_split(f2_add(sum0, sum1), s0, s1);
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) pk[g >> 2][(g & 3) * 8 + (j >> 1)] = pack_h2(e[j], e[j + 1]);
+        for (int j = 0; j < 16; j += 2) pk[g * 8 + (j >> 1)] = pack_h2(e[j], e[j + 1]);
         l = fmaf(s0 + s1, kp_ex2(fminf(-cg[g], 126.f)), l);
-        if (g == 3) kp_tmem_st32(trow + slot * 128, pk[0]);
       }
-      kp_tmem_st32(trow + slot * 128 + 32, pk[1]);
-      kp_tmem_st_wait();
+      if (ok) {
+        kp_tmem_st32(trow + slot * 128 + hf * 32, pk);
+        kp_tmem_st_wait();
+      }
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&bar.p_full[slot]);
+      if (ok && lane == 0) kp_arrive_leader(&bar.p_full[slot]);
     }
-    // ---- O of this tile's last product
-    if (ok && t1 > t0) {
-      if (!tc::mbar_wait(&bar.o_last[tile], 0, abort, KP_WAIT_NS)) s_abort = 1;
+    // ---- the row's l, and its O after the last product
+    s_half[n_tiles & 1][hf][r] = l;
+    kp_soft_sync();
+    l = s_half[n_tiles & 1][0][r] + s_half[n_tiles & 1][1][r];
+    if (ok && n_tiles > 0) {
+      if (!tc::mbar_wait(&bar.o_last, 0, abort, KP_WAIT_NS)) s_abort = 1;
       ok = !__any_sync(0xffffffffu, *abort != 0);
       tc::tc_fence_after();
     }
     if (ok) {
-      const float v = kv8_ex2(lvref);
-      const int i = p.row_of(R), hr = R - i * p.rep;
+      const float v = kp_ex2(lvref);
+      const int i = p.row_of(R), hr = R - i * p.rep, r_pair = rank * 128 + r;
       const size_t row = ((size_t)b * p.Hq + h * p.rep + hr) * p.L + i;
       const bool live = R < rows;
-      if (p.splits > 1) {
-        if (live) p.ml_part[tile_id * ROWS + r] = make_float2(m - shift, l);
-      } else if (live && p.lse) {
-        p.lse[row] = l == 0.f ? -INFINITY : (m - shift + log2f(l)) * 0.69314718055994531f;
+      if (live && hf == 0) {
+        if (p.splits > 1)
+          p.ml_part[tile_id * KP_ROWS + r_pair] = make_float2(m - shift, l);
+        else if (p.lse)
+          p.lse[row] = l == 0.f ? -INFINITY : (m - shift + log2f(l)) * 0.69314718055994531f;
       }
       const float inv = p.splits > 1 ? v : l == 0.f ? 0.f : v / l;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
+      for (int c0 = hf * (D / 2); c0 < (hf + 1) * (D / 2); c0 += 32) {
         uint32_t x[32];
-        if (t1 > t0) {
-          tc::tmem_ld32(trow + 256 + tile * D + c0, x);
+        if (n_tiles > 0) {
+          tc::tmem_ld32(trow + 256 + c0, x);
           tc::tmem_ld_wait();
         } else {
 #pragma unroll
@@ -535,8 +599,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
         __syncwarp();
         if (!live) {
         } else if (p.splits > 1) {
-          if (t1 > t0) {
-            float4 *d4 = reinterpret_cast<float4 *>(p.o_part + (tile_id * ROWS + r) * D + c0);
+          if (n_tiles > 0) {
+            float4 *d4 = reinterpret_cast<float4 *>(p.o_part + (tile_id * KP_ROWS + r_pair) * D + c0);
 #pragma unroll
             for (int q = 0; q < 8; ++q)
               d4[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
@@ -549,14 +613,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prefill_kernel(Kv8AttnParam
                                pack_bf2(y[8 * q + 4], y[8 * q + 5]),
                                pack_bf2(y[8 * q + 6], y[8 * q + 7]));
         }
+        __syncwarp();
       }
     }
   }
   tc::tc_fence_before();
   __syncthreads();
-  tc::tc_fence_after();
   if (tid == 0 && *abort) flag_status(p.status, VB_STATUS_TIMEOUT);
-  if (warp == 0) tc::tmem_dealloc(tmem, 512);
+  kp_cluster_sync();  // no product reads the other CTA's operands any more
+  tc::tc_fence_after();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
 }
 
 template <int D>
@@ -577,14 +645,14 @@ int kp_launch(const Kv8AttnParams &p, cudaStream_t s) {
       return set_error(VB_ERR_CUDA, "kv8_prefill_kernel attributes: %s", cudaGetErrorString(e));
     ready = true;
   }
-  vb_launch(kv8_prefill_kernel<D>, dim3(p.row_tiles * p.splits, p.c.kv_heads, p.c.batch),
-            dim3(KP_THREADS), H::SMEM, s, true, p);
+  vb_launch(kv8_prefill_kernel<D>, dim3(2 * p.row_tiles * p.splits, p.c.kv_heads, p.c.batch),
+            dim3(KP_THREADS), H::SMEM, s, false, p);
   return check_launch("kv8_prefill_kernel");
 }
 
 }  // namespace
 
-int kv8_prefill_rows(int dim) { return dim == 256 ? KpShape<256>::NT * 128 : 256; }
+int kv8_prefill_rows() { return KP_ROWS; }
 
 int kv8_prefill_launch(const Kv8AttnParams &p, cudaStream_t s) {
   switch (p.c.dim) {
