@@ -10,17 +10,21 @@ namespace vb {
 // the ratio of two scales finite in float32 (values below 2^-41 read as 0).
 constexpr float KV8_MIN_SCALE = 9.094947017729282e-13f;  // 2^-40
 
-// Pool page `idx` of a sequence's table, or -1 (flagged) when the table is too
-// short or names a page outside the pool.
+// Entry `idx` of a sequence's page table (-1 past its end). Looking at the value
+// is left to kv8_page_ok, so that a prefetch does not wait for the load.
+__device__ __forceinline__ int kv8_page_load(const int32_t *table, int max_pages, int idx) {
+  return idx >= 0 && idx < max_pages ? __ldg(table + idx) : -1;
+}
+// The pool page, or -1 (flagged) when the table is too short or names a page
+// outside the pool.
+__device__ __forceinline__ int kv8_page_ok(int id, int pages, int32_t *status) {
+  if ((unsigned)id < (unsigned)pages) return id;
+  flag_status(status, VB_STATUS_BOUNDS);
+  return -1;
+}
 __device__ __forceinline__ int kv8_page(const int32_t *table, int max_pages, int pages, int idx,
                                         int32_t *status) {
-  int id = -1;
-  if (idx >= 0 && idx < max_pages) id = table[idx];
-  if ((unsigned)id >= (unsigned)pages) {
-    flag_status(status, VB_STATUS_BOUNDS);
-    id = -1;
-  }
-  return id;
+  return kv8_page_ok(kv8_page_load(table, max_pages, idx), pages, status);
 }
 
 // Rows of one sequence in this call: counts[b] clipped to [0, n], or n.

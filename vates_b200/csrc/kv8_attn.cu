@@ -260,39 +260,44 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
     const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + ch * 16;
     const int8_t *vbase = p.c.v_codes + (size_t)h * p.c.page * D + ch * 16;
 
-    // Page of the 16-key group lane % NG of a tile; -1: none (past the last key,
-    // or flagged). Such rows read page 0 and get no weight.
-    auto group_page = [&](int t) {
+    // Table entry of the 16-key group lane % NG of a tile (-1: past the last key).
+    // Rows without a page read page 0 and get no weight.
+    auto group_entry = [&](int t) {
       const int key = t * KT + (lane % NG) * 16;
-      return t < t1 && key < kend
-                 ? kv8_page(table, p.c.max_pages, p.c.pages, key >> p.shift, p.status) : -1;
+      return t < t1 && key < kend ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : -1;
     };
     // K scale of the group (-1 masks it) and V scale
-    auto group_scales = [&](int id, float &ks, float &vs) {
-      ks = id >= 0 ? __ldg(p.c.k_scales + (size_t)id * H + h) : -1.f;
-      vs = id >= 0 ? __ldg(p.c.v_scales + (size_t)id * H + h) : 0.f;
+    auto group_scales = [&](int entry, float &ks, float &vs) {
+      const bool there = (unsigned)entry < (unsigned)p.c.pages;
+      ks = there ? __ldg(p.c.k_scales + (size_t)entry * H + h) : -1.f;
+      vs = there ? __ldg(p.c.v_scales + (size_t)entry * H + h) : 0.f;
     };
-    auto issue = [&](int t, int stage, int id) {
+    auto issue = [&](int t, int stage, int entry) {
+      int id = entry;
+      if ((unsigned)entry >= (unsigned)p.c.pages) {
+        if (t * KT + (lane % NG) * 16 < kend) flag_status(p.status, VB_STATUS_BOUNDS);
+        id = 0;
+      }
       uint8_t *dst = smem + stage * (2 * KA_TILE) + copy_at;
       const int in_page = (t * KT) & (p.c.page - 1);  // 0 unless a page is longer than a tile
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const int kl = key0 + i * STEP;
-        const uint32_t pg = (uint32_t)max(0, __shfl_sync(0xffffffffu, id, kl >> 4));
+        const uint32_t pg = (uint32_t)__shfl_sync(0xffffffffu, id, kl >> 4);
         const unsigned long long at = (unsigned long long)pg * pool_step +
                                       (uint32_t)((in_page + (kl & (p.c.page - 1))) * D);
         cp_async16(dst + i * STEP * D, kbase + at);
         cp_async16(dst + KA_TILE + i * STEP * D, vbase + at);
       }
     };
-    // pages of the tiles t + 1 (id1) and t + 2 (id2) at the start of tile t
-    int id1 = group_page(t0);
+    // entries of the tiles t + 1 (id1) and t + 2 (id2) at the start of tile t
+    int id1 = group_entry(t0);
     float ks_l, vs_l;
     group_scales(id1, ks_l, vs_l);
     issue(t0, 0, id1);
     cp_async_commit();
-    id1 = group_page(t0 + 1);
-    int id2 = group_page(t0 + 2);
+    id1 = group_entry(t0 + 1);
+    int id2 = group_entry(t0 + 2);
     if (tid < 2) s_move[tid] = 0;
 
     // ---- queries, in the order of the B fragments: D / 8 lanes per row
@@ -363,7 +368,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
       float ks_n, vs_n;  // of tile t + 1
       group_scales(id1, ks_n, vs_n);
       id1 = id2;
-      id2 = group_page(t + 3);
+      id2 = group_entry(t + 3);
       const uint8_t *st = smem + stage * (2 * KA_TILE);
       stage ^= 1;
 

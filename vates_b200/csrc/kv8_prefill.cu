@@ -19,12 +19,13 @@
 //   * one thread of the pair issues S = Q K^T of the next key tile before
 //     O += P V of the current one, so the tensor cores work while the softmax
 //     runs; two S slots alternate;
-//   * two softmax warpgroups per CTA, a thread per row and 64 keys (a row's two
-//     threads exchange their maxima in shared memory): the running maximum only
-//     moves when it grows by more than 2^4 (then O and l are rescaled), and
-//     P = 2^(z - m) s_V / v goes over S in TMEM as the f16 A operand of the second
-//     product. v is a power of two at least every V scale so far. l is summed in
-//     float32 from the unrounded weights.
+//   * two softmax warpgroups per CTA, a thread per row, take the key tiles in
+//     turn: one's exponentials run while the other waits for its products. What a
+//     tile needs of the one before it is the running maximum, which is handed
+//     over before the exponentials. It only moves when it grows by more than 2^4
+//     (then O is rescaled), and P = 2^(z - m) s_V / v goes over S in TMEM as the
+//     f16 A operand of the second product. v is a power of two at least every V
+//     scale so far. l is summed in float32 from the unrounded weights.
 // A wait names the n-th completion of a barrier by its parity alone, so when it
 // begins, completion n - 1 must have happened and n + 1 must not: S of a tile
 // waits for O of the last tile in its slot, and the last O and the end have
@@ -66,7 +67,7 @@ struct KpShape {
   static constexpr int SMEM = V_OFF + KP_STAGES * V_HALF + 1024;
 };
 // Registers per thread of the four warpgroups; 128 at launch.
-constexpr int KP_R_MMA = 40, KP_R_CONV = 104, KP_R_SOFT = 184;
+constexpr int KP_R_MMA = 64, KP_R_CONV = 144, KP_R_SOFT = 152;
 static_assert(KP_R_MMA + KP_R_CONV + 2 * KP_R_SOFT == 4 * 128, "register shares");
 
 // Byte offset of 16-byte chunk c of row r in a 128-row x 64-column block.
@@ -88,6 +89,20 @@ __host__ __device__ constexpr uint32_t kp_idesc(int N, bool b_mn) {  // f16 x f1
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(256 >> 4) << 24);
 }
+// The order of volatile statements is kept, so a group's exponentials are issued
+// back to back.
+__device__ __forceinline__ float kp_ex2(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float kp_max3(uint32_t a, uint32_t b, uint32_t c) {
+  float r;
+  asm volatile("max.f32 %0, %1, %2, %3;"
+      : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return r;
+}
+
 // The pair's products, issued by one thread of CTA 0: rows 0-127 of A and D are
 // CTA 0's, 128-255 CTA 1's; each holds half of B's N. The whole warp comes here
 // (its values are then uniform); `one` is true in the lane that issues.
@@ -136,8 +151,17 @@ __device__ __forceinline__ void kp_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The 256 softmax threads of a CTA.
-__device__ __forceinline__ void kp_soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// The 256 softmax threads of a CTA meet; one half of them hands over to the other
+// (`from`: the warpgroup that arrives).
+__device__ __forceinline__ void kp_soft_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
+__device__ __forceinline__ void kp_hand_over(int from) {
+  asm volatile("bar.arrive %0, 256;" ::"r"(1 + from) : "memory");
+}
+__device__ __forceinline__ void kp_take_over(int from) {
+  asm volatile("bar.sync %0, 256;" ::"r"(1 + from) : "memory");
+}
+// 2^(a - b), 1 where both are the same (infinities too).
+__device__ __forceinline__ float kp_ratio(float a, float b) { return a == b ? 1.f : kp_ex2(a - b); }
 __device__ __forceinline__ void kp_tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
@@ -150,6 +174,15 @@ __device__ __forceinline__ void kp_tmem_st32(uint32_t taddr, const uint32_t (&r)
       "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void kp_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void kp_tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -160,20 +193,6 @@ __device__ __forceinline__ void kp_regs_dec() {
 template <int N>
 __device__ __forceinline__ void kp_regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// The order of volatile statements is kept, so a group's exponentials are issued
-// back to back.
-__device__ __forceinline__ float kp_ex2(float x) {
-  float y;
-  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float kp_max3(uint32_t a, uint32_t b, uint32_t c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;"
-      : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
-  return r;
 }
 
 struct KpBarriers {
@@ -190,7 +209,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   __shared__ __align__(8) KpBarriers bar;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  __shared__ float s_fac[128], s_half[2][2][128];
+  __shared__ float s_fac[128], s_m[128], s_l[2][128], s_lv[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
   pdl_launch_dependents();
   pdl_wait();
@@ -219,7 +238,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       tc::mbar_init(&bar.k_empty[i], 1);
       tc::mbar_init(&bar.v_empty[i], 1);
       tc::mbar_init(&bar.s_full[i], 1);
-      tc::mbar_init(&bar.p_full[i], 2 * 8);   // softmax warps of both CTAs
+      tc::mbar_init(&bar.p_full[i], 2 * 4);   // softmax warps of a tile, both CTAs
     }
     tc::mbar_init(&bar.o_done, 1);
     tc::mbar_init(&bar.o_last, 1);
@@ -323,19 +342,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     __syncwarp();
   } else if (wg == 1) {
     // ================================================== converters
-    kp_regs_dec<KP_R_CONV>();
+    kp_regs_inc<KP_R_CONV>();
     const int ctid = tid - 128;
     // K: 64 keys of all dims; V: 128 keys of half of the dims; 16 codes at a time
     constexpr int KC = D / 16, KSTEP = 128 / KC, KN = 64 / KSTEP;
     constexpr int VC = H::VD / 16, VSTEP = 128 / VC, VN = 128 / VSTEP;
     const int kch = ctid % KC, kkey = ctid / KC, vch = ctid % VC, vkey = ctid / VC;
     uint4 kr[KN], vr[VN];
-    // pool page of the 16-key group lane % 8 of tile t; rows without a page (past
-    // the last key, or flagged) read page 0: their weights are 0
-    auto group_page = [&](int t) {
+    // table entry of the 16-key group lane % 8 of tile t, and later its pool page;
+    // rows without one (past the last key, or flagged) read page 0: their weights
+    // are 0
+    auto group_entry = [&](int t) {
       const int key = t * KP_KT + (lane & 7) * 16;
-      return t < t1 && key < kend
-                 ? max(0, kv8_page(table, p.c.max_pages, p.c.pages, key >> p.shift, p.status)) : 0;
+      return t < t1 && key < kend ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : 0;
+    };
+    auto group_page = [&](int entry) {
+      return max(0, kv8_page_ok(entry, p.c.pages, p.status));
     };
     const size_t pool_step = (size_t)p.c.kv_heads * p.c.page * D;
     const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + kch * 16;
@@ -386,11 +408,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       return !__any_sync(0xffffffffu, *abort != 0);
     };
     const bool has_v = D > 64 || rank == 0;
-    int id_v = group_page(t0), id_k = group_page(t0 + 1);  // of tiles n + 1 and n + 2
+    // of tiles n + 1 and n + 2
+    int id_v = group_page(group_entry(t0)), id_k = group_page(group_entry(t0 + 1));
     load_k(id_v);
     if (has_v) load_v(id_v);
     for (int n = -1; n < n_tiles; ++n) {  // K of tile n + 1, V of tile n
-      const int id_next = group_page(t0 + n + 3);
+      const int entry = group_entry(t0 + n + 3);
       if (n + 1 < n_tiles) {
         const int st = (n + 1) % KP_STAGES;
         if (!wait(&bar.k_empty[st], (n + 1) / KP_STAGES - 1)) break;
@@ -398,8 +421,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < KN; ++i) store(kr[i], tile, H::K_BLOCK, kkey + i * KSTEP, kch);
         publish(&bar.k_full[st]);
-        load_k(id_k);
       }
+      const int id_next = group_page(entry);  // before rows are asked for: it would wait for them
+      if (n + 1 < n_tiles) load_k(id_k);
       if (n >= 0) {
         const int st = n % KP_STAGES;
         if (!wait(&bar.v_empty[st], n / KP_STAGES - 1)) break;
@@ -415,9 +439,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       id_k = id_next;
     }
   } else {
-    // ============================== softmax, a thread per row and 64 keys of a tile
+    // ================================================== softmax, a thread per row
     kp_regs_inc<KP_R_SOFT>();
-    const int hf = wg - 2, r = tid & 127, R = r_base + r;
+    const int hf = wg - 2, r = tid & 127, R = r_base + r;  // tiles hf, hf + 2, ...; S slot hf
     const int vis = R < rows ? sp.visible(p.row_of(R)) : 0;
     const float fac = s_fac[r];
     const uint32_t trow = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
@@ -425,147 +449,159 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     const float shift = one ? KP_SHIFT_ONE : KP_SHIFT;
     float m = -INFINITY, l = 0.f, lvref = KP_NO_SCALE;
     // scales of the 16-key group lane % 8 of a tile: K scale (-1: no such page)
-    // and log2 of the V scale, loaded a tile ahead, page numbers two ahead
-    auto group_page = [&](int t) {
+    // and log2 of the V scale, loaded two tiles ahead, page numbers four
+    auto group_entry = [&](int t) {
       const int key = t * KP_KT + (lane & 7) * 16;
-      return t < t1 && key < kend
-                 ? kv8_page(table, p.c.max_pages, p.c.pages, key >> p.shift, nullptr) : -1;
+      return t < t1 && key < kend ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : -1;
     };
-    auto group_scales = [&](int id, float &ks, float &vs) {
-      ks = id >= 0 ? __ldg(p.c.k_scales + (size_t)id * p.c.kv_heads + h) : -1.f;
-      vs = id >= 0 ? __ldg(p.c.v_scales + (size_t)id * p.c.kv_heads + h) : 0.f;
+    auto group_scales = [&](int entry, float &ks, float &vs) {
+      const bool there = (unsigned)entry < (unsigned)p.c.pages;
+      ks = there ? __ldg(p.c.k_scales + (size_t)entry * p.c.kv_heads + h) : -1.f;
+      vs = there ? __ldg(p.c.v_scales + (size_t)entry * p.c.kv_heads + h) : 0.f;
     };
     float ks_n, vs_n;
-    group_scales(group_page(t0), ks_n, vs_n);
-    int id_n = group_page(t0 + 1);
-    // After a wait has given up, the tiles are gone through without their work:
-    // the two warpgroups meet in every tile.
+    group_scales(group_entry(t0 + hf), ks_n, vs_n);
+    int entry_n = group_entry(t0 + hf + 2);
+    // After a wait has given up, the tiles are gone through with what TMEM holds
+    // and without further waits: the warpgroups hand over to each other in every
+    // tile.
     bool ok = true;
-    for (int n = 0; n < n_tiles; ++n) {
-      const int t = t0 + n, slot = n & 1;
+    for (int n = hf; n < n_tiles; n += 2) {
+      const int t = t0 + n;
       const float ks_l = ks_n, lv_l = vs_n > 0.f ? log2f(vs_n) : KP_NO_SCALE;
-      group_scales(id_n, ks_n, vs_n);
-      id_n = group_page(t + 2);
-      // v: a power of two at least every V scale so far
+      group_scales(entry_n, ks_n, vs_n);
+      entry_n = group_entry(t + 4);
       float lv_top = lv_l;
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1)
         lv_top = fmaxf(lv_top, __shfl_xor_sync(0xffffffffu, lv_top, o));
-      const float lv_new = one ? lv_top : fmaxf(lvref, ceilf(lv_top));
       const uint32_t missing = __ballot_sync(0xffffffffu, ks_l < 0.f) & 0xFFu;
 
-      if (ok && !tc::mbar_wait(&bar.s_full[slot], (uint32_t)((n >> 1) & 1), abort, KP_WAIT_NS))
+      if (ok && !tc::mbar_wait(&bar.s_full[hf], (uint32_t)((n >> 1) & 1), abort, KP_WAIT_NS))
         s_abort = 1;
       ok = !__any_sync(0xffffffffu, *abort != 0);
       tc::tc_fence_after();
-      uint32_t s[2][32];
-      if (ok) {
-        tc::tmem_ld32(trow + slot * 128 + hf * 64, s[0]);
-        tc::tmem_ld32(trow + slot * 128 + hf * 64 + 32, s[1]);
+      // S is read twice, 32 columns at a time, rather than kept in registers, in
+      // rolled loops: the roles' code together has to fit the instruction cache
+      const int lim = vis - t * KP_KT;  // visible keys of this tile
+      const bool masked = lim < KP_KT || missing;
+      auto mask = [&](uint32_t (&v)[32], int c) {  // columns 32 c .. of the tile
+        const int n = lim - 32 * c;
+        uint32_t keep = n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+        if ((missing >> (2 * c)) & 1) keep &= 0xFFFF0000u;
+        if ((missing >> (2 * c)) & 2) keep &= 0x0000FFFFu;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (!((keep >> j) & 1)) v[j] = 0xFF800000u;
+      };
+      // K factor of a 16-key group; scale 0: every code of the page is 0 (1 keeps
+      // -inf * 0 out)
+      auto factor = [&](int g) {
+        const float ks = __shfl_sync(0xffffffffu, ks_l, g);
+        return fac * (ks > 0.f ? ks : 1.f);
+      };
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tc::tmem_ld32(trow + hf * 128 + c * 32, v);
         tc::tmem_ld_wait();
-      }
-      const int lim = vis - t * KP_KT - hf * 64;  // visible keys of these 64
-      if (lim < 64 || missing) {
+        if (masked) mask(v, c);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const bool gone = (missing >> (hf * 4 + g)) & 1;
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (gone || g * 16 + j >= lim) s[g >> 1][(g & 1) * 16 + j] = 0xFF800000u;
+        for (int gg = 0; gg < 2; ++gg) {
+          const uint32_t *u = v + gg * 16;
+          float x0 = kp_max3(u[0], u[1], u[2]), x1 = kp_max3(u[3], u[4], u[5]);
+          float x2 = kp_max3(u[6], u[7], u[8]), x3 = kp_max3(u[9], u[10], u[11]);
+          x0 = kp_max3(__float_as_uint(x0), u[12], u[13]);
+          x1 = kp_max3(__float_as_uint(x1), u[14], u[15]);
+          top = fmaxf(top, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * factor(2 * c + gg));
         }
       }
-      float f[4];
-      float top = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float ks = __shfl_sync(0xffffffffu, ks_l, hf * 4 + g);
-        // scale 0: every code of the page is 0 (1 keeps -inf * 0 out)
-        f[g] = fac * (ks > 0.f ? ks : 1.f);
-        const uint32_t *v = s[g >> 1] + (g & 1) * 16;
-        float x0 = kp_max3(v[0], v[1], v[2]), x1 = kp_max3(v[3], v[4], v[5]);
-        float x2 = kp_max3(v[6], v[7], v[8]), x3 = kp_max3(v[9], v[10], v[11]);
-        x0 = kp_max3(__float_as_uint(x0), v[12], v[13]);
-        x1 = kp_max3(__float_as_uint(x1), v[14], v[15]);
-        top = fmaxf(top, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * f[g]);
+      // maximum and v after the tile before this one, and after this one
+      float m_prev = -INFINITY, lv_prev = KP_NO_SCALE;
+      if (n > 0) {
+        kp_take_over(hf ^ 1);
+        m_prev = s_m[r];
+        lv_prev = s_lv[hf ^ 1];
       }
-      // the row's other half; both have S in registers from here on
-      s_half[slot][hf][r] = top;
-      tc::tc_fence_before();
-      kp_soft_sync();
-      tc::tc_fence_after();
-      top = fmaxf(top, s_half[slot][hf ^ 1][r]);
-      const bool move = top > m + KP_MOVE;
-      const float to = move ? top : m;
-      const float alpha = move ? kp_ex2(m - to) : 1.f;
-      m = to;
-      l *= alpha;
-      if (ok && n > 0 && (lv_new > lvref || __any_sync(0xffffffffu, move))) {
-        // rescale this thread's half of the row's O
+      const bool move = top > m_prev + KP_MOVE;
+      const float m_new = move ? top : m_prev;
+      lvref = one ? lv_top : fmaxf(lv_prev, ceilf(lv_top));
+      s_m[r] = m_new;
+      if (r == 0) s_lv[hf] = lvref;
+      if (n + 1 < n_tiles) kp_hand_over(hf);
+      l *= kp_ratio(m, m_new);  // (the other warpgroup may have moved it too)
+      m = m_new;
+      if (ok && n > 0 && (lvref > lv_prev || __any_sync(0xffffffffu, move))) {  // rescale O
         if (!tc::mbar_wait(&bar.o_done, (uint32_t)((n - 1) & 1), abort, KP_WAIT_NS)) s_abort = 1;
         ok = !__any_sync(0xffffffffu, *abort != 0);
         tc::tc_fence_after();
-        const float a = alpha * kp_ex2(lvref - lv_new);
+        const float a = kp_ratio(m_prev, m_new) * kp_ex2(lv_prev - lvref);
         if (ok) {
 #pragma unroll 1
-          for (int c0 = 0; c0 < D / 2; c0 += 32) {
+          for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t v[32];
-            tc::tmem_ld32(trow + 256 + hf * (D / 2) + c0, v);
+            tc::tmem_ld32(trow + 256 + c0, v);
             tc::tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
-            kp_tmem_st32(trow + 256 + hf * (D / 2) + c0, v);
+            kp_tmem_st32(trow + 256 + c0, v);
           }
           kp_tmem_st_wait();
         }
       }
-      lvref = lv_new;
       const float sub = shift - (m == -INFINITY ? 0.f : m);
-      // Groups of 16: the arguments of the next one are formed before this one's
-      // exponentials are used, so that a warp does not wait for each.
-      float x[2][16], cg[4];
-      auto arguments = [&](int g) {
-        const float lv = __shfl_sync(0xffffffffu, lv_l, hf * 4 + g);
-        cg[g] = lv > KP_NO_SCALE ? lv - lvref : 0.f;
-        const f2 ff = f2_make(f[g], f[g]), cc = f2_make(sub + cg[g], sub + cg[g]);
+      // (P, 16 columns, only goes over columns that have been read)
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32], pk[16];
+        tc::tmem_ld32(trow + hf * 128 + c * 32, v);
+        tc::tmem_ld_wait();
+        if (masked) mask(v, c);
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const uint32_t *v = s[g >> 1] + (g & 1) * 16 + j;
-          f2_split(f2_fma(f2_make(__uint_as_float(v[0]), __uint_as_float(v[1])), ff, cc),
-                   x[g & 1][j], x[g & 1][j + 1]);
+        for (int gg = 0; gg < 2; ++gg) {
+          const int g = 2 * c + gg;
+          const float lv = __shfl_sync(0xffffffffu, lv_l, g), f = factor(g);
+          const float cg = lv > KP_NO_SCALE ? lv - lvref : 0.f;
+          const f2 ff = f2_make(f, f), cc = f2_make(sub + cg, sub + cg);
+          float e[16];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2)
+            f2_split(f2_fma(f2_make(__uint_as_float(v[gg * 16 + j]),
+                                    __uint_as_float(v[gg * 16 + j + 1])), ff, cc),
+                     e[j], e[j + 1]);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) e[j] = kp_ex2(e[j]);
+          f2 sum0 = f2_make(e[0], e[1]), sum1 = f2_make(e[2], e[3]);
+#pragma unroll
+          for (int j = 4; j < 16; j += 4) {
+            sum0 = f2_add(sum0, f2_make(e[j], e[j + 1]));
+            sum1 = f2_add(sum1, f2_make(e[j + 2], e[j + 3]));
+          }
+          float s0, s1;
+          f2_split(f2_add(sum0, sum1), s0, s1);
+          l = fmaf(s0 + s1, kp_ex2(fminf(-cg, 126.f)), l);
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) pk[gg * 8 + (j >> 1)] = pack_h2(e[j], e[j + 1]);
         }
-      };
-      arguments(0);
-      uint32_t pk[32];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float e[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) e[j] = kp_ex2(x[g & 1][j]);
-        if (g < 3) arguments(g + 1);
-        f2 sum0 = f2_make(e[0], e[1]), sum1 = f2_make(e[2], e[3]);
-#pragma unroll
-        for (int j = 4; j < 16; j += 4) {
-          sum0 = f2_add(sum0, f2_make(e[j], e[j + 1]));
-          sum1 = f2_add(sum1, f2_make(e[j + 2], e[j + 3]));
-        }
-        float s0, s1;
-        f2_split(f2_add(sum0, sum1), s0, s1);
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) pk[g * 8 + (j >> 1)] = pack_h2(e[j], e[j + 1]);
-        l = fmaf(s0 + s1, kp_ex2(fminf(-cg[g], 126.f)), l);
+        kp_tmem_st16(trow + hf * 128 + c * 16, pk);
       }
-      if (ok) {
-        kp_tmem_st32(trow + slot * 128 + hf * 32, pk);
-        kp_tmem_st_wait();
-      }
+      kp_tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();
-      if (ok && lane == 0) kp_arrive_leader(&bar.p_full[slot]);
+      if (ok && lane == 0) kp_arrive_leader(&bar.p_full[hf]);
     }
-    // ---- the row's l, and its O after the last product
-    s_half[n_tiles & 1][hf][r] = l;
+    // ---- the row's m, v and l after the last tile, and its O after the last product
     kp_soft_sync();
-    l = s_half[n_tiles & 1][0][r] + s_half[n_tiles & 1][1][r];
+    if (n_tiles > 0) {
+      const float m_end = s_m[r];
+      l *= kp_ratio(m, m_end);
+      m = m_end;
+      lvref = s_lv[(n_tiles - 1) & 1];
+    }
+    s_l[hf][r] = l;
+    kp_soft_sync();
+    l = s_l[0][r] + s_l[1][r];
     if (ok && n_tiles > 0) {
       if (!tc::mbar_wait(&bar.o_last, 0, abort, KP_WAIT_NS)) s_abort = 1;
       ok = !__any_sync(0xffffffffu, *abort != 0);
