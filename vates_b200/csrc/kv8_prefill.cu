@@ -62,6 +62,8 @@ struct KpShape {
   // all of V and the columns of O from 64 on are not used.
   static constexpr int VD = D == 256 ? 128 : 64;
   static constexpr int V_HALF = 128 * VD * 2;
+  // S slots in TMEM, 128 columns each, before the columns of O
+  static constexpr int SLOTS = D == 256 ? 2 : 3, O_COL = SLOTS * 128;
   static constexpr int K_OFF = Q_BYTES;
   static constexpr int V_OFF = K_OFF + KP_STAGES * K_HALF;
   static constexpr int SMEM = V_OFF + KP_STAGES * V_HALF + 1024;
@@ -196,7 +198,7 @@ __device__ __forceinline__ void kp_regs_inc() {
 }
 
 struct KpBarriers {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done, o_last, drain;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[3], p_full[3], o_done[3], o_last, drain;
 };
 
 template <int D>
@@ -232,15 +234,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
 
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < KP_STAGES; ++i) {
       tc::mbar_init(&bar.k_full[i], 2 * 4);   // converter warps of both CTAs
       tc::mbar_init(&bar.v_full[i], 2 * 4);
       tc::mbar_init(&bar.k_empty[i], 1);
       tc::mbar_init(&bar.v_empty[i], 1);
+    }
+    for (int i = 0; i < H::SLOTS; ++i) {
       tc::mbar_init(&bar.s_full[i], 1);
       tc::mbar_init(&bar.p_full[i], 2 * 4);   // softmax warps of a tile, both CTAs
+      tc::mbar_init(&bar.o_done[i], 1);
     }
-    tc::mbar_init(&bar.o_done, 1);
     tc::mbar_init(&bar.o_last, 1);
     tc::mbar_init(&bar.drain, 1);
     s_abort = 0;
@@ -285,6 +289,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   const uint32_t tmem = s_tmem;
   volatile int *abort = &s_abort;
   const uint32_t sbase = tc::smem_u32(smem);
+  // The warp waits for the n-th completion (from 0) of a barrier; false after a
+  // wait of this CTA has given up.
+  auto wait = [&](uint64_t *m, int n) {
+    const bool there = tc::mbar_wait(m, (uint32_t)(n & 1), abort, KP_WAIT_NS);
+    if (!there) s_abort = 1;
+    return __all_sync(0xffffffffu, there);
+  };
 
   if (wg == 0) {
     // ================================================== tensor-core issuer
@@ -296,41 +307,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       const uint64_t q_desc = tc::smem_desc_sw128(sbase);
       const uint64_t k_desc = tc::smem_desc_sw128(sbase + H::K_OFF);
       const uint64_t v_desc = kp_desc_mn(sbase + H::V_OFF);
-      auto wait = [&](uint64_t *m, int n) {  // n-th completion (from 0) of a barrier
-        if (!tc::mbar_wait(m, (uint32_t)(n & 1), abort, KP_WAIT_NS)) s_abort = 1;
-        return !__any_sync(0xffffffffu, *abort != 0);
-      };
       bool ok = true;
-      for (int w = 0; w <= n_tiles && ok; ++w) {
+      for (int w = 0; w < n_tiles + H::SLOTS - 1 && ok; ++w) {
         if (w < n_tiles) {  // S of tile w
-          const int st = w % KP_STAGES;
-          // the slot's P has been read: O of tile w - 2 is done
-          if (w >= 2) ok = wait(&bar.o_done, w - 2);
+          const int st = w % KP_STAGES, slot = w % H::SLOTS;
+          // the slot's P has been read: O of tile w - SLOTS is done
+          if (w >= H::SLOTS) ok = wait(&bar.o_done[slot], w / H::SLOTS - 1);
           ok = ok && wait(&bar.k_full[st], w / KP_STAGES);
           if (!ok) break;
           tc::tc_fence_after();
           const uint64_t kd = k_desc + st * (H::K_HALF >> 4);
-          const uint32_t d = tmem + (w & 1) * 128;
+          const uint32_t d = tmem + slot * 128;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             kp_mma_ss(one, d, q_desc + (((kk >> 2) * KP_BLOCK + (kk & 3) * 32) >> 4),
                       kd + (((kk >> 2) * H::K_BLOCK + (kk & 3) * 32) >> 4), ID_S,
                       kk > 0 ? 1u : 0u);
-          kp_commit(one, &bar.s_full[w & 1]);
+          kp_commit(one, &bar.s_full[slot]);
           kp_commit(one, &bar.k_empty[st]);
         }
-        if (w > 0) {  // O += P V of tile w - 1
-          const int v = w - 1, st = v % KP_STAGES;
-          ok = wait(&bar.v_full[st], v / KP_STAGES) && wait(&bar.p_full[v & 1], v >> 1);
+        const int v = w - (H::SLOTS - 1);
+        if (v >= 0) {  // O += P V of tile v
+          const int st = v % KP_STAGES, slot = v % H::SLOTS;
+          ok = wait(&bar.v_full[st], v / KP_STAGES) && wait(&bar.p_full[slot], v / H::SLOTS);
           if (!ok) break;
           tc::tc_fence_after();
           const uint64_t vd = v_desc + st * (H::V_HALF >> 4);
-          const uint32_t a = tmem + (v & 1) * 128;
+          const uint32_t a = tmem + slot * 128;
 #pragma unroll
           for (int kk = 0; kk < KP_KT / 16; ++kk)
-            kp_mma_ts(one, tmem + 256, a + kk * 8, vd + (kk * 2048 >> 4), ID_O,
+            kp_mma_ts(one, tmem + H::O_COL, a + kk * 8, vd + (kk * 2048 >> 4), ID_O,
                       kk > 0 ? 1u : (v > 0 ? 1u : 0u));
-          kp_commit(one, &bar.o_done);
+          kp_commit(one, &bar.o_done[slot]);
           if (v == n_tiles - 1) kp_commit(one, &bar.o_last);
           kp_commit(one, &bar.v_empty[st]);
         }
@@ -403,10 +411,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       __syncwarp();
       if (lane == 0) kp_arrive_leader(full);
     };
-    auto wait = [&](uint64_t *m, int n) {  // n-th completion of a barrier (n < 0: none needed)
-      if (n >= 0 && !tc::mbar_wait(m, (uint32_t)(n & 1), abort, KP_WAIT_NS)) s_abort = 1;
-      return !__any_sync(0xffffffffu, *abort != 0);
-    };
     const bool has_v = D > 64 || rank == 0;
     // of tiles n + 1 and n + 2
     int id_v = group_page(group_entry(t0)), id_k = group_page(group_entry(t0 + 1));
@@ -416,7 +420,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       const int entry = group_entry(t0 + n + 3);
       if (n + 1 < n_tiles) {
         const int st = (n + 1) % KP_STAGES;
-        if (!wait(&bar.k_empty[st], (n + 1) / KP_STAGES - 1)) break;
+        if (n + 1 >= KP_STAGES && !wait(&bar.k_empty[st], (n + 1) / KP_STAGES - 1)) break;
         uint8_t *tile = smem + H::K_OFF + st * H::K_HALF;
 #pragma unroll
         for (int i = 0; i < KN; ++i) store(kr[i], tile, H::K_BLOCK, kkey + i * KSTEP, kch);
@@ -426,7 +430,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       if (n + 1 < n_tiles) load_k(id_k);
       if (n >= 0) {
         const int st = n % KP_STAGES;
-        if (!wait(&bar.v_empty[st], n / KP_STAGES - 1)) break;
+        if (n >= KP_STAGES && !wait(&bar.v_empty[st], n / KP_STAGES - 1)) break;
         if (has_v) {
           uint8_t *tile = smem + H::V_OFF + st * H::V_HALF;
 #pragma unroll
@@ -477,9 +481,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         lv_top = fmaxf(lv_top, __shfl_xor_sync(0xffffffffu, lv_top, o));
       const uint32_t missing = __ballot_sync(0xffffffffu, ks_l < 0.f) & 0xFFu;
 
-      if (ok && !tc::mbar_wait(&bar.s_full[hf], (uint32_t)((n >> 1) & 1), abort, KP_WAIT_NS))
-        s_abort = 1;
-      ok = !__any_sync(0xffffffffu, *abort != 0);
+      const int slot = n % H::SLOTS;
+      const uint32_t srow = trow + slot * 128;
+      ok = ok && wait(&bar.s_full[slot], n / H::SLOTS);
       tc::tc_fence_after();
       // S is read twice, 32 columns at a time, rather than kept in registers, in
       // rolled loops: the roles' code together has to fit the instruction cache
@@ -496,15 +500,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       };
       // K factor of a 16-key group; scale 0: every code of the page is 0 (1 keeps
       // -inf * 0 out)
-      auto factor = [&](int g) {
-        const float ks = __shfl_sync(0xffffffffu, ks_l, g);
-        return fac * (ks > 0.f ? ks : 1.f);
-      };
+      const float kf_l = ks_l > 0.f ? ks_l : 1.f;
+      auto factor = [&](int g) { return fac * __shfl_sync(0xffffffffu, kf_l, g); };
       float top = -INFINITY;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t v[32];
-        tc::tmem_ld32(trow + hf * 128 + c * 32, v);
+        tc::tmem_ld32(srow + c * 32, v);
         tc::tmem_ld_wait();
         if (masked) mask(v, c);
 #pragma unroll
@@ -533,37 +535,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       l *= kp_ratio(m, m_new);  // (the other warpgroup may have moved it too)
       m = m_new;
       if (ok && n > 0 && (lvref > lv_prev || __any_sync(0xffffffffu, move))) {  // rescale O
-        if (!tc::mbar_wait(&bar.o_done, (uint32_t)((n - 1) & 1), abort, KP_WAIT_NS)) s_abort = 1;
-        ok = !__any_sync(0xffffffffu, *abort != 0);
+        ok = wait(&bar.o_done[(n - 1) % H::SLOTS], (n - 1) / H::SLOTS);
         tc::tc_fence_after();
         const float a = kp_ratio(m_prev, m_new) * kp_ex2(lv_prev - lvref);
         if (ok) {
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t v[32];
-            tc::tmem_ld32(trow + 256 + c0, v);
+            tc::tmem_ld32(trow + H::O_COL + c0, v);
             tc::tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
-            kp_tmem_st32(trow + 256 + c0, v);
+            kp_tmem_st32(trow + H::O_COL + c0, v);
           }
           kp_tmem_st_wait();
         }
       }
       const float sub = shift - (m == -INFINITY ? 0.f : m);
+      // log2 of V scale / v of the lane's group, and the way back for l
+      const float cg_l = lv_l > KP_NO_SCALE ? lv_l - lvref : 0.f;
+      const float back_l = kp_ex2(fminf(-cg_l, 126.f));
       // (P, 16 columns, only goes over columns that have been read)
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t v[32], pk[16];
-        tc::tmem_ld32(trow + hf * 128 + c * 32, v);
+        tc::tmem_ld32(srow + c * 32, v);
         tc::tmem_ld_wait();
         if (masked) mask(v, c);
 #pragma unroll
         for (int gg = 0; gg < 2; ++gg) {
           const int g = 2 * c + gg;
-          const float lv = __shfl_sync(0xffffffffu, lv_l, g), f = factor(g);
-          const float cg = lv > KP_NO_SCALE ? lv - lvref : 0.f;
-          const f2 ff = f2_make(f, f), cc = f2_make(sub + cg, sub + cg);
+          const float f = factor(g), cg = sub + __shfl_sync(0xffffffffu, cg_l, g);
+          const float back = __shfl_sync(0xffffffffu, back_l, g);
+          const f2 ff = f2_make(f, f), cc = f2_make(cg, cg);
           float e[16];
 #pragma unroll
           for (int j = 0; j < 16; j += 2)
@@ -580,16 +584,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
           }
           float s0, s1;
           f2_split(f2_add(sum0, sum1), s0, s1);
-          l = fmaf(s0 + s1, kp_ex2(fminf(-cg, 126.f)), l);
+          l = fmaf(s0 + s1, back, l);
 #pragma unroll
           for (int j = 0; j < 16; j += 2) pk[gg * 8 + (j >> 1)] = pack_h2(e[j], e[j + 1]);
         }
-        kp_tmem_st16(trow + hf * 128 + c * 16, pk);
+        kp_tmem_st16(srow + c * 16, pk);
       }
       kp_tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();
-      if (ok && lane == 0) kp_arrive_leader(&bar.p_full[hf]);
+      if (ok && lane == 0) kp_arrive_leader(&bar.p_full[slot]);
     }
     // ---- the row's m, v and l after the last tile, and its O after the last product
     kp_soft_sync();
@@ -603,8 +607,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     kp_soft_sync();
     l = s_l[0][r] + s_l[1][r];
     if (ok && n_tiles > 0) {
-      if (!tc::mbar_wait(&bar.o_last, 0, abort, KP_WAIT_NS)) s_abort = 1;
-      ok = !__any_sync(0xffffffffu, *abort != 0);
+      ok = wait(&bar.o_last, 0);
       tc::tc_fence_after();
     }
     if (ok) {
@@ -623,7 +626,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       for (int c0 = hf * (D / 2); c0 < (hf + 1) * (D / 2); c0 += 32) {
         uint32_t x[32];
         if (n_tiles > 0) {
-          tc::tmem_ld32(trow + 256 + c0, x);
+          tc::tmem_ld32(trow + H::O_COL + c0, x);
           tc::tmem_ld_wait();
         } else {
 #pragma unroll
