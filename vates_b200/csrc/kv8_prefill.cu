@@ -49,8 +49,8 @@ constexpr uint64_t KP_WAIT_NS = 2000000000ull;
 // 2^-25 (2^-29) of the largest are as exact as the largest, and 2^-35 is the
 // smallest that is kept.
 constexpr float KP_SHIFT_ONE = 15.5f;
-constexpr float KP_SHIFT = 11.f;
-constexpr float KP_MOVE = 4.f;
+constexpr float KP_SHIFT = 6.f;
+constexpr float KP_MOVE = 9.f;
 constexpr float KP_NO_SCALE = -1000.f;  // log2 of the V scale of an all-zero page
 
 template <int D>
@@ -69,7 +69,7 @@ struct KpShape {
   static constexpr int SMEM = V_OFF + KP_STAGES * V_HALF + 1024;
 };
 // Registers per thread of the four warpgroups; 128 at launch.
-constexpr int KP_R_MMA = 64, KP_R_CONV = 144, KP_R_SOFT = 152;
+constexpr int KP_R_MMA = 24, KP_R_CONV = 136, KP_R_SOFT = 176;
 static_assert(KP_R_MMA + KP_R_CONV + 2 * KP_R_SOFT == 4 * 128, "register shares");
 
 // Byte offset of 16-byte chunk c of row r in a 128-row x 64-column block.
@@ -504,19 +504,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       auto factor = [&](int g) { return fac * __shfl_sync(0xffffffffu, kf_l, g); };
       float top = -INFINITY;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tc::tmem_ld32(srow + c * 32, v);
+      for (int c = 0; c < 2; ++c) {
+        uint32_t v[32], w[32];
+        tc::tmem_ld32(srow + c * 64, v);
+        tc::tmem_ld32(srow + c * 64 + 32, w);
         tc::tmem_ld_wait();
-        if (masked) mask(v, c);
+        if (masked) { mask(v, 2 * c); mask(w, 2 * c + 1); }
 #pragma unroll
-        for (int gg = 0; gg < 2; ++gg) {
-          const uint32_t *u = v + gg * 16;
+        for (int gg = 0; gg < 4; ++gg) {
+          const uint32_t *u = (gg & 2 ? w : v) + (gg & 1) * 16;
           float x0 = kp_max3(u[0], u[1], u[2]), x1 = kp_max3(u[3], u[4], u[5]);
           float x2 = kp_max3(u[6], u[7], u[8]), x3 = kp_max3(u[9], u[10], u[11]);
           x0 = kp_max3(__float_as_uint(x0), u[12], u[13]);
           x1 = kp_max3(__float_as_uint(x1), u[14], u[15]);
-          top = fmaxf(top, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * factor(2 * c + gg));
+          top = fmaxf(top, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * factor(4 * c + gg));
         }
       }
       // maximum and v after the tile before this one, and after this one
