@@ -218,11 +218,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
 
   // ---- the pair's rows and keys, this CTA's rows r_base .. + 127
   const int rank = blockIdx.x & 1;
-  const int split = (blockIdx.x >> 1) % p.splits;
-  const int rt = p.row_tiles - 1 - (blockIdx.x >> 1) / p.splits;  // longest (causal) rows first
-  const int h = blockIdx.y, b = blockIdx.z;
+  const int units = p.c.batch * p.c.kv_heads * p.splits, unit = (blockIdx.x >> 1) % units;
+  const int rt = p.row_tiles - 1 - (blockIdx.x >> 1) / units;  // longest (causal) rows first
+  const int split = unit % p.splits, h = unit / p.splits % p.c.kv_heads;
+  const int b = unit / p.splits / p.c.kv_heads;
   const int pair_base = rt * KP_ROWS, r_base = pair_base + rank * 128, rows = p.L * p.rep;
-  const Kv8Span sp = kv8_span(p, b, blockIdx.x == 0 && h == 0 && tid == 0);
+  const Kv8Span sp = kv8_span(p, b, rt == p.row_tiles - 1 && split == 0 && rank == 0 && h == 0 && tid == 0);
   const int i_last = p.row_of(max(0, min(min(pair_base + KP_ROWS, rows), sp.q_len * p.rep) - 1));
   const int kend = pair_base < sp.q_len * p.rep ? sp.visible(i_last) : 0;
   const int tiles = (kend + KP_KT - 1) / KP_KT;
@@ -685,7 +686,7 @@ int kp_launch(const Kv8AttnParams &p, cudaStream_t s) {
       return set_error(VB_ERR_CUDA, "kv8_prefill_kernel attributes: %s", cudaGetErrorString(e));
     ready = true;
   }
-  vb_launch(kv8_prefill_kernel<D>, dim3(2 * p.row_tiles * p.splits, p.c.kv_heads, p.c.batch),
+  vb_launch(kv8_prefill_kernel<D>, dim3(2 * p.row_tiles * p.splits * p.c.kv_heads * p.c.batch),
             dim3(KP_THREADS), H::SMEM, s, false, p);
   return check_launch("kv8_prefill_kernel");
 }
