@@ -69,7 +69,7 @@ struct KpShape {
   static constexpr int SMEM = V_OFF + KP_STAGES * V_HALF + 1024;
 };
 // Registers per thread of the four warpgroups; 128 at launch.
-constexpr int KP_R_MMA = 24, KP_R_CONV = 136, KP_R_SOFT = 176;
+constexpr int KP_R_MMA = 24, KP_R_CONV = 168, KP_R_SOFT = 160;
 static_assert(KP_R_MMA + KP_R_CONV + 2 * KP_R_SOFT == 4 * 128, "register shares");
 
 // Byte offset of 16-byte chunk c of row r in a 128-row x 64-column block.
@@ -185,6 +185,19 @@ __device__ __forceinline__ void kp_tmem_st16(uint32_t taddr, const uint32_t (&r)
       "r"(r[15])
       : "memory");
 }
+// 32 bytes, whole (one sector) where the address allows it: a row's 16-byte
+// pieces on their own took twice the time.
+__device__ __forceinline__ void kp_store32(void *p, const uint32_t (&x)[8], bool whole) {
+  if (whole) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(x[0]),
+                 "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                 : "memory");
+  } else {
+    uint4 *d4 = reinterpret_cast<uint4 *>(p);
+    d4[0] = make_uint4(x[0], x[1], x[2], x[3]);
+    d4[1] = make_uint4(x[4], x[5], x[6], x[7]);
+  }
+}
 __device__ __forceinline__ void kp_tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -259,27 +272,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
 
-  // ---- queries: D / 8 lanes per row, f16 after the row's power of two; all
-  // loads before the first use
+  // ---- queries: D / 8 lanes per row, f16 after the row's power of two. They come
+  // through shared memory so that both loops can stay rolled: code that runs once
+  // costs mostly its fetching.
   {
-    constexpr int LPR = D / 8, PASS = KP_THREADS / LPR, NP = 128 / PASS;
+    constexpr int LPR = D / 8, PASS = KP_THREADS / LPR;
     const int c8 = tid % LPR;
-    uint4 w[NP];
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      const int R = r_base + tid / LPR + k * PASS, i = p.row_of(R), hr = R - i * p.rep;
-      w[k] = make_uint4(0, 0, 0, 0);
-      if (n_tiles > 0 && R < rows && i < sp.q_len)
-        w[k] = kv8_load8(p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql +
-                             c8 * 8,
-                         p.vec);
+    auto place = [&](int r) {
+      return reinterpret_cast<uint4 *>(smem + (c8 >> 3) * KP_BLOCK + kp_sw(r, c8 & 7));
+    };
+#pragma unroll 1
+    for (int r = tid / LPR; r < 128; r += PASS) {
+      const int R = r_base + r, i = p.row_of(R), hr = R - i * p.rep;
+      const uint16_t *src =
+          p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql + c8 * 8;
+      const bool there = n_tiles > 0 && R < rows && i < sp.q_len;
+      if (there && p.vec)
+        cp_async16(place(r), src);
+      else
+        *place(r) = there ? kv8_load8(src, false) : make_uint4(0, 0, 0, 0);
     }
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      const int r = tid / LPR + k * PASS;
-      const float pw = kv8_q_scale<LPR>(w[k]);
+    cp_async_commit();
+    cp_async_wait<0>();
+#pragma unroll 2
+    for (int r = tid / LPR; r < 128; r += PASS) {
+      uint4 w = *place(r);
+      const float pw = kv8_q_scale<LPR>(w);
       if (c8 == 0) s_fac[r] = p.scale_log2 / pw;
-      *reinterpret_cast<uint4 *>(smem + (c8 >> 3) * KP_BLOCK + kp_sw(r, c8 & 7)) = w[k];
+      *place(r) = w;
     }
   }
   tc::fence_proxy_async_smem();
@@ -623,6 +643,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         else if (p.lse)
           p.lse[row] = l == 0.f ? -INFINITY : (m - shift + log2f(l)) * 0.69314718055994531f;
       }
+      const bool out32 = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
       const float inv = p.splits > 1 ? v : l == 0.f ? 0.f : v / l;
 #pragma unroll 1
       for (int c0 = hf * (D / 2); c0 < (hf + 1) * (D / 2); c0 += 32) {
@@ -640,19 +661,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         __syncwarp();
         if (!live) {
         } else if (p.splits > 1) {
+          float *d = p.o_part + (tile_id * KP_ROWS + r_pair) * D + c0;
           if (n_tiles > 0) {
-            float4 *d4 = reinterpret_cast<float4 *>(p.o_part + (tile_id * KP_ROWS + r_pair) * D + c0);
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              d4[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+            for (int q = 0; q < 32; q += 8) {
+              uint32_t w[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(y[q + j]);
+              kp_store32(d + q, w, true);
+            }
           }
         } else {
-          uint4 *d4 = reinterpret_cast<uint4 *>(p.out + row * D + c0);
+          uint16_t *d = p.out + row * D + c0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            d4[q] = make_uint4(pack_bf2(y[8 * q], y[8 * q + 1]), pack_bf2(y[8 * q + 2], y[8 * q + 3]),
-                               pack_bf2(y[8 * q + 4], y[8 * q + 5]),
-                               pack_bf2(y[8 * q + 6], y[8 * q + 7]));
+          for (int q = 0; q < 32; q += 16) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = pack_bf2(y[q + 2 * j], y[q + 2 * j + 1]);
+            kp_store32(d + q, w, out32);
+          }
         }
         __syncwarp();
       }
