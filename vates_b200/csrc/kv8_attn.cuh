@@ -92,23 +92,24 @@ __device__ __forceinline__ uint4 kv8_load8(const uint16_t *q, bool vec) {
   return make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16),
                     q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
 }
+// Two bf16 times the row's power of two, as f16.
+__device__ __forceinline__ uint32_t kv8_q_h2(uint32_t w, float pw) {
+  float lo, hi;
+  f2_split(f2_mul(f2_make(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)),
+                  f2_make(pw, pw)),
+           lo, hi);
+  return pack_h2(lo, hi);
+}
 // The lane's 8 bf16 of a row that LPR lanes hold together become f16 times the
-// row's power of two, which is returned.
+// row's power of two, which is returned. Magnitudes of bf16 compare as integers.
 template <int LPR>
 __device__ __forceinline__ float kv8_q_scale(uint4 &v) {
-  uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  float x[8], amax = 0.f;
+  uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
+                        __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] = __uint_as_float((j & 1) ? (w[j >> 1] & 0xFFFF0000u) : (w[j >> 1] << 16));
-    amax = fmaxf(amax, fabsf(x[j]));
-  }
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const float pw = kv8_q_power(amax);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = pack_h2(x[2 * j] * pw, x[2 * j + 1] * pw);
-  v = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int o = LPR / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float pw = kv8_q_power(__uint_as_float(max(m << 16, m & 0xFFFF0000u)));
+  v = make_uint4(kv8_q_h2(v.x, pw), kv8_q_h2(v.y, pw), kv8_q_h2(v.z, pw), kv8_q_h2(v.w, pw));
   return pw;
 }
 

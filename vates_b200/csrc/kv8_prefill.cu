@@ -69,7 +69,7 @@ struct KpShape {
   static constexpr int SMEM = V_OFF + KP_STAGES * V_HALF + 1024;
 };
 // Registers per thread of the four warpgroups; 128 at launch.
-constexpr int KP_R_MMA = 24, KP_R_CONV = 168, KP_R_SOFT = 160;
+constexpr int KP_R_MMA = 56, KP_R_CONV = 136, KP_R_SOFT = 160;
 static_assert(KP_R_MMA + KP_R_CONV + 2 * KP_R_SOFT == 4 * 128, "register shares");
 
 // Byte offset of 16-byte chunk c of row r in a 128-row x 64-column block.
@@ -149,8 +149,12 @@ __device__ __forceinline__ void kp_arrive_leader(uint64_t *bar) {
       " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(tc::smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void kp_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+// Relaxed: nothing of what a thread has written to global memory needs to be there
+// for the other CTA, and waiting for it cost most of a microsecond.
+__device__ __forceinline__ void kp_cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void kp_cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The 256 softmax threads of a CTA meet; one half of them hands over to the other
@@ -185,18 +189,10 @@ __device__ __forceinline__ void kp_tmem_st16(uint32_t taddr, const uint32_t (&r)
       "r"(r[15])
       : "memory");
 }
-// 32 bytes, whole (one sector) where the address allows it: a row's 16-byte
-// pieces on their own took twice the time.
-__device__ __forceinline__ void kp_store32(void *p, const uint32_t (&x)[8], bool whole) {
-  if (whole) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(x[0]),
-                 "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
-                 : "memory");
-  } else {
-    uint4 *d4 = reinterpret_cast<uint4 *>(p);
-    d4[0] = make_uint4(x[0], x[1], x[2], x[3]);
-    d4[1] = make_uint4(x[4], x[5], x[6], x[7]);
-  }
+__device__ __forceinline__ void kp_store32(float *p, const float *x) {  // one whole sector
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(x[0]),
+               "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
 }
 __device__ __forceinline__ void kp_tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -211,7 +207,7 @@ __device__ __forceinline__ void kp_regs_inc() {
 }
 
 struct KpBarriers {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[3], p_full[3], o_done[3], o_last, drain;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[3], p_full[3], o_done[3], q_full, o_last, drain;
 };
 
 template <int D>
@@ -247,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   const size_t tile_id = (((size_t)b * p.c.kv_heads + h) * p.row_tiles + rt) * p.splits + split;
   const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
 
-  if (tid == 0) {
+  if (tid == 32) {
     for (int i = 0; i < KP_STAGES; ++i) {
       tc::mbar_init(&bar.k_full[i], 2 * 4);   // converter warps of both CTAs
       tc::mbar_init(&bar.v_full[i], 2 * 4);
@@ -259,6 +255,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       tc::mbar_init(&bar.p_full[i], 2 * 4);   // softmax warps of a tile, both CTAs
       tc::mbar_init(&bar.o_done[i], 1);
     }
+    tc::mbar_init(&bar.q_full, 2);  // both CTAs
     tc::mbar_init(&bar.o_last, 1);
     tc::mbar_init(&bar.drain, 1);
     s_abort = 0;
@@ -272,42 +269,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
 
-  // ---- queries: D / 8 lanes per row, f16 after the row's power of two. They come
-  // through shared memory so that both loops can stay rolled: code that runs once
-  // costs mostly its fetching.
-  {
-    constexpr int LPR = D / 8, PASS = KP_THREADS / LPR;
-    const int c8 = tid % LPR;
-    auto place = [&](int r) {
-      return reinterpret_cast<uint4 *>(smem + (c8 >> 3) * KP_BLOCK + kp_sw(r, c8 & 7));
-    };
-#pragma unroll 1
-    for (int r = tid / LPR; r < 128; r += PASS) {
-      const int R = r_base + r, i = p.row_of(R), hr = R - i * p.rep;
-      const uint16_t *src =
-          p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql + c8 * 8;
-      const bool there = n_tiles > 0 && R < rows && i < sp.q_len;
-      if (there && p.vec)
-        cp_async16(place(r), src);
-      else
-        *place(r) = there ? kv8_load8(src, false) : make_uint4(0, 0, 0, 0);
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-#pragma unroll 2
-    for (int r = tid / LPR; r < 128; r += PASS) {
-      uint4 w = *place(r);
-      const float pw = kv8_q_scale<LPR>(w);
-      if (c8 == 0) s_fac[r] = p.scale_log2 / pw;
-      *place(r) = w;
-    }
-  }
-  tc::fence_proxy_async_smem();
-  tc::tc_fence_before();
-  __syncthreads();
-  kp_cluster_sync();  // barriers, TMEM and queries of both CTAs are there
-  tc::tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  __syncwarp();
+  kp_cluster_arrive();
+  // Every role: barriers and TMEM of both CTAs are there. First loads come before it.
+  uint32_t tmem = 0;
+  auto ready = [&]() {
+    tc::tc_fence_before();
+    __syncthreads();
+    kp_cluster_wait();
+    tc::tc_fence_after();
+    tmem = s_tmem;
+  };
   volatile int *abort = &s_abort;
   const uint32_t sbase = tc::smem_u32(smem);
   // The warp waits for the n-th completion (from 0) of a barrier; false after a
@@ -321,6 +293,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   if (wg == 0) {
     // ================================================== tensor-core issuer
     kp_regs_dec<KP_R_MMA>();
+    ready();
     if (warp == 0 && rank == 0) {
       constexpr uint32_t ID_S = kp_idesc(KP_KT, false), ID_O = kp_idesc(2 * H::VD, true);
       const uint32_t one = kp_elect();
@@ -328,7 +301,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       const uint64_t q_desc = tc::smem_desc_sw128(sbase);
       const uint64_t k_desc = tc::smem_desc_sw128(sbase + H::K_OFF);
       const uint64_t v_desc = kp_desc_mn(sbase + H::V_OFF);
-      bool ok = true;
+      bool ok = n_tiles == 0 || wait(&bar.q_full, 0);
       for (int w = 0; w < n_tiles + H::SLOTS - 1 && ok; ++w) {
         if (w < n_tiles) {  // S of tile w
           const int st = w % KP_STAGES, slot = w % H::SLOTS;
@@ -437,6 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     int id_v = group_page(group_entry(t0)), id_k = group_page(group_entry(t0 + 1));
     load_k(id_v);
     if (has_v) load_v(id_v);
+    ready();
     for (int n = -1; n < n_tiles; ++n) {  // K of tile n + 1, V of tile n
       const int entry = group_entry(t0 + n + 3);
       if (n + 1 < n_tiles) {
@@ -468,8 +442,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     kp_regs_inc<KP_R_SOFT>();
     const int hf = wg - 2, r = tid & 127, R = r_base + r;  // tiles hf, hf + 2, ...; S slot hf
     const int vis = R < rows ? sp.visible(p.row_of(R)) : 0;
-    const float fac = s_fac[r];
-    const uint32_t trow = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
     const bool one = n_tiles == 1;
     const float shift = one ? KP_SHIFT_ONE : KP_SHIFT;
     float m = -INFINITY, l = 0.f, lvref = KP_NO_SCALE;
@@ -484,9 +456,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       ks = there ? __ldg(p.c.k_scales + (size_t)entry * p.c.kv_heads + h) : -1.f;
       vs = there ? __ldg(p.c.v_scales + (size_t)entry * p.c.kv_heads + h) : 0.f;
     };
-    float ks_n, vs_n;
-    group_scales(group_entry(t0 + hf), ks_n, vs_n);
+    const int entry_0 = group_entry(t0 + hf);
     int entry_n = group_entry(t0 + hf + 2);
+    // Queries: D / 8 lanes per row, f16 after the row's power of two. They come
+    // through shared memory so that both loops can stay rolled: code that runs once
+    // costs mostly its fetching.
+    constexpr int LPR = D / 8, PASS = 256 / LPR;
+    const int qtid = tid - 256, c8 = qtid % LPR;
+    auto place = [&](int qr) {
+      return reinterpret_cast<uint4 *>(smem + (c8 >> 3) * KP_BLOCK + kp_sw(qr, c8 & 7));
+    };
+    if (n_tiles > 0) {
+#pragma unroll 2
+      for (int qr = qtid / LPR; qr < 128; qr += PASS) {
+        const int Rq = r_base + qr, i = p.row_of(Rq), hr = Rq - i * p.rep;
+        const uint16_t *src =
+            p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql + c8 * 8;
+        const bool there = Rq < rows && i < sp.q_len;
+        if (there && p.vec)
+          cp_async16(place(qr), src);
+        else
+          *place(qr) = there ? kv8_load8(src, false) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    cp_async_commit();
+    float ks_n, vs_n;
+    group_scales(entry_0, ks_n, vs_n);
+    ready();
+    cp_async_wait<0>();
+    if (n_tiles > 0) {
+      // two neighbouring lanes take a row; magnitudes of bf16 compare as integers
+      kp_soft_sync();
+      const int qr = qtid >> 1, qh = qtid & 1;
+      auto chunk = [&](int c) {  // c-th 8 elements of the lane's half row
+        if (D > 64) c ^= qh << 2;  // (the two lanes in different banks)
+        const int q8 = qh * (D / 16) + c;
+        return reinterpret_cast<uint4 *>(smem + (q8 >> 3) * KP_BLOCK + kp_sw(qr, q8 & 7));
+      };
+      uint32_t mag = 0;
+#pragma unroll 4
+      for (int c = 0; c < D / 16; ++c) {
+        const uint4 w = *chunk(c);
+        mag = __vmaxu2(mag, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu),
+                                     __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+      }
+      mag = __vmaxu2(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
+      const float pw = kv8_q_power(__uint_as_float(max(mag << 16, mag & 0xFFFF0000u)));
+#pragma unroll 4
+      for (int c = 0; c < D / 16; ++c) {
+        uint4 w = *chunk(c);
+        w = make_uint4(kv8_q_h2(w.x, pw), kv8_q_h2(w.y, pw), kv8_q_h2(w.z, pw), kv8_q_h2(w.w, pw));
+        *chunk(c) = w;
+      }
+      // scale / pw; not less than 2^-80, where z is 0 for any codes: times a K scale
+      // (2^-40 and up) it must stay above 0, since masked scores are -inf times it
+      if (qh == 0)
+        s_fac[qr] = fmaxf(p.scale_log2 * __uint_as_float(0x7F000000u - __float_as_uint(pw)),
+                          8.27e-25f);
+      tc::fence_proxy_async_smem();
+      kp_soft_sync();
+      if (tid == 256) kp_arrive_leader(&bar.q_full);
+    }
+    const float fac = n_tiles > 0 ? s_fac[r] : 0.f;
+    const uint32_t trow = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
     // After a wait has given up, the tiles are gone through with what TMEM holds
     // and without further waits: the warpgroups hand over to each other in every
     // tile.
@@ -643,7 +675,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         else if (p.lse)
           p.lse[row] = l == 0.f ? -INFINITY : (m - shift + log2f(l)) * 0.69314718055994531f;
       }
-      const bool out32 = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+      // the warp's 32 rows x 32 dims go through the queries' place, which no product
+      // reads any more, so that a store covers whole 64-byte pieces of 8 rows
+      uint8_t *turn = smem + (warp - 8) * 2048;
       const float inv = p.splits > 1 ? v : l == 0.f ? 0.f : v / l;
 #pragma unroll 1
       for (int c0 = hf * (D / 2); c0 < (hf + 1) * (D / 2); c0 += 32) {
@@ -659,26 +693,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(x[j]) * inv;
         __syncwarp();
-        if (!live) {
-        } else if (p.splits > 1) {
-          float *d = p.o_part + (tile_id * KP_ROWS + r_pair) * D + c0;
-          if (n_tiles > 0) {
+        if (p.splits > 1) {
+          if (live && n_tiles > 0) {
+            float *d = p.o_part + (tile_id * KP_ROWS + r_pair) * D + c0;
 #pragma unroll
-            for (int q = 0; q < 32; q += 8) {
-              uint32_t w[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(y[q + j]);
-              kp_store32(d + q, w, true);
-            }
+            for (int q = 0; q < 32; q += 8) kp_store32(d + q, y + q);
           }
         } else {
-          uint16_t *d = p.out + row * D + c0;
 #pragma unroll
-          for (int q = 0; q < 32; q += 16) {
-            uint32_t w[8];
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4 *>(turn + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
+                make_uint4(pack_bf2(y[8 * q], y[8 * q + 1]), pack_bf2(y[8 * q + 2], y[8 * q + 3]),
+                           pack_bf2(y[8 * q + 4], y[8 * q + 5]),
+                           pack_bf2(y[8 * q + 6], y[8 * q + 7]));
+          __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = pack_bf2(y[q + 2 * j], y[q + 2 * j + 1]);
-            kp_store32(d + q, w, out32);
+          for (int k = 0; k < 4; ++k) {
+            const int s = k * 8 + (lane >> 2), q = lane & 3;
+            const uint32_t srow = __shfl_sync(0xffffffffu, live ? (uint32_t)row : 0xFFFFFFFFu, s);
+            const uint4 x4 =
+                *reinterpret_cast<const uint4 *>(turn + s * 64 + ((q ^ (s >> 1 & 3)) << 4));
+            if (srow != 0xFFFFFFFFu)
+              *reinterpret_cast<uint4 *>(p.out + (size_t)srow * D + c0 + q * 8) = x4;
           }
         }
         __syncwarp();
@@ -688,7 +724,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   tc::tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort) flag_status(p.status, VB_STATUS_TIMEOUT);
-  kp_cluster_sync();  // no product reads the other CTA's operands any more
+  // no product reads the other CTA's operands any more, and all that the leader's
+  // products signal has come
+  if (warp == 0 && rank == 1) tc::mbar_wait(&bar.drain, 0, nullptr, KP_WAIT_NS);
+  __syncwarp();
+  kp_cluster_arrive();
+  kp_cluster_wait();
   tc::tc_fence_after();
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
