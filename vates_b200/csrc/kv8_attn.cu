@@ -797,9 +797,27 @@ struct Kv8Plan {
   bool wide;            // many partial results per row
 };
 
+// Key ranges per row tile for `base` row tiles of up to `tiles` key tiles. Time in
+// key tiles: waves of 74 pairs of CTAs, each with its keys and 3 for its start and
+// end, and where there are several ranges their joining. Ranges have to promise a
+// tenth: 80 row tiles over 16,384 keys of 256 take 374 us in ranges and 452 whole, 8
+// over 4,096 27 and 61, 38 over 131,072 keys of 128 890 and 1,594, but 104 over 3,000
+// keys of 128 82 in two ranges and 70 whole (promise: 1 %).
+int kv8_ranges(long long base, long long tiles) {
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= 74 && s <= tiles && (s == 1 || base * s <= 8 * 74); ++s) {
+    const double waves = (double)((base * s + 73) / 74);
+    const double joined = s > 1 ? 2 + base * s / 32. : 0;
+    const double cost = waves * (3 + (double)((tiles + s - 1) / s)) + joined;
+    if (cost < least * (best == 1 && s > 1 ? 0.9 : 1.)) least = cost, best = s;
+  }
+  return best;
+}
+
 // Up to 32 rows per kv head: kv8_attn_kernel, 8, 16 or 32 rows, its CTAs on
 // each of 148 SMs (fewer when the table holds fewer tiles). More rows: the
-// tcgen05 kernel, a pair of CTAs per two SMs, key ranges as many as fill 148 SMs.
+// tcgen05 kernel, a pair of CTAs per two SMs.
 Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   Kv8Plan pl;
   const long long rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
@@ -809,10 +827,9 @@ Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   if (pl.tensor) {
     pl.tile_rows = kv8_prefill_rows();
     pl.row_tiles = (int)((rows + pl.tile_rows - 1) / pl.tile_rows);
-    const long long base = units * pl.row_tiles, most = (cap + 127) / 128;
-    long long s = 74 / base;  // pairs of CTAs
-    s = s < 1 ? 1 : s > most ? most : s;
-    pl.splits = (int)s;
+    const long long base = units * pl.row_tiles, tiles = (cap + 127) / 128;
+    const int s = kv8_ranges(base, tiles);
+    pl.splits = s;
     pl.ctas = 0;
     pl.parts = s == 1 ? 0 : (size_t)(base * s);
   } else {

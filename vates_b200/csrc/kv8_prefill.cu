@@ -16,13 +16,13 @@
 //     ahead of V, page numbers another tile ahead) and write them as f16 operands
 //     in 128-byte swizzled shared memory, two stages: K K-major, V as it lies
 //     (MN-major operand);
-//   * one thread of the pair issues S = Q K^T of the next key tile before
-//     O += P V of the current one, so the tensor cores work while the softmax
-//     runs; two S slots alternate;
+//   * one thread of the pair issues S = Q K^T one key tile ahead of O += P V (two
+//     for heads of 64 and 128, which leave TMEM columns for a third S slot), so the
+//     tensor cores work while the softmax runs;
 //   * two softmax warpgroups per CTA, a thread per row, take the key tiles in
 //     turn: one's exponentials run while the other waits for its products. What a
 //     tile needs of the one before it is the running maximum, which is handed
-//     over before the exponentials. It only moves when it grows by more than 2^4
+//     over before the exponentials. It only moves when it grows by more than 2^9
 //     (then O is rescaled), and P = 2^(z - m) s_V / v goes over S in TMEM as the
 //     f16 A operand of the second product. v is a power of two at least every V
 //     scale so far. l is summed in float32 from the unrounded weights.
@@ -30,6 +30,13 @@
 // begins, completion n - 1 must have happened and n + 1 must not: S of a tile
 // waits for O of the last tile in its slot, and the last O and the end have
 // barriers of their own. Every wait is bounded (2 s, then VB_STATUS_TIMEOUT).
+//
+// What bounds it: 4,096 rows over 32,768 keys of 256 take 1.97 to 2.05 ms, 1.0
+// PFLOP/s of the 1.7 that a library product reaches in a burst. A tile of 128 keys
+// takes some 2.3 us, of which the products fill 1.45; the rest is the chain S, maximum,
+// exponentials, O of one tile, of which only two are in TMEM (O takes the other half).
+// For heads of 64 it is the softmax (a tile 1.1 us; exponentials alone fill 0.55). A
+// launch without keys takes 4.5 us, one with a single tile 8.5.
 #include "kv8_attn.cuh"
 #include "tc100.cuh"
 
@@ -45,9 +52,10 @@ constexpr uint64_t KP_WAIT_NS = 2000000000ull;
 // Weights as f16 are 2^(z - m + shift) s_V / v, at most 2^15.5. A range of one
 // tile knows its maximum and its largest V scale at once and uses all of that;
 // a longer one leaves room for the maximum to grow by KP_MOVE (in log2) before
-// O has to be rescaled. f16 keeps 11 bits down to 2^-14, so weights down to
-// 2^-25 (2^-29) of the largest are as exact as the largest, and 2^-35 is the
-// smallest that is kept.
+// O has to be rescaled, which stalls the pair of CTAs (a shift of 11 and a move of 4
+// cost 6 % more time over 32,768 keys, a third more over 2,048). f16 keeps 11 bits down
+// to 2^-14, so weights down to 2^-20 (2^-29) of the largest are as exact as the
+// largest, and 2^-30 is the smallest that is kept.
 constexpr float KP_SHIFT_ONE = 15.5f;
 constexpr float KP_SHIFT = 6.f;
 constexpr float KP_MOVE = 9.f;
