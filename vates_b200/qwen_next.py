@@ -31,6 +31,8 @@ import numpy as np
 import torch
 
 from ._lib import check, lib
+from .kv8 import PagedKV8Cache
+from .logprobs import TokenLogprobs, token_logprobs
 from .moe_block import MoeBlock, Workspace
 from .pool import QuantPool, _mix, ptr, stream_handle
 from .quant_kv import build_block_so4, so4_blocks
@@ -225,11 +227,17 @@ def make_decoder_layer(cfg: QwenNextConfig, seed: int, layer: int, moe_ws: Works
 
 class QwenNextModel:
     """The main model, its MTP head and the device state of the speculative
-    loop. ``max_tokens`` (<= 8) is the largest row count of one forward."""
+    loop. ``max_tokens`` (<= 8) is the largest row count of one forward.
+    ``kv``: the cache of the full-attention layers, "isoquant" (K4/V3) or "kv8"
+    (int8 pages, :class:`vates_b200.kv8.PagedKV8Cache`)."""
 
     def __init__(self, cfg: QwenNextConfig, seed: int = 4, cache_len: int = 8192,
-                 verify_len: int = 4, drafts: int = 3, device="cuda", out_cap: int = 65536):
+                 verify_len: int = 4, drafts: int = 3, device="cuda", out_cap: int = 65536,
+                 kv: str = "isoquant"):
         assert 1 <= verify_len <= drafts + 1 <= 8
+        if kv not in ("isoquant", "kv8"):
+            raise ValueError(f'kv={kv!r}: "isoquant" or "kv8"')
+        self.kv = kv
         self.cfg, self.seed, self.device = cfg, seed, device
         self.V, self.K = verify_len, drafts
         self.max_t = 8
@@ -274,6 +282,10 @@ class QwenNextModel:
             elif lay is self.mtp_layer:
                 m.cache = {"k": torch.zeros((cfg.kv_heads, cap, D), dtype=bf, device=dev),
                            "v": torch.zeros((cfg.kv_heads, cap, D), dtype=bf, device=dev)}
+            elif self.kv == "kv8":
+                n = -(-cap // 64)
+                m.cache = PagedKV8Cache.empty(n, cfg.kv_heads, D, 1, n, 64, dev)
+                m.cache.page_table.copy_(torch.arange(n, dtype=i32)[None])
             else:
                 m.cache = {
                     "kc": torch.zeros((cfg.kv_heads, cap, D * 4 // 32), dtype=i32, device=dev),
@@ -372,6 +384,22 @@ class QwenNextModel:
                                          b["gout"].data_ptr(), self.attn_ws.data_ptr(),
                                          self.attn_ws.numel(), stream_handle(st)),
                   "vb_kv_bf16_attn_at")
+        elif self.kv == "kv8":
+            check(lib.vb_attn_prepare(b["proj"].data_ptr(), cfg.attn_proj, T, cfg.q_heads,
+                                      cfg.kv_heads, D, m.q_norm.data_ptr(), m.k_norm.data_ptr(),
+                                      cfg.eps, cfg.rope_dims, cfg.rope_base, pos_ptr, pos_add,
+                                      None, b["q"].data_ptr(), b["krow"].data_ptr(),
+                                      b["vrow"].data_ptr(), 0, b["status"].data_ptr(),
+                                      stream_handle(st)), "vb_attn_prepare")
+            rows = lambda k, n: b[k].view(-1)[:n * T * D].view(1, n, T, D)
+            pos = b["state"][SP_POS:SP_POS + 1]
+            m.cache.append(rows("krow", cfg.kv_heads), rows("vrow", cfg.kv_heads), pos,
+                           pos_add=pos_add, status=b["status"], stream=st)
+            m.cache.attend(rows("q", cfg.q_heads), pos, len_add=T + pos_add,
+                           out=rows("attn", cfg.q_heads), status=b["status"], stream=st)
+            check(lib.vb_attn_gate(b["attn"].data_ptr(), b["proj"].data_ptr(), cfg.attn_proj, T,
+                                   cfg.q_heads, b["gout"].data_ptr(), stream_handle(st)),
+                  "vb_attn_gate")
         else:
             c = m.cache
             if self.fused_append:
@@ -410,7 +438,7 @@ class QwenNextModel:
                                            b["gout"].data_ptr(), self.attn_ws.data_ptr(),
                                            self.attn_ws.numel(), stream_handle(st)),
                   "vb_kv_decode_attn_at")
-        # (the output gate is applied by the attention's combine pass)
+        # (the other caches' attention applies the output gate in its combine pass)
         m.o_proj(b["gout"], h, T, residual=x, stream=st)
 
     def _moe(self, lay: DecoderLayer, h, out, T, st):
@@ -561,6 +589,15 @@ class QwenNextModel:
     def prefill(self, prompt_ids, use_graphs: bool = True):
         """Run the prompt through the main model in chunks of ``V`` rows;
         leaves the first generated token pending (ids[0]) and counted."""
+        self._prompt(prompt_ids, use_graphs)
+        # the first generated token (generate.py:459-461): produced = [x]
+        st = self.buf["state"]
+        self.buf["out"][0] = self.buf["ids"][0]
+        st[SP_NOUT] = 1
+        return self.buf["ids"][0]
+
+    def _prompt(self, prompt_ids, use_graphs: bool, after=None):
+        """The chunks of a prompt, ``after(rows done, rows of the chunk)`` each."""
         self.reset()
         prompt = torch.as_tensor(np.asarray(prompt_ids, np.int32))
         n = prompt.numel()
@@ -573,12 +610,23 @@ class QwenNextModel:
                 self._graph(("prefill", T), lambda s, T=T: self.prefill_chunk(T, s)).replay()
             else:
                 self.prefill_chunk(T)
+            if after is not None:
+                after(done, T)
             done += T
-        # the first generated token (generate.py:459-461): produced = [x]
-        st = self.buf["state"]
-        self.buf["out"][0] = self.buf["ids"][0]
-        st[SP_NOUT] = 1
-        return self.buf["ids"][0]
+
+    def score(self, prompt_ids, top: int = 0, use_graphs: bool = True) -> TokenLogprobs:
+        """Log probability of every prompt token after the first, given the ones
+        before it, with rank, entropy and the ``top`` best alternatives
+        (:func:`vates_b200.logprobs.token_logprobs`; ``len(prompt) - 1`` rows).
+        Leaves the caches as :meth:`prefill` of all but the last token does."""
+        ids = np.asarray(prompt_ids, np.int32)
+        assert len(ids) >= 2, "the first token has nothing before it"
+        follow = torch.from_numpy(ids[1:].copy()).to(self.device)
+        parts = []
+        self._prompt(ids[:-1], use_graphs, lambda done, T: parts.append(
+            token_logprobs(self.buf["logits"][:T], follow[done:done + T], top,
+                           status=self.buf["status"])))
+        return TokenLogprobs(*(torch.cat(x) for x in zip(*parts)))
 
     def generate(self, prompt_ids, max_new: int, use_graphs: bool = True):
         """Greedy MTP self-speculative decoding (generate.py:424-961, batch
