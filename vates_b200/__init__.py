@@ -2,7 +2,8 @@
 
 - fused quantized MoE (decode/MTP-verify block, expert-major prefill),
 - pool slot-table gather,
-- IsoQuant K4/V3 KV cache quantize + quantized GQA attention.
+- IsoQuant K4/V3 KV cache quantize + quantized GQA attention,
+- int8 paged KV cache (write, read back, attention) and token log probabilities.
 
 Every compute module imports ``vates_b200._lib``, which loads
 ``libvates_b200.so`` (built in-tree with ``python -m vates_b200.build``) and
