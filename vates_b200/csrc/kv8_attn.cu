@@ -27,8 +27,8 @@
 // Shares of one (sequence, kv head) are joined by the last of its CTAs to finish
 // (ticket), or, when there are many, by kv8_combine_wide_kernel.
 //
-// What bounds it: one row over 131,072 keys, 16/2 heads of 256, takes 40.8 us for 134
-// MB (3.3 TB/s; a copy 20.8): in the middle HBM is at 0.85 of a copy, the start and
+// What bounds it: one row over 131,072 keys, 16/2 heads of 256, takes 37.7 us for 134
+// MB (3.6 TB/s; a copy 20.8): in the middle HBM is at 0.85 of a copy, the start and
 // the joining of 222 partial results take the rest. 16 sequences x 4 rows over up to
 // 8,190 keys, 32/8 heads of 128: 49 us for 127 MB, bound by instructions (issue 50 %
 // with the 12 warps that registers and the rings leave room for).
@@ -683,6 +683,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
 
 // ------------------------------------------------------------------- combine
 constexpr int KC_THREADS = 256;
+constexpr int KC_FIRST = 8;  // partial results a thread reads ahead
 constexpr int KC_MAX = 512;  // most partial results of one row
 
 // The prefill kernel's row tiles with few key ranges each: a thread joins four
@@ -736,7 +737,7 @@ template <int D>
 __global__ void __launch_bounds__(KC_THREADS) kv8_combine_wide_kernel(Kv8AttnParams p,
                                                                       int tile_rows) {
   __shared__ float s_w[KC_MAX];
-  __shared__ float4 s_acc[KC_THREADS];
+  __shared__ float4 s_acc[KC_THREADS / 32][8];
   __shared__ float s_red[KC_THREADS / 32], s_ls[KC_THREADS / 32];
   pdl_launch_dependents();
   pdl_wait();
@@ -746,6 +747,17 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_combine_wide_kernel(Kv8AttnPar
   const int d4 = blockIdx.y * 8 + (tid & 7), grp = tid >> 3, r = R % tile_rows;
   const Kv8Parts q = kv8_parts<D>(p, bh, b, R / tile_rows);
   if (p.units && q.n <= 1) return;
+  auto part = [&](int s) {
+    return __ldcg(reinterpret_cast<const float4 *>(p.o_part + (q.at(s) * tile_rows + r) * D) + d4);
+  };
+  // the first 256 are on their way while the weights are made (a result without
+  // keys has none written: it is read, but not used)
+  float4 x[KC_FIRST];
+#pragma unroll
+  for (int k = 0; k < KC_FIRST; ++k) {
+    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (grp + 32 * k < q.n) x[k] = part(grp + 32 * k);
+  }
   float M = -INFINITY, ls = 0.f;
   float2 ml[KC_MAX / KC_THREADS];
 #pragma unroll
@@ -774,23 +786,32 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_combine_wide_kernel(Kv8AttnPar
 #pragma unroll
   for (int w = 0; w < KC_THREADS / 32; ++w) ls += s_ls[w];
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int s = grp; s < q.n; s += 32) {
-    const float w = s_w[s];
+  auto add = [&](float w, const float4 &y) {
     if (w > 0.f) {
-      const float4 x =
-          __ldcg(reinterpret_cast<const float4 *>(p.o_part + (q.at(s) * tile_rows + r) * D) + d4);
-      a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y);
-      a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w);
+      a.x = fmaf(w, y.x, a.x); a.y = fmaf(w, y.y, a.y);
+      a.z = fmaf(w, y.z, a.z); a.w = fmaf(w, y.w, a.w);
     }
+  };
+#pragma unroll
+  for (int k = 0; k < KC_FIRST; ++k)
+    if (grp + 32 * k < q.n) add(s_w[grp + 32 * k], x[k]);
+#pragma unroll 8
+  for (int s = grp + 32 * KC_FIRST; s < q.n; s += 32) {
+    const float w = s_w[s];
+    if (w > 0.f) add(w, part(s));
   }
-  s_acc[tid] = a;
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) {
+    a.x += __shfl_xor_sync(0xffffffffu, a.x, o); a.y += __shfl_xor_sync(0xffffffffu, a.y, o);
+    a.z += __shfl_xor_sync(0xffffffffu, a.z, o); a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+  }
+  if ((tid & 31) < 8) s_acc[tid >> 5][tid & 7] = a;
   __syncthreads();
   if (tid >= 8) return;
 #pragma unroll
-  for (int k = 1; k < 32; ++k) {
-    const float4 x = s_acc[k * 8 + tid];
-    a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+  for (int k = 1; k < KC_THREADS / 32; ++k) {
+    const float4 y = s_acc[k][tid];
+    a.x += y.x; a.y += y.y; a.z += y.z; a.w += y.w;
   }
   kv8_finish(p, D, b, h, R, d4, M, ls, a);
 }
