@@ -828,7 +828,7 @@ struct Kv8Plan {
 // key tiles: waves of 74 pairs of CTAs, each with its keys and 3 for its start and
 // end, and where there are several ranges their joining. Ranges have to promise a
 // tenth: 80 row tiles over 16,384 keys of 256 take 374 us in ranges and 452 whole, 8
-// over 4,096 27 and 61, 38 over 131,072 keys of 128 890 and 1,594, but 104 over 3,000
+// over 4,096 27 and 61, 38 over 131,072 keys of 128 780 and 1,594, but 104 over 3,000
 // keys of 128 82 in two ranges and 70 whole (promise: 1 %).
 int kv8_ranges(long long base, long long tiles) {
   int best = 1;
