@@ -20,11 +20,11 @@
 // ties; the k largest keys are the answer.
 //
 // One CTA per row, or per slice of a row when there are few rows: the last
-// slice of a row (ticket) joins the slices in order.
+// slice of a row (ticket) joins the slices in a fixed order.
 //
 // 2,048 rows of 151,936 bf16, top 20, take 153 to 168 us (3.7 to 4.1 TB/s, a copy 97):
 // 12 instructions a logit, issue 66 %, exponentials 51 % of their pipe. 4 rows, top 5:
-// 5 us on the device.
+// 9.6 us on the device, one row, top 32: 10.2.
 #include "common.cuh"
 
 namespace vb {
@@ -37,7 +37,9 @@ constexpr int LP_MAX_TOP = 32;
 constexpr int LP_SHORT = 8 * LP_THREADS;         // rows up to here go logit by logit
 constexpr int LP_BATCH = LP_THREADS * 8;         // most keys one look can add
 constexpr int LP_CAP = LP_BATCH + LP_MAX_TOP;
-constexpr int LP_RANK_ALL = LP_THREADS;          // up to here every key is ranked at once
+// Up to here every key is ranked at once, beyond it the k-th is bisected for first (one
+// row, 304 keys: 16.6 us and 30.9; 30 rows, 608 keys: 38.3 and 36.2).
+constexpr int LP_RANK_ALL = 512;
 constexpr int LP_MAX_PARTS = 64;
 constexpr int LP_CTAS = 4;                       // per SM: one's tail behind the others' loads
 constexpr int LP_FILL = LP_CTAS * 148;
@@ -505,28 +507,49 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) token_logprobs_kernel(LpP
       s_last = atomicAdd(p.tickets + row, 1u) == (uint32_t)p.parts - 1;
       if (s_last) p.tickets[row] = 0;
       s_n = 0;
+      s_tmp[0] = ~0ull;
     }
     __syncthreads();
     if (!s_last) return;
     __threadfence();
     if (k > 0) {
       const unsigned long long *keys = p.part_keys + (size_t)row * p.parts * k;
+      // The lists are in descending order: with j * parts >= k, at least k keys reach
+      // the least of the slices' j-th ones, and only those are looked at (19 slices,
+      // 20 best: some 80 of 380).
+      if (tid < p.parts)
+        atomicMin(s_tmp, __ldcg(keys + tid * k + (k + p.parts - 1) / p.parts - 1));
+      __syncthreads();
+      const unsigned long long least = s_tmp[0];
+#pragma unroll 2
       for (int i = tid; i < p.parts * k; i += LP_THREADS) {
         const unsigned long long key = __ldcg(keys + i);
-        if (key) s_buf[atomicAdd(&s_n, 1)] = key;
+        if (key && key >= least) s_buf[atomicAdd(&s_n, 1)] = key;
       }
       __syncthreads();
       const int n = s_n;
       lp_select(s_buf, n, k, s_list, s_tmp, &s_n, s_cnt);
     }
-    if (tid == 0) {
+    if (tid < 32) {  // lane i takes slices i and i + 32
       const LpStats *st = p.part_stats + (size_t)row * p.parts;
       m = LP_FLOOR; s = t = 0.f; best = -INFINITY; ahead = 0;
-      for (int i = 0; i < p.parts; ++i) {
-        lp_join(m, s, t, __ldcg(&st[i].m), __ldcg(&st[i].s), __ldcg(&st[i].t), c);
-        best = fmaxf(best, __ldcg(&st[i].best));
-        ahead += __ldcg(&st[i].ahead);
+#pragma unroll
+      for (int i = 0; i < LP_MAX_PARTS; i += 32) {
+        if (i + tid >= p.parts) continue;
+        const float4 a = __ldcg(reinterpret_cast<const float4 *>(st + i + tid));
+        lp_join(m, s, t, a.x, a.y, a.z, c);
+        best = fmaxf(best, a.w);
+        ahead += __ldcg(&st[i + tid].ahead);
       }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
+        const float s2 = __shfl_xor_sync(0xffffffffu, s, o);
+        const float t2 = __shfl_xor_sync(0xffffffffu, t, o);
+        lp_join(m, s, t, m2, s2, t2, c);
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+      }
+      ahead = __reduce_add_sync(0xffffffffu, ahead);
     }
   }
   if (tid == 0) {
