@@ -25,7 +25,7 @@
 // new values and form the weights again. Otherwise the weights stand as
 // they are and a tile costs two barriers.
 // Shares of one (sequence, kv head) are joined by the last of its CTAs to finish
-// (ticket), or, when there are many, by kv8_combine_wide_kernel.
+// (ticket), or, when there are few units, by kv8_combine_wide_kernel.
 //
 // What bounds it: one row over 131,072 keys, 16/2 heads of 256, takes 37.7 us for 134
 // MB (3.6 TB/s; a copy 20.8): in the middle HBM is at 0.85 of a copy, the start and
@@ -869,14 +869,20 @@ Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
     pl.ctas = (int)(tiles < full ? tiles : full);
     pl.parts = (size_t)pl.ctas * 2;
   }
-  // Decode: the last CTA of a unit joins its 444 / units partial results or so, a
-  // kernel of its own once there are more than 24 (units of 16 rows over 8,192 keys
-  // of 128: 8 units 15.4 us wide and 27.9 by the last CTA, 16 units 22.1 and 25.4, 32
-  // 31.7 and 30.1, 128 90 and 71). Ranges of the prefill kernel: the wide kernel for
-  // many of few rows (256 rows 87 us and 93, 1,280 rows 116 and 105, 1,600 rows 115
-  // and 82).
-  pl.wide = pl.tensor ? pl.splits > 8 && units * rows <= 512
-                      : pl.ctas > 24 * units || units > KA_TICKETS;
+  // Decode: up to 16 units that several CTAs share are joined by the wide kernel, more
+  // by the last CTA of each, which then work side by side (wide and last CTA, on the
+  // device: heads of 128, 16 rows over 4,000 keys: 2 units 9.6 us and 15.8, 8 12.1 and
+  // 17.6, 24 21.3 and 21.9, 48 33.8 and 25.8; heads of 256, 8 rows: 2 9.8 and 21.1, 24
+  // 24.6 and 24.2, 48 38.1 and 29.1). Few results are left to the last CTA as well: a
+  // second launch costs a call outside a graph 2 us (1 row over 901 keys, 16/2 heads of
+  // 256: 8.8 and 12.3 on the device, 17.4 and 15.4 a call; 32 rows always gain, 1,000
+  // keys of 64 10.9 and 15.8, and so do many results, 7 rows over 58,182 keys of 64 in
+  // 8 units 21.9 and 27.2). Ranges of the prefill kernel: the wide kernel for many
+  // of few rows (256 rows 87 us and 93, 1,280 rows 116 and 105, 1,600 rows 115 and 82).
+  const bool shared = units <= 16 && pl.ctas > units &&
+                      (rows > 16 || pl.ctas > 24 * units ||
+                       pl.ctas * rows * a->cache.dim > 40000 * units);
+  pl.wide = pl.tensor ? pl.splits > 8 && units * rows <= 512 : shared || units > KA_TICKETS;
   pl.unit_bytes = pl.wide && !pl.tensor ? align_up(units * sizeof(int2), 16) : 0;
   pl.bytes = pl.parts == 0 ? 0
                            : KA_TICKETS * sizeof(uint32_t) + pl.unit_bytes +
