@@ -76,8 +76,8 @@ __device__ __forceinline__ void store16(uint16_t *q, const uint32_t (&x)[8], int
 // rows stay in registers between the maximum and the codes, so each is read
 // once. NV vectors of 16 elements per thread cover page * dim <= NV * 4096.
 // HBM-bound (2 bytes read and 1 written per element: 2 x 65,536 rows of 2 heads of
-// 256 take 138 us, 5.8 TB/s or 0.90 of a copy); 16 elements per thread and 32-byte
-// loads keep it from being instruction-bound. A step's few rows cost the launch, 3 us.
+// 256 take 60 us, 6.7 TB/s, a copy's rate); 16 elements per thread and 32-byte loads
+// keep it from being instruction-bound. A step's few rows cost the launch, 3 us.
 template <int NV>
 __global__ void __launch_bounds__(KW_THREADS) kv8_append_kernel(Kv8AppendParams p) {
   __shared__ uint32_t s_max[KW_THREADS / 32];
