@@ -735,6 +735,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   // no product reads the other CTA's operands any more, and all that the leader's
   // products signal has come
   if (warp == 0 && rank == 1) tc::mbar_wait(&bar.drain, 0, nullptr, KP_WAIT_NS);
+  // (after a wait gave up, arrivals may be under way that nothing has waited for)
+  if (*abort) asm volatile("fence.acq_rel.cluster;" ::: "memory");
   __syncwarp();
   kp_cluster_arrive();
   kp_cluster_wait();
