@@ -310,6 +310,36 @@ def test_attend_long_sequence(cuda):
         check_attend(c, bf16(rng, (2, 2, L, 128), 3.0).cuda(), [20001, 5], None, ref=ref)
 
 
+@pytest.mark.parametrize("batch,heads,rep,L,dim,keys", [
+    (1, 1, 8, 1, 256, 400), (1, 2, 8, 1, 256, 4000),     # few results to join, and many
+    (1, 1, 8, 4, 64, 600), (2, 8, 4, 4, 64, 1500),       # 32 rows; 16 units of 16
+    (5, 4, 2, 4, 64, 1500), (17, 1, 3, 1, 128, 700),     # more units than 16
+    (1, 1, 2, 40, 256, 3000), (1, 1, 4, 150, 128, 4000),  # prompts: ranges of few rows, of many
+    (1, 2, 1, 300, 64, 2500)])
+def test_attend_joined_ranges(cuda, batch, heads, rep, L, dim, keys):
+    """Ranges of keys joined in every way, whose maxima differ by far more than the
+    running maximum is let lag (queries along the key of one position), then again
+    on the same workspace for shorter sequences. All values are 2, so that the result
+    is 2 whatever the weights are (each rounded to f16 once, 2^-11, the result to
+    bf16, 2^-8) and the log-sum-exp tells of them."""
+    rng = np.random.default_rng(keys + dim + batch)
+    c = make_cache(rng, batch, heads, dim, 64, -(-keys // 64))
+    c.v_codes.fill_(100)
+    c.v_scales.fill_(0.02)
+    ref = Plain(c)
+    q = bf16(rng, (batch, heads * rep, L, dim), 2.0)
+    far = ref.rows(0, 0, keys)[:, keys * 2 // 3]
+    q[0, ::rep] += torch.from_numpy(far).to(torch.bfloat16)[:, None]
+    q = q.cuda()
+    for lens in ([keys - 37 * b for b in range(batch)],
+                 [max(L, keys // 5 - b) for b in range(batch)]):
+        out, lse = c.attend(q, ints(lens), return_lse=True)
+        _, want, _, ltol = attend_plain(ref, q.float().cpu().numpy().astype(np.float64), lens,
+                                        [L] * batch, dim ** -0.5, True)
+        assert (out.float() - 2.0).abs().max() <= 2.0 * (2.0 ** -8 + 2.0 ** -11)
+        assert (np.abs(lse.cpu().numpy() - want) <= ltol).all()
+
+
 def test_attend_strides_len_add_and_out(cuda):
     """Queries in a projection's layout at an odd offset, lengths given without
     this step's rows, a caller's output."""

@@ -221,3 +221,21 @@ def test_python_refusals(cuda):
         token_logprobs(x.half(), t)
     with pytest.raises(_lib.VbError):
         token_logprobs(x, t, temperature=0.0)
+
+
+@pytest.mark.parametrize("kind", ["equal", "few", "one_slice", "steps"])
+@pytest.mark.parametrize("rows,top", [(1, 32), (3, 20), (40, 7)])
+def test_best_across_slices(cuda, kind, rows, top):
+    """Best logits that lie in one slice, in all, in fewer places than are asked for
+    (the others -inf), and equal ones that go by id."""
+    rng = np.random.default_rng(rows + top)
+    V = 151936
+    x = np.zeros((rows, V), np.float32)
+    if kind == "few":
+        x[:] = -np.inf
+        x[:, rng.choice(V, 40, replace=False)] = rng.standard_normal(40).astype(np.float32)
+    elif kind == "one_slice":
+        x[:, 70000:70100] = 1 + np.arange(100, dtype=np.float32) / 32
+    elif kind == "steps":
+        x[:] = np.floor(np.arange(V) / 5000) / 4
+    check(torch.from_numpy(x).to(torch.bfloat16), rng.integers(0, 40, rows) * 3001, top)
