@@ -47,6 +47,10 @@ enum {
 
 int vb_version(void);
 const char *vb_last_error(void);
+/* Number of the graph capture that `stream` is part of (0: none, or the stream
+ * cannot be asked). A host that keeps scratch per stream needs it: a captured
+ * call is replayed later, so its scratch cannot be the stream's. */
+uint64_t vb_stream_capture_id(vb_stream_t stream);
 
 /* Nine-tensor quantized expert pool, MLX affine format (uint32-packed codes,
  * continuous LSB-first bitstream per row; bf16 scale and bias per group).
@@ -558,8 +562,10 @@ int vb_kv8_read(const VbKv8ReadArgs *args, vb_stream_t stream);
  * lse -inf. q bf16 [batch, q_heads, L, dim] with element strides {batch, head,
  * row}; out bf16 [batch, q_heads, L, dim] and lse float32 [batch, q_heads, L]
  * contiguous; query head hq reads kv head hq / (q_heads / kv_heads).
- * workspace: vb_kv8_attn_workspace_size bytes, zero-filled once, left reusable
- * by every call (of one stream at a time). */
+ * workspace: vb_kv8_attn_workspace_size bytes, of which the first
+ * VB_KV8_ATTN_WORKSPACE_HEAD have to be zero at the first call and are zero
+ * after every call (of one stream at a time). */
+#define VB_KV8_ATTN_WORKSPACE_HEAD 65536
 typedef struct VbKv8AttnArgs {
   VbKv8Cache cache;
   const uint16_t *q;
@@ -588,7 +594,9 @@ int vb_kv8_attn(const VbKv8AttnArgs *args, vb_stream_t stream);
  * Sums in float32. Logits of -inf are tokens that cannot follow. A row with a
  * NaN or +inf, or of -inf alone, has NaN logprob, entropy and top_logprobs. A
  * token outside [0, vocab) flags VB_STATUS_BOUNDS: logprob NaN, rank -1.
- * Workspace: zero-filled once, left reusable by every call. */
+ * Workspace: the first VB_TOKEN_LOGPROBS_WORKSPACE_HEAD bytes have to be zero
+ * at the first call and are zero after every call (of one stream at a time). */
+#define VB_TOKEN_LOGPROBS_WORKSPACE_HEAD 2048
 typedef struct VbTokenLogprobsArgs {
   const void *logits;
   const int32_t *tokens; /* [rows] */

@@ -1,0 +1,73 @@
+"""Scratch shared by the calls of a stream: who gets which buffer, with the
+capture state of the stream faked (no GPU needed)."""
+import pytest
+import torch
+
+from vates_b200 import scratch
+from vates_b200.scratch import Scratch
+
+CPU = torch.device("cpu")
+
+
+@pytest.fixture
+def capture(monkeypatch):
+    state = {"id": 0}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["id"] > 0)
+
+    class Lib:
+        @staticmethod
+        def vb_stream_capture_id(st):
+            return state["id"]
+
+    monkeypatch.setattr(scratch, "lib", Lib)
+    return state
+
+
+def test_calls_of_a_stream_share_a_buffer(capture):
+    s = Scratch(16)
+    a = s.get(100, CPU, 1)
+    assert a.numel() >= 100 and not a.any()
+    assert s.get(50, CPU, 1) is a and s.get(50, CPU, 2) is not a
+    b = s.get(200, CPU, 1)
+    assert b.numel() >= 200 and s.get(100, CPU, 1) is b
+    assert s.get(1, CPU, 3).numel() >= 16
+
+
+def test_a_capture_never_takes_or_leaves_an_eager_buffer(capture):
+    s = Scratch(16)
+    eager = s.get(100, CPU, 1)
+    capture["id"] = 7
+    a = s.get(50, CPU, 1)
+    assert a is not eager and not a[:16].any()
+    assert s.get(40, CPU, 1) is a          # the calls of one capture
+    assert s.get(40, CPU, 2) is not a      # a stream that was forked in it
+    capture["id"] = 0
+    assert s.get(100, CPU, 1) is eager
+    capture["id"] = 8
+    b = s.get(50, CPU, 1)
+    assert b is not a and b is not eager and not b[:16].any()
+
+
+def test_a_first_call_in_a_capture_leaves_nothing_behind(capture):
+    """Its zero fill has not run when the capture ends."""
+    s = Scratch(16)
+    capture["id"] = 3
+    a = s.get(50, CPU, 1)
+    a.fill_(9)
+    capture["id"] = 0
+    b = s.get(50, CPU, 1)
+    assert b is not a and not b.any()
+
+
+def test_a_larger_call_in_a_capture(capture):
+    s = Scratch(16)
+    capture["id"] = 3
+    a = s.get(50, CPU, 1)
+    b = s.get(500, CPU, 1)
+    assert b is not a and b.numel() >= 500 and not b[:16].any() and s.get(50, CPU, 1) is b
+
+
+def test_a_capture_without_a_number_shares_nothing(capture, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    s = Scratch(16)
+    assert s.get(50, CPU, 1) is not s.get(50, CPU, 1)

@@ -16,6 +16,8 @@ VB_STATUS_MISS = 1
 VB_STATUS_BOUNDS = 2
 VB_STATUS_TIMEOUT = 4
 VB_STATUS_NONFINITE = 8
+VB_KV8_ATTN_WORKSPACE_HEAD = 65536
+VB_TOKEN_LOGPROBS_WORKSPACE_HEAD = 2048
 VB_ERR_CAPACITY = 4
 VB_DECODE_ROUTE_ONLY = 1
 
@@ -149,6 +151,7 @@ _SZ = C.c_size_t
 _SIGNATURES = {
     "vb_version": (_I32, []),
     "vb_last_error": (C.c_char_p, []),
+    "vb_stream_capture_id": (C.c_uint64, [_P]),
     "vb_slot_remap": (_I32, [_P, _P, _P, _I64, _I32, _P, _P, _P]),
     "vb_fused_moe_workspace_size": (_SZ, [_I32, _I32]),
     "vb_fused_moe_slots": (_I32, [_P, _P, _P, C.POINTER(VbQuantPool), _I32, _I32, _I32,

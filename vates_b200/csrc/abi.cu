@@ -87,6 +87,16 @@ int vb_version(void) { return 100; }
 
 const char *vb_last_error(void) { return g_last_error; }
 
+uint64_t vb_stream_capture_id(vb_stream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(as_stream(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 int vb_slot_remap(const uint32_t *ids, const int32_t *table, int32_t *local,
                   int64_t n, int32_t table_size, int32_t *miss_count,
                   int32_t *status, vb_stream_t stream) {

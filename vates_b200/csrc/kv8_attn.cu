@@ -41,6 +41,7 @@ constexpr int KA_THREADS = 128;
 constexpr int KA_TILE = 16384;          // bytes of K, and of V, per tile
 constexpr int KA_STAGES = 2;
 constexpr int KA_TICKETS = 16384;       // units that a ticket word can join
+static_assert(KA_TICKETS * sizeof(uint32_t) == VB_KV8_ATTN_WORKSPACE_HEAD, "ticket words");
 constexpr float KA_SHIFT = 13.f;        // weights as f16 are at most 2^(13 + 2)
 constexpr float KA_MOVE = 2.f;
 

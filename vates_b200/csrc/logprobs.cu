@@ -43,7 +43,8 @@ constexpr int LP_RANK_ALL = 512;
 constexpr int LP_MAX_PARTS = 64;
 constexpr int LP_CTAS = 4;                       // per SM: one's tail behind the others' loads
 constexpr int LP_FILL = LP_CTAS * 148;
-constexpr size_t LP_TICKETS = 2048;              // bytes: a word per row of a split call
+// bytes: a word per row of a split call
+constexpr size_t LP_TICKETS = VB_TOKEN_LOGPROBS_WORKSPACE_HEAD;
 static_assert(LP_FILL / 2 * sizeof(uint32_t) <= LP_TICKETS, "rows of a split call");
 static_assert(LP_SHORT <= LP_CAP, "keys of a short row");
 static_assert(LP_MAX_PARTS * LP_MAX_TOP <= LP_CAP, "keys of a split row");

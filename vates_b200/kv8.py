@@ -4,7 +4,8 @@ A pool of pages holds int8 codes ``[pages, kv_heads, page, head_dim]`` for K
 and for V with one float32 scale per page and head (``value = code * scale``);
 a table ``[batch, max_pages]`` names the pool page of every ``page``
 consecutive positions of a sequence. Positions and lengths are device tensors,
-so a step that writes and attends can be captured in a CUDA graph.
+so a step that writes and attends can be captured in a CUDA graph, which then
+owns the scratch of its calls (:mod:`vates_b200.scratch`).
 
 Half the bytes of a bf16 cache, several sequences of different lengths, any
 number of query heads per key/value head and head sizes 64, 128 and 256; the
@@ -18,11 +19,16 @@ import ctypes as C
 
 import torch
 
+from . import _lib
 from ._lib import (VbKv8AppendArgs, VbKv8AttnArgs, VbKv8Cache, VbKv8ReadArgs, check, lib)
 from .pool import ptr, stream_handle
+from .scratch import Scratch
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
+# partial results of the key ranges; one for the caches of all layers, whose
+# attention on a stream runs one after another
+_scratch = Scratch(_lib.VB_KV8_ATTN_WORKSPACE_HEAD)
 
 
 def _rows(t: torch.Tensor, what: str, shape) -> torch.Tensor:
@@ -81,7 +87,6 @@ class PagedKV8Cache:
         self.k_codes, self.v_codes = k_codes, v_codes
         self.k_scales, self.v_scales = k_scales, v_scales
         self.pages, self.kv_heads, self.page, self.head_dim = pages, heads, page, dim
-        self._ws = {}
         self.page_table = page_table
 
     @property
@@ -196,18 +201,10 @@ class PagedKV8Cache:
             need = self._need[Hq, L] = lib.vb_kv8_attn_workspace_size(C.byref(a))
         st = stream_handle()
         if need:
-            ws = self._workspace(need, st, q.device)
+            ws = _scratch.get(need, q.device, st)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         check(lib.vb_kv8_attn(C.byref(a), st), "vb_kv8_attn")
         return (out, lse) if return_lse else out
-
-    def _workspace(self, need: int, st: int, device) -> torch.Tensor:
-        """Scratch of the key ranges' partial results, one per stream; zeroed when
-        made, left reusable by every call."""
-        ws = self._ws.get(st)
-        if ws is None or ws.numel() < need:
-            ws = self._ws[st] = torch.zeros(need, dtype=torch.uint8, device=device)
-        return ws
 
 
 __all__ = ["PagedKV8Cache"]

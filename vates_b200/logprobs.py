@@ -7,12 +7,13 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import VbTokenLogprobsArgs, check, lib
+from ._lib import VB_TOKEN_LOGPROBS_WORKSPACE_HEAD, VbTokenLogprobsArgs, check, lib
 from .pool import ptr, stream_handle
+from .scratch import Scratch
 
 MAX_TOP = 32
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
-_workspaces: dict = {}
+_scratch = Scratch(VB_TOKEN_LOGPROBS_WORKSPACE_HEAD)
 
 
 class TokenLogprobs(NamedTuple):
@@ -27,18 +28,13 @@ _needs: dict = {}
 
 
 def _workspace(rows: int, vocab: int, top: int, st: int, device) -> torch.Tensor:
-    """Scratch of rows split over several CTAs, one per device and stream;
-    zeroed when made, left reusable by every call."""
+    """Scratch of rows split over several CTAs."""
     need = _needs.get((rows, vocab, top))
     if need is None:
         if len(_needs) > 4096:
             _needs.clear()
         need = _needs[rows, vocab, top] = lib.vb_token_logprobs_workspace_size(rows, vocab, top)
-    ws = _workspaces.get((device, st))
-    if ws is None or ws.numel() < need:
-        ws = torch.zeros(max(need, 1 << 16), dtype=torch.uint8, device=device)
-        _workspaces[device, st] = ws
-    return ws
+    return _scratch.get(max(need, 1 << 16), device, st)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
