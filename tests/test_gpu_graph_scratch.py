@@ -1,5 +1,5 @@
-"""Attention over the 8-bit cache and log probabilities in CUDA graphs: graphs
-that were captured without a warm-up, that outlive larger calls, and that run
+"""Attention over the 8-bit cache, log probabilities and the MoE block in CUDA
+graphs: graphs that were captured without a warm-up, that outlive larger calls, and that run
 side by side give what an eager call gives."""
 import numpy as np
 import pytest
@@ -140,3 +140,32 @@ def test_graphs_side_by_side(cuda, kind):
                 g.replay()
         torch.cuda.synchronize()
         assert same(oa, want_a) and same(ob, want_b)
+
+
+def test_moe_block_graph_outlives_a_larger_call(cuda):
+    """A block of one token captured, then one of eight called: the graph's scratch
+    (its barrier's counter among it) is nobody else's. And a graph whose capture
+    is the first call on its workspace."""
+    from vates_b200.moe_block import Workspace
+    from vates_b200.synth import config0, input_tokens
+    blk, _ = config0(seed=0)
+    x1, x8 = input_tokens(31, 1), input_tokens(32, 8)
+    blk.workspace = Workspace()
+    want1, want8 = (t.clone() for t in warm(lambda: blk.decode(x1), lambda: blk.decode(x8)))
+    for first_in_capture in (False, True):
+        blk.workspace = Workspace()
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = torch.empty_like(want1)
+        if not first_in_capture:
+            blk.decode(x1)
+        torch.cuda.synchronize()
+        g, _ = capture(lambda: blk.decode(x1, out=out, status=status))
+        assert torch.equal(blk.decode(x8), want8)
+        taken = [torch.full((n,), 0x5A, dtype=torch.uint8, device="cuda")
+                 for n in [1 << 14] * 8 + [1 << 17] * 8 + [1 << 20] * 8]
+        for _ in range(3):
+            out.fill_(7)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want1) and int(status) == 0
+        assert all(bool((t == 0x5A).all()) for t in taken)

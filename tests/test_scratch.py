@@ -71,3 +71,22 @@ def test_a_capture_without_a_number_shares_nothing(capture, monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     s = Scratch(16)
     assert s.get(50, CPU, 1) is not s.get(50, CPU, 1)
+
+
+def test_moe_workspace_keeps_what_graphs_may_hold(capture, monkeypatch):
+    from vates_b200 import moe_block
+    monkeypatch.setattr(moe_block, "stream_handle", lambda: 1)
+    w = moe_block.Workspace(CPU)
+    capture["id"] = 2
+    first = w.get(64)  # nothing was there: the graph's own
+    assert not first.any() and w.buf is None
+    capture["id"] = 0
+    small = w.get(64)
+    assert small is not first and not small.any()
+    capture["id"] = 5
+    assert w.get(64) is small
+    assert w.get(128) is not small and w.buf is small
+    capture["id"] = 0
+    large = w.get(128)
+    assert large is w.buf and not large.any() and w.get(64) is large
+    assert any(t is small for t in w._outgrown)

@@ -13,21 +13,30 @@ import torch
 
 from ._lib import VbMoeDecodeArgs, check, lib
 from .pool import QuantPool, ptr, stream_handle
+from .scratch import Scratch
 
 DECODE_SEQ_MAX = 8  # block.py:22 (_DECODE_SEQ_MAX)
 
 
 class Workspace:
     """Grow-only, zero-initialised device scratch buffer shared by the calls
-    of one stream (the decode kernels keep a counter in its first word and
-    leave it at zero)."""
+    of one stream (the decode kernels keep their barrier's counter in its first
+    word). A buffer that has been outgrown is kept: a CUDA graph may hold its
+    address. A capture that would outgrow it takes a buffer of its own, whose
+    zero fill is part of the graph."""
 
     def __init__(self, device="cuda"):
         self.device = device
         self.buf = None
+        self._outgrown = []
+        self._captured = Scratch()
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf is None or self.buf.numel() < nbytes:
+            if torch.cuda.is_current_stream_capturing():
+                return self._captured.get(max(nbytes, 1), self.device, stream_handle())
+            if self.buf is not None:
+                self._outgrown.append(self.buf)
             self.buf = torch.zeros(max(nbytes, 1), dtype=torch.uint8, device=self.device)
         return self.buf
 

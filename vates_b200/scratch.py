@@ -17,9 +17,9 @@ from ._lib import lib
 
 class Scratch:
     """Buffers by stream, and by stream and capture. ``head``: bytes at the
-    start that a call needs zeroed."""
+    start that a call needs zeroed (0: all)."""
 
-    def __init__(self, head: int):
+    def __init__(self, head: int = 0):
         self.head = head
         self._eager: dict = {}
         self._captured: dict = {}  # (device, stream) -> (capture, buffer) of the last capture
@@ -32,7 +32,7 @@ class Scratch:
             held, buf = self._captured.get((device, st), (None, None))
             if not capture or held != capture or buf.numel() < nbytes:
                 buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-                buf[:self.head].zero_()
+                buf[:self.head or nbytes].zero_()
                 self._captured[device, st] = capture, buf
             return buf
         buf = self._eager.get((device, st))
