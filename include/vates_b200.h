@@ -511,6 +511,7 @@ int vb_kv_bf16_attn_at(const uint16_t *q, const uint16_t *k_cache, const uint16_
 /* ---------------------------------------------------------------------------
  * Paged 8-bit KV cache (no reference counterpart): int8 codes with one float32
  * scale per page and kv head, for K and for V; a stored value is code * scale.
+ * Scales are finite and not negative; 0 makes the page's values 0.
  * page_table[b][i] is the pool page of positions [i * page, (i + 1) * page) of
  * sequence b. Pages written by a call must not be shared between sequences.
  * dim in {64, 128, 256}, page in {16, 32, 64, 128}; codes 16-byte aligned. A

@@ -59,7 +59,7 @@ constexpr uint64_t KP_WAIT_NS = 2000000000ull;
 constexpr float KP_SHIFT_ONE = 15.5f;
 constexpr float KP_SHIFT = 6.f;
 constexpr float KP_MOVE = 9.f;
-constexpr float KP_NO_SCALE = -1000.f;  // log2 of the V scale of an all-zero page
+constexpr float KP_NO_SCALE = -1000.f;  // log2 of a V scale of 0
 
 template <int D>
 struct KpShape {
@@ -196,6 +196,12 @@ __device__ __forceinline__ void kp_tmem_st16(uint32_t taddr, const uint32_t (&r)
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
       "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void kp_tmem_zero8(uint32_t taddr) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(
+                   taddr),
+               "r"(0)
+               : "memory");
 }
 __device__ __forceinline__ void kp_store32(float *p, const float *x) {  // one whole sector
   asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(x[0]),
@@ -516,11 +522,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         w = make_uint4(kv8_q_h2(w.x, pw), kv8_q_h2(w.y, pw), kv8_q_h2(w.z, pw), kv8_q_h2(w.w, pw));
         *chunk(c) = w;
       }
-      // scale / pw; not less than 2^-80, where z is 0 for any codes: times a K scale
-      // (2^-40 and up) it must stay above 0, since masked scores are -inf times it
-      if (qh == 0)
-        s_fac[qr] = fmaxf(p.scale_log2 * __uint_as_float(0x7F000000u - __float_as_uint(pw)),
-                          8.27e-25f);
+      if (qh == 0) s_fac[qr] = p.scale_log2 / pw;
       tc::fence_proxy_async_smem();
       kp_soft_sync();
       if (tid == 256) kp_arrive_leader(&bar.q_full);
@@ -541,6 +543,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       for (int o = 4; o > 0; o >>= 1)
         lv_top = fmaxf(lv_top, __shfl_xor_sync(0xffffffffu, lv_top, o));
       const uint32_t missing = __ballot_sync(0xffffffffu, ks_l < 0.f) & 0xFFu;
+      // groups whose V scale is 0: their weights count for l alone
+      const uint32_t blank = __ballot_sync(0xffffffffu, lv_l == KP_NO_SCALE) & 0xFFu & ~missing;
 
       const int slot = n % H::SLOTS;
       const uint32_t srow = trow + slot * 128;
@@ -559,10 +563,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         for (int j = 0; j < 32; ++j)
           if (!((keep >> j) & 1)) v[j] = 0xFF800000u;
       };
-      // K factor of a 16-key group; scale 0: every code of the page is 0 (1 keeps
-      // -inf * 0 out)
-      const float kf_l = ks_l > 0.f ? ks_l : 1.f;
-      auto factor = [&](int g) { return fac * __shfl_sync(0xffffffffu, kf_l, g); };
+      // K factor of a 16-key group; at least 2^-100, where z is 0 for any codes and a
+      // masked score stays -inf (scale 0 makes every score of the page 0)
+      const float kf_l = fmaxf(ks_l, 0.f);
+      auto factor = [&](int g) {
+        return fmaf(fac, __shfl_sync(0xffffffffu, kf_l, g), 7.9e-31f);
+      };
       float top = -INFINITY;
 #pragma unroll 1
       for (int c = 0; c < 2; ++c) {
@@ -653,6 +659,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         kp_tmem_st16(srow + c * 16, pk);
       }
       kp_tmem_st_wait();
+      if (blank) {  // (rare, so the weights are first written as if they counted)
+#pragma unroll 1
+        for (int g = 0; g < 8; ++g)
+          if ((blank >> g) & 1) kp_tmem_zero8(srow + g * 8);
+        kp_tmem_st_wait();
+      }
       tc::tc_fence_before();
       __syncwarp();
       if (ok && lane == 0) kp_arrive_leader(&bar.p_full[slot]);
