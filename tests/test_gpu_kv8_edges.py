@@ -55,3 +55,14 @@ def test_pages_blanked_by_their_scale(cuda, L, rep, keys, dim, page):
     # equal weights of 2^6 to 2^15.5 whose sum is exact: log2 of it (below 2^5 each,
     # within an ulp) and two float32 steps
     assert (lse.cpu() - seen).abs().max() <= 2.0 ** -17
+
+
+@both
+def test_keys_of_vanishing_values_keep_their_weight(cuda, L, rep, keys, dim, page):
+    """Equal scores over pages whose V scales lie 2^140 apart: the small values add
+    nothing, but their keys are as likely as the others."""
+    c, q = setup(L, rep, keys, dim, page)
+    c.k_scales.zero_()
+    c.v_scales.fill_(2.0 ** -40)
+    c.v_scales[pages(c, 0.0, 0.5)] = 2.0 ** 100
+    check_attend(c, q.cuda(), [keys], None, causal=False)

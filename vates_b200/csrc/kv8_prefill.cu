@@ -620,9 +620,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         }
       }
       const float sub = shift - (m == -INFINITY ? 0.f : m);
-      // log2 of V scale / v of the lane's group, and the way back for l
-      const float cg_l = lv_l > KP_NO_SCALE ? lv_l - lvref : 0.f;
-      const float back_l = kp_ex2(fminf(-cg_l, 126.f));
+      // log2 of V scale / v of the lane's group, and the way back for l: bounded, so that
+      // exponentials whose weight rounds to 0 in f16 are there for l
+      const float cg_l = lv_l > KP_NO_SCALE ? fmaxf(lv_l - lvref, -60.f) : 0.f;
+      const float back_l = kp_ex2(-cg_l);
       // (P, 16 columns, only goes over columns that have been read)
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
