@@ -66,3 +66,51 @@ def test_keys_of_vanishing_values_keep_their_weight(cuda, L, rep, keys, dim, pag
     c.v_scales.fill_(2.0 ** -40)
     c.v_scales[pages(c, 0.0, 0.5)] = 2.0 ** 100
     check_attend(c, q.cuda(), [keys], None, causal=False)
+
+
+@both
+def test_large_and_small_queries(cuda, L, rep, keys, dim, page):
+    """A power of two per row keeps queries of any size exact."""
+    c, q = setup(L, rep, keys, dim, page)
+    flat = q.view(-1, dim)
+    flat[0] *= 2.0 ** 60
+    flat[1] *= 2.0 ** -60
+    flat[-1] = 0
+    c.k_scales.mul_(2.0 ** -30)
+    check_attend(c, q.cuda(), [keys], None)
+
+
+@both
+@pytest.mark.parametrize("power", [18, 22, 24, 26, 27, 28, 30, 33, 40, 60])
+def test_scores_of_any_size(cuda, L, rep, keys, dim, page, power):
+    """Scores of 2^power, where float32 is coarser than the exponentials' range: one
+    key stands out for each row (its codes are the signs of the row's query, the
+    others' products are half as large at most), so its value is the result."""
+    c, q = setup(L, rep, keys, dim, page, seed=power)
+    rng = np.random.default_rng(power)
+    sign = torch.from_numpy(rng.choice([-1, 1], (rep * L, dim)).astype(np.float32))
+    # the row's own key, spread over the sequence
+    at = torch.arange(rep * L) * (keys // (rep * L)) + (keys - 1) % max(1, keys // (rep * L))
+    c.k_scales.fill_(2.0 ** -10)
+    c.k_codes.clamp_(-30, 30)
+    ids = c.page_table[0].long()[torch.div(at, page, rounding_mode="floor").cuda()]
+    c.k_codes[ids, 0, (at % page).cuda()] = (sign * 120).to(torch.int8).cuda()
+    # sum over dims of 120 |q| 2^-10 scale = 2^power ln 2
+    amp = 2.0 ** power * math.log(2) / (dim * 120 * 2.0 ** -10 * dim ** -0.5)
+    mag = torch.from_numpy(rng.uniform(0.9, 1.1, (rep * L, dim)).astype(np.float32)) * amp
+    q = (sign * mag).to(torch.bfloat16).view(1, rep, L, dim)
+    out, lse = c.attend(q.cuda(), ints([keys]), causal=False, return_lse=True)
+    ref = Plain(c)
+    V, K = ref.rows(1, 0, keys)[0], ref.rows(0, 0, keys)[0]
+    z = (q.double().view(-1, dim).numpy() @ K.T) * dim ** -0.5
+    best = z.argmax(1)
+    assert np.array_equal(best, at.numpy())
+    two = np.sort(z, 1)
+    assert keys == 1 or (two[:, -1] - two[:, -2] >= 2.0 ** (power - 3)).all()
+    # the value, rounded to f16 weights' 2^-11 of it, and to bf16
+    want = V[best].reshape(rep, L, dim)
+    got = out[0].double().cpu().numpy()
+    assert (np.abs(got - want) <= np.abs(want) * (2.0 ** -8 + 2.0 ** -11)).all()
+    zt = z.max(1).reshape(rep, L)
+    # float32 sums of dim products and three float32 steps
+    assert (np.abs(lse[0].cpu().numpy() - zt) <= zt * (dim * 2.0 ** -24 + 2.0 ** -21)).all()

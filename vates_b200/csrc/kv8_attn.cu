@@ -42,7 +42,10 @@ constexpr int KA_TILE = 16384;          // bytes of K, and of V, per tile
 constexpr int KA_STAGES = 2;
 constexpr int KA_TICKETS = 16384;       // units that a ticket word can join
 static_assert(KA_TICKETS * sizeof(uint32_t) == VB_KV8_ATTN_WORKSPACE_HEAD, "ticket words");
-constexpr float KA_SHIFT = 13.f;        // weights as f16 are at most 2^(13 + 2)
+// Weights as f16 are 2^(z - m) s_V / v with m the row's maximum less KA_SHIFT, until
+// the maximum has grown by more than KA_MOVE: at most 2^15. m is rounded up and what a
+// score may reach down, so that this holds for scores of any size.
+constexpr float KA_SHIFT = 13.f;
 constexpr float KA_MOVE = 2.f;
 
 template <int D, int NR>  // NR groups of 8 query rows
@@ -418,7 +421,11 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
 #pragma unroll
       for (int o2 = NG / 2; o2 > 0; o2 >>= 1)
         vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o2));
-      float vs[MW];
+      float vs[MW], lim[NR][2];
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) lim[n][u] = __fadd_rd(m[n][u], KA_SHIFT + KA_MOVE);
       bool over = vmax > vref;
 #pragma unroll
       for (int j = 0; j < MW; ++j) {
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
           for (int u = 0; u < 4; ++u) {
             const float z = acc[j][n][u] * (fac[n][u & 1] * ks);
             acc[j][n][u] = key + (u >> 1) * 8 < vis[n][u & 1] ? z : -INFINITY;
-            over |= acc[j][n][u] > m[n][u & 1] + KA_MOVE;
+            over |= acc[j][n][u] > lim[n][u & 1];
           }
       }
       ks_l = ks_n;
@@ -444,8 +451,8 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
       auto weights = [&]() {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          const float sub0 = KA_SHIFT - (m[n][0] == -INFINITY ? 0.f : m[n][0]);
-          const float sub1 = KA_SHIFT - (m[n][1] == -INFINITY ? 0.f : m[n][1]);
+          const float sub0 = m[n][0] == -INFINITY ? 0.f : m[n][0];
+          const float sub1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
           add[n][0] = add[n][1] = 0.f;
 #pragma unroll
           for (int j = 0; j < MW; ++j) {
@@ -453,8 +460,8 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
             const int key = (warp * MW + j) * 16 + g;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {  // keys g and g + 8
-              const float e0 = kv8_ex2(acc[j][n][2 * u] + sub0);
-              const float e1 = kv8_ex2(acc[j][n][2 * u + 1] + sub1);
+              const float e0 = kv8_ex2(acc[j][n][2 * u] - sub0);
+              const float e1 = kv8_ex2(acc[j][n][2 * u + 1] - sub1);
               add[n][0] += e0;
               add[n][1] += e1;
               *reinterpret_cast<uint32_t *>(s_p + (n * KT + key + 8 * u) * 16 + c * 4) =
@@ -488,8 +495,9 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int r = n * 8 + 2 * c + u;
-            const float mn = fmaxf(fmaxf(fmaxf(s_max[0][r], s_max[1][r]),
-                                         fmaxf(s_max[2][r], s_max[3][r])), m[n][u]);
+            const float top = fmaxf(fmaxf(s_max[0][r], s_max[1][r]),
+                                    fmaxf(s_max[2][r], s_max[3][r]));
+            const float mn = fmaxf(__fadd_ru(top, -KA_SHIFT), m[n][u]);
             const float alpha = mn == -INFINITY ? 0.f : kv8_ex2(m[n][u] - mn);
             m[n][u] = mn;
             l[n][u] *= alpha;
@@ -567,10 +575,10 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
         const float mul = !whole ? vref : ls == 0.f ? 0.f : vref / ls;  // 0: sees no key
         if (warp == 0 && g == 0) {
           if (!whole)
-            p.ml_part[slot * ROWS + r] = make_float2(m[n][u] - KA_SHIFT, ls);
+            p.ml_part[slot * ROWS + r] = make_float2(m[n][u], ls);
           else if (p.lse)
             p.lse[row] = ls == 0.f ? -INFINITY
-                                   : (m[n][u] - KA_SHIFT + log2f(ls)) * 0.69314718055994531f;
+                                   : (m[n][u] + log2f(ls)) * 0.69314718055994531f;
         }
 #pragma unroll
         for (int d = 0; d < T::ND; ++d) {

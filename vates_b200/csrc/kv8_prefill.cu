@@ -49,13 +49,14 @@ constexpr int KP_STAGES = 2;            // K, and V, operand tiles
 constexpr int KP_ROWS = 256;            // query rows of a pair of CTAs
 constexpr int KP_BLOCK = 16384;         // 128 rows x 64 f16, 128-byte swizzle
 constexpr uint64_t KP_WAIT_NS = 2000000000ull;
-// Weights as f16 are 2^(z - m + shift) s_V / v, at most 2^15.5. A range of one
-// tile knows its maximum and its largest V scale at once and uses all of that;
-// a longer one leaves room for the maximum to grow by KP_MOVE (in log2) before
-// O has to be rescaled, which stalls the pair of CTAs (a shift of 11 and a move of 4
-// cost 6 % more time over 32,768 keys, a third more over 2,048). f16 keeps 11 bits down
-// to 2^-14, so weights down to 2^-20 (2^-29) of the largest are as exact as the
-// largest, and 2^-30 is the smallest that is kept.
+// Weights as f16 are 2^(z - m) s_V / v, m the row's maximum less a shift, at most
+// 2^15.5: m is rounded up and what a score may reach down, so that this holds for scores
+// of any size. A range of one tile knows its maximum and its largest V scale at once and
+// uses all of that; a longer one leaves room for the maximum to grow by KP_MOVE (in
+// log2) before O has to be rescaled, which stalls the pair of CTAs (a shift of 11 and a
+// move of 4 cost 6 % more time over 32,768 keys, a third more over 2,048). f16 keeps 11
+// bits down to 2^-14, so weights down to 2^-20 (2^-29) of the largest are as exact as
+// the largest, and 2^-30 is the smallest that is kept.
 constexpr float KP_SHIFT_ONE = 15.5f;
 constexpr float KP_SHIFT = 6.f;
 constexpr float KP_MOVE = 9.f;
@@ -566,9 +567,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       // K factor of a 16-key group; at least 2^-100, where z is 0 for any codes and a
       // masked score stays -inf (scale 0 makes every score of the page 0)
       const float kf_l = fmaxf(ks_l, 0.f);
-      auto factor = [&](int g) {
-        return fmaf(fac, __shfl_sync(0xffffffffu, kf_l, g), 7.9e-31f);
-      };
+      float fq = fac, least = 7.9e-31f;
+      auto factor = [&](int g) { return fmaf(fq, __shfl_sync(0xffffffffu, kf_l, g), least); };
       float top = -INFINITY;
 #pragma unroll 1
       for (int c = 0; c < 2; ++c) {
@@ -594,8 +594,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         m_prev = s_m[r];
         lv_prev = s_lv[hf ^ 1];
       }
-      const bool move = top > m_prev + KP_MOVE;
-      const float m_new = move ? top : m_prev;
+      const bool move = top > __fadd_rd(m_prev, KP_SHIFT + KP_MOVE);
+      const float m_new = move ? __fadd_ru(top, -shift) : m_prev;
       lvref = one ? lv_top : fmaxf(lv_prev, ceilf(lv_top));
       s_m[r] = m_new;
       if (r == 0) s_lv[hf] = lvref;
@@ -619,7 +619,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
           kp_tmem_st_wait();
         }
       }
-      const float sub = shift - (m == -INFINITY ? 0.f : m);
+      float sub = m == -INFINITY ? 0.f : -m;
+      // Scores so large that a product, which z - m takes unrounded below, may lie whole
+      // powers of two off the rounded maximum: the row's S becomes z - m first, rounded
+      // alike.
+      const bool large = fabsf(sub) > 65536.f;
+      if (__any_sync(0xffffffffu, large)) {
+#pragma unroll 1
+        for (int g = 0; g < 8; ++g) {
+          const float f = factor(g);
+          uint32_t v[16];
+          tc::tmem_ld16(srow + g * 16, v);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (large) v[j] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(v[j]), f), sub));
+          kp_tmem_st16(srow + g * 16, v);
+        }
+        kp_tmem_st_wait();
+        if (large) {
+          sub = fq = 0.f;
+          least = 1.f;
+        }
+      }
       // log2 of V scale / v of the lane's group, and the way back for l: bounded, so that
       // exponentials whose weight rounds to 0 in f16 are there for l
       const float cg_l = lv_l > KP_NO_SCALE ? fmaxf(lv_l - lvref, -60.f) : 0.f;
@@ -634,7 +656,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
 #pragma unroll
         for (int gg = 0; gg < 2; ++gg) {
           const int g = 2 * c + gg;
-          const float f = factor(g), cg = sub + __shfl_sync(0xffffffffu, cg_l, g);
+          const float f = factor(g), cg = __fadd_rd(sub, __shfl_sync(0xffffffffu, cg_l, g));
           const float back = __shfl_sync(0xffffffffu, back_l, g);
           const f2 ff = f2_make(f, f), cc = f2_make(cg, cg);
           float e[16];
@@ -692,9 +714,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       const bool live = R < rows;
       if (live && hf == 0) {
         if (p.splits > 1)
-          p.ml_part[tile_id * KP_ROWS + r_pair] = make_float2(m - shift, l);
+          p.ml_part[tile_id * KP_ROWS + r_pair] = make_float2(m, l);
         else if (p.lse)
-          p.lse[row] = l == 0.f ? -INFINITY : (m - shift + log2f(l)) * 0.69314718055994531f;
+          p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
       }
       // the warp's 32 rows x 32 dims go through the queries' place, which no product
       // reads any more, so that a store covers whole 64-byte pieces of 8 rows
