@@ -69,6 +69,78 @@ def test_keys_of_vanishing_values_keep_their_weight(cuda, L, rep, keys, dim, pag
 
 
 @both
+def test_unequal_pages(cuda, L, rep, keys, dim, page):
+    """K and V scales of neighbouring pages up to 2^10 apart, a page of vanishing
+    values, V scales that grow along the sequence (the sums so far are rescaled)."""
+    c, q = setup(L, rep, keys, dim, page)
+    rng = np.random.default_rng(keys)
+    n = c.page_table.shape[1]
+    ids = c.page_table[0].long()
+    c.v_scales[ids] = torch.from_numpy((0.02 * 2.0 ** rng.uniform(-10, 0, (n, 1)))
+                                       .astype(np.float32)).cuda()
+    c.k_scales[ids] = torch.from_numpy((0.02 * 2.0 ** rng.uniform(-10, 0, (n, 1)))
+                                       .astype(np.float32)).cuda()
+    c.v_scales[pages(c, 0.6)] = 2.0 ** -30
+    check_attend(c, q.cuda(), [keys], None)
+    c.v_scales[ids] = torch.from_numpy((2.0 ** np.linspace(-14, -3, n))
+                                       .astype(np.float32)[:, None]).cuda()
+    check_attend(c, q.cuda(), [keys], None)
+
+
+@both
+def test_garbage_past_the_end_is_not_read(cuda, L, rep, keys, dim, page):
+    c, q = setup(L, rep, keys, dim, page, heads=2)
+    q = q.cuda()
+    before = c.attend(q, ints([keys]), return_lse=True)
+    ids = c.page_table[0].long()
+    last = (keys - 1) // page
+    c.k_codes[ids[last], :, (keys - 1) % page + 1:] = 127
+    c.v_codes[ids[last], :, (keys - 1) % page + 1:] = -127
+    c.k_scales[ids[last + 1:]] = math.nan
+    c.v_scales[ids[last + 1:]] = math.inf
+    c.page_table[0, last + 1:] = -1
+    for a, b in zip(before, c.attend(q, ints([keys]), return_lse=True)):
+        assert torch.equal(a, b)
+
+
+@both
+def test_missing_pages_are_masked(cuda, L, rep, keys, dim, page):
+    """Entries without a page, and pages outside the pool, in the middle of the
+    table: their keys have no weight, and the call says so."""
+    c, q = setup(L, rep, keys, dim, page)
+    n = -(-keys // page)
+    gone = sorted({1 % n, n // 2})
+    ref = Plain(c)
+    for i, e in zip(gone, (-1, 10 ** 6)):
+        c.page_table[0, i] = e
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = c.attend(q.cuda(), ints([keys]), causal=False, return_lse=True, status=status)
+    assert int(status) == _lib.VB_STATUS_BOUNDS
+    left = [p for p in range(keys) if p // page not in gone]
+    rows = ref.rows
+    ref.rows = lambda kv, b, m: rows(kv, b, keys)[:, left]
+    want, wl, tol, ltol = attend_plain(ref, q.float().numpy().astype(np.float64), [len(left)],
+                                       [L], dim ** -0.5, False)
+    assert (np.abs(out.float().cpu().numpy() - want) <= tol).all()
+    assert (np.abs(lse.cpu().numpy() - wl) <= ltol).all()
+
+
+@both
+def test_nonfinite_queries_stay_in_their_row(cuda, L, rep, keys, dim, page):
+    c, q = setup(L, rep, keys, dim, page)
+    q = q.cuda()
+    clean, cl = c.attend(q, ints([keys]), return_lse=True)
+    bad = torch.zeros((rep, L), dtype=torch.bool)
+    for h, i, x in ((0, 0, math.nan), (1, L - 1, math.inf), (rep - 1, L // 2, -math.inf)):
+        q[0, h, i, dim // 3] = x
+        bad[h, i] = True
+    out, lse = c.attend(q, ints([keys]), return_lse=True)
+    bad = bad.cuda()
+    assert out[0][bad].isnan().all() and lse[0][bad].isnan().all()
+    assert torch.equal(out[0][~bad], clean[0][~bad]) and torch.equal(lse[0][~bad], cl[0][~bad])
+
+
+@both
 def test_large_and_small_queries(cuda, L, rep, keys, dim, page):
     """A power of two per row keeps queries of any size exact."""
     c, q = setup(L, rep, keys, dim, page)
@@ -78,6 +150,60 @@ def test_large_and_small_queries(cuda, L, rep, keys, dim, page):
     flat[-1] = 0
     c.k_scales.mul_(2.0 ** -30)
     check_attend(c, q.cuda(), [keys], None)
+
+
+@both
+@pytest.mark.parametrize("odd", [0, 3])
+def test_strided_queries(cuda, L, rep, keys, dim, page, odd):
+    """Queries in a projection's layout, at an even and at an odd offset; rows that
+    see no key among them."""
+    rng = np.random.default_rng(keys + odd)
+    c = make_cache(rng, 2, 2, dim, page, -(-keys // page))
+    Hq = 2 * rep
+    base = bf16(rng, (2, L, Hq * dim + 2 * odd), 2.0).cuda()
+    q = base[..., odd:Hq * dim + odd].unflatten(-1, (Hq, dim)).transpose(1, 2)
+    lens = [keys, max(1, L // 2)]
+    a = check_attend(c, q, lens, None)
+    assert torch.equal(a, c.attend(q.contiguous(), ints(lens)))
+    check_attend(c, q, lens, [max(1, L - 1), max(1, L // 3)], causal=False)
+    # a broadcast head
+    wide = q[:, :1].expand(2, Hq, L, dim)
+    assert torch.equal(c.attend(wide, ints(lens)), c.attend(wide.contiguous(), ints(lens)))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_many_rows_over_every_page_size(cuda, dim, page):
+    rng = np.random.default_rng(dim + page)
+    c = make_cache(rng, 2, 2, dim, page, -(-700 // page))
+    q = bf16(rng, (2, 6, 50, dim), 2.0).cuda()
+    for keys in (127, 128, 129, 257, 700):
+        check_attend(c, q, [keys, 700 - keys], [50, min(50, 700 - keys)])
+
+
+@pytest.mark.parametrize("L,rep", ROWS)
+@pytest.mark.parametrize("ratio", [-10, -20, -26, -30])
+@pytest.mark.parametrize("keys", [100, 1000])
+def test_weight_on_a_page_of_small_values(cuda, L, rep, ratio, keys):
+    """Nearly all of a row's weight on a page whose values lie far below another
+    page's. A weight times its V scale over the largest one seen is an f16 number of
+    at least 2^6 times (the weight over the row's largest); what it loses below f16's
+    normal numbers is 2^-25 at most, of l >= 2^6: n 2^-31 of the largest value."""
+    dim, page = 128, 16
+    c, q = setup(L, rep, keys, dim, page, heads=1)
+    ids = c.page_table[0].long()
+    c.k_codes[ids[2:]] = 0
+    c.k_codes[ids[0]] = 0
+    c.k_codes[ids[1]] = 100
+    c.k_scales[ids] = 0.05
+    q = q.abs() + 0.5
+    c.v_scales[ids] = 1.0
+    c.v_scales[ids[1]] = 2.0 ** ratio
+    out = c.attend(q.cuda(), ints([keys]), causal=False).float().cpu().numpy()
+    want, _, tol, _ = attend_plain(Plain(c), q.float().numpy().astype(np.float64), [keys], [L],
+                                   dim ** -0.5, False)
+    # (every other key's weight is e^-28 or less, and its share of the row is in `tol`)
+    assert (np.abs(out - want) <= tol + 2.0 ** -31 * keys * 127).all()
 
 
 @both
