@@ -589,7 +589,7 @@ int vb_kv8_attn(const VbKv8AttnArgs *args, vb_stream_t stream);
  * logits [rows, vocab] (dtype 0 = bf16, 1 = float32; row_stride elements):
  *   logprob = x_t / T - lse,   lse = log sum_j exp(x_j / T)
  *   rank    = number of tokens ahead of t (greater logit, or equal and a lower
- *             id), entropy = lse - sum_j p_j x_j / T
+ *             id; none is ahead of or behind a NaN), entropy = lse - sum_j p_j x_j / T
  *   top_ids, top_logprobs [rows, top]: the best tokens, best first, ties to
  *             the lowest id; top in [0, 32], top <= vocab.
  * Sums in float32. Logits of -inf are tokens that cannot follow. A row with a

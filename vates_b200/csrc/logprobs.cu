@@ -89,8 +89,9 @@ __device__ __forceinline__ float lp_unorder(uint32_t o) {
 __device__ __forceinline__ unsigned long long lp_key(float x, int id) {
   return ((unsigned long long)lp_order(x) << 32) | (uint32_t)~id;
 }
-// The next larger value of the type (NaN after +inf: nothing compares).
+// The next larger value of the type (NaN after +inf and NaN: nothing compares).
 __device__ __forceinline__ float lp_next(float x, bool bf16) {
+  if (x != x) return x;
   const uint32_t step = bf16 ? 0x10000u : 1u;
   if (x == 0.f) return __uint_as_float(step);
   const uint32_t u = __float_as_uint(x);
