@@ -3,7 +3,7 @@
 //
 // With m the largest logit so far, c = log2(e) / T and y_j = (x_j - m) c:
 //   s = sum 2^y_j,  t = sum 2^y_j y_j   (float32)
-//   logprob = ((x_t - m) c - log2 s) ln 2,  entropy = (log2 s - t / s) ln 2.
+//   logprob = (x_t - m) / T - log2 s ln 2,  entropy = (log2 s - t / s) ln 2.
 // When m moves, with d = (m_old - m_new) c: t <- 2^d (t + d s), s <- 2^d s, so
 // the running maximum is carried per thread and the row is read once. Logits
 // enter the sums at no less than -1e32 (2^y = 0 beside any larger one), which
@@ -68,7 +68,7 @@ struct LpParams {
   unsigned long long *part_keys;  // [rows, parts, top]
   uint32_t *tickets;              // [rows], zero between calls
   int64_t row_stride;
-  float c;                        // log2(e) / temperature
+  float c, inv_t;                 // log2(e) / temperature, 1 / temperature
   int vocab, top, parts;
 };
 
@@ -197,10 +197,6 @@ struct LpRow {
   }
 };
 
-// A logit as it enters y (-inf stays, for results of that token alone).
-__device__ __forceinline__ float lp_floor(float x) {
-  return x < LP_FLOOR && x > -INFINITY ? LP_FLOOR : x;
-}
 __device__ __forceinline__ void lp_move(float &m, float &s, float &t, float to, float c) {
   if (to > m) {
     const float d = fmaxf((m - to) * c, -1000.f), a = lp_ex2(d);
@@ -555,24 +551,41 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) token_logprobs_kernel(LpP
     }
   }
   if (tid == 0) {
-    if (best <= LP_FLOOR) {  // every logit counts as LP_FLOOR: all are equal
-      s = (float)p.vocab;
-      t = 0.f;
-    }
+    s_b[0] = best;
     s_m[0] = m;
-    s_s[0] = best == -INFINITY ? NAN : log2f(s);
-    const float l2 = s_s[0];
-    p.logprob[row] = tok_ok ? ((lp_floor(xt) - m) * c - l2) * LP_LN2 : NAN;
-    p.entropy[row] = (l2 - t / s) * LP_LN2;
+    s_s[0] = s;
+    s_t[0] = t;
+  }
+  __syncthreads();
+  best = s_b[0]; m = s_m[0]; s = s_s[0]; t = s_t[0];
+  // Every logit of the row counted as LP_FLOOR. There the least difference of two values
+  // is beyond any exponent, so those equal to the largest one share the probability.
+  if (best <= LP_FLOOR && best > -INFINITY) {
+    int n = 0;
+    for (int id = tid; id < p.vocab; id += LP_THREADS) n += V::load(r.x + id) == best;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((tid & 31) == 0) s_cnt[tid >> 5] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < LP_WARPS; ++w) n += s_cnt[w];
+    // (a NaN in the row has come to s)
+    s = s == s ? (float)n : s;
+    t = 0.f;
+    m = best;
+  }
+  const float lse = best == -INFINITY ? NAN : log2f(s) * LP_LN2;  // of the logits less m
+  if (tid == 0) {
+    p.logprob[row] = tok_ok ? (xt - m) * p.inv_t - lse : NAN;
+    p.entropy[row] = lse - t / s * LP_LN2;
     p.rank[row] = tok_ok ? ahead : -1;
     if (!tok_ok) flag_status(p.status, VB_STATUS_BOUNDS);
   }
-  __syncthreads();
   if (tid < k) {
     const unsigned long long key = s_list[tid];
     p.top_ids[(size_t)row * k + tid] = (int32_t)~(uint32_t)key;
     p.top_logprobs[(size_t)row * k + tid] =
-        ((lp_floor(lp_unorder((uint32_t)(key >> 32))) - s_m[0]) * c - s_s[0]) * LP_LN2;
+        (lp_unorder((uint32_t)(key >> 32)) - m) * p.inv_t - lse;
   }
 }
 
@@ -634,6 +647,7 @@ int vb_token_logprobs(const VbTokenLogprobsArgs *a, vb_stream_t stream) {
   p.part_keys = reinterpret_cast<unsigned long long *>(w);
   p.row_stride = a->row_stride;
   p.c = (float)(1.4426950408889634 / (double)a->temperature);
+  p.inv_t = (float)(1.0 / (double)a->temperature);
   p.vocab = a->vocab; p.top = a->top;
   const dim3 grid(a->rows * p.parts), block(LP_THREADS);
   if (a->dtype == 0)
