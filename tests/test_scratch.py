@@ -73,6 +73,12 @@ def test_a_capture_without_a_number_shares_nothing(capture, monkeypatch):
     assert s.get(50, CPU, 1) is not s.get(50, CPU, 1)
 
 
+def test_the_default_stream_is_not_asked(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: 1 / 0)
+    s = Scratch(16)
+    assert s.get(50, CPU, 0) is s.get(50, CPU, 0)
+
+
 def test_moe_workspace_keeps_what_graphs_may_hold(capture, monkeypatch):
     from vates_b200 import moe_block
     monkeypatch.setattr(moe_block, "stream_handle", lambda: 1)

@@ -13,7 +13,8 @@ from .scratch import Scratch
 
 MAX_TOP = 32
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
-_scratch = Scratch(VB_TOKEN_LOGPROBS_WORKSPACE_HEAD)
+_scratch = Scratch(VB_TOKEN_LOGPROBS_WORKSPACE_HEAD)  # rows split over several CTAs
+_needs: dict = {}  # its bytes by (rows, vocab, top)
 
 
 class TokenLogprobs(NamedTuple):
@@ -22,19 +23,6 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor       # float32 [rows], nats
     top_ids: torch.Tensor       # int32 [rows, top], best first, ties to the lowest id
     top_logprobs: torch.Tensor  # float32 [rows, top]
-
-
-_needs: dict = {}
-
-
-def _workspace(rows: int, vocab: int, top: int, st: int, device) -> torch.Tensor:
-    """Scratch of rows split over several CTAs."""
-    need = _needs.get((rows, vocab, top))
-    if need is None:
-        if len(_needs) > 4096:
-            _needs.clear()
-        need = _needs[rows, vocab, top] = lib.vb_token_logprobs_workspace_size(rows, vocab, top)
-    return _scratch.get(max(need, 1 << 16), device, st)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
@@ -68,7 +56,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     tlp = lp.new_empty((rows, top))
     ids = rank.new_empty((rows, top))
     st = stream_handle()
-    ws = _workspace(rows, vocab, top, st, logits.device)
+    need = _needs.get((rows, vocab, top))
+    if need is None:
+        if len(_needs) > 4096:
+            _needs.clear()
+        need = _needs[rows, vocab, top] = max(
+            1 << 16, lib.vb_token_logprobs_workspace_size(rows, vocab, top))
+    ws = _scratch.get(need, logits.device, st)
     a = VbTokenLogprobsArgs(logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(),
                             rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), ptr(status),
                             ws.data_ptr(), ws.numel(), logits.stride(0), temperature, rows, vocab,

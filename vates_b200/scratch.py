@@ -26,18 +26,18 @@ class Scratch:
 
     def get(self, nbytes: int, device, st: int) -> torch.Tensor:
         """At least ``nbytes`` for a call on ``st``, the current stream."""
-        nbytes = max(nbytes, self.head)
-        if torch.cuda.is_current_stream_capturing():
+        # (the default stream, handle 0, cannot be captured)
+        if st and torch.cuda.is_current_stream_capturing():
             capture = lib.vb_stream_capture_id(st)
             held, buf = self._captured.get((device, st), (None, None))
             if not capture or held != capture or buf.numel() < nbytes:
-                buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                buf = torch.empty(max(nbytes, self.head), dtype=torch.uint8, device=device)
                 buf[:self.head or nbytes].zero_()
                 self._captured[device, st] = capture, buf
             return buf
         buf = self._eager.get((device, st))
         if buf is None or buf.numel() < nbytes:
-            buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            buf = torch.zeros(max(nbytes, self.head), dtype=torch.uint8, device=device)
             self._eager[device, st] = buf
         return buf
 
