@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #include "../../include/vates_b200.h"
@@ -244,6 +245,19 @@ __device__ __forceinline__ void cp_async_wait() {
 }
 
 }  // namespace vb
+
+// Sets what belongs to a kernel on a device (its attributes) once on each: `set`
+// returns VB_OK or an error. From the 65th device on, every time.
+template <typename F>
+static inline int once_per_device(std::atomic<uint64_t> &done, F set) {
+  int dev = 64;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 64;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return VB_OK;
+  const int rc = set();
+  if (rc == VB_OK) done.fetch_or(bit, std::memory_order_release);
+  return rc;
+}
 
 // Kernel launch with an optional programmatic-dependent-launch attribute.
 template <typename... KArgs, typename... Args>

@@ -902,14 +902,15 @@ Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
 template <int D, int NR>
 int kv8_launch(const Kv8AttnParams &p, int ctas, cudaStream_t s) {
   using T = Kv8Tile<D, NR>;
-  static bool ready = false;
-  if (!ready) {
+  static std::atomic<uint64_t> ready{0};
+  const int rc = once_per_device(ready, [] {
     const cudaError_t e = cudaFuncSetAttribute(
         kv8_attn_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
-    if (e != cudaSuccess)
-      return set_error(VB_ERR_CUDA, "kv8_attn_kernel attributes: %s", cudaGetErrorString(e));
-    ready = true;
-  }
+    return e == cudaSuccess ? VB_OK
+                            : set_error(VB_ERR_CUDA, "kv8_attn_kernel attributes: %s",
+                                        cudaGetErrorString(e));
+  });
+  if (rc != VB_OK) return rc;
   // Dependent launch for short calls only: started before the kernel ahead has
   // left its SMs, a full grid is placed unevenly (131,072 keys: 53 us instead of
   // 41; 901 keys: 15.0 us instead of 16.3).

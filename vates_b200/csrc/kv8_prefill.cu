@@ -784,8 +784,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
 template <int D>
 int kp_launch(const Kv8AttnParams &p, cudaStream_t s) {
   using H = KpShape<D>;
-  static bool ready = false;
-  if (!ready) {
+  static std::atomic<uint64_t> ready{0};
+  const int rc = once_per_device(ready, [] {
     cudaFuncAttributes fa;
     cudaError_t e = cudaFuncGetAttributes(&fa, kv8_prefill_kernel<D>);
     // the warpgroups' register shares add up to 128 per thread at launch
@@ -795,10 +795,11 @@ int kp_launch(const Kv8AttnParams &p, cudaStream_t s) {
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(kv8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                H::SMEM);
-    if (e != cudaSuccess)
-      return set_error(VB_ERR_CUDA, "kv8_prefill_kernel attributes: %s", cudaGetErrorString(e));
-    ready = true;
-  }
+    return e == cudaSuccess ? VB_OK
+                            : set_error(VB_ERR_CUDA, "kv8_prefill_kernel attributes: %s",
+                                        cudaGetErrorString(e));
+  });
+  if (rc != VB_OK) return rc;
   vb_launch(kv8_prefill_kernel<D>, dim3(2 * p.row_tiles * p.splits * p.c.kv_heads * p.c.batch),
             dim3(KP_THREADS), H::SMEM, s, false, p);
   return check_launch("kv8_prefill_kernel");
