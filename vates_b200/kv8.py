@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import (VbKv8AppendArgs, VbKv8AttnArgs, VbKv8Cache, VbKv8ReadArgs, check, lib)
-from .pool import ptr, stream_handle
+from .pool import current_device, on_device, ptr, status_ptr, stream_handle
 from .scratch import Scratch
 
 PAGE_SIZES = (16, 32, 64, 128)
@@ -31,21 +31,24 @@ HEAD_DIMS = (64, 128, 256)
 _scratch = Scratch(_lib.VB_KV8_ATTN_WORKSPACE_HEAD)
 
 
-def _rows(t: torch.Tensor, what: str, shape) -> torch.Tensor:
+def _rows(t: torch.Tensor, what: str, shape, device: int) -> torch.Tensor:
     """``t`` as bf16 rows on the GPU with contiguous dims (other strides stay)."""
-    if t.dtype != torch.bfloat16 or not t.is_cuda:
-        raise ValueError(f"{what}: a bfloat16 CUDA tensor is needed, got {t.dtype} on {t.device}")
+    if t.dtype != torch.bfloat16 or t.get_device() != device:
+        raise ValueError(f"{what}: a bfloat16 tensor on cuda:{device} is needed, got {t.dtype} on "
+                         f"{t.device}")
     if t.shape != shape:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     return t if t.stride(3) == 1 else t.contiguous()
 
 
-def _ints(t: torch.Tensor | None, what: str, batch: int) -> int | None:
+def _ints(t: torch.Tensor | None, what: str, batch: int, device: int) -> int | None:
     """Device pointer of a contiguous int32 ``[batch]`` tensor."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or not t.is_cuda or t.numel() != batch or not t.is_contiguous():
-        raise ValueError(f"{what}: a contiguous int32 CUDA tensor of {batch} values is needed")
+    if t.dtype != torch.int32 or t.get_device() != device or t.numel() != batch \
+            or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 tensor of {batch} values on cuda:{device} "
+                         f"is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -73,6 +76,7 @@ class PagedKV8Cache:
         if k_codes.dim() != 4:
             raise ValueError("codes are [pages, kv_heads, page, head_dim]")
         pages, heads, page, dim = k_codes.shape
+        self.device = k_codes.device
         if page not in PAGE_SIZES or dim not in HEAD_DIMS:
             raise ValueError(f"page of {page} rows (one of {PAGE_SIZES}), head_dim {dim} "
                              f"(one of {HEAD_DIMS})")
@@ -81,12 +85,13 @@ class PagedKV8Cache:
                              (k_scales, (pages, heads), torch.float32),
                              (v_scales, (pages, heads), torch.float32)):
             if tuple(t.shape) != tuple(shape) or t.dtype != dt or not t.is_contiguous() \
-                    or not t.is_cuda:
+                    or not t.is_cuda or t.device != self.device:
                 raise ValueError(f"cache tensor: contiguous CUDA {dt} {tuple(shape)} is needed, "
                                  f"got {t.dtype} {tuple(t.shape)} on {t.device}")
         self.k_codes, self.v_codes = k_codes, v_codes
         self.k_scales, self.v_scales = k_scales, v_scales
         self.pages, self.kv_heads, self.page, self.head_dim = pages, heads, page, dim
+        self._index = k_codes.get_device()
         self.page_table = page_table
 
     @property
@@ -95,9 +100,10 @@ class PagedKV8Cache:
 
     @page_table.setter
     def page_table(self, t: torch.Tensor):
-        if t.dim() != 2 or t.dtype != torch.int32 or not t.is_contiguous() or not t.is_cuda:
-            raise ValueError("page_table: a contiguous int32 CUDA [batch, max_pages] tensor is "
-                             f"needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.dim() != 2 or t.dtype != torch.int32 or not t.is_contiguous() \
+                or t.device != self.device:
+            raise ValueError("page_table: a contiguous int32 [batch, max_pages] tensor on "
+                             f"{self.device} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
         self._table = t
         self.batch = t.shape[0]
         # argument structures with the cache filled in, copied for each call
@@ -135,17 +141,19 @@ class PagedKV8Cache:
         table set VB_STATUS_BOUNDS in ``status`` and are dropped; an infinity is
         stored as the page's largest value, a NaN as 0, with
         VB_STATUS_NONFINITE."""
-        if stream is not None:  # with it as the current stream, copies are made on it
-            with torch.cuda.stream(stream):
+        # with it as the current stream, copies are made on it
+        if stream is not None or current_device() != self._index:
+            with on_device(self.device, stream):
                 return self.append(keys, values, pos, counts, pos_add, status)
         B, n = self.batch, keys.shape[2] if keys.dim() == 4 else -1
         shape = (B, self.kv_heads, n, self.head_dim)
-        keys, values = _rows(keys, "keys", shape), _rows(values, "values", shape)
+        dev = self._index
+        keys, values = _rows(keys, "keys", shape, dev), _rows(values, "values", shape, dev)
         a = VbKv8AppendArgs.from_buffer_copy(self._append_args)
         a.keys, a.values = keys.data_ptr(), values.data_ptr()
         a.k_strides, a.v_strides = _strides(keys), _strides(values)
-        a.pos, a.counts = _ints(pos, "pos", B), _ints(counts, "counts", B)
-        a.status, a.pos_add, a.n = ptr(status), pos_add, n
+        a.pos, a.counts = _ints(pos, "pos", B, dev), _ints(counts, "counts", B, dev)
+        a.status, a.pos_add, a.n = status_ptr(status, dev), pos_add, n
         check(lib.vb_kv8_append(C.byref(a), stream_handle()), "vb_kv8_append")
 
     # -------------------------------------------------------------- read back
@@ -153,16 +161,17 @@ class PagedKV8Cache:
         """``(keys, values)`` bf16 ``[batch, kv_heads, n, head_dim]``: the rows
         at positions ``start[b] + i`` (``start`` None: 0), zero from ``lens[b]``
         on."""
-        if stream is not None:  # with it as the current stream, results belong to it
-            with torch.cuda.stream(stream):
+        # with it as the current stream, results belong to it
+        if stream is not None or current_device() != self._index:
+            with on_device(self.device, stream):
                 return self.read(lens, n, start, status)
-        B = self.batch
+        B, dev = self.batch, self._index
         keys = self.k_codes.new_empty((B, self.kv_heads, n, self.head_dim), dtype=torch.bfloat16)
         values = torch.empty_like(keys)
         a = VbKv8ReadArgs.from_buffer_copy(self._read_args)
-        a.lens, a.start = _ints(lens, "lens", B), _ints(start, "start", B)
+        a.lens, a.start = _ints(lens, "lens", B, dev), _ints(start, "start", B, dev)
         a.keys, a.values = keys.data_ptr(), values.data_ptr()
-        a.status, a.n = ptr(status), n
+        a.status, a.n = status_ptr(status, dev), n
         check(lib.vb_kv8_read(C.byref(a), stream_handle()), "vb_kv8_read")
         return keys, values
 
@@ -176,24 +185,27 @@ class PagedKV8Cache:
         nothing, and rows from ``q_lens[b]`` on, are zero (log-sum-exp -inf).
         Returns bf16 ``[batch, q_heads, L, head_dim]``, with ``return_lse``
         also float32 ``[batch, q_heads, L]`` (natural log)."""
-        if stream is not None:  # with it as the current stream, results belong to it
-            with torch.cuda.stream(stream):
+        # with it as the current stream, results belong to it
+        if stream is not None or current_device() != self._index:
+            with on_device(self.device, stream):
                 return self.attend(q, lens, q_lens, len_add, scale, causal, out, return_lse,
                                    status)
-        B, D = self.batch, self.head_dim
+        B, D, dev = self.batch, self.head_dim, self._index
         if q.dim() != 4:
             raise ValueError(f"q: [batch, q_heads, L, head_dim] is needed, got {tuple(q.shape)}")
         Hq, L = q.shape[1], q.shape[2]
-        q = _rows(q, "q", (B, Hq, L, D))
+        q = _rows(q, "q", (B, Hq, L, D), dev)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
-            raise ValueError("out: contiguous bfloat16 of q's shape is needed")
+        elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() \
+                or out.get_device() != dev:
+            raise ValueError(f"out: contiguous bfloat16 of q's shape on cuda:{dev} is needed, got "
+                             f"{out.dtype} {tuple(out.shape)} on {out.device}")
         lse = q.new_empty((B, Hq, L), dtype=torch.float32) if return_lse else None
         a = VbKv8AttnArgs.from_buffer_copy(self._attn_args)
         a.q, a.q_strides = q.data_ptr(), _strides(q)
-        a.lens, a.q_lens = _ints(lens, "lens", B), _ints(q_lens, "q_lens", B)
-        a.out, a.lse, a.status = out.data_ptr(), ptr(lse), ptr(status)
+        a.lens, a.q_lens = _ints(lens, "lens", B, dev), _ints(q_lens, "q_lens", B, dev)
+        a.out, a.lse, a.status = out.data_ptr(), ptr(lse), status_ptr(status, dev)
         a.scale = D ** -0.5 if scale is None else scale
         a.q_heads, a.L, a.len_add, a.causal = Hq, L, len_add, causal
         need = self._need.get((Hq, L))
@@ -201,7 +213,7 @@ class PagedKV8Cache:
             need = self._need[Hq, L] = lib.vb_kv8_attn_workspace_size(C.byref(a))
         st = stream_handle()
         if need:
-            ws = _scratch.get(need, q.device, st)
+            ws = _scratch.get(need, self.device, st)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         check(lib.vb_kv8_attn(C.byref(a), st), "vb_kv8_attn")
         return (out, lse) if return_lse else out

@@ -8,7 +8,7 @@ from typing import NamedTuple
 import torch
 
 from ._lib import VB_TOKEN_LOGPROBS_WORKSPACE_HEAD, VbTokenLogprobsArgs, check, lib
-from .pool import ptr, stream_handle
+from .pool import current_device, on_device, status_ptr, stream_handle
 from .scratch import Scratch
 
 MAX_TOP = 32
@@ -35,17 +35,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     that cannot follow. A NaN or +inf in a row makes its floating results NaN;
     a token outside the vocabulary gives NaN and rank -1 and sets
     VB_STATUS_BOUNDS in ``status``."""
-    if stream is not None:  # with it as the current stream, results belong to it
-        with torch.cuda.stream(stream):
+    dev = logits.get_device()
+    # with it as the current stream, results belong to it
+    if dev >= 0 and (stream is not None or current_device() != dev):
+        with on_device(logits.device, stream):
             return token_logprobs(logits, tokens, top, temperature, status)
-    if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
+    if logits.dim() != 2 or logits.dtype not in _DTYPES or dev < 0:
         raise ValueError("logits: bfloat16 or float32 CUDA [rows, vocab] are needed, got "
                          f"{logits.dtype} {tuple(logits.shape)} on {logits.device}")
     rows, vocab = logits.shape
-    if tokens.dtype != torch.int32 or tuple(tokens.shape) != (rows,) or not tokens.is_cuda \
-            or not tokens.is_contiguous():
-        raise ValueError(f"tokens: contiguous int32 CUDA [{rows}] is needed, got {tokens.dtype} "
-                         f"{tuple(tokens.shape)}")
+    if tokens.dtype != torch.int32 or tuple(tokens.shape) != (rows,) \
+            or tokens.get_device() != dev or not tokens.is_contiguous():
+        raise ValueError(f"tokens: contiguous int32 [{rows}] on {logits.device} is needed, got "
+                         f"{tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top={top}: 0 to {MAX_TOP} and at most the vocabulary ({vocab})")
     if logits.stride(1) != 1 and vocab > 1:
@@ -64,7 +66,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
             1 << 16, lib.vb_token_logprobs_workspace_size(rows, vocab, top))
     ws = _scratch.get(need, logits.device, st)
     a = VbTokenLogprobsArgs(logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(),
-                            rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), ptr(status),
+                            rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), status_ptr(status, dev),
                             ws.data_ptr(), ws.numel(), logits.stride(0), temperature, rows, vocab,
                             top, _DTYPES[logits.dtype])
     check(lib.vb_token_logprobs(C.byref(a), st), "vb_token_logprobs")

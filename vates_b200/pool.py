@@ -32,6 +32,29 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def status_ptr(t, device: int) -> int | None:
+    """Pointer of an optional status word, an int32 tensor on GPU ``device``."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.get_device() != device or t.numel() < 1:
+        raise ValueError(f"status: an int32 tensor on cuda:{device} is needed, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def on_device(device: torch.device, stream):
+    """Context in which ``device`` is the current one, and ``stream`` (if it is
+    given) the current stream."""
+    if stream is None:
+        return torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"stream on {stream.device}, tensors on {device}")
+    return torch.cuda.stream(stream)
+
+
+current_device = torch._C._cuda_getDevice
+
+
 def blob_layout(hidden: int, inter: int, bits: int, group: int):
     """Segments ``(key, shape, dtype, nbytes, offset)`` and the row stride of
     one expert blob (blob_layout.py:18-32, affine format v1)."""
