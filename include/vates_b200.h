@@ -555,8 +555,13 @@ typedef struct VbKv8ReadArgs {
 } VbKv8ReadArgs;
 int vb_kv8_read(const VbKv8ReadArgs *args, vb_stream_t stream);
 
-/* Attention over the cache: out = softmax(scale * q K^T) V in float32, one
- * rounding to bf16, and lse (nullable) = log sum exp of the scaled scores.
+/* Attention over the cache: out = softmax(scale * q K^T) V, rounded to bf16, and
+ * lse (nullable) = log sum exp of the scaled scores. Scores, maxima, sums and lse
+ * are float32. The second product takes f16: a weight times its page's V scale over
+ * the largest V scale v among the keys read so far. Let r be that, over the row's
+ * largest weight: 11 bits are kept down to r = 2^-20, fewer below it, none below
+ * 2^-31 (up to 32 query rows per kv head: 2^-27 and 2^-38), so beside the rounding
+ * of out a value may be off by n 2^-31 (n 2^-38) times 127 v for n keys.
  * Sequence b holds keys_b = lens[b] + len_add keys and q_lens[b] (nullable: L)
  * query rows; causal: query i sees keys < keys_b - q_lens[b] + i + 1, else all
  * keys_b. A row that sees nothing, and every row from q_lens[b] on, is 0 with

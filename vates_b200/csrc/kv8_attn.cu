@@ -6,8 +6,9 @@
 // The codes are exact in f16 and so are the queries after a power of two per
 // row, so q . code runs on f16 tensor-core products with float32 sums; the
 // scales are applied to the sums. The weights are rounded to f16 (11 bits)
-// after a factor s_V(page) / v, v the largest V scale so far; l is summed in
-// float32 from the unrounded weights.
+// after a factor s_V(page) / v, v the largest V scale so far: the codes are f16, so the
+// weights have to be; an eighth of what out loses to bf16. l is summed in float32
+// from the unrounded weights.
 //
 // A CTA (4 warps, two or three CTAs per SM) owns an equal share of all sequences' key
 // tiles (16 KB of K and of V each) and all query rows, up to 32, of the kv head
@@ -30,8 +31,10 @@
 // What bounds it: one row over 131,072 keys, 16/2 heads of 256, takes 37.7 us for 134
 // MB (3.6 TB/s; a copy 20.8): in the middle HBM is at 0.85 of a copy, the start and
 // the joining of 222 partial results take the rest. 16 sequences x 4 rows over up to
-// 8,190 keys, 32/8 heads of 128: 49 us for 127 MB, bound by instructions (issue 50 %
-// with the 12 warps that registers and the rings leave room for).
+// 8,190 keys, 32/8 heads of 128: 49 us for 127 MB (a copy 19.7), bound by latency:
+// with the 12 warps that registers and the rings leave room for, issue slots are half
+// used and HBM at a third; warps wait for products, shared memory and each other. With
+// 32 rows (8 warps): 16 sequences of 8,190 keys 103 us for 268 MB.
 #include "kv8_attn.cuh"
 
 namespace vb {
@@ -851,6 +854,10 @@ int kv8_ranges(long long base, long long tiles) {
   return best;
 }
 
+// The plan follows from the table's width (lengths are on the device): the times below
+// are of tables as long as their sequences. In a table for 131,072 positions one row
+// over 901 keys takes 8.8 us on the device (11.4 in one for 901), 512 rows over 512
+// keys of 16/2 heads of 256 49.7 us (18.5), over 8,192 keys 116 (79).
 // Up to 32 rows per kv head: kv8_attn_kernel, 8, 16 or 32 rows, its CTAs on
 // each of 148 SMs (fewer when the table holds fewer tiles). More rows: the
 // tcgen05 kernel, a pair of CTAs per two SMs. (32 rows: 16 sequences of 8,190 keys, 8
@@ -912,8 +919,8 @@ int kv8_launch(const Kv8AttnParams &p, int ctas, cudaStream_t s) {
   });
   if (rc != VB_OK) return rc;
   // Dependent launch for short calls only: started before the kernel ahead has
-  // left its SMs, a full grid is placed unevenly (131,072 keys: 53 us instead of
-  // 41; 901 keys: 15.0 us instead of 16.3).
+  // left its SMs, a full grid is placed unevenly (131,072 keys: 49.6 us instead of
+  // 37.7; 901 keys: 12.1 us instead of 14.1).
   vb_launch(kv8_attn_kernel<D, NR>, dim3(ctas), dim3(KA_THREADS), T::SMEM, s, ctas <= 148, p);
   return check_launch("kv8_attn_kernel");
 }

@@ -24,7 +24,8 @@
 //     tile needs of the one before it is the running maximum, which is handed
 //     over before the exponentials. It only moves when it grows by more than 2^9
 //     (then O is rescaled), and P = 2^(z - m) s_V / v goes over S in TMEM as the
-//     f16 A operand of the second product. v is a power of two at least every V
+//     f16 A operand of the second product (the codes are f16, so the weights have to
+//     be; an eighth of what out loses to bf16). v is a power of two at least every V
 //     scale so far. l is summed in float32 from the unrounded weights.
 // A wait names the n-th completion of a barrier by its parity alone, so when it
 // begins, completion n - 1 must have happened and n + 1 must not: S of a tile
