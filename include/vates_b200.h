@@ -527,8 +527,8 @@ typedef struct VbKv8Cache {
 /* Quantise bf16 rows as they are written: row i < counts[b] (nullable: n) of
  * sequence b goes to position pos[b] + pos_add + i. A page's scale is
  * max|x| / 127 (at least 2^-40; 0 while every value is 0) over all rows written
- * since its first row; when it grows, the older rows of the page are rewritten
- * as rint(code * old / new). Positions read on the device. Infinities are
+ * since its first row (rows that are written over later among them); when it
+ * grows, the older rows of the page are rewritten as rint(code * old / new). Positions read on the device. Infinities are
  * stored as +-127 * scale, NaN as 0, and flag VB_STATUS_NONFINITE. keys and
  * values [batch, kv_heads, n, dim] with element strides {batch, head, row} and
  * contiguous dims. */

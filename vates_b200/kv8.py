@@ -137,7 +137,10 @@ class PagedKV8Cache:
         without ``counts``) of ``keys``/``values`` bf16 ``[batch, kv_heads, n,
         head_dim]`` goes to position ``pos[b] + pos_add + i``. A page's scale is
         max|x| / 127 over the rows it received; when new rows raise it, the
-        page's older codes are rounded again under the new scale. Rows past the
+        page's older codes are rounded again under the new scale. Writing again
+        from an earlier position (rows taken back) keeps the scale that the
+        rows taken back gave the page, unless it starts at the page's first
+        row. Rows past the
         table set VB_STATUS_BOUNDS in ``status`` and are dropped; an infinity is
         stored as the page's largest value, a NaN as 0, with
         VB_STATUS_NONFINITE."""

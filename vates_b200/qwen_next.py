@@ -229,7 +229,9 @@ class QwenNextModel:
     """The main model, its MTP head and the device state of the speculative
     loop. ``max_tokens`` (<= 8) is the largest row count of one forward.
     ``kv``: the cache of the full-attention layers, "isoquant" (K4/V3) or "kv8"
-    (int8 pages, :class:`vates_b200.kv8.PagedKV8Cache`)."""
+    (int8 pages, :class:`vates_b200.kv8.PagedKV8Cache`; a rejected draft may
+    leave its page a larger scale, so where logits are close the tokens can depend
+    on the drafts)."""
 
     def __init__(self, cfg: QwenNextConfig, seed: int = 4, cache_len: int = 8192,
                  verify_len: int = 4, drafts: int = 3, device="cuda", out_cap: int = 65536,
