@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import (VbKv8AppendArgs, VbKv8AttnArgs, VbKv8Cache, VbKv8ReadArgs, check, lib)
-from .pool import current_device, on_device, ptr, status_ptr, stream_handle
+from .pool import current_device, current_stream, on_device, ptr, status_ptr
 from .scratch import Scratch
 
 PAGE_SIZES = (16, 32, 64, 128)
@@ -156,8 +156,10 @@ class PagedKV8Cache:
         a.keys, a.values = keys.data_ptr(), values.data_ptr()
         a.k_strides, a.v_strides = _strides(keys), _strides(values)
         a.pos, a.counts = _ints(pos, "pos", B, dev), _ints(counts, "counts", B, dev)
-        a.status, a.pos_add, a.n = status_ptr(status, dev), pos_add, n
-        check(lib.vb_kv8_append(C.byref(a), stream_handle()), "vb_kv8_append")
+        a.pos_add, a.n = pos_add, n
+        if status is not None:
+            a.status = status_ptr(status, dev)
+        check(lib.vb_kv8_append(C.byref(a), current_stream(dev)), "vb_kv8_append")
 
     # -------------------------------------------------------------- read back
     def read(self, lens, n: int, start=None, status=None, stream=None):
@@ -174,8 +176,10 @@ class PagedKV8Cache:
         a = VbKv8ReadArgs.from_buffer_copy(self._read_args)
         a.lens, a.start = _ints(lens, "lens", B, dev), _ints(start, "start", B, dev)
         a.keys, a.values = keys.data_ptr(), values.data_ptr()
-        a.status, a.n = status_ptr(status, dev), n
-        check(lib.vb_kv8_read(C.byref(a), stream_handle()), "vb_kv8_read")
+        a.n = n
+        if status is not None:
+            a.status = status_ptr(status, dev)
+        check(lib.vb_kv8_read(C.byref(a), current_stream(dev)), "vb_kv8_read")
         return keys, values
 
     # -------------------------------------------------------------- attention
@@ -208,13 +212,15 @@ class PagedKV8Cache:
         a = VbKv8AttnArgs.from_buffer_copy(self._attn_args)
         a.q, a.q_strides = q.data_ptr(), _strides(q)
         a.lens, a.q_lens = _ints(lens, "lens", B, dev), _ints(q_lens, "q_lens", B, dev)
-        a.out, a.lse, a.status = out.data_ptr(), ptr(lse), status_ptr(status, dev)
+        a.out, a.lse = out.data_ptr(), ptr(lse)
+        if status is not None:
+            a.status = status_ptr(status, dev)
         a.scale = D ** -0.5 if scale is None else scale
         a.q_heads, a.L, a.len_add, a.causal = Hq, L, len_add, causal
         need = self._need.get((Hq, L))
         if need is None:
             need = self._need[Hq, L] = lib.vb_kv8_attn_workspace_size(C.byref(a))
-        st = stream_handle()
+        st = current_stream(dev)
         if need:
             ws = _scratch.get(need, self.device, st)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()

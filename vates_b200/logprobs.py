@@ -8,7 +8,7 @@ from typing import NamedTuple
 import torch
 
 from ._lib import VB_TOKEN_LOGPROBS_WORKSPACE_HEAD, VbTokenLogprobsArgs, check, lib
-from .pool import current_device, on_device, status_ptr, stream_handle
+from .pool import current_device, current_stream, on_device, status_ptr
 from .scratch import Scratch
 
 MAX_TOP = 32
@@ -57,7 +57,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     rank = torch.empty_like(tokens)
     tlp = lp.new_empty((rows, top))
     ids = rank.new_empty((rows, top))
-    st = stream_handle()
+    st = current_stream(dev)
     need = _needs.get((rows, vocab, top))
     if need is None:
         if len(_needs) > 4096:
@@ -66,7 +66,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
             1 << 16, lib.vb_token_logprobs_workspace_size(rows, vocab, top))
     ws = _scratch.get(need, logits.device, st)
     a = VbTokenLogprobsArgs(logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(),
-                            rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), status_ptr(status, dev),
+                            rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(),
+                            None if status is None else status_ptr(status, dev),
                             ws.data_ptr(), ws.numel(), logits.stride(0), temperature, rows, vocab,
                             top, _DTYPES[logits.dtype])
     check(lib.vb_token_logprobs(C.byref(a), st), "vb_token_logprobs")

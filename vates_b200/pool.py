@@ -21,10 +21,14 @@ KEYS = ("gate_w", "gate_s", "gate_b", "up_w", "up_s", "up_b",
         "down_w", "down_s", "down_b")
 
 
+# the current device, and the handle of its current stream, without building objects
+current_device = torch._C._cuda_getDevice
+current_stream = torch._C._cuda_getCurrentRawStream
+
+
 def stream_handle(stream=None) -> int:
     if stream is None:
-        # the handle of torch.cuda.current_stream() without building its object
-        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+        return current_stream(current_device())
     return stream.cuda_stream
 
 
@@ -32,10 +36,8 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def status_ptr(t, device: int) -> int | None:
-    """Pointer of an optional status word, an int32 tensor on GPU ``device``."""
-    if t is None:
-        return None
+def status_ptr(t: torch.Tensor, device: int) -> int:
+    """Pointer of a status word, an int32 tensor on GPU ``device``."""
     if t.dtype != torch.int32 or t.get_device() != device or t.numel() < 1:
         raise ValueError(f"status: an int32 tensor on cuda:{device} is needed, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
@@ -50,9 +52,6 @@ def on_device(device: torch.device, stream):
     if stream.device != device:
         raise ValueError(f"stream on {stream.device}, tensors on {device}")
     return torch.cuda.stream(stream)
-
-
-current_device = torch._C._cuda_getDevice
 
 
 def blob_layout(hidden: int, inter: int, bits: int, group: int):
