@@ -240,3 +240,15 @@ def test_scores_of_any_size(cuda, L, rep, keys, dim, page, power):
     zt = z.max(1).reshape(rep, L)
     # float32 sums of dim products and three float32 steps
     assert (np.abs(lse[0].cpu().numpy() - zt) <= zt * (dim * 2.0 ** -24 + 2.0 ** -21)).all()
+
+
+@both
+def test_scales_below_float32s_normal_numbers(cuda, L, rep, keys, dim, page):
+    """They read as 0 or as what they are: nothing but numbers as small comes out."""
+    c, q = setup(L, rep, keys, dim, page)
+    for tiny in (2.0 ** -149, 2.0 ** -130, 2.0 ** -126):
+        c.v_scales.fill_(tiny)
+        c.k_scales.fill_(tiny)
+        out, lse = c.attend(q.cuda(), ints([keys]), causal=False, return_lse=True)
+        assert (out.abs().float() <= 128 * tiny).all()
+        assert (lse - math.log(keys)).abs().max() <= 2.0 ** -17

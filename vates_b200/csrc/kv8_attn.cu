@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
           }
         __syncthreads();
         const float vnew = fmaxf(vref, vmax);
-        vinv = vnew > 0.f ? __frcp_rn(vnew) : 0.f;
+        vinv = vnew >= 1.1754944e-38f ? __frcp_rn(vnew) : 0.f;  // (below 2^-126: read as 0)
         const float vold = vref * vinv;
         vref = vnew;
 #pragma unroll
