@@ -73,6 +73,24 @@ def test_a_capture_without_a_number_shares_nothing(capture, monkeypatch):
     assert s.get(50, CPU, 1) is not s.get(50, CPU, 1)
 
 
+def test_buffers_of_captures_are_let_go(capture):
+    """A graph's pool keeps its memory: what is held here is the last capture's, and
+    that only until the next eager call. (A capture that is under way then takes
+    another buffer, which it fills again.)"""
+    s = Scratch(16)
+    for capture["id"] in (3, 4):
+        for st in (1, 2):
+            s.get(50, CPU, st)
+    assert len(s._captured) == 2 and s._capture == 4
+    a = s.get(50, CPU, 1)
+    capture["id"] = 0
+    s.get(50, CPU, 9)
+    assert not s._captured
+    capture["id"] = 4
+    b = s.get(50, CPU, 1)
+    assert b is not a and not b[:16].any()
+
+
 def test_the_default_stream_is_not_asked(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: 1 / 0)
     s = Scratch(16)

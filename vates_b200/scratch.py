@@ -22,19 +22,25 @@ class Scratch:
     def __init__(self, head: int = 0):
         self.head = head
         self._eager: dict = {}
-        self._captured: dict = {}  # (device, stream) -> (capture, buffer) of the last capture
+        self._capture = 0          # the capture that the buffers below belong to
+        self._captured: dict = {}
 
     def get(self, nbytes: int, device, st: int) -> torch.Tensor:
         """At least ``nbytes`` for a call on ``st``, the current stream."""
         # (the default stream, handle 0, cannot be captured)
         if st and torch.cuda.is_current_stream_capturing():
             capture = lib.vb_stream_capture_id(st)
-            held, buf = self._captured.get((device, st), (None, None))
-            if not capture or held != capture or buf.numel() < nbytes:
+            if not capture or capture != self._capture:
+                self._captured.clear()
+                self._capture = capture
+            buf = self._captured.get((device, st))
+            if buf is None or buf.numel() < nbytes:
                 buf = torch.empty(max(nbytes, self.head), dtype=torch.uint8, device=device)
                 buf[:self.head or nbytes].zero_()
-                self._captured[device, st] = capture, buf
+                self._captured[device, st] = buf
             return buf
+        if self._captured:  # the graphs' pools keep them now
+            self._captured.clear()
         buf = self._eager.get((device, st))
         if buf is None or buf.numel() < nbytes:
             buf = torch.zeros(max(nbytes, self.head), dtype=torch.uint8, device=device)
