@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from test_gpu_kv8 import bf16, ints, make_cache
+from vates_b200 import _lib
 from vates_b200.logprobs import token_logprobs
 
 pytestmark = pytest.mark.gpu
@@ -169,3 +170,24 @@ def test_moe_block_graph_outlives_a_larger_call(cuda):
             torch.cuda.synchronize()
             assert torch.equal(out, want1) and int(status) == 0
         assert all(bool((t == 0x5A).all()) for t in taken)
+
+
+def test_callers_workspace(cuda):
+    rng = np.random.default_rng(3)
+    c = make_cache(rng, 3, 8, 128, 32, 96)
+    for L in (1, 40):
+        q = bf16(rng, (3, 16, L, 128)).cuda()
+        lens = ints([3000, 2000, 1000])
+        want = c.attend(q, lens)
+        need = c.attend_workspace_size(16, L)
+        ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        for stream in (None, side):
+            assert torch.equal(c.attend(q, lens, workspace=ws, stream=stream), want)
+            torch.cuda.synchronize()
+        with pytest.raises(_lib.VbError, match="workspace"):
+            c.attend(q, lens, workspace=ws[:need - 1])
+        for bad in (ws.cpu(), ws.view(torch.int8)):
+            with pytest.raises(ValueError, match="workspace"):
+                c.attend(q, lens, workspace=bad)

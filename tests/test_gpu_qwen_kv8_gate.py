@@ -1,4 +1,5 @@
-"""Output gate of the decode stack's attention over the 8-bit cache, against float64."""
+"""The decode stack's attention over the 8-bit cache: its output gate against the exact
+sigmoid, and the scratch that it uses."""
 import numpy as np
 import pytest
 
@@ -40,3 +41,24 @@ def test_layer_gate_vs_float64(cuda):
             hit |= got == (o * f).bfloat16()
         assert hit.all()
         assert np.abs(gate).max() > 1 and s.std() > 0.1
+
+
+def test_one_workspace_for_all_layers_and_graphs(cuda, monkeypatch):
+    """The model's attention takes its scratch from the model, in every graph, and
+    leaves the ticket words zero."""
+    import torch
+    from vates_b200 import _lib, kv8
+    from vates_b200.qwen_next import QwenNextModel, tiny_config
+    model = QwenNextModel(tiny_config(), seed=4, cache_len=4096, verify_len=4, drafts=3, kv="kv8")
+    ids = np.random.default_rng(1).integers(0, model.cfg.vocab, 203).astype(np.int32)
+    want, _ = model.generate(ids, 12, use_graphs=False)
+
+    class Closed:
+        def get(self, *a):
+            raise AssertionError("scratch of the module")
+
+    monkeypatch.setattr(kv8, "_scratch", Closed())
+    got, stats = model.generate(ids, 12)
+    assert np.array_equal(got, want) and stats["status"] == 0
+    torch.cuda.synchronize()
+    assert not model.kv8_ws[:_lib.VB_KV8_ATTN_WORKSPACE_HEAD].any()

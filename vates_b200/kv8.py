@@ -184,19 +184,23 @@ class PagedKV8Cache:
 
     # -------------------------------------------------------------- attention
     def attend(self, q, lens, q_lens=None, len_add: int = 0, scale: float | None = None,
-               causal: bool = True, out=None, return_lse: bool = False, status=None, stream=None):
+               causal: bool = True, out=None, return_lse: bool = False, status=None, stream=None,
+               workspace=None):
         """``softmax(scale * q K^T) V`` over the ``lens[b] + len_add`` keys of
         every sequence. ``q`` bf16 ``[batch, q_heads, L, head_dim]``; query row
         ``i < q_lens[b]`` (``L`` without) is the sequence's row ``keys - q_lens
         + i`` and with ``causal`` sees the keys up to itself. Rows that see
         nothing, and rows from ``q_lens[b]`` on, are zero (log-sum-exp -inf).
         Returns bf16 ``[batch, q_heads, L, head_dim]``, with ``return_lse``
-        also float32 ``[batch, q_heads, L]`` (natural log)."""
+        also float32 ``[batch, q_heads, L]`` (natural log). ``workspace``: the
+        caller's scratch (:meth:`attend_workspace_size` bytes, uint8, zeros
+        before its first call) for calls that never overlap, in graphs or not;
+        without it a call finds its own."""
         # with it as the current stream, results belong to it
         if stream is not None or current_device() != self._index:
             with on_device(self.device, stream):
                 return self.attend(q, lens, q_lens, len_add, scale, causal, out, return_lse,
-                                   status)
+                                   status, workspace=workspace)
         B, D, dev = self.batch, self.head_dim, self._index
         if q.dim() != 4:
             raise ValueError(f"q: [batch, q_heads, L, head_dim] is needed, got {tuple(q.shape)}")
@@ -221,11 +225,24 @@ class PagedKV8Cache:
         if need is None:
             need = self._need[Hq, L] = lib.vb_kv8_attn_workspace_size(C.byref(a))
         st = current_stream(dev)
-        if need:
+        if workspace is not None:
+            if workspace.dtype != torch.uint8 or workspace.get_device() != dev \
+                    or not workspace.is_contiguous():
+                raise ValueError(f"workspace: contiguous uint8 on cuda:{dev} is needed, got "
+                                 f"{workspace.dtype} on {workspace.device}")
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        elif need:
             ws = _scratch.get(need, self.device, st)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         check(lib.vb_kv8_attn(C.byref(a), st), "vb_kv8_attn")
         return (out, lse) if return_lse else out
+
+    def attend_workspace_size(self, q_heads: int, L: int) -> int:
+        """Bytes of scratch that :meth:`attend` needs for ``L`` rows of
+        ``q_heads`` heads with the present page table."""
+        a = VbKv8AttnArgs.from_buffer_copy(self._attn_args)
+        a.q_heads, a.L = q_heads, L
+        return lib.vb_kv8_attn_workspace_size(C.byref(a))
 
 
 __all__ = ["PagedKV8Cache"]

@@ -315,6 +315,12 @@ class QwenNextModel:
         self.attn_ws = torch.zeros(
             lib.vb_kv_attn_workspace_size(1, cfg.q_heads, T, D, cap) + 256, dtype=torch.uint8,
             device=dev)
+        if self.kv == "kv8":  # one for all layers and graphs, which run one after another
+            paged = [l.mixer.cache for l in self.layers
+                     if isinstance(getattr(l.mixer, "cache", None), PagedKV8Cache)]
+            self.kv8_ws = torch.zeros(max([1] + [c.attend_workspace_size(cfg.q_heads, t)
+                                                 for c in paged for t in range(1, T + 1)]),
+                                      dtype=torch.uint8, device=dev)
         self.argmax_ws = torch.zeros(max(lib.vb_argmax_workspace_size(T), 16),
                                      dtype=torch.uint8, device=dev)
         need = lib.vb_moe_decode_workspace_size(T, cfg.hidden, cfg.inter, cfg.experts,
@@ -398,7 +404,8 @@ class QwenNextModel:
             m.cache.append(rows("krow", cfg.kv_heads), rows("vrow", cfg.kv_heads), pos,
                            pos_add=pos_add, status=b["status"], stream=st)
             m.cache.attend(rows("q", cfg.q_heads), pos, len_add=T + pos_add,
-                           out=rows("attn", cfg.q_heads), status=b["status"], stream=st)
+                           out=rows("attn", cfg.q_heads), status=b["status"], stream=st,
+                           workspace=self.kv8_ws)
             check(lib.vb_attn_gate(b["attn"].data_ptr(), b["proj"].data_ptr(), cfg.attn_proj, T,
                                    cfg.q_heads, b["gout"].data_ptr(), stream_handle(st)),
                   "vb_attn_gate")
