@@ -184,8 +184,9 @@ def test_callers_workspace(cuda):
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         for stream in (None, side):
-            assert torch.equal(c.attend(q, lens, workspace=ws, stream=stream), want)
-            torch.cuda.synchronize()
+            got = c.attend(q, lens, workspace=ws, stream=stream)
+            torch.cuda.synchronize()  # (results on another stream than the comparison's)
+            assert torch.equal(got, want)
         with pytest.raises(_lib.VbError, match="workspace"):
             c.attend(q, lens, workspace=ws[:need - 1])
         for bad in (ws.cpu(), ws.view(torch.int8)):
