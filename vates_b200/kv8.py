@@ -69,8 +69,9 @@ def _strides(t: torch.Tensor):
 class PagedKV8Cache:
     """One layer's cache. The tensors are the caller's (or :meth:`empty`'s) and
     may be shared between caches with different tables; a page that is written
-    must belong to one sequence only. The table may be edited in place or
-    replaced (:attr:`page_table`) between calls."""
+    must belong to one sequence only. Scales are finite and not negative. The
+    table may be edited in place or replaced (:attr:`page_table`) between calls;
+    a CUDA graph keeps reading the one it was captured with."""
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales, page_table):
         if k_codes.dim() != 4:
@@ -103,7 +104,8 @@ class PagedKV8Cache:
         if t.dim() != 2 or t.dtype != torch.int32 or not t.is_contiguous() \
                 or t.device != self.device:
             raise ValueError("page_table: a contiguous int32 [batch, max_pages] tensor on "
-                             f"{self.device} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+                             f"{self.device} is needed, got {t.dtype} {tuple(t.shape)} on "
+                             f"{t.device}")
         self._table = t
         self.batch = t.shape[0]
         # argument structures with the cache filled in, copied for each call
