@@ -590,6 +590,28 @@ size_t vb_kv8_attn_workspace_size(const VbKv8AttnArgs *args);
 int vb_kv8_attn(const VbKv8AttnArgs *args, vb_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Rotary positions with several axes (no reference counterpart): q and k bf16
+ * [batch, heads, L, dim] (element strides {batch, head, row}, contiguous dims),
+ * the first rope_dims dims of every row rotated in pairs (i, i + rope_dims / 2) by
+ * positions[axis[i]][b][t] * turns[i] turns, after an RMS norm with weight
+ * q_norm / k_norm (nullable, bf16 [dim]). float32, rounded once. turns and axis
+ * [rope_dims / 2] are host memory, read before the call returns. An output may
+ * be its input; dim 16 to 256 and rope_dims multiples of 16.
+ * ------------------------------------------------------------------------- */
+typedef struct VbRotateArgs {
+  const uint16_t *q, *k;
+  uint16_t *q_out, *k_out;
+  const uint16_t *q_norm, *k_norm;
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3];
+  const int32_t *positions; /* [axes, batch, L] */
+  const double *turns;      /* frequency / 2 pi */
+  const uint8_t *axis;      /* below axes */
+  float eps;
+  int32_t batch, L, q_heads, kv_heads, dim, rope_dims, axes;
+} VbRotateArgs;
+int vb_rotate_axes(const VbRotateArgs *args, vb_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Log probabilities of given tokens (no reference counterpart). Per row of
  * logits [rows, vocab] (dtype 0 = bf16, 1 = float32; row_stride elements):
  *   logprob = x_t / T - lse,   lse = log sum_j exp(x_j / T)

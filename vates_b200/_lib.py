@@ -70,6 +70,17 @@ class VbKv8AttnArgs(C.Structure):
                 ("L", C.c_int32), ("len_add", C.c_int32), ("causal", C.c_int32)]
 
 
+class VbRotateArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_out", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("q_strides", C.c_int64 * 3), ("k_strides", C.c_int64 * 3),
+                ("q_out_strides", C.c_int64 * 3), ("k_out_strides", C.c_int64 * 3),
+                ("positions", C.c_void_p), ("turns", C.c_void_p), ("axis", C.c_void_p),
+                ("eps", C.c_float), ("batch", C.c_int32), ("L", C.c_int32),
+                ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32),
+                ("rope_dims", C.c_int32), ("axes", C.c_int32)]
+
+
 class VbTokenLogprobsArgs(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("tokens", C.c_void_p), ("logprob", C.c_void_p),
                 ("entropy", C.c_void_p), ("rank", C.c_void_p), ("top_ids", C.c_void_p),
@@ -187,6 +198,7 @@ _SIGNATURES = {
     "vb_kv8_read": (_I32, [C.POINTER(VbKv8ReadArgs), _P]),
     "vb_kv8_attn_workspace_size": (_SZ, [C.POINTER(VbKv8AttnArgs)]),
     "vb_kv8_attn": (_I32, [C.POINTER(VbKv8AttnArgs), _P]),
+    "vb_rotate_axes": (_I32, [C.POINTER(VbRotateArgs), _P]),
     "vb_token_logprobs_workspace_size": (_SZ, [_I32, _I32, _I32]),
     "vb_token_logprobs": (_I32, [C.POINTER(VbTokenLogprobsArgs), _P]),
     "vb_res_create": (_P, [_I32, _I32, _I32, _I32, _I32]),

@@ -38,6 +38,7 @@ SOURCES = [
     "kv8_attn.cu",
     "kv8_prefill.cu",
     "logprobs.cu",
+    "rotary.cu",
 ]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

@@ -1,0 +1,130 @@
+"""Rotary positions with several axes (time, height, width of images and video)
+for tokens whose positions are given (``vb_rotate_axes``), with the RMS norm of
+q and k that some models have before it.
+
+Attention over a cache does not care in which row a key lies, so once rows have
+been evicted (:meth:`vates_b200.kv8.PagedKV8Cache.evict`) the position of a new
+token is no longer the row it is written to: it is given here instead.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from ._lib import VbRotateArgs, check, lib
+from .pool import current_device, current_stream, on_device, ptr
+
+_TABLES: dict = {}
+_STRIDES: dict = {}
+
+
+def pair_axes(sections, interleaved: bool = False) -> tuple:
+    """The axis of every rotated pair from the number of pairs per axis: one
+    section after another, or, ``interleaved``, dealt out in turn (0, 1, 2, 0,
+    1, 2, ...) for as long as an axis has pairs left."""
+    sections = [int(n) for n in sections]
+    if any(n < 0 for n in sections):
+        raise ValueError(f"sections={sections}: pairs per axis, none negative")
+    if not interleaved:
+        return tuple(a for a, n in enumerate(sections) for _ in range(n))
+    return tuple(a for i in range(max(sections, default=0))
+                 for a, n in enumerate(sections) if i < n)
+
+
+def _table(axes: tuple, base: float):
+    """C arrays of the pairs' axes and of their frequencies in turns."""
+    t = _TABLES.get((axes, base))
+    if t is None:
+        n = len(axes)
+        if not 1.0 < base < math.inf:
+            raise ValueError(f"base={base}: a finite number above 1 is needed")
+        if n > 128 or n % 8 or n == 0 or any(not 0 <= a < 255 for a in axes):
+            raise ValueError(f"axes: one axis (0 to 254) per pair, a multiple of 8 of them and at "
+                             f"most 128, got {n}")
+        if len(_TABLES) > 256:
+            _TABLES.clear()
+        t = _TABLES[axes, base] = (
+            (C.c_uint8 * n)(*axes),
+            (C.c_double * n)(*[base ** (-i / n) / (2.0 * math.pi) for i in range(n)]),
+            max(axes) + 1)
+    return t
+
+
+def _strides(t: torch.Tensor):
+    s = t.stride()
+    a = _STRIDES.get(s)
+    if a is None:
+        if len(_STRIDES) > 4096:
+            _STRIDES.clear()
+        a = _STRIDES[s] = (C.c_int64 * 3)(*s[:3])
+    return a
+
+
+def _check(t: torch.Tensor, what: str, shape, dev: int):
+    if t.dtype != torch.bfloat16 or t.get_device() != dev or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: bfloat16 {tuple(shape)} on cuda:{dev} is needed, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+
+
+def _out(t: torch.Tensor, out: torch.Tensor | None, what: str, dev: int) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    _check(out, what, t.shape, dev)
+    if out.stride(3) != 1:
+        raise ValueError(f"{what}: contiguous dims are needed, strides {out.stride()}")
+    return out
+
+
+def rotate_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes,
+                base: float = 10_000_000.0, q_norm=None, k_norm=None, eps: float = 1e-6,
+                q_out=None, k_out=None, stream=None):
+    """``(q, k)`` with the first ``2 len(axes)`` dims of every row rotated: pair
+    ``(i, i + len(axes))`` of token ``t`` of sequence ``b`` by the angle
+    ``positions[axes[i], b, t] * base ** (-i / len(axes))``.
+
+    ``q`` bf16 ``[batch, heads, L, dim]`` and ``k`` ``[batch, kv_heads, L, dim]``
+    (any strides with contiguous dims, a projection's layout for one); ``dim`` a
+    multiple of 16, at most 256. ``positions`` int32 ``[axes, batch, L]``, any
+    values; ``axes`` the axis of every pair (:func:`pair_axes`), a multiple of 8
+    pairs. ``q_norm``, ``k_norm`` bf16 ``[dim]``: rows are RMS-normalised and
+    multiplied by it first. Float32 throughout, rounded to bf16 once. Results are
+    new contiguous tensors, or ``q_out`` and ``k_out``, which may be ``q`` and
+    ``k`` themselves but must not overlap them in any other way."""
+    dev = q.get_device()
+    # with it as the current stream, results belong to it
+    if dev >= 0 and (stream is not None or current_device() != dev):
+        with on_device(q.device, stream):
+            return rotate_axes(q, k, positions, axes, base, q_norm, k_norm, eps, q_out, k_out)
+    if q.dim() != 4 or k.dim() != 4 or dev < 0:
+        raise ValueError("q, k: CUDA [batch, heads, L, dim] are needed, got "
+                         f"{tuple(q.shape)} and {tuple(k.shape)} on {q.device}")
+    B, Hq, L, D = q.shape
+    Hk = k.shape[1]
+    _check(q, "q", q.shape, dev)
+    _check(k, "k", (B, Hk, L, D), dev)
+    axis, turns, least = _table(axes if type(axes) is tuple else tuple(int(a) for a in axes), base)
+    if positions.dtype != torch.int32 or positions.get_device() != dev \
+            or positions.dim() != 3 or tuple(positions.shape[1:]) != (B, L) \
+            or positions.shape[0] < least or not positions.is_contiguous():
+        raise ValueError(f"positions: contiguous int32 [axes >= {least}, {B}, {L}] on cuda:{dev} "
+                         f"is needed, got {positions.dtype} {tuple(positions.shape)} on "
+                         f"{positions.device}")
+    for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None:
+            _check(w, what, (D,), dev)
+            if not w.is_contiguous():
+                raise ValueError(f"{what}: a contiguous tensor is needed")
+    q_out, k_out = _out(q, q_out, "q_out", dev), _out(k, k_out, "k_out", dev)
+    q = q if q.stride(3) == 1 else q.contiguous()
+    k = k if k.stride(3) == 1 else k.contiguous()
+    a = VbRotateArgs(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), ptr(q_norm),
+                     ptr(k_norm), _strides(q), _strides(k), _strides(q_out), _strides(k_out),
+                     positions.data_ptr(), C.cast(turns, C.c_void_p), C.cast(axis, C.c_void_p),
+                     eps, B, L, Hq, Hk, D, 2 * len(axis), positions.shape[0])
+    check(lib.vb_rotate_axes(C.byref(a), current_stream(dev)), "vb_rotate_axes")
+    return q_out, k_out
+
+
+__all__ = ["pair_axes", "rotate_axes"]
