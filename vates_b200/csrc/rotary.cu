@@ -16,8 +16,9 @@ namespace {
 
 constexpr int RT_THREADS = 256;
 constexpr int RT_PAIRS = 128;      // most rotated pairs of a row
-constexpr int RT_TABLE = 1024;     // (token, pair) sines and cosines of a CTA
-constexpr int RT_AHEAD = 4;        // rows that a thread has in flight
+constexpr int RT_TABLE = 2048;     // (token, pair) sines and cosines of a CTA
+constexpr int RT_TOKENS = 32;      // most tokens of a CTA
+constexpr int RT_AHEAD = 2;        // rows that a thread has in flight
 
 struct RotateParams {
   const uint16_t *src[2];          // q, k
@@ -26,22 +27,21 @@ struct RotateParams {
   int64_t s_in[2][3], s_out[2][3]; // element strides of batch, head, row
   const int32_t *positions;        // [axes][tokens]
   int64_t tokens;                  // batch * L
-  int L, heads[2], dim, half, per; // per: tokens of a CTA
+  int L, heads[2], dim, half, per, groups;  // tokens of a CTA, CTAs of a sequence
   float eps;
   bool keep;                       // dims from R on are in place already
   double turns[RT_PAIRS];          // frequency / 2 pi
   uint8_t axis[RT_PAIRS];
 };
 
-__device__ __forceinline__ void rt_load(float (&x)[8], const uint16_t *p, bool vec) {
-  uint32_t w[4];
-  if (vec) {
-    const uint4 v = ldg_v4(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = p[2 * j] | ((uint32_t)p[2 * j + 1] << 16);
-  }
+// 8 bf16
+__device__ __forceinline__ uint4 rt_load(const uint16_t *p, bool vec) {
+  if (vec) return ldg_v4(p);
+  return make_uint4(p[0] | ((uint32_t)p[1] << 16), p[2] | ((uint32_t)p[3] << 16),
+                    p[4] | ((uint32_t)p[5] << 16), p[6] | ((uint32_t)p[7] << 16));
+}
+__device__ __forceinline__ void rt_floats(float (&x)[8], const uint4 &v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     x[2 * j] = __uint_as_float(w[j] << 16);
@@ -64,74 +64,84 @@ __device__ __forceinline__ void rt_store(uint16_t *p, const float (&x)[8], bool 
 }
 
 // LPR lanes hold a row, 16 dims each: the first R / 16 of them 8 pairs, the
-// others 16 dims that only the norm changes. A CTA makes the sines of its tokens
-// and then goes through their rows, all heads of a token one after another.
+// others 16 dims that only the norm changes. A CTA takes some tokens of one
+// sequence, all heads: it makes their sines once, and then goes through the rows
+// head by head, so that what it writes to [batch, heads, L, dim] is contiguous.
 template <int LPR, bool NORM>
-__global__ void __launch_bounds__(RT_THREADS) rotate_kernel(const __grid_constant__ RotateParams p,
+__global__ void __launch_bounds__(RT_THREADS, 4) rotate_kernel(const __grid_constant__ RotateParams p,
                                                             bool vec) {
-  __shared__ float2 s_cs[RT_TABLE];
+  __shared__ float2 s_cs[RT_TABLE];  // [token][pair % 8][pair / 8]
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, heads = p.heads[0] + p.heads[1];
-  const int64_t t0 = (int64_t)blockIdx.x * p.per;
-  const int n = (int)min((int64_t)p.per, p.tokens - t0);
+  const int tid = threadIdx.x;
+  const int b = blockIdx.x / p.groups, i0 = (blockIdx.x - b * p.groups) * p.per;
+  const int n = min(p.per, p.L - i0);
+  const uint32_t n_inv = (uint32_t)(0xFFFFFFFFu / n) + 1;  // r / n for r * n < 2^32; n = 1: 0
   const int j = tid % LPR, turned = p.half >> 3;
   // dims of this lane: two runs of eight
   const int d0 = j < turned ? j * 8 : 2 * p.half + (j - turned) * 16;
   const int d1 = j < turned ? p.half + j * 8 : d0 + 8;
   const bool live = j * 16 < p.dim && !(p.keep && j >= turned);
   constexpr int STEP = RT_THREADS / LPR;
-  const int rows = n * heads;
-  bool ready = false;
-  for (int r0 = tid / LPR; r0 - tid / LPR < rows; r0 += STEP * RT_AHEAD) {
-    float a[RT_AHEAD][8], b[RT_AHEAD][8];
+  const int rows = n * (p.heads[0] + p.heads[1]);
+  // row r: token, q (0) or k (1), and head
+  auto place = [&](int r, int &t, int &kind, int &h) {
+    const int hh = n == 1 ? r : (int)__umulhi((uint32_t)r, n_inv);
+    t = r - hh * n;
+    kind = hh >= p.heads[0];
+    h = kind ? hh - p.heads[0] : hh;
+  };
+  auto fetch = [&](int r0, uint4 (&x)[RT_AHEAD], uint4 (&y)[RT_AHEAD]) {
 #pragma unroll
     for (int k = 0; k < RT_AHEAD; ++k) {
       const int r = r0 + k * STEP;
+      x[k] = y[k] = make_uint4(0, 0, 0, 0);
       if (r < rows && live) {
-        const int t = r / heads, hh = r - t * heads, kind = hh >= p.heads[0];
-        const int h = kind ? hh - p.heads[0] : hh;
-        const int64_t at = t0 + t, bb = at / p.L, i = at - bb * p.L;
-        const uint16_t *src = p.src[kind] + bb * p.s_in[kind][0] + h * p.s_in[kind][1] +
-                              i * p.s_in[kind][2];
-        rt_load(a[k], src + d0, vec);
-        rt_load(b[k], src + d1, vec);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) a[k][e] = b[k][e] = 0.f;
+        int t, kind, h;
+        place(r, t, kind, h);
+        const int64_t *st = p.s_in[kind];
+        const uint16_t *src = p.src[kind] + b * st[0] + h * st[1] + (i0 + t) * st[2];
+        x[k] = rt_load(src + d0, vec);
+        y[k] = rt_load(src + d1, vec);
       }
     }
-    if (!ready) {  // while the first rows are on their way
-      for (int x = tid; x < n * p.half; x += RT_THREADS) {
-        const int t = x / p.half, i = x - t * p.half;
-        const double turn = p.positions[p.axis[i] * p.tokens + t0 + t] * p.turns[i];
-        float2 cs;
-        sincospif(2.f * (float)(turn - rint(turn)), &cs.y, &cs.x);
-        s_cs[x] = cs;
-      }
-      __syncthreads();
-      ready = true;
-    }
+  };
+  uint4 x[RT_AHEAD], y[RT_AHEAD];
+  fetch(tid / LPR, x, y);
+  // sines while the first rows are on their way
+  for (int z = tid; z < n * p.half; z += RT_THREADS) {
+    const int t = z / p.half, i = z - t * p.half;
+    const double turn = p.positions[p.axis[i] * p.tokens + (int64_t)b * p.L + i0 + t] * p.turns[i];
+    float2 cs;
+    sincospif(2.f * (float)(turn - rint(turn)), &cs.y, &cs.x);
+    s_cs[t * p.half + (i & 7) * turned + (i >> 3)] = cs;
+  }
+  __syncthreads();
+  for (int r0 = tid / LPR; r0 - tid / LPR < rows; r0 += STEP * RT_AHEAD) {
 #pragma unroll
     for (int k = 0; k < RT_AHEAD; ++k) {
       const int r = r0 + k * STEP;
-      const int t = r / heads, hh = r - t * heads, kind = hh >= p.heads[0];
+      int t, kind, h;
+      place(r, t, kind, h);
+      float u[8], v[8];
+      rt_floats(u, x[k]);
+      rt_floats(v, y[k]);
       if constexpr (NORM) {
         const uint16_t *w = p.norm[kind];
         float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(a[k][e], a[k][e], fmaf(b[k][e], b[k][e], ss));
+        for (int e = 0; e < 8; ++e) ss = fmaf(u[e], u[e], fmaf(v[e], v[e], ss));
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (w && live) {
           const float inv = rsqrtf(ss / p.dim + p.eps);
-          float wa[8], wb[8];
-          rt_load(wa, w + d0, vec);
-          rt_load(wb, w + d1, vec);
+          float wu[8], wv[8];
+          rt_floats(wu, rt_load(w + d0, vec));
+          rt_floats(wv, rt_load(w + d1, vec));
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            a[k][e] *= inv * wa[e];
-            b[k][e] *= inv * wb[e];
+            u[e] *= inv * wu[e];
+            v[e] *= inv * wv[e];
           }
         }
       }
@@ -139,19 +149,18 @@ __global__ void __launch_bounds__(RT_THREADS) rotate_kernel(const __grid_constan
       if (j < turned) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float2 cs = s_cs[t * p.half + j * 8 + e];
-          const float x = a[k][e], y = b[k][e];
-          a[k][e] = fmaf(x, cs.x, -y * cs.y);
-          b[k][e] = fmaf(y, cs.x, x * cs.y);
+          const float2 cs = s_cs[t * p.half + e * turned + j];
+          const float c = u[e], s = v[e];
+          u[e] = fmaf(c, cs.x, -s * cs.y);
+          v[e] = fmaf(s, cs.x, c * cs.y);
         }
       }
-      const int h = kind ? hh - p.heads[0] : hh;
-      const int64_t at = t0 + t, bb = at / p.L, i = at - bb * p.L;
-      uint16_t *dst = p.dst[kind] + bb * p.s_out[kind][0] + h * p.s_out[kind][1] +
-                      i * p.s_out[kind][2];
-      rt_store(dst + d0, a[k], vec);
-      rt_store(dst + d1, b[k], vec);
+      const int64_t *st = p.s_out[kind];
+      uint16_t *dst = p.dst[kind] + b * st[0] + h * st[1] + (i0 + t) * st[2];
+      rt_store(dst + d0, u, vec);
+      rt_store(dst + d1, v, vec);
     }
+    if (r0 - tid / LPR + STEP * RT_AHEAD < rows) fetch(r0 + STEP * RT_AHEAD, x, y);
   }
 }
 
@@ -175,7 +184,7 @@ extern "C" int vb_rotate_axes(const VbRotateArgs *a, vb_stream_t stream) {
   VB_REQUIRE(a->rope_dims >= 16 && a->rope_dims <= a->dim && a->rope_dims % 16 == 0,
              "vb_rotate_axes: %d rotated dims of %d (a multiple of 16)", a->rope_dims, a->dim);
   VB_REQUIRE(a->batch >= 0 && a->L >= 0 && a->q_heads >= 0 && a->kv_heads >= 0 &&
-                 a->q_heads <= 1 << 20 && a->kv_heads <= 1 << 20,
+                 a->q_heads <= 32768 && a->kv_heads <= 32768,
              "vb_rotate_axes: batch=%d L=%d heads=%d, %d", a->batch, a->L, a->q_heads,
              a->kv_heads);
   VB_REQUIRE(a->axes >= 1 && a->axes <= 255, "vb_rotate_axes: %d axes (1 to 255)", a->axes);
@@ -221,17 +230,16 @@ extern "C" int vb_rotate_axes(const VbRotateArgs *a, vb_stream_t stream) {
     }
   }
   p.keep = same;
-  // Tokens of a CTA: as many as give each thread a full turn of rows, fewer while that
-  // leaves SMs without work.
-  const int lpr = a->dim > 128 ? 16 : a->dim > 64 ? 8 : 4;
-  int per = RT_THREADS / lpr * RT_AHEAD / heads;
-  per = per < RT_TABLE / p.half ? per : RT_TABLE / p.half;
-  if (per > p.tokens / 296) per = (int)(p.tokens / 296);
+  // Tokens of a CTA: up to 32, fewer while that leaves SMs without work.
+  int per = RT_TABLE / p.half < RT_TOKENS ? RT_TABLE / p.half : RT_TOKENS;
+  if (per > p.tokens / 592) per = (int)(p.tokens / 592);
   p.per = per > 1 ? per : 1;
-  const int64_t ctas = (p.tokens + p.per - 1) / p.per;
+  p.groups = (a->L + p.per - 1) / p.per;
+  const int64_t ctas = (int64_t)p.groups * a->batch;
   VB_REQUIRE(ctas <= 0x7fffffffll, "vb_rotate_axes: too many tokens");
   const bool vec = odd % 8 == 0;
   cudaStream_t s = as_stream(stream);
+  const int lpr = a->dim > 128 ? 16 : a->dim > 64 ? 8 : 4;
   if (lpr == 16) rt_launch<16>(p, (unsigned)ctas, vec, s);
   else if (lpr == 8) rt_launch<8>(p, (unsigned)ctas, vec, s);
   else rt_launch<4>(p, (unsigned)ctas, vec, s);

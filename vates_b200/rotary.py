@@ -14,10 +14,10 @@ import math
 import torch
 
 from ._lib import VbRotateArgs, check, lib
-from .pool import current_device, current_stream, on_device, ptr
+from .pool import current_device, current_stream, on_device
 
-_TABLES: dict = {}
-_STRIDES: dict = {}
+# argument structures without pointers, and the host tables they refer to, by layout
+_LAYOUTS: dict = {}
 
 
 def pair_axes(sections, interleaved: bool = False) -> tuple:
@@ -33,44 +33,40 @@ def pair_axes(sections, interleaved: bool = False) -> tuple:
                  for a, n in enumerate(sections) if i < n)
 
 
-def _table(axes: tuple, base: float):
-    """C arrays of the pairs' axes and of their frequencies in turns."""
-    t = _TABLES.get((axes, base))
-    if t is None:
+def _layout(q, k, q_out, k_out, axes, base, eps, count):
+    """The arguments of a call but its tensors' addresses (made once per layout)."""
+    key = (q.shape, k.shape, q.stride(), k.stride(), q_out.stride(), k_out.stride(), axes, base,
+           eps, count)
+    got = _LAYOUTS.get(key)
+    if got is None:
         n = len(axes)
         if not 1.0 < base < math.inf:
             raise ValueError(f"base={base}: a finite number above 1 is needed")
-        if n > 128 or n % 8 or n == 0 or any(not 0 <= a < 255 for a in axes):
-            raise ValueError(f"axes: one axis (0 to 254) per pair, a multiple of 8 of them and at "
-                             f"most 128, got {n}")
-        if len(_TABLES) > 256:
-            _TABLES.clear()
-        t = _TABLES[axes, base] = (
-            (C.c_uint8 * n)(*axes),
-            (C.c_double * n)(*[base ** (-i / n) / (2.0 * math.pi) for i in range(n)]),
-            max(axes) + 1)
-    return t
-
-
-def _strides(t: torch.Tensor):
-    s = t.stride()
-    a = _STRIDES.get(s)
-    if a is None:
-        if len(_STRIDES) > 4096:
-            _STRIDES.clear()
-        a = _STRIDES[s] = (C.c_int64 * 3)(*s[:3])
-    return a
+        if n > 128 or n % 8 or n == 0 or any(not 0 <= a < count for a in axes):
+            raise ValueError(f"axes: one axis per pair (of {count} in positions), a multiple of 8 "
+                             f"pairs and at most 128, got {n} pairs of the axes {sorted(set(axes))}")
+        axis = (C.c_uint8 * n)(*axes)
+        turns = (C.c_double * n)(*[base ** (-i / n) / (2.0 * math.pi) for i in range(n)])
+        B, Hq, L, D = q.shape
+        strides = [(C.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, q_out, k_out)]
+        a = VbRotateArgs(None, None, None, None, None, None, *strides, None,
+                         C.cast(turns, C.c_void_p), C.cast(axis, C.c_void_p), eps, B, L, Hq,
+                         k.shape[1], D, 2 * n, count)
+        if len(_LAYOUTS) > 4096:
+            _LAYOUTS.clear()
+        got = _LAYOUTS[key] = (bytes(a), axis, turns)
+    return got
 
 
 def _check(t: torch.Tensor, what: str, shape, dev: int):
-    if t.dtype != torch.bfloat16 or t.get_device() != dev or tuple(t.shape) != tuple(shape):
+    if t.dtype != torch.bfloat16 or t.get_device() != dev or t.shape != shape:
         raise ValueError(f"{what}: bfloat16 {tuple(shape)} on cuda:{dev} is needed, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
 
 
 def _out(t: torch.Tensor, out: torch.Tensor | None, what: str, dev: int) -> torch.Tensor:
     if out is None:
-        return torch.empty_like(t, memory_format=torch.contiguous_format)
+        return torch.empty(t.shape, dtype=torch.bfloat16, device=t.device)
     _check(out, what, t.shape, dev)
     if out.stride(3) != 1:
         raise ValueError(f"{what}: contiguous dims are needed, strides {out.stride()}")
@@ -100,17 +96,14 @@ def rotate_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes,
     if q.dim() != 4 or k.dim() != 4 or dev < 0:
         raise ValueError("q, k: CUDA [batch, heads, L, dim] are needed, got "
                          f"{tuple(q.shape)} and {tuple(k.shape)} on {q.device}")
-    B, Hq, L, D = q.shape
-    Hk = k.shape[1]
+    B, _, L, D = q.shape
     _check(q, "q", q.shape, dev)
-    _check(k, "k", (B, Hk, L, D), dev)
-    axis, turns, least = _table(axes if type(axes) is tuple else tuple(int(a) for a in axes), base)
+    _check(k, "k", (B, k.shape[1], L, D), dev)
     if positions.dtype != torch.int32 or positions.get_device() != dev \
-            or positions.dim() != 3 or tuple(positions.shape[1:]) != (B, L) \
-            or positions.shape[0] < least or not positions.is_contiguous():
-        raise ValueError(f"positions: contiguous int32 [axes >= {least}, {B}, {L}] on cuda:{dev} "
-                         f"is needed, got {positions.dtype} {tuple(positions.shape)} on "
-                         f"{positions.device}")
+            or positions.dim() != 3 or positions.shape[1:] != (B, L) \
+            or not positions.is_contiguous():
+        raise ValueError(f"positions: contiguous int32 [axes, {B}, {L}] on cuda:{dev} is needed, "
+                         f"got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
     for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if w is not None:
             _check(w, what, (D,), dev)
@@ -119,10 +112,15 @@ def rotate_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes,
     q_out, k_out = _out(q, q_out, "q_out", dev), _out(k, k_out, "k_out", dev)
     q = q if q.stride(3) == 1 else q.contiguous()
     k = k if k.stride(3) == 1 else k.contiguous()
-    a = VbRotateArgs(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), ptr(q_norm),
-                     ptr(k_norm), _strides(q), _strides(k), _strides(q_out), _strides(k_out),
-                     positions.data_ptr(), C.cast(turns, C.c_void_p), C.cast(axis, C.c_void_p),
-                     eps, B, L, Hq, Hk, D, 2 * len(axis), positions.shape[0])
+    layout = _layout(q, k, q_out, k_out, axes if type(axes) is tuple else
+                     tuple(int(a) for a in axes), base, eps, positions.shape[0])
+    a = VbRotateArgs.from_buffer_copy(layout[0])
+    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
+    a.positions = positions.data_ptr()
+    if q_norm is not None:
+        a.q_norm = q_norm.data_ptr()
+    if k_norm is not None:
+        a.k_norm = k_norm.data_ptr()
     check(lib.vb_rotate_axes(C.byref(a), current_stream(dev)), "vb_rotate_axes")
     return q_out, k_out
 
