@@ -589,6 +589,59 @@ typedef struct VbKv8AttnArgs {
 size_t vb_kv8_attn_workspace_size(const VbKv8AttnArgs *args);
 int vb_kv8_attn(const VbKv8AttnArgs *args, vb_stream_t stream);
 
+/* The attention weight that every cached row receives from some query rows,
+ * added to weights float32 [batch, kv_heads, room] (row j of a sequence at j):
+ *   sum over the query heads of the kv head and the rows i < q_lens[b] that see j
+ *   of exp(scale * q_i . k_j - lse_i),
+ * rows, keys and masks as in vb_kv8_attn and lse [batch, q_heads, L] from it. The
+ * last fresh[b] (nullable: q_lens[b]) rows of a sequence are new: their weights
+ * start at 0 and, with positions int32 [batch, kv_heads, room] (nullable), row j
+ * takes position seen[b] - keys_b + j, seen[b] the tokens of the sequence so far.
+ * Rows from keys_b on are left as they are. A query row whose lse is not finite
+ * adds nothing (VB_STATUS_NONFINITE but for -inf). A sequence with more keys than
+ * room is left as it is (VB_STATUS_BOUNDS). */
+typedef struct VbKv8WeighArgs {
+  VbKv8Cache cache;
+  const uint16_t *q;
+  int64_t q_strides[3];
+  const float *lse;
+  const int32_t *lens;   /* [batch] */
+  const int32_t *q_lens; /* [batch] or NULL */
+  const int32_t *fresh;  /* [batch] or NULL */
+  const int32_t *seen;   /* [batch], with positions */
+  float *weights;
+  int32_t *positions; /* nullable */
+  int32_t *status;    /* nullable */
+  float scale;
+  int32_t q_heads, L, len_add, causal, room;
+} VbKv8WeighArgs;
+int vb_kv8_weigh(const VbKv8WeighArgs *args, vb_stream_t stream);
+
+/* Evict rows: of every sequence with n = lens[b] > keep rows, each kv head keeps
+ * `keep`, the first in the order (protected, weight, lower row). Protected are rows
+ * below first and rows whose position (positions nullable: the row's number) is
+ * above newest - recent, newest the largest of the n; a NaN weight is below all
+ * others. The evicted rows below keep are replaced in order by the kept rows from
+ * keep on, with their weights and positions; rows from keep on are left as they
+ * are. A page that receives rows takes the largest scale of the pages that its live
+ * rows come from, and codes become rint(code * old / new). lens_out[b] =
+ * min(n, keep), not the same memory as lens. first + recent <= keep. Pages that rows
+ * leave or enter must belong to one sequence only (those below `first` are not
+ * touched where they end on a page). workspace: vb_kv8_evict_workspace_size bytes. */
+typedef struct VbKv8EvictArgs {
+  VbKv8Cache cache;
+  float *weights;     /* [batch, kv_heads, room] */
+  int32_t *positions; /* the same, nullable */
+  const int32_t *lens;
+  int32_t *lens_out;
+  int32_t *status; /* nullable */
+  void *workspace;
+  size_t workspace_bytes;
+  int32_t room, keep, first, recent;
+} VbKv8EvictArgs;
+size_t vb_kv8_evict_workspace_size(const VbKv8EvictArgs *args);
+int vb_kv8_evict(const VbKv8EvictArgs *args, vb_stream_t stream);
+
 /* ---------------------------------------------------------------------------
  * Rotary positions with several axes (no reference counterpart): q and k bf16
  * [batch, heads, L, dim] (element strides {batch, head, row}, contiguous dims),

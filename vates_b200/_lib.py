@@ -70,6 +70,23 @@ class VbKv8AttnArgs(C.Structure):
                 ("L", C.c_int32), ("len_add", C.c_int32), ("causal", C.c_int32)]
 
 
+class VbKv8WeighArgs(C.Structure):
+    _fields_ = [("cache", VbKv8Cache), ("q", C.c_void_p), ("q_strides", C.c_int64 * 3),
+                ("lse", C.c_void_p), ("lens", C.c_void_p), ("q_lens", C.c_void_p),
+                ("fresh", C.c_void_p), ("seen", C.c_void_p), ("weights", C.c_void_p),
+                ("positions", C.c_void_p), ("status", C.c_void_p), ("scale", C.c_float),
+                ("q_heads", C.c_int32), ("L", C.c_int32), ("len_add", C.c_int32),
+                ("causal", C.c_int32), ("room", C.c_int32)]
+
+
+class VbKv8EvictArgs(C.Structure):
+    _fields_ = [("cache", VbKv8Cache), ("weights", C.c_void_p), ("positions", C.c_void_p),
+                ("lens", C.c_void_p), ("lens_out", C.c_void_p), ("status", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("room", C.c_int32), ("keep", C.c_int32), ("first", C.c_int32),
+                ("recent", C.c_int32)]
+
+
 class VbRotateArgs(C.Structure):
     _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p),
                 ("k_out", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
@@ -198,6 +215,9 @@ _SIGNATURES = {
     "vb_kv8_read": (_I32, [C.POINTER(VbKv8ReadArgs), _P]),
     "vb_kv8_attn_workspace_size": (_SZ, [C.POINTER(VbKv8AttnArgs)]),
     "vb_kv8_attn": (_I32, [C.POINTER(VbKv8AttnArgs), _P]),
+    "vb_kv8_weigh": (_I32, [C.POINTER(VbKv8WeighArgs), _P]),
+    "vb_kv8_evict_workspace_size": (_SZ, [C.POINTER(VbKv8EvictArgs)]),
+    "vb_kv8_evict": (_I32, [C.POINTER(VbKv8EvictArgs), _P]),
     "vb_rotate_axes": (_I32, [C.POINTER(VbRotateArgs), _P]),
     "vb_token_logprobs_workspace_size": (_SZ, [_I32, _I32, _I32]),
     "vb_token_logprobs": (_I32, [C.POINTER(VbTokenLogprobsArgs), _P]),

@@ -37,6 +37,8 @@ SOURCES = [
     "kv8_cache.cu",
     "kv8_attn.cu",
     "kv8_prefill.cu",
+    "kv8_weigh.cu",
+    "kv8_evict.cu",
     "logprobs.cu",
     "rotary.cu",
 ]

@@ -35,6 +35,32 @@ __device__ __forceinline__ int kv8_rows(const int32_t *counts, int b, int n, int
   return min(max(c, 0), n);
 }
 
+// 0x4B400000 + c as a float is 1.5 * 2^23 + c: adding 1.5 * 2^23 rounds to the
+// nearest integer (ties to even) and leaves its two's complement in the low
+// byte; exact for |v| <= 2^21.
+__device__ __forceinline__ uint32_t rint_bits(float v) {
+  return __float_as_uint(__fadd_rn(v, 12582912.f));
+}
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// Byte j of a word of codes + 128 as float: 2^23 + u is exact, and so is the
+// difference.
+__device__ __forceinline__ float code_f32(uint32_t u, int j) {
+  return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + j)) - 8388736.f;
+}
+// 16 codes under another scale: rint(code * (old / new)), as the append kernel
+// rewrites a page that grows.
+__device__ __forceinline__ uint4 kv8_recode(const uint4 &o, float ratio) {
+  const uint32_t w[4] = {o.x ^ 0x80808080u, o.y ^ 0x80808080u, o.z ^ 0x80808080u,
+                         o.w ^ 0x80808080u};
+  uint32_t c[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) c[j] = rint_bits(__fmul_rn(code_f32(w[j >> 2], j & 3), ratio));
+  return make_uint4(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]),
+                    pack4(c[8], c[9], c[10], c[11]), pack4(c[12], c[13], c[14], c[15]));
+}
+
 // log2 of a page size (16, 32, 64 or 128), or -1.
 static inline int kv8_page_shift(int page) {
   return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;

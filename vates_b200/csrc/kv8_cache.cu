@@ -25,20 +25,6 @@ struct Kv8AppendParams {
   int pos_add, n, shift, dshift, align;  // log2 of the page and of dim / 16; bytes
 };
 
-// 0x4B400000 + c as a float is 1.5 * 2^23 + c: adding 1.5 * 2^23 rounds to the
-// nearest integer (ties to even) and leaves its two's complement in the low
-// byte; exact for |v| <= 2^21.
-__device__ __forceinline__ uint32_t rint_bits(float v) {
-  return __float_as_uint(__fadd_rn(v, 12582912.f));
-}
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-// Byte j of a word of codes + 128 as float: 2^23 + u is exact, and so is the
-// difference.
-__device__ __forceinline__ float code_f32(uint32_t u, int j) {
-  return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + j)) - 8388736.f;
-}
 // Code of one value, any bits.
 __device__ __forceinline__ uint32_t code_any(float x, float inv) {
   const float v = x == x && inv > 0.f ? fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f) : 0.f;

@@ -20,7 +20,8 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import (VbKv8AppendArgs, VbKv8AttnArgs, VbKv8Cache, VbKv8ReadArgs, check, lib)
+from ._lib import (VbKv8AppendArgs, VbKv8AttnArgs, VbKv8Cache, VbKv8EvictArgs, VbKv8ReadArgs,
+                   VbKv8WeighArgs, check, lib)
 from .pool import current_device, current_stream, on_device, ptr, status_ptr
 from .scratch import Scratch
 
@@ -29,6 +30,7 @@ HEAD_DIMS = (64, 128, 256)
 # partial results of the key ranges; one for the caches of all layers, whose
 # attention on a stream runs one after another
 _scratch = Scratch(_lib.VB_KV8_ATTN_WORKSPACE_HEAD)
+_evict_scratch = Scratch(16)  # lists that a call makes itself
 
 
 def _rows(t: torch.Tensor, what: str, shape, device: int) -> torch.Tensor:
@@ -115,7 +117,9 @@ class PagedKV8Cache:
         self._append_args = bytes(VbKv8AppendArgs(c))
         self._read_args = bytes(VbKv8ReadArgs(c))
         self._attn_args = bytes(VbKv8AttnArgs(c))
-        self._need = {}  # workspace bytes by (q_heads, L)
+        self._weigh_args = bytes(VbKv8WeighArgs(c))
+        self._evict_args = bytes(VbKv8EvictArgs(c))
+        self._need = {}  # workspace bytes by (q_heads, L), of evict by (room, keep)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, batch: int, max_pages: int,
@@ -245,6 +249,105 @@ class PagedKV8Cache:
         a = VbKv8AttnArgs.from_buffer_copy(self._attn_args)
         a.q_heads, a.L = q_heads, L
         return lib.vb_kv8_attn_workspace_size(C.byref(a))
+
+    # --------------------------------------------------------------- eviction
+    def _tracked(self, t: torch.Tensor, what: str, dtype, room: int | None) -> int:
+        """Pointer of a contiguous ``[batch, kv_heads, room]`` tensor."""
+        if t.dtype != dtype or t.get_device() != self._index or t.dim() != 3 \
+                or t.shape[0] != self.batch or t.shape[1] != self.kv_heads \
+                or (room is not None and t.shape[2] != room) or not t.is_contiguous():
+            raise ValueError(f"{what}: contiguous {dtype} [{self.batch}, {self.kv_heads}, "
+                             f"{'rows' if room is None else room}] on cuda:{self._index} is needed,"
+                             f" got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t.data_ptr()
+
+    def weigh(self, q, lse, lens, weights, q_lens=None, new=None, len_add: int = 0,
+              scale: float | None = None, causal: bool = True, positions=None, seen=None,
+              status=None, stream=None):
+        """Add the attention weight that every row receives from the rows of ``q``
+        to ``weights`` float32 ``[batch, kv_heads, rows]`` (row ``j`` of a sequence
+        at ``j``): over the query heads of a kv head and the query rows that see
+        ``j``, the sum of ``exp(scale * q_i . k_j - lse_i)``. ``q``, ``lens``,
+        ``q_lens``, ``len_add``, ``scale`` and ``causal`` as in :meth:`attend`,
+        ``lse`` its log-sum-exp of the same rows. The last ``new[b]`` rows of a
+        sequence (``q_lens[b]`` without it; int32 ``[batch]``) are new to
+        ``weights``: they start at 0 and, with ``positions`` int32 of
+        ``weights``' shape and ``seen`` int32 ``[batch]``, the sequence's tokens so
+        far, take their token's position: ``seen[b] - 1`` for the last of them.
+        Rows behind a sequence's last one are left as they are. Query rows whose
+        ``lse`` is not finite add nothing (VB_STATUS_NONFINITE in ``status`` but for
+        -inf); a sequence longer than ``rows`` is left out with VB_STATUS_BOUNDS."""
+        if stream is not None or current_device() != self._index:
+            with on_device(self.device, stream):
+                return self.weigh(q, lse, lens, weights, q_lens, new, len_add, scale, causal,
+                                  positions, seen, status)
+        B, D, dev = self.batch, self.head_dim, self._index
+        if q.dim() != 4:
+            raise ValueError(f"q: [batch, q_heads, L, head_dim] is needed, got {tuple(q.shape)}")
+        Hq, L = q.shape[1], q.shape[2]
+        q = _rows(q, "q", (B, Hq, L, D), dev)
+        if lse.dtype != torch.float32 or lse.get_device() != dev or lse.shape != (B, Hq, L) \
+                or not lse.is_contiguous():
+            raise ValueError(f"lse: contiguous float32 {(B, Hq, L)} on cuda:{dev} is needed, got "
+                             f"{lse.dtype} {tuple(lse.shape)} on {lse.device}")
+        a = VbKv8WeighArgs.from_buffer_copy(self._weigh_args)
+        a.weights = self._tracked(weights, "weights", torch.float32, None)
+        a.room = room = weights.shape[2]
+        if positions is not None:
+            if seen is None:
+                raise ValueError("positions need seen, the tokens of every sequence so far")
+            a.positions = self._tracked(positions, "positions", torch.int32, room)
+            a.seen = _ints(seen, "seen", B, dev)
+        a.q, a.q_strides, a.lse = q.data_ptr(), _strides(q), lse.data_ptr()
+        a.lens, a.q_lens = _ints(lens, "lens", B, dev), _ints(q_lens, "q_lens", B, dev)
+        a.fresh = _ints(new, "new", B, dev)
+        if status is not None:
+            a.status = status_ptr(status, dev)
+        a.scale = D ** -0.5 if scale is None else scale
+        a.q_heads, a.L, a.len_add, a.causal = Hq, L, len_add, causal
+        check(lib.vb_kv8_weigh(C.byref(a), current_stream(dev)), "vb_kv8_weigh")
+
+    def evict(self, weights, lens, keep: int, first: int = 0, recent: int = 0, positions=None,
+              status=None, stream=None):
+        """Every sequence with more than ``keep`` rows keeps ``keep`` of them, each kv
+        head its own: those with the largest ``weights`` (:meth:`weigh`; ties to the
+        lower row, NaN last), before them the rows below ``first`` and the
+        ``recent`` newest, by ``positions`` (int32 like ``weights``; without it a row's
+        number, right until the first eviction). Returns the lengths after it, int32
+        ``[batch]``.
+
+        The evicted rows below ``keep`` are replaced, in order, by the kept rows from
+        ``keep`` on, in the cache, ``weights`` and ``positions`` alike, so the kept
+        rows stay where they are otherwise and the order of rows is no longer the order
+        of tokens; ``causal`` attention still hides nothing it should not, as long as
+        eviction comes before the step's own rows are appended. A page that receives
+        rows takes the largest scale of the pages that its rows come from, and codes of
+        a smaller one are rounded again (half a step of the new scale at most). Pages of
+        more than one sequence must lie below ``first``."""
+        if stream is not None or current_device() != self._index:
+            with on_device(self.device, stream):
+                return self.evict(weights, lens, keep, first, recent, positions, status)
+        dev = self._index
+        a = VbKv8EvictArgs.from_buffer_copy(self._evict_args)
+        a.weights = self._tracked(weights, "weights", torch.float32, None)
+        a.room = room = weights.shape[2]
+        if positions is not None:
+            a.positions = self._tracked(positions, "positions", torch.int32, room)
+        a.lens = _ints(lens, "lens", self.batch, dev)
+        a.keep, a.first, a.recent = keep, first, recent
+        if status is not None:
+            a.status = status_ptr(status, dev)
+        need = self._need.get(("evict", room, keep))
+        if need is None:
+            need = self._need["evict", room, keep] = lib.vb_kv8_evict_workspace_size(C.byref(a))
+        st = current_stream(dev)
+        if need:
+            ws = _evict_scratch.get(need, self.device, st)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        after = torch.empty_like(lens)
+        a.lens_out = after.data_ptr()
+        check(lib.vb_kv8_evict(C.byref(a), st), "vb_kv8_evict")
+        return after
 
 
 __all__ = ["PagedKV8Cache"]
