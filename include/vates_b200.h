@@ -589,6 +589,23 @@ typedef struct VbKv8AttnArgs {
 size_t vb_kv8_attn_workspace_size(const VbKv8AttnArgs *args);
 int vb_kv8_attn(const VbKv8AttnArgs *args, vb_stream_t stream);
 
+/* Attention of a batch whose sequences share a prefix in groups: what vb_kv8_attn
+ * gives, but the keys that a group has in common are attended once for the rows of
+ * all of its sequences. host_groups int32 [groups][3], host memory, in order and
+ * without overlap: first sequence, sequences, rows of the prefix (whole pages, the
+ * same pool pages in the table of each of them as far as it holds that many keys).
+ * segments int32 [groups + batch][4], device: {first, sequences, 0, rows} per group,
+ * then {b, 1, rows of its group or 0, 2^31 - 1} per sequence; group_of int32 [batch],
+ * device: the group or -1. workspace: vb_kv8_attn_shared_workspace_size bytes, its
+ * head as in vb_kv8_attn. batch * kv_heads <= 16384. */
+typedef struct VbKv8SharedArgs {
+  VbKv8AttnArgs attn;
+  const int32_t *segments, *group_of, *host_groups;
+  int32_t groups;
+} VbKv8SharedArgs;
+size_t vb_kv8_attn_shared_workspace_size(const VbKv8SharedArgs *args);
+int vb_kv8_attn_shared(const VbKv8SharedArgs *args, vb_stream_t stream);
+
 /* The attention weight that every cached row receives from some query rows,
  * added to weights float32 [batch, kv_heads, room] (row j of a sequence at j):
  *   sum over the query heads of the kv head and the rows i < q_lens[b] that see j

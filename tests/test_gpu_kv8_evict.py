@@ -76,7 +76,8 @@ def check_weigh(c, q, lens, q_lens=None, new=None, causal=True, len_add=0, extra
         if positions:
             pos[b, :, n - m:n] = seen[b] - m + np.arange(m)
     got = w.cpu().numpy()
-    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) - tol).max()
+    bad = np.abs(got - want) > tol
+    assert not bad.any(), (int(bad.sum()), (np.abs(got - want) - tol).max())
     for b in range(B):  # rows behind the last one
         assert np.array_equal(got[b, :, lens[b]:], w0[b, :, lens[b]:])
     assert np.array_equal(p.cpu().numpy(), pos)

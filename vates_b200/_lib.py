@@ -70,6 +70,11 @@ class VbKv8AttnArgs(C.Structure):
                 ("L", C.c_int32), ("len_add", C.c_int32), ("causal", C.c_int32)]
 
 
+class VbKv8SharedArgs(C.Structure):
+    _fields_ = [("attn", VbKv8AttnArgs), ("segments", C.c_void_p), ("group_of", C.c_void_p),
+                ("host_groups", C.c_void_p), ("groups", C.c_int32)]
+
+
 class VbKv8WeighArgs(C.Structure):
     _fields_ = [("cache", VbKv8Cache), ("q", C.c_void_p), ("q_strides", C.c_int64 * 3),
                 ("lse", C.c_void_p), ("lens", C.c_void_p), ("q_lens", C.c_void_p),
@@ -215,6 +220,8 @@ _SIGNATURES = {
     "vb_kv8_read": (_I32, [C.POINTER(VbKv8ReadArgs), _P]),
     "vb_kv8_attn_workspace_size": (_SZ, [C.POINTER(VbKv8AttnArgs)]),
     "vb_kv8_attn": (_I32, [C.POINTER(VbKv8AttnArgs), _P]),
+    "vb_kv8_attn_shared_workspace_size": (_SZ, [C.POINTER(VbKv8SharedArgs)]),
+    "vb_kv8_attn_shared": (_I32, [C.POINTER(VbKv8SharedArgs), _P]),
     "vb_kv8_weigh": (_I32, [C.POINTER(VbKv8WeighArgs), _P]),
     "vb_kv8_evict_workspace_size": (_SZ, [C.POINTER(VbKv8EvictArgs)]),
     "vb_kv8_evict": (_I32, [C.POINTER(VbKv8EvictArgs), _P]),

@@ -109,20 +109,39 @@ struct Kv8Deal {
   }
 };
 
-// Key tiles of sequence b.
-template <int KT>
+// Keys of segment u that its rows see, and the sequence that sees all of them, whose
+// table has their pages (the first of those that see most).
+__device__ __forceinline__ int kv8_seg_keys(const Kv8AttnParams &p, const int4 &s, bool flag,
+                                            int &owner) {
+  int most = 0;
+  owner = s.x;
+  for (int b = s.x; b < s.x + s.y; ++b) {
+    const Kv8Span sp = kv8_span(p, b, flag);
+    const int n = sp.q_len > 0 ? kv8_reach(s, sp.visible(sp.q_len - 1)) : 0;
+    if (n > most) most = n, owner = b;
+  }
+  return most;
+}
+
+// Key tiles of sequence b, or segment b.
+template <int KT, bool SEG>
 __device__ __forceinline__ int kv8_tiles(const Kv8AttnParams &p, int b, bool flag) {
+  if constexpr (SEG) {
+    int owner;
+    return (kv8_seg_keys(p, p.segs[b], flag, owner) + KT - 1) / KT;
+  }
   const Kv8Span sp = kv8_span(p, b, flag);
   return sp.q_len > 0 ? (sp.visible(sp.q_len - 1) + KT - 1) / KT : 0;
 }
 
 // Tiles of all sequences together; every thread of the CTA gets it.
-template <int KT>
+template <int KT, bool SEG>
 __device__ __forceinline__ unsigned long long kv8_all_tiles(const Kv8AttnParams &p, bool flag,
                                                             unsigned long long *s_sum) {
-  if (p.c.batch == 1) return kv8_tiles<KT>(p, 0, flag && threadIdx.x == 0);
+  const int B = SEG ? p.n_segs : p.c.batch;
+  if (B == 1) return kv8_tiles<KT, SEG>(p, 0, flag && threadIdx.x == 0);
   unsigned long long y = 0;
-  for (int b = threadIdx.x; b < p.c.batch; b += KA_THREADS) y += kv8_tiles<KT>(p, b, flag);
+  for (int b = threadIdx.x; b < B; b += KA_THREADS) y += kv8_tiles<KT, SEG>(p, b, flag);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
   if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = y;
@@ -174,7 +193,7 @@ __device__ __forceinline__ void ldsm_x2_trans(uint32_t &r0, uint32_t &r1, const 
                : "r"((uint32_t)__cvta_generic_to_shared(p)));
 }
 
-template <int D, int NR>
+template <int D, int NR, bool SEG>
 __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_kernel(Kv8AttnParams p) {
   using T = Kv8Tile<D, NR>;
   constexpr int KT = T::KT, ROWS = 8 * NR, MW = T::MW, NM = T::NM;
@@ -187,11 +206,17 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   pdl_launch_dependents();
   pdl_wait();
-  const int H = p.c.kv_heads, rows = p.L * p.rep;
+  const int H = p.c.kv_heads, B = SEG ? p.n_segs : p.c.batch;
+  int rows = p.L * p.rep;
 
   // ---- rows of sequences without visible keys
-  for (int z = blockIdx.x; z < p.c.batch; z += gridDim.x) {
-    if (kv8_tiles<KT>(p, z, false) > 0) continue;
+  for (int z = blockIdx.x; z < B; z += gridDim.x) {
+    if (kv8_tiles<KT, SEG>(p, z, false) > 0) continue;
+    if constexpr (SEG) {
+      for (int i = tid; i < H * ROWS; i += KA_THREADS)
+        p.ml_res[(size_t)z * H * ROWS + i] = make_float2(-INFINITY, 0.f);
+      continue;
+    }
     const size_t row0 = (size_t)z * p.Hq * p.L, n = (size_t)p.Hq * p.L;
     for (size_t i = tid; i < n * (D / 8); i += KA_THREADS)
       reinterpret_cast<uint4 *>(p.out + row0 * D)[i] = make_uint4(0, 0, 0, 0);
@@ -200,17 +225,17 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
   }
 
   // ---- this CTA's tiles, and the sequence its range begins in
-  const Kv8Deal deal(kv8_all_tiles<KT>(p, blockIdx.x == 0, s_sum) * H, gridDim.x);
+  const Kv8Deal deal(kv8_all_tiles<KT, SEG>(p, blockIdx.x == 0, s_sum) * H, gridDim.x);
   unsigned long long w0 = deal.begin(blockIdx.x);
   const unsigned long long w1 = deal.begin(blockIdx.x + 1);
   if (w0 == w1) return;
   int b = 0;
   unsigned long long b_begin = 0;  // tiles of the sequences before b, all heads
-  if (p.c.batch > 1) {
+  if (B > 1) {
     if (warp == 0) {  // 32 sequences at a time
-      for (int b0 = 0; b0 < p.c.batch; b0 += 32) {
-        unsigned long long n = b0 + lane < p.c.batch
-                                   ? (unsigned long long)kv8_tiles<KT>(p, b0 + lane, false) * H : 0;
+      for (int b0 = 0; b0 < B; b0 += 32) {
+        unsigned long long n =
+            b0 + lane < B ? (unsigned long long)kv8_tiles<KT, SEG>(p, b0 + lane, false) * H : 0;
         unsigned long long inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -255,8 +280,17 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
 
   while (w0 < w1) {
     // ---- the unit at w0: sequence b, head h, tiles [t0, t1) of `tiles`
-    const Kv8Span sp = kv8_span(p, b, false);
-    const int kend = sp.q_len > 0 ? sp.visible(sp.q_len - 1) : 0;
+    Kv8Span sp;
+    int4 seg = make_int4(0, 0, 0, 0);
+    int kend, owner = b;
+    if constexpr (SEG) {
+      seg = p.segs[b];
+      rows = seg.y * p.L * p.rep;
+      kend = kv8_seg_keys(p, seg, false, owner);
+    } else {
+      sp = kv8_span(p, b, false);
+      kend = sp.q_len > 0 ? sp.visible(sp.q_len - 1) : 0;
+    }
     const int tiles = (kend + KT - 1) / KT;
     const unsigned long long off = w0 - b_begin;
     if (off >= (unsigned long long)tiles * H) {  // past this sequence
@@ -269,7 +303,9 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
     const int t1 = (int)min((unsigned long long)tiles, t0 + (w1 - w0));
     const unsigned long long u0 = w0 - t0;  // the unit's first tile
     w0 += t1 - t0;
-    const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
+    // (a segment's first key is the first of a page)
+    const int pages_before = SEG ? seg.z >> p.shift : 0, table_len = p.c.max_pages - pages_before;
+    const int32_t *table = p.c.page_table + (size_t)owner * p.c.max_pages + pages_before;
     const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + ch * 16;
     const int8_t *vbase = p.c.v_codes + (size_t)h * p.c.page * D + ch * 16;
 
@@ -277,7 +313,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
     // Rows without a page read page 0 and get no weight.
     auto group_entry = [&](int t) {
       const int key = t * KT + (lane % NG) * 16;
-      return t < t1 && key < kend ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : -1;
+      return t < t1 && key < kend ? kv8_page_load(table, table_len, key >> p.shift) : -1;
     };
     // K scale of the group (-1 masks it) and V scale
     auto group_scales = [&](int entry, float &ks, float &vs) {
@@ -320,10 +356,21 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
       uint4 w[NP];
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
-        const int r = tid / LPR + k * PASS, i = p.row_of(r), hr = r - i * p.rep;
+        const int r = tid / LPR + k * PASS;
+        int bq = b, i, hr;
+        bool there;
+        if constexpr (SEG) {
+          const Kv8SegRow x = kv8_seg_row(p, seg, r);
+          bq = x.b; i = x.i; hr = x.hr;
+          there = x.vis > 0;
+        } else {
+          i = p.row_of(r);
+          hr = r - i * p.rep;
+          there = r < rows && i < sp.q_len;
+        }
         w[k] = make_uint4(0, 0, 0, 0);
-        if (r < rows && i < sp.q_len)
-          w[k] = kv8_load8(p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh +
+        if (there)
+          w[k] = kv8_load8(p.q + bq * p.qb + (int64_t)(h * p.rep + hr) * p.qh +
                                (int64_t)i * p.ql + c8 * 8,
                            p.vec);
       }
@@ -354,7 +401,10 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int r = n * 8 + 2 * c + u;
-        vis[n][u] = r < rows ? sp.visible(p.row_of(r)) : 0;
+        if constexpr (SEG)
+          vis[n][u] = kv8_seg_row(p, seg, r).vis;
+        else
+          vis[n][u] = r < rows ? sp.visible(p.row_of(r)) : 0;
         m[n][u] = -INFINITY;
         l[n][u] = 0.f;
       }
@@ -573,12 +623,15 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
         const int r = n * 8 + 2 * c + u;
         if (r >= rows) continue;
         const float ls = (s_l[0][r] + s_l[1][r]) + (s_l[2][r] + s_l[3][r]);
-        const int i = p.row_of(r);
-        const size_t row = ((size_t)b * p.Hq + h * p.rep + r - i * p.rep) * p.L + i;
-        const float mul = !whole ? vref : ls == 0.f ? 0.f : vref / ls;  // 0: sees no key
+        const int i = SEG ? 0 : p.row_of(r);
+        const size_t row = SEG ? ((size_t)b * H + h) * ROWS + r
+                               : ((size_t)b * p.Hq + h * p.rep + r - i * p.rep) * p.L + i;
+        const float mul = !whole || SEG ? vref : ls == 0.f ? 0.f : vref / ls;  // 0: sees no key
         if (warp == 0 && g == 0) {
           if (!whole)
             p.ml_part[slot * ROWS + r] = make_float2(m[n][u], ls);
+          else if (SEG)
+            p.ml_res[row] = make_float2(m[n][u], ls);
           else if (p.lse)
             p.lse[row] = ls == 0.f ? -INFINITY
                                    : (m[n][u] + log2f(ls)) * 0.69314718055994531f;
@@ -589,8 +642,8 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
 #pragma unroll
           for (int k = 0; k < DL; ++k) f[k] = o[2 * d + (k >> 1)][n][(k & 1) * 2 + u] * mul;
           const int dim = warp * T::DW + d * 32 + g * DL;
-          if (!whole) {
-            float *dst = p.o_part + (slot * ROWS + r) * D + dim;
+          if (!whole || SEG) {
+            float *dst = (whole ? p.o_res + row * D : p.o_part + (slot * ROWS + r) * D) + dim;
             if constexpr (DL == 4)
               *reinterpret_cast<float4 *>(dst) = make_float4(f[0], f[1], f[2], f[3]);
             else
@@ -605,7 +658,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
         }
       }
     // the CTAs that share the unit: s_share[1] from s_share[0] on
-    if (!whole && p.wide) {
+    if (!whole && p.wide && !SEG) {
       if (t0 == 0 && tid == 0)
         p.units[b * H + h] =
             make_int2(blockIdx.x, (int)(deal.owner(u0 + tiles - 1) - blockIdx.x) + 1);
@@ -682,11 +735,19 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
 #pragma unroll
           for (int i = 0; i < IG; ++i) {
             const int r = r0 + (i0 + i) * RT;
-            if (r < rows) kv8_finish(p, D, b, h, r, d4, s_max[0][r], s_l[0][r], a[i]);
+            if constexpr (SEG) {
+              const size_t row = ((size_t)b * H + h) * ROWS + r;
+              if (r < rows) {
+                *(reinterpret_cast<float4 *>(p.o_res + row * D) + d4) = a[i];
+                if (d4 == 0) p.ml_res[row] = make_float2(s_max[0][r], s_l[0][r]);
+              }
+            } else if (r < rows) {
+              kv8_finish(p, D, b, h, r, d4, s_max[0][r], s_l[0][r], a[i]);
+            }
           }
         }
       }
-    } else if (p.wide && tid == 0) {
+    } else if (p.wide && !SEG && tid == 0) {
       p.units[b * H + h] = make_int2(blockIdx.x, 1);
     }
     if (w0 < w1) __syncthreads();  // s_l has been read
@@ -729,7 +790,7 @@ __device__ __forceinline__ Kv8Parts kv8_parts(const Kv8AttnParams &p, int bh, in
   Kv8Parts q;
   if (p.units) {
     const int2 u = __ldcg(p.units + bh);  // (left from an earlier call if there are no tiles)
-    q.n = kv8_tiles<KA_TILE / D>(p, b, false) > 0 ? u.y : 0;
+    q.n = kv8_tiles<KA_TILE / D, false>(p, b, false) > 0 ? u.y : 0;
     q.first = (size_t)u.x * 2 + 1;
     q.step = 2;
     q.skip = 1;
@@ -906,13 +967,13 @@ Kv8Plan kv8_plan(const VbKv8AttnArgs *a) {
   return pl;
 }
 
-template <int D, int NR>
+template <int D, int NR, bool SEG>
 int kv8_launch(const Kv8AttnParams &p, int ctas, cudaStream_t s) {
   using T = Kv8Tile<D, NR>;
   static std::atomic<uint64_t> ready{0};
   const int rc = once_per_device(ready, [] {
     const cudaError_t e = cudaFuncSetAttribute(
-        kv8_attn_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+        kv8_attn_kernel<D, NR, SEG>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
     return e == cudaSuccess ? VB_OK
                             : set_error(VB_ERR_CUDA, "kv8_attn_kernel attributes: %s",
                                         cudaGetErrorString(e));
@@ -921,16 +982,16 @@ int kv8_launch(const Kv8AttnParams &p, int ctas, cudaStream_t s) {
   // Dependent launch for short calls only: started before the kernel ahead has
   // left its SMs, a full grid is placed unevenly (131,072 keys: 49.6 us instead of
   // 37.7; 901 keys: 12.1 us instead of 14.1).
-  vb_launch(kv8_attn_kernel<D, NR>, dim3(ctas), dim3(KA_THREADS), T::SMEM, s, ctas <= 148, p);
+  vb_launch(kv8_attn_kernel<D, NR, SEG>, dim3(ctas), dim3(KA_THREADS), T::SMEM, s, ctas <= 148, p);
   return check_launch("kv8_attn_kernel");
 }
 
 template <int D>
 int kv8_run(const Kv8AttnParams &p, const Kv8Plan &pl, cudaStream_t s) {
   const int rc = pl.tensor ? kv8_prefill_launch(p, s)
-                 : pl.tile_rows == 8  ? kv8_launch<D, 1>(p, pl.ctas, s)
-                 : pl.tile_rows == 16 ? kv8_launch<D, 2>(p, pl.ctas, s)
-                                      : kv8_launch<D, 4>(p, pl.ctas, s);
+                 : pl.tile_rows == 8  ? kv8_launch<D, 1, false>(p, pl.ctas, s)
+                 : pl.tile_rows == 16 ? kv8_launch<D, 2, false>(p, pl.ctas, s)
+                                      : kv8_launch<D, 4, false>(p, pl.ctas, s);
   if (rc != VB_OK || pl.parts == 0 || (!pl.tensor && !pl.wide)) return rc;
   const unsigned units = p.c.batch * p.c.kv_heads, rows = p.L * p.rep;
   constexpr unsigned RPC = KC_THREADS * 4 / D;
@@ -943,6 +1004,177 @@ int kv8_run(const Kv8AttnParams &p, const Kv8Plan &pl, cudaStream_t s) {
   return check_launch("kv8_combine_kernel");
 }
 
+// ------------------------------------------------------------ shared prefixes
+// The keys that a group of sequences have in common are attended once for the rows
+// of all of them, the keys of each alone after it by its own rows, and the results
+// of both are joined: weights 2^(m - M) of a row's partial results.
+struct Kv8Parted {             // where the results of some segments are
+  const float *o;
+  const float2 *ml;
+  int tile_rows, row_tiles, splits;
+  __device__ size_t at(int u, int H, int h, int R, int s) const {
+    const int t = R / tile_rows;
+    return (((size_t)(u * H + h) * row_tiles + t) * splits + s) * tile_rows + R - t * tile_rows;
+  }
+};
+struct Kv8SharedParams {
+  Kv8AttnParams p;
+  Kv8Parted pre, own;
+  const int4 *groups;
+  const int32_t *group_of;     // per sequence, -1: none
+};
+
+// A thread joins four dims of one row.
+template <int D>
+__global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __grid_constant__ Kv8SharedParams w) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const Kv8AttnParams &p = w.p;
+  constexpr int RPC = KC_THREADS * 4 / D;
+  const long long row = (long long)blockIdx.x * RPC + threadIdx.x / (D / 4);
+  const int d4 = threadIdx.x % (D / 4), per = p.Hq * p.L;
+  if (row >= (long long)p.c.batch * per) return;
+  const int b = (int)(row / per), x = (int)(row - (long long)b * per);
+  const int hq = x / p.L, i = x - hq * p.L, h = hq / p.rep, R = i * p.rep + hq - h * p.rep;
+  const int H = p.c.kv_heads, g = w.group_of[b];
+  const int n_pre = g >= 0 ? w.pre.splits : 0, n = n_pre + w.own.splits;
+  const int R_pre = g >= 0 ? (b - w.groups[g].x) * p.L * p.rep + R : 0;
+  auto source = [&](int s, const float *&o, const float2 *&ml) {
+    const Kv8Parted &q = s < n_pre ? w.pre : w.own;
+    const size_t at = s < n_pre ? q.at(g, H, h, R_pre, s) : q.at(b, H, h, R, s - n_pre);
+    o = q.o + at * D;
+    ml = q.ml + at;
+  };
+  float M = -INFINITY, ls = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float *o;
+    const float2 *ml;
+    source(s, o, ml);
+    M = fmaxf(M, __ldcg(ml).x);
+  }
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float *o;
+    const float2 *mlp;
+    source(s, o, mlp);
+    const float2 ml = __ldcg(mlp);
+    const float4 y = __ldcg(reinterpret_cast<const float4 *>(o) + d4);
+    const float f = ml.x == -INFINITY ? 0.f : kv8_ex2(ml.x - M);
+    ls = fmaf(f, ml.y, ls);
+    if (f > 0.f) {  // keys that the row does not see left no O
+      a.x = fmaf(f, y.x, a.x); a.y = fmaf(f, y.y, a.y);
+      a.z = fmaf(f, y.z, a.z); a.w = fmaf(f, y.w, a.w);
+    }
+  }
+  kv8_finish(p, D, b, h, R, d4, M, ls, a);
+}
+
+// One side of the work: the groups' segments, or each sequence's own.
+struct Kv8Side {
+  bool tensor;
+  int tile_rows, row_tiles, splits, ctas;
+  size_t results, parts;       // rows of results, of partial results of kv8_attn_kernel
+};
+// `base`: row tiles of all segments and heads, `tiles`: key tiles of the longest segment
+// (128 keys) or of all of them together (kv8_attn_kernel).
+Kv8Side kv8_side(const VbKv8AttnArgs *a, long long segs, long long rows, long long base,
+                 long long longest, long long all) {
+  Kv8Side s;
+  const long long units = segs * a->cache.kv_heads;
+  s.tensor = rows > 32;
+  if (s.tensor) {
+    s.tile_rows = kv8_prefill_rows();
+    s.row_tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
+    s.splits = kv8_ranges(base, longest);
+    s.ctas = 0;
+    s.parts = 0;
+  } else {
+    s.tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    s.row_tiles = s.splits = 1;
+    const int full = 148 * (s.tile_rows == 32 ? Kv8Tile<64, 4>::CTAS : Kv8Tile<64, 1>::CTAS);
+    s.ctas = (int)(all < 1 ? 1 : all < full ? all : full);
+    s.parts = (size_t)s.ctas * 2 * s.tile_rows;
+  }
+  s.results = (size_t)(units * s.row_tiles * s.splits) * s.tile_rows;
+  return s;
+}
+
+struct Kv8SharedPlan {
+  Kv8Side pre, own;
+  size_t pre_at, own_at, part_at, bytes;  // results and partial results in the workspace
+};
+Kv8SharedPlan kv8_shared_plan(const VbKv8SharedArgs *s) {
+  const VbKv8AttnArgs *a = &s->attn;
+  const long long H = a->cache.kv_heads, rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
+  const long long cap = (long long)a->cache.max_pages * a->cache.page, kt = KA_TILE / a->cache.dim;
+  const long long tile = kv8_prefill_rows();
+  long long most = 0, base = 0, longest = 0, all = 0, own = cap * a->cache.batch;
+  for (int g = 0; g < s->groups; ++g) {
+    const int32_t *x = s->host_groups + 3 * g;
+    const long long r = x[1] * rows;
+    most = r > most ? r : most;
+    longest = x[2] > longest ? x[2] : longest;
+    base += (r + tile - 1) / tile * H;
+    all += (x[2] + kt - 1) / kt * H;
+    own -= (long long)x[1] * x[2];
+  }
+  Kv8SharedPlan pl;
+  pl.pre = kv8_side(a, s->groups, most, base, (longest + 127) / 128, all);
+  pl.own = kv8_side(a, a->cache.batch, rows, a->cache.batch * H * ((rows + tile - 1) / tile),
+                    (own / a->cache.batch + 127) / 128, (own + kt - 1) / kt * H);
+  const size_t width = (a->cache.dim + 2) * sizeof(float);
+  pl.pre_at = KA_TICKETS * sizeof(uint32_t);
+  pl.own_at = pl.pre_at + align_up(pl.pre.results * width, 16);
+  pl.part_at = pl.own_at + align_up(pl.own.results * width, 16);
+  const size_t parts = pl.pre.parts > pl.own.parts ? pl.pre.parts : pl.own.parts;
+  pl.bytes = pl.part_at + parts * width;
+  return pl;
+}
+
+template <int D>
+int kv8_side_run(Kv8AttnParams p, const Kv8Side &s, uint8_t *results, Kv8Parted &out,
+                 cudaStream_t st) {
+  float *o = reinterpret_cast<float *>(results);
+  float2 *ml = reinterpret_cast<float2 *>(o + s.results * D);
+  out.o = o; out.ml = ml;
+  out.tile_rows = s.tile_rows; out.row_tiles = s.row_tiles; out.splits = s.splits;
+  p.row_tiles = s.row_tiles; p.splits = s.splits;
+  if (s.tensor) {
+    p.o_part = o; p.ml_part = ml;
+    return kv8_prefill_launch_segments(p, st);
+  }
+  p.ml_part = reinterpret_cast<float2 *>(p.o_part + s.parts * D);
+  p.o_res = o; p.ml_res = ml;
+  return s.tile_rows == 8    ? kv8_launch<D, 1, true>(p, s.ctas, st)
+         : s.tile_rows == 16 ? kv8_launch<D, 2, true>(p, s.ctas, st)
+                             : kv8_launch<D, 4, true>(p, s.ctas, st);
+}
+
+template <int D>
+int kv8_shared_run(Kv8AttnParams p, const Kv8SharedPlan &pl, const VbKv8SharedArgs *a, uint8_t *ws,
+                   cudaStream_t s) {
+  Kv8SharedParams w;
+  w.groups = reinterpret_cast<const int4 *>(a->segments);
+  w.group_of = a->group_of;
+  p.o_part = reinterpret_cast<float *>(ws + pl.part_at);
+  p.segs = w.groups;
+  p.n_segs = a->groups;
+  int rc = kv8_side_run<D>(p, pl.pre, ws + pl.pre_at, w.pre, s);
+  if (rc != VB_OK) return rc;
+  p.segs = w.groups + a->groups;
+  p.n_segs = p.c.batch;
+  rc = kv8_side_run<D>(p, pl.own, ws + pl.own_at, w.own, s);
+  if (rc != VB_OK) return rc;
+  w.p = p;
+  constexpr int RPC = KC_THREADS * 4 / D;
+  const long long rows = (long long)p.c.batch * p.Hq * p.L;
+  vb_launch(kv8_shared_join_kernel<D>, dim3((unsigned)((rows + RPC - 1) / RPC)), dim3(KC_THREADS), 0,
+            s, true, w);
+  return check_launch("kv8_shared_join_kernel");
+}
+
 int kv8_attn_check(const VbKv8AttnArgs *a) {
   VB_REQUIRE(a, "vb_kv8_attn: null args");
   const int rc = kv8_check(&a->cache, "vb_kv8_attn");
@@ -953,6 +1185,47 @@ int kv8_attn_check(const VbKv8AttnArgs *a) {
              a->cache.kv_heads);
   VB_REQUIRE(a->L >= 0 && (long long)a->L * a->q_heads <= 1 << 24,
              "vb_kv8_attn: L=%d rows of %d heads", a->L, a->q_heads);
+  return VB_OK;
+}
+
+// What both entries pass on.
+Kv8AttnParams kv8_params(const VbKv8AttnArgs *a) {
+  Kv8AttnParams p = {};
+  p.c = a->cache;
+  p.q = a->q;
+  p.qb = a->q_strides[0]; p.qh = a->q_strides[1]; p.ql = a->q_strides[2];
+  p.lens = a->lens; p.q_lens = a->q_lens;
+  p.out = a->out; p.lse = a->lse; p.status = a->status;
+  p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
+  p.Hq = a->q_heads; p.L = a->L; p.rep = a->q_heads / a->cache.kv_heads;
+  p.len_add = a->len_add; p.causal = a->causal ? 1 : 0;
+  p.shift = kv8_page_shift(a->cache.page);
+  p.vec = ((uintptr_t)a->q % 16) == 0 && p.qb % 8 == 0 && p.qh % 8 == 0 && p.ql % 8 == 0;
+  p.rep_inv = (uint32_t)((1ull << 32) / (uint32_t)p.rep) + (p.rep > 1);
+  return p;
+}
+
+int kv8_shared_check(const VbKv8SharedArgs *s) {
+  VB_REQUIRE(s, "vb_kv8_attn_shared: null args");
+  const int rc = kv8_attn_check(&s->attn);
+  if (rc != VB_OK) return rc;
+  const VbKv8Cache &c = s->attn.cache;
+  VB_REQUIRE(s->groups >= 1 && s->groups <= c.batch && s->host_groups,
+             "vb_kv8_attn_shared: %d groups of %d sequences", s->groups, c.batch);
+  int end = 0;
+  for (int g = 0; g < s->groups; ++g) {
+    const int32_t *x = s->host_groups + 3 * g;
+    VB_REQUIRE(x[0] >= end && x[1] >= 1 && (long long)x[0] + x[1] <= c.batch && x[2] >= c.page &&
+                   x[2] % c.page == 0 && x[2] / c.page <= c.max_pages,
+               "vb_kv8_attn_shared: group %d: sequences %d + %d of %d (in order), %d rows in pages "
+               "of %d, %d of them",
+               g, x[0], x[1], c.batch, x[2], c.page, c.max_pages);
+    end = x[0] + x[1];
+  }
+  VB_REQUIRE((long long)c.batch * c.kv_heads <= KA_TICKETS &&
+                 (long long)c.batch * s->attn.q_heads * s->attn.L <= 1 << 28,
+             "vb_kv8_attn_shared: %d sequences of %d kv heads, %d rows of %d heads each", c.batch,
+             c.kv_heads, s->attn.L, s->attn.q_heads);
   return VB_OK;
 }
 
@@ -983,19 +1256,8 @@ int vb_kv8_attn(const VbKv8AttnArgs *a, vb_stream_t stream) {
   VB_REQUIRE((long long)a->cache.kv_heads * pl.row_tiles <= 65535 &&
                  (long long)a->cache.batch * a->q_heads * a->L <= 0x7fffffffll,
              "vb_kv8_attn: too many rows");
-  Kv8AttnParams p;
-  p.c = a->cache;
-  p.q = a->q;
-  p.qb = a->q_strides[0]; p.qh = a->q_strides[1]; p.ql = a->q_strides[2];
-  p.lens = a->lens; p.q_lens = a->q_lens;
-  p.out = a->out; p.lse = a->lse; p.status = a->status;
-  p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
-  p.Hq = a->q_heads; p.L = a->L; p.rep = a->q_heads / a->cache.kv_heads;
-  p.len_add = a->len_add; p.causal = a->causal ? 1 : 0;
-  p.shift = kv8_page_shift(a->cache.page);
-  p.vec = ((uintptr_t)a->q % 16) == 0 && p.qb % 8 == 0 && p.qh % 8 == 0 && p.ql % 8 == 0;
+  Kv8AttnParams p = kv8_params(a);
   p.row_tiles = pl.row_tiles; p.splits = pl.splits;
-  p.rep_inv = (uint32_t)((1ull << 32) / (uint32_t)p.rep) + (p.rep > 1);
   // the tickets lie at the same place in every call: they are zero between calls
   uint8_t *ws = static_cast<uint8_t *>(a->workspace);
   p.tickets = reinterpret_cast<uint32_t *>(ws);
@@ -1009,6 +1271,39 @@ int vb_kv8_attn(const VbKv8AttnArgs *a, vb_stream_t stream) {
     case 64: return kv8_run<64>(p, pl, s);
     case 128: return kv8_run<128>(p, pl, s);
     default: return kv8_run<256>(p, pl, s);
+  }
+}
+
+size_t vb_kv8_attn_shared_workspace_size(const VbKv8SharedArgs *a) {
+  if (kv8_shared_check(a) != VB_OK || a->attn.L == 0) return 0;
+  return kv8_shared_plan(a).bytes;
+}
+
+int vb_kv8_attn_shared(const VbKv8SharedArgs *s, vb_stream_t stream) {
+  const int rc = kv8_shared_check(s);
+  if (rc != VB_OK) return rc;
+  const VbKv8AttnArgs *a = &s->attn;
+  if (a->L == 0) return VB_OK;
+  VB_REQUIRE(a->q && a->lens && a->out && s->segments && s->group_of,
+             "vb_kv8_attn_shared: null tensor");
+  VB_REQUIRE(((uintptr_t)a->out % 16) == 0 && ((uintptr_t)s->segments % 16) == 0,
+             "vb_kv8_attn_shared: out and segments must be 16-byte aligned");
+  VB_REQUIRE(a->scale > 0.f && a->scale < 1e30f, "vb_kv8_attn_shared: scale %g", (double)a->scale);
+  const Kv8SharedPlan pl = kv8_shared_plan(s);
+  for (const Kv8Side *x : {&pl.pre, &pl.own})
+    VB_REQUIRE((x->results / x->tile_rows) <= 1u << 29, "vb_kv8_attn_shared: too many rows");
+  if (!a->workspace || a->workspace_bytes < pl.bytes)
+    return set_error(VB_ERR_WORKSPACE, "vb_kv8_attn_shared: workspace %zu < %zu bytes",
+                     a->workspace_bytes, pl.bytes);
+  VB_REQUIRE(((uintptr_t)a->workspace % 16) == 0, "vb_kv8_attn_shared: workspace alignment");
+  Kv8AttnParams p = kv8_params(a);
+  uint8_t *ws = static_cast<uint8_t *>(a->workspace);
+  p.tickets = reinterpret_cast<uint32_t *>(ws);
+  cudaStream_t st = as_stream(stream);
+  switch (a->cache.dim) {
+    case 64: return kv8_shared_run<64>(p, pl, s, ws, st);
+    case 128: return kv8_shared_run<128>(p, pl, s, ws, st);
+    default: return kv8_shared_run<256>(p, pl, s, ws, st);
   }
 }
 

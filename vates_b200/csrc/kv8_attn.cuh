@@ -26,6 +26,15 @@ struct Kv8AttnParams {
   int Hq, L, rep, len_add, causal, shift, vec;
   int row_tiles, splits;
   uint32_t rep_inv;  // floor(2^32 / rep) + 1
+  // Segments in the place of sequences: (first sequence, sequences, first key, end):
+  // all query rows of those sequences over the keys [first, end) that they have in
+  // common, at most as far as each row sees. Their results, rows of unnormalised O and
+  // (m, l), are joined later: by kv8_attn_kernel one per row, in o_res and ml_res; by
+  // the prefill kernel one per range of keys, as above.
+  const int4 *segs;
+  int n_segs;
+  float *o_res;
+  float2 *ml_res;
   // Query row R (< 2^24) of the flattened (row, head of the group) order is
   // query R / rep: exact by one product while R * rep < 2^32.
   __device__ __forceinline__ int row_of(int R) const {
@@ -54,6 +63,24 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnParams &p, int b, bool 
   s.off = s.keys - s.q_len;
   s.causal = p.causal;
   return s;
+}
+
+// Keys of segment s that the rows of sequence b of it see, from its first key on.
+__device__ __forceinline__ int kv8_reach(const int4 &s, int visible) {
+  return max(0, min(visible, s.w) - s.z);
+}
+// Query row R of a segment's flattened (sequence, row, head of the group) order.
+struct Kv8SegRow {
+  int b, i, hr, vis;  // sequence, query, head of the group; keys seen (0: no such row)
+};
+__device__ __forceinline__ Kv8SegRow kv8_seg_row(const Kv8AttnParams &p, const int4 &s, int R) {
+  const int per = p.L * p.rep, m = R / per, r = R - m * per;
+  Kv8SegRow x;
+  x.b = s.x + min(m, s.y - 1);
+  x.i = p.row_of(r);
+  x.hr = r - x.i * p.rep;
+  x.vis = m < s.y ? kv8_reach(s, kv8_span(p, x.b, false).visible(x.i)) : 0;
+  return x;
 }
 
 __device__ __forceinline__ float kv8_ex2(float x) {
@@ -116,5 +143,6 @@ __device__ __forceinline__ float kv8_q_scale(uint4 &v) {
 // Rows per row tile of the prefill kernel, and its launch (kv8_prefill.cu).
 int kv8_prefill_rows();
 int kv8_prefill_launch(const Kv8AttnParams &p, cudaStream_t s);
+int kv8_prefill_launch_segments(const Kv8AttnParams &p, cudaStream_t s);
 
 }  // namespace vb

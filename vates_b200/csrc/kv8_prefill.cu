@@ -226,7 +226,9 @@ struct KpBarriers {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[3], p_full[3], o_done[3], q_full, o_last, drain;
 };
 
-template <int D>
+// SEG: segments in the place of sequences (kv8_attn.cuh), each with its own number of
+// row tiles, up to p.row_tiles.
+template <int D, bool SEG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     kv8_prefill_kernel(Kv8AttnParams p) {
   using H = KpShape<D>;
@@ -243,21 +245,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
 
   // ---- the pair's rows and keys, this CTA's rows r_base .. + 127
   const int rank = blockIdx.x & 1;
-  const int units = p.c.batch * p.c.kv_heads * p.splits, unit = (blockIdx.x >> 1) % units;
+  const int units = (SEG ? p.n_segs : p.c.batch) * p.c.kv_heads * p.splits, unit = (blockIdx.x >> 1) % units;
   const int rt = p.row_tiles - 1 - (blockIdx.x >> 1) / units;  // longest (causal) rows first
   const int split = unit % p.splits, h = unit / p.splits % p.c.kv_heads;
   const int b = unit / p.splits / p.c.kv_heads;
-  const int pair_base = rt * KP_ROWS, r_base = pair_base + rank * 128, rows = p.L * p.rep;
-  const Kv8Span sp = kv8_span(p, b, rt == p.row_tiles - 1 && split == 0 && rank == 0 && h == 0 && tid == 0);
-  const int i_last = p.row_of(max(0, min(min(pair_base + KP_ROWS, rows), sp.q_len * p.rep) - 1));
-  const int kend = pair_base < sp.q_len * p.rep ? sp.visible(i_last) : 0;
+  const int pair_base = rt * KP_ROWS, r_base = pair_base + rank * 128;
+  int4 seg = make_int4(0, 0, 0, 0);
+  int rows = p.L * p.rep;
+  if constexpr (SEG) {
+    seg = p.segs[b];
+    rows *= seg.y;
+    if (pair_base >= rows) return;  // (both CTAs, before either waits for the other)
+  }
+  Kv8Span sp;
+  int kend, owner = b;
+  if constexpr (SEG) {
+    // keys that the tile's rows see, and a sequence that sees as many: its table has them.
+    // Every warp looks at all of the tile's sequences, 32 at a time.
+    const int per = p.L * p.rep, m0 = pair_base / per;
+    const int m1 = min(seg.y - 1, (min(pair_base + KP_ROWS, rows) - 1) / per);
+    kend = 0;
+    owner = seg.x + m0;
+    for (int m = m0; m <= m1; m += 32) {
+      int n = 0;
+      if (m + lane <= m1) {
+        const Kv8Span s = kv8_span(p, seg.x + m + lane, split == 0 && rank == 0 && h == 0 && warp == 0);
+        // (a row tile that ends or begins within a sequence may see less)
+        n = s.q_len > 0 ? kv8_reach(seg, s.visible(s.q_len - 1)) : 0;
+      }
+      const int most = (int)__reduce_max_sync(0xffffffffu, (unsigned)n);
+      if (most > kend) {
+        kend = most;
+        owner = seg.x + m + __ffs(__ballot_sync(0xffffffffu, n == most)) - 1;
+      }
+    }
+  } else {
+    sp = kv8_span(p, b, rt == p.row_tiles - 1 && split == 0 && rank == 0 && h == 0 && tid == 0);
+    const int i_last = p.row_of(max(0, min(min(pair_base + KP_ROWS, rows), sp.q_len * p.rep) - 1));
+    kend = pair_base < sp.q_len * p.rep ? sp.visible(i_last) : 0;
+  }
+  // The row R of the tile: sequence, query, head of the group, keys seen.
+  auto row_at = [&](int R) {
+    Kv8SegRow x;
+    if constexpr (SEG) {
+      x = kv8_seg_row(p, seg, R);
+    } else {
+      x.b = b;
+      x.i = p.row_of(R);
+      x.hr = R - x.i * p.rep;
+      x.vis = R < rows && x.i < sp.q_len;  // (whether it is there; for queries only)
+    }
+    return x;
+  };
   const int tiles = (kend + KP_KT - 1) / KP_KT;
   const int share = tiles / p.splits, rest = tiles % p.splits;
   const int t0 = split * share + min(split, rest);
   const int t1 = t0 + share + (split < rest);
   const int n_tiles = t1 - t0;
   const size_t tile_id = (((size_t)b * p.c.kv_heads + h) * p.row_tiles + rt) * p.splits + split;
-  const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
+  // (a segment's first key is the first of a page)
+  const int pages_before = SEG ? seg.z >> p.shift : 0, table_len = p.c.max_pages - pages_before;
+  const int32_t *table = p.c.page_table + (size_t)owner * p.c.max_pages + pages_before;
 
   if (tid == 32) {
     for (int i = 0; i < KP_STAGES; ++i) {
@@ -372,7 +420,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     // are 0
     auto group_entry = [&](int t) {
       const int key = t * KP_KT + (lane & 7) * 16;
-      return t < t1 && key < kend ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : 0;
+      return t < t1 && key < kend ? kv8_page_load(table, table_len, key >> p.shift) : 0;
     };
     auto group_page = [&](int entry) {
       return max(0, kv8_page_ok(entry, p.c.pages, p.status));
@@ -457,7 +505,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     // ================================================== softmax, a thread per row
     kp_regs_inc<KP_R_SOFT>();
     const int hf = wg - 2, r = tid & 127, R = r_base + r;  // tiles hf, hf + 2, ...; S slot hf
-    const int vis = R < rows ? sp.visible(p.row_of(R)) : 0;
+    int vis;
+    if constexpr (SEG)
+      vis = R < rows ? row_at(R).vis : 0;
+    else
+      vis = R < rows ? sp.visible(p.row_of(R)) : 0;
     const bool one = n_tiles == 1;
     const float shift = one ? KP_SHIFT_ONE : KP_SHIFT;
     float m = -INFINITY, l = 0.f, lvref = KP_NO_SCALE;
@@ -465,7 +517,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     // and log2 of the V scale, loaded two tiles ahead, page numbers four
     auto group_entry = [&](int t) {
       const int key = t * KP_KT + (lane & 7) * 16;
-      return t < t1 && key < kend ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : -1;
+      return t < t1 && key < kend ? kv8_page_load(table, table_len, key >> p.shift) : -1;
     };
     auto group_scales = [&](int entry, float &ks, float &vs) {
       const bool there = (unsigned)entry < (unsigned)p.c.pages;
@@ -485,10 +537,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     if (n_tiles > 0) {
 #pragma unroll 2
       for (int qr = qtid / LPR; qr < 128; qr += PASS) {
-        const int Rq = r_base + qr, i = p.row_of(Rq), hr = Rq - i * p.rep;
+        const Kv8SegRow x = row_at(r_base + qr);
         const uint16_t *src =
-            p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql + c8 * 8;
-        const bool there = Rq < rows && i < sp.q_len;
+            p.q + x.b * p.qb + (int64_t)(h * p.rep + x.hr) * p.qh + (int64_t)x.i * p.ql + c8 * 8;
+        const bool there = x.vis > 0;
         if (there && p.vec)
           cp_async16(place(qr), src);
         else
@@ -714,7 +766,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       const size_t row = ((size_t)b * p.Hq + h * p.rep + hr) * p.L + i;
       const bool live = R < rows;
       if (live && hf == 0) {
-        if (p.splits > 1)
+        if (SEG || p.splits > 1)
           p.ml_part[tile_id * KP_ROWS + r_pair] = make_float2(m, l);
         else if (p.lse)
           p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
@@ -722,7 +774,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       // the warp's 32 rows x 32 dims go through the queries' place, which no product
       // reads any more, so that a store covers whole 64-byte pieces of 8 rows
       uint8_t *turn = smem + (warp - 8) * 2048;
-      const float inv = p.splits > 1 ? v : l == 0.f ? 0.f : v / l;
+      const float inv = SEG || p.splits > 1 ? v : l == 0.f ? 0.f : v / l;
 #pragma unroll 1
       for (int c0 = hf * (D / 2); c0 < (hf + 1) * (D / 2); c0 += 32) {
         uint32_t x[32];
@@ -737,7 +789,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(x[j]) * inv;
         __syncwarp();
-        if (p.splits > 1) {
+        if (SEG || p.splits > 1) {
           if (live && n_tiles > 0) {
             float *d = p.o_part + (tile_id * KP_ROWS + r_pair) * D + c0;
 #pragma unroll
@@ -782,26 +834,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
                  : "memory");
 }
 
-template <int D>
+template <int D, bool SEG>
 int kp_launch(const Kv8AttnParams &p, cudaStream_t s) {
   using H = KpShape<D>;
   static std::atomic<uint64_t> ready{0};
   const int rc = once_per_device(ready, [] {
     cudaFuncAttributes fa;
-    cudaError_t e = cudaFuncGetAttributes(&fa, kv8_prefill_kernel<D>);
+    cudaError_t e = cudaFuncGetAttributes(&fa, kv8_prefill_kernel<D, SEG>);
     // the warpgroups' register shares add up to 128 per thread at launch
     if (e == cudaSuccess && fa.numRegs != 128)
       return set_error(VB_ERR_CUDA, "kv8_prefill_kernel: built with %d registers, 128 needed",
                        fa.numRegs);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(kv8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      e = cudaFuncSetAttribute(kv8_prefill_kernel<D, SEG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                H::SMEM);
     return e == cudaSuccess ? VB_OK
                             : set_error(VB_ERR_CUDA, "kv8_prefill_kernel attributes: %s",
                                         cudaGetErrorString(e));
   });
   if (rc != VB_OK) return rc;
-  vb_launch(kv8_prefill_kernel<D>, dim3(2 * p.row_tiles * p.splits * p.c.kv_heads * p.c.batch),
+  vb_launch(kv8_prefill_kernel<D, SEG>,
+            dim3(2 * p.row_tiles * p.splits * p.c.kv_heads * (SEG ? p.n_segs : p.c.batch)),
             dim3(KP_THREADS), H::SMEM, s, false, p);
   return check_launch("kv8_prefill_kernel");
 }
@@ -812,9 +865,17 @@ int kv8_prefill_rows() { return KP_ROWS; }
 
 int kv8_prefill_launch(const Kv8AttnParams &p, cudaStream_t s) {
   switch (p.c.dim) {
-    case 64: return kp_launch<64>(p, s);
-    case 128: return kp_launch<128>(p, s);
-    default: return kp_launch<256>(p, s);
+    case 64: return kp_launch<64, false>(p, s);
+    case 128: return kp_launch<128, false>(p, s);
+    default: return kp_launch<256, false>(p, s);
+  }
+}
+
+int kv8_prefill_launch_segments(const Kv8AttnParams &p, cudaStream_t s) {
+  switch (p.c.dim) {
+    case 64: return kp_launch<64, true>(p, s);
+    case 128: return kp_launch<128, true>(p, s);
+    default: return kp_launch<256, true>(p, s);
   }
 }
 

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import (VbKv8AppendArgs, VbKv8AttnArgs, VbKv8Cache, VbKv8EvictArgs, VbKv8ReadArgs,
-                   VbKv8WeighArgs, check, lib)
+                   VbKv8SharedArgs, VbKv8WeighArgs, check, lib)
 from .pool import current_device, current_stream, on_device, ptr, status_ptr
 from .scratch import Scratch
 
@@ -66,6 +66,40 @@ def _strides(t: torch.Tensor):
             _STRIDES.clear()
         a = _STRIDES[s] = (C.c_int64 * 3)(*s[:3])
     return a
+
+
+class SharedPrefix:
+    """Which sequences of a batch share the rows they begin with: ``groups`` of
+    ``(first, count, rows)``, the ``count`` sequences from ``first`` on whose first
+    ``rows`` rows (whole pages) are the same pool pages in the page table of each of
+    them, as far as it holds that many keys; in order, each sequence in one group at
+    most. For :meth:`PagedKV8Cache.attend_shared` of ``cache`` and of every other one
+    with its batch, page size and device, as those of the other layers. A CUDA graph
+    keeps the groups it was captured with."""
+
+    def __init__(self, cache: "PagedKV8Cache", groups):
+        self.batch, self.page, self.device = cache.batch, cache.page, cache.device
+        self.groups = tuple((int(f), int(n), int(rows)) for f, n, rows in groups)
+        end, most = 0, cache.page_table.shape[1] * self.page
+        for first, count, rows in self.groups:
+            if first < end or count < 1 or first + count > self.batch or rows < self.page \
+                    or rows % self.page or rows > most:
+                raise ValueError(f"group {(first, count, rows)}: sequences of {self.batch} in order,"
+                                 f" rows in whole pages of {self.page}, at most {most}")
+            end = first + count
+        # a group of one gains nothing: its sequence is attended as a whole
+        kept = [g for g in self.groups if g[1] > 1]
+        group_of, start = [-1] * self.batch, [0] * self.batch
+        for g, (first, count, rows) in enumerate(kept):
+            group_of[first:first + count] = [g] * count
+            start[first:first + count] = [rows] * count
+        segments = [(f, n, 0, rows) for f, n, rows in kept]
+        segments += [(b, 1, s, 0x7fffffff) for b, s in enumerate(start)]
+        self._segments = torch.tensor(segments, dtype=torch.int32, device=self.device)
+        self._group_of = torch.tensor(group_of, dtype=torch.int32, device=self.device)
+        self._host = (C.c_int32 * (3 * len(kept)))(*[x for g in kept for x in g])
+        self._count = len(kept)
+        self._need: dict = {}  # workspace bytes by (cache layout, q_heads, L)
 
 
 class PagedKV8Cache:
@@ -119,6 +153,7 @@ class PagedKV8Cache:
         self._attn_args = bytes(VbKv8AttnArgs(c))
         self._weigh_args = bytes(VbKv8WeighArgs(c))
         self._evict_args = bytes(VbKv8EvictArgs(c))
+        self._shared_args = bytes(VbKv8SharedArgs(VbKv8AttnArgs(c)))
         self._need = {}  # workspace bytes by (q_heads, L), of evict by (room, keep)
 
     @classmethod
@@ -207,6 +242,75 @@ class PagedKV8Cache:
             with on_device(self.device, stream):
                 return self.attend(q, lens, q_lens, len_add, scale, causal, out, return_lse,
                                    status, workspace=workspace)
+        dev = self._index
+        a = VbKv8AttnArgs.from_buffer_copy(self._attn_args)
+        q, out, lse = self._attn_fill(a, q, lens, q_lens, len_add, scale, causal, out, return_lse,
+                                      status)
+        Hq, L = a.q_heads, a.L
+        need = self._need.get((Hq, L))
+        if need is None:
+            need = self._need[Hq, L] = lib.vb_kv8_attn_workspace_size(C.byref(a))
+        st = current_stream(dev)
+        self._attn_workspace(a, workspace, need, st)
+        check(lib.vb_kv8_attn(C.byref(a), st), "vb_kv8_attn")
+        return (out, lse) if return_lse else out
+
+    def attend_shared(self, q, lens, shared: SharedPrefix, q_lens=None, len_add: int = 0,
+                      scale: float | None = None, causal: bool = True, out=None,
+                      return_lse: bool = False, status=None, stream=None, workspace=None):
+        """What :meth:`attend` gives for a batch whose sequences share the rows they
+        begin with in groups (:class:`SharedPrefix`): those are read, and multiplied,
+        once for the query rows of all sequences of a group. ``lens`` and positions
+        count the shared rows, as in every other call. ``workspace``: as in
+        :meth:`attend`, of :meth:`shared_workspace_size` bytes."""
+        if stream is not None or current_device() != self._index:
+            with on_device(self.device, stream):
+                return self.attend_shared(q, lens, shared, q_lens, len_add, scale, causal, out,
+                                          return_lse, status, workspace=workspace)
+        if not shared._count:
+            self._shared_fits(shared)
+            return self.attend(q, lens, q_lens, len_add, scale, causal, out, return_lse, status,
+                               workspace=workspace)
+        s, dev = self._shared_fill(shared), self._index
+        q, out, lse = self._attn_fill(s.attn, q, lens, q_lens, len_add, scale, causal, out,
+                                      return_lse, status)
+        st = current_stream(dev)
+        self._attn_workspace(s.attn, workspace, self._shared_need(shared, s), st)
+        check(lib.vb_kv8_attn_shared(C.byref(s), st), "vb_kv8_attn_shared")
+        return (out, lse) if return_lse else out
+
+    def shared_workspace_size(self, shared: SharedPrefix, q_heads: int, L: int) -> int:
+        """Bytes of scratch that :meth:`attend_shared` needs for ``L`` rows of
+        ``q_heads`` heads with the present page table."""
+        if not shared._count:
+            return self.attend_workspace_size(q_heads, L)
+        s = self._shared_fill(shared)
+        s.attn.q_heads, s.attn.L = q_heads, L
+        return self._shared_need(shared, s)
+
+    def _shared_fits(self, shared: SharedPrefix):
+        if shared.batch != self.batch or shared.page != self.page or shared.device != self.device:
+            raise ValueError(f"shared: groups of {shared.batch} sequences in pages of {shared.page} "
+                             f"on {shared.device}, the cache has {self.batch} in pages of "
+                             f"{self.page} on {self.device}")
+
+    def _shared_fill(self, shared: SharedPrefix) -> VbKv8SharedArgs:
+        self._shared_fits(shared)
+        s = VbKv8SharedArgs.from_buffer_copy(self._shared_args)
+        s.segments, s.group_of = shared._segments.data_ptr(), shared._group_of.data_ptr()
+        s.host_groups, s.groups = C.addressof(shared._host), shared._count
+        return s
+
+    def _shared_need(self, shared: SharedPrefix, s: VbKv8SharedArgs) -> int:
+        key = (self.kv_heads, self.head_dim, self._table.shape[1], s.attn.q_heads, s.attn.L)
+        need = shared._need.get(key)
+        if need is None:
+            need = shared._need[key] = lib.vb_kv8_attn_shared_workspace_size(C.byref(s))
+        return need
+
+    def _attn_fill(self, a: VbKv8AttnArgs, q, lens, q_lens, len_add, scale, causal, out,
+                   return_lse, status):
+        """Checks the arguments of attention and puts them into ``a``."""
         B, D, dev = self.batch, self.head_dim, self._index
         if q.dim() != 4:
             raise ValueError(f"q: [batch, q_heads, L, head_dim] is needed, got {tuple(q.shape)}")
@@ -219,7 +323,6 @@ class PagedKV8Cache:
             raise ValueError(f"out: contiguous bfloat16 of q's shape on cuda:{dev} is needed, got "
                              f"{out.dtype} {tuple(out.shape)} on {out.device}")
         lse = q.new_empty((B, Hq, L), dtype=torch.float32) if return_lse else None
-        a = VbKv8AttnArgs.from_buffer_copy(self._attn_args)
         a.q, a.q_strides = q.data_ptr(), _strides(q)
         a.lens, a.q_lens = _ints(lens, "lens", B, dev), _ints(q_lens, "q_lens", B, dev)
         a.out, a.lse = out.data_ptr(), ptr(lse)
@@ -227,10 +330,10 @@ class PagedKV8Cache:
             a.status = status_ptr(status, dev)
         a.scale = D ** -0.5 if scale is None else scale
         a.q_heads, a.L, a.len_add, a.causal = Hq, L, len_add, causal
-        need = self._need.get((Hq, L))
-        if need is None:
-            need = self._need[Hq, L] = lib.vb_kv8_attn_workspace_size(C.byref(a))
-        st = current_stream(dev)
+        return q, out, lse
+
+    def _attn_workspace(self, a: VbKv8AttnArgs, workspace, need: int, st: int):
+        dev = self._index
         if workspace is not None:
             if workspace.dtype != torch.uint8 or workspace.get_device() != dev \
                     or not workspace.is_contiguous():
@@ -240,8 +343,6 @@ class PagedKV8Cache:
         elif need:
             ws = _scratch.get(need, self.device, st)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        check(lib.vb_kv8_attn(C.byref(a), st), "vb_kv8_attn")
-        return (out, lse) if return_lse else out
 
     def attend_workspace_size(self, q_heads: int, L: int) -> int:
         """Bytes of scratch that :meth:`attend` needs for ``L`` rows of
@@ -350,4 +451,4 @@ class PagedKV8Cache:
         return after
 
 
-__all__ = ["PagedKV8Cache"]
+__all__ = ["PagedKV8Cache", "SharedPrefix"]
