@@ -596,8 +596,8 @@ int vb_kv8_attn(const VbKv8AttnArgs *args, vb_stream_t stream);
  * same pool pages in the table of each of them as far as it holds that many keys).
  * segments int32 [groups + batch][4], device: {first, sequences, 0, rows} per group,
  * then {b, 1, rows of its group or 0, 2^31 - 1} per sequence; group_of int32 [batch],
- * device: the group or -1. workspace: vb_kv8_attn_shared_workspace_size bytes, its
- * head as in vb_kv8_attn. batch * kv_heads <= 16384. */
+ * device: the group or -1. workspace: vb_kv8_attn_shared_workspace_size bytes, whose
+ * first VB_KV8_ATTN_WORKSPACE_HEAD are left as they are. */
 typedef struct VbKv8SharedArgs {
   VbKv8AttnArgs attn;
   const int32_t *segments, *group_of, *host_groups;

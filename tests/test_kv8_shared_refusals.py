@@ -36,7 +36,7 @@ def test_groups(groups):
                                  dict(attn=dict(workspace=FAKE + 8)), dict(segments=None),
                                  dict(segments=FAKE + 4), dict(group_of=None),
                                  dict(host_groups=None), dict(cache=dict(dim=96)),
-                                 dict(cache=dict(batch=16384, kv_heads=2))], ids=str)
+                                 dict(cache=dict(batch=65535, kv_heads=256), attn=dict(q_heads=256))], ids=str)
 def test_refusals(bad):
     assert lib.vb_kv8_attn_shared(C.byref(_args(**bad)), None) == 1
     assert lib.vb_last_error()

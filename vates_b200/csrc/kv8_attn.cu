@@ -213,8 +213,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
   for (int z = blockIdx.x; z < B; z += gridDim.x) {
     if (kv8_tiles<KT, SEG>(p, z, false) > 0) continue;
     if constexpr (SEG) {
-      for (int i = tid; i < H * ROWS; i += KA_THREADS)
-        p.ml_res[(size_t)z * H * ROWS + i] = make_float2(-INFINITY, 0.f);
+      for (int i = tid; i < H; i += KA_THREADS) p.units[(size_t)z * H + i] = make_int2(0, 0);
       continue;
     }
     const size_t row0 = (size_t)z * p.Hq * p.L, n = (size_t)p.Hq * p.L;
@@ -658,7 +657,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
         }
       }
     // the CTAs that share the unit: s_share[1] from s_share[0] on
-    if (!whole && p.wide && !SEG) {
+    if (SEG || (!whole && p.wide)) {  // another kernel does
       if (t0 == 0 && tid == 0)
         p.units[b * H + h] =
             make_int2(blockIdx.x, (int)(deal.owner(u0 + tiles - 1) - blockIdx.x) + 1);
@@ -735,19 +734,11 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
 #pragma unroll
           for (int i = 0; i < IG; ++i) {
             const int r = r0 + (i0 + i) * RT;
-            if constexpr (SEG) {
-              const size_t row = ((size_t)b * H + h) * ROWS + r;
-              if (r < rows) {
-                *(reinterpret_cast<float4 *>(p.o_res + row * D) + d4) = a[i];
-                if (d4 == 0) p.ml_res[row] = make_float2(s_max[0][r], s_l[0][r]);
-              }
-            } else if (r < rows) {
-              kv8_finish(p, D, b, h, r, d4, s_max[0][r], s_l[0][r], a[i]);
-            }
+            if (r < rows) kv8_finish(p, D, b, h, r, d4, s_max[0][r], s_l[0][r], a[i]);
           }
         }
       }
-    } else if (p.wide && !SEG && tid == 0) {
+    } else if (p.wide && tid == 0) {
       p.units[b * H + h] = make_int2(blockIdx.x, 1);
     }
     if (w0 < w1) __syncthreads();  // s_l has been read
@@ -1009,14 +1000,45 @@ int kv8_run(const Kv8AttnParams &p, const Kv8Plan &pl, cudaStream_t s) {
 // of all of them, the keys of each alone after it by its own rows, and the results
 // of both are joined: weights 2^(m - M) of a row's partial results.
 struct Kv8Parted {             // where the results of some segments are
+  const float *o, *o_part;
+  const float2 *ml, *ml_part;
+  // kv8_attn_kernel: its units, from unit `first` on: one result of each row (o, ml), or
+  // several (o_part, ml_part): slot 1 of the unit's first CTA and slot 0 of the following
+  // ones. The prefill kernel (null): `splits` of each row tile.
+  const int2 *units;
+  int first, tile_rows, row_tiles, splits;
+};
+// One row's results in there.
+struct Kv8PartedRow {
   const float *o;
   const float2 *ml;
-  int tile_rows, row_tiles, splits;
-  __device__ size_t at(int u, int H, int h, int R, int s) const {
-    const int t = R / tile_rows;
-    return (((size_t)(u * H + h) * row_tiles + t) * splits + s) * tile_rows + R - t * tile_rows;
-  }
+  int n, step, skip;           // rows from one result to the next; less once
+  __device__ int at(int s) const { return s * step - (s > 0 ? skip : 0); }
 };
+template <int D>
+__device__ __forceinline__ Kv8PartedRow kv8_parted_row(const Kv8Parted &q, int unit, int R) {
+  Kv8PartedRow x;
+  size_t row;
+  x.skip = 0;
+  if (q.units) {
+    unit += q.first;
+    const int2 u = __ldcg(q.units + unit);
+    x.n = u.y;
+    x.step = 2 * q.tile_rows;
+    x.skip = u.y > 1 ? q.tile_rows : 0;
+    row = u.y > 1 ? ((size_t)u.x * 2 + 1) * q.tile_rows + R : (size_t)unit * q.tile_rows + R;
+    x.o = (u.y > 1 ? q.o_part : q.o) + row * D;
+    x.ml = (u.y > 1 ? q.ml_part : q.ml) + row;
+  } else {
+    const int t = R / q.tile_rows;
+    x.n = q.splits;
+    x.step = q.tile_rows;
+    row = ((size_t)unit * q.row_tiles + t) * q.splits * q.tile_rows + R - t * q.tile_rows;
+    x.o = q.o + row * D;
+    x.ml = q.ml + row;
+  }
+  return x;
+}
 struct Kv8SharedParams {
   Kv8AttnParams p;
   Kv8Parted pre, own;
@@ -1024,66 +1046,104 @@ struct Kv8SharedParams {
   const int32_t *group_of;     // per sequence, -1: none
 };
 
-// A thread joins four dims of one row.
-template <int D>
+// PG threads join four dims of one row, each every PG-th result, four at a time.
+template <int D, int PG>
 __global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __grid_constant__ Kv8SharedParams w) {
+  constexpr int LR = D / 4, RPC = KC_THREADS / (LR * PG), AHEAD = 4;
+  __shared__ float4 s_a[PG > 1 ? KC_THREADS : 1];
+  __shared__ float2 s_ml[PG > 1 ? KC_THREADS : 1];
   pdl_launch_dependents();
   pdl_wait();
   const Kv8AttnParams &p = w.p;
-  constexpr int RPC = KC_THREADS * 4 / D;
-  const long long row = (long long)blockIdx.x * RPC + threadIdx.x / (D / 4);
-  const int d4 = threadIdx.x % (D / 4), per = p.Hq * p.L;
-  if (row >= (long long)p.c.batch * per) return;
-  const int b = (int)(row / per), x = (int)(row - (long long)b * per);
-  const int hq = x / p.L, i = x - hq * p.L, h = hq / p.rep, R = i * p.rep + hq - h * p.rep;
-  const int H = p.c.kv_heads, g = w.group_of[b];
-  const int n_pre = g >= 0 ? w.pre.splits : 0, n = n_pre + w.own.splits;
-  const int R_pre = g >= 0 ? (b - w.groups[g].x) * p.L * p.rep + R : 0;
-  auto source = [&](int s, const float *&o, const float2 *&ml) {
-    const Kv8Parted &q = s < n_pre ? w.pre : w.own;
-    const size_t at = s < n_pre ? q.at(g, H, h, R_pre, s) : q.at(b, H, h, R, s - n_pre);
-    o = q.o + at * D;
-    ml = q.ml + at;
-  };
+  const int tid = threadIdx.x, d4 = tid % LR, pg = tid / LR % PG;
+  const int row = blockIdx.x * RPC + tid / (LR * PG), per = p.Hq * p.L;
+  const bool there = row < p.c.batch * per;
+  int b = 0, h = 0, R = 0;
   float M = -INFINITY, ls = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float *o;
-    const float2 *ml;
-    source(s, o, ml);
-    M = fmaxf(M, __ldcg(ml).x);
-  }
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float *o;
-    const float2 *mlp;
-    source(s, o, mlp);
-    const float2 ml = __ldcg(mlp);
-    const float4 y = __ldcg(reinterpret_cast<const float4 *>(o) + d4);
-    const float f = ml.x == -INFINITY ? 0.f : kv8_ex2(ml.x - M);
-    ls = fmaf(f, ml.y, ls);
-    if (f > 0.f) {  // keys that the row does not see left no O
+  if (there) {
+    b = row / per;
+    const int x = row - b * per, hq = x / p.L, i = x - hq * p.L, H = p.c.kv_heads;
+    h = hq / p.rep;
+    R = i * p.rep + hq - h * p.rep;
+    const int g = w.group_of[b];
+    Kv8PartedRow pre, own = kv8_parted_row<D>(w.own, b * H + h, R);
+    pre.n = 0;
+    if (g >= 0) pre = kv8_parted_row<D>(w.pre, g * H + h, (b - w.groups[g].x) * p.L * p.rep + R);
+    const int n = pre.n + own.n;
+    for (int s0 = pg; s0 < n; s0 += PG * AHEAD) {
+      float2 ml[AHEAD];
+      float4 y[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int s = s0 + k * PG;
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (s < n) {  // (keys that the row does not see left no O: it is not used)
+          const Kv8PartedRow &q = s < pre.n ? pre : own;
+          const int at = q.at(s < pre.n ? s : s - pre.n);
+          ml[k] = __ldcg(q.ml + at);
+          y[k] = __ldcg(reinterpret_cast<const float4 *>(q.o + (size_t)at * D) + d4);
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) top = fmaxf(top, ml[k].x);
+      const float back = M == -INFINITY ? 0.f : kv8_ex2(M - top);
+      M = top;
+      ls *= back;
+      a.x *= back; a.y *= back; a.z *= back; a.w *= back;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (ml[k].x == -INFINITY) continue;
+        const float f = kv8_ex2(ml[k].x - M);
+        ls = fmaf(f, ml[k].y, ls);
+        if (f > 0.f) {
+          a.x = fmaf(f, y[k].x, a.x); a.y = fmaf(f, y[k].y, a.y);
+          a.z = fmaf(f, y[k].z, a.z); a.w = fmaf(f, y[k].w, a.w);
+        }
+      }
+    }
+  }
+  if constexpr (PG > 1) {
+    s_a[tid] = a;
+    s_ml[tid] = make_float2(M, ls);
+    __syncthreads();
+    if (pg > 0) return;
+#pragma unroll
+    for (int k = 1; k < PG; ++k) M = fmaxf(M, s_ml[tid + k * LR].x);
+    ls = 0.f;
+    a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < PG; ++k) {
+      const float2 ml = s_ml[tid + k * LR];
+      const float4 y = s_a[tid + k * LR];
+      const float f = ml.x == -INFINITY ? 0.f : kv8_ex2(ml.x - M);
+      ls = fmaf(f, ml.y, ls);
       a.x = fmaf(f, y.x, a.x); a.y = fmaf(f, y.y, a.y);
       a.z = fmaf(f, y.z, a.z); a.w = fmaf(f, y.w, a.w);
     }
   }
-  kv8_finish(p, D, b, h, R, d4, M, ls, a);
+  if (there) kv8_finish(p, D, b, h, R, d4, M, ls, a);
 }
 
-// One side of the work: the groups' segments, or each sequence's own.
+// One side of the work: the groups' segments, or each sequence's own, or both.
 struct Kv8Side {
   bool tensor;
   int tile_rows, row_tiles, splits, ctas;
-  size_t results, parts;       // rows of results, of partial results of kv8_attn_kernel
+  size_t units, results, parts;  // units; rows of results, of partial results
+  size_t bytes(int dim) const {
+    return align_up(units * sizeof(int2), 16) +
+           align_up((results + parts) * (dim + 2) * sizeof(float), 16);
+  }
 };
-// `base`: row tiles of all segments and heads, `tiles`: key tiles of the longest segment
-// (128 keys) or of all of them together (kv8_attn_kernel).
+// `base`: row tiles of all segments and heads, `longest`: key tiles of the longest
+// segment (prefill kernel), `all`: of all segments and heads (kv8_attn_kernel).
 Kv8Side kv8_side(const VbKv8AttnArgs *a, long long segs, long long rows, long long base,
                  long long longest, long long all) {
   Kv8Side s;
   const long long units = segs * a->cache.kv_heads;
   s.tensor = rows > 32;
+  s.units = s.tensor ? 0 : (size_t)units;
   if (s.tensor) {
     s.tile_rows = kv8_prefill_rows();
     s.row_tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
@@ -1101,16 +1161,19 @@ Kv8Side kv8_side(const VbKv8AttnArgs *a, long long segs, long long rows, long lo
   return s;
 }
 
+// Where both sides go through kv8_attn_kernel and there are no more key tiles than
+// CTAs, one launch does both.
 struct Kv8SharedPlan {
-  Kv8Side pre, own;
-  size_t pre_at, own_at, part_at, bytes;  // results and partial results in the workspace
+  bool both;
+  Kv8Side pre, own;            // (both: own)
+  size_t pre_at, own_at, bytes;
 };
 Kv8SharedPlan kv8_shared_plan(const VbKv8SharedArgs *s) {
   const VbKv8AttnArgs *a = &s->attn;
   const long long H = a->cache.kv_heads, rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
   const long long cap = (long long)a->cache.max_pages * a->cache.page, kt = KA_TILE / a->cache.dim;
-  const long long tile = kv8_prefill_rows();
-  long long most = 0, base = 0, longest = 0, all = 0, own = cap * a->cache.batch;
+  const long long tile = kv8_prefill_rows(), B = a->cache.batch;
+  long long most = 0, base = 0, longest = 0, all = 0, own = cap * B;
   for (int g = 0; g < s->groups; ++g) {
     const int32_t *x = s->host_groups + 3 * g;
     const long long r = x[1] * rows;
@@ -1120,32 +1183,37 @@ Kv8SharedPlan kv8_shared_plan(const VbKv8SharedArgs *s) {
     all += (x[2] + kt - 1) / kt * H;
     own -= (long long)x[1] * x[2];
   }
+  const long long own_all = (own + kt - 1) / kt * H + B * H;  // (a part of a tile each)
   Kv8SharedPlan pl;
-  pl.pre = kv8_side(a, s->groups, most, base, (longest + 127) / 128, all);
-  pl.own = kv8_side(a, a->cache.batch, rows, a->cache.batch * H * ((rows + tile - 1) / tile),
-                    (own / a->cache.batch + 127) / 128, (own + kt - 1) / kt * H);
-  const size_t width = (a->cache.dim + 2) * sizeof(float);
-  pl.pre_at = KA_TICKETS * sizeof(uint32_t);
-  pl.own_at = pl.pre_at + align_up(pl.pre.results * width, 16);
-  pl.part_at = pl.own_at + align_up(pl.own.results * width, 16);
-  const size_t parts = pl.pre.parts > pl.own.parts ? pl.pre.parts : pl.own.parts;
-  pl.bytes = pl.part_at + parts * width;
+  pl.both = most <= 32 && all + own_all <= 148 * 2;
+  if (pl.both) {
+    pl.own = pl.pre = kv8_side(a, s->groups + B, most, 0, 0, all + own_all);
+  } else {
+    pl.pre = kv8_side(a, s->groups, most, base, (longest + 127) / 128, all);
+    pl.own = kv8_side(a, B, rows, B * H * ((rows + tile - 1) / tile), (own / B + 127) / 128, own_all);
+  }
+  // (the words ahead of it are left to vb_kv8_attn, whose scratch it may be)
+  pl.pre_at = pl.own_at = KA_TICKETS * sizeof(uint32_t);
+  if (!pl.both) pl.own_at += pl.pre.bytes(a->cache.dim);
+  pl.bytes = pl.own_at + pl.own.bytes(a->cache.dim);
   return pl;
 }
 
 template <int D>
-int kv8_side_run(Kv8AttnParams p, const Kv8Side &s, uint8_t *results, Kv8Parted &out,
-                 cudaStream_t st) {
-  float *o = reinterpret_cast<float *>(results);
-  float2 *ml = reinterpret_cast<float2 *>(o + s.results * D);
-  out.o = o; out.ml = ml;
-  out.tile_rows = s.tile_rows; out.row_tiles = s.row_tiles; out.splits = s.splits;
+int kv8_side_run(Kv8AttnParams p, const Kv8Side &s, uint8_t *ws, Kv8Parted &out, cudaStream_t st) {
+  int2 *units = s.tensor ? nullptr : reinterpret_cast<int2 *>(ws);
+  float *o = reinterpret_cast<float *>(ws + align_up(s.units * sizeof(int2), 16));
+  float *o_part = o + s.results * D;
+  float2 *ml = reinterpret_cast<float2 *>(o_part + s.parts * D), *ml_part = ml + s.results;
+  out.o = o; out.o_part = o_part; out.ml = ml; out.ml_part = ml_part; out.units = units;
+  out.first = 0; out.tile_rows = s.tile_rows; out.row_tiles = s.row_tiles; out.splits = s.splits;
   p.row_tiles = s.row_tiles; p.splits = s.splits;
   if (s.tensor) {
     p.o_part = o; p.ml_part = ml;
     return kv8_prefill_launch_segments(p, st);
   }
-  p.ml_part = reinterpret_cast<float2 *>(p.o_part + s.parts * D);
+  p.units = units;
+  p.o_part = o_part; p.ml_part = ml_part;
   p.o_res = o; p.ml_res = ml;
   return s.tile_rows == 8    ? kv8_launch<D, 1, true>(p, s.ctas, st)
          : s.tile_rows == 16 ? kv8_launch<D, 2, true>(p, s.ctas, st)
@@ -1158,20 +1226,32 @@ int kv8_shared_run(Kv8AttnParams p, const Kv8SharedPlan &pl, const VbKv8SharedAr
   Kv8SharedParams w;
   w.groups = reinterpret_cast<const int4 *>(a->segments);
   w.group_of = a->group_of;
-  p.o_part = reinterpret_cast<float *>(ws + pl.part_at);
   p.segs = w.groups;
   p.n_segs = a->groups;
-  int rc = kv8_side_run<D>(p, pl.pre, ws + pl.pre_at, w.pre, s);
-  if (rc != VB_OK) return rc;
-  p.segs = w.groups + a->groups;
-  p.n_segs = p.c.batch;
-  rc = kv8_side_run<D>(p, pl.own, ws + pl.own_at, w.own, s);
-  if (rc != VB_OK) return rc;
+  if (pl.both) {
+    p.n_segs += p.c.batch;
+    const int rc = kv8_side_run<D>(p, pl.own, ws + pl.own_at, w.own, s);
+    if (rc != VB_OK) return rc;
+    w.pre = w.own;
+    w.own.first = a->groups * p.c.kv_heads;
+  } else {
+    int rc = kv8_side_run<D>(p, pl.pre, ws + pl.pre_at, w.pre, s);
+    if (rc != VB_OK) return rc;
+    p.segs += a->groups;
+    p.n_segs = p.c.batch;
+    rc = kv8_side_run<D>(p, pl.own, ws + pl.own_at, w.own, s);
+    if (rc != VB_OK) return rc;
+  }
   w.p = p;
-  constexpr int RPC = KC_THREADS * 4 / D;
   const long long rows = (long long)p.c.batch * p.Hq * p.L;
-  vb_launch(kv8_shared_join_kernel<D>, dim3((unsigned)((rows + RPC - 1) / RPC)), dim3(KC_THREADS), 0,
-            s, true, w);
+  // few rows: four threads for each four dims
+  constexpr int RPC = KC_THREADS * 4 / D;
+  if (rows <= 8192)
+    vb_launch(kv8_shared_join_kernel<D, 4>, dim3((unsigned)((rows * 4 + RPC - 1) / RPC)),
+              dim3(KC_THREADS), 0, s, true, w);
+  else
+    vb_launch(kv8_shared_join_kernel<D, 1>, dim3((unsigned)((rows + RPC - 1) / RPC)),
+              dim3(KC_THREADS), 0, s, true, w);
   return check_launch("kv8_shared_join_kernel");
 }
 
@@ -1222,8 +1302,8 @@ int kv8_shared_check(const VbKv8SharedArgs *s) {
                g, x[0], x[1], c.batch, x[2], c.page, c.max_pages);
     end = x[0] + x[1];
   }
-  VB_REQUIRE((long long)c.batch * c.kv_heads <= KA_TICKETS &&
-                 (long long)c.batch * s->attn.q_heads * s->attn.L <= 1 << 28,
+  VB_REQUIRE((long long)c.batch * s->attn.q_heads * s->attn.L <= 1 << 28 &&
+                 2ll * c.batch * c.kv_heads <= 1 << 24,
              "vb_kv8_attn_shared: %d sequences of %d kv heads, %d rows of %d heads each", c.batch,
              c.kv_heads, s->attn.L, s->attn.q_heads);
   return VB_OK;
@@ -1298,7 +1378,6 @@ int vb_kv8_attn_shared(const VbKv8SharedArgs *s, vb_stream_t stream) {
   VB_REQUIRE(((uintptr_t)a->workspace % 16) == 0, "vb_kv8_attn_shared: workspace alignment");
   Kv8AttnParams p = kv8_params(a);
   uint8_t *ws = static_cast<uint8_t *>(a->workspace);
-  p.tickets = reinterpret_cast<uint32_t *>(ws);
   cudaStream_t st = as_stream(stream);
   switch (a->cache.dim) {
     case 64: return kv8_shared_run<64>(p, pl, s, ws, st);

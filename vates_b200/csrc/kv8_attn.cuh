@@ -28,9 +28,9 @@ struct Kv8AttnParams {
   uint32_t rep_inv;  // floor(2^32 / rep) + 1
   // Segments in the place of sequences: (first sequence, sequences, first key, end):
   // all query rows of those sequences over the keys [first, end) that they have in
-  // common, at most as far as each row sees. Their results, rows of unnormalised O and
-  // (m, l), are joined later: by kv8_attn_kernel one per row, in o_res and ml_res; by
-  // the prefill kernel one per range of keys, as above.
+  // common, at most as far as each row sees. Another kernel joins their results, rows of
+  // unnormalised O and (m, l): partial results as above, and for a unit that one CTA of
+  // kv8_attn_kernel has whole, in o_res and ml_res.
   const int4 *segs;
   int n_segs;
   float *o_res;
