@@ -616,7 +616,8 @@ int vb_kv8_attn_shared(const VbKv8SharedArgs *args, vb_stream_t stream);
  * takes position seen[b] - keys_b + j, seen[b] the tokens of the sequence so far.
  * Rows from keys_b on are left as they are. A query row whose lse is not finite
  * adds nothing (VB_STATUS_NONFINITE but for -inf). A sequence with more keys than
- * room is left as it is (VB_STATUS_BOUNDS). */
+ * room is left as it is (VB_STATUS_BOUNDS). workspace: vb_kv8_weigh_workspace_size
+ * bytes (0 up to 32 rows per kv head). */
 typedef struct VbKv8WeighArgs {
   VbKv8Cache cache;
   const uint16_t *q;
@@ -629,9 +630,12 @@ typedef struct VbKv8WeighArgs {
   float *weights;
   int32_t *positions; /* nullable */
   int32_t *status;    /* nullable */
+  void *workspace;
+  size_t workspace_bytes;
   float scale;
   int32_t q_heads, L, len_add, causal, room;
 } VbKv8WeighArgs;
+size_t vb_kv8_weigh_workspace_size(const VbKv8WeighArgs *args);
 int vb_kv8_weigh(const VbKv8WeighArgs *args, vb_stream_t stream);
 
 /* Evict rows: of every sequence with n = lens[b] > keep rows, each kv head keeps

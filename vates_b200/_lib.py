@@ -79,7 +79,8 @@ class VbKv8WeighArgs(C.Structure):
     _fields_ = [("cache", VbKv8Cache), ("q", C.c_void_p), ("q_strides", C.c_int64 * 3),
                 ("lse", C.c_void_p), ("lens", C.c_void_p), ("q_lens", C.c_void_p),
                 ("fresh", C.c_void_p), ("seen", C.c_void_p), ("weights", C.c_void_p),
-                ("positions", C.c_void_p), ("status", C.c_void_p), ("scale", C.c_float),
+                ("positions", C.c_void_p), ("status", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("scale", C.c_float),
                 ("q_heads", C.c_int32), ("L", C.c_int32), ("len_add", C.c_int32),
                 ("causal", C.c_int32), ("room", C.c_int32)]
 
@@ -222,6 +223,7 @@ _SIGNATURES = {
     "vb_kv8_attn": (_I32, [C.POINTER(VbKv8AttnArgs), _P]),
     "vb_kv8_attn_shared_workspace_size": (_SZ, [C.POINTER(VbKv8SharedArgs)]),
     "vb_kv8_attn_shared": (_I32, [C.POINTER(VbKv8SharedArgs), _P]),
+    "vb_kv8_weigh_workspace_size": (_SZ, [C.POINTER(VbKv8WeighArgs)]),
     "vb_kv8_weigh": (_I32, [C.POINTER(VbKv8WeighArgs), _P]),
     "vb_kv8_evict_workspace_size": (_SZ, [C.POINTER(VbKv8EvictArgs)]),
     "vb_kv8_evict": (_I32, [C.POINTER(VbKv8EvictArgs), _P]),

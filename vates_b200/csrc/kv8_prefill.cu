@@ -39,7 +39,7 @@
 // For heads of 64 it is the softmax (a tile 1.1 us; exponentials alone fill 0.55). A
 // launch without keys takes 4.6 us, one with a single tile 8.9 (heads of 256: 6.2, 13.6).
 #include "kv8_attn.cuh"
-#include "tc100.cuh"
+#include "kv8_pair.cuh"
 
 namespace vb {
 namespace {
@@ -48,8 +48,6 @@ constexpr int KP_THREADS = 512;
 constexpr int KP_KT = 128;              // keys per tile
 constexpr int KP_STAGES = 2;            // K, and V, operand tiles
 constexpr int KP_ROWS = 256;            // query rows of a pair of CTAs
-constexpr int KP_BLOCK = 16384;         // 128 rows x 64 f16, 128-byte swizzle
-constexpr uint64_t KP_WAIT_NS = 2000000000ull;
 // Weights as f16 are 2^(z - m) s_V / v, m the row's maximum less a shift, at most
 // 2^15.5: m is rounded up and what a score may reach down, so that this holds for scores
 // of any size. A range of one tile knows its maximum and its largest V scale at once and
@@ -82,10 +80,6 @@ struct KpShape {
 constexpr int KP_R_MMA = 56, KP_R_CONV = 136, KP_R_SOFT = 160;
 static_assert(KP_R_MMA + KP_R_CONV + 2 * KP_R_SOFT == 4 * 128, "register shares");
 
-// Byte offset of 16-byte chunk c of row r in a 128-row x 64-column block.
-__device__ __forceinline__ uint32_t kp_sw(int r, int c) {
-  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
-}
 // MN-major operand, 128-byte swizzle: lines of 64 elements along N, 8-line
 // groups along K 1024 bytes apart, 64-element column blocks KP_BLOCK apart.
 __device__ __forceinline__ uint64_t kp_desc_mn(uint32_t saddr) {
@@ -96,10 +90,6 @@ __device__ __forceinline__ uint64_t kp_desc_mn(uint32_t saddr) {
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
   return d;
-}
-__host__ __device__ constexpr uint32_t kp_idesc(int N, bool b_mn) {  // f16 x f16 -> f32, M = 256
-  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
-         ((uint32_t)(256 >> 4) << 24);
 }
 // The order of volatile statements is kept, so a group's exponentials are issued
 // back to back.
@@ -115,23 +105,6 @@ __device__ __forceinline__ float kp_max3(uint32_t a, uint32_t b, uint32_t c) {
   return r;
 }
 
-// The pair's products, issued by one thread of CTA 0: rows 0-127 of A and D are
-// CTA 0's, 128-255 CTA 1's; each holds half of B's N. The whole warp comes here
-// (its values are then uniform); `one` is true in the lane that issues.
-__device__ __forceinline__ uint32_t kp_elect() {
-  uint32_t r;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n"
-               : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void kp_mma_ss(uint32_t one, uint32_t d_tmem, uint64_t adesc,
-                                          uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-      " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
-      : "memory");
-}
 __device__ __forceinline__ void kp_mma_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem,
                                           uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -139,33 +112,6 @@ __device__ __forceinline__ void kp_mma_ts(uint32_t one, uint32_t d_tmem, uint32_
       " @q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(one)
       : "memory");
-}
-// Arrive on this barrier of both CTAs once all products issued so far are done.
-__device__ __forceinline__ void kp_commit(uint32_t one, uint64_t *bar) {
-  asm volatile(
-      "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
-      " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster"
-      ".b64 [%0], %1;\n}\n" ::"r"(tc::smem_u32(bar)),
-      "h"((uint16_t)3), "r"(one)
-      : "memory");
-}
-// Arrive on CTA 0's barrier, from either CTA. What the arrival stands for is
-// ordered before it on its own SM: operands in shared memory by the proxy fence,
-// P and O in TMEM by tcgen05.wait. A release of cluster scope in its place costs
-// about 1,300 cycles an arrival.
-__device__ __forceinline__ void kp_arrive_leader(uint64_t *bar) {
-  asm volatile(
-      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n"
-      " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(tc::smem_u32(bar))
-      : "memory");
-}
-// Relaxed: nothing of what a thread has written to global memory needs to be there
-// for the other CTA, and waiting for it cost most of a microsecond.
-__device__ __forceinline__ void kp_cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void kp_cluster_wait() {
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The 256 softmax threads of a CTA meet; one half of them hands over to the other
 // (`from`: the warpgroup that arrives).
@@ -444,26 +390,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         vr[i] = ldg_nc_v4(vbase + pg * pool_step + (key & (p.c.page - 1)) * D);
       }
     };
-    // 16 codes of chunk ch -> two 16-byte chunks of row r; neighbouring 64-dim
-    // blocks store them in opposite order so that the eight lanes of a store pass
-    // hit all banks
-    auto store = [&](const uint4 &x, uint8_t *tile, int block, int r, int ch) {
-      const int e0 = (ch >> 2) & 1, c = 2 * (ch & 3);
-      const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u,
-                             x.w ^ 0x80808080u};
-      uint4 o[2];
-      o[0] = make_uint4(h2_codes(__byte_perm(w[0], 0x64646464u, 0x4140)),
-                        h2_codes(__byte_perm(w[0], 0x64646464u, 0x4342)),
-                        h2_codes(__byte_perm(w[1], 0x64646464u, 0x4140)),
-                        h2_codes(__byte_perm(w[1], 0x64646464u, 0x4342)));
-      o[1] = make_uint4(h2_codes(__byte_perm(w[2], 0x64646464u, 0x4140)),
-                        h2_codes(__byte_perm(w[2], 0x64646464u, 0x4342)),
-                        h2_codes(__byte_perm(w[3], 0x64646464u, 0x4140)),
-                        h2_codes(__byte_perm(w[3], 0x64646464u, 0x4342)));
-      uint8_t *base = tile + (ch >> 2) * block;
-      *reinterpret_cast<uint4 *>(base + kp_sw(r, c + e0)) = e0 ? o[1] : o[0];
-      *reinterpret_cast<uint4 *>(base + kp_sw(r, c + 1 - e0)) = e0 ? o[0] : o[1];
-    };
     auto publish = [&](uint64_t *full) {
       tc::fence_proxy_async_smem();
       __syncwarp();
@@ -482,7 +408,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         if (n + 1 >= KP_STAGES && !wait(&bar.k_empty[st], (n + 1) / KP_STAGES - 1)) break;
         uint8_t *tile = smem + H::K_OFF + st * H::K_HALF;
 #pragma unroll
-        for (int i = 0; i < KN; ++i) store(kr[i], tile, H::K_BLOCK, kkey + i * KSTEP, kch);
+        for (int i = 0; i < KN; ++i) kp_store_codes(kr[i], tile, H::K_BLOCK, kkey + i * KSTEP, kch);
         publish(&bar.k_full[st]);
       }
       const int id_next = group_page(entry);  // before rows are asked for: it would wait for them
@@ -493,7 +419,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
         if (has_v) {
           uint8_t *tile = smem + H::V_OFF + st * H::V_HALF;
 #pragma unroll
-          for (int i = 0; i < VN; ++i) store(vr[i], tile, KP_BLOCK, vkey + i * VSTEP, vch);
+          for (int i = 0; i < VN; ++i) kp_store_codes(vr[i], tile, KP_BLOCK, vkey + i * VSTEP, vch);
         }
         publish(&bar.v_full[st]);
         if (has_v) load_v(id_v);

@@ -5,20 +5,25 @@
 //
 // with lse_i from the attention itself, so no row needs another key than j and
 // V is not read. The products are those of the attention kernels: codes and
-// queries (after a power of two per row) are exact in f16, sums float32.
+// queries (after a power of two per row) are exact in f16, sums float32, and a
+// key's weights are added in one order, whatever the launch.
 //
-// A warp takes 16 keys at a time straight from global memory into the fragments
-// of the product S^T = K q^T (lane (g, c) has 16 consecutive bytes of keys g and
-// g + 8, four k-steps), and all query rows of the kv head in turn, 8 to a
-// fragment, from shared memory. A key's weights are added up in the lane, then
-// over the four lanes that have the key: one order, whatever the launch.
-#include "kv8_attn.cuh"
+// Up to 32 query rows per kv head (kv8_weigh_kernel, HBM-bound: a byte per cached
+// value of K): a warp takes 16 keys at a time, brought by cp.async into a ring of
+// its own in which every lane finds the 16-byte pieces that it asked for itself,
+// already in the order of the fragments of S^T = K q^T (lane (g, c) has 16
+// consecutive bytes of keys g and g + 8, four k-steps), so that nothing in the
+// loop waits for another thread. Rows come eight to a fragment.
+//
+// More rows (kv8_weigh_rows_kernel, a window at a prompt's end or a prompt's chunk;
+// tensor-core- and exponential-bound): a pair of CTAs (tcgen05 cta_group::2) takes
+// 256 keys at a time, 128 each, as the M rows of the product and 64 to 256 query
+// rows as its N columns, so a thread has a key in its TMEM lane and adds its
+// weights by itself. Queries are made ready once by a kernel ahead of it.
+#include "kv8_pair.cuh"
 
 namespace vb {
 namespace {
-
-constexpr int WG_THREADS = 128;
-constexpr int WG_ROWS = 32;  // query rows in shared memory at a time
 
 struct Kv8WeighParams {
   Kv8AttnParams a;           // out, lse (written) and workspace are not used
@@ -26,8 +31,43 @@ struct Kv8WeighParams {
   const int32_t *fresh, *seen;  // new rows at the end (null: the query rows), tokens so far
   float *weights;
   int32_t *positions;
-  int room, groups;          // 16-key groups of a warp
+  int room, groups;          // groups: 16-key groups of a warp
+  // of kv8_weigh_rows_kernel
+  uint16_t *q16;             // [batch, kv heads, padded rows, dim]: f16 queries
+  float2 *row;               // their score factor, log2 sum (+inf: does not count)
+  int padded, ranges;        // rows, key ranges of a (sequence, head)
 };
+
+// Keys of sequence b, and the first of its new rows; false: left out.
+struct Kv8WeighSpan {
+  Kv8Span sp;
+  int fresh;
+};
+__device__ __forceinline__ bool wg_span(const Kv8WeighParams &w, int b, bool flag, Kv8WeighSpan &s) {
+  s.sp = kv8_span(w.a, b, flag);
+  int32_t *status = flag ? w.a.status : nullptr;
+  if (s.sp.keys > w.room) {
+    flag_status(status, VB_STATUS_BOUNDS);
+    return false;
+  }
+  s.fresh = s.sp.keys - (w.fresh ? kv8_rows(w.fresh, b, s.sp.keys, status)
+                                 : min(s.sp.q_len, s.sp.keys));
+  return true;
+}
+// Adds a key's sum; `first`: the call's first sum of it, with which a new row begins.
+__device__ __forceinline__ void wg_add(const Kv8WeighParams &w, const Kv8WeighSpan &s, int b,
+                                       size_t at, int key, float sum, bool first, float old) {
+  const bool is_new = first && key >= s.fresh;
+  if (is_new || sum != 0.f) w.weights[at + key] = (is_new ? 0.f : old) + sum;
+  if (is_new && w.positions) w.positions[at + key] = w.seen[b] - (s.sp.keys - key);
+}
+
+// ------------------------------------------------------------ few query rows
+constexpr int WG_THREADS = 128;
+constexpr int WG_WARPS = WG_THREADS / 32;
+constexpr int WG_RING = 12288;             // bytes of a warp's ring
+template <int D>
+constexpr int wg_stages() { return WG_RING / (D * 16); }   // 16 keys each
 
 __device__ __forceinline__ void wg_mma(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
@@ -36,162 +76,555 @@ __device__ __forceinline__ void wg_mma(float (&d)[4], const uint4 &a, uint32_t b
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
-template <int D>
+template <int D, int NR>  // NR groups of 8 query rows
 __global__ void __launch_bounds__(WG_THREADS) kv8_weigh_kernel(const __grid_constant__ Kv8WeighParams w) {
   const Kv8AttnParams &p = w.a;
-  __shared__ uint32_t s_q[WG_ROWS / 8 * D * 4];  // [8 rows][D/32][32 lanes][4]
-  __shared__ float2 s_row[WG_ROWS];              // score factor, log2 sum
-  __shared__ int s_vis[WG_ROWS];
+  constexpr int ROWS = 8 * NR, PIECES = D / 32, STAGES = wg_stages<D>();
+  extern __shared__ __align__(16) uint8_t ring[];  // [warp][stage][piece][lane][16]
+  __shared__ uint32_t s_q[NR * D * 4];             // [8 rows][D/32][32 lanes][4]
+  __shared__ float2 s_row[ROWS];                   // score factor, log2 sum
+  __shared__ int s_vis[ROWS];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int H = p.c.kv_heads, b = blockIdx.z, h = blockIdx.y;
-  const bool flag = blockIdx.x == 0 && h == 0 && tid == 0;
-  Kv8Span sp = kv8_span(p, b, flag);
-  if (sp.keys > w.room) {
-    if (flag) flag_status(p.status, VB_STATUS_BOUNDS);
-    return;
+  Kv8WeighSpan s;
+  if (!wg_span(w, b, blockIdx.x == 0 && h == 0 && tid == 0, s)) return;
+  const int keys = s.sp.keys, key_first = blockIdx.x * (WG_WARPS * 16) * w.groups;
+  if (key_first >= keys) return;
+  const int rows = s.sp.q_len * p.rep;
+  const size_t at0 = ((size_t)b * H + h) * w.room, page_bytes = (size_t)p.c.page * D;
+  auto first_key = [&](int it) { return key_first + (it * WG_WARPS + warp) * 16; };
+  // page and K scale (-1: no such page) of the group that this lane looks up
+  int id = -1;
+  float ks_l = -1.f;
+  if (lane < w.groups && first_key(lane) < keys) {
+    id = kv8_page(p.c.page_table + (size_t)b * p.c.max_pages, p.c.max_pages, p.c.pages,
+                  first_key(lane) >> p.shift, p.status);
+    if (id >= 0) ks_l = __ldg(p.c.k_scales + (size_t)id * H + h);
   }
-  const int fresh = sp.keys - (w.fresh ? kv8_rows(w.fresh, b, sp.keys, flag ? p.status : nullptr)
-                                       : min(sp.q_len, sp.keys));
-  const int key_first = blockIdx.x * (WG_THREADS / 32 * 16) * w.groups;
-  if (key_first >= sp.keys) return;
-  const int rows = sp.q_len * p.rep;
-  const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
-  const size_t at0 = ((size_t)b * H + h) * w.room;
-  const size_t page_bytes = (size_t)p.c.page * D;
-
-  for (int grp = 0; grp < w.groups; ++grp) {
-    const int key0 = key_first + (grp * (WG_THREADS / 32) + warp) * 16;  // uniform in the warp
-    const bool some = key0 < sp.keys;
-    uint4 lo[D / 64], hi[D / 64];
-    float ks = 0.f;
-    if (some) {
-      const int id = kv8_page(table, p.c.max_pages, p.c.pages, key0 >> p.shift,
-                              lane == 0 ? p.status : nullptr);
-      if (id >= 0) {
-        const size_t ph = (size_t)id * H + h;
-        const int8_t *k = p.c.k_codes + ph * page_bytes +
-                          (size_t)((key0 & (p.c.page - 1)) + g) * D + c * 16;
-        ks = __ldg(p.c.k_scales + ph);
+  uint8_t *mine = ring + (warp * STAGES * PIECES * 32 + lane) * 16;
+  auto issue = [&](int it) {
+    const int pg = max(0, __shfl_sync(0xffffffffu, id, it & 31));
+    if (it < w.groups && first_key(it) < keys) {
+      const int8_t *k = p.c.k_codes + ((size_t)pg * H + h) * page_bytes +
+                        (size_t)((first_key(it) & (p.c.page - 1)) + g) * D + c * 16;
+      uint8_t *dst = mine + it % STAGES * (PIECES * 512);
 #pragma unroll
-        for (int s = 0; s < D / 64; ++s) {
-          lo[s] = ldg_nc_v4(k + s * 64);
-          hi[s] = ldg_nc_v4(k + s * 64 + 8 * D);
-        }
-      } else {
-        ks = -1.f;
+      for (int x = 0; x < D / 64; ++x) {
+        cp_async16(dst + 2 * x * 512, k + x * 64);
+        cp_async16(dst + (2 * x + 1) * 512, k + x * 64 + 8 * D);
       }
     }
-    if (ks < 0.f || !some) {
+    cp_async_commit();
+  };
 #pragma unroll
-      for (int s = 0; s < D / 64; ++s) lo[s] = hi[s] = make_uint4(0, 0, 0, 0);
+  for (int it = 0; it < STAGES - 1; ++it) issue(it);
+
+  // ---- queries in the order of the B fragments: D / 8 lanes per row
+  {
+    constexpr int LPR = D / 8, PASS = WG_THREADS / LPR, NP = (ROWS + PASS - 1) / PASS;
+    const int c8 = tid % LPR;
+    uint4 v[NP];
+    float l[NP];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int r = tid / LPR + k * PASS, i = p.row_of(r), hq = h * p.rep + r - i * p.rep;
+      v[k] = make_uint4(0, 0, 0, 0);
+      l[k] = -INFINITY;
+      if (r < rows) {
+        v[k] = kv8_load8(p.q + b * p.qb + (int64_t)hq * p.qh + (int64_t)i * p.ql + c8 * 8, p.vec);
+        l[k] = w.lse[((size_t)b * p.Hq + hq) * p.L + i];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int r = tid / LPR + k * PASS;
+      const float pw = kv8_q_scale<LPR>(v[k]);
+      if (r >= ROWS) continue;  // (8 rows of 64: half of the threads)
+      if (c8 == 0) {
+        const bool counts = fabsf(l[k]) <= 3.4028235e38f;
+        if (!counts && l[k] != -INFINITY && key_first == 0) flag_status(p.status, VB_STATUS_NONFINITE);
+        s_row[r] = make_float2(p.scale_log2 / pw, l[k] * 1.4426950408889634f);
+        s_vis[r] = counts ? s.sp.visible(p.row_of(r)) : 0;
+      }
+      const int fl = (r & 7) * 4 + ((c8 & 7) >> 1);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int step = (c8 >> 3) * 4 + (c8 & 1) * 2 + j;
+        *reinterpret_cast<uint2 *>(
+            s_q + (((r >> 3) * (D / 32) + (step >> 1)) * 32 + fl) * 4 + (step & 1) * 2) =
+            j ? make_uint2(v[k].z, v[k].w) : make_uint2(v[k].x, v[k].y);
+      }
+    }
+  }
+  __syncthreads();
+  float2 row[NR][2];
+  int vis[NR][2];
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      row[n][u] = s_row[n * 8 + 2 * c + u];
+      vis[n][u] = s_vis[n * 8 + 2 * c + u];
+    }
+
+  for (int it = 0; it < w.groups; ++it) {
+    const int key0 = first_key(it);
+    if (key0 >= keys) break;
+    const int key = key0 + g + 8 * c;  // (c < 2) the key that this lane adds to
+    float old = 0.f;
+    if (c < 2 && key < keys) old = w.weights[at0 + key];
+    issue(it + STAGES - 1);
+    cp_async_wait<STAGES - 1>();
+    const uint8_t *st = mine + it % STAGES * (PIECES * 512);
+    const float ks = __shfl_sync(0xffffffffu, ks_l, it & 31);
+    float acc[NR][2][4];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) acc[n][u >> 2][u & 3] = 0.f;
+#pragma unroll
+    for (int x = 0; x < D / 64; ++x) {
+      const uint4 lo = *reinterpret_cast<const uint4 *>(st + 2 * x * 512);
+      const uint4 hi = *reinterpret_cast<const uint4 *>(st + (2 * x + 1) * 512);
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const uint32_t y = (r4 == 0 ? lo.x : r4 == 1 ? lo.y : r4 == 2 ? lo.z : lo.w) ^ 0x80808080u;
+        const uint32_t z = (r4 == 0 ? hi.x : r4 == 1 ? hi.y : r4 == 2 ? hi.z : hi.w) ^ 0x80808080u;
+        const uint4 a = make_uint4(h2_codes(__byte_perm(y, 0x64646464u, 0x4140)),
+                                   h2_codes(__byte_perm(z, 0x64646464u, 0x4140)),
+                                   h2_codes(__byte_perm(y, 0x64646464u, 0x4342)),
+                                   h2_codes(__byte_perm(z, 0x64646464u, 0x4342)));
+        const int step = x * 4 + r4;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const uint2 bq = *reinterpret_cast<const uint2 *>(
+              s_q + ((n * (D / 32) + (step >> 1)) * 32 + lane) * 4 + (step & 1) * 2);
+          wg_mma(acc[n][step & 1], a, bq.x, bq.y);
+        }
+      }
     }
     float sum0 = 0.f, sum1 = 0.f;  // keys g and g + 8
-    for (int r0 = 0; r0 < rows; r0 += WG_ROWS) {
-      if (grp == 0 || rows > WG_ROWS) {
-        // ---- queries in the order of the B fragments: D / 8 lanes per row
-        if (grp > 0 || r0 > 0) __syncthreads();
-        constexpr int LPR = D / 8, PASS = WG_THREADS / LPR;
-        const int c8 = tid % LPR;
-#pragma unroll 4
-        for (int k = 0; k < WG_ROWS / PASS; ++k) {
-          const int r = tid / LPR + k * PASS, R = r0 + r, i = p.row_of(R), hr = R - i * p.rep;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (R < rows)
-            v = kv8_load8(p.q + b * p.qb + (int64_t)(h * p.rep + hr) * p.qh + (int64_t)i * p.ql +
-                              c8 * 8, p.vec);
-          const float pw = kv8_q_scale<LPR>(v);
-          if (c8 == 0) {
-            float l = -INFINITY;
-            if (R < rows) l = w.lse[((size_t)b * p.Hq + h * p.rep + hr) * p.L + i];
-            const bool counts = fabsf(l) <= 3.4028235e38f;
-            if (!counts && l != -INFINITY && key_first == 0 && grp == 0 && R < rows)
-              flag_status(p.status, VB_STATUS_NONFINITE);
-            s_row[r] = make_float2(p.scale_log2 / pw, l * 1.4426950408889634f);
-            s_vis[r] = counts ? sp.visible(i) : 0;
-          }
-          const int fl = (r & 7) * 4 + ((c8 & 7) >> 1);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int step = (c8 >> 3) * 4 + (c8 & 1) * 2 + j;
-            *reinterpret_cast<uint2 *>(
-                s_q + (((r >> 3) * (D / 32) + (step >> 1)) * 32 + fl) * 4 + (step & 1) * 2) =
-                j ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y);
-          }
-        }
-        __syncthreads();
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {  // rows 8 n + 2 c + u
+        const float f = row[n][u].x * ks;
+        const float z0 = fmaf(acc[n][0][u] + acc[n][1][u], f, -row[n][u].y);
+        const float z1 = fmaf(acc[n][0][2 + u] + acc[n][1][2 + u], f, -row[n][u].y);
+        if (key0 + g < vis[n][u]) sum0 += kv8_ex2(z0);
+        if (key0 + g + 8 < vis[n][u]) sum1 += kv8_ex2(z1);
       }
-      const int eights = (min(rows - r0, WG_ROWS) + 7) >> 3;
-      for (int n = 0; n < eights; ++n) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < D / 64; ++s) {
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const uint32_t x = (r4 == 0 ? lo[s].x : r4 == 1 ? lo[s].y : r4 == 2 ? lo[s].z : lo[s].w) ^ 0x80808080u;
-            const uint32_t y = (r4 == 0 ? hi[s].x : r4 == 1 ? hi[s].y : r4 == 2 ? hi[s].z : hi[s].w) ^ 0x80808080u;
-            const uint4 a = make_uint4(h2_codes(__byte_perm(x, 0x64646464u, 0x4140)),
-                                       h2_codes(__byte_perm(y, 0x64646464u, 0x4140)),
-                                       h2_codes(__byte_perm(x, 0x64646464u, 0x4342)),
-                                       h2_codes(__byte_perm(y, 0x64646464u, 0x4342)));
-            const int step = s * 4 + r4;
-            const uint2 bq = *reinterpret_cast<const uint2 *>(
-                s_q + ((n * (D / 32) + (step >> 1)) * 32 + lane) * 4 + (step & 1) * 2);
-            wg_mma(acc, a, bq.x, bq.y);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {  // rows 8 n + 2 c + u
-          const int r = n * 8 + 2 * c + u;
-          const float2 f = s_row[r];
-          const int vis = s_vis[r];
-          const float z0 = fmaf(acc[u], f.x * ks, -f.y), z1 = fmaf(acc[2 + u], f.x * ks, -f.y);
-          if (key0 + g < vis) sum0 += kv8_ex2(z0);
-          if (key0 + g + 8 < vis) sum1 += kv8_ex2(z1);
-        }
-      }
-    }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
       sum0 += __shfl_xor_sync(0xffffffffu, sum0, o);
       sum1 += __shfl_xor_sync(0xffffffffu, sum1, o);
     }
-    if (some && c < 2) {
-      const int key = key0 + g + 8 * c;
-      const float sum = ks < 0.f ? 0.f : c ? sum1 : sum0;
-      if (key < sp.keys) {
-        const bool is_new = key >= fresh;
-        if (is_new || sum != 0.f) w.weights[at0 + key] = (is_new ? 0.f : w.weights[at0 + key]) + sum;
-        if (is_new && w.positions) w.positions[at0 + key] = w.seen[b] - (sp.keys - key);
-      }
-    }
+    if (c < 2 && key < keys) wg_add(w, s, b, at0, key, ks < 0.f ? 0.f : c ? sum1 : sum0, true, old);
   }
 }
 
+// ----------------------------------------------------------- many query rows
+constexpr int WR_THREADS = 640;            // issue, two warpgroups that convert, two that add
+constexpr int WR_KEYS = 256;               // keys of a pair of CTAs
+constexpr int WR_COLS = 256;               // query rows at a time
+
 template <int D>
-int wg_run(Kv8WeighParams &w, cudaStream_t s) {
-  const VbKv8Cache &c = w.a.c;
-  const long long cap = (long long)c.max_pages * c.page;
-  const long long keys = cap < w.room ? cap : w.room, per = WG_THREADS / 32 * 16;
-  const long long units = (long long)c.batch * c.kv_heads;
-  // keys of a CTA: a few groups a warp once that still fills the SMs
-  w.groups = 1;
-  while (w.groups < 4 && (keys + per * w.groups - 1) / (per * w.groups) * units > 148 * 16)
-    w.groups *= 2;
-  const long long blocks = (keys + per * w.groups - 1) / (per * w.groups);
-  if (blocks == 0) return VB_OK;
-  vb_launch(kv8_weigh_kernel<D>, dim3((unsigned)blocks, c.kv_heads, c.batch), dim3(WG_THREADS), 0, s,
-            true, w);
+struct WrShape {
+  static constexpr int TILE = 128 * D * 2;                // f16 of 128 keys, or query rows
+  static constexpr int K_OFF = TILE;                      // after the queries: two stages
+  static constexpr int SMEM = 3 * TILE + 1024;
+};
+
+// f16 queries, row after row of a (sequence, kv head), and what turns a product into
+// a weight; rows that are not there, or have no finite lse, count for nothing.
+template <int D>
+__global__ void __launch_bounds__(256) kv8_weigh_q_kernel(const __grid_constant__ Kv8WeighParams w) {
+  constexpr int LPR = D / 8;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Kv8AttnParams &p = w.a;
+  const long long at = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int c8 = threadIdx.x % LPR, H = p.c.kv_heads;
+  const int unit = (int)(at / w.padded), R = (int)(at - (long long)unit * w.padded);
+  if (unit >= p.c.batch * H) return;  // (whole rows of lanes; a row's lanes stay together)
+  const int b = unit / H, h = unit - b * H, i = p.row_of(R), hq = h * p.rep + R - i * p.rep;
+  const Kv8Span sp = kv8_span(p, b, false);
+  uint4 v = make_uint4(0, 0, 0, 0);
+  float l = -INFINITY;
+  if (i < sp.q_len) {
+    v = kv8_load8(p.q + b * p.qb + (int64_t)hq * p.qh + (int64_t)i * p.ql + c8 * 8, p.vec);
+    l = w.lse[((size_t)b * p.Hq + hq) * p.L + i];
+  }
+  const float pw = kv8_q_scale<LPR>(v);
+  *(reinterpret_cast<uint4 *>(w.q16 + (size_t)at * D) + c8) = v;
+  if (c8 == 0) {
+    const bool counts = fabsf(l) <= 3.4028235e38f;
+    if (!counts && l != -INFINITY) flag_status(p.status, VB_STATUS_NONFINITE);
+    w.row[at] = make_float2(p.scale_log2 / pw, counts ? l * 1.4426950408889634f : INFINITY);
+  }
+}
+
+struct WrBarriers {
+  uint64_t k_full[2], k_empty[2], s_full[2], s_free[2], q_full, drain;
+};
+
+template <int D>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
+    kv8_weigh_rows_kernel(const __grid_constant__ Kv8WeighParams w) {
+  using S = WrShape<D>;
+  const Kv8AttnParams &p = w.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~uintptr_t(1023));
+  __shared__ __align__(8) WrBarriers bar;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ float4 s_row[2][WR_COLS / 2];  // factors and log2 sums of two columns
+  __shared__ float s_sum[2][128];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- the pair's keys: tiles [t0, t1) of 256
+  const int rank = blockIdx.x & 1, H = p.c.kv_heads;
+  const int range = (blockIdx.x >> 1) % w.ranges, unit = (blockIdx.x >> 1) / w.ranges;
+  const int b = unit / H, h = unit - b * H;
+  Kv8WeighSpan s;
+  if (!wg_span(w, b, range == 0 && rank == 0 && h == 0 && tid == 0, s)) return;
+  const int keys = s.sp.keys, rows = s.sp.q_len * p.rep;
+  const size_t at0 = (size_t)unit * w.room;
+  if (rows == 0) {  // new rows alone
+    for (int key = s.fresh + blockIdx.x % (2 * w.ranges) * WR_THREADS + tid; key < keys;
+         key += 2 * w.ranges * WR_THREADS)
+      wg_add(w, s, b, at0, key, 0.f, true, 0.f);
+    return;
+  }
+  const int tiles = (keys + WR_KEYS - 1) / WR_KEYS, share = tiles / w.ranges, rest = tiles % w.ranges;
+  const int t0 = range * share + min(range, rest), n_tiles = share + (range < rest);
+  if (n_tiles == 0) return;  // (both CTAs)
+  const int chunks = (rows + WR_COLS - 1) / WR_COLS, steps = chunks * n_tiles;
+  // columns of a chunk: up to 256, a multiple of 64
+  auto columns = [&](int ch) { return min(WR_COLS, (rows - ch * WR_COLS + 63) & ~63); };
+
+  if (tid == 32) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bar.k_full[i], 2 * 8);   // converter warps of both CTAs
+      tc::mbar_init(&bar.k_empty[i], 1);
+      tc::mbar_init(&bar.s_full[i], 1);
+      tc::mbar_init(&bar.s_free[i], 2 * 8);   // adding warps of both CTAs
+    }
+    tc::mbar_init(&bar.q_full, 2);  // both CTAs
+    tc::mbar_init(&bar.drain, 1);
+    s_abort = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     tc::smem_u32(&s_tmem)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  __syncwarp();
+  kp_cluster_arrive();
+  uint32_t tmem = 0;
+  auto ready = [&]() {  // barriers and TMEM of both CTAs are there
+    tc::tc_fence_before();
+    __syncthreads();
+    kp_cluster_wait();
+    tc::tc_fence_after();
+    tmem = s_tmem;
+  };
+  volatile int *abort = &s_abort;
+  const uint32_t sbase = tc::smem_u32(smem);
+  // The warp waits for the n-th completion (from 0) of a barrier; false after a wait of
+  // this CTA has given up.
+  auto wait = [&](uint64_t *m, int n) {
+    const bool there = tc::mbar_wait(m, (uint32_t)(n & 1), abort, KP_WAIT_NS);
+    if (!there) s_abort = 1;
+    return __all_sync(0xffffffffu, there);
+  };
+
+  if (wg == 0) {
+    // ================================================== tensor-core issuer
+    ready();
+    if (warp == 0 && rank == 0) {
+      const uint32_t one = kp_elect();
+      const uint64_t q_desc = tc::smem_desc_sw128(sbase);
+      const uint64_t k_desc = tc::smem_desc_sw128(sbase + S::K_OFF);
+      bool ok = true;
+      for (int n = 0, ch = 0, t = 0; n < steps && ok; ++n) {
+        const int st = n & 1;
+        if (t == 0) ok = wait(&bar.q_full, ch);
+        ok = ok && wait(&bar.k_full[st], n >> 1);
+        if (n >= 2) ok = ok && wait(&bar.s_free[st], (n >> 1) - 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint32_t idesc = kp_idesc(columns(ch), false);
+        const uint64_t kd = k_desc + st * (S::TILE >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const int off = ((kk >> 2) * KP_BLOCK + (kk & 3) * 32) >> 4;
+          kp_mma_ss(one, tmem + st * 256, kd + off, q_desc + off, idesc, kk > 0 ? 1u : 0u);
+        }
+        kp_commit(one, &bar.s_full[st]);
+        kp_commit(one, &bar.k_empty[st]);
+        if (++t == n_tiles) t = 0, ++ch;
+      }
+      // nothing of the pair may be in flight when TMEM is freed
+      kp_commit(one, &bar.drain);
+      if (!tc::mbar_wait(&bar.drain, 0, nullptr, KP_WAIT_NS)) s_abort = 1;
+    }
+    __syncwarp();
+  } else if (wg < 3) {
+    // ================================================== converters
+    const int ctid = tid - 128;
+    constexpr int KC = D / 16, KSTEP = 256 / KC, KN = 128 / KSTEP;
+    const int ch = ctid % KC, kkey = ctid / KC;
+    const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
+    const size_t pool_step = (size_t)H * p.c.page * D;
+    const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + ch * 16;
+    // page of the 16-key group lane % 8 of this CTA's half of tile t; rows without one
+    // (past the last key, or flagged) read page 0: nothing is added to them
+    auto group_page = [&](int t) {
+      const int key = t * WR_KEYS + rank * 128 + (lane & 7) * 16;
+      return key < keys ? max(0, kv8_page(table, p.c.max_pages, p.c.pages, key >> p.shift, p.status))
+                        : 0;
+    };
+    uint4 kr[KN];
+    auto load = [&](int id) {
+#pragma unroll
+      for (int i = 0; i < KN; ++i) {
+        const int key = kkey + i * KSTEP;  // a tile's half starts on a page boundary
+        const int pg = __shfl_sync(0xffffffffu, id, key >> 4);
+        kr[i] = ldg_nc_v4(kbase + pg * pool_step + (key & (p.c.page - 1)) * D);
+      }
+    };
+    load(group_page(t0));
+    int t = n_tiles > 1 ? 1 : 0;
+    int id = group_page(t0 + t);
+    ready();
+    for (int n = 0; n < steps; ++n) {
+      const int st = n & 1;
+      if (n >= 2 && !wait(&bar.k_empty[st], (n >> 1) - 1)) break;
+      uint8_t *tile = smem + S::K_OFF + st * S::TILE;
+#pragma unroll
+      for (int i = 0; i < KN; ++i) kp_store_codes(kr[i], tile, KP_BLOCK, kkey + i * KSTEP, ch);
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) kp_arrive_leader(&bar.k_full[st]);
+      if (n + 1 < steps) load(id);
+      if (++t == n_tiles) t = 0;
+      id = group_page(t0 + t);
+    }
+  } else {
+    // ================================================== weights, a thread per key
+    const int e = wg - 3, atid = tid - 384, r = tid & 127;  // half of the columns; the CTA's key
+    const float2 *row = w.row + (size_t)unit * w.padded;
+    const uint16_t *q16 = w.q16 + (size_t)unit * w.padded * D;
+    // this CTA's half of a chunk's queries, and the factors of all of its columns
+    auto load_q = [&](int ch) {
+      const int half = columns(ch) / 2, first = ch * WR_COLS + rank * half;
+      for (int x = atid; x < half * (D / 8); x += 256) {
+        const int qr = x / (D / 8), c8 = x % (D / 8);
+        cp_async16(smem + (c8 >> 3) * KP_BLOCK + kp_sw(qr, c8 & 7),
+                   q16 + (size_t)(first + qr) * D + c8 * 8);
+      }
+      cp_async_commit();
+      if (atid < 2 * half) {
+        const float2 f = row[ch * WR_COLS + atid];
+        float *d = reinterpret_cast<float *>(&s_row[ch & 1][atid >> 1]) + (atid & 1);
+        d[0] = f.x;
+        d[2] = -f.y;
+      }
+    };
+    auto publish_q = [&]() {
+      cp_async_wait<0>();
+      tc::fence_proxy_async_smem();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (atid == 0) kp_arrive_leader(&bar.q_full);
+    };
+    load_q(0);
+    // K scale of this thread's key (-1: no such page), a tile ahead
+    const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
+    auto scale_of = [&](int t) {
+      const int key = t * WR_KEYS + rank * 128 + r;
+      const int id = key < keys ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : -1;
+      return (unsigned)id < (unsigned)p.c.pages ? __ldg(p.c.k_scales + (size_t)id * H + h) : -1.f;
+    };
+    float ks_n = scale_of(t0);
+    ready();
+    publish_q();
+    const uint32_t trow = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
+    // keys that every query row sees
+    const int seen_by_all = s.sp.causal ? max(0, s.sp.off + 1) : keys;
+    bool ok = true;
+    for (int n = 0, ch = 0, t = 0; n < steps; ++n) {
+      const int st = n & 1, cols = columns(ch);
+      const float ks = ks_n;
+      const bool last = t == n_tiles - 1, more = last && ch + 1 < chunks;
+      if (n + 1 < steps) ks_n = scale_of(last ? t0 : t0 + t + 1);
+      const int key = (t0 + t) * WR_KEYS + rank * 128 + r;
+      float old = 0.f;
+      if (e == 0 && key < keys) old = w.weights[at0 + key];
+      ok = ok && wait(&bar.s_full[st], n >> 1);
+      tc::tc_fence_after();
+      if (more && ok) load_q(ch + 1);  // no product of this chunk is left
+      float sum = 0.f;
+      const float4 *tab = s_row[ch & 1] + e * (cols / 4);
+      const bool masked = (t0 + t) * WR_KEYS + rank * 128 + 128 > seen_by_all;
+      const f2 kk = f2_make(ks, ks);
+      f2 s0 = f2_make(0.f, 0.f), s1 = s0;
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols / 2; c0 += 32) {
+        uint32_t v[32];
+        tc::tmem_ld32(trow + st * 256 + e * (cols / 2) + c0, v);
+        tc::tmem_ld_wait();
+        if (masked) {  // (rare) some query rows do not see this key
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float *x = reinterpret_cast<const float *>(tab + (c0 + j) / 2) + (j & 1);
+            const int R = ch * WR_COLS + e * (cols / 2) + c0 + j;
+            const float z = fmaf(__uint_as_float(v[j]) * ks, x[0], x[2]);
+            if (key < s.sp.visible(p.row_of(R))) sum += kv8_ex2(z);
+          }
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 x = tab[(c0 + j) / 2], y = tab[(c0 + j) / 2 + 1];
+          float z[4];
+          f2_split(f2_fma(f2_mul(f2_make(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), kk),
+                          f2_make(x.x, x.y), f2_make(x.z, x.w)), z[0], z[1]);
+          f2_split(f2_fma(f2_mul(f2_make(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), kk),
+                          f2_make(y.x, y.y), f2_make(y.z, y.w)), z[2], z[3]);
+          s0 = f2_add(s0, f2_make(kv8_ex2(z[0]), kv8_ex2(z[1])));
+          s1 = f2_add(s1, f2_make(kv8_ex2(z[2]), kv8_ex2(z[3])));
+        }
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (ok && lane == 0) kp_arrive_leader(&bar.s_free[st]);
+      float a0, a1, a2, a3;
+      f2_split(s0, a0, a1);
+      f2_split(s1, a2, a3);
+      sum += (a0 + a1) + (a2 + a3);
+      if (e == 1) s_sum[st][r] = sum;
+      if (more && ok) {
+        publish_q();
+      } else {
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      if (e == 0 && ok && key < keys)
+        wg_add(w, s, b, at0, key, ks < 0.f ? 0.f : sum + s_sum[st][r], ch == 0, old);
+      if (last) t = 0, ++ch;
+      else ++t;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort) flag_status(p.status, VB_STATUS_TIMEOUT);
+  // no product reads the other CTA's operands any more, and all that the leader's
+  // products signal has come
+  if (warp == 0 && rank == 1) tc::mbar_wait(&bar.drain, 0, nullptr, KP_WAIT_NS);
+  // (after a wait gave up, arrivals may be under way that nothing has waited for)
+  if (*abort) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  __syncwarp();
+  kp_cluster_arrive();
+  kp_cluster_wait();
+  tc::tc_fence_after();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+}
+
+// ---------------------------------------------------------------------- plan
+struct WeighPlan {
+  bool tensor;
+  int padded, ranges;
+  size_t q_bytes, bytes;
+};
+
+WeighPlan wg_plan(const VbKv8WeighArgs *a) {
+  WeighPlan pl = {};
+  const long long rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
+  const long long units = (long long)a->cache.batch * a->cache.kv_heads;
+  pl.tensor = rows > 32;
+  if (!pl.tensor) return pl;
+  pl.padded = (int)((rows + WR_COLS - 1) / WR_COLS) * WR_COLS;
+  // Key ranges per (sequence, head): the fewest waves of 74 pairs of CTAs, each with its
+  // tiles and about two tiles' time for its start and end.
+  const long long cap = (long long)a->cache.max_pages * a->cache.page;
+  const long long tiles = ((cap < a->room ? cap : a->room) + WR_KEYS - 1) / WR_KEYS;
+  double least = 1e300;
+  pl.ranges = 1;
+  for (int r = 1; r <= 74 && r <= tiles; ++r) {
+    const double cost = (double)((units * r + 73) / 74) * (2 + (double)((tiles + r - 1) / r));
+    if (cost < least) least = cost, pl.ranges = r;
+  }
+  pl.q_bytes = (size_t)units * pl.padded * a->cache.dim * 2;
+  pl.bytes = pl.q_bytes + (size_t)units * pl.padded * sizeof(float2);
+  return pl;
+}
+
+template <int D, int NR>
+int wg_launch(const Kv8WeighParams &w, unsigned blocks, cudaStream_t s) {
+  constexpr int SMEM = WG_WARPS * wg_stages<D>() * D * 16;
+  static std::atomic<uint64_t> ready{0};
+  const int rc = once_per_device(ready, [] {
+    const cudaError_t e = cudaFuncSetAttribute(
+        kv8_weigh_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    return e == cudaSuccess ? VB_OK
+                            : set_error(VB_ERR_CUDA, "kv8_weigh_kernel attributes: %s",
+                                        cudaGetErrorString(e));
+  });
+  if (rc != VB_OK) return rc;
+  vb_launch(kv8_weigh_kernel<D, NR>, dim3(blocks, w.a.c.kv_heads, w.a.c.batch), dim3(WG_THREADS),
+            SMEM, s, true, w);
   return check_launch("kv8_weigh_kernel");
 }
 
-}  // namespace
-}  // namespace vb
+template <int D>
+int wg_run(Kv8WeighParams &w, const WeighPlan &pl, cudaStream_t s) {
+  const VbKv8Cache &c = w.a.c;
+  const long long cap = (long long)c.max_pages * c.page;
+  const long long keys = cap < w.room ? cap : w.room, per = WG_WARPS * 16;
+  const long long units = (long long)c.batch * c.kv_heads;
+  if (keys == 0) return VB_OK;
+  if (pl.tensor) {
+    using S = WrShape<D>;
+    static std::atomic<uint64_t> ready{0};
+    const int rc = once_per_device(ready, [] {
+      const cudaError_t e = cudaFuncSetAttribute(
+          kv8_weigh_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+      return e == cudaSuccess ? VB_OK
+                              : set_error(VB_ERR_CUDA, "kv8_weigh_rows_kernel attributes: %s",
+                                          cudaGetErrorString(e));
+    });
+    if (rc != VB_OK) return rc;
+    const long long rows = units * pl.padded, rpc = 256 * 8 / D;
+    vb_launch(kv8_weigh_q_kernel<D>, dim3((unsigned)((rows + rpc - 1) / rpc)), dim3(256), 0, s, true,
+              w);
+    const int rc2 = check_launch("kv8_weigh_q_kernel");
+    if (rc2 != VB_OK) return rc2;
+    vb_launch(kv8_weigh_rows_kernel<D>, dim3((unsigned)(2 * units * w.ranges)), dim3(WR_THREADS),
+              S::SMEM, s, true, w);
+    return check_launch("kv8_weigh_rows_kernel");
+  }
+  // Groups of a warp: 8, fewer while that leaves SMs without work.
+  w.groups = 8;
+  while (w.groups > 1 && (keys + per * w.groups - 1) / (per * w.groups) * units < 148 * 4)
+    w.groups /= 2;
+  const unsigned blocks = (unsigned)((keys + per * w.groups - 1) / (per * w.groups));
+  const int rows = w.a.L * w.a.rep;
+  return rows <= 8 ? wg_launch<D, 1>(w, blocks, s)
+         : rows <= 16 ? wg_launch<D, 2>(w, blocks, s)
+                      : wg_launch<D, 4>(w, blocks, s);
+}
 
-using namespace vb;
-
-extern "C" int vb_kv8_weigh(const VbKv8WeighArgs *a, vb_stream_t stream) {
+int wg_check(const VbKv8WeighArgs *a) {
   VB_REQUIRE(a, "vb_kv8_weigh: null args");
   const int rc = kv8_check(&a->cache, "vb_kv8_weigh");
   if (rc != VB_OK) return rc;
@@ -201,12 +634,37 @@ extern "C" int vb_kv8_weigh(const VbKv8WeighArgs *a, vb_stream_t stream) {
              a->cache.kv_heads);
   VB_REQUIRE(a->L >= 0 && (long long)a->L * a->q_heads <= 1 << 24,
              "vb_kv8_weigh: L=%d rows of %d heads", a->L, a->q_heads);
+  VB_REQUIRE((long long)a->cache.batch * a->cache.kv_heads <= 1 << 21 &&
+                 (long long)a->cache.batch * a->q_heads * a->L <= 1 << 28,
+             "vb_kv8_weigh: %d sequences of %d kv heads, %d rows of %d heads each", a->cache.batch,
+             a->cache.kv_heads, a->L, a->q_heads);
   VB_REQUIRE(a->room >= 0 && a->room <= 0x7fffffff - 65536, "vb_kv8_weigh: room=%d", a->room);
+  return VB_OK;
+}
+
+}  // namespace
+}  // namespace vb
+
+using namespace vb;
+
+extern "C" {
+
+size_t vb_kv8_weigh_workspace_size(const VbKv8WeighArgs *a) {
+  return wg_check(a) == VB_OK ? wg_plan(a).bytes : 0;
+}
+
+int vb_kv8_weigh(const VbKv8WeighArgs *a, vb_stream_t stream) {
+  const int rc = wg_check(a);
+  if (rc != VB_OK) return rc;
   VB_REQUIRE(a->lens && (a->L == 0 || (a->q && a->lse)) && (a->weights || a->room == 0),
              "vb_kv8_weigh: null tensor");
   VB_REQUIRE(!a->positions || a->seen, "vb_kv8_weigh: positions without seen");
   VB_REQUIRE(a->scale > 0.f && a->scale < 1e30f, "vb_kv8_weigh: scale %g", (double)a->scale);
-  VB_REQUIRE(a->cache.kv_heads <= 65535, "vb_kv8_weigh: too many heads");
+  const WeighPlan pl = wg_plan(a);
+  if (pl.bytes && (!a->workspace || a->workspace_bytes < pl.bytes))
+    return set_error(VB_ERR_WORKSPACE, "vb_kv8_weigh: workspace %zu < %zu bytes",
+                     a->workspace_bytes, pl.bytes);
+  VB_REQUIRE(((uintptr_t)a->workspace % 16) == 0, "vb_kv8_weigh: workspace alignment");
   Kv8WeighParams w = {};
   Kv8AttnParams &p = w.a;
   p.c = a->cache;
@@ -221,10 +679,15 @@ extern "C" int vb_kv8_weigh(const VbKv8WeighArgs *a, vb_stream_t stream) {
   p.rep_inv = (uint32_t)((1ull << 32) / (uint32_t)p.rep) + (p.rep > 1);
   w.lse = a->lse; w.fresh = a->fresh; w.seen = a->seen;
   w.weights = a->weights; w.positions = a->positions; w.room = a->room;
+  w.q16 = static_cast<uint16_t *>(a->workspace);
+  w.row = reinterpret_cast<float2 *>(static_cast<uint8_t *>(a->workspace) + pl.q_bytes);
+  w.padded = pl.padded; w.ranges = pl.ranges;
   cudaStream_t s = as_stream(stream);
   switch (a->cache.dim) {
-    case 64: return wg_run<64>(w, s);
-    case 128: return wg_run<128>(w, s);
-    default: return wg_run<256>(w, s);
+    case 64: return wg_run<64>(w, pl, s);
+    case 128: return wg_run<128>(w, pl, s);
+    default: return wg_run<256>(w, pl, s);
   }
 }
+
+}  // extern "C"

@@ -30,7 +30,7 @@ HEAD_DIMS = (64, 128, 256)
 # partial results of the key ranges; one for the caches of all layers, whose
 # attention on a stream runs one after another
 _scratch = Scratch(_lib.VB_KV8_ATTN_WORKSPACE_HEAD)
-_evict_scratch = Scratch(16)  # lists that a call makes itself
+_lists = Scratch(16)  # what calls of weigh and evict make for themselves
 
 
 def _rows(t: torch.Tensor, what: str, shape, device: int) -> torch.Tensor:
@@ -154,7 +154,7 @@ class PagedKV8Cache:
         self._weigh_args = bytes(VbKv8WeighArgs(c))
         self._evict_args = bytes(VbKv8EvictArgs(c))
         self._shared_args = bytes(VbKv8SharedArgs(VbKv8AttnArgs(c)))
-        self._need = {}  # workspace bytes by (q_heads, L), of evict by (room, keep)
+        self._need = {}  # workspace bytes by (q_heads, L), of others by name and sizes
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, batch: int, max_pages: int,
@@ -406,7 +406,14 @@ class PagedKV8Cache:
             a.status = status_ptr(status, dev)
         a.scale = D ** -0.5 if scale is None else scale
         a.q_heads, a.L, a.len_add, a.causal = Hq, L, len_add, causal
-        check(lib.vb_kv8_weigh(C.byref(a), current_stream(dev)), "vb_kv8_weigh")
+        need = self._need.get(("weigh", Hq, L, room))
+        if need is None:
+            need = self._need["weigh", Hq, L, room] = lib.vb_kv8_weigh_workspace_size(C.byref(a))
+        st = current_stream(dev)
+        if need:
+            ws = _lists.get(need, self.device, st)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        check(lib.vb_kv8_weigh(C.byref(a), st), "vb_kv8_weigh")
 
     def evict(self, weights, lens, keep: int, first: int = 0, recent: int = 0, positions=None,
               status=None, stream=None):
@@ -443,7 +450,7 @@ class PagedKV8Cache:
             need = self._need["evict", room, keep] = lib.vb_kv8_evict_workspace_size(C.byref(a))
         st = current_stream(dev)
         if need:
-            ws = _evict_scratch.get(need, self.device, st)
+            ws = _lists.get(need, self.device, st)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         after = torch.empty_like(lens)
         a.lens_out = after.data_ptr()
