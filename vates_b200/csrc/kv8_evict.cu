@@ -11,20 +11,20 @@
 // the pages that its live rows come from, s; codes become rint(code * (from / s)),
 // which leaves the rows of that page as they are.
 //
-// A cluster of up to 8 CTAs owns one (sequence, kv head). Weights become 32-bit
-// keys in their order (kept in shared memory); three histograms of 11, 11 and 10
-// bits, added up over the cluster, give the last key that stays. Ballots count
-// and number holes and moving rows, in order, and then a warp takes a page of K
-// or V at a time.
-// Nothing is written that another warp still reads: rows move from `keep` on to
-// below it, and the scale of the page in which `keep` falls is read beforehand.
+// kv8_evict_select_kernel: a cluster of up to 8 CTAs owns one (sequence, kv head).
+// Weights become 32-bit keys in their order (kept in shared memory); three
+// histograms of 11, 11 and 10 bits, added up over the cluster, give the last key
+// that stays. Ballots count and number holes and moving rows, in order.
+// kv8_evict_move_kernel: a CTA fills the holes of one page after another, half of it
+// K's and half V's, and moves weights and positions with K. Nothing is written that
+// another CTA still reads: rows move from `keep` on to below it, and the scale of the
+// page in which `keep` falls is taken down by the first kernel.
 #include "kv8.cuh"
 
 namespace vb {
 namespace {
 
-constexpr int EV_THREADS = 1024;
-constexpr int EV_WARPS = EV_THREADS / 32;
+constexpr int EV_CTAS = 8;            // most CTAs of a cluster
 constexpr int EV_BINS = 2048;
 constexpr int EV_KEYS = 24576;        // most keys of a CTA in shared memory
 constexpr uint32_t EV_SAFE = 0xFFFFFFFFu;
@@ -36,7 +36,9 @@ struct Kv8EvictParams {
   const int32_t *lens;
   int32_t *lens_out;
   int32_t *status;
-  int32_t *lists;            // per (sequence, head): holes, moving rows, first hole of a page
+  // per (sequence, head): holes, moving rows, first hole of a page, and the K and V scale
+  // of the page in which `keep` falls
+  int32_t *lists;
   long long list_stride;
   int most;                  // room of a list
   int room, cap, keep, first, recent, shift, cached;
@@ -52,26 +54,31 @@ __device__ __forceinline__ uint32_t ev_ctas() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-// All threads of the cluster meet; what they wrote, shared or global, is visible.
-__device__ __forceinline__ void ev_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;"
-               ::: "memory");
+// All threads of the cluster meet; what they wrote to shared memory is visible.
+__device__ __forceinline__ void ev_sync(uint32_t ctas) {
+  if (ctas == 1)
+    __syncthreads();
+  else
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;"
+                 ::: "memory");
 }
-// A word of CTA `rank`'s shared memory.
+// A word of CTA `rank`'s shared memory. (Not ordered among themselves, so that several are
+// on their way at once; the barriers around them are.)
 __device__ __forceinline__ uint32_t ev_peer(const void *p, uint32_t rank) {
   uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(rank));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(r) : "r"(a) : "memory");
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(r) : "r"(a));
   return r;
 }
 
-__global__ void __launch_bounds__(EV_THREADS) kv8_evict_kernel(const __grid_constant__ Kv8EvictParams p) {
+template <int EV_THREADS>
+__global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const __grid_constant__ Kv8EvictParams p) {
+  constexpr int EV_WARPS = EV_THREADS / 32, EV_PER = EV_BINS / EV_THREADS;
   extern __shared__ uint32_t s_keys[];
   __shared__ uint32_t s_hist[2][EV_BINS];
   __shared__ uint32_t s_warp[2][EV_WARPS], s_total[3];  // total: ties; holes, moving rows
   __shared__ uint32_t s_bin, s_above, s_count;
   __shared__ int s_newest;
-  __shared__ float s_edge[2];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -92,50 +99,61 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_kernel(const __grid_cons
   const int turns = (int)((n + (long long)C * EV_THREADS - 1) / ((long long)C * EV_THREADS));
   const int at0 = warp * turns * 32 + lane, row0 = (int)rank * EV_THREADS * turns + at0;
 
-  // ---- the newest position
+  auto order = [&](float w) {
+    w += 0.f;  // (-0 is 0)
+    const uint32_t k = __float_as_uint(w);
+    return w != w ? 0u : k >> 31 ? ~k : k | 0x80000000u;
+  };
+  // ---- the newest position, while the weights are on their way too
   long long late = 0x7fffffffffffll;  // positions above it are protected
   if (p.recent > 0) {
     int newest = n - 1;
     if (positions) {
       newest = -0x7fffffff - 1;
+#pragma unroll 4
       for (int t = 0; t < turns; ++t)
-        if (row0 + t * 32 < n) newest = max(newest, positions[row0 + t * 32]);
+        if (row0 + t * 32 < n) {
+          newest = max(newest, positions[row0 + t * 32]);
+          if (at0 + t * 32 < p.cached) s_keys[at0 + t * 32] = order(weights[row0 + t * 32]);
+        }
       newest = __reduce_max_sync(0xffffffffu, newest);
       if (lane == 0) s_warp[0][warp] = (uint32_t)newest;
       __syncthreads();
       if (warp == 0) {
-        newest = __reduce_max_sync(0xffffffffu, (int)s_warp[0][lane]);
+        newest = __reduce_max_sync(0xffffffffu, (int)s_warp[0][lane % EV_WARPS]);
         if (lane == 0) s_newest = newest;
       }
-      ev_sync();
-      for (uint32_t r = 0; r < C; ++r) newest = max(newest, (int)ev_peer(&s_newest, r));
+      ev_sync(C);
+      newest = (int)ev_peer(&s_newest, min((uint32_t)lane, C - 1));
+      newest = __reduce_max_sync(0xffffffffu, newest);
     }
     late = (long long)newest - p.recent;
   }
-  auto make_key = [&](int i) {
-    const float w = weights[i] + 0.f;
-    uint32_t k = __float_as_uint(w);
-    k = w != w ? 0u : k >> 31 ? ~k : k | 0x80000000u;
-    return i < p.first || (positions ? positions[i] : i) > late ? EV_SAFE : k;
+  const bool ordered = p.recent > 0 && positions;  // s_keys has the weights' order already
+  auto make_key = [&](int i, int at) {
+    if (i < p.first || (p.recent > 0 && (positions ? positions[i] : i) > late)) return EV_SAFE;
+    return ordered && at < p.cached ? s_keys[at] : order(weights[i]);
   };
   auto key = [&](int t) {
-    return at0 + t * 32 < p.cached ? s_keys[at0 + t * 32] : make_key(row0 + t * 32);
+    return at0 + t * 32 < p.cached ? s_keys[at0 + t * 32] : make_key(row0 + t * 32, at0 + t * 32);
   };
 
   // ---- the key of the last row that stays: `need` of the rows that have it do
-  uint32_t prefix = 0, need = (uint32_t)p.keep;
+  uint32_t last = 0, prefix = 0, need = (uint32_t)p.keep;
+  bool ties = true;  // not all rows with the last key stay: the lower ones
 #pragma unroll 1
-  for (int d = 0; d < 3; ++d) {
+  for (int d = 0; d < 3 && ties; ++d) {
     const int low = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
     uint32_t *hist = s_hist[d & 1];
     for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
     __syncthreads();
+#pragma unroll 4
     for (int t = 0; t < turns; ++t) {
       const int i = row0 + t * 32;
-      if (i >= n) break;
+      if (i >= n) continue;
       uint32_t k;
       if (d == 0) {
-        k = make_key(i);
+        k = make_key(i, at0 + t * 32);
         if (at0 + t * 32 < p.cached) s_keys[at0 + t * 32] = k;
       } else {
         k = key(t);
@@ -143,14 +161,29 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_kernel(const __grid_cons
       if (d == 0 || k >> (low + bits) == prefix)
         atomicAdd(hist + ((k >> low) & ((1u << bits) - 1)), 1u);
     }
-    ev_sync();
-    // bins from the top: thread tid has 2047 - 2 tid and 2046 - 2 tid
-    uint32_t hi = 0, lo = 0;
-    for (uint32_t r = 0; r < C; ++r) {
-      hi += ev_peer(hist + EV_BINS - 1 - 2 * tid, r);
-      lo += ev_peer(hist + EV_BINS - 2 - 2 * tid, r);
+    ev_sync(C);
+    // bins from the top: thread tid has EV_PER of them from EV_BINS - 1 - EV_PER tid down
+    uint32_t bin[EV_PER], mine = 0;
+    const uint32_t *top = hist + EV_BINS - 1 - EV_PER * tid;
+    if (C == 1) {
+#pragma unroll
+      for (int x = 0; x < EV_PER; ++x) bin[x] = top[-x];
+    } else {
+      uint32_t y[EV_CTAS][EV_PER];
+#pragma unroll
+      for (int r = 0; r < EV_CTAS; ++r)
+#pragma unroll
+        for (int x = 0; x < EV_PER; ++x) y[r][x] = ev_peer(top - x, min((uint32_t)r, C - 1));
+#pragma unroll
+      for (int x = 0; x < EV_PER; ++x) {
+        bin[x] = 0;
+#pragma unroll
+        for (int r = 0; r < EV_CTAS; ++r) bin[x] += r < C ? y[r][x] : 0u;
+      }
     }
-    uint32_t inc = hi + lo;
+#pragma unroll
+    for (int x = 0; x < EV_PER; ++x) mine += bin[x];
+    uint32_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
@@ -159,20 +192,23 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_kernel(const __grid_cons
     if (lane == 31) s_warp[0][warp] = inc;
     __syncthreads();
     uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[0][lane] : 0u);
-    before += inc - hi - lo;
-    if (before < need && need <= before + hi + lo) {
-      const bool upper = need <= before + hi;
-      s_bin = EV_BINS - 1 - 2 * tid - (upper ? 0 : 1);
-      s_above = before + (upper ? 0 : hi);
-      s_count = upper ? hi : lo;
+    before += inc - mine;
+#pragma unroll
+    for (int x = 0; x < EV_PER; ++x) {
+      if (before < need && need <= before + bin[x]) {
+        s_bin = EV_BINS - 1 - EV_PER * tid - x;
+        s_above = before;
+        s_count = bin[x];
+      }
+      before += bin[x];
     }
     __syncthreads();
     need -= s_above;
     prefix = prefix << bits | s_bin;
+    last = prefix << low;
+    ties = need < s_count;  // all rows of the bin stay: no need to look closer
     __syncthreads();  // s_warp, s_bin are free again
   }
-  const uint32_t last = prefix;
-  const bool ties = need < s_count;  // not all rows with the last key stay: the lower ones
 
   // Exclusive sums over the warps and CTAs before this warp of up to two counts.
   auto before = [&](uint32_t a, uint32_t c, int slot, uint32_t &sa, uint32_t &sc) {
@@ -181,7 +217,8 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_kernel(const __grid_cons
       s_warp[1][warp] = c;
     }
     __syncthreads();
-    const uint32_t ta = s_warp[0][lane], tc = s_warp[1][lane];
+    const uint32_t ta = lane < EV_WARPS ? s_warp[0][lane] : 0u;
+    const uint32_t tc = lane < EV_WARPS ? s_warp[1][lane] : 0u;
     sa = __reduce_add_sync(0xffffffffu, lane < warp ? ta : 0u);
     sc = __reduce_add_sync(0xffffffffu, lane < warp ? tc : 0u);
     if (warp == 0) {
@@ -192,10 +229,12 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_kernel(const __grid_cons
         if (slot) s_total[2] = all_c;
       }
     }
-    ev_sync();
-    for (uint32_t r = 0; r < rank; ++r) {
-      sa += ev_peer(s_total + slot, r);
-      if (slot) sc += ev_peer(s_total + 2, r);
+    ev_sync(C);
+    if (rank > 0) {
+      const uint32_t r = min((uint32_t)lane, rank - 1);
+      const uint32_t pa = ev_peer(s_total + slot, r), pc = ev_peer(s_total + (slot ? 2 : 0), r);
+      sa += __reduce_add_sync(0xffffffffu, lane < rank ? pa : 0u);
+      sc += __reduce_add_sync(0xffffffffu, lane < rank ? pc : 0u);
     }
   };
   uint32_t tie0 = 0, unused;
@@ -216,19 +255,20 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_kernel(const __grid_cons
     tie += __popc(same);
     return s;
   };
-  uint32_t n_holes = 0, n_moving = 0, tie = tie0;
+  uint32_t n_holes = 0, n_moving = 0, tie = tie0, bits = 0;  // bit t: row t stays (t < 32)
   for (int t = 0; t < turns; ++t) {
     const int i = row0 + t * 32;
     const bool s = stays(t, tie);
+    if (t < 32) bits |= (uint32_t)s << t;
     n_holes += __popc(__ballot_sync(0xffffffffu, !s && i < p.keep));
     n_moving += __popc(__ballot_sync(0xffffffffu, s && i >= p.keep));
   }
   uint32_t hole, move;
   before(n_holes, n_moving, 1, hole, move);
-  tie = tie0;
+  uint32_t tie1 = tie0;
   for (int t = 0; t < turns; ++t) {
     const int i = row0 + t * 32;
-    const bool s = stays(t, tie);
+    const bool s = turns <= 32 ? (bits >> t) & 1 : stays(t, tie1);
     const uint32_t hb = __ballot_sync(0xffffffffu, !s && i < p.keep);
     const uint32_t mb = __ballot_sync(0xffffffffu, s && i >= p.keep);
     if (i < p.keep && (i & (p.c.page - 1)) == 0)
@@ -241,103 +281,140 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_kernel(const __grid_cons
     move += __popc(mb);
   }
   // the page in which `keep` falls: rows of it may move, and its scale may change
-  const int edge = p.keep >> p.shift;
-  if (tid < 2) {
-    const int id = kv8_page(table, p.c.max_pages, p.c.pages, edge, nullptr);
-    s_edge[tid] = id < 0 ? 0.f
-                         : (tid ? p.c.v_scales : p.c.k_scales)[(size_t)id * p.c.kv_heads + h];
+  if (rank == 0 && tid < 2) {
+    const int id = kv8_page(table, p.c.max_pages, p.c.pages, p.keep >> p.shift, nullptr);
+    const float *scales = tid ? p.c.v_scales : p.c.k_scales;
+    firsts[((p.keep + p.c.page - 1) >> p.shift) + 1 + tid] =
+        id < 0 ? 0 : __float_as_int(scales[(size_t)id * p.c.kv_heads + h]);
   }
-  ev_sync();
+  if (C > 1) ev_sync(C);  // no CTA ends while another may still read its shared memory
+}
 
-  // ---- a warp takes a page of K or V at a time
-  const int pages = (p.keep + p.c.page - 1) >> p.shift, D = p.c.dim, lpr = D >> 4;
+constexpr int EM_THREADS = 256;
+constexpr int EM_HALF = 128;  // threads of K, and of V: one for each row of the largest page
+constexpr int EM_AHEAD = 4;   // pieces of 16 codes that a thread has in flight
+
+__global__ void __launch_bounds__(EM_THREADS, 6) kv8_evict_move_kernel(const __grid_constant__ Kv8EvictParams p) {
+  __shared__ int s_src[2][EM_HALF], s_sid[2][EM_HALF], s_row[2][EM_HALF];
+  __shared__ float s_from[2][EM_HALF], s_top[2][4];
+  __shared__ uint32_t s_filled[2][4][4];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int kv = threadIdx.x / EM_HALF, tid = threadIdx.x % EM_HALF, warp = tid >> 5;
+  const int lane = tid & 31, unit = blockIdx.y, b = unit / p.c.kv_heads, h = unit - b * p.c.kv_heads;
+  if (p.lens[b] <= p.keep) return;
+  const int pages = (p.keep + p.c.page - 1) >> p.shift, edge = p.keep >> p.shift;
+  const int32_t *holes = p.lists + unit * p.list_stride, *moving = holes + p.most,
+                *firsts = moving + p.most;
+  const float edge_scale = __int_as_float(firsts[pages + 1 + kv]);
+  const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
+  const int D = p.c.dim, lpr = D >> 4, lsh = D == 64 ? 2 : D == 128 ? 3 : 4;
   const size_t page_bytes = (size_t)p.c.page * D;
-  for (int task = (int)rank * EV_WARPS + warp; task < 2 * pages; task += (int)C * EV_WARPS) {
-    const int pg = task >> 1, kv = task & 1;
-    const int j0 = __ldcg(firsts + pg), j1 = __ldcg(firsts + pg + 1);
-    if (j0 == j1) continue;
-    const int id = kv8_page(table, p.c.max_pages, p.c.pages, pg, lane == 0 ? p.status : nullptr);
-    if (id < 0) continue;
-    int8_t *codes = kv ? p.c.v_codes : p.c.k_codes;
-    float *scales = kv ? p.c.v_scales : p.c.k_scales;
-    int8_t *dst = codes + ((size_t)id * p.c.kv_heads + h) * page_bytes;
-    const int live = min(p.c.page, p.keep - (pg << p.shift));
-    const bool stay = j1 - j0 < live;
-    const float old = pg == edge ? s_edge[kv] : scales[(size_t)id * p.c.kv_heads + h];
-    float top = stay ? old : 0.f;
-    // where the row of hole j comes from: its page and that page's scale
-    auto from = [&](int j, int &src, int &sid, float &s) {
-      src = __ldcg(moving + j);
-      sid = kv8_page(table, p.c.max_pages, p.c.pages, src >> p.shift, p.status);
-      s = sid < 0 ? 0.f : (src >> p.shift) == edge ? s_edge[kv]
-                        : scales[(size_t)sid * p.c.kv_heads + h];
-    };
-    uint32_t filled[4] = {0, 0, 0, 0};  // rows of the page that are holes
-    for (int j = j0; j < j1; j += 32) {
-      uint32_t bit = 0;
-      int word = 4;
-      if (j + lane < j1) {
-        int src, sid;
-        float s;
-        from(j + lane, src, sid, s);
-        top = fmaxf(top, s);
-        const int r = __ldcg(holes + j + lane) & (p.c.page - 1);
-        word = r >> 5;
-        bit = 1u << (r & 31);
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        filled[w] |= __reduce_or_sync(0xffffffffu, word == w ? bit : 0u);
+  int8_t *codes = kv ? p.c.v_codes : p.c.k_codes;
+  float *scales = kv ? p.c.v_scales : p.c.k_scales;
+  auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory"); };
+
+  // the CTA's pages, 32 at a time: their first hole and the number of holes
+  for (int pg0 = blockIdx.x; pg0 < pages; pg0 += 32 * gridDim.x) {
+    const int mine = pg0 + lane * gridDim.x;
+    int first_l = 0, count_l = 0;
+    if (mine < pages) {
+      first_l = firsts[mine];
+      count_l = firsts[mine + 1] - first_l;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (stay && top > old) {  // the rows that stay take the larger scale
-      const float ratio = __fdiv_rn(old, top);
-#pragma unroll 4
-      for (int x = lane; x < live * lpr; x += 32) {
-        const int r = x / lpr;
-        const uint32_t f = r < 64 ? (r < 32 ? filled[0] : filled[1])
-                                  : (r < 96 ? filled[2] : filled[3]);
-        if ((f >> (r & 31)) & 1) continue;
-        uint4 *at = reinterpret_cast<uint4 *>(dst) + x;
-        *at = kv8_recode(*at, ratio);
-      }
-    }
-    const int per = 32 / lpr, sub = lane / lpr, ch = lane % lpr;
-    for (int j = j0; j < j1; j += 32) {
-      int src = 0, sid = -1, row = 0;
-      float s = 0.f;
-      if (j + lane < j1) {
-        from(j + lane, src, sid, s);
-        row = __ldcg(holes + j + lane);
+    for (uint32_t todo = __ballot_sync(0xffffffffu, count_l > 0); todo; todo &= todo - 1) {
+      const int at = __ffs(todo) - 1, pg = pg0 + at * gridDim.x;
+      const int j0 = __shfl_sync(0xffffffffu, first_l, at);
+      const int count = __shfl_sync(0xffffffffu, count_l, at);
+      const int id = kv8_page(table, p.c.max_pages, p.c.pages, pg, tid == 0 ? p.status : nullptr);
+      if (id < 0) continue;
+      const int live = min(p.c.page, p.keep - (pg << p.shift));
+      const bool stay = count < live;
+      const float old = pg == edge ? edge_scale : scales[(size_t)id * p.c.kv_heads + h];
+      // ---- hole `tid` of the page, and where its new row comes from
+      int src = -1, sid = -1, row = 0;
+      float from = 0.f;
+      if (tid < count) {
+        src = moving[j0 + tid];
+        row = holes[j0 + tid];
+        sid = kv8_page(table, p.c.max_pages, p.c.pages, src >> p.shift, p.status);
+        if (sid >= 0)
+          from = (src >> p.shift) == edge ? edge_scale : scales[(size_t)sid * p.c.kv_heads + h];
+        s_src[kv][tid] = src & (p.c.page - 1);
+        s_sid[kv][tid] = sid;
+        s_row[kv][tid] = row & (p.c.page - 1);
+        s_from[kv][tid] = from;
         if (kv == 0) {
-          weights[row] = weights[src];
-          if (positions) positions[row] = positions[src];
+          const size_t w = (size_t)unit * p.room;
+          p.weights[w + row] = p.weights[w + src];
+          if (p.positions) p.positions[w + row] = p.positions[w + src];
         }
       }
-      const float ratio = top > 0.f ? __fdiv_rn(s, top) : 1.f;
-      const int count = min(32, j1 - j);
-#pragma unroll 4
-      for (int k = 0; k < count; k += per) {
-        const int o = k + sub;
-        const int osrc = __shfl_sync(0xffffffffu, src, o & 31);
-        const int osid = __shfl_sync(0xffffffffu, sid, o & 31);
-        const int orow = __shfl_sync(0xffffffffu, row, o & 31);
-        const float orat = __shfl_sync(0xffffffffu, ratio, o & 31);
-        if (o >= count || osid < 0) continue;
-        const uint4 x = *(reinterpret_cast<const uint4 *>(
-                              codes + ((size_t)osid * p.c.kv_heads + h) * page_bytes +
-                              (size_t)(osrc & (p.c.page - 1)) * D) + ch);
-        *(reinterpret_cast<uint4 *>(dst + (size_t)(orow & (p.c.page - 1)) * D) + ch) =
-            orat == 1.f ? x : kv8_recode(x, orat);
+      const int r = row & (p.c.page - 1);
+      float top = from;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t f = __reduce_or_sync(0xffffffffu, src >= 0 && r >> 5 == w ? 1u << (r & 31) : 0u);
+        if (lane == 0) s_filled[kv][w][warp] = f;
       }
+      if (lane == 0) s_top[kv][warp] = top;
+      meet();
+      top = stay ? old : 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, s_top[kv][w]);
+
+      // ---- rows that move, and rows that stay but take a larger scale
+      uint4 *dst = reinterpret_cast<uint4 *>(codes + ((size_t)id * p.c.kv_heads + h) * page_bytes);
+      for (int x0 = tid; x0 < count << lsh; x0 += EM_HALF * EM_AHEAD) {
+        uint4 v[EM_AHEAD];
+#pragma unroll
+        for (int k = 0; k < EM_AHEAD; ++k) {
+          const int x = x0 + k * EM_HALF, o = x >> lsh;
+          if (o < count && s_sid[kv][o] >= 0)
+            v[k] = reinterpret_cast<const uint4 *>(
+                codes + ((size_t)s_sid[kv][o] * p.c.kv_heads + h) * page_bytes)[
+                (s_src[kv][o] << lsh) + (x & (lpr - 1))];
+        }
+#pragma unroll
+        for (int k = 0; k < EM_AHEAD; ++k) {
+          const int x = x0 + k * EM_HALF, o = x >> lsh;
+          if (o < count && s_sid[kv][o] >= 0) {
+            const float ratio = top > 0.f ? __fdiv_rn(s_from[kv][o], top) : 1.f;
+            dst[(s_row[kv][o] << lsh) + (x & (lpr - 1))] = ratio == 1.f ? v[k] : kv8_recode(v[k], ratio);
+          }
+        }
+      }
+      if (stay && top > old) {
+        const float ratio = __fdiv_rn(old, top);
+        uint32_t filled[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          filled[w] = s_filled[kv][w][0] | s_filled[kv][w][1] | s_filled[kv][w][2] | s_filled[kv][w][3];
+        auto stays = [&](int x) {
+          const int y = x >> lsh;
+          const uint32_t f = y < 64 ? (y < 32 ? filled[0] : filled[1]) : (y < 96 ? filled[2] : filled[3]);
+          return y < live && !((f >> (y & 31)) & 1);
+        };
+        for (int x0 = tid; x0 < live << lsh; x0 += EM_HALF * EM_AHEAD) {
+          uint4 v[EM_AHEAD];
+#pragma unroll
+          for (int k = 0; k < EM_AHEAD; ++k)
+            if (stays(x0 + k * EM_HALF)) v[k] = dst[x0 + k * EM_HALF];
+#pragma unroll
+          for (int k = 0; k < EM_AHEAD; ++k)
+            if (stays(x0 + k * EM_HALF)) dst[x0 + k * EM_HALF] = kv8_recode(v[k], ratio);
+        }
+      }
+      if (tid == 0 && top != old) scales[(size_t)id * p.c.kv_heads + h] = top;
+      meet();  // the page's holes have been read
     }
-    if (lane == 0 && top != old) scales[(size_t)id * p.c.kv_heads + h] = top;
   }
 }
 
 struct EvictPlan {
-  int cap, most, ctas, cached;
+  int cap, most, threads, ctas, cached;
   long long stride;
   size_t bytes;
 };
@@ -351,14 +428,44 @@ EvictPlan ev_plan(const VbKv8EvictArgs *a) {
   const int over = pl.cap > a->keep ? pl.cap - a->keep : 0;
   pl.most = over < a->keep ? over : a->keep;
   const long long units = (long long)a->cache.batch * a->cache.kv_heads;
+  // Up to 8 rows a thread; 1024 threads a CTA where that does not cost a second wave.
+  pl.threads = units <= 148 ? 1024 : 512;
   pl.ctas = 1;
-  while (pl.ctas < 8 && units * pl.ctas * 2 <= 148 && pl.cap > 2 * EV_THREADS * pl.ctas)
+  while (pl.ctas < EV_CTAS && units * pl.ctas * 2 <= 148 && pl.cap > 8 * pl.threads * pl.ctas)
     pl.ctas *= 2;
-  const long long per = align_up((pl.cap + pl.ctas - 1) / pl.ctas, EV_THREADS);
+  const long long per = align_up((pl.cap + pl.ctas - 1) / pl.ctas, pl.threads);
   pl.cached = (int)(per < EV_KEYS ? per : EV_KEYS);
-  pl.stride = 2ll * pl.most + (a->keep + a->cache.page - 1) / a->cache.page + 1;
+  pl.stride = 2ll * pl.most + (a->keep + a->cache.page - 1) / a->cache.page + 3;
   pl.bytes = pl.most ? (size_t)(units * pl.stride) * sizeof(int32_t) : 0;
   return pl;
+}
+
+template <int T>
+int ev_select(const Kv8EvictParams &p, const EvictPlan &pl, long long units, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  const int set = once_per_device(ready, [] {
+    const cudaError_t e = cudaFuncSetAttribute(
+        kv8_evict_select_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4);
+    return e == cudaSuccess ? VB_OK
+                            : set_error(VB_ERR_CUDA, "kv8_evict_select_kernel attributes: %s",
+                                        cudaGetErrorString(e));
+  });
+  if (set != VB_OK) return set;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * pl.ctas));
+  cfg.blockDim = dim3(T);
+  cfg.dynamicSmemBytes = (size_t)pl.cached * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = pl.ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kv8_evict_select_kernel<T>, p);
+  return check_launch("kv8_evict_select_kernel");
 }
 
 int ev_check(const VbKv8EvictArgs *a) {
@@ -367,6 +474,9 @@ int ev_check(const VbKv8EvictArgs *a) {
   if (rc != VB_OK) return rc;
   VB_REQUIRE(a->keep >= 1 && a->room >= 0 && a->room <= 0x7fffffff - 65536,
              "vb_kv8_evict: keep=%d room=%d", a->keep, a->room);
+  VB_REQUIRE((long long)a->cache.batch * a->cache.kv_heads <= 65535,
+             "vb_kv8_evict: %d sequences of %d kv heads (at most 65535 together)", a->cache.batch,
+             a->cache.kv_heads);
   VB_REQUIRE(a->first >= 0 && a->recent >= 0 && (long long)a->first + a->recent <= a->keep,
              "vb_kv8_evict: first=%d recent=%d of keep=%d", a->first, a->recent, a->keep);
   return VB_OK;
@@ -394,7 +504,6 @@ int vb_kv8_evict(const VbKv8EvictArgs *a, vb_stream_t stream) {
                      a->workspace_bytes, pl.bytes);
   VB_REQUIRE(((uintptr_t)a->workspace % 16) == 0, "vb_kv8_evict: workspace alignment");
   const long long units = (long long)a->cache.batch * a->cache.kv_heads;
-  VB_REQUIRE(units * pl.ctas <= 0x7fffffffll, "vb_kv8_evict: too many sequences and heads");
   Kv8EvictParams p;
   p.c = a->cache;
   p.weights = a->weights; p.positions = a->positions;
@@ -404,30 +513,15 @@ int vb_kv8_evict(const VbKv8EvictArgs *a, vb_stream_t stream) {
   p.room = a->room; p.cap = pl.cap; p.keep = a->keep; p.first = a->first; p.recent = a->recent;
   p.shift = kv8_page_shift(a->cache.page);
   p.cached = pl.cached;
-  static std::atomic<uint64_t> ready{0};
-  const int set = once_per_device(ready, [] {
-    const cudaError_t e = cudaFuncSetAttribute(
-        kv8_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4);
-    return e == cudaSuccess ? VB_OK
-                            : set_error(VB_ERR_CUDA, "kv8_evict_kernel attributes: %s",
-                                        cudaGetErrorString(e));
-  });
-  if (set != VB_OK) return set;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * pl.ctas));
-  cfg.blockDim = dim3(EV_THREADS);
-  cfg.dynamicSmemBytes = (size_t)pl.cached * 4;
-  cfg.stream = as_stream(stream);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = pl.ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  cudaLaunchKernelEx(&cfg, kv8_evict_kernel, p);
-  return check_launch("kv8_evict_kernel");
+  const int rc2 = pl.threads == 1024 ? ev_select<1024>(p, pl, units, as_stream(stream))
+                                     : ev_select<512>(p, pl, units, as_stream(stream));
+  if (rc2 != VB_OK || pl.most == 0) return rc2;
+  // CTAs of a (sequence, head): one a page, fewer once that fills the SMs several times
+  const int pages = (a->keep + a->cache.page - 1) / a->cache.page;
+  const long long few = (148 * 16 + units - 1) / units;
+  vb_launch(kv8_evict_move_kernel, dim3((unsigned)(pages < few ? pages : few), (unsigned)units),
+            dim3(EM_THREADS), 0, as_stream(stream), true, p);
+  return check_launch("kv8_evict_move_kernel");
 }
 
 }  // extern "C"

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(WG_THREADS) kv8_weigh_kernel(const __grid_cons
   if (lane < w.groups && first_key(lane) < keys) {
     id = kv8_page(p.c.page_table + (size_t)b * p.c.max_pages, p.c.max_pages, p.c.pages,
                   first_key(lane) >> p.shift, p.status);
-    if (id >= 0) ks_l = __ldg(p.c.k_scales + (size_t)id * H + h);
+    if (id >= 0) ks_l = __ldcg(p.c.k_scales + (size_t)id * H + h);
   }
   uint8_t *mine = ring + (warp * STAGES * PIECES * 32 + lane) * 16;
   auto issue = [&](int it) {
@@ -399,7 +399,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
       for (int i = 0; i < KN; ++i) {
         const int key = kkey + i * KSTEP;  // a tile's half starts on a page boundary
         const int pg = __shfl_sync(0xffffffffu, id, key >> 4);
-        kr[i] = ldg_nc_v4(kbase + pg * pool_step + (key & (p.c.page - 1)) * D);
+        kr[i] = __ldcg(reinterpret_cast<const uint4 *>(kbase + pg * pool_step +
+                                                       (key & (p.c.page - 1)) * D));
       }
     };
     load(group_page(t0));
@@ -452,7 +453,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
     auto scale_of = [&](int t) {
       const int key = t * WR_KEYS + rank * 128 + r;
       const int id = key < keys ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : -1;
-      return (unsigned)id < (unsigned)p.c.pages ? __ldg(p.c.k_scales + (size_t)id * H + h) : -1.f;
+      return (unsigned)id < (unsigned)p.c.pages ? __ldcg(p.c.k_scales + (size_t)id * H + h) : -1.f;
     };
     float ks_n = scale_of(t0);
     ready();
