@@ -12,9 +12,11 @@
 // which leaves the rows of that page as they are.
 //
 // kv8_evict_select_kernel: a cluster of up to 8 CTAs owns one (sequence, kv head).
-// Weights become 32-bit keys in their order (kept in shared memory); three
-// histograms of 11, 11 and 10 bits, added up over the cluster, give the last key
-// that stays. Ballots count and number holes and moving rows, in order.
+// Weights become 32-bit keys in their order (kept in shared memory); up to three
+// histograms of 11, 11 and 10 bits give the last key that stays: every CTA adds the
+// bins that it has rows in to those of all others (reading all bins of all others
+// instead took 5 us of 20 for 65,536 rows). Ballots count and number holes and
+// moving rows, in order.
 // kv8_evict_move_kernel: a CTA fills the holes of one page after another, half of it
 // K's and half V's, and moves weights and positions with K. Nothing is written that
 // another CTA still reads: rows move from `keep` on to below it, and the scale of the
@@ -26,7 +28,8 @@ namespace {
 
 constexpr int EV_CTAS = 8;            // most CTAs of a cluster
 constexpr int EV_BINS = 2048;
-constexpr int EV_KEYS = 24576;        // most keys of a CTA in shared memory
+constexpr int EV_HELD = 16;           // rows that a thread holds the keys of
+constexpr int EV_KEYS = 24576;        // else: most keys of a CTA in shared memory
 constexpr uint32_t EV_SAFE = 0xFFFFFFFFu;
 
 struct Kv8EvictParams {
@@ -62,6 +65,12 @@ __device__ __forceinline__ void ev_sync(uint32_t ctas) {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;"
                  ::: "memory");
 }
+// Adds to a word of CTA `rank`'s shared memory.
+__device__ __forceinline__ void ev_peer_add(uint32_t *p, uint32_t rank, uint32_t x) {
+  uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(rank));
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
+}
 // A word of CTA `rank`'s shared memory. (Not ordered among themselves, so that several are
 // on their way at once; the barriers around them are.)
 __device__ __forceinline__ uint32_t ev_peer(const void *p, uint32_t rank) {
@@ -71,11 +80,14 @@ __device__ __forceinline__ uint32_t ev_peer(const void *p, uint32_t rank) {
   return r;
 }
 
-template <int EV_THREADS>
+// HELD: a thread has up to EV_HELD rows, whose keys stay in registers (each pass over
+// the rows costs instructions more than anything else); else keys are in shared memory,
+// up to p.cached of them.
+template <int EV_THREADS, bool HELD>
 __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const __grid_constant__ Kv8EvictParams p) {
   constexpr int EV_WARPS = EV_THREADS / 32, EV_PER = EV_BINS / EV_THREADS;
   extern __shared__ uint32_t s_keys[];
-  __shared__ uint32_t s_hist[2][EV_BINS];
+  __shared__ uint32_t s_hist[EV_BINS], s_all[3][EV_BINS];  // the CTA's; the cluster's
   __shared__ uint32_t s_warp[2][EV_WARPS], s_total[3];  // total: ties; holes, moving rows
   __shared__ uint32_t s_bin, s_above, s_count;
   __shared__ int s_newest;
@@ -104,38 +116,88 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const __gr
     const uint32_t k = __float_as_uint(w);
     return w != w ? 0u : k >> 31 ? ~k : k | 0x80000000u;
   };
-  // ---- the newest position, while the weights are on their way too
-  long long late = 0x7fffffffffffll;  // positions above it are protected
-  if (p.recent > 0) {
-    int newest = n - 1;
-    if (positions) {
-      newest = -0x7fffffff - 1;
-#pragma unroll 4
-      for (int t = 0; t < turns; ++t)
-        if (row0 + t * 32 < n) {
-          newest = max(newest, positions[row0 + t * 32]);
-          if (at0 + t * 32 < p.cached) s_keys[at0 + t * 32] = order(weights[row0 + t * 32]);
-        }
-      newest = __reduce_max_sync(0xffffffffu, newest);
-      if (lane == 0) s_warp[0][warp] = (uint32_t)newest;
-      __syncthreads();
-      if (warp == 0) {
-        newest = __reduce_max_sync(0xffffffffu, (int)s_warp[0][lane % EV_WARPS]);
-        if (lane == 0) s_newest = newest;
-      }
-      ev_sync(C);
-      newest = (int)ev_peer(&s_newest, min((uint32_t)lane, C - 1));
-      newest = __reduce_max_sync(0xffffffffu, newest);
+  for (int i = tid; i < EV_BINS; i += EV_THREADS)
+    s_hist[i] = s_all[0][i] = s_all[1][i] = s_all[2][i] = 0;
+  // Goes through the warp's rows: f(turn, row number).
+  auto rows = [&](auto f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int t = 0; t < EV_HELD; ++t)
+        if (t < turns) f(t, row0 + t * 32);
+    } else {
+      for (int t = 0; t < turns; ++t) f(t, row0 + t * 32);
     }
-    late = (long long)newest - p.recent;
-  }
-  const bool ordered = p.recent > 0 && positions;  // s_keys has the weights' order already
-  auto make_key = [&](int i, int at) {
-    if (i < p.first || (p.recent > 0 && (positions ? positions[i] : i) > late)) return EV_SAFE;
-    return ordered && at < p.cached ? s_keys[at] : order(weights[i]);
   };
-  auto key = [&](int t) {
-    return at0 + t * 32 < p.cached ? s_keys[at0 + t * 32] : make_key(row0 + t * 32, at0 + t * 32);
+  // ---- the weights' order, and the newest position
+  const bool dated = p.recent > 0 && positions;
+  int newest = -0x7fffffff - 1;
+  uint32_t held[HELD ? EV_HELD : 1];
+  int date[HELD ? EV_HELD : 1];
+  if constexpr (HELD) {
+    rows([&](int t, int i) {
+      held[t] = __float_as_uint(i < n ? weights[i] : 0.f);
+      date[t] = !dated ? i : i < n ? positions[i] : newest;
+    });
+    rows([&](int t, int i) {
+      held[t] = order(__uint_as_float(held[t]));
+      if (dated) newest = max(newest, date[t]);
+    });
+  } else {
+    for (int t0 = 0; t0 < turns; t0 += 4) {
+      float w[4];
+      int q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = row0 + (t0 + k) * 32, at = at0 + (t0 + k) * 32;
+        const bool there = t0 + k < turns && i < n;
+        w[k] = there && at < p.cached ? weights[i] : 0.f;
+        q[k] = there && dated ? positions[i] : newest;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int at = at0 + (t0 + k) * 32;
+        newest = max(newest, q[k]);
+        if (t0 + k < turns && at < p.cached) s_keys[at] = order(w[k]);
+      }
+    }
+  }
+  if (dated) {
+    newest = __reduce_max_sync(0xffffffffu, newest);
+    if (lane == 0) s_warp[0][warp] = (uint32_t)newest;
+    __syncthreads();
+    if (warp == 0) {
+      newest = __reduce_max_sync(0xffffffffu, (int)s_warp[0][lane % EV_WARPS]);
+      if (lane == 0) s_newest = newest;
+    }
+  }
+  ev_sync(C);  // (and all bins are zero)
+  if (dated) {
+    newest = (int)ev_peer(&s_newest, min((uint32_t)lane, C - 1));
+    newest = __reduce_max_sync(0xffffffffu, newest);
+  } else {
+    newest = n - 1;
+  }
+  // positions above it are protected
+  const long long late = p.recent > 0 ? (long long)newest - p.recent : 0x7fffffffffffll;
+  if constexpr (HELD) {
+    rows([&](int t, int i) {
+      if (i < p.first || date[t] > late) held[t] = EV_SAFE;
+    });
+  } else {
+    rows([&](int t, int i) {
+      const int at = at0 + t * 32;
+      if (at < p.cached && (i < p.first || (dated && i < n ? positions[i] : i) > late))
+        s_keys[at] = EV_SAFE;
+    });
+  }
+  auto key = [&](int t, int i) {
+    if constexpr (HELD) {
+      return held[t];
+    } else {
+      const int at = at0 + t * 32;
+      if (at < p.cached) return s_keys[at];
+      return i < p.first || (dated ? positions[i] : i) > late ? EV_SAFE : order(weights[i]);
+    }
   };
 
   // ---- the key of the last row that stays: `need` of the rows that have it do
@@ -144,43 +206,30 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const __gr
 #pragma unroll 1
   for (int d = 0; d < 3 && ties; ++d) {
     const int low = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
-    uint32_t *hist = s_hist[d & 1];
-    for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
-    __syncthreads();
-#pragma unroll 4
-    for (int t = 0; t < turns; ++t) {
-      const int i = row0 + t * 32;
-      if (i >= n) continue;
-      uint32_t k;
-      if (d == 0) {
-        k = make_key(i, at0 + t * 32);
-        if (at0 + t * 32 < p.cached) s_keys[at0 + t * 32] = k;
-      } else {
-        k = key(t);
-      }
+    if (d > 0 && C > 1) {
+      for (int i = tid; i < EV_BINS; i += EV_THREADS) s_hist[i] = 0;
+      __syncthreads();
+    }
+    uint32_t *hist = C > 1 ? s_hist : s_all[d];
+    rows([&](int t, int i) {
+      if (i >= n) return;
+      const uint32_t k = key(t, i);
       if (d == 0 || k >> (low + bits) == prefix)
         atomicAdd(hist + ((k >> low) & ((1u << bits) - 1)), 1u);
+    });
+    __syncthreads();
+    if (C > 1) {
+      for (int i = tid; i < EV_BINS; i += EV_THREADS) {
+        const uint32_t x = s_hist[i];
+        if (x)
+          for (uint32_t r = 0; r < C; ++r) ev_peer_add(s_all[d] + i, r, x);
+      }
+      ev_sync(C);
     }
-    ev_sync(C);
     // bins from the top: thread tid has EV_PER of them from EV_BINS - 1 - EV_PER tid down
     uint32_t bin[EV_PER], mine = 0;
-    const uint32_t *top = hist + EV_BINS - 1 - EV_PER * tid;
-    if (C == 1) {
 #pragma unroll
-      for (int x = 0; x < EV_PER; ++x) bin[x] = top[-x];
-    } else {
-      uint32_t y[EV_CTAS][EV_PER];
-#pragma unroll
-      for (int r = 0; r < EV_CTAS; ++r)
-#pragma unroll
-        for (int x = 0; x < EV_PER; ++x) y[r][x] = ev_peer(top - x, min((uint32_t)r, C - 1));
-#pragma unroll
-      for (int x = 0; x < EV_PER; ++x) {
-        bin[x] = 0;
-#pragma unroll
-        for (int r = 0; r < EV_CTAS; ++r) bin[x] += r < C ? y[r][x] : 0u;
-      }
-    }
+    for (int x = 0; x < EV_PER; ++x) bin[x] = s_all[d][EV_BINS - 1 - EV_PER * tid - x];
 #pragma unroll
     for (int x = 0; x < EV_PER; ++x) mine += bin[x];
     uint32_t inc = mine;
@@ -240,46 +289,45 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const __gr
   uint32_t tie0 = 0, unused;
   if (ties) {
     uint32_t mine = 0;
-    for (int t = 0; t < turns; ++t)
-      mine += __popc(__ballot_sync(0xffffffffu, row0 + t * 32 < n && key(t) == last));
+    rows([&](int t, int i) {
+      mine += __popc(__ballot_sync(0xffffffffu, i < n && key(t, i) == last));
+    });
     before(mine, 0, 0, tie0, unused);
   }
   const uint32_t below = (1u << lane) - 1;
-  // whether row t of this lane stays; `tie`: rows with the last key before this turn
-  auto stays = [&](int t, uint32_t &tie) {
-    const bool there = row0 + t * 32 < n;
-    const uint32_t k = there ? key(t) : 0u;
-    if (!ties) return there && k >= last;
-    const uint32_t same = __ballot_sync(0xffffffffu, there && k == last);
-    const bool s = there && (k > last || (k == last && tie + __popc(same & below) < need));
+  // whether a row stays; `tie`: rows with the last key before this turn
+  auto stays = [&](int t, int i, uint32_t &tie) {
+    const uint32_t k = i < n ? key(t, i) : 0u;
+    if (!ties) return i < n && k >= last;
+    const uint32_t same = __ballot_sync(0xffffffffu, i < n && k == last);
+    const bool s = i < n && (k > last || (k == last && tie + __popc(same & below) < need));
     tie += __popc(same);
     return s;
   };
-  uint32_t n_holes = 0, n_moving = 0, tie = tie0, bits = 0;  // bit t: row t stays (t < 32)
-  for (int t = 0; t < turns; ++t) {
-    const int i = row0 + t * 32;
-    const bool s = stays(t, tie);
-    if (t < 32) bits |= (uint32_t)s << t;
+  uint32_t n_holes = 0, n_moving = 0, tie = tie0;
+  rows([&](int t, int i) {
+    const bool s = stays(t, i, tie);
     n_holes += __popc(__ballot_sync(0xffffffffu, !s && i < p.keep));
     n_moving += __popc(__ballot_sync(0xffffffffu, s && i >= p.keep));
-  }
+  });
   uint32_t hole, move;
   before(n_holes, n_moving, 1, hole, move);
-  uint32_t tie1 = tie0;
-  for (int t = 0; t < turns; ++t) {
-    const int i = row0 + t * 32;
-    const bool s = turns <= 32 ? (bits >> t) & 1 : stays(t, tie1);
+  tie = tie0;
+  rows([&](int t, int i) {
+    const bool s = stays(t, i, tie);
     const uint32_t hb = __ballot_sync(0xffffffffu, !s && i < p.keep);
     const uint32_t mb = __ballot_sync(0xffffffffu, s && i >= p.keep);
-    if (i < p.keep && (i & (p.c.page - 1)) == 0)
-      firsts[i >> p.shift] = (int)(hole + __popc(hb & below));
-    if (i == p.keep - 1)  // the number of holes behind the last page
-      firsts[(p.keep + p.c.page - 1) >> p.shift] = (int)(hole + __popc(hb & (below * 2 + 1)));
-    if ((hb >> lane) & 1) holes[hole + __popc(hb & below)] = i;
+    if (i < p.keep) {
+      const uint32_t at = hole + __popc(hb & below), mine = (hb >> lane) & 1;
+      if ((i & (p.c.page - 1)) == 0) firsts[i >> p.shift] = (int)at;
+      if (i == p.keep - 1)  // the number of holes, behind the last page
+        firsts[(p.keep + p.c.page - 1) >> p.shift] = (int)(at + mine);
+      if (mine) holes[at] = i;
+    }
     if ((mb >> lane) & 1) moving[move + __popc(mb & below)] = i;
     hole += __popc(hb);
     move += __popc(mb);
-  }
+  });
   // the page in which `keep` falls: rows of it may move, and its scale may change
   if (rank == 0 && tid < 2) {
     const int id = kv8_page(table, p.c.max_pages, p.c.pages, p.keep >> p.shift, nullptr);
@@ -294,7 +342,7 @@ constexpr int EM_THREADS = 256;
 constexpr int EM_HALF = 128;  // threads of K, and of V: one for each row of the largest page
 constexpr int EM_AHEAD = 4;   // pieces of 16 codes that a thread has in flight
 
-__global__ void __launch_bounds__(EM_THREADS, 6) kv8_evict_move_kernel(const __grid_constant__ Kv8EvictParams p) {
+__global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __grid_constant__ Kv8EvictParams p) {
   __shared__ int s_src[2][EM_HALF], s_sid[2][EM_HALF], s_row[2][EM_HALF];
   __shared__ float s_from[2][EM_HALF], s_top[2][4];
   __shared__ uint32_t s_filled[2][4][4];
@@ -415,6 +463,7 @@ __global__ void __launch_bounds__(EM_THREADS, 6) kv8_evict_move_kernel(const __g
 
 struct EvictPlan {
   int cap, most, threads, ctas, cached;
+  bool held;
   long long stride;
   size_t bytes;
 };
@@ -428,24 +477,27 @@ EvictPlan ev_plan(const VbKv8EvictArgs *a) {
   const int over = pl.cap > a->keep ? pl.cap - a->keep : 0;
   pl.most = over < a->keep ? over : a->keep;
   const long long units = (long long)a->cache.batch * a->cache.kv_heads;
-  // Up to 8 rows a thread; 1024 threads a CTA where that does not cost a second wave.
+  // Up to 8 rows a thread, then more CTAs, as long as every one of 1024 threads has an SM
+  // (4,160 rows of 2 heads: one CTA a head 8.7 us, four 12: each barrier of a cluster
+  // costs half a microsecond, a row of a thread 0.6 in all).
   pl.threads = units <= 148 ? 1024 : 512;
   pl.ctas = 1;
   while (pl.ctas < EV_CTAS && units * pl.ctas * 2 <= 148 && pl.cap > 8 * pl.threads * pl.ctas)
     pl.ctas *= 2;
   const long long per = align_up((pl.cap + pl.ctas - 1) / pl.ctas, pl.threads);
-  pl.cached = (int)(per < EV_KEYS ? per : EV_KEYS);
+  pl.held = per <= EV_HELD * pl.threads;
+  pl.cached = (int)(pl.held ? 0 : per < EV_KEYS ? per : EV_KEYS);
   pl.stride = 2ll * pl.most + (a->keep + a->cache.page - 1) / a->cache.page + 3;
   pl.bytes = pl.most ? (size_t)(units * pl.stride) * sizeof(int32_t) : 0;
   return pl;
 }
 
-template <int T>
+template <int T, bool HELD>
 int ev_select(const Kv8EvictParams &p, const EvictPlan &pl, long long units, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
   const int set = once_per_device(ready, [] {
     const cudaError_t e = cudaFuncSetAttribute(
-        kv8_evict_select_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4);
+        kv8_evict_select_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4);
     return e == cudaSuccess ? VB_OK
                             : set_error(VB_ERR_CUDA, "kv8_evict_select_kernel attributes: %s",
                                         cudaGetErrorString(e));
@@ -464,7 +516,7 @@ int ev_select(const Kv8EvictParams &p, const EvictPlan &pl, long long units, cud
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaLaunchKernelEx(&cfg, kv8_evict_select_kernel<T>, p);
+  cudaLaunchKernelEx(&cfg, kv8_evict_select_kernel<T, HELD>, p);
   return check_launch("kv8_evict_select_kernel");
 }
 
@@ -513,14 +565,17 @@ int vb_kv8_evict(const VbKv8EvictArgs *a, vb_stream_t stream) {
   p.room = a->room; p.cap = pl.cap; p.keep = a->keep; p.first = a->first; p.recent = a->recent;
   p.shift = kv8_page_shift(a->cache.page);
   p.cached = pl.cached;
-  const int rc2 = pl.threads == 1024 ? ev_select<1024>(p, pl, units, as_stream(stream))
-                                     : ev_select<512>(p, pl, units, as_stream(stream));
+  cudaStream_t s = as_stream(stream);
+  const int rc2 = pl.threads == 1024 ? (pl.held ? ev_select<1024, true>(p, pl, units, s)
+                                                : ev_select<1024, false>(p, pl, units, s))
+                                     : (pl.held ? ev_select<512, true>(p, pl, units, s)
+                                                : ev_select<512, false>(p, pl, units, s));
   if (rc2 != VB_OK || pl.most == 0) return rc2;
   // CTAs of a (sequence, head): one a page, fewer once that fills the SMs several times
   const int pages = (a->keep + a->cache.page - 1) / a->cache.page;
   const long long few = (148 * 16 + units - 1) / units;
   vb_launch(kv8_evict_move_kernel, dim3((unsigned)(pages < few ? pages : few), (unsigned)units),
-            dim3(EM_THREADS), 0, as_stream(stream), true, p);
+            dim3(EM_THREADS), 0, s, true, p);
   return check_launch("kv8_evict_move_kernel");
 }
 
