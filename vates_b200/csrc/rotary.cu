@@ -16,9 +16,6 @@ namespace {
 
 constexpr int RT_THREADS = 256;
 constexpr int RT_PAIRS = 128;      // most rotated pairs of a row
-constexpr int RT_TABLE = 2048;     // (token, pair) sines and cosines of a CTA
-constexpr int RT_TOKENS = 32;      // most tokens of a CTA
-constexpr int RT_AHEAD = 2;        // rows that a thread has in flight
 
 struct RotateParams {
   const uint16_t *src[2];          // q, k
@@ -27,7 +24,7 @@ struct RotateParams {
   int64_t s_in[2][3], s_out[2][3]; // element strides of batch, head, row
   const int32_t *positions;        // [axes][tokens]
   int64_t tokens;                  // batch * L
-  int L, heads[2], dim, half, per, groups;  // tokens of a CTA, CTAs of a sequence
+  int L, heads[2], dim, half, per, groups;  // log2 of a CTA's tokens, CTAs of a sequence
   float eps;
   bool keep;                       // dims from R on are in place already
   double turns[RT_PAIRS];          // frequency / 2 pi
@@ -40,18 +37,20 @@ __device__ __forceinline__ uint4 rt_load(const uint16_t *p, bool vec) {
   return make_uint4(p[0] | ((uint32_t)p[1] << 16), p[2] | ((uint32_t)p[3] << 16),
                     p[4] | ((uint32_t)p[5] << 16), p[6] | ((uint32_t)p[7] << 16));
 }
-__device__ __forceinline__ void rt_floats(float (&x)[8], const uint4 &v) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[2 * j] = __uint_as_float(w[j] << 16);
-    x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-  }
+__device__ __forceinline__ f2 rt_pair(uint32_t w) {
+  return f2_make(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
-__device__ __forceinline__ void rt_store(uint16_t *p, const float (&x)[8], bool vec) {
+__device__ __forceinline__ void rt_pairs(f2 (&x)[4], const uint4 &v) {
+  x[0] = rt_pair(v.x); x[1] = rt_pair(v.y); x[2] = rt_pair(v.z); x[3] = rt_pair(v.w);
+}
+__device__ __forceinline__ void rt_store(uint16_t *p, const f2 (&x)[4], bool vec) {
   uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = pack_bf2(x[2 * j], x[2 * j + 1]);
+  for (int j = 0; j < 4; ++j) {
+    float a, b;
+    f2_split(x[j], a, b);
+    w[j] = pack_bf2(a, b);
+  }
   if (vec) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
@@ -64,103 +63,117 @@ __device__ __forceinline__ void rt_store(uint16_t *p, const float (&x)[8], bool 
 }
 
 // LPR lanes hold a row, 16 dims each: the first R / 16 of them 8 pairs, the
-// others 16 dims that only the norm changes. A CTA takes some tokens of one
-// sequence, all heads: it makes their sines once, and then goes through the rows
-// head by head, so that what it writes to [batch, heads, L, dim] is contiguous.
+// others 16 dims that only the norm changes. A CTA takes up to STEP = 256 / LPR
+// tokens of one sequence, a power of two of them; its STEP rows at a time are those
+// tokens of one head, or of several heads where it has fewer tokens. So a thread
+// stays with one token: its sines are made once, and from head to head only a
+// pointer moves.
+// Rows of a thread in flight, and CTAs per SM: 2 and 4, with a norm, whose registers
+// leave room for 3 CTAs, 3 and 3 (65,536 tokens of 16/2 heads of 256 with it 258 us, 306
+// the other way; 2 x 8,191 of 32/8 heads of 128 without it 79 and 83).
 template <int LPR, bool NORM>
-__global__ void __launch_bounds__(RT_THREADS, 4) rotate_kernel(const __grid_constant__ RotateParams p,
-                                                            bool vec) {
-  __shared__ float2 s_cs[RT_TABLE];  // [token][pair % 8][pair / 8]
+__global__ void __launch_bounds__(RT_THREADS, NORM ? 3 : 4) rotate_kernel(const __grid_constant__ RotateParams p,
+                                                               bool vec) {
+  constexpr int STEP = RT_THREADS / LPR, RT_AHEAD = NORM ? 3 : 2;
+  __shared__ float2 s_cs[STEP * LPR * 8];  // [token][pair % 8][pair / 8]
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x;
-  const int b = blockIdx.x / p.groups, i0 = (blockIdx.x - b * p.groups) * p.per;
-  const int n = min(p.per, p.L - i0);
-  const uint32_t n_inv = (uint32_t)(0xFFFFFFFFu / n) + 1;  // r / n for r * n < 2^32; n = 1: 0
-  const int j = tid % LPR, turned = p.half >> 3;
+  const int tid = threadIdx.x, j = tid % LPR, turned = p.half >> 3;
+  const int b = blockIdx.x / p.groups, i0 = (blockIdx.x - b * p.groups) << p.per;
+  const int n = min(1 << p.per, p.L - i0);
+  const int t = (tid / LPR) & ((1 << p.per) - 1), h0 = (tid / LPR) >> p.per, h_step = STEP >> p.per;
+  const int heads = p.heads[0] + p.heads[1];
   // dims of this lane: two runs of eight
   const int d0 = j < turned ? j * 8 : 2 * p.half + (j - turned) * 16;
   const int d1 = j < turned ? p.half + j * 8 : d0 + 8;
-  const bool live = j * 16 < p.dim && !(p.keep && j >= turned);
-  constexpr int STEP = RT_THREADS / LPR;
-  const int rows = n * (p.heads[0] + p.heads[1]);
-  // row r: token, q (0) or k (1), and head
-  auto place = [&](int r, int &t, int &kind, int &h) {
-    const int hh = n == 1 ? r : (int)__umulhi((uint32_t)r, n_inv);
-    t = r - hh * n;
-    kind = hh >= p.heads[0];
-    h = kind ? hh - p.heads[0] : hh;
-  };
-  auto fetch = [&](int r0, uint4 (&x)[RT_AHEAD], uint4 (&y)[RT_AHEAD]) {
+  const bool live = t < n && j * 16 < p.dim && !(p.keep && j >= turned);
+  const int64_t in0 = b * p.s_in[0][0] + (i0 + t) * p.s_in[0][2];
+  const int64_t in1 = b * p.s_in[1][0] + (i0 + t) * p.s_in[1][2] - p.heads[0] * p.s_in[1][1];
+  uint4 x[RT_AHEAD], y[RT_AHEAD];
+  auto fetch = [&](int h) {
 #pragma unroll
-    for (int k = 0; k < RT_AHEAD; ++k) {
-      const int r = r0 + k * STEP;
+    for (int k = 0; k < RT_AHEAD; ++k, h += h_step) {
       x[k] = y[k] = make_uint4(0, 0, 0, 0);
-      if (r < rows && live) {
-        int t, kind, h;
-        place(r, t, kind, h);
-        const int64_t *st = p.s_in[kind];
-        const uint16_t *src = p.src[kind] + b * st[0] + h * st[1] + (i0 + t) * st[2];
+      if (h < heads && live) {
+        const uint16_t *src = h < p.heads[0] ? p.src[0] + in0 + h * p.s_in[0][1]
+                                             : p.src[1] + in1 + h * p.s_in[1][1];
         x[k] = rt_load(src + d0, vec);
         y[k] = rt_load(src + d1, vec);
       }
     }
   };
-  uint4 x[RT_AHEAD], y[RT_AHEAD];
-  fetch(tid / LPR, x, y);
+  fetch(h0);
   // sines while the first rows are on their way
   for (int z = tid; z < n * p.half; z += RT_THREADS) {
-    const int t = z / p.half, i = z - t * p.half;
-    const double turn = p.positions[p.axis[i] * p.tokens + (int64_t)b * p.L + i0 + t] * p.turns[i];
+    const int u = z / p.half, i = z - u * p.half;
+    const double turn = p.positions[p.axis[i] * p.tokens + (int64_t)b * p.L + i0 + u] * p.turns[i];
     float2 cs;
     sincospif(2.f * (float)(turn - rint(turn)), &cs.y, &cs.x);
-    s_cs[t * p.half + (i & 7) * turned + (i >> 3)] = cs;
+    s_cs[u * p.half + (i & 7) * turned + (i >> 3)] = cs;
   }
   __syncthreads();
-  for (int r0 = tid / LPR; r0 - tid / LPR < rows; r0 += STEP * RT_AHEAD) {
+  f2 cs[4], sn[4];
+  if (j < turned && t < n) {
+    const float2 *e = s_cs + t * p.half + j;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 a = e[2 * k * turned], c = e[(2 * k + 1) * turned];
+      cs[k] = f2_make(a.x, c.x);
+      sn[k] = f2_make(a.y, c.y);
+    }
+  }
+  const f2 minus = f2_make(-1.f, -1.f);
+  const int64_t out0 = b * p.s_out[0][0] + (i0 + t) * p.s_out[0][2];
+  const int64_t out1 = b * p.s_out[1][0] + (i0 + t) * p.s_out[1][2] - p.heads[0] * p.s_out[1][1];
+  // (all lanes of a row, and of its warp, go through the same heads or one more)
+  for (int h = h0; h - h0 < heads; h += h_step * RT_AHEAD) {
 #pragma unroll
     for (int k = 0; k < RT_AHEAD; ++k) {
-      const int r = r0 + k * STEP;
-      int t, kind, h;
-      place(r, t, kind, h);
-      float u[8], v[8];
-      rt_floats(u, x[k]);
-      rt_floats(v, y[k]);
+      const int hk = h + k * h_step;
+      const bool q = hk < p.heads[0];
+      f2 u[4], v[4];
+      rt_pairs(u, x[k]);
+      rt_pairs(v, y[k]);
       if constexpr (NORM) {
-        const uint16_t *w = p.norm[kind];
-        float ss = 0.f;
+        const uint16_t *w = q ? p.norm[0] : p.norm[1];
+        f2 s2 = f2_mul(u[0], u[0]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(u[e], u[e], fmaf(v[e], v[e], ss));
+        for (int e = 0; e < 4; ++e) {
+          if (e > 0) s2 = f2_fma(u[e], u[e], s2);
+          s2 = f2_fma(v[e], v[e], s2);
+        }
+        float ss, s1;
+        f2_split(s2, ss, s1);
+        ss += s1;
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (w && live) {
           const float inv = rsqrtf(ss / p.dim + p.eps);
-          float wu[8], wv[8];
-          rt_floats(wu, rt_load(w + d0, vec));
-          rt_floats(wv, rt_load(w + d1, vec));
+          const f2 inv2 = f2_make(inv, inv);
+          f2 wu[4], wv[4];
+          rt_pairs(wu, rt_load(w + d0, vec));
+          rt_pairs(wv, rt_load(w + d1, vec));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            u[e] *= inv * wu[e];
-            v[e] *= inv * wv[e];
+          for (int e = 0; e < 4; ++e) {
+            u[e] = f2_mul(u[e], f2_mul(wu[e], inv2));
+            v[e] = f2_mul(v[e], f2_mul(wv[e], inv2));
           }
         }
       }
-      if (r >= rows || !live) continue;
+      if (hk >= heads || !live) continue;
       if (j < turned) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 cs = s_cs[t * p.half + e * turned + j];
-          const float c = u[e], s = v[e];
-          u[e] = fmaf(c, cs.x, -s * cs.y);
-          v[e] = fmaf(s, cs.x, c * cs.y);
+        for (int e = 0; e < 4; ++e) {
+          const f2 c = u[e], s = v[e];
+          u[e] = f2_fma(c, cs[e], f2_mul(f2_mul(s, sn[e]), minus));
+          v[e] = f2_fma(s, cs[e], f2_mul(c, sn[e]));
         }
       }
-      const int64_t *st = p.s_out[kind];
-      uint16_t *dst = p.dst[kind] + b * st[0] + h * st[1] + (i0 + t) * st[2];
+      uint16_t *dst = q ? p.dst[0] + out0 + hk * p.s_out[0][1] : p.dst[1] + out1 + hk * p.s_out[1][1];
       rt_store(dst + d0, u, vec);
       rt_store(dst + d1, v, vec);
     }
-    if (r0 - tid / LPR + STEP * RT_AHEAD < rows) fetch(r0 + STEP * RT_AHEAD, x, y);
+    fetch(h + h_step * RT_AHEAD);
   }
 }
 
@@ -230,16 +243,16 @@ extern "C" int vb_rotate_axes(const VbRotateArgs *a, vb_stream_t stream) {
     }
   }
   p.keep = same;
-  // Tokens of a CTA: up to 32, fewer while that leaves SMs without work.
-  int per = RT_TABLE / p.half < RT_TOKENS ? RT_TABLE / p.half : RT_TOKENS;
-  if (per > p.tokens / 592) per = (int)(p.tokens / 592);
-  p.per = per > 1 ? per : 1;
-  p.groups = (a->L + p.per - 1) / p.per;
+  // Tokens of a CTA (a power of two): as many as it has rows at a time, fewer while that
+  // leaves SMs without work.
+  const int lpr = a->dim > 128 ? 16 : a->dim > 64 ? 8 : 4;
+  p.per = lpr == 16 ? 4 : lpr == 8 ? 5 : 6;
+  while (p.per > 0 && (p.tokens >> p.per) < 296) --p.per;
+  p.groups = (a->L + (1 << p.per) - 1) >> p.per;
   const int64_t ctas = (int64_t)p.groups * a->batch;
   VB_REQUIRE(ctas <= 0x7fffffffll, "vb_rotate_axes: too many tokens");
   const bool vec = odd % 8 == 0;
   cudaStream_t s = as_stream(stream);
-  const int lpr = a->dim > 128 ? 16 : a->dim > 64 ? 8 : 4;
   if (lpr == 16) rt_launch<16>(p, (unsigned)ctas, vec, s);
   else if (lpr == 8) rt_launch<8>(p, (unsigned)ctas, vec, s);
   else rt_launch<4>(p, (unsigned)ctas, vec, s);

@@ -66,7 +66,7 @@ def _check(t: torch.Tensor, what: str, shape, dev: int):
 
 def _out(t: torch.Tensor, out: torch.Tensor | None, what: str, dev: int) -> torch.Tensor:
     if out is None:
-        return torch.empty(t.shape, dtype=torch.bfloat16, device=t.device)
+        return t.new_empty(t.shape)
     _check(out, what, t.shape, dev)
     if out.stride(3) != 1:
         raise ValueError(f"{what}: contiguous dims are needed, strides {out.stride()}")
