@@ -1053,23 +1053,26 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __gri
   __shared__ float4 s_a[PG > 1 ? KC_THREADS : 1];
   __shared__ float2 s_ml[PG > 1 ? KC_THREADS : 1];
   pdl_launch_dependents();
-  pdl_wait();
   const Kv8AttnParams &p = w.p;
-  const int tid = threadIdx.x, d4 = tid % LR, pg = tid / LR % PG;
+  const int tid = threadIdx.x, d4 = tid % LR, pg = tid / LR % PG, H = p.c.kv_heads;
   const int row = blockIdx.x * RPC + tid / (LR * PG), per = p.Hq * p.L;
   const bool there = row < p.c.batch * per;
-  int b = 0, h = 0, R = 0;
+  int b = 0, h = 0, R = 0, g = -1, R_pre = 0;
   float M = -INFINITY, ls = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (there) {
+  if (there) {  // (the groups are the plan's, nothing that a kernel ahead writes)
     b = row / per;
-    const int x = row - b * per, hq = x / p.L, i = x - hq * p.L, H = p.c.kv_heads;
+    const int x = row - b * per, hq = x / p.L, i = x - hq * p.L;
     h = hq / p.rep;
     R = i * p.rep + hq - h * p.rep;
-    const int g = w.group_of[b];
+    g = w.group_of[b];
+    if (g >= 0) R_pre = (b - w.groups[g].x) * p.L * p.rep + R;
+  }
+  pdl_wait();
+  if (there) {
     Kv8PartedRow pre, own = kv8_parted_row<D>(w.own, b * H + h, R);
     pre.n = 0;
-    if (g >= 0) pre = kv8_parted_row<D>(w.pre, g * H + h, (b - w.groups[g].x) * p.L * p.rep + R);
+    if (g >= 0) pre = kv8_parted_row<D>(w.pre, g * H + h, R_pre);
     const int n = pre.n + own.n;
     for (int s0 = pg; s0 < n; s0 += PG * AHEAD) {
       float2 ml[AHEAD];
@@ -1244,10 +1247,11 @@ int kv8_shared_run(Kv8AttnParams p, const Kv8SharedPlan &pl, const VbKv8SharedAr
   }
   w.p = p;
   const long long rows = (long long)p.c.batch * p.Hq * p.L;
-  // few rows: four threads for each four dims
+  // few rows: two threads for each four dims (4,096 rows of 10 results 22 us, by one thread
+  // 14; 1,536 rows of 3 6 and 8)
   constexpr int RPC = KC_THREADS * 4 / D;
-  if (rows <= 8192)
-    vb_launch(kv8_shared_join_kernel<D, 4>, dim3((unsigned)((rows * 4 + RPC - 1) / RPC)),
+  if (rows <= 2048)
+    vb_launch(kv8_shared_join_kernel<D, 2>, dim3((unsigned)((rows * 2 + RPC - 1) / RPC)),
               dim3(KC_THREADS), 0, s, true, w);
   else
     vb_launch(kv8_shared_join_kernel<D, 1>, dim3((unsigned)((rows + RPC - 1) / RPC)),

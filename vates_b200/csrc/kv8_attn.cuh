@@ -74,7 +74,7 @@ struct Kv8SegRow {
   int b, i, hr, vis;  // sequence, query, head of the group; keys seen (0: no such row)
 };
 __device__ __forceinline__ Kv8SegRow kv8_seg_row(const Kv8AttnParams &p, const int4 &s, int R) {
-  const int per = p.L * p.rep, m = R / per, r = R - m * per;
+  const int per = p.L * p.rep, m = s.y == 1 ? R >= per : R / per, r = R - m * per;
   Kv8SegRow x;
   x.b = s.x + min(m, s.y - 1);
   x.i = p.row_of(r);

@@ -65,9 +65,11 @@ __device__ __forceinline__ void wg_add(const Kv8WeighParams &w, const Kv8WeighSp
 // ------------------------------------------------------------ few query rows
 constexpr int WG_THREADS = 128;
 constexpr int WG_WARPS = WG_THREADS / 32;
-constexpr int WG_RING = 12288;             // bytes of a warp's ring
+// Stages of 16 keys in a warp's ring: as little in flight per warp as still hides its own
+// computing, so that more warps fit (heads of 128, 3, 4 and 6 stages: 31, 34 and 40 us;
+// of 256, 2 and 3: 17 and 22).
 template <int D>
-constexpr int wg_stages() { return WG_RING / (D * 16); }   // 16 keys each
+constexpr int wg_stages() { return D == 64 ? 3 : 2; }
 
 __device__ __forceinline__ void wg_mma(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
@@ -159,6 +161,17 @@ __global__ void __launch_bounds__(WG_THREADS) kv8_weigh_kernel(const __grid_cons
     }
   }
   __syncthreads();
+  // the fragments of eight rows stay in registers
+  constexpr bool HELD = NR == 1;
+  uint2 held[HELD ? D / 16 : 1];
+  auto fragment = [&](int n, int step) {
+    return *reinterpret_cast<const uint2 *>(
+        s_q + ((n * (D / 32) + (step >> 1)) * 32 + lane) * 4 + (step & 1) * 2);
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) held[k] = fragment(0, k);
+  }
   float2 row[NR][2];
   int vis[NR][2];
 #pragma unroll
@@ -199,8 +212,7 @@ __global__ void __launch_bounds__(WG_THREADS) kv8_weigh_kernel(const __grid_cons
         const int step = x * 4 + r4;
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          const uint2 bq = *reinterpret_cast<const uint2 *>(
-              s_q + ((n * (D / 32) + (step >> 1)) * 32 + lane) * 4 + (step & 1) * 2);
+          const uint2 bq = HELD ? held[HELD ? step : 0] : fragment(n, step);
           wg_mma(acc[n][step & 1], a, bq.x, bq.y);
         }
       }
