@@ -596,14 +596,19 @@ int vb_kv8_attn(const VbKv8AttnArgs *args, vb_stream_t stream);
  * same pool pages in the table of each of them as far as it holds that many keys).
  * segments int32 [groups + batch][4], device: {first, sequences, 0, rows} per group,
  * then {b, 1, rows of its group or 0, 2^31 - 1} per sequence; group_of int32 [batch],
- * device: the group or -1. workspace: vb_kv8_attn_shared_workspace_size bytes, whose
- * first VB_KV8_ATTN_WORKSPACE_HEAD are left as they are. */
+ * device: the group or -1. least: the bytes of K and V that are not read again by the
+ * sequences of a group, together, from which on the groups are attended as such, below
+ * it every sequence by itself (-1: where that was measured to be faster). workspace:
+ * vb_kv8_attn_shared_workspace_size bytes, its head as in vb_kv8_attn. */
 typedef struct VbKv8SharedArgs {
   VbKv8AttnArgs attn;
   const int32_t *segments, *group_of, *host_groups;
+  int64_t least;
   int32_t groups;
 } VbKv8SharedArgs;
 size_t vb_kv8_attn_shared_workspace_size(const VbKv8SharedArgs *args);
+/* 1: the groups are attended as such, 0: every sequence by itself (or bad arguments). */
+int vb_kv8_attn_shares(const VbKv8SharedArgs *args);
 int vb_kv8_attn_shared(const VbKv8SharedArgs *args, vb_stream_t stream);
 
 /* The attention weight that every cached row receives from some query rows,

@@ -17,7 +17,7 @@ def share(c, groups):
     for first, count, rows in groups:
         n = rows // c.page
         c.page_table[first:first + count, :n] = c.page_table[first, :n].clone()
-    return SharedPrefix(c, groups)
+    return SharedPrefix(c, groups, least=0)  # however little it saves
 
 
 def check(c, q, groups, lens, q_lens=None, causal=True, len_add=0, scale=None, plan=None, ref=None, **kw):
@@ -129,6 +129,24 @@ def test_like_attention_of_each(cuda):
     assert (la - lb).abs().max() <= 1e-3 * la.abs().max()
 
 
+def test_little_is_not_shared(cuda):
+    """Groups that save little: the attention of every sequence by itself, bit for bit."""
+    rng = np.random.default_rng(13)
+    c = make_cache(rng, 6, 2, 128, 32, 30)
+    lens = ints([960, 700, 643, 800, 642, 900])
+    share(c, [(0, 6, 640)])
+    saved = 5 * 640 * 2 * 128 * 2
+    for L, least in ((2, None), (9, None), (2, saved + 1)):
+        q = bf16(rng, (6, 16, L, 128)).cuda()
+        plan = SharedPrefix(c, [(0, 6, 640)], least)
+        a, la = c.attend(q, lens, return_lse=True)
+        b, lb = c.attend_shared(q, lens, plan, return_lse=True)
+        assert torch.equal(a, b) and torch.equal(la, lb)
+        assert c.shared_workspace_size(plan, 16, L) == c.attend_workspace_size(16, L)
+    q = bf16(rng, (6, 16, 2, 128)).cuda()
+    check(c, q, None, lens.tolist(), plan=SharedPrefix(c, [(0, 6, 640)], saved))
+
+
 def test_pages_that_are_not_there(cuda):
     rng = np.random.default_rng(8)
     for count in (3, 12):
@@ -207,12 +225,14 @@ def test_python_refusals(cuda):
                 [(0, 2, 144)], [(0, 2, 16), (1, 2, 16)], [(2, 2, 16), (0, 2, 16)]):
         with pytest.raises(ValueError):
             SharedPrefix(c, bad)
-    plan = SharedPrefix(c, [(0, 4, 64)])
+    with pytest.raises(ValueError):
+        SharedPrefix(c, [(0, 2, 16)], least=-1)
+    plan = SharedPrefix(c, [(0, 4, 64)], 0)
     q, lens = bf16(rng, (4, 4, 1, 64)).cuda(), ints([70] * 4)
     for bad in (dict(q=q.float()), dict(q=q[:2]), dict(lens=lens[:2]), dict(scale=0.0),
                 dict(shared=SharedPrefix(make_cache(rng, 3, 2, 64, 16, 8), [(0, 2, 16)])),
                 dict(shared=SharedPrefix(make_cache(rng, 4, 2, 64, 32, 8), [(0, 2, 32)])),
-                dict(shared=SharedPrefix(make_cache(rng, 4, 2, 64, 16, 9), [(0, 2, 144)])),
+                dict(shared=SharedPrefix(make_cache(rng, 4, 2, 64, 16, 9), [(0, 2, 144)], 0)),
                 dict(workspace=torch.zeros(64, dtype=torch.uint8, device="cuda"))):
         with pytest.raises((ValueError, RuntimeError)):
             c.attend_shared(**{**dict(q=q, lens=lens, shared=plan), **bad})

@@ -43,7 +43,7 @@ def test_refusals(bad):
 
 
 def test_workspace_and_no_rows():
-    a = _args()
+    a = _args(least=0)
     need = lib.vb_kv8_attn_shared_workspace_size(C.byref(a))
     assert need > _lib.VB_KV8_ATTN_WORKSPACE_HEAD
     a.attn.workspace_bytes = need - 1

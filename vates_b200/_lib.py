@@ -72,7 +72,7 @@ class VbKv8AttnArgs(C.Structure):
 
 class VbKv8SharedArgs(C.Structure):
     _fields_ = [("attn", VbKv8AttnArgs), ("segments", C.c_void_p), ("group_of", C.c_void_p),
-                ("host_groups", C.c_void_p), ("groups", C.c_int32)]
+                ("host_groups", C.c_void_p), ("least", C.c_int64), ("groups", C.c_int32)]
 
 
 class VbKv8WeighArgs(C.Structure):
@@ -222,6 +222,7 @@ _SIGNATURES = {
     "vb_kv8_attn_workspace_size": (_SZ, [C.POINTER(VbKv8AttnArgs)]),
     "vb_kv8_attn": (_I32, [C.POINTER(VbKv8AttnArgs), _P]),
     "vb_kv8_attn_shared_workspace_size": (_SZ, [C.POINTER(VbKv8SharedArgs)]),
+    "vb_kv8_attn_shares": (_I32, [C.POINTER(VbKv8SharedArgs)]),
     "vb_kv8_attn_shared": (_I32, [C.POINTER(VbKv8SharedArgs), _P]),
     "vb_kv8_weigh_workspace_size": (_SZ, [C.POINTER(VbKv8WeighArgs)]),
     "vb_kv8_weigh": (_I32, [C.POINTER(VbKv8WeighArgs), _P]),

@@ -204,8 +204,11 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
   __shared__ unsigned long long s_sum[KA_THREADS / 32], s_begin;
   __shared__ int s_b, s_move[2], s_share[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  pdl_launch_dependents();
-  pdl_wait();
+  // `beside`: the kernel ahead lets this one start when its own inputs are there, which
+  // are this one's too; it is waited for at the end, for the kernel that joins both.
+  if (!SEG) pdl_launch_dependents();
+  if (!SEG || !p.beside) pdl_wait();
+  if (SEG) pdl_launch_dependents();
   const int H = p.c.kv_heads, B = SEG ? p.n_segs : p.c.batch;
   int rows = p.L * p.rep;
 
@@ -227,7 +230,10 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
   const Kv8Deal deal(kv8_all_tiles<KT, SEG>(p, blockIdx.x == 0, s_sum) * H, gridDim.x);
   unsigned long long w0 = deal.begin(blockIdx.x);
   const unsigned long long w1 = deal.begin(blockIdx.x + 1);
-  if (w0 == w1) return;
+  if (w0 == w1) {
+    if (SEG && p.beside) pdl_wait();
+    return;
+  }
   int b = 0;
   unsigned long long b_begin = 0;  // tiles of the sequences before b, all heads
   if (B > 1) {
@@ -743,6 +749,7 @@ __global__ void __launch_bounds__(KA_THREADS, Kv8Tile<D, NR>::CTAS) kv8_attn_ker
     }
     if (w0 < w1) __syncthreads();  // s_l has been read
   }
+  if (SEG && p.beside) pdl_wait();
 }
 
 // ------------------------------------------------------------------- combine
@@ -973,7 +980,8 @@ int kv8_launch(const Kv8AttnParams &p, int ctas, cudaStream_t s) {
   // Dependent launch for short calls only: started before the kernel ahead has
   // left its SMs, a full grid is placed unevenly (131,072 keys: 49.6 us instead of
   // 37.7; 901 keys: 12.1 us instead of 14.1).
-  vb_launch(kv8_attn_kernel<D, NR, SEG>, dim3(ctas), dim3(KA_THREADS), T::SMEM, s, ctas <= 148, p);
+  vb_launch(kv8_attn_kernel<D, NR, SEG>, dim3(ctas), dim3(KA_THREADS), T::SMEM, s,
+            ctas <= 148 || (SEG && p.beside), p);
   return check_launch("kv8_attn_kernel");
 }
 
@@ -1049,7 +1057,7 @@ struct Kv8SharedParams {
 // PG threads join four dims of one row, each every PG-th result, four at a time.
 template <int D, int PG>
 __global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __grid_constant__ Kv8SharedParams w) {
-  constexpr int LR = D / 4, RPC = KC_THREADS / (LR * PG), AHEAD = 4;
+  constexpr int LR = D / 4, RPC = KC_THREADS / (LR * PG), AHEAD = PG > 2 ? 8 : 4;
   __shared__ float4 s_a[PG > 1 ? KC_THREADS : 1];
   __shared__ float2 s_ml[PG > 1 ? KC_THREADS : 1];
   pdl_launch_dependents();
@@ -1164,6 +1172,22 @@ Kv8Side kv8_side(const VbKv8AttnArgs *a, long long segs, long long rows, long lo
   return s;
 }
 
+// Sequences that read the same pages read them from the L2 after the first, so what
+// sharing saves is L2 traffic and products; it costs a second kernel beside the first
+// and one that joins. It is worth it from 80 MB on (16 sequences x 2 rows, 64/8 heads of 64,
+// 326 MB: 36 us and 64 apart; 35 x 1, 3/2 of 256, 798 MB: 43 and 115; 28 MB: 18 us apart
+// and 23; 67 MB: 23 and 24), or 27 MB with more than 32 rows per kv head, which go
+// through the prefill kernel (30 MB: 31 and 67; 18 MB: 38 and 27).
+bool kv8_worth_sharing(const VbKv8SharedArgs *s) {
+  const VbKv8AttnArgs *a = &s->attn;
+  long long saved = 0;
+  for (int g = 0; g < s->groups; ++g)
+    saved += (long long)(s->host_groups[3 * g + 1] - 1) * s->host_groups[3 * g + 2];
+  saved *= 2ll * a->cache.kv_heads * a->cache.dim;
+  const bool many = (long long)a->L * (a->q_heads / a->cache.kv_heads) > 32;
+  return saved >= (s->least >= 0 ? s->least : many ? 27000000 : 80000000);
+}
+
 // Where both sides go through kv8_attn_kernel and there are no more key tiles than
 // CTAs, one launch does both.
 struct Kv8SharedPlan {
@@ -1242,6 +1266,7 @@ int kv8_shared_run(Kv8AttnParams p, const Kv8SharedPlan &pl, const VbKv8SharedAr
     if (rc != VB_OK) return rc;
     p.segs += a->groups;
     p.n_segs = p.c.batch;
+    p.beside = !pl.own.tensor;
     rc = kv8_side_run<D>(p, pl.own, ws + pl.own_at, w.own, s);
     if (rc != VB_OK) return rc;
   }
@@ -1250,7 +1275,10 @@ int kv8_shared_run(Kv8AttnParams p, const Kv8SharedPlan &pl, const VbKv8SharedAr
   // few rows: two threads for each four dims (4,096 rows of 10 results 22 us, by one thread
   // 14; 1,536 rows of 3 6 and 8)
   constexpr int RPC = KC_THREADS * 4 / D;
-  if (rows <= 2048)
+  if (rows <= 1024)
+    vb_launch(kv8_shared_join_kernel<D, 1024 / D>, dim3((unsigned)rows), dim3(KC_THREADS), 0, s,
+              true, w);
+  else if (rows <= 2048)
     vb_launch(kv8_shared_join_kernel<D, 2>, dim3((unsigned)((rows * 2 + RPC - 1) / RPC)),
               dim3(KC_THREADS), 0, s, true, w);
   else
@@ -1358,9 +1386,13 @@ int vb_kv8_attn(const VbKv8AttnArgs *a, vb_stream_t stream) {
   }
 }
 
+int vb_kv8_attn_shares(const VbKv8SharedArgs *a) {
+  return kv8_shared_check(a) == VB_OK && kv8_worth_sharing(a);
+}
+
 size_t vb_kv8_attn_shared_workspace_size(const VbKv8SharedArgs *a) {
   if (kv8_shared_check(a) != VB_OK || a->attn.L == 0) return 0;
-  return kv8_shared_plan(a).bytes;
+  return kv8_worth_sharing(a) ? kv8_shared_plan(a).bytes : kv8_plan(&a->attn).bytes;
 }
 
 int vb_kv8_attn_shared(const VbKv8SharedArgs *s, vb_stream_t stream) {
@@ -1373,6 +1405,7 @@ int vb_kv8_attn_shared(const VbKv8SharedArgs *s, vb_stream_t stream) {
   VB_REQUIRE(((uintptr_t)a->out % 16) == 0 && ((uintptr_t)s->segments % 16) == 0,
              "vb_kv8_attn_shared: out and segments must be 16-byte aligned");
   VB_REQUIRE(a->scale > 0.f && a->scale < 1e30f, "vb_kv8_attn_shared: scale %g", (double)a->scale);
+  if (!kv8_worth_sharing(s)) return vb_kv8_attn(a, stream);
   const Kv8SharedPlan pl = kv8_shared_plan(s);
   for (const Kv8Side *x : {&pl.pre, &pl.own})
     VB_REQUIRE((x->results / x->tile_rows) <= 1u << 29, "vb_kv8_attn_shared: too many rows");

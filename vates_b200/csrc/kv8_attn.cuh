@@ -33,6 +33,7 @@ struct Kv8AttnParams {
   // kv8_attn_kernel has whole, in o_res and ml_res.
   const int4 *segs;
   int n_segs;
+  bool beside;       // runs beside the kernel ahead of it, of which it needs nothing
   float *o_res;
   float2 *ml_res;
   // Query row R (< 2^24) of the flattened (row, head of the group) order is

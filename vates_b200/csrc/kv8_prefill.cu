@@ -186,8 +186,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   __shared__ int s_abort;
   __shared__ float s_fac[128], s_m[128], s_l[2][128], s_lv[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
-  pdl_launch_dependents();
+  if (!SEG) pdl_launch_dependents();
   pdl_wait();
+  if (SEG) pdl_launch_dependents();  // (it may need what this one waited for)
 
   // ---- the pair's rows and keys, this CTA's rows r_base .. + 127
   const int rank = blockIdx.x & 1;

@@ -75,9 +75,14 @@ class SharedPrefix:
     them, as far as it holds that many keys; in order, each sequence in one group at
     most. For :meth:`PagedKV8Cache.attend_shared` of ``cache`` and of every other one
     with its batch, page size and device, as those of the other layers. A CUDA graph
-    keeps the groups it was captured with."""
+    keeps to the groups it was captured with, and needs this object for as long as it is
+    replayed.
 
-    def __init__(self, cache: "PagedKV8Cache", groups):
+    Sharing costs two more kernels, so a call whose groups save fewer than ``least``
+    bytes of K and V (:attr:`groups`' rows, for all but one of their sequences) attends
+    every sequence by itself; without ``least``, where that was measured to be faster."""
+
+    def __init__(self, cache: "PagedKV8Cache", groups, least: int | None = None):
         self.batch, self.page, self.device = cache.batch, cache.page, cache.device
         self.groups = tuple((int(f), int(n), int(rows)) for f, n, rows in groups)
         end, most = 0, cache.page_table.shape[1] * self.page
@@ -99,7 +104,13 @@ class SharedPrefix:
         self._group_of = torch.tensor(group_of, dtype=torch.int32, device=self.device)
         self._host = (C.c_int32 * (3 * len(kept)))(*[x for g in kept for x in g])
         self._count = len(kept)
-        self._need: dict = {}  # workspace bytes by (cache layout, q_heads, L)
+        self._longest = max([rows // self.page for _, _, rows in kept], default=0)
+        if least is not None and least < 0:
+            raise ValueError(f"least={least}: a number of bytes")
+        self._least = -1 if least is None else least
+        # workspace bytes, and whether groups are attended as such, by (cache layout, q_heads, L)
+        self._need: dict = {}
+        self._shares: dict = {}
 
 
 class PagedKV8Cache:
@@ -260,15 +271,14 @@ class PagedKV8Cache:
                       return_lse: bool = False, status=None, stream=None, workspace=None):
         """What :meth:`attend` gives for a batch whose sequences share the rows they
         begin with in groups (:class:`SharedPrefix`): those are read, and multiplied,
-        once for the query rows of all sequences of a group. ``lens`` and positions
-        count the shared rows, as in every other call. ``workspace``: as in
-        :meth:`attend`, of :meth:`shared_workspace_size` bytes."""
+        once for the query rows of all sequences of a group, where that saves enough.
+        ``lens`` and positions count the shared rows, as in every other call.
+        ``workspace``: as in :meth:`attend`, of :meth:`shared_workspace_size` bytes."""
         if stream is not None or current_device() != self._index:
             with on_device(self.device, stream):
                 return self.attend_shared(q, lens, shared, q_lens, len_add, scale, causal, out,
                                           return_lse, status, workspace=workspace)
-        if not shared._count:
-            self._shared_fits(shared)
+        if q.dim() == 4 and not self._shares(shared, q.shape[1], q.shape[2]):
             return self.attend(q, lens, q_lens, len_add, scale, causal, out, return_lse, status,
                                workspace=workspace)
         s, dev = self._shared_fill(shared), self._index
@@ -282,23 +292,36 @@ class PagedKV8Cache:
     def shared_workspace_size(self, shared: SharedPrefix, q_heads: int, L: int) -> int:
         """Bytes of scratch that :meth:`attend_shared` needs for ``L`` rows of
         ``q_heads`` heads with the present page table."""
-        if not shared._count:
+        if not self._shares(shared, q_heads, L):
             return self.attend_workspace_size(q_heads, L)
         s = self._shared_fill(shared)
         s.attn.q_heads, s.attn.L = q_heads, L
         return self._shared_need(shared, s)
 
-    def _shared_fits(self, shared: SharedPrefix):
-        if shared.batch != self.batch or shared.page != self.page or shared.device != self.device:
+    def _shares(self, shared: SharedPrefix, q_heads: int, L: int) -> bool:
+        """Whether the groups of ``shared`` are attended as such."""
+        if shared.batch != self.batch or shared.page != self.page \
+                or shared.device != self.device or shared._longest > self._table.shape[1]:
             raise ValueError(f"shared: groups of {shared.batch} sequences in pages of {shared.page} "
-                             f"on {shared.device}, the cache has {self.batch} in pages of "
-                             f"{self.page} on {self.device}")
+                             f"on {shared.device}, up to {shared._longest}; the cache has "
+                             f"{self.batch} in pages of {self.page} on {self.device}, "
+                             f"{self._table.shape[1]} each")
+        key = (self.kv_heads, self.head_dim, self._table.shape[1], q_heads, L)
+        shares = shared._shares.get(key)
+        if shares is None:
+            shares = False
+            if shared._count:
+                s = self._shared_fill(shared)
+                s.attn.q_heads, s.attn.L = q_heads, L
+                shares = bool(lib.vb_kv8_attn_shares(C.byref(s)))
+            shared._shares[key] = shares
+        return shares
 
     def _shared_fill(self, shared: SharedPrefix) -> VbKv8SharedArgs:
-        self._shared_fits(shared)
         s = VbKv8SharedArgs.from_buffer_copy(self._shared_args)
         s.segments, s.group_of = shared._segments.data_ptr(), shared._group_of.data_ptr()
         s.host_groups, s.groups = C.addressof(shared._host), shared._count
+        s.least = shared._least
         return s
 
     def _shared_need(self, shared: SharedPrefix, s: VbKv8SharedArgs) -> int:
