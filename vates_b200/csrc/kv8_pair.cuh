@@ -84,6 +84,14 @@ __device__ __forceinline__ void kp_cluster_arrive() {
 __device__ __forceinline__ void kp_cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+template <int N>
+__device__ __forceinline__ void kp_regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void kp_regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 }  // namespace
 }  // namespace vb

@@ -159,15 +159,6 @@ __device__ __forceinline__ void kp_store32(float *p, const float *x) {  // one w
 __device__ __forceinline__ void kp_tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-template <int N>
-__device__ __forceinline__ void kp_regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void kp_regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 struct KpBarriers {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[3], p_full[3], o_done[3], q_full, o_last, drain;
 };

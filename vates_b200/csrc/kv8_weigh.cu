@@ -238,9 +238,12 @@ __global__ void __launch_bounds__(WG_THREADS) kv8_weigh_kernel(const __grid_cons
 }
 
 // ----------------------------------------------------------- many query rows
-constexpr int WR_THREADS = 640;            // issue, two warpgroups that convert, two that add
+constexpr int WR_THREADS = 896;            // a warpgroup issues, two convert, four add
 constexpr int WR_KEYS = 256;               // keys of a pair of CTAs
 constexpr int WR_COLS = 256;               // query rows at a time
+// Registers per thread of the warpgroups; 72 at launch.
+constexpr int WR_REGS = 72, WR_R_MMA = 32, WR_R_CONV = 88, WR_R_ADD = 72;
+static_assert(WR_R_MMA + 2 * WR_R_CONV + 4 * WR_R_ADD <= 7 * WR_REGS, "register shares");
 
 template <int D>
 struct WrShape {
@@ -274,8 +277,13 @@ __global__ void __launch_bounds__(256) kv8_weigh_q_kernel(const __grid_constant_
   if (c8 == 0) {
     const bool counts = fabsf(l) <= 3.4028235e38f;
     if (!counts && l != -INFINITY) flag_status(p.status, VB_STATUS_NONFINITE);
-    w.row[at] = make_float2(p.scale_log2 / pw, counts ? l * 1.4426950408889634f : INFINITY);
+    w.row[at] = make_float2(fmaxf(p.scale_log2 / pw, 1.1754944e-38f), counts ? l * 1.4426950408889634f : INFINITY);
   }
+}
+
+// Some of the threads that add meet.
+__device__ __forceinline__ void wr_meet(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 struct WrBarriers {
@@ -293,8 +301,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
   __shared__ __align__(8) WrBarriers bar;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  __shared__ float4 s_row[2][WR_COLS / 2];  // factors and log2 sums of two columns
-  __shared__ float s_sum[2][128];
+  __shared__ float4 s_row[2][WR_COLS / 2];  // of a chunk: factors and log2 sums of two columns
+  __shared__ float s_sum[2][2][128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
   pdl_launch_dependents();
   pdl_wait();
@@ -361,6 +369,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
 
   if (wg == 0) {
     // ================================================== tensor-core issuer
+    kp_regs_dec<WR_R_MMA>();
     ready();
     if (warp == 0 && rank == 0) {
       const uint32_t one = kp_elect();
@@ -392,19 +401,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
     __syncwarp();
   } else if (wg < 3) {
     // ================================================== converters
+    kp_regs_inc<WR_R_CONV>();
     const int ctid = tid - 128;
     constexpr int KC = D / 16, KSTEP = 256 / KC, KN = 128 / KSTEP;
     const int ch = ctid % KC, kkey = ctid / KC;
     const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
     const size_t pool_step = (size_t)H * p.c.page * D;
     const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + ch * 16;
-    // page of the 16-key group lane % 8 of this CTA's half of tile t; rows without one
-    // (past the last key, or flagged) read page 0: nothing is added to them
-    auto group_page = [&](int t) {
+    // table entry of the 16-key group lane % 8 of this CTA's half of a tile, asked for well
+    // before it is looked at; rows without a page (past the last key, or flagged) read
+    // page 0: nothing is added to them
+    auto entry_of = [&](int t) {
       const int key = t * WR_KEYS + rank * 128 + (lane & 7) * 16;
-      return key < keys ? max(0, kv8_page(table, p.c.max_pages, p.c.pages, key >> p.shift, p.status))
-                        : 0;
+      return key < keys ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : 0;
     };
+    auto page_of = [&](int entry) { return max(0, kv8_page_ok(entry, p.c.pages, p.status)); };
+    auto next = [&](int t) { return t + 1 == n_tiles ? 0 : t + 1; };
     uint4 kr[KN];
     auto load = [&](int id) {
 #pragma unroll
@@ -415,12 +427,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
                                                        (key & (p.c.page - 1)) * D));
       }
     };
-    load(group_page(t0));
-    int t = n_tiles > 1 ? 1 : 0;
-    int id = group_page(t0 + t);
+    const int first = entry_of(t0);
+    int t = next(0), entry = entry_of(t0 + t);
+    load(page_of(first));
     ready();
     for (int n = 0; n < steps; ++n) {
-      const int st = n & 1;
+      const int st = n & 1, entry_now = entry;
+      t = next(t);
+      entry = entry_of(t0 + t);
       if (n >= 2 && !wait(&bar.k_empty[st], (n >> 1) - 1)) break;
       uint8_t *tile = smem + S::K_OFF + st * S::TILE;
 #pragma unroll
@@ -428,82 +442,97 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) kp_arrive_leader(&bar.k_full[st]);
-      if (n + 1 < steps) load(id);
-      if (++t == n_tiles) t = 0;
-      id = group_page(t0 + t);
+      if (n + 1 < steps) load(page_of(entry_now));
     }
   } else {
     // ================================================== weights, a thread per key
-    const int e = wg - 3, atid = tid - 384, r = tid & 127;  // half of the columns; the CTA's key
+    // Two pairs of warpgroups take the tiles in turn, so that one's exponentials run while
+    // the other waits for its products (all four on each tile: 36 us instead of 34 for
+    // 256 rows of each of 2 kv heads over 131,072 keys of 64, 47 and 45 for keys of 256).
+    kp_regs_dec<WR_R_ADD>();
+    const int e = wg - 3, pair = e >> 1, half = e & 1, r = tid & 127;  // half of the columns; a key
     const float2 *row = w.row + (size_t)unit * w.padded;
     const uint16_t *q16 = w.q16 + (size_t)unit * w.padded * D;
-    // this CTA's half of a chunk's queries, and the factors of all of its columns
-    auto load_q = [&](int ch) {
-      const int half = columns(ch) / 2, first = ch * WR_COLS + rank * half;
-      for (int x = atid; x < half * (D / 8); x += 256) {
+    // This CTA's half of a chunk's queries, and the factors of all of its columns, by
+    // `threads` threads, this one the `at`-th.
+    auto load_q = [&](int ch, int at, int threads) {
+      const int rows = columns(ch) / 2, first = ch * WR_COLS + rank * rows;
+      for (int x = at; x < rows * (D / 8); x += threads) {
         const int qr = x / (D / 8), c8 = x % (D / 8);
         cp_async16(smem + (c8 >> 3) * KP_BLOCK + kp_sw(qr, c8 & 7),
                    q16 + (size_t)(first + qr) * D + c8 * 8);
       }
       cp_async_commit();
-      if (atid < 2 * half) {
-        const float2 f = row[ch * WR_COLS + atid];
-        float *d = reinterpret_cast<float *>(&s_row[ch & 1][atid >> 1]) + (atid & 1);
+      if (at < 2 * rows) {
+        const float2 f = row[ch * WR_COLS + at];
+        float *d = reinterpret_cast<float *>(&s_row[ch & 1][at >> 1]) + (at & 1);
         d[0] = f.x;
         d[2] = -f.y;
       }
     };
-    auto publish_q = [&]() {
+    auto publish_q = [&](int id, int threads, bool one) {
       cp_async_wait<0>();
       tc::fence_proxy_async_smem();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (atid == 0) kp_arrive_leader(&bar.q_full);
+      wr_meet(id, threads);
+      if (one) kp_arrive_leader(&bar.q_full);
     };
-    load_q(0);
-    // K scale of this thread's key (-1: no such page), a tile ahead
+    load_q(0, tid - 384, 512);
+    // K scale of this thread's key (-1: no such page), a tile ahead, and its table entry
+    // another one
     const int32_t *table = p.c.page_table + (size_t)b * p.c.max_pages;
-    auto scale_of = [&](int t) {
+    auto entry_of = [&](int t) {
       const int key = t * WR_KEYS + rank * 128 + r;
-      const int id = key < keys ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : -1;
-      return (unsigned)id < (unsigned)p.c.pages ? __ldcg(p.c.k_scales + (size_t)id * H + h) : -1.f;
+      return key < keys ? kv8_page_load(table, p.c.max_pages, key >> p.shift) : -1;
     };
-    float ks_n = scale_of(t0);
+    auto scale_of = [&](int entry) {
+      return (unsigned)entry < (unsigned)p.c.pages
+                 ? __ldcg(p.c.k_scales + (size_t)entry * H + h) : -1.f;
+    };
+    auto ahead = [&](int t, int by) { return (t + by) % n_tiles; };
+    int t = ahead(0, pair), t_next = ahead(t, 2);
+    const int entry_0 = entry_of(t0 + t);
+    int entry_n = entry_of(t0 + t_next);
+    float ks_n = scale_of(entry_0);
     ready();
-    publish_q();
+    publish_q(1, 512, tid == 384);
     const uint32_t trow = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
     // keys that every query row sees
     const int seen_by_all = s.sp.causal ? max(0, s.sp.off + 1) : keys;
     bool ok = true;
-    for (int n = 0, ch = 0, t = 0; n < steps; ++n) {
-      const int st = n & 1, cols = columns(ch);
+    for (int n = pair, ch = 0; n < steps; n += 2) {  // tile t of chunk ch, in S slot n % 2
+      // From chunk to chunk the pairs meet: a key's sum goes on where the other may have left
+      // it. (Both come here for every chunk, whichever of its tiles they have.)
+      for (; ch < n / n_tiles; ++ch) wr_meet(8, 512);
+      const int cols = columns(ch), use = n >> 1;
       const float ks = ks_n;
-      const bool last = t == n_tiles - 1, more = last && ch + 1 < chunks;
-      if (n + 1 < steps) ks_n = scale_of(last ? t0 : t0 + t + 1);
+      const bool more = t == n_tiles - 1 && ch + 1 < chunks;
+      ks_n = scale_of(entry_n);
       const int key = (t0 + t) * WR_KEYS + rank * 128 + r;
-      float old = 0.f;
-      if (e == 0 && key < keys) old = w.weights[at0 + key];
-      ok = ok && wait(&bar.s_full[st], n >> 1);
-      tc::tc_fence_after();
-      if (more && ok) load_q(ch + 1);  // no product of this chunk is left
-      float sum = 0.f;
-      const float4 *tab = s_row[ch & 1] + e * (cols / 4);
       const bool masked = (t0 + t) * WR_KEYS + rank * 128 + 128 > seen_by_all;
-      const f2 kk = f2_make(ks, ks);
+      t = t_next;
+      t_next = ahead(t, 2);
+      entry_n = entry_of(t0 + t_next);
+      float old = 0.f;
+      if (half == 0 && key < keys) old = w.weights[at0 + key];
+      ok = ok && wait(&bar.s_full[pair], use);
+      tc::tc_fence_after();
+      if (more && ok) load_q(ch + 1, tid - 384 - 256 * pair, 256);  // no product of this chunk is left
+      const int first = half * (cols / 2);
+      const float4 *tab = s_row[ch & 1] + first / 2;
+      // (at least 2^-100, where the score is 0 for any codes and a hidden one stays -inf)
+      const f2 kk = f2_make(fmaxf(ks, 7.9e-31f), fmaxf(ks, 7.9e-31f));
+      const int from = s.sp.causal ? max(0, key - s.sp.off) * p.rep : 0;
       f2 s0 = f2_make(0.f, 0.f), s1 = s0;
 #pragma unroll 1
       for (int c0 = 0; c0 < cols / 2; c0 += 32) {
         uint32_t v[32];
-        tc::tmem_ld32(trow + st * 256 + e * (cols / 2) + c0, v);
+        tc::tmem_ld32(trow + pair * 256 + first + c0, v);
         tc::tmem_ld_wait();
-        if (masked) {  // (rare) some query rows do not see this key
+        if (masked) {  // query rows from `from` on see this key
+          const int hidden = from - (ch * WR_COLS + first + c0);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float *x = reinterpret_cast<const float *>(tab + (c0 + j) / 2) + (j & 1);
-            const int R = ch * WR_COLS + e * (cols / 2) + c0 + j;
-            const float z = fmaf(__uint_as_float(v[j]) * ks, x[0], x[2]);
-            if (key < s.sp.visible(p.row_of(R))) sum += kv8_ex2(z);
-          }
-          continue;
+          for (int j = 0; j < 32; ++j)
+            if (j < hidden) v[j] = 0xFF800000u;
         }
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
@@ -519,22 +548,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
       }
       tc::tc_fence_before();
       __syncwarp();
-      if (ok && lane == 0) kp_arrive_leader(&bar.s_free[st]);
+      if (ok && lane == 0) kp_arrive_leader(&bar.s_free[pair]);
       float a0, a1, a2, a3;
       f2_split(s0, a0, a1);
       f2_split(s1, a2, a3);
-      sum += (a0 + a1) + (a2 + a3);
-      if (e == 1) s_sum[st][r] = sum;
-      if (more && ok) {
-        publish_q();
+      const float sum = (a0 + a1) + (a2 + a3);
+      // One warpgroup of the pair adds the sums of both. The other need not wait for it:
+      // before it is here with the second tile from now, the first has given back the slot of
+      // the next, and so read this one's sums.
+      const int id = 2 + 2 * pair + (use & 1);
+      if (half) {
+        s_sum[pair][use & 1][r] = sum;
+        asm volatile("bar.arrive %0, 256;" ::"r"(id) : "memory");
       } else {
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        wr_meet(id, 256);
+        if (ok && key < keys)
+          wg_add(w, s, b, at0, key, ks < 0.f ? 0.f : sum + s_sum[pair][use & 1][r], ch == 0, old);
       }
-      if (e == 0 && ok && key < keys)
-        wg_add(w, s, b, at0, key, ks < 0.f ? 0.f : sum + s_sum[st][r], ch == 0, old);
-      if (last) t = 0, ++ch;
-      else ++t;
+      if (more && ok) publish_q(6 + pair, 256, tid == 384 + 256 * pair);
+      if (n + 2 >= steps)
+        for (; ch < chunks - 1; ++ch) wr_meet(8, 512);
     }
+    if (pair >= steps)
+      for (int ch = 0; ch < chunks - 1; ++ch) wr_meet(8, 512);
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -610,7 +646,13 @@ int wg_run(Kv8WeighParams &w, const WeighPlan &pl, cudaStream_t s) {
     using S = WrShape<D>;
     static std::atomic<uint64_t> ready{0};
     const int rc = once_per_device(ready, [] {
-      const cudaError_t e = cudaFuncSetAttribute(
+      cudaFuncAttributes fa;
+      cudaError_t e = cudaFuncGetAttributes(&fa, kv8_weigh_rows_kernel<D>);
+      // the warpgroups' register shares are parts of what the block is launched with
+      if (e == cudaSuccess && fa.numRegs != WR_REGS)
+        return set_error(VB_ERR_CUDA, "kv8_weigh_rows_kernel: built with %d registers, %d needed",
+                         fa.numRegs, WR_REGS);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(
           kv8_weigh_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
       return e == cudaSuccess ? VB_OK
                               : set_error(VB_ERR_CUDA, "kv8_weigh_rows_kernel attributes: %s",
