@@ -8,6 +8,7 @@ import torch
 
 from test_gpu_kv8 import Plain, bf16, ints, make_cache
 from vates_b200 import _lib
+from vates_b200.kv8 import PagedKV8Cache, SharedPrefix
 
 pytestmark = pytest.mark.gpu
 F32 = np.float32
@@ -306,6 +307,32 @@ def test_evict_more_protected_than_kept(cuda):
     assert torch.equal(c.k_codes, before)
 
 
+def test_evict_many_heads(cuda):
+    """More (sequence, head) pairs than a grid has rows in its second dimension."""
+    rng = np.random.default_rng(14)
+    heads = 16384
+    c = PagedKV8Cache.empty(9, heads, 64, 5, 2, 16)
+    c.page_table.copy_(torch.arange(10, dtype=torch.int32).view(5, 2).clamp(max=8))
+    c.k_codes.random_(-127, 128)
+    c.v_codes.random_(-127, 128)
+    c.k_scales.fill_(0.5)
+    c.v_scales.fill_(0.25)
+    w = torch.rand((5, heads, 32), device="cuda")
+    lens = [20, 3, 31, 28, 16]
+    before, w0 = [t.clone() for t in (c.k_codes, c.v_codes)], w.clone()
+    assert c.evict(w, ints(lens), 12).tolist() == [min(n, 12) for n in lens]
+    for b, n in enumerate(lens[:4]):
+        kept = torch.argsort(-w0[b, :, :n], dim=-1, stable=True)[:, :min(n, 12)].sort(-1).values
+        assert torch.equal(w[b, :, :min(n, 12)].sort(-1).values,
+                           w0[b, :, :n].gather(-1, kept).sort(-1).values)
+        # equal scales: the kept rows themselves, in some order
+        for t, old in zip((c.k_codes, c.v_codes), before):
+            rows = [x[c.page_table[b].long()].permute(1, 0, 2, 3).reshape(heads, 32, 64).double().sum(-1)
+                    for x in (t, old)]
+            m = min(n, 12)
+            assert torch.equal(rows[0][:, :m].sort(-1).values, rows[1].gather(-1, kept).sort(-1).values)
+
+
 @pytest.mark.parametrize("rows,keep,units", [(5000, 4000, 1), (20000, 3000, 1), (70000, 5001, 2),
                                              (70000, 60000, 1), (300000, 70000, 1)])
 def test_evict_long(cuda, rows, keep, units):
@@ -402,6 +429,36 @@ def test_shared_pages_below_first_are_left(cuda):
     c.evict(torch.rand((3, 2, 320), device="cuda"), ints([320, 200, 260]), 128, first=64, recent=20)
     for t, o in zip((c.k_codes, c.v_codes, c.k_scales, c.v_scales), old):
         assert torch.equal(t[ids], o)
+
+
+def test_offsets_past_32_bits(cuda):
+    """Pages at the end of a pool of more than 4 GB, by every kernel."""
+    rng = np.random.default_rng(20)
+    heads, dim, page, pages = 8, 256, 128, 17000  # 4.5 GB of K
+    c = PagedKV8Cache.empty(pages, heads, dim, 2, 6, page)
+    c.page_table.copy_(torch.tensor([[16999, 3, 16998, 8300, 16990, 16991],
+                                     [16999, 3, 16000, 1, 16997, 16996]], dtype=torch.int32))
+    small = make_cache(rng, 2, heads, dim, page, 6)
+    small.page_table[1, :2] = small.page_table[0, :2]
+    for a, b in ((c.k_codes, small.k_codes), (c.v_codes, small.v_codes),
+                 (c.k_scales, small.k_scales), (c.v_scales, small.v_scales)):
+        a[c.page_table.long()] = b[small.page_table.long()]
+    lens = ints([768, 700])
+    for L, rep in ((1, 4), (40, 2)):
+        q = bf16(rng, (2, heads * rep, L, dim)).cuda()
+        plan = [SharedPrefix(x, [(0, 2, 256)], 0) for x in (c, small)]
+        (a, la), (b, lb) = (x.attend_shared(q, lens, p, return_lse=True)
+                            for x, p in zip((c, small), plan))
+        assert torch.equal(a, b) and torch.equal(la, lb)
+        w = [torch.zeros((2, heads, 768), device="cuda") for _ in range(2)]
+        c.weigh(q, la, lens, w[0])
+        small.weigh(q, lb, lens, w[1])
+        assert torch.equal(*w) and w[0].any()
+    after = [x.evict(y, lens, 400, first=256) for x, y in zip((c, small), w)]
+    assert torch.equal(*after) and torch.equal(*w)
+    for a, b in zip(c.read(after[0], 400), small.read(after[0], 400)):
+        assert torch.equal(a, b)
+    del c
 
 
 def test_python_refusals(cuda):

@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
   pdl_launch_dependents();
   pdl_wait();
   const int kv = threadIdx.x / EM_HALF, tid = threadIdx.x % EM_HALF, warp = tid >> 5;
-  const int lane = tid & 31, unit = blockIdx.y, b = unit / p.c.kv_heads, h = unit - b * p.c.kv_heads;
+  const int lane = tid & 31, unit = blockIdx.x, b = unit / p.c.kv_heads, h = unit - b * p.c.kv_heads;
   if (p.lens[b] <= p.keep) return;
   const int pages = (p.keep + p.c.page - 1) >> p.shift, edge = p.keep >> p.shift;
   const int32_t *holes = p.lists + unit * p.list_stride, *moving = holes + p.most,
@@ -363,15 +363,15 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
   auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory"); };
 
   // the CTA's pages, 32 at a time: their first hole and the number of holes
-  for (int pg0 = blockIdx.x; pg0 < pages; pg0 += 32 * gridDim.x) {
-    const int mine = pg0 + lane * gridDim.x;
+  for (int pg0 = blockIdx.y; pg0 < pages; pg0 += 32 * gridDim.y) {
+    const int mine = pg0 + lane * gridDim.y;
     int first_l = 0, count_l = 0;
     if (mine < pages) {
       first_l = firsts[mine];
       count_l = firsts[mine + 1] - first_l;
     }
     for (uint32_t todo = __ballot_sync(0xffffffffu, count_l > 0); todo; todo &= todo - 1) {
-      const int at = __ffs(todo) - 1, pg = pg0 + at * gridDim.x;
+      const int at = __ffs(todo) - 1, pg = pg0 + at * gridDim.y;
       const int j0 = __shfl_sync(0xffffffffu, first_l, at);
       const int count = __shfl_sync(0xffffffffu, count_l, at);
       const int id = kv8_page(table, p.c.max_pages, p.c.pages, pg, tid == 0 ? p.status : nullptr);
@@ -487,7 +487,7 @@ EvictPlan ev_plan(const VbKv8EvictArgs *a) {
   const long long per = align_up((pl.cap + pl.ctas - 1) / pl.ctas, pl.threads);
   pl.held = per <= EV_HELD * pl.threads;
   pl.cached = (int)(pl.held ? 0 : per < EV_KEYS ? per : EV_KEYS);
-  pl.stride = 2ll * pl.most + (a->keep + a->cache.page - 1) / a->cache.page + 3;
+  pl.stride = 2ll * pl.most + ((long long)a->keep + a->cache.page - 1) / a->cache.page + 3;
   pl.bytes = pl.most ? (size_t)(units * pl.stride) * sizeof(int32_t) : 0;
   return pl;
 }
@@ -526,9 +526,8 @@ int ev_check(const VbKv8EvictArgs *a) {
   if (rc != VB_OK) return rc;
   VB_REQUIRE(a->keep >= 1 && a->room >= 0 && a->room <= 0x7fffffff - 65536,
              "vb_kv8_evict: keep=%d room=%d", a->keep, a->room);
-  VB_REQUIRE((long long)a->cache.batch * a->cache.kv_heads <= 65535,
-             "vb_kv8_evict: %d sequences of %d kv heads (at most 65535 together)", a->cache.batch,
-             a->cache.kv_heads);
+  VB_REQUIRE((long long)a->cache.batch * a->cache.kv_heads <= 1 << 28,
+             "vb_kv8_evict: %d sequences of %d kv heads", a->cache.batch, a->cache.kv_heads);
   VB_REQUIRE(a->first >= 0 && a->recent >= 0 && (long long)a->first + a->recent <= a->keep,
              "vb_kv8_evict: first=%d recent=%d of keep=%d", a->first, a->recent, a->keep);
   return VB_OK;
@@ -574,7 +573,7 @@ int vb_kv8_evict(const VbKv8EvictArgs *a, vb_stream_t stream) {
   // CTAs of a (sequence, head): one a page, fewer once that fills the SMs several times
   const int pages = (a->keep + a->cache.page - 1) / a->cache.page;
   const long long few = (148 * 16 + units - 1) / units;
-  vb_launch(kv8_evict_move_kernel, dim3((unsigned)(pages < few ? pages : few), (unsigned)units),
+  vb_launch(kv8_evict_move_kernel, dim3((unsigned)units, (unsigned)(pages < few ? pages : few)),
             dim3(EM_THREADS), 0, s, true, p);
   return check_launch("kv8_evict_move_kernel");
 }
