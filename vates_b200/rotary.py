@@ -16,7 +16,8 @@ import torch
 from ._lib import VbRotateArgs, check, lib
 from .pool import current_device, current_stream, on_device
 
-# argument structures without pointers, and the host tables they refer to, by layout
+# Argument structures without pointers, and the host tables they refer to, by layout: the
+# types, shapes and strides of a call's tensors and its other arguments, checked once.
 _LAYOUTS: dict = {}
 
 
@@ -33,44 +34,43 @@ def pair_axes(sections, interleaved: bool = False) -> tuple:
                  for a, n in enumerate(sections) if i < n)
 
 
-def _layout(q, k, q_out, k_out, axes, base, eps, count):
-    """The arguments of a call but its tensors' addresses (made once per layout)."""
-    key = (q.shape, k.shape, q.stride(), k.stride(), q_out.stride(), k_out.stride(), axes, base,
-           eps, count)
-    got = _LAYOUTS.get(key)
-    if got is None:
-        n = len(axes)
-        if not 1.0 < base < math.inf:
-            raise ValueError(f"base={base}: a finite number above 1 is needed")
-        if n > 128 or n % 8 or n == 0 or any(not 0 <= a < count for a in axes):
-            raise ValueError(f"axes: one axis per pair (of {count} in positions), a multiple of 8 "
-                             f"pairs and at most 128, got {n} pairs of the axes {sorted(set(axes))}")
-        axis = (C.c_uint8 * n)(*axes)
-        turns = (C.c_double * n)(*[base ** (-i / n) / (2.0 * math.pi) for i in range(n)])
-        B, Hq, L, D = q.shape
-        strides = [(C.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, q_out, k_out)]
-        a = VbRotateArgs(None, None, None, None, None, None, *strides, None,
-                         C.cast(turns, C.c_void_p), C.cast(axis, C.c_void_p), eps, B, L, Hq,
-                         k.shape[1], D, 2 * n, count)
-        if len(_LAYOUTS) > 4096:
-            _LAYOUTS.clear()
-        got = _LAYOUTS[key] = (bytes(a), axis, turns)
+def _check(t: torch.Tensor, what: str, shape):
+    if t.dtype != torch.bfloat16 or t.shape != shape or t.stride()[-1:] not in ((1,), ()):
+        raise ValueError(f"{what}: bfloat16 {tuple(shape)} with contiguous dims is needed, got "
+                         f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _layout(key, q, k, positions, axes, base, eps, q_norm, k_norm, q_out, k_out):
+    """The arguments of a call but its tensors' addresses."""
+    B, Hq, L, D = q.shape
+    _check(q, "q", q.shape)
+    _check(k, "k", (B, k.shape[1], L, D))
+    for t, shape, what in ((q_norm, (D,), "q_norm"), (k_norm, (D,), "k_norm"),
+                           (q_out, q.shape, "q_out"), (k_out, k.shape, "k_out")):
+        if t is not None:
+            _check(t, what, shape)
+    if positions.dtype != torch.int32 or positions.dim() != 3 or positions.shape[1:] != (B, L) \
+            or not positions.is_contiguous():
+        raise ValueError(f"positions: contiguous int32 [axes, {B}, {L}] is needed, got "
+                         f"{positions.dtype} {tuple(positions.shape)}")
+    if not 1.0 < base < math.inf:
+        raise ValueError(f"base={base}: a finite number above 1 is needed")
+    n, count = len(axes), positions.shape[0]
+    if n > 128 or n % 8 or n == 0 or any(not 0 <= a < count for a in axes):
+        raise ValueError(f"axes: one axis per pair (of {count} in positions), a multiple of 8 "
+                         f"pairs and at most 128, got {n} pairs of the axes {sorted(set(axes))}")
+    axis = (C.c_uint8 * n)(*axes)
+    turns = (C.c_double * n)(*[base ** (-i / n) / (2.0 * math.pi) for i in range(n)])
+    dense = lambda h: (h * L * D, L * D, D)
+    strides = [(C.c_int64 * 3)(*x[:3]) for x in
+               (q.stride(), k.stride(), dense(Hq) if q_out is None else q_out.stride(),
+                dense(k.shape[1]) if k_out is None else k_out.stride())]
+    a = VbRotateArgs(None, None, None, None, None, None, *strides, None, C.cast(turns, C.c_void_p),
+                     C.cast(axis, C.c_void_p), eps, B, L, Hq, k.shape[1], D, 2 * n, count)
+    if len(_LAYOUTS) > 4096:
+        _LAYOUTS.clear()
+    _LAYOUTS[key] = got = (bytes(a), axis, turns)
     return got
-
-
-def _check(t: torch.Tensor, what: str, shape, dev: int):
-    if t.dtype != torch.bfloat16 or t.get_device() != dev or t.shape != shape:
-        raise ValueError(f"{what}: bfloat16 {tuple(shape)} on cuda:{dev} is needed, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
-
-
-def _out(t: torch.Tensor, out: torch.Tensor | None, what: str, dev: int) -> torch.Tensor:
-    if out is None:
-        return t.new_empty(t.shape)
-    _check(out, what, t.shape, dev)
-    if out.stride(3) != 1:
-        raise ValueError(f"{what}: contiguous dims are needed, strides {out.stride()}")
-    return out
 
 
 def rotate_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes,
@@ -96,24 +96,26 @@ def rotate_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes,
     if q.dim() != 4 or k.dim() != 4 or dev < 0:
         raise ValueError("q, k: CUDA [batch, heads, L, dim] are needed, got "
                          f"{tuple(q.shape)} and {tuple(k.shape)} on {q.device}")
-    B, _, L, D = q.shape
-    _check(q, "q", q.shape, dev)
-    _check(k, "k", (B, k.shape[1], L, D), dev)
-    if positions.dtype != torch.int32 or positions.get_device() != dev \
-            or positions.dim() != 3 or positions.shape[1:] != (B, L) \
-            or not positions.is_contiguous():
-        raise ValueError(f"positions: contiguous int32 [axes, {B}, {L}] on cuda:{dev} is needed, "
-                         f"got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
-    for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None:
-            _check(w, what, (D,), dev)
-            if not w.is_contiguous():
-                raise ValueError(f"{what}: a contiguous tensor is needed")
-    q_out, k_out = _out(q, q_out, "q_out", dev), _out(k, k_out, "k_out", dev)
-    q = q if q.stride(3) == 1 else q.contiguous()
-    k = k if k.stride(3) == 1 else k.contiguous()
-    layout = _layout(q, k, q_out, k_out, axes if type(axes) is tuple else
-                     tuple(int(a) for a in axes), base, eps, positions.shape[0])
+    others = [t for t in (k, positions, q_norm, k_norm, q_out, k_out) if t is not None]
+    for t in others:
+        if t.get_device() != dev:
+            raise ValueError(f"a tensor on {t.device}, q on cuda:{dev}")
+    if q.stride(3) != 1 and q.numel():
+        q = q.contiguous()
+    if k.stride(3) != 1 and k.numel():
+        k = k.contiguous()
+    if type(axes) is not tuple:
+        axes = tuple(int(a) for a in axes)
+    key = (q.dtype, q.shape, q.stride(), axes, base, eps,
+           *[x for t in others for x in (t.dtype, t.shape, t.stride())],
+           q_norm is None, k_norm is None, q_out is None, k_out is None)
+    layout = _LAYOUTS.get(key)
+    if layout is None:
+        layout = _layout(key, q, k, positions, axes, base, eps, q_norm, k_norm, q_out, k_out)
+    if q_out is None:
+        q_out = q.new_empty(q.shape)
+    if k_out is None:
+        k_out = k.new_empty(k.shape)
     a = VbRotateArgs.from_buffer_copy(layout[0])
     a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
     a.positions = positions.data_ptr()
