@@ -243,11 +243,16 @@ extern "C" int vb_rotate_axes(const VbRotateArgs *a, vb_stream_t stream) {
     }
   }
   p.keep = same;
-  // Tokens of a CTA (a power of two): as many as it has rows at a time, fewer while that
-  // leaves SMs without work.
+  // Tokens of a CTA (a power of two): as many as it has rows at a time, fewer as long as
+  // there are fewer than 16 CTAs an SM, the last of which would keep few SMs busy (2 x 8,191
+  // tokens of 32/8 heads of 128: 32, 16, 8, 4 and 2 tokens 80, 72, 66, 63 and 69 us), and
+  // every thread still has all its rows in flight (4,096 tokens of 16/2 heads of 256: 8 tokens
+  // 23 us, one 42); fewer than that where SMs would have none.
   const int lpr = a->dim > 128 ? 16 : a->dim > 64 ? 8 : 4;
+  const int turn = RT_THREADS / lpr * (p.norm[0] || p.norm[1] ? 3 : 2);
   p.per = lpr == 16 ? 4 : lpr == 8 ? 5 : 6;
-  while (p.per > 0 && (p.tokens >> p.per) < 296) --p.per;
+  while (p.per > 0 && (p.tokens >> p.per) < 148 * 16 && (int64_t)heads << p.per >= 2 * turn) --p.per;
+  while (p.per > 0 && (p.tokens >> p.per) < 148 * 2) --p.per;
   p.groups = (a->L + (1 << p.per) - 1) >> p.per;
   const int64_t ctas = (int64_t)p.groups * a->batch;
   VB_REQUIRE(ctas <= 0x7fffffffll, "vb_rotate_axes: too many tokens");
