@@ -98,10 +98,12 @@ class SharedPrefix:
         for g, (first, count, rows) in enumerate(kept):
             group_of[first:first + count] = [g] * count
             start[first:first + count] = [rows] * count
-        segments = [(f, n, 0, rows) for f, n, rows in kept]
-        segments += [(b, 1, s, 0x7fffffff) for b, s in enumerate(start)]
-        self._segments = torch.tensor(segments, dtype=torch.int32, device=self.device)
-        self._group_of = torch.tensor(group_of, dtype=torch.int32, device=self.device)
+        words = [x for f, n, rows in kept for x in (f, n, 0, rows)]
+        words += [x for b, s in enumerate(start) for x in (b, 1, s, 0x7fffffff)]
+        # segments, then the groups of sequences
+        self._words = torch.tensor(words + group_of, dtype=torch.int32).to(self.device)
+        self._segments = self._words.data_ptr()
+        self._group_of = self._segments + 4 * len(words)
         self._host = (C.c_int32 * (3 * len(kept)))(*[x for g in kept for x in g])
         self._count = len(kept)
         self._longest = max([rows // self.page for _, _, rows in kept], default=0)
@@ -319,7 +321,7 @@ class PagedKV8Cache:
 
     def _shared_fill(self, shared: SharedPrefix) -> VbKv8SharedArgs:
         s = VbKv8SharedArgs.from_buffer_copy(self._shared_args)
-        s.segments, s.group_of = shared._segments.data_ptr(), shared._group_of.data_ptr()
+        s.segments, s.group_of = shared._segments, shared._group_of
         s.host_groups, s.groups = C.addressof(shared._host), shared._count
         s.least = shared._least
         return s
