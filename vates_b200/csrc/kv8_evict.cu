@@ -17,9 +17,9 @@
 // bins that it has rows in to those of all others (reading all bins of all others
 // instead took 5 us of 20 for 65,536 rows). Ballots count and number holes and
 // moving rows, in order.
-// kv8_evict_move_kernel: a CTA fills the holes of one page after another, half of it
-// K's and half V's, and moves weights and positions with K. Nothing is written that
-// another CTA still reads: rows move from `keep` on to below it, and the scale of the
+// kv8_evict_move_kernel: groups of 32 to 128 threads fill the holes of one page of K or
+// V after another, and move weights and positions with K. Nothing is written that
+// another group still reads: rows move from `keep` on to below it, and the scale of the
 // page in which `keep` falls is taken down by the first kernel.
 #include "kv8.cuh"
 
@@ -339,16 +339,18 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const __gr
 }
 
 constexpr int EM_THREADS = 256;
-constexpr int EM_HALF = 128;  // threads of K, and of V: one for each row of the largest page
 constexpr int EM_AHEAD = 4;   // pieces of 16 codes that a thread has in flight
 
+// G: threads for a page of K or of V, no fewer than it has rows.
+template <int G>
 __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __grid_constant__ Kv8EvictParams p) {
-  __shared__ int s_src[2][EM_HALF], s_sid[2][EM_HALF], s_row[2][EM_HALF];
-  __shared__ float s_from[2][EM_HALF], s_top[2][4];
-  __shared__ uint32_t s_filled[2][4][4];
+  constexpr int GROUPS = EM_THREADS / G, SLOTS = GROUPS / 2, WARPS = G / 32;
+  __shared__ int s_src[GROUPS][G], s_sid[GROUPS][G], s_row[GROUPS][G];
+  __shared__ float s_from[GROUPS][G], s_top[GROUPS][WARPS];
+  __shared__ uint32_t s_filled[GROUPS][4][WARPS];
   pdl_launch_dependents();
   pdl_wait();
-  const int kv = threadIdx.x / EM_HALF, tid = threadIdx.x % EM_HALF, warp = tid >> 5;
+  const int gi = threadIdx.x / G, kv = gi & 1, tid = threadIdx.x % G, warp = tid >> 5;
   const int lane = tid & 31, unit = blockIdx.x, b = unit / p.c.kv_heads, h = unit - b * p.c.kv_heads;
   if (p.lens[b] <= p.keep) return;
   const int pages = (p.keep + p.c.page - 1) >> p.shift, edge = p.keep >> p.shift;
@@ -360,18 +362,19 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
   const size_t page_bytes = (size_t)p.c.page * D;
   int8_t *codes = kv ? p.c.v_codes : p.c.k_codes;
   float *scales = kv ? p.c.v_scales : p.c.k_scales;
-  auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory"); };
+  auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + gi), "n"(G) : "memory"); };
 
-  // the CTA's pages, 32 at a time: their first hole and the number of holes
-  for (int pg0 = blockIdx.y; pg0 < pages; pg0 += 32 * gridDim.y) {
-    const int mine = pg0 + lane * gridDim.y;
+  // the group's pages, 32 at a time: their first hole and the number of holes
+  const int stride = gridDim.y * SLOTS;
+  for (int pg0 = blockIdx.y * SLOTS + (gi >> 1); pg0 < pages; pg0 += 32 * stride) {
+    const int mine = pg0 + lane * stride;
     int first_l = 0, count_l = 0;
     if (mine < pages) {
       first_l = firsts[mine];
       count_l = firsts[mine + 1] - first_l;
     }
     for (uint32_t todo = __ballot_sync(0xffffffffu, count_l > 0); todo; todo &= todo - 1) {
-      const int at = __ffs(todo) - 1, pg = pg0 + at * gridDim.y;
+      const int at = __ffs(todo) - 1, pg = pg0 + at * stride;
       const int j0 = __shfl_sync(0xffffffffu, first_l, at);
       const int count = __shfl_sync(0xffffffffu, count_l, at);
       const int id = kv8_page(table, p.c.max_pages, p.c.pages, pg, tid == 0 ? p.status : nullptr);
@@ -388,10 +391,10 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
         sid = kv8_page(table, p.c.max_pages, p.c.pages, src >> p.shift, p.status);
         if (sid >= 0)
           from = (src >> p.shift) == edge ? edge_scale : scales[(size_t)sid * p.c.kv_heads + h];
-        s_src[kv][tid] = src & (p.c.page - 1);
-        s_sid[kv][tid] = sid;
-        s_row[kv][tid] = row & (p.c.page - 1);
-        s_from[kv][tid] = from;
+        s_src[gi][tid] = src & (p.c.page - 1);
+        s_sid[gi][tid] = sid;
+        s_row[gi][tid] = row & (p.c.page - 1);
+        s_from[gi][tid] = from;
         if (kv == 0) {
           const size_t w = (size_t)unit * p.room;
           p.weights[w + row] = p.weights[w + src];
@@ -405,32 +408,32 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const uint32_t f = __reduce_or_sync(0xffffffffu, src >= 0 && r >> 5 == w ? 1u << (r & 31) : 0u);
-        if (lane == 0) s_filled[kv][w][warp] = f;
+        if (lane == 0) s_filled[gi][w][warp] = f;
       }
-      if (lane == 0) s_top[kv][warp] = top;
+      if (lane == 0) s_top[gi][warp] = top;
       meet();
       top = stay ? old : 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, s_top[kv][w]);
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_top[gi][w]);
 
       // ---- rows that move, and rows that stay but take a larger scale
       uint4 *dst = reinterpret_cast<uint4 *>(codes + ((size_t)id * p.c.kv_heads + h) * page_bytes);
-      for (int x0 = tid; x0 < count << lsh; x0 += EM_HALF * EM_AHEAD) {
+      for (int x0 = tid; x0 < count << lsh; x0 += G * EM_AHEAD) {
         uint4 v[EM_AHEAD];
 #pragma unroll
         for (int k = 0; k < EM_AHEAD; ++k) {
-          const int x = x0 + k * EM_HALF, o = x >> lsh;
-          if (o < count && s_sid[kv][o] >= 0)
+          const int x = x0 + k * G, o = x >> lsh;
+          if (o < count && s_sid[gi][o] >= 0)
             v[k] = reinterpret_cast<const uint4 *>(
-                codes + ((size_t)s_sid[kv][o] * p.c.kv_heads + h) * page_bytes)[
-                (s_src[kv][o] << lsh) + (x & (lpr - 1))];
+                codes + ((size_t)s_sid[gi][o] * p.c.kv_heads + h) * page_bytes)[
+                (s_src[gi][o] << lsh) + (x & (lpr - 1))];
         }
 #pragma unroll
         for (int k = 0; k < EM_AHEAD; ++k) {
-          const int x = x0 + k * EM_HALF, o = x >> lsh;
-          if (o < count && s_sid[kv][o] >= 0) {
-            const float ratio = top > 0.f ? __fdiv_rn(s_from[kv][o], top) : 1.f;
-            dst[(s_row[kv][o] << lsh) + (x & (lpr - 1))] = ratio == 1.f ? v[k] : kv8_recode(v[k], ratio);
+          const int x = x0 + k * G, o = x >> lsh;
+          if (o < count && s_sid[gi][o] >= 0) {
+            const float ratio = top > 0.f ? __fdiv_rn(s_from[gi][o], top) : 1.f;
+            dst[(s_row[gi][o] << lsh) + (x & (lpr - 1))] = ratio == 1.f ? v[k] : kv8_recode(v[k], ratio);
           }
         }
       }
@@ -438,21 +441,24 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
         const float ratio = __fdiv_rn(old, top);
         uint32_t filled[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-          filled[w] = s_filled[kv][w][0] | s_filled[kv][w][1] | s_filled[kv][w][2] | s_filled[kv][w][3];
+        for (int w = 0; w < 4; ++w) {
+          filled[w] = 0;
+#pragma unroll
+          for (int x = 0; x < WARPS; ++x) filled[w] |= s_filled[gi][w][x];
+        }
         auto stays = [&](int x) {
           const int y = x >> lsh;
           const uint32_t f = y < 64 ? (y < 32 ? filled[0] : filled[1]) : (y < 96 ? filled[2] : filled[3]);
           return y < live && !((f >> (y & 31)) & 1);
         };
-        for (int x0 = tid; x0 < live << lsh; x0 += EM_HALF * EM_AHEAD) {
+        for (int x0 = tid; x0 < live << lsh; x0 += G * EM_AHEAD) {
           uint4 v[EM_AHEAD];
 #pragma unroll
           for (int k = 0; k < EM_AHEAD; ++k)
-            if (stays(x0 + k * EM_HALF)) v[k] = dst[x0 + k * EM_HALF];
+            if (stays(x0 + k * G)) v[k] = dst[x0 + k * G];
 #pragma unroll
           for (int k = 0; k < EM_AHEAD; ++k)
-            if (stays(x0 + k * EM_HALF)) dst[x0 + k * EM_HALF] = kv8_recode(v[k], ratio);
+            if (stays(x0 + k * G)) dst[x0 + k * G] = kv8_recode(v[k], ratio);
         }
       }
       if (tid == 0 && top != old) scales[(size_t)id * p.c.kv_heads + h] = top;
@@ -570,11 +576,18 @@ int vb_kv8_evict(const VbKv8EvictArgs *a, vb_stream_t stream) {
                                      : (pl.held ? ev_select<512, true>(p, pl, units, s)
                                                 : ev_select<512, false>(p, pl, units, s));
   if (rc2 != VB_OK || pl.most == 0) return rc2;
-  // CTAs of a (sequence, head): one a page, fewer once that fills the SMs several times
+  // Threads for a page: up to eight pieces of 16 codes each, and no fewer than rows.
   const int pages = (a->keep + a->cache.page - 1) / a->cache.page;
+  const int pieces = a->cache.page * a->cache.dim / 16, page = a->cache.page;
+  const int group = page <= 32 && pieces <= 256 ? 32 : page <= 64 && pieces <= 512 ? 64 : 128;
+  // CTAs of a (sequence, head): enough for all pages, fewer once that fills the SMs several
+  // times
+  const int per = EM_THREADS / (2 * group), want = (pages + per - 1) / per;
   const long long few = (148 * 16 + units - 1) / units;
-  vb_launch(kv8_evict_move_kernel, dim3((unsigned)units, (unsigned)(pages < few ? pages : few)),
-            dim3(EM_THREADS), 0, s, true, p);
+  const dim3 grid((unsigned)units, (unsigned)(want < few ? want : few)), block(EM_THREADS);
+  if (group == 32) vb_launch(kv8_evict_move_kernel<32>, grid, block, 0, s, true, p);
+  else if (group == 64) vb_launch(kv8_evict_move_kernel<64>, grid, block, 0, s, true, p);
+  else vb_launch(kv8_evict_move_kernel<128>, grid, block, 0, s, true, p);
   return check_launch("kv8_evict_move_kernel");
 }
 
