@@ -20,6 +20,14 @@
 // 256 keys at a time, 128 each, as the M rows of the product and 64 to 256 query
 // rows as its N columns, so a thread has a key in its TMEM lane and adds its
 // weights by itself. Queries are made ready once by a kernel ahead of it.
+//
+// What bounds it: 32 sequences of up to 8,190 keys, 32/8 heads of 128, take 30 us for 128
+// MB (4.3 TB/s, a copy 19.6): issue slots are half used (five instructions turn four codes
+// into f16) and warps wait for their keys; one sequence of 901 keys costs the launch, 3.5.
+// 64 rows of 16/2 heads of 256 over 32,768 keys take 29 us (products alone 10.4): two
+// chunks of 256 rows over three or four tiles a pair, 1.8 us each, 4 for the queries and 8
+// to begin and end; over 131,072 keys a tile of 256 x 256 takes 2.4 us, of which the
+// exponentials fill their pipe for 1.1.
 #include "kv8_pair.cuh"
 
 namespace vb {

