@@ -285,7 +285,9 @@ __global__ void __launch_bounds__(256) kv8_weigh_q_kernel(const __grid_constant_
   if (c8 == 0) {
     const bool counts = fabsf(l) <= 3.4028235e38f;
     if (!counts && l != -INFINITY) flag_status(p.status, VB_STATUS_NONFINITE);
-    w.row[at] = make_float2(fmaxf(p.scale_log2 / pw, 1.1754944e-38f), counts ? l * 1.4426950408889634f : INFINITY);
+    // (a factor above 0: times -inf, what a row does not see)
+    w.row[at] = make_float2(fmaxf(p.scale_log2 / pw, 1.1754944e-38f),
+                            counts ? l * 1.4426950408889634f : INFINITY);
   }
 }
 
@@ -506,6 +508,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
     const uint32_t trow = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
     // keys that every query row sees
     const int seen_by_all = s.sp.causal ? max(0, s.sp.off + 1) : keys;
+    // After a wait has given up, the tiles are gone through without further ones, as the
+    // warpgroups meet in every tile.
     bool ok = true;
     for (int n = pair, ch = 0; n < steps; n += 2) {  // tile t of chunk ch, in S slot n % 2
       // From chunk to chunk the pairs meet: a key's sum goes on where the other may have left
@@ -563,17 +567,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
       const float sum = (a0 + a1) + (a2 + a3);
       // One warpgroup of the pair adds the sums of both. The other need not wait for it:
       // before it is here with the second tile from now, the first has given back the slot of
-      // the next, and so read this one's sums.
+      // the next, and so read this one's sums. (Not so after a wait has given up: a second
+      // arrival could then complete the barrier without the first, which would wait for good.)
       const int id = 2 + 2 * pair + (use & 1);
       if (half) {
         s_sum[pair][use & 1][r] = sum;
-        asm volatile("bar.arrive %0, 256;" ::"r"(id) : "memory");
+        if (ok) asm volatile("bar.arrive %0, 256;" ::"r"(id) : "memory");
+        else wr_meet(id, 256);
       } else {
         wr_meet(id, 256);
         if (ok && key < keys)
           wg_add(w, s, b, at0, key, ks < 0.f ? 0.f : sum + s_sum[pair][use & 1][r], ch == 0, old);
       }
-      if (more && ok) publish_q(6 + pair, 256, tid == 384 + 256 * pair);
+      if (more) publish_q(6 + pair, 256, ok && tid == 384 + 256 * pair);
       if (n + 2 >= steps)
         for (; ch < chunks - 1; ++ch) wr_meet(8, 512);
     }
