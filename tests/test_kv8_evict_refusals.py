@@ -61,3 +61,13 @@ def test_evict_workspace():
 def test_no_rows_are_accepted():
     a = _lib.VbKv8WeighArgs(cache=_cache(), lens=FAKE, scale=1.0, q_heads=4, L=0, room=0)
     assert lib.vb_kv8_weigh(C.byref(a), None) == 0
+
+
+def test_weigh_tiles_are_counted_in_31_bits():
+    d = dict(q=FAKE, lse=FAKE, lens=FAKE, weights=FAKE, scale=1.0, room=1 << 29, workspace=FAKE,
+             workspace_bytes=1)
+    for L, rc in ((256 * 1022, 3), (256 * 1023, 1), (256 * 65536, 1)):
+        a = _lib.VbKv8WeighArgs(cache=_cache(max_pages=1 << 25, kv_heads=1), q_heads=1, L=L, **d)
+        a.cache.page = 16
+        assert lib.vb_kv8_weigh(C.byref(a), None) == rc
+        assert (lib.vb_kv8_weigh_workspace_size(C.byref(a)) > 0) == (rc == 3)

@@ -708,6 +708,11 @@ int wg_check(const VbKv8WeighArgs *a) {
              "vb_kv8_weigh: %d sequences of %d kv heads, %d rows of %d heads each", a->cache.batch,
              a->cache.kv_heads, a->L, a->q_heads);
   VB_REQUIRE(a->room >= 0 && a->room <= 0x7fffffff - 65536, "vb_kv8_weigh: room=%d", a->room);
+  // (a CTA counts its tiles of 256 rows by 256 keys in 31 bits)
+  const long long cap = (long long)a->cache.max_pages * a->cache.page;
+  const long long rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
+  VB_REQUIRE((rows / 256 + 1) * ((cap < a->room ? cap : a->room) / 256 + 1) <= 0x7fffffff,
+             "vb_kv8_weigh: %lld query rows of a kv head over %d keys", rows, a->room);
   return VB_OK;
 }
 
