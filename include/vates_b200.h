@@ -653,7 +653,9 @@ int vb_kv8_weigh(const VbKv8WeighArgs *args, vb_stream_t stream);
  * rows come from, and codes become rint(code * old / new). lens_out[b] =
  * min(n, keep), not the same memory as lens. first + recent <= keep. Pages that rows
  * leave or enter must belong to one sequence only (those below `first` are not
- * touched where they end on a page). workspace: vb_kv8_evict_workspace_size bytes. */
+ * touched where they end on a page). A length beyond the table or room counts as that
+ * many rows, and rows to or from a page that is not there do not move (both
+ * VB_STATUS_BOUNDS). workspace: vb_kv8_evict_workspace_size bytes. */
 typedef struct VbKv8EvictArgs {
   VbKv8Cache cache;
   float *weights;     /* [batch, kv_heads, room] */

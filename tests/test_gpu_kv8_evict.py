@@ -73,7 +73,12 @@ def check_weigh(c, q, lens, q_lens=None, new=None, causal=True, len_add=0, extra
         n, m = lens[b], min(lens[b], ql[b] if new is None else new[b])
         want[b, :, n - m:n] = 0
         want[b, :, :n] += sums[b]
-        tol[b, :, :n] = tols[b] + want[b, :, :n] * 2.0 ** -23
+        # What a weight grows by comes in passes over 256 query rows (one for few rows). Each
+        # is added to the float32 weight, which only grows: off by half a step, 2^-24, of
+        # `want` at most. With 5 passes and terms that are small beside the weight, that is
+        # 5 2^-24 of it, not the 2^-23 that one or two take.
+        passes = max(2, -(-ql[b] * (Hq // H) // 256))
+        tol[b, :, :n] = tols[b] + want[b, :, :n] * passes * 2.0 ** -24
         if positions:
             pos[b, :, n - m:n] = seen[b] - m + np.arange(m)
     got = w.cpu().numpy()
@@ -107,7 +112,8 @@ def test_weigh_edges(cuda, keys):
 
 @pytest.mark.parametrize("dim,page,L,rep,keys", [(64, 16, 33, 3, 700), (128, 64, 70, 5, 515),
                                                  (256, 64, 64, 8, 1500), (256, 128, 5, 16, 2100),
-                                                 (64, 32, 300, 4, 300), (128, 32, 257, 1, 4000)])
+                                                 (64, 32, 300, 4, 300), (128, 32, 257, 1, 4000),
+                                                 (64, 64, 600, 2, 20000), (256, 32, 96, 8, 900)])
 def test_weigh_windows(cuda, dim, page, L, rep, keys):
     """More query rows than one pass over them takes; windows at a prompt's end."""
     rng = np.random.default_rng(dim + L)
@@ -343,6 +349,15 @@ def test_evict_long(cuda, rows, keep, units):
     check_evict(c, rng, [rows], keep, first=64, recent=keep // 3, weights=w)
 
 
+def test_evict_long_and_many(cuda):
+    """One CTA for each of more heads than there are SMs, over more keys than it holds."""
+    rng = np.random.default_rng(19)
+    c = make_cache(rng, 10, 16, 64, 128, 72)
+    w = rng.exponential(1.0, (10, 16, 72 * 128)).astype(F32)
+    lens = [9216, 9001, 8193, 8192, 700, 129, 128, 1, 0, 9215]
+    check_evict(c, rng, lens, 128, first=4, recent=30, weights=w)
+
+
 def test_evict_scales(cuda):
     """Scales of zero, pages whose rows all leave, and equal scales, which leave the
     codes as they are."""
@@ -418,6 +433,49 @@ def test_evict_streams_and_graphs(cuda):
     side.synchronize()
     assert got.tolist() == evict_plain(ref, want, None, [401, 777], 100, 0, 0)
     assert np.array_equal(c.v_codes.cpu().numpy(), ref.codes[1])
+
+
+def test_graphs_on_two_streams_at_once(cuda):
+    """Captured windows and evictions have scratch of their own: replayed beside one
+    another and beside eager calls."""
+    rng = np.random.default_rng(17)
+    caches = [make_cache(rng, 2, 2, 64, 16, 60) for _ in range(3)]
+    qs = [bf16(rng, (2, 8, 40, 64)).cuda() for _ in range(3)]
+    lens = ints([960, 700])
+    lses = [c.attend(q, lens, return_lse=True)[1] for c, q in zip(caches, qs)]
+    ws = [torch.zeros((2, 2, 960), device="cuda") for _ in range(3)]
+    want = []
+    for c, q, lse in zip(caches, qs, lses):
+        w = torch.zeros((2, 2, 960), device="cuda")
+        c.weigh(q, lse, lens, w)
+        want.append(w.clone())
+    graphs = []
+    for c, q, lse, w in zip(caches[:2], qs, lses, ws):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            w.zero_()
+            c.weigh(q, lse, lens, w)
+            keep = w.clone()
+            after = c.evict(w, lens, 300, recent=20)
+        graphs.append((g, keep, after))
+    refs = [(Plain(c), w.cpu().numpy().copy()) for c, w in zip(caches, want)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for (g, _, _), st in zip(graphs, streams):
+        with torch.cuda.stream(st):
+            g.replay()
+    caches[2].weigh(qs[2], lses[2], lens, ws[2])
+    done = caches[2].evict(ws[2], lens, 300, recent=20)
+    torch.cuda.synchronize()
+    for i, (c, (ref, w)) in enumerate(zip(caches, refs)):
+        if i < 2:
+            assert torch.equal(graphs[i][1], want[i])
+        got = graphs[i][2] if i < 2 else done
+        assert got.tolist() == evict_plain(ref, w, None, [960, 700], 300, 0, 20)
+        assert np.array_equal(ws[i].cpu().numpy(), w)
+        assert np.array_equal(c.k_codes.cpu().numpy(), ref.codes[0])
+        assert np.array_equal(c.v_codes.cpu().numpy(), ref.codes[1])
+    del g, graphs
 
 
 def test_shared_pages_below_first_are_left(cuda):

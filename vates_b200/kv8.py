@@ -456,7 +456,9 @@ class PagedKV8Cache:
         eviction comes before the step's own rows are appended. A page that receives
         rows takes the largest scale of the pages that its rows come from, and codes of
         a smaller one are rounded again (half a step of the new scale at most). Pages of
-        more than one sequence must lie below ``first``."""
+        more than one sequence must lie below ``first``. Lengths beyond the page table or
+        ``weights`` count as that many rows, and rows to or from a page that is not there
+        do not move (VB_STATUS_BOUNDS in ``status``)."""
         if stream is not None or current_device() != self._index:
             with on_device(self.device, stream):
                 return self.evict(weights, lens, keep, first, recent, positions, status)
