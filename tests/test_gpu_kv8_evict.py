@@ -535,7 +535,8 @@ def test_python_refusals(cuda):
             c.weigh(**{**ok, **bad})
     ok = dict(weights=w, lens=lens, keep=8)
     for bad in (dict(keep=0), dict(keep=-1), dict(first=9), dict(first=-1), dict(recent=-1),
-                dict(first=4, recent=5), dict(weights=w[:, :1]), dict(lens=lens[:1]),
+                dict(first=4, recent=5), dict(keep=(1 << 32) + 8), dict(first=1 << 32),
+                dict(recent=-1 << 32), dict(weights=w[:, :1]), dict(lens=lens[:1]),
                 dict(lens=lens.cpu()), dict(positions=p[:1]), dict(positions=p.float())):
         with pytest.raises((ValueError, RuntimeError)):
             c.evict(**{**ok, **bad})

@@ -469,6 +469,9 @@ class PagedKV8Cache:
         if positions is not None:
             a.positions = self._tracked(positions, "positions", torch.int32, room)
         a.lens = _ints(lens, "lens", self.batch, dev)
+        if not (0 < keep < 1 << 31 and 0 <= first and 0 <= recent and first + recent <= keep):
+            raise ValueError(f"keep={keep} (1 to 2^31 - 1), first={first}, recent={recent}: neither "
+                             "is negative, together they are at most keep")
         a.keep, a.first, a.recent = keep, first, recent
         if status is not None:
             a.status = status_ptr(status, dev)
