@@ -568,7 +568,7 @@ int vb_kv8_read(const VbKv8ReadArgs *args, vb_stream_t stream);
  * lse -inf. q bf16 [batch, q_heads, L, dim] with element strides {batch, head,
  * row}; out bf16 [batch, q_heads, L, dim] and lse float32 [batch, q_heads, L]
  * contiguous; query head hq reads kv head hq / (q_heads / kv_heads).
- * workspace: vb_kv8_attn_workspace_size bytes, of which the first
+ * workspace (32-byte aligned): vb_kv8_attn_workspace_size bytes, of which the first
  * VB_KV8_ATTN_WORKSPACE_HEAD have to be zero at the first call and are zero
  * after every call (of one stream at a time). */
 #define VB_KV8_ATTN_WORKSPACE_HEAD 65536

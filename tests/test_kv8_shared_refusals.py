@@ -52,3 +52,15 @@ def test_workspace_and_no_rows():
     assert lib.vb_kv8_attn_shared(C.byref(a), None) == 3
     a.attn.L = 0
     assert lib.vb_kv8_attn_shared(C.byref(a), None) == 0
+
+
+def test_workspace_of_the_prefill_kernel():
+    """It stores 32 bytes at a time."""
+    for off in (16, 48):
+        a = _args(attn=dict(q_heads=80, workspace=FAKE + off), least=0)
+        assert lib.vb_kv8_attn_shared(C.byref(a), None) == 1
+        assert b"alignment" in lib.vb_last_error()
+        a = _args(attn=dict(q_heads=80, workspace=FAKE + off), cache=dict(max_pages=4096)).attn
+        assert lib.vb_kv8_attn_workspace_size(C.byref(a)) > 0
+        assert lib.vb_kv8_attn(C.byref(a), None) == 1
+        assert b"alignment" in lib.vb_last_error()

@@ -1370,7 +1370,9 @@ int vb_kv8_attn(const VbKv8AttnArgs *a, vb_stream_t stream) {
   if (pl.bytes && (!a->workspace || a->workspace_bytes < pl.bytes))
     return set_error(VB_ERR_WORKSPACE, "vb_kv8_attn: workspace %zu < %zu bytes",
                      a->workspace_bytes, pl.bytes);
-  VB_REQUIRE(((uintptr_t)a->workspace % 16) == 0, "vb_kv8_attn: workspace alignment");
+  // (the prefill kernel stores whole sectors of 32 bytes)
+  VB_REQUIRE(((uintptr_t)a->workspace % (pl.tensor && pl.bytes ? 32 : 16)) == 0,
+             "vb_kv8_attn: workspace alignment");
   VB_REQUIRE((long long)a->cache.kv_heads * pl.row_tiles <= 65535 &&
                  (long long)a->cache.batch * a->q_heads * a->L <= 0x7fffffffll,
              "vb_kv8_attn: too many rows");
@@ -1418,7 +1420,8 @@ int vb_kv8_attn_shared(const VbKv8SharedArgs *s, vb_stream_t stream) {
   if (!a->workspace || a->workspace_bytes < pl.bytes)
     return set_error(VB_ERR_WORKSPACE, "vb_kv8_attn_shared: workspace %zu < %zu bytes",
                      a->workspace_bytes, pl.bytes);
-  VB_REQUIRE(((uintptr_t)a->workspace % 16) == 0, "vb_kv8_attn_shared: workspace alignment");
+  VB_REQUIRE(((uintptr_t)a->workspace % (pl.pre.tensor ? 32 : 16)) == 0,
+             "vb_kv8_attn_shared: workspace alignment");
   Kv8AttnParams p = kv8_params(a);
   uint8_t *ws = static_cast<uint8_t *>(a->workspace);
   cudaStream_t st = as_stream(stream);

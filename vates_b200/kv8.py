@@ -247,7 +247,7 @@ class PagedKV8Cache:
         nothing, and rows from ``q_lens[b]`` on, are zero (log-sum-exp -inf).
         Returns bf16 ``[batch, q_heads, L, head_dim]``, with ``return_lse``
         also float32 ``[batch, q_heads, L]`` (natural log). ``workspace``: the
-        caller's scratch (:meth:`attend_workspace_size` bytes, uint8, zeros
+        caller's scratch (:meth:`attend_workspace_size` bytes, uint8, 32-byte aligned, zeros
         before its first call) for calls that never overlap, in graphs or not;
         without it a call finds its own."""
         # with it as the current stream, results belong to it
