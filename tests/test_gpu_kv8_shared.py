@@ -113,6 +113,41 @@ def test_long_prefixes(cuda, B, L, rep, dim, page, rows, tail):
     check(c, q, [(0, B, rows)], lens, ql)
 
 
+@pytest.mark.parametrize("groups,count,L,rep", [(40, 20, 1, 4), (300, 2, 3, 12), (9, 40, 2, 20),
+                                                (1, 520, 1, 2), (2, 3, 130, 2)])
+def test_rows_that_are_not_there(cuda, groups, count, L, rep):
+    """Row tiles are filled by the rows of this pass: many groups, sequences without
+    rows, groups without any, groups whose rows begin anywhere in a tile."""
+    rng = np.random.default_rng(groups + count)
+    B = groups * count + 1
+    c = make_cache(rng, B, 1, 64, 16, 24)
+    q = bf16(rng, (B, rep, L, 64), 1.5).cuda()
+    ql = [int(n) for n in rng.integers(0, L + 1, B)]
+    for g in range(1, groups, 3):
+        ql[g * count:(g + 1) * count] = [0] * count
+    prefix = [16 * int(n) for n in rng.integers(1, 20, groups)]
+    lens = [prefix[min(b // count, groups - 1)] + n + int(rng.integers(0, 40)) for b, n in enumerate(ql)]
+    check(c, q, [(g * count, count, prefix[g]) for g in range(groups)], lens, ql)
+
+
+def test_bad_row_counts_are_flagged(cuda):
+    """Counts and lengths out of range are cut off, as in attention, and flagged."""
+    rng = np.random.default_rng(21)
+    c = make_cache(rng, 12, 1, 64, 16, 24)
+    q = bf16(rng, (12, 40, 1, 64)).cuda()
+    plan = share(c, [(0, 12, 160)])
+    lens, ql = [170 + b for b in range(12)], [1] * 12
+    for bad_lens, bad_ql in (({}, {3: 2}), ({}, {4: -1}), ({5: 385}, {}), ({6: -1}, {6: 0})):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        n = [bad_lens.get(b, x) for b, x in enumerate(lens)]
+        m = [bad_ql.get(b, x) for b, x in enumerate(ql)]
+        got = c.attend_shared(q, ints(n), plan, ints(m), status=status)
+        assert int(status) == _lib.VB_STATUS_BOUNDS
+        want = c.attend_shared(q, ints([min(max(x, 0), 384) for x in n]), plan,
+                               ints([min(max(x, 0), 1) for x in m]))
+        assert torch.equal(got, want)
+
+
 def test_like_attention_of_each(cuda):
     """Scores of hundreds, where one key has all the weight, are split between the two
     parts too: compared with the attention of every sequence by itself."""

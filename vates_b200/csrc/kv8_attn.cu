@@ -1018,9 +1018,10 @@ struct Kv8Parted {             // where the results of some segments are
   const float2 *ml, *ml_part;
   // kv8_attn_kernel: its units, from unit `first` on: one result of each row (o, ml), or
   // several (o_part, ml_part): slot 1 of the unit's first CTA and slot 0 of the following
-  // ones. The prefill kernel (null): `splits` of each row tile.
+  // ones. The prefill kernel (null): places[0] of each row tile.
   const int2 *units;
-  int first, tile_rows, row_tiles, splits;
+  const int32_t *places;
+  int first, tile_rows;
 };
 // One row's results in there.
 struct Kv8PartedRow {
@@ -1029,8 +1030,10 @@ struct Kv8PartedRow {
   int n, step, skip;           // rows from one result to the next; less once
   __device__ int at(int s) const { return s * step - (s > 0 ? skip : 0); }
 };
+// `unit`, R: segment and head, and the row in it; b, h, r: sequence, head, its row.
 template <int D>
-__device__ __forceinline__ Kv8PartedRow kv8_parted_row(const Kv8Parted &q, int unit, int R) {
+__device__ __forceinline__ Kv8PartedRow kv8_parted_row(const Kv8Parted &q, int H, int unit, int R,
+                                                       int b, int h, int r, bool live) {
   Kv8PartedRow x;
   size_t row;
   x.skip = 0;
@@ -1044,10 +1047,14 @@ __device__ __forceinline__ Kv8PartedRow kv8_parted_row(const Kv8Parted &q, int u
     x.o = (u.y > 1 ? q.o_part : q.o) + row * D;
     x.ml = (u.y > 1 ? q.ml_part : q.ml) + row;
   } else {
-    const int t = R / q.tile_rows;
-    x.n = q.splits;
+    x.n = 0;
     x.step = q.tile_rows;
-    row = ((size_t)unit * q.row_tiles + t) * q.splits * q.tile_rows + R - t * q.tile_rows;
+    row = 0;
+    if (live) {  // (the others have no place)
+      x.n = __ldcg(q.places);
+      const int at = __ldcg(q.places + 1 + b) + r, t = at / q.tile_rows;
+      row = ((size_t)t * H + h) * x.n * q.tile_rows + at - t * q.tile_rows;
+    }
     x.o = q.o + row * D;
     x.ml = q.ml + row;
   }
@@ -1071,12 +1078,13 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __gri
   const int tid = threadIdx.x, d4 = tid % LR, pg = tid / LR % PG, H = p.c.kv_heads;
   const int row = blockIdx.x * RPC + tid / (LR * PG), per = p.Hq * p.L;
   const bool there = row < p.c.batch * per;
-  int b = 0, h = 0, R = 0, g = -1, R_pre = 0;
+  int b = 0, h = 0, i = 0, R = 0, g = -1, R_pre = 0;
   float M = -INFINITY, ls = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   if (there) {  // (the groups are the plan's, nothing that a kernel ahead writes)
     b = row / per;
-    const int x = row - b * per, hq = x / p.L, i = x - hq * p.L;
+    const int x = row - b * per, hq = x / p.L;
+    i = x - hq * p.L;
     h = hq / p.rep;
     R = i * p.rep + hq - h * p.rep;
     g = w.group_of[b];
@@ -1084,9 +1092,10 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __gri
   }
   pdl_wait();
   if (there) {
-    Kv8PartedRow pre, own = kv8_parted_row<D>(w.own, b * H + h, R);
+    const bool live = i < kv8_rows(p.q_lens, b, p.L, nullptr);
+    Kv8PartedRow pre, own = kv8_parted_row<D>(w.own, H, b * H + h, R, b, h, R, live);
     pre.n = 0;
-    if (g >= 0) pre = kv8_parted_row<D>(w.pre, g * H + h, R_pre);
+    if (g >= 0) pre = kv8_parted_row<D>(w.pre, H, g * H + h, R_pre, b, h, R, live);
     const int n = pre.n + own.n;
     for (int s0 = pg; s0 < n; s0 += PG * AHEAD) {
       float2 ml[AHEAD];
@@ -1146,35 +1155,49 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __gri
 // One side of the work: the groups' segments, or each sequence's own, or both.
 struct Kv8Side {
   bool tensor;
-  int tile_rows, row_tiles, splits, ctas;
+  int tile_rows, ctas, splits, pairs, longest, seg_lanes;
+  bool deal;
   size_t units, results, parts;  // units; rows of results, of partial results
+  size_t places;                 // prefill kernel
+  size_t unit_bytes() const {  // (what the prefill kernel stores begins on a line)
+    return align_up(units * sizeof(int2) + places * sizeof(int32_t), 128);
+  }
   size_t bytes(int dim) const {
-    return align_up(units * sizeof(int2), 16) +
-           align_up((results + parts) * (dim + 2) * sizeof(float), 16);
+    return unit_bytes() +
+           align_up((results + parts) * (dim + 2) * sizeof(float), 32);
   }
 };
-// `base`: row tiles of all segments and heads, `longest`: key tiles of the longest
-// segment (prefill kernel), `all`: of all segments and heads (kv8_attn_kernel).
-Kv8Side kv8_side(const VbKv8AttnArgs *a, long long segs, long long rows, long long base,
-                 long long longest, long long all) {
-  Kv8Side s;
+// `rows`: most rows of a segment, `seqs`: sequences of all; `base`: row tiles of all segments
+// and heads, `longest`: key tiles of the longest segment (prefill kernel), `all`: of all
+// segments and heads (kv8_attn_kernel).
+Kv8Side kv8_side(const VbKv8AttnArgs *a, long long segs, long long seqs, long long rows,
+                 long long base, long long longest, long long all) {
+  Kv8Side s = {};
   const long long units = segs * a->cache.kv_heads;
   s.tensor = rows > 32;
   s.units = s.tensor ? 0 : (size_t)units;
   if (s.tensor) {
+    // Segments of several row tiles: the ranges that the kernel takes when all rows are
+    // there, and a wave at least, as fewer row tiles take more ranges. (With one each there
+    // is nothing to deal, which takes 2 us.)
     s.tile_rows = kv8_prefill_rows();
-    s.row_tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
     s.splits = kv8_ranges(base, longest);
-    s.ctas = 0;
-    s.parts = 0;
+    s.deal = rows > s.tile_rows;
+    const long long least = base * (longest < 1 ? 1 : longest), wave = least < 74 ? least : 74;
+    const long long all = base * s.splits;
+    s.pairs = (int)(s.deal && all < wave ? wave : all);
+    s.longest = (int)longest;
+    s.places = (size_t)a->cache.batch + 1;
+    s.seg_lanes = 1;
+    while (s.seg_lanes < 32 && s.seg_lanes * segs < seqs) s.seg_lanes *= 2;
+    s.results = (size_t)s.pairs * s.tile_rows;
   } else {
     s.tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-    s.row_tiles = s.splits = 1;
     const int full = 148 * (s.tile_rows == 32 ? Kv8Tile<64, 4>::CTAS : Kv8Tile<64, 1>::CTAS);
     s.ctas = (int)(all < 1 ? 1 : all < full ? all : full);
     s.parts = (size_t)s.ctas * 2 * s.tile_rows;
+    s.results = (size_t)units * s.tile_rows;
   }
-  s.results = (size_t)(units * s.row_tiles * s.splits) * s.tile_rows;
   return s;
 }
 
@@ -1206,7 +1229,7 @@ Kv8SharedPlan kv8_shared_plan(const VbKv8SharedArgs *s) {
   const long long H = a->cache.kv_heads, rows = (long long)a->L * (a->q_heads / a->cache.kv_heads);
   const long long cap = (long long)a->cache.max_pages * a->cache.page, kt = KA_TILE / a->cache.dim;
   const long long tile = kv8_prefill_rows(), B = a->cache.batch;
-  long long most = 0, base = 0, longest = 0, all = 0, own = cap * B;
+  long long most = 0, base = 0, longest = 0, all = 0, own = cap * B, seqs = 0;
   for (int g = 0; g < s->groups; ++g) {
     const int32_t *x = s->host_groups + 3 * g;
     const long long r = x[1] * rows;
@@ -1215,15 +1238,17 @@ Kv8SharedPlan kv8_shared_plan(const VbKv8SharedArgs *s) {
     base += (r + tile - 1) / tile * H;
     all += (x[2] + kt - 1) / kt * H;
     own -= (long long)x[1] * x[2];
+    seqs += x[1];
   }
   const long long own_all = (own + kt - 1) / kt * H + B * H;  // (a part of a tile each)
   Kv8SharedPlan pl;
   pl.both = most <= 32 && all + own_all <= 148 * 2;
   if (pl.both) {
-    pl.own = pl.pre = kv8_side(a, s->groups + B, most, 0, 0, all + own_all);
+    pl.own = pl.pre = kv8_side(a, s->groups + B, seqs + B, most, 0, 0, all + own_all);
   } else {
-    pl.pre = kv8_side(a, s->groups, most, base, (longest + 127) / 128, all);
-    pl.own = kv8_side(a, B, rows, B * H * ((rows + tile - 1) / tile), (own / B + 127) / 128, own_all);
+    pl.pre = kv8_side(a, s->groups, seqs, most, base, (longest + 127) / 128, all);
+    pl.own =
+        kv8_side(a, B, B, rows, B * H * ((rows + tile - 1) / tile), (own / B + 127) / 128, own_all);
   }
   // (the words ahead of it are left to vb_kv8_attn, whose scratch it may be)
   pl.pre_at = pl.own_at = KA_TICKETS * sizeof(uint32_t);
@@ -1235,13 +1260,15 @@ Kv8SharedPlan kv8_shared_plan(const VbKv8SharedArgs *s) {
 template <int D>
 int kv8_side_run(Kv8AttnParams p, const Kv8Side &s, uint8_t *ws, Kv8Parted &out, cudaStream_t st) {
   int2 *units = s.tensor ? nullptr : reinterpret_cast<int2 *>(ws);
-  float *o = reinterpret_cast<float *>(ws + align_up(s.units * sizeof(int2), 16));
+  float *o = reinterpret_cast<float *>(ws + s.unit_bytes());
   float *o_part = o + s.results * D;
   float2 *ml = reinterpret_cast<float2 *>(o_part + s.parts * D), *ml_part = ml + s.results;
   out.o = o; out.o_part = o_part; out.ml = ml; out.ml_part = ml_part; out.units = units;
-  out.first = 0; out.tile_rows = s.tile_rows; out.row_tiles = s.row_tiles; out.splits = s.splits;
-  p.row_tiles = s.row_tiles; p.splits = s.splits;
+  out.first = 0; out.tile_rows = s.tile_rows; out.places = nullptr;
   if (s.tensor) {
+    out.places = p.places = reinterpret_cast<int32_t *>(ws);
+    p.splits = s.splits; p.deal = s.deal;
+    p.pairs = s.pairs; p.longest = s.longest; p.seg_lanes = s.seg_lanes;
     p.o_part = o; p.ml_part = ml;
     return kv8_prefill_launch_segments(p, st);
   }

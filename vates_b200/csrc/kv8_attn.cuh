@@ -31,8 +31,15 @@ struct Kv8AttnParams {
   // common, at most as far as each row sees. Another kernel joins their results, rows of
   // unnormalised O and (m, l): partial results as above, and for a unit that one CTA of
   // kv8_attn_kernel has whole, in o_res and ml_res.
+  // The prefill kernel packs the rows that are there of a segment's sequences and leaves,
+  // for the kernel that joins, its key ranges per row tile and the first row of every
+  // sequence in places[0] and places[1 + sequence].
   const int4 *segs;
   int n_segs;
+  int32_t *places;
+  int pairs, longest;  // pairs of CTAs, key tiles of the longest segment
+  int seg_lanes;       // lanes that count the rows of a segment: a power of two
+  bool deal;           // segments of several row tiles: dealt by the rows that there are
   bool beside;       // runs beside the kernel ahead of it, of which it needs nothing
   float *o_res;
   float2 *ml_res;
@@ -70,10 +77,10 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnParams &p, int b, bool 
 __device__ __forceinline__ int kv8_reach(const int4 &s, int visible) {
   return max(0, min(visible, s.w) - s.z);
 }
-// Query row R of a segment's flattened (sequence, row, head of the group) order.
 struct Kv8SegRow {
   int b, i, hr, vis;  // sequence, query, head of the group; keys seen (0: no such row)
 };
+// Query row R of a segment's flattened (sequence, row, head of the group) order.
 __device__ __forceinline__ Kv8SegRow kv8_seg_row(const Kv8AttnParams &p, const int4 &s, int R) {
   const int per = p.L * p.rep, m = s.y == 1 ? R >= per : R / per, r = R - m * per;
   Kv8SegRow x;

@@ -163,8 +163,115 @@ struct KpBarriers {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[3], p_full[3], o_done[3], q_full, o_last, drain;
 };
 
-// SEG: segments in the place of sequences (kv8_attn.cuh), each with its own number of
-// row tiles, up to p.row_tiles.
+// Segments (kv8_attn.cuh): what a pair of CTAs is to do, from the rows that there are.
+// Lengths are on the device, so the tiles and key ranges are dealt here: 64 sequences
+// with 162 of 64 x 4 rows behind 32,768 keys, 16/2 heads of 256, fill 12 tiles instead of 16.
+struct KpDeal {
+  int4 seg;
+  int pair;            // tile, head and range as a number
+  int tile, in_seg;    // row tile, of all and within the segment
+  int h, split, splits;
+};
+// What is the same in all lanes, for the compiler to know: without it the roles' loops count
+// as divergent, and a key tile takes half as long again.
+__device__ __forceinline__ int kp_uniform(int x) {
+  return (int)__reduce_max_sync(0xffffffffu, (unsigned)x);
+}
+// Key ranges per row tile for `base` row tiles of up to `tiles` key tiles, by the rule
+// of kv8_ranges; the same in every lane.
+__device__ __forceinline__ int kp_ranges(int base, int tiles, int pairs) {
+  const int most = min(pairs, 8 * 74);
+  if (base > most) return 1;
+  // (at most 8 waves of 2^24 tiles; 32 x the time, up to 2^20 of it)
+  auto cost = [&](int s) {
+    return 32u * (unsigned)((base * s + 73) / 74) * (3 + min((tiles + s - 1) / s, 1 << 16)) +
+           (s > 1 ? 64 + base * s : 0);
+  };
+  unsigned best = ~0u;
+  int at = 1;
+  for (int s = (threadIdx.x & 31) + 1; s <= min(74, tiles) && base * s <= most; s += 32)
+    if (s > 1 && cost(s) < best) best = cost(s), at = s;
+  const unsigned least = __reduce_min_sync(0xffffffffu, best);
+  at = (int)__reduce_min_sync(0xffffffffu, best == least ? (unsigned)at : 74u);
+  return least < cost(1) / 10 * 9 ? at : 1;
+}
+// False if there is nothing for the pair; the same for all threads of both CTAs. s_seg,
+// s_tiles: KP_THREADS of them.
+__device__ __forceinline__ bool kp_deal(const Kv8AttnParams &p, int4 *s_seg, int *s_tiles, KpDeal &d) {
+  // Pairs without work come first, all at once: behind the others, on the few SMs that
+  // those leave, they would hold up the next kernel (230 us for the sequences above, 272).
+  const int tid = threadIdx.x, lane = tid & 31, pair = p.pairs - 1 - (blockIdx.x >> 1);
+  d.pair = pair;
+  const int lanes = p.seg_lanes, per = KP_THREADS / lanes;
+  // row tiles of the segments from c0 on
+  auto count = [&](int c0) {
+    const int g = c0 + tid / lanes;
+    int n = 0;
+    if (g < p.n_segs) {
+      const int4 s = p.segs[g];
+      if ((tid & (lanes - 1)) == 0) s_seg[tid / lanes] = s;
+      for (int m = tid & (lanes - 1); m < s.y; m += lanes)
+        n += blockIdx.x == 0 ? kv8_span(p, s.x + m, true).q_len
+                             : kv8_rows(p.q_lens, s.x + m, p.L, nullptr);
+    }
+    __syncwarp();
+    for (int o = lanes / 2; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if ((tid & (lanes - 1)) == 0) s_tiles[tid / lanes] = (n * p.rep + KP_ROWS - 1) / KP_ROWS;
+    __syncthreads();
+  };
+  const int H = p.c.kv_heads;
+  if (!p.deal) {  // a row tile for each segment
+    d.splits = p.splits;
+    d.split = pair % d.splits;
+    d.h = pair / d.splits % H;
+    d.tile = pair / d.splits / H;
+    d.in_seg = 0;
+    d.seg = p.segs[d.tile];
+    if (pair == 0 && tid == 0 && (blockIdx.x & 1) == 0) p.places[0] = d.splits;
+    return true;
+  }
+  int total = 0;
+  for (int c0 = 0; c0 < p.n_segs; c0 += per) {
+    if (c0 > 0) __syncthreads();  // (the last ones have been read)
+    count(c0);
+    int n = 0;
+    for (int i = lane; i < per; i += 32) n += s_tiles[i];
+    total += __reduce_add_sync(0xffffffffu, n);
+  }
+  d.splits = kp_ranges(total * H, p.longest, p.pairs);
+  if (pair == 0 && tid == 0 && (blockIdx.x & 1) == 0) p.places[0] = d.splits;
+  if (pair >= (long long)total * H * d.splits) return false;
+  d.split = pair % d.splits;
+  d.h = pair / d.splits % H;
+  d.tile = pair / d.splits / H;
+  int before = 0;
+  for (int c0 = 0; c0 < p.n_segs; c0 += per) {
+    if (p.n_segs > per) {
+      __syncthreads();
+      count(c0);
+    }
+    for (int i = 0; i < per; i += 32) {  // (zeros behind the last segment)
+      const int n = i + lane < per ? s_tiles[i + lane] : 0;
+      int end = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += up;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, d.tile < before + end);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        d.seg = s_seg[i + l];
+        d.in_seg = d.tile - before - __shfl_sync(0xffffffffu, end - n, l);
+        return true;
+      }
+      before += __shfl_sync(0xffffffffu, end, 31);
+    }
+  }
+  return false;  // (not reached)
+}
+
+// SEG: segments in the place of sequences.
 template <int D, bool SEG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     kv8_prefill_kernel(Kv8AttnParams p) {
@@ -183,40 +290,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
 
   // ---- the pair's rows and keys, this CTA's rows r_base .. + 127
   const int rank = blockIdx.x & 1;
-  const int units = (SEG ? p.n_segs : p.c.batch) * p.c.kv_heads * p.splits, unit = (blockIdx.x >> 1) % units;
-  const int rt = p.row_tiles - 1 - (blockIdx.x >> 1) / units;  // longest (causal) rows first
-  const int split = unit % p.splits, h = unit / p.splits % p.c.kv_heads;
-  const int b = unit / p.splits / p.c.kv_heads;
-  const int pair_base = rt * KP_ROWS, r_base = pair_base + rank * 128;
-  int4 seg = make_int4(0, 0, 0, 0);
-  int rows = p.L * p.rep;
+  int rt, split, h, b, rows, splits = p.splits;
+  KpDeal deal = {};
+  // What this CTA's rows are: sequence, query, head of the group, keys seen. (Where keys
+  // come, after everyone has looked.)
+  int4 *s_row = reinterpret_cast<int4 *>(smem + H::K_OFF);
   if constexpr (SEG) {
-    seg = p.segs[b];
-    rows *= seg.y;
-    if (pair_base >= rows) return;  // (both CTAs, before either waits for the other)
+    // (in the operands' place)
+    if (!kp_deal(p, reinterpret_cast<int4 *>(smem), reinterpret_cast<int *>(smem + 16 * KP_THREADS),
+                 deal))
+      return;
+    rt = kp_uniform(deal.in_seg); split = kp_uniform(deal.split); splits = kp_uniform(deal.splits);
+    h = kp_uniform(deal.h); b = 0;
+    deal.tile = kp_uniform(deal.tile);
+    deal.seg = make_int4(kp_uniform(deal.seg.x), kp_uniform(deal.seg.y), kp_uniform(deal.seg.z),
+                         kp_uniform(deal.seg.w));
+  } else {
+    const int units = p.c.batch * p.c.kv_heads * splits, unit = (blockIdx.x >> 1) % units;
+    rt = p.row_tiles - 1 - (blockIdx.x >> 1) / units;  // longest (causal) rows first
+    split = unit % splits; h = unit / splits % p.c.kv_heads; b = unit / splits / p.c.kv_heads;
+    rows = p.L * p.rep;
   }
+  const int4 seg = deal.seg;
+  const int pair_base = rt * KP_ROWS, r_base = pair_base + rank * 128;
   Kv8Span sp;
   int kend, owner = b;
   if constexpr (SEG) {
-    // keys that the tile's rows see, and a sequence that sees as many: its table has them.
-    // Every warp looks at all of the tile's sequences, 32 at a time.
-    const int per = p.L * p.rep, m0 = pair_base / per;
-    const int m1 = min(seg.y - 1, (min(pair_base + KP_ROWS, rows) - 1) / per);
-    kend = 0;
-    owner = seg.x + m0;
-    for (int m = m0; m <= m1; m += 32) {
+    // The tile's sequences, keys that its rows see, and a sequence that sees as many: its
+    // table has them. Every warp looks at all sequences up to them, 32 at a time.
+    int2 *s_seq = reinterpret_cast<int2 *>(s_row + 128);  // their first rows, sequences
+    int n_seq = 0;
+    kend = rows = 0;
+    owner = seg.x;
+    const bool flag = !p.deal && split == 0 && h == 0 && rank == 0 && warp == 0;
+    for (int m = 0; m < seg.y && (!p.deal || rows < pair_base + KP_ROWS); m += 32) {
+      const bool there = m + lane < seg.y;
+      const int bq = seg.x + m + lane;
       int n = 0;
-      if (m + lane <= m1) {
-        const Kv8Span s = kv8_span(p, seg.x + m + lane, split == 0 && rank == 0 && h == 0 && warp == 0);
-        // (a row tile that ends or begins within a sequence may see less)
-        n = s.q_len > 0 ? kv8_reach(seg, s.visible(s.q_len - 1)) : 0;
+      if (there)
+        n = flag ? kv8_span(p, bq, true).q_len : kv8_rows(p.q_lens, bq, p.L, nullptr);
+      n *= p.rep;
+      int end = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += up;
       }
-      const int most = (int)__reduce_max_sync(0xffffffffu, (unsigned)n);
+      const int begin = rows + end - n;
+      rows += __shfl_sync(0xffffffffu, end, 31);
+      int seen = 0;
+      if (n > 0 && begin < pair_base + KP_ROWS && begin + n > pair_base) {
+        const Kv8Span s = kv8_span(p, bq, false);
+        // (a row tile that ends or begins within a sequence may see less)
+        seen = kv8_reach(seg, s.visible(s.q_len - 1));
+        if (begin >= pair_base && split == 0 && h == 0 && rank == 0 && warp == 0)
+          p.places[1 + bq] = deal.tile * KP_ROWS + begin - pair_base;
+      }
+      const int most = (int)__reduce_max_sync(0xffffffffu, (unsigned)seen);
       if (most > kend) {
         kend = most;
-        owner = seg.x + m + __ffs(__ballot_sync(0xffffffffu, n == most)) - 1;
+        owner = seg.x + m + __ffs(__ballot_sync(0xffffffffu, seen == most)) - 1;
       }
+      const bool here = n > 0 && begin < r_base + 128 && begin + n > r_base;
+      const uint32_t all = __ballot_sync(0xffffffffu, here);
+      if (here && warp == 0) s_seq[n_seq + __popc(all & ((1u << lane) - 1))] = make_int2(begin, bq);
+      n_seq += __popc(all);
     }
+    rows = kp_uniform(rows);
+    kend = kp_uniform(kend);
+    owner = kp_uniform(owner);
+    __syncthreads();
+    if (tid < 128) {
+      const int R = r_base + tid;
+      int4 x = make_int4(seg.x, 0, 0, 0);
+      if (R < rows) {
+        int at = 0;  // the last sequence that begins at R or before
+#pragma unroll
+        for (int o = 64; o > 0; o >>= 1)
+          if (at + o < n_seq && s_seq[at + o].x <= R) at += o;
+        const int2 q = s_seq[at];
+        x.x = q.y;
+        x.y = p.row_of(R - q.x);
+        x.z = R - q.x - x.y * p.rep;
+        x.w = kv8_reach(seg, kv8_span(p, q.y, false).visible(x.y));
+      }
+      s_row[tid] = x;
+    }
+    __syncthreads();
   } else {
     sp = kv8_span(p, b, rt == p.row_tiles - 1 && split == 0 && rank == 0 && h == 0 && tid == 0);
     const int i_last = p.row_of(max(0, min(min(pair_base + KP_ROWS, rows), sp.q_len * p.rep) - 1));
@@ -226,7 +386,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   auto row_at = [&](int R) {
     Kv8SegRow x;
     if constexpr (SEG) {
-      x = kv8_seg_row(p, seg, R);
+      const int4 v = s_row[R - r_base];
+      x.b = v.x; x.i = v.y; x.hr = v.z; x.vis = v.w;
     } else {
       x.b = b;
       x.i = p.row_of(R);
@@ -236,11 +397,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     return x;
   };
   const int tiles = (kend + KP_KT - 1) / KP_KT;
-  const int share = tiles / p.splits, rest = tiles % p.splits;
+  const int share = tiles / splits, rest = tiles % splits;
   const int t0 = split * share + min(split, rest);
   const int t1 = t0 + share + (split < rest);
   const int n_tiles = t1 - t0;
-  const size_t tile_id = (((size_t)b * p.c.kv_heads + h) * p.row_tiles + rt) * p.splits + split;
+  const size_t tile_id =
+      SEG ? deal.pair : (((size_t)b * p.c.kv_heads + h) * p.row_tiles + rt) * splits + split;
   // (a segment's first key is the first of a page)
   const int pages_before = SEG ? seg.z >> p.shift : 0, table_len = p.c.max_pages - pages_before;
   const int32_t *table = p.c.page_table + (size_t)owner * p.c.max_pages + pages_before;
@@ -360,12 +522,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
       const int key = t * KP_KT + (lane & 7) * 16;
       return t < t1 && key < kend ? kv8_page_load(table, table_len, key >> p.shift) : 0;
     };
+    // (segments: the head's page, counted over all heads: h, which was dealt, costs registers
+    // in the bases, for heads of 256 31 of the rows on their way and a key tile a sixth)
     auto group_page = [&](int entry) {
-      return max(0, kv8_page_ok(entry, p.c.pages, p.status));
+      const int id = max(0, kv8_page_ok(entry, p.c.pages, p.status));
+      return SEG ? id * p.c.kv_heads + h : id;
     };
-    const size_t pool_step = (size_t)p.c.kv_heads * p.c.page * D;
-    const int8_t *kbase = p.c.k_codes + (size_t)h * p.c.page * D + kch * 16;
-    const int8_t *vbase = p.c.v_codes + (size_t)h * p.c.page * D + rank * H::VD + vch * 16;
+    const size_t pool_step = (size_t)(SEG ? 1 : p.c.kv_heads) * p.c.page * D;
+    const size_t head = SEG ? 0 : (size_t)h * p.c.page * D;
+    const int8_t *kbase = p.c.k_codes + head + kch * 16;
+    const int8_t *vbase = p.c.v_codes + head + rank * H::VD + vch * 16;
     auto load_k = [&](int id) {
 #pragma unroll
       for (int i = 0; i < KN; ++i) {
@@ -425,7 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
     const int hf = wg - 2, r = tid & 127, R = r_base + r;  // tiles hf, hf + 2, ...; S slot hf
     int vis;
     if constexpr (SEG)
-      vis = R < rows ? row_at(R).vis : 0;
+      vis = row_at(R).vis;
     else
       vis = R < rows ? sp.visible(p.row_of(R)) : 0;
     const bool one = n_tiles == 1;
@@ -771,9 +937,8 @@ int kp_launch(const Kv8AttnParams &p, cudaStream_t s) {
                                         cudaGetErrorString(e));
   });
   if (rc != VB_OK) return rc;
-  vb_launch(kv8_prefill_kernel<D, SEG>,
-            dim3(2 * p.row_tiles * p.splits * p.c.kv_heads * (SEG ? p.n_segs : p.c.batch)),
-            dim3(KP_THREADS), H::SMEM, s, false, p);
+  const unsigned pairs = SEG ? p.pairs : p.row_tiles * p.splits * p.c.kv_heads * p.c.batch;
+  vb_launch(kv8_prefill_kernel<D, SEG>, dim3(2 * pairs), dim3(KP_THREADS), H::SMEM, s, false, p);
   return check_launch("kv8_prefill_kernel");
 }
 
