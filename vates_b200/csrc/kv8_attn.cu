@@ -1009,10 +1009,10 @@ int kv8_run(const Kv8AttnParams &p, const Kv8Plan &pl, cudaStream_t s) {
 // of both are joined: weights 2^(m - M) of a row's partial results.
 //
 // What bounds it: the products of the prefix, at the prefill kernel's rate. 64 sequences x
-// 4 rows behind 32,768 keys, 16/2 heads of 256 (91 GFLOP, 55 us at a library product's
-// rate) take 230 us: the prefix 155, the own rows 39, partly beside it, the joining 14; each
-// sequence by itself 512. 48 x 1 row behind three prompts of up to 6,400 keys, 32/8 heads of
-// 128: 72 us, apart 91: the groups' 60 rows fill a quarter of a row tile.
+// up to 4 rows (167) behind 32,768 keys, 16/2 heads of 256 (91 GFLOP, 55 us at a library
+// product's rate) take 153 us (the kernels one by one from cold caches: the prefix 125, the own
+// rows 55, the joining 14); each sequence by itself 512. 48 x 1 row behind three prompts of up to 6,400 keys, 32/8 heads of
+// 128: 69 us, apart 90: the groups' 60 rows fill a quarter of a row tile.
 struct Kv8Parted {             // where the results of some segments are
   const float *o, *o_part;
   const float2 *ml, *ml_part;
@@ -1078,21 +1078,23 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __gri
   const int tid = threadIdx.x, d4 = tid % LR, pg = tid / LR % PG, H = p.c.kv_heads;
   const int row = blockIdx.x * RPC + tid / (LR * PG), per = p.Hq * p.L;
   const bool there = row < p.c.batch * per;
-  int b = 0, h = 0, i = 0, R = 0, g = -1, R_pre = 0;
+  int b = 0, h = 0, R = 0, g = -1, R_pre = 0;
+  bool live = false;
   float M = -INFINITY, ls = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (there) {  // (the groups are the plan's, nothing that a kernel ahead writes)
+  // (the groups are the plan's, and rows per sequence are there since the first of the
+  // kernels ahead has begun)
+  if (there) {
     b = row / per;
-    const int x = row - b * per, hq = x / p.L;
-    i = x - hq * p.L;
+    const int x = row - b * per, hq = x / p.L, i = x - hq * p.L;
     h = hq / p.rep;
     R = i * p.rep + hq - h * p.rep;
     g = w.group_of[b];
     if (g >= 0) R_pre = (b - w.groups[g].x) * p.L * p.rep + R;
+    live = i < kv8_rows(p.q_lens, b, p.L, nullptr);
   }
   pdl_wait();
   if (there) {
-    const bool live = i < kv8_rows(p.q_lens, b, p.L, nullptr);
     Kv8PartedRow pre, own = kv8_parted_row<D>(w.own, H, b * H + h, R, b, h, R, live);
     pre.n = 0;
     if (g >= 0) pre = kv8_parted_row<D>(w.pre, H, g * H + h, R_pre, b, h, R, live);

@@ -165,10 +165,10 @@ struct KpBarriers {
 
 // Segments (kv8_attn.cuh): what a pair of CTAs is to do, from the rows that there are.
 // Lengths are on the device, so the tiles and key ranges are dealt here: 64 sequences
-// with 162 of 64 x 4 rows behind 32,768 keys, 16/2 heads of 256, fill 12 tiles instead of 16.
+// with 167 of 64 x 4 rows behind 32,768 keys, 16/2 heads of 256, fill 12 tiles instead of 16:
+// 152 us for 211. It takes 2 us.
 struct KpDeal {
   int4 seg;
-  int pair;            // tile, head and range as a number
   int tile, in_seg;    // row tile, of all and within the segment
   int h, split, splits;
 };
@@ -198,10 +198,7 @@ __device__ __forceinline__ int kp_ranges(int base, int tiles, int pairs) {
 // False if there is nothing for the pair; the same for all threads of both CTAs. s_seg,
 // s_tiles: KP_THREADS of them.
 __device__ __forceinline__ bool kp_deal(const Kv8AttnParams &p, int4 *s_seg, int *s_tiles, KpDeal &d) {
-  // Pairs without work come first, all at once: behind the others, on the few SMs that
-  // those leave, they would hold up the next kernel (230 us for the sequences above, 272).
-  const int tid = threadIdx.x, lane = tid & 31, pair = p.pairs - 1 - (blockIdx.x >> 1);
-  d.pair = pair;
+  const int tid = threadIdx.x, lane = tid & 31, pair = blockIdx.x >> 1;
   const int lanes = p.seg_lanes, per = KP_THREADS / lanes;
   // row tiles of the segments from c0 on
   auto count = [&](int c0) {
@@ -402,7 +399,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KP_THREADS, 1)
   const int t1 = t0 + share + (split < rest);
   const int n_tiles = t1 - t0;
   const size_t tile_id =
-      SEG ? deal.pair : (((size_t)b * p.c.kv_heads + h) * p.row_tiles + rt) * splits + split;
+      SEG ? blockIdx.x >> 1 : (((size_t)b * p.c.kv_heads + h) * p.row_tiles + rt) * splits + split;
   // (a segment's first key is the first of a page)
   const int pages_before = SEG ? seg.z >> p.shift : 0, table_len = p.c.max_pages - pages_before;
   const int32_t *table = p.c.page_table + (size_t)owner * p.c.max_pages + pages_before;
