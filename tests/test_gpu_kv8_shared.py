@@ -114,13 +114,14 @@ def test_long_prefixes(cuda, B, L, rep, dim, page, rows, tail):
 
 
 @pytest.mark.parametrize("groups,count,L,rep", [(40, 20, 1, 4), (300, 2, 3, 12), (9, 40, 2, 20),
-                                                (1, 520, 1, 2), (2, 3, 130, 2)])
+                                                (1, 520, 1, 2), (2, 3, 130, 2), (20, 20, 1, 16),
+                                                (260, 2, 130, 2)])
 def test_rows_that_are_not_there(cuda, groups, count, L, rep):
     """Row tiles are filled by the rows of this pass: many groups, sequences without
     rows, groups without any, groups whose rows begin anywhere in a tile."""
     rng = np.random.default_rng(groups + count)
     B = groups * count + 1
-    c = make_cache(rng, B, 1, 64, 16, 24)
+    c = make_cache(rng, B, 1, 64, 16, 32)
     q = bf16(rng, (B, rep, L, 64), 1.5).cuda()
     ql = [int(n) for n in rng.integers(0, L + 1, B)]
     for g in range(1, groups, 3):
@@ -128,6 +129,25 @@ def test_rows_that_are_not_there(cuda, groups, count, L, rep):
     prefix = [16 * int(n) for n in rng.integers(1, 20, groups)]
     lens = [prefix[min(b // count, groups - 1)] + n + int(rng.integers(0, 40)) for b, n in enumerate(ql)]
     check(c, q, [(g * count, count, prefix[g]) for g in range(groups)], lens, ql)
+
+
+def test_a_graph_deals_anew_in_each_replay(cuda):
+    """Rows per sequence change under a captured call: from all to few, to none."""
+    rng = np.random.default_rng(22)
+    c = make_cache(rng, 33, 2, 128, 32, 70)
+    q = bf16(rng, (33, 16, 4, 128)).cuda()
+    plan = share(c, [(0, 16, 2048), (16, 17, 1024)])
+    lens, ql = ints([2060 + b for b in range(16)] + [1030 + b for b in range(17)]), ints([4] * 33)
+    ref = Plain(c)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = c.attend_shared(q, lens, plan, ql, return_lse=True)
+    for rows in ([4] * 33, [int(n) for n in rng.integers(0, 5, 33)], [0] * 16 + [1] * 17, [0] * 33,
+                 [0] * 32 + [4]):
+        ql.copy_(ints(rows))
+        g.replay()
+        a, la = check(c, q, None, lens.tolist(), rows, plan=plan, ref=ref)
+        assert torch.equal(a, out) and torch.equal(la, lse)
 
 
 def test_bad_row_counts_are_flagged(cuda):
