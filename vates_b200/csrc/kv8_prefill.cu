@@ -182,7 +182,7 @@ __device__ __forceinline__ int kp_uniform(int x) {
 __device__ __forceinline__ int kp_ranges(int base, int tiles, int pairs) {
   const int most = min(pairs, 8 * 74);
   if (base > most) return 1;
-  // (at most 8 waves of 2^24 tiles; 32 x the time, up to 2^20 of it)
+  // (32 x the time, of at most 8 waves; ranges of more than 2^16 tiles count as that long)
   auto cost = [&](int s) {
     return 32u * (unsigned)((base * s + 73) / 74) * (3 + min((tiles + s - 1) / s, 1 << 16)) +
            (s > 1 ? 64 + base * s : 0);
