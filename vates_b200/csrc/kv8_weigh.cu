@@ -261,7 +261,8 @@ struct WrShape {
 };
 
 // f16 queries, row after row of a (sequence, kv head), and what turns a product into
-// a weight; rows that are not there, or have no finite lse, count for nothing.
+// a weight; rows that are not there, or have no finite lse, count for nothing: they are
+// zeros, as the product of a NaN, or of an infinity, is not made -inf by any log2 sum.
 template <int D>
 __global__ void __launch_bounds__(256) kv8_weigh_q_kernel(const __grid_constant__ Kv8WeighParams w) {
   constexpr int LPR = D / 8;
@@ -280,10 +281,11 @@ __global__ void __launch_bounds__(256) kv8_weigh_q_kernel(const __grid_constant_
     v = kv8_load8(p.q + b * p.qb + (int64_t)hq * p.qh + (int64_t)i * p.ql + c8 * 8, p.vec);
     l = w.lse[((size_t)b * p.Hq + hq) * p.L + i];
   }
+  const bool counts = fabsf(l) <= 3.4028235e38f;
+  if (!counts) v = make_uint4(0, 0, 0, 0);
   const float pw = kv8_q_scale<LPR>(v);
   *(reinterpret_cast<uint4 *>(w.q16 + (size_t)at * D) + c8) = v;
   if (c8 == 0) {
-    const bool counts = fabsf(l) <= 3.4028235e38f;
     if (!counts && l != -INFINITY) flag_status(p.status, VB_STATUS_NONFINITE);
     // (a factor above 0: times -inf, what a row does not see)
     w.row[at] = make_float2(fmaxf(p.scale_log2 / pw, 1.1754944e-38f),
