@@ -1122,8 +1122,8 @@ __global__ void __launch_bounds__(KC_THREADS) kv8_shared_join_kernel(const __gri
       a.x *= back; a.y *= back; a.z *= back; a.w *= back;
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
-        if (ml[k].x == -INFINITY) continue;
-        const float f = kv8_ex2(ml[k].x - M);
+        // (the scores of a NaN query leave no maximum, and a NaN for a sum: it stays)
+        const float f = ml[k].x == -INFINITY ? 0.f : kv8_ex2(ml[k].x - M);
         ls = fmaf(f, ml[k].y, ls);
         if (f > 0.f) {
           a.x = fmaf(f, y[k].x, a.x); a.y = fmaf(f, y[k].y, a.y);
