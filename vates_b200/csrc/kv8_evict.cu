@@ -353,6 +353,7 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
   __shared__ int s_src[GROUPS][G], s_sid[GROUPS][G], s_row[GROUPS][G];
   __shared__ float s_from[GROUPS][G], s_top[GROUPS][WARPS];
   __shared__ uint32_t s_filled[GROUPS][4][WARPS];
+  __shared__ int s_moved[GROUPS][WARPS];
   pdl_launch_dependents();
   pdl_wait();
   const int gi = threadIdx.x / G, kv = gi & 1, tid = threadIdx.x % G, warp = tid >> 5;
@@ -385,9 +386,9 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
       const int id = kv8_page(table, p.c.max_pages, p.c.pages, pg, tid == 0 ? p.status : nullptr);
       if (id < 0) continue;
       const int live = min(p.c.page, p.keep - (pg << p.shift));
-      const bool stay = count < live;
       const float old = pg == edge ? edge_scale : scales[(size_t)id * p.c.kv_heads + h];
-      // ---- hole `tid` of the page, and where its new row comes from
+      // ---- hole `tid` of the page, and where its new row comes from; from a page that is
+      // not there none does, and the hole's own row stays
       int src = -1, sid = -1, row = 0;
       float from = 0.f;
       if (tid < count) {
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
         s_sid[gi][tid] = sid;
         s_row[gi][tid] = row & (p.c.page - 1);
         s_from[gi][tid] = from;
-        if (kv == 0) {
+        if (kv == 0 && sid >= 0) {
           const size_t w = (size_t)unit * p.room;
           p.weights[w + row] = p.weights[w + src];
           if (p.positions) p.positions[w + row] = p.positions[w + src];
@@ -412,11 +413,19 @@ __global__ void __launch_bounds__(EM_THREADS, 4) kv8_evict_move_kernel(const __g
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint32_t f = __reduce_or_sync(0xffffffffu, src >= 0 && r >> 5 == w ? 1u << (r & 31) : 0u);
+        const uint32_t f = __reduce_or_sync(0xffffffffu, sid >= 0 && r >> 5 == w ? 1u << (r & 31) : 0u);
         if (lane == 0) s_filled[gi][w][warp] = f;
       }
-      if (lane == 0) s_top[gi][warp] = top;
+      const uint32_t all = __ballot_sync(0xffffffffu, sid >= 0);
+      if (lane == 0) {
+        s_top[gi][warp] = top;
+        s_moved[gi][warp] = __popc(all);
+      }
       meet();
+      int moved = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) moved += s_moved[gi][w];
+      const bool stay = moved < live;
       top = stay ? old : 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_top[gi][w]);
