@@ -9,6 +9,7 @@ import torch
 from test_gpu_kv8 import bf16, ints, make_cache
 from test_gpu_kv8_evict import check_weigh
 from vates_b200 import _lib
+from vates_b200.kv8 import PagedKV8Cache
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +76,23 @@ def test_no_row_counts(cuda):
     assert lse.isnan().all()
     w = check_weigh(c, q, lens, new=[0, 7], lse=lse)
     assert not w[1, :, 93:100].any()
+
+
+@pytest.mark.parametrize("L", [4, 40])
+def test_longest_sequence(cuda, L):
+    """As many keys as a table may have, less than 2^31 - 65536, which all lie in one page:
+    new rows alone, without query rows, and then a row that sees them all."""
+    keys, pad = (1 << 31) - 65536 - 128, 1 << 31
+    c = PagedKV8Cache.empty(1, 1, 64, 1, keys // 128, 128)
+    c.page_table.zero_()
+    # what lies in front of the weights is not written
+    room = torch.ones(pad + keys, device="cuda")
+    w = room[pad:].view(1, 1, keys)
+    q, lse = torch.zeros((1, 1, L, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((1, 1, L), device="cuda")
+    c.weigh(q, lse, ints([keys]), w, ints([0]), new=ints([100_000]))
+    assert float(room[:-100_000].min()) == float(room[:-100_000].max()) == 1
+    assert not room[-100_000:].any()
+    c.weigh(q, lse, ints([keys]), w, ints([1]), new=ints([9]), causal=False)
+    assert float(room[:pad].min()) == float(room[:pad].max()) == 1
+    assert float(w[..., :-100_000].min()) == float(w[..., :-100_000].max()) == 2
+    assert float(w[..., -100_000:].min()) == float(w[..., -100_000:].max()) == 1

@@ -327,10 +327,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
   if (!wg_span(w, b, range == 0 && rank == 0 && h == 0 && tid == 0, s)) return;
   const int keys = s.sp.keys, rows = s.sp.q_len * p.rep;
   const size_t at0 = (size_t)unit * w.room;
-  if (rows == 0) {  // new rows alone
-    for (int key = s.fresh + blockIdx.x % (2 * w.ranges) * WR_THREADS + tid; key < keys;
+  if (rows == 0) {  // new rows alone (64 bits: a stride may lead past 31)
+    for (long long key = (long long)s.fresh + blockIdx.x % (2 * w.ranges) * WR_THREADS + tid; key < keys;
          key += 2 * w.ranges * WR_THREADS)
-      wg_add(w, s, b, at0, key, 0.f, true, 0.f);
+      wg_add(w, s, b, at0, (int)key, 0.f, true, 0.f);
     return;
   }
   const int tiles = (keys + WR_KEYS - 1) / WR_KEYS, share = tiles / w.ranges, rest = tiles % w.ranges;
