@@ -104,6 +104,7 @@ class SharedPrefix:
         self._words = torch.tensor(words + group_of, dtype=torch.int32).to(self.device)
         self._segments = self._words.data_ptr()
         self._group_of = self._segments + 4 * len(words)
+        self._stream = current_stream(self._words.get_device())  # whose memory _words is
         self._host = (C.c_int32 * (3 * len(kept)))(*[x for g in kept for x in g])
         self._count = len(kept)
         self._longest = max([rows // self.page for _, _, rows in kept], default=0)
@@ -288,6 +289,8 @@ class PagedKV8Cache:
                                       return_lse, status)
         st = current_stream(dev)
         self._attn_workspace(s.attn, workspace, self._shared_need(shared, s), st)
+        if st != shared._stream:  # a plan that is let go now is read by the kernels all the same
+            shared._words.record_stream(torch.cuda.current_stream(dev))
         check(lib.vb_kv8_attn_shared(C.byref(s), st), "vb_kv8_attn_shared")
         return (out, lse) if return_lse else out
 
