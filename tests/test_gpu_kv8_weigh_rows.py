@@ -78,6 +78,20 @@ def test_no_row_counts(cuda):
     assert not w[1, :, 93:100].any()
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("L", [2, 33, 200])
+def test_scales_of_zero_and_tiny_ones(cuda, L, causal):
+    """A page with scale 0 has scores of 0 whatever its codes and the queries are, and the
+    smallest scales count as any other."""
+    rng = np.random.default_rng(L)
+    c = make_cache(rng, 2, 2, 128, 16, 40)
+    q = bf16(rng, (2, 4, L, 128)) * 2.0 ** 100
+    c.k_scales.fill_(0)
+    check_weigh(c, q.cuda(), [640, 201], causal=causal)
+    c.k_scales[::2] = 2.0 ** -110
+    check_weigh(c, q.cuda(), [640, 201], causal=causal, scale=2.0 ** -3)
+
+
 @pytest.mark.parametrize("L", [4, 40])
 def test_longest_sequence(cuda, L):
     """As many keys as a table may have, less than 2^31 - 65536, which all lie in one page:

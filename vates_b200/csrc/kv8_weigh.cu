@@ -522,7 +522,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
       const bool more = t == n_tiles - 1 && ch + 1 < chunks;
       ks_n = scale_of(entry_n);
       const int key = (t0 + t) * WR_KEYS + rank * 128 + r;
-      const bool masked = (t0 + t) * WR_KEYS + rank * 128 + 128 > seen_by_all;
+      const bool masked = (t0 + t) * WR_KEYS + rank * 128 + 128 > seen_by_all ||
+                          __any_sync(0xffffffffu, ks == 0.f);
       t = t_next;
       t_next = ahead(t, 2);
       entry_n = entry_of(t0 + t_next);
@@ -533,8 +534,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
       if (more && ok) load_q(ch + 1, tid - 384 - 256 * pair, 256);  // no product of this chunk is left
       const int first = half * (cols / 2);
       const float4 *tab = s_row[ch & 1] + first / 2;
-      // (at least 2^-100, where the score is 0 for any codes and a hidden one stays -inf)
-      const f2 kk = f2_make(fmaxf(ks, 7.9e-31f), fmaxf(ks, 7.9e-31f));
+      // Scale 0: scores of 0 whatever the codes, by products of 0 and a factor above 0, with
+      // which a hidden one stays -inf. (No scale stands for 0: a query may undo it.)
+      const uint32_t code = ks == 0.f ? 0u : 0xFFFFFFFFu;
+      const float kf = ks > 0.f ? ks : 1.f;
+      const f2 kk = f2_make(kf, kf);
       const int from = s.sp.causal ? max(0, key - s.sp.off) * p.rep : 0;
       f2 s0 = f2_make(0.f, 0.f), s1 = s0;
 #pragma unroll 1
@@ -546,7 +550,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WR_THREADS, 1)
           const int hidden = from - (ch * WR_COLS + first + c0);
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (j < hidden) v[j] = 0xFF800000u;
+            v[j] = j < hidden ? 0xFF800000u : v[j] & code;
         }
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
