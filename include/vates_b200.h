@@ -677,7 +677,8 @@ int vb_kv8_evict(const VbKv8EvictArgs *args, vb_stream_t stream);
  * positions[axis[i]][b][t] * turns[i] turns, after an RMS norm with weight
  * q_norm / k_norm (nullable, bf16 [dim]). float32, rounded once. turns and axis
  * [rope_dims / 2] are host memory, read before the call returns. An output may
- * be its input; dim 16 to 256 and rope_dims multiples of 16.
+ * be its input, and has each row in a place of its own; dim 16 to 256 and rope_dims
+ * multiples of 16.
  * ------------------------------------------------------------------------- */
 typedef struct VbRotateArgs {
   const uint16_t *q, *k;

@@ -34,6 +34,17 @@ def test_refusals(bad):
     assert b"vb_rotate_axes" in lib.vb_last_error()
 
 
+@pytest.mark.parametrize("out", ["q_out_strides", "k_out_strides"])
+@pytest.mark.parametrize("strides", [(0, 256, 128), (1024, 0, 128), (1024, 256, 0)])
+def test_outputs_whose_rows_share_a_place(out, strides):
+    """An expanded tensor, be it the input itself (whose rows may)."""
+    three = C.c_int64 * 3
+    dense = dict(q_out_strides=three(1024, 256, 128), k_out_strides=three(512, 256, 128))
+    a = _args(batch=2, **{**dense, out: three(*strides)})
+    assert lib.vb_rotate_axes(C.byref(a), None) == 1
+    assert b"one place" in lib.vb_last_error()
+
+
 def test_no_tokens_are_accepted():
     assert lib.vb_rotate_axes(C.byref(_args(L=0)), None) == 0
     assert lib.vb_rotate_axes(C.byref(_args(q_heads=0, kv_heads=0)), None) == 0

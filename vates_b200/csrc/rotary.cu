@@ -240,7 +240,10 @@ extern "C" int vb_rotate_axes(const VbRotateArgs *a, vb_stream_t stream) {
     odd |= (int64_t)((uintptr_t)p.src[i] / 2) | (int64_t)((uintptr_t)p.dst[i] / 2) |
            (int64_t)((uintptr_t)p.norm[i] / 2);
     same = same && p.src[i] == p.dst[i] && !p.norm[i];
+    const int extent[3] = {a->batch, p.heads[i], a->L};
     for (int k = 0; k < 3; ++k) {
+      VB_REQUIRE(extent[k] == 1 || (i ? a->k_out_strides[k] : a->q_out_strides[k]) != 0,
+                 "vb_rotate_axes: rows of an output in one place (a stride of 0)");
       p.s_in[i][k] = i ? a->k_strides[k] : a->q_strides[k];
       p.s_out[i][k] = i ? a->k_out_strides[k] : a->q_out_strides[k];
       odd |= p.s_in[i][k] | p.s_out[i][k];

@@ -87,7 +87,8 @@ def rotate_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes,
     pairs. ``q_norm``, ``k_norm`` bf16 ``[dim]``: rows are RMS-normalised and
     multiplied by it first. Float32 throughout, rounded to bf16 once. Results are
     new contiguous tensors, or ``q_out`` and ``k_out``, which may be ``q`` and
-    ``k`` themselves but must not overlap them in any other way."""
+    ``k`` themselves but must not overlap them in any other way, nor hold two rows in
+    one place (an expanded tensor)."""
     dev = q.get_device()
     # with it as the current stream, results belong to it
     if dev >= 0 and (stream is not None or current_device() != dev):
