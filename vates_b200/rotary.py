@@ -35,7 +35,9 @@ def pair_axes(sections, interleaved: bool = False) -> tuple:
 
 
 def _check(t: torch.Tensor, what: str, shape):
-    if t.dtype != torch.bfloat16 or t.shape != shape or t.stride()[-1:] not in ((1,), ()):
+    # (an empty tensor's strides may be anything)
+    if t.dtype != torch.bfloat16 or t.shape != shape \
+            or (t.numel() and t.stride()[-1:] not in ((1,), ())):
         raise ValueError(f"{what}: bfloat16 {tuple(shape)} with contiguous dims is needed, got "
                          f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
 
