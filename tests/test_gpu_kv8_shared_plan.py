@@ -23,10 +23,15 @@ def test_a_plan_of_one_step_on_another_stream(cuda, count, L, made_on_side):
     torch.cuda.synchronize()
     with torch.cuda.stream(here):
         plan = SharedPrefix(c, [(0, count, 480)], 0)
-    busy, at, n = (here, plan._segments, plan._words.numel()) if made_on_side else \
-        (there, plan._segments, plan._words.numel())
+        # (both streams have memory of their own before one is busy: asking for more may wait)
+        others = [torch.empty(plan._words.numel(), dtype=torch.int32, device="cuda") for _ in range(64)]
+    at, n = plan._segments, plan._words.numel()
+    busy = here if made_on_side else there
+    got = c.attend_shared(q, lens, plan, stream=busy)
+    torch.cuda.synchronize()
+    del got, others
     with torch.cuda.stream(busy):
-        torch.cuda._sleep(200_000_000)
+        torch.cuda._sleep(1_000_000_000)
     got = c.attend_shared(q, lens, plan, stream=busy)
     del plan
     with torch.cuda.stream(here):
