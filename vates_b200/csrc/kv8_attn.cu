@@ -1208,7 +1208,8 @@ Kv8Side kv8_side(const VbKv8AttnArgs *a, long long segs, long long seqs, long lo
 // and one that joins. It is worth it from 80 MB on (16 sequences x 2 rows, 64/8 heads of 64,
 // 326 MB: 36 us and 64 apart; 35 x 1, 3/2 of 256, 798 MB: 43 and 115; 28 MB: 18 us apart
 // and 23; 67 MB: 23 and 24), or 27 MB with more than 32 rows per kv head, which go
-// through the prefill kernel (30 MB: 31 and 67; 18 MB: 38 and 27).
+// through the prefill kernel (30 MB: 31 and 67; 18 MB: 38 and 27). Bytes alone decide:
+// the rows that a call has are on the device.
 bool kv8_worth_sharing(const VbKv8SharedArgs *s) {
   const VbKv8AttnArgs *a = &s->attn;
   long long saved = 0;

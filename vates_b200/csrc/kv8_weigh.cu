@@ -8,12 +8,12 @@
 // queries (after a power of two per row) are exact in f16, sums float32, and a
 // key's weights are added in one order, whatever the launch.
 //
-// Up to 32 query rows per kv head (kv8_weigh_kernel, HBM-bound: a byte per cached
-// value of K): a warp takes 16 keys at a time, brought by cp.async into a ring of
-// its own in which every lane finds the 16-byte pieces that it asked for itself,
-// already in the order of the fragments of S^T = K q^T (lane (g, c) has 16
-// consecutive bytes of keys g and g + 8, four k-steps), so that nothing in the
-// loop waits for another thread. Rows come eight to a fragment.
+// Up to 32 query rows per kv head (kv8_weigh_kernel, which reads a byte per cached value
+// of K): a warp takes 16 keys at a time, brought by cp.async into a ring of its own in
+// which every lane finds the 16-byte pieces that it asked for itself, already in the
+// order of the fragments of S^T = K q^T (lane (g, c) has 16 consecutive bytes of keys
+// g and g + 8, four k-steps), so that nothing in the loop waits for another thread. Rows
+// come eight to a fragment.
 //
 // More rows (kv8_weigh_rows_kernel, a window at a prompt's end or a prompt's chunk;
 // tensor-core- and exponential-bound): a pair of CTAs (tcgen05 cta_group::2) takes
@@ -22,8 +22,9 @@
 // weights by itself. Queries are made ready once by a kernel ahead of it.
 //
 // What bounds it: 32 sequences of up to 8,190 keys, 32/8 heads of 128, take 30 us for 128
-// MB (4.3 TB/s, a copy 19.6): issue slots are half used (five instructions turn four codes
-// into f16) and warps wait for their keys; one sequence of 901 keys costs the launch, 3.5.
+// MB (4.3 TB/s, a copy 19.6): neither HBM nor the issue slots are more than half used
+// (five instructions turn four codes into f16); warps wait for their keys, and each of the
+// short CTAs for its page numbers and queries first; one sequence of 901 keys costs the launch, 3.5.
 // 64 rows of 16/2 heads of 256 over 32,768 keys take 29 us (products alone 10.4): two
 // chunks of 256 rows over three or four tiles a pair, 1.8 us each, 4 for the queries and 8
 // to begin and end; over 131,072 keys a tile of 256 x 256 takes 2.4 us, of which the

@@ -74,8 +74,9 @@ __device__ __forceinline__ void rt_store(uint16_t *p, const f2 (&x)[4], bool vec
 // stays with one token: its sines are made once, and from head to head only a
 // pointer moves.
 // Rows of a thread in flight, and CTAs per SM: 2 and 4, with a norm, whose registers
-// leave room for 3 CTAs, 3 and 3 (65,536 tokens of 16/2 heads of 256 with it 258 us, 306
-// the other way; 2 x 8,191 of 32/8 heads of 128 without it 79 and 83).
+// leave room for 3 CTAs, 3 and 3 (65,536 tokens of 16/2 heads of 256 with it 248 to 258 us
+// a call, 306 the other way). Without it 2 x 8,191 of 32/8 heads of 128 take 64.5, and 59 to
+// 61 with 3 and 3: the choice was made when a CTA took more tokens (79 and 83).
 template <int LPR, bool NORM>
 __global__ void __launch_bounds__(RT_THREADS, NORM ? 3 : 4) rotate_kernel(const __grid_constant__ RotateParams p,
                                                                bool vec) {
